@@ -577,6 +577,74 @@ int t2h_add(const void* x, const void* y, void* out, int dtype, uint64_t n, void
  * SLICE_LAST_TOKEN_F32_TO_F16 (src/models/optimized_qwen3/shaders/slice_last_token_f32_to_f16.py:19-60). */
 int t2h_slice_last_token(const float* x, void* out, int out_dtype, uint32_t b, uint32_t s, uint32_t h, void* stream);
 
+/* ---------------------------------------------------- 8-bit KV cache --- */
+/* A KV cache in 8 bits, with one fp32 scale for each block of T2H_KV_Q8_BLOCK tokens, sequence and KV head (keys and
+ * values apart), in place of the bf16 caches above: half the bytes that an attention reads.  No counterpart in the
+ * reference, whose caches are fp16 (src/models/optimized_qwen3/tensors/model.py:104-150).
+ * cache: host array of six device pointers, d = 128 and n_blocks = s_cap / 64 (s_cap a multiple of 64):
+ *   k int8 [n_seq][n_blocks][nk][64][d]   v int8 [n_seq][n_blocks][nk][d][64]   k_scale, v_scale fp32 [n_seq][n_blocks][nk]
+ *   k_tail bf16 [n_seq][nk][64][d]        v_tail bf16 [n_seq][nk][d][64]        (fp32 4-byte, the others 16-byte aligned)
+ * A whole block's values are code * scale, scale = max|x| / 127 over its bf16 values x, code = x / scale rounded once, ties
+ * to even.  The tokens of a sequence's last, unfinished block are bf16 rows in the tail and are rounded when the block's
+ * last token arrives, so that the cache depends on the tokens and not on the chunks they came in.  A block of values under
+ * 1.3e-28 is held as zeros; one with a NaN or an infinity reads as NaN.
+ * lengths (device int32 [n_seq]): the tokens that each sequence holds before the call; calls do not advance them, so that
+ * the layers of a step share them.  A negative length: the sequence takes no part, its outputs are zeros.  Tokens past s_cap
+ * are dropped: they are not written, and their queries see the s_cap cached ones.  A sequence goes on from its length
+ * only: to go back before its last whole block, write its tokens anew.
+ * counts (device int32 [n_seq], or NULL for n each): new tokens of each sequence, the first of its n rows; outputs of the
+ * rows behind them are zeros.
+ * rope_offsets (device int32 [n_seq], or NULL): position of a token = its place in the cache + offset, as after an eviction.
+ * nh / nk is a whole number up to 16. */
+#define T2H_KV_Q8_BLOCK 64
+
+/* t2h_qk_norm_rope_cache for such a cache: per-head RMSNorm (q_norm_w / k_norm_w, both or neither) and rotate-half RoPE
+ * (theta <= 0: none; angles in fp64) of q [n_seq * n, q_row] and k [n_seq * n, k_row], fp32, head h at columns 128 h;
+ * q -> q_out bf16 [n_seq * n, nh, 128], k and v -> the cache. */
+int t2h_qk_norm_rope_cache_q8(const float* q, uint64_t q_row, const float* k, uint64_t k_row, const float* v,
+                              uint64_t v_row, const float* q_norm_w, const float* k_norm_w, float eps, float theta,
+                              const int32_t* lengths, const int32_t* counts, const int32_t* rope_offsets, uint32_t n,
+                              uint32_t n_seq, uint32_t nh, uint32_t nk, uint32_t d, void* q_out, void* const* cache,
+                              uint32_t s_cap, void* stream);
+/* t2h_attn_decode for such a cache and n_seq sequences of any lengths: one new token each, normalised, rotated, written,
+ * then out bf16 [n_seq, nh, 128] = softmax(q . k / sqrt(128)) . v over the cache with it (q stays fp32).
+ * weights / weights_out (fp32 [n_seq, nk, s_cap], both or neither, the same or distinct): weights_out = weights + the
+ * softmax weight that each cached token got, summed over the q heads of the KV head; a new token's begins at 0, and
+ * elements behind the last token are left as they are.
+ * workspace: t2h_attn_decode_q8_workspace_bytes() bytes, 16-byte aligned, no initialisation; calls that share one must not
+ * overlap in time. */
+size_t t2h_attn_decode_q8_workspace_bytes(uint32_t n_seq, uint32_t nh, uint32_t nk, uint32_t d, uint32_t s_cap,
+                                          int weights);
+int t2h_attn_decode_q8(const float* q, uint64_t q_row, const float* k_new, uint64_t k_row, const float* v_new,
+                       uint64_t v_row, const float* q_norm_w, const float* k_norm_w, float eps, float theta,
+                       const int32_t* lengths, const int32_t* rope_offsets, void* const* cache, uint32_t s_cap,
+                       const float* weights, float* weights_out, void* out, uint32_t n_seq, uint32_t nh, uint32_t nk,
+                       uint32_t d, void* workspace, size_t workspace_bytes, void* stream);
+/* Causal attention of a chunk that t2h_qk_norm_rope_cache_q8 has written, with the same lengths and counts: query t of
+ * q bf16 [n_seq, n, nh, 128] sees tokens 0 .. length + t.  out as q (both 16-byte aligned); scale <= 0 means 1 / sqrt(128);
+ * weights and workspace as above (the weights of all the chunk's queries). */
+size_t t2h_flash_attn_prefill_q8_workspace_bytes(uint32_t n, uint32_t n_seq, uint32_t nh, uint32_t nk, uint32_t s_cap,
+                                                 int weights);
+int t2h_flash_attn_prefill_q8(const void* q, void* const* cache, uint32_t s_cap, const int32_t* lengths,
+                              const int32_t* counts, const float* weights, float* weights_out, void* out, uint32_t n,
+                              uint32_t n_seq, uint32_t nh, uint32_t nk, uint32_t d, float scale, void* workspace,
+                              size_t workspace_bytes, void* stream);
+/* The cache as bf16 rows [n_seq, s_cap, nk, 128], the layout of the other caches, zeros behind each length. */
+int t2h_kv_cache_q8_dequantize(void* const* cache, uint32_t s_cap, const int32_t* lengths, uint32_t n_seq, uint32_t nk,
+                               uint32_t d, void* k_out, void* v_out, void* stream);
+/* Eviction by accumulated weight (weights fp32 [n_seq, nk, s_cap]): of a sequence's F whole blocks of tokens each KV head
+ * keeps 64 min(F, keep_blocks), in their order: the first `sink`, the last `recent`, then those of the most weight (ties:
+ * the earliest; NaN ranks above numbers).  sink + recent <= 64 keep_blocks.  They form whole blocks that are rounded anew
+ * under their own scales; the tail stays.  kept int32 [n_seq, nk, 64 keep_blocks]: the tokens that stayed, ascending, then
+ * -1.  lengths_out [n_seq] (not lengths itself): the lengths after it; rope_offsets grow by what a length lost.
+ * weights_out [n_seq, nk, s_cap_out]: the weights of what stays (elements behind it are left).
+ * cache_out and weights_out are the inputs themselves, or distinct and of a capacity s_cap_out >= 64 (keep_blocks + 1) or
+ * >= s_cap. */
+int t2h_kv_cache_q8_evict(void* const* cache, uint32_t s_cap, const int32_t* lengths, const float* weights,
+                          uint32_t keep_blocks, uint32_t sink, uint32_t recent, uint32_t n_seq, uint32_t nk, uint32_t d,
+                          void* const* cache_out, uint32_t s_cap_out, float* weights_out, int32_t* kept,
+                          int32_t* lengths_out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

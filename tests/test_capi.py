@@ -149,3 +149,57 @@ def test_missing_library_fails_loudly(monkeypatch, tmp_path):
     monkeypatch.setattr(_lib, "_lib", None)
     with pytest.raises(RuntimeError, match="missing"):
         _lib.lib()
+
+
+def test_kv_q8_argument_validation(lib):
+    """The 8-bit KV cache's entry points refuse before any launch."""
+    fake, odd = 0x1000, 0x1002
+    six = lambda *p: (ctypes.c_void_p * 6)(*p)  # noqa: E731
+    c = six(*[fake] * 6)
+    write = lambda **m: lib.t2h_qk_norm_rope_cache_q8(*{**dict(  # noqa: E731
+        q=fake, qr=512, k=fake, kr=256, v=fake, vr=256, qw=None, kw=None, eps=1e-6, theta=0.0, ln=fake, ct=None, off=None,
+        n=4, s=1, nh=4, nk=2, d=128, out=fake, c=c, cap=128, st=None), **m}.values())
+    decode = lambda **m: lib.t2h_attn_decode_q8(*{**dict(  # noqa: E731
+        q=fake, qr=512, k=fake, kr=256, v=fake, vr=256, qw=None, kw=None, eps=1e-6, theta=0.0, ln=fake, off=None, c=c, cap=128,
+        w=None, wo=None, out=fake, s=1, nh=4, nk=2, d=128, ws=fake, nb=1 << 20, st=None), **m}.values())
+    chunk = lambda **m: lib.t2h_flash_attn_prefill_q8(*{**dict(  # noqa: E731
+        q=fake, c=c, cap=128, ln=fake, ct=None, w=None, wo=None, out=fake, n=4, s=1, nh=4, nk=2, d=128, scale=0.0, ws=fake,
+        nb=1 << 20, st=None), **m}.values())
+    evict = lambda **m: lib.t2h_kv_cache_q8_evict(*{**dict(  # noqa: E731
+        c=c, cap=128, ln=fake, w=fake, keep=1, sink=0, recent=0, s=1, nk=2, d=128, o=c, ocap=128, wo=fake, kept=fake, lo=fake,
+        st=None), **m}.values())
+    read = lambda **m: lib.t2h_kv_cache_q8_dequantize(*{**dict(  # noqa: E731
+        c=c, cap=128, ln=fake, s=1, nk=2, d=128, k=fake, v=fake, st=None), **m}.values())
+    for fn in (write, decode, chunk, evict, read):
+        assert fn(ln=None) == 1
+        assert fn(c=None) == 1
+        assert fn(c=six(fake, fake, None, fake, fake, fake)) == 1
+        assert fn(d=64) == 4
+        assert fn(cap=100) == 2 and fn(cap=0) == 2
+        assert fn(s=0) == 2 and fn(nk=0) == 2
+        assert fn(c=six(odd, fake, fake, fake, fake, fake)) == 7
+        assert fn(c=six(fake, fake, fake, odd, fake, fake)) == 7
+        assert fn(s=1 << 23) == 2
+    for fn in (write, decode, chunk):
+        assert fn(nh=5) == 2
+        assert fn(nh=34, qr=34 * 128) == 4 if fn is not chunk else fn(nh=34) == 4
+        assert fn(out=None) == 1 and fn(q=None) == 1
+    for fn in (write, decode):
+        assert fn(qw=fake) == 1
+        assert fn(qr=511) == 2 and fn(kr=255) == 2 and fn(vr=0) == 2
+    for fn in (decode, chunk):
+        assert fn(w=fake) == 1 and fn(wo=fake) == 1
+        assert fn(nb=8) == 6
+        assert fn(ws=0x1008) == 7 and fn(ws=None) == 1
+    assert write(n=0) == 0 and chunk(n=0) == 0
+    assert lib.t2h_attn_decode_q8_workspace_bytes(1, 4, 2, 64, 128, 0) == 0
+    assert lib.t2h_attn_decode_q8_workspace_bytes(1, 4, 2, 128, 100, 0) == 0
+    assert lib.t2h_attn_decode_q8_workspace_bytes(1, 4, 2, 128, 128, 1) > 0
+    assert evict(keep=0) == 5 and evict(sink=65) == 5 and evict(sink=40, recent=40) == 5
+    assert evict(w=None) == 1 and evict(kept=None) == 1 and evict(lo=None) == 1
+    # in place by half, and a smaller output that could not hold what stays
+    assert evict(o=six(fake, fake, fake, fake, fake, 0x2000)) == 5
+    other = six(*[0x2000] * 6)
+    assert evict(o=other, ocap=64, wo=0x3000) == 2
+    assert evict(ocap=192) == 2 and evict(o=other, ocap=192) == 2
+    assert evict(o=None) == 1

@@ -125,6 +125,15 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "t2h_token_select_chunks": (_i32, [_vp, _vp, _u32, _vp, _vp, _vp]),
     "t2h_add": (_i32, [_vp, _vp, _vp, _i32, _u64, _vp]),
     "t2h_slice_last_token": (_i32, [_vp, _vp, _i32, _u32, _u32, _u32, _vp]),
+    "t2h_qk_norm_rope_cache_q8": (_i32, [_vp, _u64, _vp, _u64, _vp, _u64, _vp, _vp, _f32, _f32, _vp, _vp, _vp]
+                                  + [_u32] * 5 + [_vp, _vp, _u32, _vp]),
+    "t2h_attn_decode_q8_workspace_bytes": (_sz, [_u32] * 5 + [_i32]),
+    "t2h_attn_decode_q8": (_i32, [_vp, _u64, _vp, _u64, _vp, _u64, _vp, _vp, _f32, _f32, _vp, _vp, _vp, _u32, _vp, _vp,
+                                  _vp] + [_u32] * 4 + [_vp, _sz, _vp]),
+    "t2h_flash_attn_prefill_q8_workspace_bytes": (_sz, [_u32] * 5 + [_i32]),
+    "t2h_flash_attn_prefill_q8": (_i32, [_vp, _vp, _u32, _vp, _vp, _vp, _vp, _vp] + [_u32] * 5 + [_f32, _vp, _sz, _vp]),
+    "t2h_kv_cache_q8_dequantize": (_i32, [_vp, _u32, _vp, _u32, _u32, _u32, _vp, _vp, _vp]),
+    "t2h_kv_cache_q8_evict": (_i32, [_vp, _u32, _vp, _vp] + [_u32] * 6 + [_vp, _u32, _vp, _vp, _vp, _vp]),
 }
 
 

@@ -1,0 +1,577 @@
+// Writing, reading back and evicting the 8-bit KV cache (layout and rounding: kv_q8.h).
+#include <math.h>
+
+#include "kv_q8.h"
+#include "kv_q8_args.h"
+#include "rope.h"
+
+namespace t2h {
+
+// ------------------------------------------------------------------------------------------------- chunk write --
+//
+// For every token t of a chunk, per head: RMSNorm over 128 dims and rotate-half RoPE at position length + offset + t of
+// q and k; q goes out in bf16, k and v go to the cache.  Bound by memory: a token's q, k and v are read once in fp32.
+// One launch holds two kinds of blocks: those of q (a wave takes 8 heads of a token), and one for each (sequence, cache
+// block that the chunk touches, KV head), which holds the 64 tokens in registers because a finished block's scale needs
+// all of them before the first is rounded.
+
+struct Q8WriteArgs {
+    const float* q;
+    const float* k;
+    const float* v;
+    size_t q_row, k_row, v_row;
+    const float* q_norm_w;
+    const float* k_norm_w;
+    float eps;
+    double log2_theta;  // rope: whether to rotate
+    int rope;
+    const int32_t* lengths;
+    const int32_t* counts;
+    const int32_t* offsets;
+    uint32_t n, n_seq, nh;
+    uint32_t kv_blocks;  // cache blocks that n tokens can touch
+    uint32_t kv_grid;    // kv_blocks * nk * n_seq
+    uint16_t* q_out;
+    float* q_f32;  // or q in fp32
+    KvQ8 c;
+};
+
+constexpr int Q8W_HEADS = 8;  // q heads a wave
+
+__device__ __forceinline__ void q8_write_q(const Q8WriteArgs& a, uint64_t unit) {
+    const int lane = threadIdx.x & 63;
+    const uint32_t groups = (a.nh + Q8W_HEADS - 1) / Q8W_HEADS;
+    if (unit >= (uint64_t)a.n_seq * a.n * groups) return;
+    const uint64_t row = unit / groups;
+    const uint32_t h0 = (uint32_t)(unit - row * groups) * Q8W_HEADS;
+    const uint32_t seq = (uint32_t)(row / a.n), t = (uint32_t)(row - (uint64_t)seq * a.n);
+    uint16_t* out = a.q_out + (row * a.nh + h0) * Q8_D;
+    const uint32_t heads = a.nh - h0 < Q8W_HEADS ? a.nh - h0 : Q8W_HEADS;
+    const int len = a.lengths[seq];
+    const int count = a.counts ? a.counts[seq] : (int)a.n;
+    if (len < 0 || (int)t >= count) {  // padding
+        if (a.q_f32) return;
+        for (uint32_t j = 0; j < heads; ++j) reinterpret_cast<uint32_t*>(out + j * Q8_D)[lane] = 0u;
+        return;
+    }
+    float x0[Q8W_HEADS], x1[Q8W_HEADS];
+#pragma unroll
+    for (int j = 0; j < Q8W_HEADS; ++j) {
+        const uint32_t h = h0 + (j < (int)heads ? j : heads - 1);  // past the last head: re-read it, store nothing
+        const float* x = a.q + row * a.q_row + (size_t)h * Q8_D;
+        x0[j] = x[lane];
+        x1[j] = x[lane + 64];
+    }
+    const bool has_w = a.q_norm_w != nullptr;
+    const float w0 = has_w ? a.q_norm_w[lane] : 1.0f, w1 = has_w ? a.q_norm_w[lane + 64] : 1.0f;
+    float cs = 1.0f, sn = 0.0f;
+    if (a.rope) rope_at(rope_turns(lane, a.log2_theta), len + (a.offsets ? a.offsets[seq] : 0) + (int)t, cs, sn);
+#pragma unroll
+    for (int j = 0; j < Q8W_HEADS; ++j) {
+        if (j >= (int)heads) break;
+        float r0, r1;
+        norm_rope_pair(x0[j], x1[j], has_w, w0, w1, a.eps, cs, sn, a.rope != 0, r0, r1);
+        if (a.q_f32) {
+            a.q_f32[(row * a.nh + h0 + j) * Q8_D + lane] = r0;
+            a.q_f32[(row * a.nh + h0 + j) * Q8_D + lane + 64] = r1;
+            continue;
+        }
+        out[j * Q8_D + lane] = (uint16_t)f32_to_bf16_bits(r0);
+        out[j * Q8_D + lane + 64] = (uint16_t)f32_to_bf16_bits(r1);
+    }
+}
+
+// One cache block of one head: tokens 64 b + 16 wave + i in wave `wave`, row i; a lane holds key dims lane and lane + 64
+// and value dims 2 lane and 2 lane + 1.
+__device__ __forceinline__ void q8_write_block(const Q8WriteArgs& a, uint32_t seq, uint32_t h, Q8Span s, int b,
+                                               uint32_t* kbytes, uint32_t* red) {
+    constexpr int ROWS = Q8_BLOCK / 4;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int p0 = b * Q8_BLOCK + wave * ROWS;
+    const bool whole = (b + 1) * Q8_BLOCK <= s.end;
+    const bool has_w = a.k_norm_w != nullptr;
+    const float w0 = has_w ? a.k_norm_w[lane] : 1.0f, w1 = has_w ? a.k_norm_w[lane + 64] : 1.0f;
+    const size_t tail = a.c.tail_at(seq, h);
+    const int base = a.lengths[seq];  // token p is row p - base of the chunk
+    const int off = a.offsets ? a.offsets[seq] : 0;
+    float k0[ROWS], k1[ROWS], v0[ROWS], v1[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        const int p = p0 + i;
+        k0[i] = k1[i] = v0[i] = v1[i] = 0.0f;
+        if (p >= s.len && p < s.end) {
+            const size_t row = (size_t)seq * a.n + (size_t)(p - base);
+            const float* kx = a.k + row * a.k_row + (size_t)h * Q8_D;
+            const float* vx = a.v + row * a.v_row + (size_t)h * Q8_D;
+            k0[i] = kx[lane];
+            k1[i] = kx[lane + 64];
+            v0[i] = vx[2 * lane];
+            v1[i] = vx[2 * lane + 1];
+        }
+    }
+    const double turns = a.rope ? rope_turns(lane, a.log2_theta) : 0.0;
+    uint32_t kmax = 0, vmax = 0;
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        const int p = p0 + i;
+        if (p >= s.len && p < s.end) {
+            float cs = 1.0f, sn = 0.0f, r0, r1;
+            if (a.rope) rope_at(turns, p + off, cs, sn);
+            norm_rope_pair(k0[i], k1[i], has_w, w0, w1, a.eps, cs, sn, a.rope != 0, r0, r1);
+            k0[i] = bf16_bits_to_f32(f32_to_bf16_bits(r0));
+            k1[i] = bf16_bits_to_f32(f32_to_bf16_bits(r1));
+            v0[i] = bf16_bits_to_f32(f32_to_bf16_bits(v0[i]));
+            v1[i] = bf16_bits_to_f32(f32_to_bf16_bits(v1[i]));
+        } else if (whole) {  // a token of the tail that this chunk completes
+            const int r = wave * ROWS + i;
+            k0[i] = bf16_bits_to_f32(a.c.kt[tail + r * Q8_D + lane]);
+            k1[i] = bf16_bits_to_f32(a.c.kt[tail + r * Q8_D + lane + 64]);
+            v0[i] = bf16_bits_to_f32(a.c.vt[tail + (2 * lane) * Q8_BLOCK + r]);
+            v1[i] = bf16_bits_to_f32(a.c.vt[tail + (2 * lane + 1) * Q8_BLOCK + r]);
+        }
+        kmax = max(kmax, max(abs_bits(k0[i]), abs_bits(k1[i])));
+        vmax = max(vmax, max(abs_bits(v0[i]), abs_bits(v1[i])));
+    }
+    if (!whole) {
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+            const int p = p0 + i, r = wave * ROWS + i;
+            if (p < s.len || p >= s.end) continue;
+            a.c.kt[tail + r * Q8_D + lane] = (uint16_t)f32_to_bf16_bits(k0[i]);
+            a.c.kt[tail + r * Q8_D + lane + 64] = (uint16_t)f32_to_bf16_bits(k1[i]);
+            a.c.vt[tail + (2 * lane) * Q8_BLOCK + r] = (uint16_t)f32_to_bf16_bits(v0[i]);
+            a.c.vt[tail + (2 * lane + 1) * Q8_BLOCK + r] = (uint16_t)f32_to_bf16_bits(v1[i]);
+        }
+        return;
+    }
+    kmax = wave_max_u32(kmax);
+    vmax = wave_max_u32(vmax);
+    if (lane == 0) {
+        red[wave] = kmax;
+        red[4 + wave] = vmax;
+    }
+    __syncthreads();
+    float ks, kinv, vs, vinv;
+    q8_scale(max(max(red[0], red[1]), max(red[2], red[3])), ks, kinv);
+    q8_scale(max(max(red[4], red[5]), max(red[6], red[7])), vs, vinv);
+    // keys: bytes through LDS, so that they leave as 16-byte stores
+    uint8_t* kb = reinterpret_cast<uint8_t*>(kbytes);
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        kb[(wave * ROWS + i) * Q8_D + lane] = (uint8_t)q8_code(k0[i], kinv);
+        kb[(wave * ROWS + i) * Q8_D + lane + 64] = (uint8_t)q8_code(k1[i], kinv);
+    }
+    const size_t at = a.c.block_at(seq, (uint32_t)b, h);
+    uint4 lo, hi;
+    lo.x = q8_pack4(v0[0], v0[1], v0[2], v0[3], vinv);
+    lo.y = q8_pack4(v0[4], v0[5], v0[6], v0[7], vinv);
+    lo.z = q8_pack4(v0[8], v0[9], v0[10], v0[11], vinv);
+    lo.w = q8_pack4(v0[12], v0[13], v0[14], v0[15], vinv);
+    hi.x = q8_pack4(v1[0], v1[1], v1[2], v1[3], vinv);
+    hi.y = q8_pack4(v1[4], v1[5], v1[6], v1[7], vinv);
+    hi.z = q8_pack4(v1[8], v1[9], v1[10], v1[11], vinv);
+    hi.w = q8_pack4(v1[12], v1[13], v1[14], v1[15], vinv);
+    int8_t* vb = a.c.v + at + (size_t)(2 * lane) * Q8_BLOCK + wave * ROWS;
+    *reinterpret_cast<uint4*>(vb) = lo;
+    *reinterpret_cast<uint4*>(vb + Q8_BLOCK) = hi;
+    __syncthreads();
+    uint4* kout = reinterpret_cast<uint4*>(a.c.k + at);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) kout[threadIdx.x + 256 * i] = reinterpret_cast<const uint4*>(kbytes)[threadIdx.x + 256 * i];
+    if (threadIdx.x == 0) {
+        a.c.ks[a.c.scale_at(seq, (uint32_t)b, h)] = ks;
+        a.c.vs[a.c.scale_at(seq, (uint32_t)b, h)] = vs;
+    }
+}
+
+__global__ __launch_bounds__(256) void q8_write_kernel(const Q8WriteArgs a) {
+    __shared__ __align__(16) uint32_t kbytes[Q8_BYTES / 4];
+    __shared__ uint32_t red[8];
+    if (blockIdx.x >= a.kv_grid) {
+        q8_write_q(a, (uint64_t)(blockIdx.x - a.kv_grid) * 4 + (threadIdx.x >> 6));
+        return;
+    }
+    const uint32_t h = blockIdx.x % a.c.nk;
+    const uint32_t rest = blockIdx.x / a.c.nk;
+    const uint32_t j = rest % a.kv_blocks, seq = rest / a.kv_blocks;
+    const Q8Span s = q8_span(a.lengths, a.counts, seq, a.n, a.c.nb);
+    if (s.len >= s.end) return;
+    const int first = s.len / Q8_BLOCK, last = (s.end - 1) / Q8_BLOCK;
+    const int b = first + (int)j;
+    if (b > last) return;
+    // The block that the old tail's rows belong to is completed before the chunk's own rest becomes the tail: where both
+    // happen, one thread block does them in that order.
+    const bool chained = last > first && s.len % Q8_BLOCK != 0 && s.end % Q8_BLOCK != 0;
+    if (chained && b == last) return;
+    q8_write_block(a, seq, h, s, b, kbytes, red);
+    if (chained && j == 0) {
+        __syncthreads();
+        q8_write_block(a, seq, h, s, last, kbytes, red);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------- read back --
+//
+// The cache's values as the token-major bf16 rows [n_seq][s_cap][nk][128] of the framework's other caches, code times
+// scale rounded once; zeros from the length on.  Bound by the bf16 rows that it writes.
+
+struct Q8ReadArgs {
+    KvQ8 c;
+    const int32_t* lengths;
+    uint16_t* k_out;
+    uint16_t* v_out;
+};
+
+__global__ __launch_bounds__(256) void q8_read_kernel(const Q8ReadArgs a) {
+    __shared__ uint32_t vb[Q8_D][Q8_BLOCK / 4 + 1];
+    const uint32_t h = blockIdx.x % a.c.nk;
+    const uint32_t rest = blockIdx.x / a.c.nk;
+    const uint32_t b = rest % a.c.nb, seq = rest / a.c.nb;
+    const int cap = (int)(a.c.nb * Q8_BLOCK);
+    const int given = a.lengths[seq];
+    const int len = given < 0 ? 0 : (given < cap ? given : cap);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int p0 = (int)b * Q8_BLOCK;
+    const bool whole = p0 + Q8_BLOCK <= len;
+    const size_t at = a.c.block_at(seq, b, h), tail = a.c.tail_at(seq, h);
+    float ks = 0.0f, vs = 0.0f;
+    if (whole) {
+        ks = a.c.ks[a.c.scale_at(seq, b, h)];
+        vs = a.c.vs[a.c.scale_at(seq, b, h)];
+        const uint32_t* v = reinterpret_cast<const uint32_t*>(a.c.v + at);
+        for (int i = threadIdx.x; i < Q8_BYTES / 4; i += 256) vb[i / 16][i % 16] = v[i];
+    }
+    __syncthreads();
+    for (int i = wave; i < Q8_BLOCK; i += 4) {
+        const int p = p0 + i;
+        uint32_t kk = 0, vv = 0;  // dims 2 lane, 2 lane + 1
+        if (whole) {
+            const uint32_t two = reinterpret_cast<const uint16_t*>(a.c.k + at + i * Q8_D)[lane];
+            kk = pack_bf16x2(q8_value(two, 0) * ks, q8_value(two, 1) * ks);
+            vv = pack_bf16x2(q8_value(vb[2 * lane][i / 4], i % 4) * vs, q8_value(vb[2 * lane + 1][i / 4], i % 4) * vs);
+        } else if (p < len) {
+            kk = reinterpret_cast<const uint32_t*>(a.c.kt + tail + i * Q8_D)[lane];
+            vv = (uint32_t)a.c.vt[tail + (2 * lane) * Q8_BLOCK + i] | (uint32_t)a.c.vt[tail + (2 * lane + 1) * Q8_BLOCK + i] << 16;
+        }
+        const size_t row = (((size_t)seq * cap + p) * a.c.nk + h) * Q8_D;
+        reinterpret_cast<uint32_t*>(a.k_out + row)[lane] = kk;
+        reinterpret_cast<uint32_t*>(a.v_out + row)[lane] = vv;
+    }
+}
+
+// --------------------------------------------------------------------------------------------------- eviction --
+//
+// Per (sequence, KV head), of the F whole blocks' tokens 64 min(F, keep) stay: the first `sink`, the last `recent`, then
+// by accumulated weight (ties: the lowest index; a NaN ranks above every number), in the order of the tokens.
+// The choice is a radix selection of the last weight that stays, 11 + 11 + 10 bits of an order-preserving key, each
+// digit one pass over the weights and a histogram in LDS; then ballots give each token its place.  A second kernel moves
+// the tokens: block by block it gathers 64 of them, finds their new scale and rounds them again.
+
+struct Q8EvictArgs {
+    KvQ8 c, o;
+    const int32_t* lengths;
+    const float* w_in;
+    float* w_out;
+    int32_t* kept;  // [n_seq][nk][64 keep]
+    int32_t* lengths_out;
+    uint32_t keep, sink, recent;
+    uint32_t jobs;  // thread blocks that share a head's output blocks (1 where output and input are the same cache)
+};
+
+__device__ __forceinline__ int q8_length(const int32_t* lengths, uint32_t seq, uint32_t nb) {
+    const int cap = (int)(nb * Q8_BLOCK), given = lengths[seq];
+    return given < 0 ? 0 : (given < cap ? given : cap);
+}
+
+__device__ __forceinline__ uint32_t evict_key(const float* w, int t, int full, const Q8EvictArgs& a) {
+    if (t < (int)a.sink || t >= full - (int)a.recent) return 0xffffffffu;
+    const float x = w[t] + 0.0f;  // -0 ranks as 0
+    if (x != x) return 0xfffffffeu;
+    const uint32_t u = __float_as_uint(x);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+constexpr int EV_THREADS = 1024;
+constexpr int EV_WAVES = EV_THREADS / 64;
+
+__global__ __launch_bounds__(EV_THREADS) void q8_evict_select_kernel(const Q8EvictArgs a) {
+    __shared__ uint32_t hist[2048];
+    __shared__ uint32_t wsum[EV_WAVES][2];
+    __shared__ uint32_t found[2];
+    const uint32_t h = blockIdx.x % a.c.nk, seq = blockIdx.x / a.c.nk;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int len = q8_length(a.lengths, seq, a.c.nb);
+    const int blocks = len / Q8_BLOCK, full = blocks * Q8_BLOCK;
+    const int most = (int)a.keep * Q8_BLOCK;
+    const int stay = full < most ? full : most;
+    int32_t* kept = a.kept + (size_t)blockIdx.x * most;
+    if (h == 0 && tid == 0) a.lengths_out[seq] = a.lengths[seq] < 0 ? a.lengths[seq] : len - full + stay;
+    for (int i = (stay < full ? stay : 0) + tid; i < most; i += EV_THREADS) kept[i] = i < stay ? i : -1;
+    if (stay == full) return;
+    const float* w = a.w_in + (size_t)blockIdx.x * a.c.nb * Q8_BLOCK;
+
+    uint32_t prefix = 0, need = (uint32_t)stay;  // of the tokens whose key begins with prefix, `need` stay
+#pragma unroll
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+        const uint32_t mask = pass == 0 ? 0u : ~0u << (shift + bits);
+        for (int i = tid; i < 2048; i += EV_THREADS) hist[i] = 0;
+        __syncthreads();
+        for (int t = tid; t < full; t += EV_THREADS) {
+            const uint32_t key = evict_key(w, t, full, a);
+            if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & ((1u << bits) - 1u)], 1u);
+        }
+        __syncthreads();
+        // bins from the top: thread i holds bins 2047 - 2 i and 2046 - 2 i
+        const uint32_t c0 = hist[2047 - 2 * tid], c1 = hist[2046 - 2 * tid];
+        uint32_t run = c0 + c1;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const uint32_t o = (uint32_t)__shfl_up((int)run, off, T2H_WAVE);
+            if (lane >= off) run += o;
+        }
+        if (lane == 63) wsum[wave][0] = run;
+        __syncthreads();
+        uint32_t before = run - c0 - c1;
+        for (int i = 0; i < wave; ++i) before += wsum[i][0];
+        if (before < need && need <= before + c0) {
+            found[0] = 2047u - 2u * (uint32_t)tid;
+            found[1] = need - before;
+        } else if (before + c0 < need && need <= before + c0 + c1) {
+            found[0] = 2046u - 2u * (uint32_t)tid;
+            found[1] = need - before - c0;
+        }
+        __syncthreads();
+        prefix |= found[0] << shift;
+        need = found[1];
+    }
+    // prefix is the smallest key that stays, and `need` of the tokens that have it; each wave takes a run of tokens
+    const int per = ((full + EV_WAVES - 1) / EV_WAVES + 63) / 64 * 64;
+    const int t0 = wave * per, t1 = t0 + per < full ? t0 + per : full;
+    uint32_t above = 0, equal = 0;
+    for (int t = t0; t < t1; t += 64) {
+        const uint32_t key = t + lane < t1 ? evict_key(w, t + lane, full, a) : 0u;
+        above += __popcll(__ballot(t + lane < t1 && key > prefix));
+        equal += __popcll(__ballot(t + lane < t1 && key == prefix));
+    }
+    if (lane == 0) {
+        wsum[wave][0] = above;
+        wsum[wave][1] = equal;
+    }
+    __syncthreads();
+    above = equal = 0;
+    for (int i = 0; i < wave; ++i) {
+        above += wsum[i][0];
+        equal += wsum[i][1];
+    }
+    const uint64_t below = (1ull << lane) - 1;
+    for (int t = t0; t < t1; t += 64) {
+        const bool in = t + lane < t1;
+        const uint32_t key = in ? evict_key(w, t + lane, full, a) : 0u;
+        const uint64_t ma = __ballot(in && key > prefix), me = __ballot(in && key == prefix);
+        const uint32_t a0 = above + __popcll(ma & below), e0 = equal + __popcll(me & below);
+        const bool stays = in && (key > prefix || (key == prefix && e0 < need));
+        if (stays) kept[a0 + (e0 < need ? e0 : need)] = t + lane;
+        above += __popcll(ma);
+        equal += __popcll(me);
+    }
+}
+
+// Keys (blockIdx.y 0, with the weights) or values (1) of one head: output blocks job, job + jobs, ...  Where the output
+// is the input's own cache one thread block walks a head's blocks in order: token i of the output comes from a token
+// j >= i, so block b is read before it is overwritten, and no later block needs what it overwrites.
+__global__ __launch_bounds__(256) void q8_evict_move_kernel(const Q8EvictArgs a) {
+    __shared__ int from[Q8_BLOCK];
+    __shared__ float fs[Q8_BLOCK];
+    __shared__ uint32_t red[4];
+    const uint32_t h = blockIdx.x % a.c.nk;
+    const uint32_t rest = blockIdx.x / a.c.nk;
+    const uint32_t job = rest % a.jobs, seq = rest / a.jobs;
+    const bool values = blockIdx.y != 0;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int len = q8_length(a.lengths, seq, a.c.nb);
+    const int blocks = len / Q8_BLOCK;
+    const int stay = blocks < (int)a.keep ? blocks : (int)a.keep;
+    const bool in_place = a.c.k == a.o.k;
+    const size_t head = (size_t)seq * a.c.nk + h;
+    const int32_t* kept = a.kept + head * a.keep * Q8_BLOCK;
+    const float* w_in = a.w_in + head * a.c.nb * Q8_BLOCK;
+    float* w_out = a.w_out + head * a.o.nb * Q8_BLOCK;
+    const bool all = stay == blocks;  // nothing leaves: blocks are copied as they are
+    if (in_place && all && a.w_in == a.w_out) return;
+    for (int b = (int)job; b < stay; b += (int)a.jobs) {
+        __syncthreads();
+        if (tid < Q8_BLOCK) {
+            const int t = kept[b * Q8_BLOCK + tid];
+            from[tid] = t;
+            fs[tid] = (values ? a.c.vs : a.c.ks)[a.c.scale_at(seq, (uint32_t)t / Q8_BLOCK, h)];
+        }
+        __syncthreads();
+        uint32_t top = 0;
+        const size_t to = a.o.block_at(seq, (uint32_t)b, h);
+        float inv, s;
+        if (!values) {
+            const int r = tid >> 2, part = tid & 3;
+            const int t = from[r];
+            const float f = fs[r];
+            const uint4* src = reinterpret_cast<const uint4*>(a.c.k + a.c.block_at(seq, (uint32_t)t / Q8_BLOCK, h) +
+                                                              (t % Q8_BLOCK) * Q8_D + part * 32);
+            uint4 x[2] = {src[0], src[1]};
+            uint32_t* u = reinterpret_cast<uint32_t*>(x);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) top = max(top, abs_bits(q8_value(u[i / 4], i % 4) * f));
+            const float wt = tid < Q8_BLOCK ? w_in[from[tid]] : 0.0f;
+            top = wave_max_u32(top);
+            if (lane == 0) red[wave] = top;
+            __syncthreads();
+            q8_scale(max(max(red[0], red[1]), max(red[2], red[3])), s, inv);
+            if (all) s = f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (!all) u[i] = q8_pack4(q8_value(u[i], 0) * f, q8_value(u[i], 1) * f, q8_value(u[i], 2) * f, q8_value(u[i], 3) * f, inv);
+            uint4* dst = reinterpret_cast<uint4*>(a.o.k + to + r * Q8_D + part * 32);
+            dst[0] = x[0];
+            dst[1] = x[1];
+            if (tid < Q8_BLOCK) w_out[b * Q8_BLOCK + tid] = wt;
+        } else {
+            // a lane is a token, a wave 32 dims: 64 tokens of a dim are a few short runs of bytes
+            const int t = from[lane];
+            const float f = fs[lane];
+            const int8_t* src = a.c.v + a.c.block_at(seq, (uint32_t)t / Q8_BLOCK, h) + (size_t)wave * 32 * Q8_BLOCK + t % Q8_BLOCK;
+            int8_t x[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[i] = src[i * Q8_BLOCK];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) top = max(top, abs_bits((float)x[i] * f));
+            top = wave_max_u32(top);
+            if (lane == 0) red[wave] = top;
+            __syncthreads();
+            q8_scale(max(max(red[0], red[1]), max(red[2], red[3])), s, inv);
+            if (all) s = f;
+            int8_t* dst = a.o.v + to + (size_t)wave * 32 * Q8_BLOCK + lane;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) dst[i * Q8_BLOCK] = all ? x[i] : (int8_t)q8_code((float)x[i] * f, inv);
+        }
+        if (tid == 0) (values ? a.o.vs : a.o.ks)[a.o.scale_at(seq, (uint32_t)b, h)] = s;
+    }
+    if (job != 0) return;
+    // the tail's tokens: their rows where the output is another cache, and their weights
+    if (!in_place) {
+        const uint4* src = reinterpret_cast<const uint4*>((values ? a.c.vt : a.c.kt) + a.c.tail_at(seq, h));
+        uint4* dst = reinterpret_cast<uint4*>((values ? a.o.vt : a.o.kt) + a.o.tail_at(seq, h));
+        for (int i = tid; i < Q8_BYTES * 2 / 16; i += 256) dst[i] = src[i];
+    }
+    if (!values) {
+        const int r = len - blocks * Q8_BLOCK;
+        const float wt = tid < r ? w_in[blocks * Q8_BLOCK + tid] : 0.0f;
+        __syncthreads();
+        if (tid < r) w_out[stay * Q8_BLOCK + tid] = wt;
+    }
+}
+
+int q8_write_launch(const float* q, uint64_t q_row, const float* k, uint64_t k_row, const float* v, uint64_t v_row,
+                    const float* q_norm_w, const float* k_norm_w, float eps, float theta, const int32_t* lengths,
+                    const int32_t* counts, const int32_t* rope_offsets, uint32_t n, uint32_t n_seq, uint32_t nh,
+                    uint32_t nk, uint32_t d, void* q_out, bool q_f32, void* const* cache, uint32_t s_cap, void* stream) {
+    Q8WriteArgs a;
+    if (!q || !k || !v || !lengths || !q_out) return T2H_ERR_NULL;
+    if ((q_norm_w == nullptr) != (k_norm_w == nullptr)) return T2H_ERR_NULL;
+    if (const int e = q8_cache(cache, s_cap, n_seq, nh, nk, d, a.c)) return e;
+    if (q_row < (uint64_t)nh * d || k_row < (uint64_t)nk * d || v_row < (uint64_t)nk * d) return T2H_ERR_SHAPE;
+    if (reinterpret_cast<uintptr_t>(q_out) & 3) return T2H_ERR_ALIGN;
+    if (n == 0) return T2H_OK;
+    const uint64_t kv_blocks = ((uint64_t)n + 2 * Q8_BLOCK - 2) / Q8_BLOCK;
+    const uint64_t kv_grid = kv_blocks * nk * n_seq;
+    const uint64_t units = (uint64_t)n_seq * n * ((nh + Q8W_HEADS - 1) / Q8W_HEADS);
+    if (n > 0x3fffffffu || kv_grid + (units + 3) / 4 > 0x7fffffffu) return T2H_ERR_SHAPE;
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.q_row = (size_t)q_row;
+    a.k_row = (size_t)k_row;
+    a.v_row = (size_t)v_row;
+    a.q_norm_w = q_norm_w;
+    a.k_norm_w = k_norm_w;
+    a.eps = eps;
+    a.rope = theta > 0.0f;
+    a.log2_theta = a.rope ? log2((double)theta) : 0.0;
+    a.lengths = lengths;
+    a.counts = counts;
+    a.offsets = rope_offsets;
+    a.n = n;
+    a.n_seq = n_seq;
+    a.nh = nh;
+    a.kv_blocks = (uint32_t)kv_blocks;
+    a.kv_grid = (uint32_t)kv_grid;
+    a.q_out = reinterpret_cast<uint16_t*>(q_out);
+    a.q_f32 = q_f32 ? reinterpret_cast<float*>(q_out) : nullptr;
+    hipLaunchKernelGGL(q8_write_kernel, dim3((uint32_t)(kv_grid + (units + 3) / 4)), dim3(256), 0,
+                       reinterpret_cast<hipStream_t>(stream), a);
+    T2H_LAUNCH_CHECK();
+    return T2H_OK;
+}
+
+}  // namespace t2h
+
+using namespace t2h;
+
+extern "C" int t2h_qk_norm_rope_cache_q8(const float* q, uint64_t q_row, const float* k, uint64_t k_row, const float* v,
+                                         uint64_t v_row, const float* q_norm_w, const float* k_norm_w, float eps,
+                                         float theta, const int32_t* lengths, const int32_t* counts,
+                                         const int32_t* rope_offsets, uint32_t n, uint32_t n_seq, uint32_t nh, uint32_t nk,
+                                         uint32_t d, void* q_out, void* const* cache, uint32_t s_cap, void* stream) {
+    return q8_write_launch(q, q_row, k, k_row, v, v_row, q_norm_w, k_norm_w, eps, theta, lengths, counts, rope_offsets, n,
+                           n_seq, nh, nk, d, q_out, false, cache, s_cap, stream);
+}
+
+extern "C" int t2h_kv_cache_q8_dequantize(void* const* cache, uint32_t s_cap, const int32_t* lengths, uint32_t n_seq,
+                                          uint32_t nk, uint32_t d, void* k_out, void* v_out, void* stream) {
+    Q8ReadArgs a;
+    if (!lengths || !k_out || !v_out) return T2H_ERR_NULL;
+    if (const int e = q8_cache(cache, s_cap, n_seq, nk, nk, d, a.c)) return e;
+    if ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 3) return T2H_ERR_ALIGN;
+    a.lengths = lengths;
+    a.k_out = reinterpret_cast<uint16_t*>(k_out);
+    a.v_out = reinterpret_cast<uint16_t*>(v_out);
+    const uint64_t grid = (uint64_t)n_seq * a.c.nb * nk;
+    if (grid > 0x7fffffffu) return T2H_ERR_SHAPE;
+    hipLaunchKernelGGL(q8_read_kernel, dim3((uint32_t)grid), dim3(256), 0, reinterpret_cast<hipStream_t>(stream), a);
+    T2H_LAUNCH_CHECK();
+    return T2H_OK;
+}
+
+extern "C" int t2h_kv_cache_q8_evict(void* const* cache, uint32_t s_cap, const int32_t* lengths, const float* weights,
+                                     uint32_t keep_blocks, uint32_t sink, uint32_t recent, uint32_t n_seq, uint32_t nk,
+                                     uint32_t d, void* const* cache_out, uint32_t s_cap_out, float* weights_out,
+                                     int32_t* kept, int32_t* lengths_out, void* stream) {
+    Q8EvictArgs a;
+    if (!lengths || !weights || !weights_out || !kept || !lengths_out) return T2H_ERR_NULL;
+    if (const int e = q8_cache(cache, s_cap, n_seq, nk, nk, d, a.c)) return e;
+    if (const int e = q8_cache(cache_out, s_cap_out, n_seq, nk, nk, d, a.o)) return e;
+    if (keep_blocks == 0 || keep_blocks > 0x1000000u) return T2H_ERR_ARG;
+    if ((uint64_t)sink + recent > (uint64_t)keep_blocks * Q8_BLOCK) return T2H_ERR_ARG;
+    // a cache of the output's capacity holds what stays and a tail
+    if ((uint64_t)s_cap_out < s_cap && s_cap_out < ((uint64_t)keep_blocks + 1) * Q8_BLOCK) return T2H_ERR_SHAPE;
+    const bool same = a.c.k == a.o.k;
+    if (same != (a.c.v == a.o.v) || same != (a.c.ks == a.o.ks) || same != (a.c.vs == a.o.vs) ||
+        same != (a.c.kt == a.o.kt) || same != (a.c.vt == a.o.vt))
+        return T2H_ERR_ARG;
+    if ((same || weights == weights_out) && s_cap != s_cap_out) return T2H_ERR_SHAPE;
+    a.lengths = lengths;
+    a.w_in = weights;
+    a.w_out = weights_out;
+    a.kept = kept;
+    a.lengths_out = lengths_out;
+    a.keep = keep_blocks;
+    a.sink = sink;
+    a.recent = recent;
+    const uint32_t most = keep_blocks < a.c.nb ? keep_blocks : a.c.nb;
+    a.jobs = same || weights == weights_out ? 1 : most;
+    const uint64_t grid = (uint64_t)n_seq * a.jobs * nk;
+    if (grid > 0x7fffffffu) return T2H_ERR_SHAPE;
+    hipLaunchKernelGGL(q8_evict_select_kernel, dim3(n_seq * nk), dim3(EV_THREADS), 0, reinterpret_cast<hipStream_t>(stream), a);
+    T2H_LAUNCH_CHECK();
+    hipLaunchKernelGGL(q8_evict_move_kernel, dim3((uint32_t)grid, 2), dim3(256), 0, reinterpret_cast<hipStream_t>(stream), a);
+    T2H_LAUNCH_CHECK();
+    return T2H_OK;
+}

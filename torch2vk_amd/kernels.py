@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+from dataclasses import dataclass
 
 import torch
 
@@ -1594,3 +1595,288 @@ def slice_last_token(x: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
         raise ValueError(f"output must be [{b}, 1, {h}], got {tuple(out.shape)}")
     call("t2h_slice_last_token", ptr(x), ptr(out), _OUT_DTYPES[out.dtype], b, s_len, h, stream_handle())
     return out
+
+
+# ---------------------------------------------------------- 8-bit KV cache --
+
+KV_Q8_BLOCK = 64  # tokens under one scale
+KV_Q8_MAX_GROUP = 16  # q heads of a KV head
+_Ptr6 = ctypes.c_void_p * 6
+
+
+@dataclass(frozen=True, eq=False)
+class KVCacheQ8:
+    """A KV cache in 8 bits for n_seq sequences of one layer, in blocks of 64 tokens (include/t2h.h, "8-bit KV cache").
+    Whole blocks: k int8 [n_seq, n_blocks, nk, 64, 128], v int8 [n_seq, n_blocks, nk, 128, 64] and their fp32 scales
+    [n_seq, n_blocks, nk]; a sequence's unfinished block: k_tail bf16 [n_seq, nk, 64, 128], v_tail bf16
+    [n_seq, nk, 128, 64].  How many tokens a sequence holds is the caller's: the int32 ``lengths`` that every call takes."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+    k_tail: torch.Tensor
+    v_tail: torch.Tensor
+
+    def __post_init__(self) -> None:
+        _check(self.k, "cache k", torch.int8)
+        if self.k.dim() != 5 or self.k.shape[3:] != (KV_Q8_BLOCK, 128) or self.k.numel() == 0:
+            raise ValueError(f"cache k must be int8 [n_seq, n_blocks, nk, {KV_Q8_BLOCK}, 128], got {tuple(self.k.shape)}")
+        n_seq, nb, nk = self.k.shape[:3]
+        for name, dtype, shape in (("v", torch.int8, (n_seq, nb, nk, 128, KV_Q8_BLOCK)),
+                                   ("k_scale", torch.float32, (n_seq, nb, nk)),
+                                   ("v_scale", torch.float32, (n_seq, nb, nk)),
+                                   ("k_tail", torch.bfloat16, (n_seq, nk, KV_Q8_BLOCK, 128)),
+                                   ("v_tail", torch.bfloat16, (n_seq, nk, 128, KV_Q8_BLOCK))):
+            t = getattr(self, name)
+            _check(t, f"cache {name}", dtype, align=4 if dtype == torch.float32 else 16)
+            if tuple(t.shape) != shape or t.device != self.k.device:
+                raise ValueError(f"cache {name} must be {shape} on {self.k.device}, got {tuple(t.shape)} on {t.device}")
+
+    @property
+    def n_seq(self) -> int:
+        return self.k.shape[0]
+
+    @property
+    def s_cap(self) -> int:
+        return self.k.shape[1] * KV_Q8_BLOCK
+
+    @property
+    def nk(self) -> int:
+        return self.k.shape[2]
+
+    def _ptrs(self):
+        return _Ptr6(self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
+                     self.k_tail.data_ptr(), self.v_tail.data_ptr())
+
+
+def kv_cache_q8(n_seq: int, s_cap: int, nk: int, d: int, device) -> KVCacheQ8:
+    """An empty 8-bit cache for n_seq sequences of up to s_cap tokens (rounded up to whole blocks)."""
+    if d != 128:
+        raise ValueError(f"the 8-bit cache is built for d = 128, got {d}")
+    if n_seq < 1 or s_cap < 1 or nk < 1:
+        raise ValueError("n_seq, s_cap and nk must be positive")
+    nb = -(-s_cap // KV_Q8_BLOCK)
+
+    def zeros(*shape, dtype):
+        return torch.zeros(shape, dtype=dtype, device=device)
+
+    return KVCacheQ8(zeros(n_seq, nb, nk, KV_Q8_BLOCK, d, dtype=torch.int8), zeros(n_seq, nb, nk, d, KV_Q8_BLOCK, dtype=torch.int8),
+                     zeros(n_seq, nb, nk, dtype=torch.float32), zeros(n_seq, nb, nk, dtype=torch.float32),
+                     zeros(n_seq, nk, KV_Q8_BLOCK, d, dtype=torch.bfloat16),
+                     zeros(n_seq, nk, d, KV_Q8_BLOCK, dtype=torch.bfloat16))
+
+
+def _q8_here(cache: KVCacheQ8, *tensors: tuple[str, torch.Tensor | None]) -> None:
+    """Everything of a call is on the current device, on whose current stream it is launched."""
+    if not isinstance(cache, KVCacheQ8):
+        raise TypeError(f"cache must be a KVCacheQ8, got {type(cache).__name__}")
+    at = cache.k.get_device()
+    if at != torch.cuda.current_device():
+        raise ValueError(f"the cache is on cuda:{at}, the current device is cuda:{torch.cuda.current_device()}")
+    for name, t in tensors:
+        if t is not None and t.get_device() != at:
+            raise ValueError(f"{name} is on {t.device}, the cache on cuda:{at}")
+
+
+def _q8_ints(t: torch.Tensor | None, name: str, n_seq: int) -> None:
+    if t is None:
+        return
+    _check(t, name, torch.int32, align=4)
+    if t.numel() != n_seq:
+        raise ValueError(f"{name} must have one entry for each of {n_seq} sequences, got {tuple(t.shape)}")
+
+
+def _q8_heads(nh: int, nk: int) -> None:
+    if nh == 0 or nh % nk or nh // nk > KV_Q8_MAX_GROUP:
+        raise ValueError(f"{nh} q heads over {nk} KV heads: 1 to {KV_Q8_MAX_GROUP} for each are built")
+
+
+def _q8_rows(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: KVCacheQ8, rows: int | None,
+             q_norm_weight: torch.Tensor | None, k_norm_weight: torch.Tensor | None) -> tuple[int, tuple[int, int, int]]:
+    """q heads of fp32 [rows, heads * 128] column blocks, and their row strides."""
+    rows = int(q.shape[0]) if rows is None else rows
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        _check_strided(t, name, torch.float32)
+        if t.dim() != 2 or t.shape[0] != rows or t.shape[1] % 128:
+            raise ValueError(f"{name} must be fp32 [{rows}, heads * 128], got {tuple(t.shape)}")
+        if t.data_ptr() % 4 or (rows > 1 and t.stride(0) < t.shape[1]):
+            raise ValueError(f"{name} must hold distinct rows")
+    nh = q.shape[1] // 128
+    if k.shape[1] != cache.nk * 128 or v.shape[1] != cache.nk * 128:
+        raise ValueError(f"k and v must have the cache's {cache.nk} heads")
+    _q8_heads(nh, cache.nk)
+    if (q_norm_weight is None) != (k_norm_weight is None):
+        raise ValueError("pass both q and k norm weights or neither")
+    for t, name in ((q_norm_weight, "q_norm_weight"), (k_norm_weight, "k_norm_weight")):
+        if t is not None:
+            _check(t, name, torch.float32, align=4)
+            if t.numel() != 128:
+                raise ValueError(f"{name} must have 128 elements")
+    return nh, tuple(max(t.stride(0), t.shape[1]) for t in (q, k, v))
+
+
+def _q8_weights(cache: KVCacheQ8, weights: torch.Tensor | None,
+                weights_out: torch.Tensor | None) -> torch.Tensor | None:
+    if weights is None:
+        if weights_out is not None:
+            raise ValueError("weights_out needs weights")
+        return None
+    out = weights if weights_out is None else weights_out
+    for t, name in ((weights, "weights"), (out, "weights_out")):
+        _check(t, name, torch.float32, align=4)
+        if tuple(t.shape) != (cache.n_seq, cache.nk, cache.s_cap):
+            raise ValueError(f"{name} must be fp32 {(cache.n_seq, cache.nk, cache.s_cap)}, got {tuple(t.shape)}")
+    return out
+
+
+def qk_norm_rope_cache_q8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_out: torch.Tensor, cache: KVCacheQ8,
+                          lengths: torch.Tensor, *, theta: float, counts: torch.Tensor | None = None,
+                          rope_offsets: torch.Tensor | None = None, q_norm_weight: torch.Tensor | None = None,
+                          k_norm_weight: torch.Tensor | None = None, eps: float = RMS_EPS) -> torch.Tensor:
+    """:func:`qk_norm_rope_cache` for an 8-bit cache: q/k per-head RMSNorm + RoPE (``theta`` 0: none), q -> q_out bf16
+    [n_seq * n, nh, 128], k and v into the cache behind the ``lengths`` tokens that it holds.  q, k, v fp32
+    [n_seq * n, heads * 128] with unit column stride.  ``counts``: new tokens of each sequence, its first rows (all n when
+    None).  Token p stands at position p + rope_offsets.  ``lengths`` is not advanced."""
+    n_rows = int(q.shape[0]) if isinstance(q, torch.Tensor) and q.dim() else 0
+    _q8_here(cache, ("q", q), ("k", k), ("v", v), ("q_out", q_out), ("lengths", lengths), ("counts", counts),
+             ("rope_offsets", rope_offsets), ("q_norm_weight", q_norm_weight), ("k_norm_weight", k_norm_weight))
+    n_seq = cache.n_seq
+    if n_rows % n_seq:
+        raise ValueError(f"{n_rows} rows do not split into {n_seq} sequences")
+    nh, (qr, kr, vr) = _q8_rows(q, k, v, cache, n_rows, q_norm_weight, k_norm_weight)
+    _check(q_out, "q_out", torch.bfloat16, align=4)
+    if q_out.numel() != n_rows * nh * 128:
+        raise ValueError(f"q_out must hold [{n_rows}, {nh}, 128]")
+    _q8_ints(lengths, "lengths", n_seq)
+    _q8_ints(counts, "counts", n_seq)
+    _q8_ints(rope_offsets, "rope_offsets", n_seq)
+    if n_rows == 0:
+        return q_out
+    call("t2h_qk_norm_rope_cache_q8", ptr(q), qr, ptr(k), kr, ptr(v), vr, ptr(q_norm_weight), ptr(k_norm_weight), eps,
+         theta, ptr(lengths), ptr(counts), ptr(rope_offsets), n_rows // n_seq, n_seq, nh, cache.nk, 128, ptr(q_out),
+         cache._ptrs(), cache.s_cap, stream_handle())
+    return q_out
+
+
+def attn_decode_q8_workspace(n_seq: int, nh: int, nk: int, d: int, s_cap: int, device, *,
+                             weights: bool = False) -> torch.Tensor:
+    """Workspace of :func:`attn_decode_q8` for such a cache; calls that share one must not overlap in time."""
+    n = int(_lib.lib().t2h_attn_decode_q8_workspace_bytes(n_seq, nh, nk, d, s_cap, int(weights)))
+    if n == 0:
+        raise ValueError(f"unsupported attention shape n_seq={n_seq} nh={nh} nk={nk} d={d} s_cap={s_cap}")
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def attn_decode_q8(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, cache: KVCacheQ8, out: torch.Tensor,
+                   lengths: torch.Tensor, workspace: torch.Tensor, *, theta: float,
+                   rope_offsets: torch.Tensor | None = None, q_norm_weight: torch.Tensor | None = None,
+                   k_norm_weight: torch.Tensor | None = None, eps: float = RMS_EPS,
+                   weights: torch.Tensor | None = None, weights_out: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`attn_decode` over an 8-bit cache, one token of each sequence: q fp32 [n_seq, nh * 128], k_new / v_new fp32
+    [n_seq, nk * 128] (row strides are free), normalised and rotated as in :func:`qk_norm_rope_cache_q8`, k and v written
+    behind the ``lengths`` cached tokens, then attention over them all; out bf16 [n_seq, nh, 128].  ``weights`` fp32
+    [n_seq, nk, s_cap]: each cached token's softmax weight, summed over the KV head's q heads, is added (in place, or into
+    ``weights_out``).  ``lengths`` is not advanced."""
+    _q8_here(cache, ("q", q), ("new_k", k_new), ("new_v", v_new), ("output", out), ("lengths", lengths),
+             ("workspace", workspace), ("rope_offsets", rope_offsets), ("q_norm_weight", q_norm_weight),
+             ("k_norm_weight", k_norm_weight), ("weights", weights), ("weights_out", weights_out))
+    n_seq = cache.n_seq
+    nh, (qr, kr, vr) = _q8_rows(q, k_new, v_new, cache, n_seq, q_norm_weight, k_norm_weight)
+    _check(out, "output", torch.bfloat16, align=4)
+    if out.numel() != n_seq * nh * 128:
+        raise ValueError(f"output must hold [{n_seq}, {nh}, 128]")
+    _q8_ints(lengths, "lengths", n_seq)
+    _q8_ints(rope_offsets, "rope_offsets", n_seq)
+    _check(workspace, "workspace", torch.uint8)
+    weights_out = _q8_weights(cache, weights, weights_out)
+    call("t2h_attn_decode_q8", ptr(q), qr, ptr(k_new), kr, ptr(v_new), vr, ptr(q_norm_weight), ptr(k_norm_weight), eps,
+         theta, ptr(lengths), ptr(rope_offsets), cache._ptrs(), cache.s_cap, ptr(weights), ptr(weights_out), ptr(out),
+         n_seq, nh, cache.nk, 128, ptr(workspace), workspace.numel(), stream_handle())
+    return out
+
+
+def flash_attn_prefill_q8(q: torch.Tensor, cache: KVCacheQ8, lengths: torch.Tensor, out: torch.Tensor | None = None, *,
+                          counts: torch.Tensor | None = None, weights: torch.Tensor | None = None,
+                          weights_out: torch.Tensor | None = None, scale: float | None = None) -> torch.Tensor:
+    """Causal attention of a chunk's queries over the 8-bit cache that :func:`qk_norm_rope_cache_q8` wrote it into (the
+    same ``lengths`` and ``counts``): query t of q bf16 [n_seq, n, nh, 128] sees tokens 0 .. length + t; rows past a
+    count give zeros.  ``weights`` as in :func:`attn_decode_q8`, of all the chunk's queries."""
+    _q8_here(cache, ("q", q), ("lengths", lengths), ("output", out), ("counts", counts), ("weights", weights),
+             ("weights_out", weights_out))
+    _check(q, "q", torch.bfloat16)
+    if q.dim() != 4 or q.shape[0] != cache.n_seq or q.shape[3] != 128:
+        raise ValueError(f"q must be bf16 [{cache.n_seq}, n, nh, 128], got {tuple(q.shape)}")
+    n_seq, n, nh, _ = q.shape
+    _q8_heads(nh, cache.nk)
+    _q8_ints(lengths, "lengths", n_seq)
+    _q8_ints(counts, "counts", n_seq)
+    weights_out = _q8_weights(cache, weights, weights_out)
+    if out is None:
+        out = torch.empty_like(q)
+    _check(out, "output", torch.bfloat16)
+    if out.shape != q.shape:
+        raise ValueError(f"output must be {tuple(q.shape)}, got {tuple(out.shape)}")
+    if n == 0:
+        return out
+    nbytes = int(_lib.lib().t2h_flash_attn_prefill_q8_workspace_bytes(n, n_seq, nh, cache.nk, cache.s_cap,
+                                                                     int(weights is not None)))
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    call("t2h_flash_attn_prefill_q8", ptr(q), cache._ptrs(), cache.s_cap, ptr(lengths), ptr(counts), ptr(weights),
+         ptr(weights_out), ptr(out), n, n_seq, nh, cache.nk, 128, float(scale or 0.0), ptr(workspace), nbytes,
+         stream_handle())
+    return out
+
+
+def kv_cache_q8_dequantize(cache: KVCacheQ8, lengths: torch.Tensor, k_out: torch.Tensor | None = None,
+                           v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The cache's keys and values as bf16 [n_seq, s_cap, nk, 128], the layout of the other caches; zeros behind
+    ``lengths``."""
+    _q8_here(cache, ("lengths", lengths), ("k_out", k_out), ("v_out", v_out))
+    _q8_ints(lengths, "lengths", cache.n_seq)
+    shape = (cache.n_seq, cache.s_cap, cache.nk, 128)
+    outs = []
+    for t, name in ((k_out, "k_out"), (v_out, "v_out")):
+        t = torch.empty(shape, dtype=torch.bfloat16, device=cache.k.device) if t is None else t
+        _check(t, name, torch.bfloat16)
+        if tuple(t.shape) != shape:
+            raise ValueError(f"{name} must be bf16 {shape}, got {tuple(t.shape)}")
+        outs.append(t)
+    call("t2h_kv_cache_q8_dequantize", cache._ptrs(), cache.s_cap, ptr(lengths), cache.n_seq, cache.nk, 128, ptr(outs[0]),
+         ptr(outs[1]), stream_handle())
+    return outs[0], outs[1]
+
+
+def kv_cache_q8_evict(cache: KVCacheQ8, lengths: torch.Tensor, weights: torch.Tensor, keep_blocks: int, *, sink: int = 0,
+                      recent: int = 0, out: KVCacheQ8 | None = None,
+                      weights_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Each KV head keeps, of its whole blocks' tokens, 64 * keep_blocks: the first ``sink``, the last ``recent``, then
+    those of the most accumulated weight (``weights`` fp32 [n_seq, nk, s_cap]; ties: the earliest), in their order; the
+    unfinished block stays.  In place, or into ``out`` and ``weights_out`` [n_seq, nk, out.s_cap] (out.s_cap at least
+    64 * (keep_blocks + 1), or the cache's).  Returns the kept tokens int32 [n_seq, nk, 64 * keep_blocks] (ascending, then
+    -1) and the new lengths; ``lengths`` itself is not changed, so that every layer of a model can be evicted by it.
+    A decode that goes on adds lengths - new lengths to its ``rope_offsets``."""
+    dest = cache if out is None else out
+    _q8_here(cache, ("lengths", lengths), ("weights", weights), ("weights_out", weights_out))
+    _q8_here(dest)
+    n_seq, nk = cache.n_seq, cache.nk
+    if dest.n_seq != n_seq or dest.nk != nk:
+        raise ValueError(f"out must hold {n_seq} sequences of {nk} heads, got {dest.n_seq} of {dest.nk}")
+    if keep_blocks < 1:
+        raise ValueError("keep_blocks must be positive")
+    if sink < 0 or recent < 0 or sink + recent > KV_Q8_BLOCK * keep_blocks:
+        raise ValueError(f"sink + recent must be 0 to {KV_Q8_BLOCK * keep_blocks}, got {sink} + {recent}")
+    if dest.s_cap < min(cache.s_cap, KV_Q8_BLOCK * (keep_blocks + 1)):
+        raise ValueError(f"out holds {dest.s_cap} tokens, {KV_Q8_BLOCK * (keep_blocks + 1)} may stay")
+    if weights_out is None:
+        weights_out = weights
+    _q8_ints(lengths, "lengths", n_seq)
+    for t, name, cap in ((weights, "weights", cache.s_cap), (weights_out, "weights_out", dest.s_cap)):
+        _check(t, name, torch.float32, align=4)
+        if tuple(t.shape) != (n_seq, nk, cap):
+            raise ValueError(f"{name} must be fp32 {(n_seq, nk, cap)}, got {tuple(t.shape)}")
+    kept = torch.empty(n_seq, nk, KV_Q8_BLOCK * keep_blocks, dtype=torch.int32, device=cache.k.device)
+    new = torch.empty_like(lengths)
+    call("t2h_kv_cache_q8_evict", cache._ptrs(), cache.s_cap, ptr(lengths), ptr(weights), keep_blocks, sink, recent, n_seq,
+         nk, 128, dest._ptrs(), dest.s_cap, ptr(weights_out), ptr(kept), ptr(new), stream_handle())
+    return kept, new
