@@ -77,14 +77,18 @@ def norm_rope(x, w, pos, theta):
 
 
 def attention(q, k, v, last, scale=D ** -0.5):
-    """q fp64 [t, nh, D], keys 0 .. last[t] of k, v [nk, s, D] -> out, sum of p |v|, p, and the largest sum of |q k|."""
+    """q fp64 [t, nh, D], keys 0 .. last[t] of k, v [nk, s, D] -> out, sum of p |v|, p, and the largest sum of |q k|.
+    The sum of p |v| has with it what fp16's least step leaves of a small p: p is held times 2^12 and the ratio of its value
+    block's scale to the largest, so the step 2^-24 is rounded to within 2^-25, that is 2^-37 of the largest |v| for each
+    key; check_out multiplies by 2^-10, hence 2^-27 here."""
     g = q.shape[1] // k.shape[0]
     k, v = k.repeat_interleave(g, 0), v.repeat_interleave(g, 0)
     score = torch.einsum("thd,hsd->hts", q, k) * scale
     mass = torch.einsum("thd,hsd->hts", q.abs(), k.abs()).amax() * scale
     seen = torch.arange(k.shape[1], device=q.device) <= last[:, None]
     p = torch.softmax(score.masked_fill(~seen, -math.inf), -1)
-    return torch.einsum("hts,hsd->thd", p, v), torch.einsum("hts,hsd->thd", p, v.abs()), p, float(mass)
+    least = 2.0 ** -27 * k.shape[1] * v.abs().amax()
+    return torch.einsum("hts,hsd->thd", p, v), torch.einsum("hts,hsd->thd", p, v.abs()) + least, p, float(mass)
 
 
 def within(got, ref, tol):

@@ -11,6 +11,559 @@
 
 namespace t2h {
 
+// ------------------------------------------------------------------------------------------- one token a sequence --
+//
+// Bound by memory: every cached byte is read once, for all q heads of its KV head.  The work is cut into units of up to
+// `chunk` consecutive cache blocks of one (sequence, KV head), equal for all sequences of a ragged batch and worked out
+// from the lengths on the device, so that a captured launch follows them; thread block (unit, head) walks one.  A wave
+// takes whole blocks of 64 tokens (its thread block's b0 + wave, + 4, ...) with no barrier in its loop:
+//   * scores S^T = K . Q^T and output O^T = V^T . P^T on the matrix cores (16 x 16 x 32, fp16 in, fp32 out), the q heads
+//     of the KV head as columns.  A lane's 16-byte loads are the operands: 16 dims of a key row, 16 tokens of a value
+//     dim.  The rows of a key tile are taken in the order that leaves a lane with the 16 tokens whose values it loads, so
+//     the softmax's weights go from one product into the other in registers, and a softmax over tokens needs two
+//     exchanges between lanes a block;
+//   * codes become fp16 exactly (bytes beside 0x64 are 1024 + code + 128), scales multiply scores and weights in fp32;
+//   * q is split into two fp16 terms (22 bits), so that scores are as good as fp32's; weights are rounded once, to 11 bits,
+//     relative to the wave's largest value scale times 2^12 (they stay normal over scales 2^26 apart);
+//   * the unfinished block's bf16 rows go through the bf16 products, with q in three and weights in two bf16 terms.
+// The wave that holds the new token writes it, and first rounds its block if that is now whole.
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int DQ_WAVES = 4;
+constexpr int DQ_ROW = Q8_D + 4;          // fp32 row in LDS, padded
+constexpr uint32_t DQ_TARGET = 2048;      // thread blocks that a call is cut into, at most (+ one a sequence and head)
+constexpr float DQ_P_SCALE = 4096.0f;
+
+struct DecodeQ8Args {
+    KvQ8 c;
+    const float* q;
+    const float* k_new;
+    const float* v_new;
+    size_t q_row, k_row, v_row;
+    const float* q_norm_w;
+    const float* k_norm_w;
+    const int32_t* lengths;
+    const int32_t* offsets;
+    const float* w_in;
+    float* w_out;
+    uint16_t* out;
+    float* part_ml;  // [units][nk][group][2]: log2 maximum, sum
+    float* part_o;   // [units][nk][group][128]
+    float* scores;   // [n_seq][nh][s_cap] log2 scores, or null
+    uint32_t n_seq, nh, group, target, units;
+    float eps, scale_log2;
+    double log2_theta;
+    int rope;
+};
+
+struct DecodeUnit {
+    uint32_t seq, first, count;  // the sequence, its first unit and how many it has
+    int chunk, blocks, len;      // blocks a unit, the sequence's blocks and its length before the call
+};
+
+__device__ __forceinline__ int dq_blocks(const DecodeQ8Args& a, uint32_t seq) {
+    const int len = a.lengths[seq];
+    return len < 0 ? 0 : len >= (int)(a.c.nb * Q8_BLOCK) ? (int)a.c.nb : len / Q8_BLOCK + 1;
+}
+
+__device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const uint32_t o = (uint32_t)__shfl_up((int)v, off, T2H_WAVE);
+        if (lane >= off) v += o;
+    }
+    return v;
+}
+
+// Blocks a unit: as many units as `target` thread blocks hold, in whole rounds of a thread block's waves.
+__device__ __forceinline__ int dq_chunk(const DecodeQ8Args& a, uint32_t total) {
+    const uint32_t c = (uint32_t)(((uint64_t)total * a.c.nk + a.target - 1) / a.target);
+    return c <= 2 ? (c ? (int)c : 1) : (int)((c + DQ_WAVES - 1) / DQ_WAVES * DQ_WAVES);
+}
+
+// The sequence that unit `unit` belongs to (by_seq false), or sequence `unit` itself; false where there is none.
+__device__ bool dq_find(const DecodeQ8Args& a, uint32_t unit, bool by_seq, DecodeUnit& u) {
+    const uint32_t lane = threadIdx.x & 63;
+    if (a.n_seq == 1) {
+        u.blocks = dq_blocks(a, 0);
+        u.chunk = dq_chunk(a, (uint32_t)u.blocks);
+        u.seq = u.first = 0;
+        u.count = (uint32_t)((u.blocks + u.chunk - 1) / u.chunk);
+        u.len = a.lengths[0];
+        return by_seq || unit < u.count;
+    }
+    uint32_t total = 0;
+    for (uint32_t i = lane; i < a.n_seq; i += 64) total += (uint32_t)dq_blocks(a, i);
+    total = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan_u32(total), 63);
+    u.chunk = dq_chunk(a, total);
+    uint32_t before = 0;
+    for (uint32_t base = 0; base < a.n_seq; base += 64) {
+        const uint32_t i = base + lane;
+        const uint32_t mine = i < a.n_seq ? ((uint32_t)dq_blocks(a, i) + u.chunk - 1) / u.chunk : 0u;
+        const uint32_t upto = before + wave_scan_u32(mine);
+        const uint64_t hit = by_seq ? __ballot(i == unit) : __ballot(unit >= upto - mine && unit < upto);
+        if (hit) {
+            const int at = __builtin_ctzll(hit);
+            u.seq = base + at;
+            u.count = (uint32_t)__builtin_amdgcn_readlane((int)mine, at);
+            u.first = (uint32_t)__builtin_amdgcn_readlane((int)(upto - mine), at);
+            u.blocks = dq_blocks(a, u.seq);
+            u.len = a.lengths[u.seq];
+            return true;
+        }
+        before = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+    }
+    return false;
+}
+
+// Four codes as fp16: 0x6400 + byte is 1024 + byte.
+__device__ __forceinline__ void codes_f16(uint32_t w, f16x2_t& lo, f16x2_t& hi) {
+    const uint32_t x = w ^ 0x80808080u;
+    const f16x2_t off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+    lo = __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(0x64646464u, x, 0x04010400u)) + off;
+    hi = __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(0x64646464u, x, 0x04030402u)) + off;
+}
+
+__device__ __forceinline__ f16x8 codes_f16x8(uint32_t w0, uint32_t w1) {
+    f16x2_t r[4];
+    codes_f16(w0, r[0], r[1]);
+    codes_f16(w1, r[2], r[3]);
+    return __builtin_bit_cast(f16x8, r);
+}
+
+__device__ __forceinline__ bf16x8 as_bf16x8(uint4 v) { return __builtin_bit_cast(bf16x8, v); }
+
+// A block that its last token finishes, rounded by one wave from the tail's rows and that token: two passes over 32 KB,
+// once in 64 tokens.  The codes are in memory for the wave itself when this returns.
+__device__ __forceinline__ void dq_round(const KvQ8& c, uint32_t seq, uint32_t h, uint32_t b, const uint16_t* key,
+                                         const uint16_t* value) {
+    const int lane = threadIdx.x & 63;
+    const size_t tail = c.tail_at(seq, h), at = c.block_at(seq, b, h);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll 1
+    for (int half = 0; half < 2; ++half) {
+        const uint16_t* rows = (half == 0 ? c.kt : c.vt) + tail;
+        // 16 values of a row: the last token's are the last row of the keys, the last value of each row of the values
+        auto load = [&](int n, uint32_t (&w)[8]) {
+            const int i = (n * 64 + lane) * 16;
+            uint4 lo = load_u4(rows + i), hi = load_u4(rows + i + 8);
+            if (half == 0 && i / Q8_D == Q8_BLOCK - 1) {
+                lo = *reinterpret_cast<const uint4*>(key + i % Q8_D);
+                hi = *reinterpret_cast<const uint4*>(key + i % Q8_D + 8);
+            }
+            if (half == 1 && i % Q8_BLOCK == Q8_BLOCK - 16) hi.w = (hi.w & 0xffffu) | (uint32_t)value[i / Q8_BLOCK] << 16;
+            w[0] = lo.x, w[1] = lo.y, w[2] = lo.z, w[3] = lo.w, w[4] = hi.x, w[5] = hi.y, w[6] = hi.z, w[7] = hi.w;
+        };
+        uint32_t top = 0;
+#pragma unroll 2
+        for (int n = 0; n < 8; ++n) {
+            uint32_t w[8];
+            load(n, w);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = max(top, max(w[i] << 16 & 0x7fffffffu, w[i] & 0x7fff0000u));
+        }
+        top = wave_max_u32(top);
+        float s, inv;
+        q8_scale(top, s, inv);
+#pragma unroll 2
+        for (int n = 0; n < 8; ++n) {
+            uint32_t w[8], packed[4];
+            load(n, w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                packed[i] = q8_pack4(__uint_as_float(w[2 * i] << 16), __uint_as_float(w[2 * i] & 0xffff0000u),
+                                     __uint_as_float(w[2 * i + 1] << 16), __uint_as_float(w[2 * i + 1] & 0xffff0000u), inv);
+            *reinterpret_cast<uint4*>((half == 0 ? c.k : c.v) + at + (n * 64 + lane) * 16) =
+                make_uint4(packed[0], packed[1], packed[2], packed[3]);
+        }
+        if (lane == 0) (half == 0 ? c.ks : c.vs)[c.scale_at(seq, b, h)] = s;
+    }
+    __threadfence_block();  // other lanes of the wave read them
+}
+
+template <bool WEIGHTS>
+__global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_decode_q8_kernel(const DecodeQ8Args a) {
+    __shared__ __align__(16) float qs[16][DQ_ROW];            // q of each head, its largest value in [1, 2)
+    __shared__ float qf[16];                                  // what that took off, with the softmax's scale and log2 e
+    __shared__ __align__(16) uint16_t fresh[2][Q8_D];         // the new token's key and value
+    __shared__ float wml[DQ_WAVES][16][2];
+    __shared__ __align__(16) float wo[DQ_WAVES][16][DQ_ROW];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t h = blockIdx.x % a.c.nk;
+    const uint32_t unit = blockIdx.x / a.c.nk;
+    DecodeUnit u;
+    if (!dq_find(a, unit, false, u)) return;  // (every wave of a thread block finds the same)
+    const int group = (int)a.group;
+    const int b0 = (int)(unit - u.first) * u.chunk;
+    const int b1 = b0 + u.chunk < u.blocks ? b0 + u.chunk : u.blocks;
+    const int c = lane & 15, g4 = lane >> 4;
+    const bool has_new = u.len < (int)(a.c.nb * Q8_BLOCK);
+    const int new_b = has_new ? u.len / Q8_BLOCK : -1;  // the block of the new token, in bf16 unless the token finishes it
+    const int r = u.len % Q8_BLOCK;
+    const int tail_b = r == Q8_BLOCK - 1 ? -1 : new_b;
+
+    // 1. the first block's codes
+    const int krow = ((c >> 2) * 16 + (c & 3)) * Q8_D + g4 * 16;  // + t * 4 rows + j * 64
+    const int vrow = c * Q8_BLOCK + g4 * 16;                      // + dt * 16 rows
+    uint4 kr[4][2], vr[8];
+    float ks = 0.0f, vs = 0.0f;
+    auto load_k = [&](int b) {
+        const int8_t* p = a.c.k + a.c.block_at(u.seq, (uint32_t)b, h) + krow;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) kr[t][j] = load_nt_u4(p + t * 4 * Q8_D + j * 64);
+        ks = a.c.ks[a.c.scale_at(u.seq, (uint32_t)b, h)];
+    };
+    auto load_v = [&](int b) {
+        const int8_t* p = a.c.v + a.c.block_at(u.seq, (uint32_t)b, h) + vrow;
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) vr[dt] = load_nt_u4(p + dt * 16 * Q8_BLOCK);
+        vs = a.c.vs[a.c.scale_at(u.seq, (uint32_t)b, h)];
+    };
+    int b = b0 + wave;
+    const bool writes = new_b >= b0 && new_b < b1 && (new_b - b0) % DQ_WAVES == wave;
+    const bool has_tail = writes && tail_b >= 0;
+    if (b < b1 && b != new_b) {
+        load_k(b);
+        load_v(b);
+    }
+
+    // 2. q and the new token
+    const int pos = u.len + (a.offsets ? a.offsets[u.seq] : 0);
+    float cs = 1.0f, sn = 0.0f;
+    if (a.rope && (wave < group || writes)) rope_at(rope_turns(lane, a.log2_theta), pos, cs, sn);
+    const bool has_w = a.q_norm_w != nullptr;
+    for (int g = wave; g < group; g += DQ_WAVES) {
+        const float* x = a.q + u.seq * a.q_row + (size_t)(h * group + g) * Q8_D;
+        const float w0 = has_w ? a.q_norm_w[lane] : 1.0f, w1 = has_w ? a.q_norm_w[lane + 64] : 1.0f;
+        float r0, r1;
+        norm_rope_pair(x[lane], x[lane + 64], has_w, w0, w1, a.eps, cs, sn, a.rope != 0, r0, r1);
+        uint32_t e = wave_max_u32(max(abs_bits(r0), abs_bits(r1))) >> 23;
+        e = e < 1 ? 1 : (e > 253 ? 253 : e);
+        const float down = __uint_as_float((254u - e) << 23);
+        qs[g][lane] = r0 * down;
+        qs[g][lane + 64] = r1 * down;
+        if (lane == 0) qf[g] = __uint_as_float(e << 23) * a.scale_log2;
+    }
+    if (writes) {
+        const float* kx = a.k_new + u.seq * a.k_row + (size_t)h * Q8_D;
+        const float* vx = a.v_new + u.seq * a.v_row + (size_t)h * Q8_D;
+        const float w0 = has_w ? a.k_norm_w[lane] : 1.0f, w1 = has_w ? a.k_norm_w[lane + 64] : 1.0f;
+        float r0, r1;
+        norm_rope_pair(kx[lane], kx[lane + 64], has_w, w0, w1, a.eps, cs, sn, a.rope != 0, r0, r1);
+        const uint16_t kb[2] = {(uint16_t)f32_to_bf16_bits(r0), (uint16_t)f32_to_bf16_bits(r1)};
+        const uint16_t vb[2] = {(uint16_t)f32_to_bf16_bits(vx[lane]), (uint16_t)f32_to_bf16_bits(vx[lane + 64])};
+        const size_t tail = a.c.tail_at(u.seq, h);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            fresh[0][lane + 64 * i] = kb[i];
+            fresh[1][lane + 64 * i] = vb[i];
+            a.c.kt[tail + r * Q8_D + lane + 64 * i] = kb[i];
+            a.c.vt[tail + (lane + 64 * i) * Q8_BLOCK + r] = vb[i];
+        }
+        if (tail_b < 0) {
+            dq_round(a.c, u.seq, h, (uint32_t)new_b, fresh[0], fresh[1]);
+            if (b == new_b) {
+                load_k(b);
+                load_v(b);
+            }
+        }
+    }
+    // the largest value scale of the wave's blocks
+    float smax = 0.0f;
+    for (int i = b0 + wave + DQ_WAVES * lane; i < b1; i += DQ_WAVES * 64)
+        if (i != tail_b) smax = fmaxf(smax, a.c.vs[a.c.scale_at(u.seq, (uint32_t)i, h)]);
+    __syncthreads();
+    f16x8 qh[2][2], ql[2][2];  // q's two terms at dims 64 j + 16 g4 + 8 i
+    const float qfac = c < group ? qf[c] : 0.0f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float x = c < group ? qs[c][64 * j + 16 * g4 + 8 * i + e] : 0.0f;
+                qh[j][i][e] = (_Float16)x;
+                ql[j][i][e] = (_Float16)(x - (float)qh[j][i][e]);
+            }
+    smax = wave_max(smax);
+
+    // 3. the wave's blocks
+    float m = -INFINITY, l = 0.0f;
+    f32x4 o[8];
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) o[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    // scores of a block (x: dot products, to be multiplied by f) -> weights; a lane's tokens are 16 g4 + 4 t + i
+    auto soften = [&](f32x4 (&x)[4], float f, int b, int live) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[t][i] *= f;
+                if (live < Q8_BLOCK && 16 * g4 + 4 * t + i >= live) x[t][i] = -INFINITY;
+                top = fmaxf(top, x[t][i]);
+            }
+        if (WEIGHTS && c < group) {
+            float* to = a.scores + ((size_t)u.seq * a.nh + h * group + c) * a.c.nb * Q8_BLOCK + b * Q8_BLOCK + 16 * g4;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) *reinterpret_cast<f32x4*>(to + 4 * t) = x[t];
+        }
+        top = fmaxf(m, xor_max<32>(xor_max<16>(top)));
+        const float base = top == -INFINITY ? 0.0f : top;
+        const float keep = __builtin_amdgcn_exp2f(m - base);
+        float sum = 0.0f;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[t][i] = __builtin_amdgcn_exp2f(x[t][i] - base);
+                sum += x[t][i];
+            }
+        l = fmaf(l, keep, sum);
+        m = top;
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) o[dt] *= keep;
+    };
+
+    for (; b < b1 && b != tail_b; b += DQ_WAVES) {
+        f32x4 x[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) x[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const f16x8 k0 = codes_f16x8(kr[t][j].x, kr[t][j].y), k1 = codes_f16x8(kr[t][j].z, kr[t][j].w);
+                x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qh[j][0], x[t], 0, 0, 0);
+                x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, ql[j][0], x[t], 0, 0, 0);
+                x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qh[j][1], x[t], 0, 0, 0);
+                x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, ql[j][1], x[t], 0, 0, 0);
+            }
+        const float fk = ks * qfac;
+        const int next = b + DQ_WAVES;
+        const bool more = next < b1 && next != tail_b;
+        if (more) load_k(next);
+        soften(x, fk, b, Q8_BLOCK);
+        const float fv = vs * (DQ_P_SCALE / (smax > 0.0f ? smax : 1.0f));
+        f16x8 p[2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) p[s][e] = (_Float16)(x[2 * s + e / 4][e % 4] * fv);
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) {
+            o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16x8(vr[dt].x, vr[dt].y), p[0], o[dt], 0, 0, 0);
+            o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16x8(vr[dt].z, vr[dt].w), p[1], o[dt], 0, 0, 0);
+        }
+        if (more) load_v(next);
+    }
+
+    if (has_tail) {  // the unfinished block, the wave's last
+        f32x4 x[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) x[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        const size_t tail = a.c.tail_at(u.seq, h);
+        // a scheduling fence a step: the compiler would have all rows in flight at once, which the loop's other path
+        // has no registers for
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            const int j = n >> 1, i = n & 1, d = 64 * j + 16 * g4 + 8 * i;
+            __builtin_amdgcn_sched_barrier(0);
+            bf16x8 q3[3];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                float y = (float)qh[j][i][e] + (float)ql[j][i][e];
+#pragma unroll
+                for (int z = 0; z < 3; ++z) {
+                    q3[z][e] = (__bf16)y;
+                    y -= (float)q3[z][e];
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const int token = (c >> 2) * 16 + t * 4 + (c & 3);
+                uint4 kk = load_u4(a.c.kt + tail + token * Q8_D + d);
+                if (token == r) kk = *reinterpret_cast<const uint4*>(&fresh[0][d]);
+#pragma unroll
+                for (int z = 0; z < 3; ++z)
+                    x[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(kk), q3[z], x[t], 0, 0, 0);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        soften(x, qfac, tail_b, r + 1);
+        const float f_unit = DQ_P_SCALE / (smax > 0.0f ? smax : 1.0f);
+        bf16x8 ph[2], pl[2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float p = x[2 * s + e / 4][e % 4] * f_unit;
+                ph[s][e] = (__bf16)p;
+                pl[s][e] = (__bf16)(p - (float)ph[s][e]);
+            }
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) {
+            __builtin_amdgcn_sched_barrier(0);
+            const int d = 16 * dt + c;
+            const uint16_t* vp = a.c.vt + tail + d * Q8_BLOCK + 16 * g4;
+            const uint32_t vnew = fresh[1][d];
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                uint4 vv = load_u4(vp + 8 * s);
+                uint32_t* w = reinterpret_cast<uint32_t*>(&vv);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {  // tokens 16 g4 + 8 s + 2 e and the next: the new one, and none behind it
+                    const int first = 16 * g4 + 8 * s + 2 * e;
+                    if (first == r) w[e] = vnew;
+                    if (first + 1 == r) w[e] = (w[e] & 0xffffu) | vnew << 16;
+                    if (first > r) w[e] = 0u;
+                }
+                o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(vv), ph[s], o[dt], 0, 0, 0);
+                o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(vv), pl[s], o[dt], 0, 0, 0);
+            }
+        }
+    }
+
+    // 4. the waves' states joined; one unit: the output itself, more: the unit's part of it
+    const float unscale = (smax > 0.0f ? smax : 1.0f) * (1.0f / DQ_P_SCALE);
+    l = xor_sum<32>(xor_sum<16>(l));
+    if (c < group) {
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) *reinterpret_cast<f32x4*>(&wo[wave][c][16 * dt + 4 * g4]) = o[dt] * unscale;
+        if (g4 == 0) {
+            wml[wave][c][0] = m;
+            wml[wave][c][1] = l;
+        }
+    }
+    __syncthreads();
+    const int waves = b1 - b0 < DQ_WAVES ? b1 - b0 : DQ_WAVES;
+    for (int i = tid; i < group * (Q8_D / 4); i += DQ_WAVES * 64) {
+        const int g = i / (Q8_D / 4), d = i % (Q8_D / 4) * 4;
+        float M = -INFINITY, L = 0.0f;
+        for (int w = 0; w < waves; ++w) M = fmaxf(M, wml[w][g][0]);
+        const float base = M == -INFINITY ? 0.0f : M;
+        f32x4 sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int w = 0; w < waves; ++w) {
+            const float f = __builtin_amdgcn_exp2f(wml[w][g][0] - base);
+            L = fmaf(f, wml[w][g][1], L);
+            sum += *reinterpret_cast<const f32x4*>(&wo[w][g][d]) * f;
+        }
+        const size_t part = ((size_t)unit * a.c.nk + h) * a.group + g;
+        if (u.count == 1) {
+            const float inv = 1.0f / L;
+            uint32_t* to = reinterpret_cast<uint32_t*>(a.out + ((size_t)u.seq * a.nh + h * group + g) * Q8_D + d);
+            to[0] = pack_bf16x2(sum[0] * inv, sum[1] * inv);
+            to[1] = pack_bf16x2(sum[2] * inv, sum[3] * inv);
+        } else {
+            *reinterpret_cast<f32x4*>(a.part_o + part * Q8_D + d) = sum;
+        }
+        if (d == 0 && (WEIGHTS || u.count > 1)) *reinterpret_cast<float2*>(a.part_ml + 2 * part) = make_float2(M, L);
+    }
+}
+
+// log2 maximum and sum of a head over the units of its sequence; every lane gets them
+__device__ __forceinline__ void dq_total(const DecodeQ8Args& a, const DecodeUnit& u, uint32_t h, uint32_t g, float& M, float& L) {
+    const float2* ml = reinterpret_cast<const float2*>(a.part_ml);
+    M = -INFINITY;
+    L = 0.0f;
+    for (uint32_t i = threadIdx.x & 63; i < u.count; i += 64) M = fmaxf(M, ml[((size_t)(u.first + i) * a.c.nk + h) * a.group + g].x);
+    M = wave_max(M);
+    const float base = M == -INFINITY ? 0.0f : M;
+    for (uint32_t i = threadIdx.x & 63; i < u.count; i += 64) {
+        const float2 x = ml[((size_t)(u.first + i) * a.c.nk + h) * a.group + g];
+        L = fmaf(__builtin_amdgcn_exp2f(x.x - base), x.y, L);
+    }
+    L = wave_sum(L);
+}
+
+constexpr int DQ_SEGMENT = 1024;  // tokens of a thread block that adds up weights
+
+// Thread blocks [0, n_seq nh): a head's units joined.  Behind them, with weights: 1024 tokens of a (sequence, KV head),
+// exp2(score - log2 sum) over its heads.
+template <bool WEIGHTS>
+__global__ __launch_bounds__(256) void attn_decode_q8_merge_kernel(const DecodeQ8Args a) {
+    __shared__ __align__(16) float part[8][Q8_D];
+    __shared__ float lse[16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    DecodeUnit u;
+    if (blockIdx.x < a.n_seq * a.nh) {
+        const uint32_t seq = blockIdx.x / a.nh, head = blockIdx.x % a.nh;
+        const uint32_t h = head / a.group, g = head % a.group;
+        dq_find(a, seq, true, u);
+        uint32_t* out = reinterpret_cast<uint32_t*>(a.out + (size_t)blockIdx.x * Q8_D);
+        if (u.count == 0 && tid < 64) out[tid] = 0u;  // takes no part
+        if (u.count <= 1) return;
+        float M, L;
+        dq_total(a, u, h, g, M, L);
+        const float base = M == -INFINITY ? 0.0f : M;
+        const int slot = tid >> 5, d = (tid & 31) * 4;
+        f32x4 sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+        for (uint32_t i = (uint32_t)slot; i < u.count; i += 8) {
+            const size_t at = ((size_t)(u.first + i) * a.c.nk + h) * a.group + g;
+            sum += *reinterpret_cast<const f32x4*>(a.part_o + at * Q8_D + d) * __builtin_amdgcn_exp2f(a.part_ml[2 * at] - base);
+        }
+        *reinterpret_cast<f32x4*>(&part[slot][d]) = sum;
+        __syncthreads();
+        if (tid < 64) {
+            float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                s0 += part[i][2 * tid];
+                s1 += part[i][2 * tid + 1];
+            }
+            const float inv = 1.0f / L;
+            out[tid] = pack_bf16x2(s0 * inv, s1 * inv);
+        }
+        return;
+    }
+    if constexpr (WEIGHTS) {
+        const uint32_t i = blockIdx.x - a.n_seq * a.nh;
+        const uint32_t h = i % a.c.nk, rest = i / a.c.nk;
+        const uint32_t segments = (a.c.nb * Q8_BLOCK + DQ_SEGMENT - 1) / DQ_SEGMENT;
+        const uint32_t seq = rest / segments;
+        const int t0 = (int)(rest % segments) * DQ_SEGMENT + 4 * tid;
+        const int len = a.lengths[seq], cap = (int)(a.c.nb * Q8_BLOCK);
+        const int end = len < 0 ? 0 : (len < cap ? len + 1 : cap);
+        if ((int)(rest % segments) * DQ_SEGMENT >= end) return;
+        dq_find(a, seq, true, u);
+        for (uint32_t g = wave; g < a.group; g += 4) {
+            float M, L;
+            dq_total(a, u, h, g, M, L);
+            if (lane == 0) lse[g] = M + log2f(L);
+        }
+        __syncthreads();
+        if (t0 >= end) return;
+        f32x4 sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (uint32_t g = 0; g < a.group; ++g) {
+            const f32x4 s = *reinterpret_cast<const f32x4*>(a.scores + ((size_t)seq * a.nh + h * a.group + g) * cap + t0);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sum[j] += __builtin_amdgcn_exp2f(s[j] - lse[g]);
+        }
+        const size_t at = ((size_t)seq * a.c.nk + h) * cap + t0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (t0 + j < end) a.w_out[at + j] = (t0 + j < len ? a.w_in[at + j] : 0.0f) + sum[j];
+    }
+}
+
+static uint32_t dq_units(uint32_t n_seq, uint32_t nk, uint32_t nb) {
+    const uint64_t a = (uint64_t)DQ_TARGET / nk + n_seq, b = (uint64_t)n_seq * nb;
+    return (uint32_t)(a < b ? a : b);
+}
+
+// ------------------------------------------------------------------------------------------------------ chunks --
+
 struct AttnQ8Args {
     KvQ8 c;
     const void* q;  // bf16 or fp32 [n_seq][n][nh][128]
@@ -137,7 +690,8 @@ extern "C" size_t t2h_attn_decode_q8_workspace_bytes(uint32_t n_seq, uint32_t nh
     if (n_seq == 0 || nk == 0 || nh == 0 || nh % nk != 0 || nh / nk > Q8_MAX_GROUP || d != (uint32_t)Q8_D || s_cap == 0 ||
         s_cap % Q8_BLOCK != 0)
         return 0;
-    return (size_t)n_seq * nh * (4 * Q8_D + 4) + 256;
+    const size_t parts = (size_t)dq_units(n_seq, nk, s_cap / Q8_BLOCK) * nh;
+    return parts * (Q8_D + 2) * 4 + 16 + (weights ? (size_t)n_seq * nh * s_cap * 4 : 0);
 }
 
 extern "C" int t2h_attn_decode_q8(const float* q, uint64_t q_row, const float* k_new, uint64_t k_row, const float* v_new,
@@ -145,29 +699,56 @@ extern "C" int t2h_attn_decode_q8(const float* q, uint64_t q_row, const float* k
                                   const int32_t* lengths, const int32_t* rope_offsets, void* const* cache, uint32_t s_cap,
                                   const float* weights, float* weights_out, void* out, uint32_t n_seq, uint32_t nh,
                                   uint32_t nk, uint32_t d, void* workspace, size_t workspace_bytes, void* stream) {
-    AttnQ8Args a;
-    if (!lengths || !out || !workspace) return T2H_ERR_NULL;
-    if ((weights == nullptr) != (weights_out == nullptr)) return T2H_ERR_NULL;
+    DecodeQ8Args a;
+    if (!q || !k_new || !v_new || !lengths || !out || !workspace) return T2H_ERR_NULL;
+    if ((weights == nullptr) != (weights_out == nullptr) || (q_norm_w == nullptr) != (k_norm_w == nullptr)) return T2H_ERR_NULL;
     if (const int e = q8_cache(cache, s_cap, n_seq, nh, nk, d, a.c)) return e;
+    if (q_row < (uint64_t)nh * d || k_row < (uint64_t)nk * d || v_row < (uint64_t)nk * d) return T2H_ERR_SHAPE;
     if (reinterpret_cast<uintptr_t>(out) & 3) return T2H_ERR_ALIGN;
     if (reinterpret_cast<uintptr_t>(workspace) & 15) return T2H_ERR_ALIGN;
     if (workspace_bytes < t2h_attn_decode_q8_workspace_bytes(n_seq, nh, nk, d, s_cap, weights != nullptr)) return T2H_ERR_WORKSPACE;
-    if (!q || !k_new || !v_new) return T2H_ERR_NULL;
-    const int e = q8_write_launch(q, q_row, k_new, k_row, v_new, v_row, q_norm_w, k_norm_w, eps, theta, lengths, nullptr,
-                                            rope_offsets, 1, n_seq, nh, nk, d, workspace, true, cache, s_cap, stream);
-    if (e) return e;
-    a.q = workspace;
-    a.out = reinterpret_cast<uint16_t*>(out);
-    a.lse = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(workspace) + (size_t)n_seq * nh * 4 * Q8_D);
+    a.q = q;
+    a.k_new = k_new;
+    a.v_new = v_new;
+    a.q_row = (size_t)q_row;
+    a.k_row = (size_t)k_row;
+    a.v_row = (size_t)v_row;
+    a.q_norm_w = q_norm_w;
+    a.k_norm_w = k_norm_w;
     a.lengths = lengths;
-    a.counts = nullptr;
+    a.offsets = rope_offsets;
     a.w_in = weights;
     a.w_out = weights_out;
-    a.n = 1;
+    a.out = reinterpret_cast<uint16_t*>(out);
     a.n_seq = n_seq;
     a.nh = nh;
-    a.scale = 1.0f / sqrtf((float)Q8_D);
-    return attn_q8_launch<true>(a, stream);
+    a.group = nh / nk;
+    a.target = DQ_TARGET;
+    a.units = dq_units(n_seq, nk, a.c.nb);
+    const size_t parts = (size_t)a.units * nh;
+    a.part_o = reinterpret_cast<float*>(workspace);
+    a.part_ml = a.part_o + parts * Q8_D;
+    a.scores = weights ? a.part_o + (parts * (Q8_D + 2) + 3) / 4 * 4 : nullptr;
+    a.eps = eps;
+    a.scale_log2 = 1.4426950408889634f / sqrtf((float)Q8_D);
+    a.rope = theta > 0.0f;
+    a.log2_theta = a.rope ? log2((double)theta) : 0.0;
+    const uint64_t grid = (uint64_t)a.units * nk;
+    const uint64_t segments = ((uint64_t)s_cap + DQ_SEGMENT - 1) / DQ_SEGMENT;
+    const uint64_t merge = (uint64_t)n_seq * nh + (weights ? (uint64_t)n_seq * nk * segments : 0);
+    if (grid > 0x7fffffffu || merge > 0x7fffffffu) return T2H_ERR_SHAPE;
+    const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    if (weights) {
+        hipLaunchKernelGGL(attn_decode_q8_kernel<true>, dim3((uint32_t)grid), dim3(DQ_WAVES * 64), 0, st, a);
+        T2H_LAUNCH_CHECK();
+        hipLaunchKernelGGL(attn_decode_q8_merge_kernel<true>, dim3((uint32_t)merge), dim3(256), 0, st, a);
+    } else {
+        hipLaunchKernelGGL(attn_decode_q8_kernel<false>, dim3((uint32_t)grid), dim3(DQ_WAVES * 64), 0, st, a);
+        T2H_LAUNCH_CHECK();
+        hipLaunchKernelGGL(attn_decode_q8_merge_kernel<false>, dim3((uint32_t)merge), dim3(256), 0, st, a);
+    }
+    T2H_LAUNCH_CHECK();
+    return T2H_OK;
 }
 
 extern "C" size_t t2h_flash_attn_prefill_q8_workspace_bytes(uint32_t n, uint32_t n_seq, uint32_t nh, uint32_t nk,
