@@ -1,8 +1,6 @@
 // Attention over the 8-bit KV cache (layout: kv_q8.h): out = softmax(q . k / sqrt(d)) . v for one token of each sequence
-// or a chunk of tokens, and the attention weight that each cached token got.
-//
-// One wave a query row: a lane is a token of the block for the scores and two dimensions for the output; one pass over
-// the keys with the running maximum and sum of the softmax, in fp32.
+// or a chunk of tokens, and the attention weight that each cached token got.  One pass over the keys with the running
+// maximum and sum of the softmax, both in fp32, scores in log2 units.
 #include <math.h>
 
 #include "kv_q8.h"
@@ -563,122 +561,430 @@ static uint32_t dq_units(uint32_t n_seq, uint32_t nk, uint32_t nb) {
 }
 
 // ------------------------------------------------------------------------------------------------------ chunks --
+//
+// Bound by the matrix cores and, as much, by the softmax's and the conversion's vector instructions.  The queries of a KV
+// head's q heads are rows of one matrix (row = t * group + g), so a key tile serves them all; a thread block takes 128 rows,
+// a wave 32, and walks the cache a block of 64 tokens at a time:
+//   * a block's codes go to registers one step ahead, become bf16 keys and fp16 values (both exact) and go to the other of
+//     two LDS buffers: one barrier a step;
+//   * S^T = K . Q^T and O^T = V^T . P^T (32 x 32 x 16), so that a lane has 32 of a row's 64 scores in registers: one
+//     exchange a step for the row's maximum, none between the products (the key rows are taken in the order that makes a
+//     lane's scores the tokens of its operand of the second one);
+//   * scales go into the exponent: p of a block is exp2(s * ks + log2(vs / largest vs so far) - max); the accumulators follow a
+//     maximum only when it has grown by more than 2^3.
+// Where there are few rows the keys are split over thread blocks, and a second kernel joins the parts.
 
-struct AttnQ8Args {
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int CQ_WAVES = 4;
+constexpr int CQ_ROWS = 32 * CQ_WAVES;  // rows a thread block
+constexpr float CQ_SLACK = 3.0f;        // log2 that a row's weights may pass 1 by: 2^12 * 2^3 is in fp16's range
+
+struct ChunkQ8Args {
     KvQ8 c;
-    const void* q;  // bf16 or fp32 [n_seq][n][nh][128]
+    const uint16_t* q;  // bf16 [n_seq][n][nh][128]
     uint16_t* out;
-    float* lse;  // [n_seq][n][nh] natural log of the softmax's denominator, or null
+    float* lse;         // log2 of the softmax's denominator [n_seq][nk][n * group], or null
+    float* part_ml;     // [splits][n_seq][nk][n * group][2]
+    float* part_o;      // the same rows of 128
     const int32_t* lengths;
     const int32_t* counts;
     const float* w_in;
     float* w_out;
-    uint32_t n, n_seq, nh;
-    float scale;
+    uint32_t n, n_seq, nh, group, tiles, splits;
+    float scale_log2;
 };
 
-// token p's key . q, and its value's dimension
-__device__ __forceinline__ float q8_key_dot(const AttnQ8Args& a, uint32_t seq, uint32_t h, int p, bool in_tail, const float* q) {
-    float s = 0.0f;
-    if (in_tail) {
-        const uint16_t* k = a.c.kt + a.c.tail_at(seq, h) + (p % Q8_BLOCK) * Q8_D;
-        for (int i = 0; i < Q8_D; ++i) s = fmaf(bf16_bits_to_f32(k[i]), q[i], s);
-        return s;
-    }
-    const uint32_t* k = reinterpret_cast<const uint32_t*>(a.c.k + a.c.block_at(seq, p / Q8_BLOCK, h) + (p % Q8_BLOCK) * Q8_D);
-    for (int i = 0; i < Q8_D; ++i) s = fmaf(q8_value(k[i / 4], i % 4), q[i], s);
-    return s * a.c.ks[a.c.scale_at(seq, p / Q8_BLOCK, h)];
+__device__ __forceinline__ f32x16 mfma_bf16(bf16x8 a, bf16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma_f16(f16x8 a, f16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
-__device__ __forceinline__ float q8_v(const AttnQ8Args& a, uint32_t seq, uint32_t h, int p, bool in_tail, int d) {
-    if (in_tail) return bf16_bits_to_f32(a.c.vt[a.c.tail_at(seq, h) + d * Q8_BLOCK + p % Q8_BLOCK]);
-    return (float)a.c.v[a.c.block_at(seq, p / Q8_BLOCK, h) + d * Q8_BLOCK + p % Q8_BLOCK] * a.c.vs[a.c.scale_at(seq, p / Q8_BLOCK, h)];
+// Eight codes as bf16 (8 bits of significand hold them).
+__device__ __forceinline__ uint4 codes_bf16x8(uint32_t w0, uint32_t w1) {
+    return make_uint4(pack_bf16x2(q8_value(w0, 0), q8_value(w0, 1)), pack_bf16x2(q8_value(w0, 2), q8_value(w0, 3)),
+                      pack_bf16x2(q8_value(w1, 0), q8_value(w1, 1)), pack_bf16x2(q8_value(w1, 2), q8_value(w1, 3)));
 }
 
-__device__ __forceinline__ float q8_q(const AttnQ8Args& a, size_t i, bool f32) {
-    return f32 ? reinterpret_cast<const float*>(a.q)[i] : bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(a.q)[i]);
-}
+// LDS places of 16 bytes: keys [64][128] and values [128][64], 2 bytes each, chunks of a row permuted by the row so that
+// the lanes of an operand's read, which are rows, meet different banks.
+__device__ __forceinline__ int cq_key_at(int token, int chunk) { return token * 16 + (chunk ^ (token & 15)); }
+__device__ __forceinline__ int cq_value_at(int d, int chunk) { return d * 8 + (chunk ^ (d & 7)); }
 
-template <bool F32>
-__global__ __launch_bounds__(64) void attn_q8_kernel(const AttnQ8Args a) {
-    __shared__ float qs[Q8_D];
-    const int lane = threadIdx.x;
-    const uint32_t h = blockIdx.x % a.nh, row = blockIdx.x / a.nh;
-    const uint32_t seq = row / a.n, t = row % a.n;
-    const uint32_t kvh = h / (a.nh / a.c.nk);
+__global__ __launch_bounds__(CQ_WAVES * 64, 2) void attn_chunk_q8_kernel(const ChunkQ8Args a) {
+    __shared__ __align__(16) uint4 keys[2][Q8_BLOCK * 16];
+    __shared__ __align__(16) uint4 values[2][Q8_D * 8];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 31, half = lane >> 5;
+    uint32_t rest = blockIdx.x;
+    const uint32_t h = rest % a.c.nk;  // neighbours work on different heads: with 8 of them an XCD's L2 holds one head's keys
+    rest /= a.c.nk;
+    const uint32_t split = rest % a.splits;
+    rest /= a.splits;
+    const uint32_t seq = rest % a.n_seq;
+    const int tile = (int)(a.tiles - 1 - rest / a.n_seq);  // the longest first
     const Q8Span s = q8_span(a.lengths, a.counts, seq, a.n, a.c.nb);
-    const size_t at = (size_t)blockIdx.x * Q8_D;
-    const int count = a.counts ? a.counts[seq] : (int)a.n;
-    const int len = a.lengths[seq];
-    int last = len < 0 || (int)t >= count ? 0 : len + (int)t + 1;
-    last = last < 0 || last > s.end ? s.end : last;
-    qs[lane] = q8_q(a, at + lane, F32);
-    qs[lane + 64] = q8_q(a, at + lane + 64, F32);
+    const int len = min(a.lengths[seq], (int)(a.c.nb * Q8_BLOCK));
+    int count = a.counts ? a.counts[seq] : (int)a.n;
+    count = len < 0 || count < 0 ? 0 : (count < (int)a.n ? count : (int)a.n);
+    const int group = (int)a.group, rows = count * group;
+    const size_t head_row = ((size_t)seq * a.c.nk + h) * a.n * group;  // of row 0 in lse and the parts
+
+    // rows of this wave: row0 + lane % 32; `last` is the last token that the lane's row sees
+    const int row0 = tile * CQ_ROWS + wave * 32;
+    const int row = row0 + col;
+    const int t = row / group, g = row - t * group;
+    const int last = row < rows ? (len + t < s.end ? len + t : s.end - 1) : -1;
+    const int wave_top = row0 + 31 < rows ? row0 + 31 : rows - 1;  // its last live row, below row0 if it has none
+    const int wave_last = wave_top >= row0 ? (len + wave_top / group < s.end ? len + wave_top / group : s.end - 1) : -1;
+    const int wave_first = row0 < rows ? (len + row0 / group < s.end ? len + row0 / group : s.end - 1) : -1;
+    const int top_row = (tile + 1) * CQ_ROWS < rows ? (tile + 1) * CQ_ROWS - 1 : rows - 1;
+    const int tile_last = tile * CQ_ROWS < rows ? (len + top_row / group < s.end ? len + top_row / group : s.end - 1) : -1;
+    const int blocks = tile_last >= 0 ? tile_last / Q8_BLOCK + 1 : 0;
+    const int b0 = (int)((int64_t)blocks * split / a.splits), b1 = (int)((int64_t)blocks * (split + 1) / a.splits);
+    const int tail_b = s.end % Q8_BLOCK ? s.end / Q8_BLOCK : -1;  // held in bf16
+    const bool has_tail = tail_b >= b0 && tail_b < b1;
+    const int whole = has_tail ? b1 - 1 : b1;
+
+    // a block's codes: 16-byte pieces tid and tid + 256, of a token (8 pieces) and of a value's dim (4)
+    uint4 kc[2], vc[2];
+    float ks = 0.0f, vs = 0.0f, ks_next = 0.0f, vs_next = 0.0f;
+    auto load = [&](int b) {
+        const size_t at = a.c.block_at(seq, (uint32_t)b, h);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            kc[i] = load_u4(a.c.k + at + (tid + 256 * i) * 16);
+            vc[i] = load_u4(a.c.v + at + (tid + 256 * i) * 16);
+        }
+        ks_next = a.c.ks[a.c.scale_at(seq, (uint32_t)b, h)];
+        vs_next = a.c.vs[a.c.scale_at(seq, (uint32_t)b, h)];
+    };
+    auto store = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int n = tid + 256 * i;
+            keys[buf][cq_key_at(n >> 3, 2 * (n & 7))] = codes_bf16x8(kc[i].x, kc[i].y);
+            keys[buf][cq_key_at(n >> 3, 2 * (n & 7) + 1)] = codes_bf16x8(kc[i].z, kc[i].w);
+            values[buf][cq_value_at(n >> 2, 2 * (n & 3))] = __builtin_bit_cast(uint4, codes_f16x8(vc[i].x, vc[i].y));
+            values[buf][cq_value_at(n >> 2, 2 * (n & 3) + 1)] = __builtin_bit_cast(uint4, codes_f16x8(vc[i].z, vc[i].w));
+        }
+    };
+    if (b0 < whole) load(b0);
+    // the row's query
+    uint4 q[8];
+    const uint16_t* qp = a.q + (((size_t)seq * a.n + (row < rows ? t : 0)) * a.nh + h * group + (row < rows ? g : 0)) * Q8_D + 8 * half;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = load_u4(qp + 16 * i);
+    float m = -INFINITY, l = 0.0f;
+    float smax = 0.0f;  // the largest value scale so far: the accumulators are in units of smax / 2^12
+    f32x16 o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[i][j] = 0.0f;
+    const int key_row = (col & 19) | (col & 8) >> 1 | (col & 4) << 1;  // of operand row `col`: bits 2 and 3 change places
+
+    // one block from LDS; f: the scores' factor, shift: log2 of the weights' (both of the whole block)
+    auto scores = [&](int buf, f32x16 (&x)[2]) {
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) x[tt][j] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                x[tt] = mfma_bf16(as_bf16x8(keys[buf][cq_key_at(32 * tt + key_row, 2 * i + half)]), as_bf16x8(q[i]), x[tt]);
+        }
+    };
+    // scores -> weights, times 2^shift where they are used and summed without it; a lane's scores j of tile tt are the
+    // tokens 32 tt + 16 (j / 8) + 8 half + j % 8
+    auto soften = [&](f32x16 (&x)[2], int b, float f, float shift) {
+        const bool edge = b * Q8_BLOCK + Q8_BLOCK - 1 > wave_first;
+        const int mine = last - b * Q8_BLOCK - 8 * half;
+        if (edge) {
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    if (32 * tt + 16 * (j >> 3) + (j & 7) > mine) x[tt][j] = -INFINITY;
+        }
+        // the maximum before the factor: ks and the scale are not negative
+        float top = -INFINITY;
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) top = fmaxf(top, x[tt][j]);
+        top = xor_max<32>(top);
+        top = top == -INFINITY ? top : top * f;
+        if (__any(top > m + CQ_SLACK)) {
+            const float now = fmaxf(m, top);
+            const float keep = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - now);
+            l *= keep;
+            m = now;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) o[i][j] *= keep;
+        }
+        const float base = (m == -INFINITY ? 0.0f : m) - shift;
+        float sum = 0.0f;
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                x[tt][j] = __builtin_amdgcn_exp2f(fmaf(x[tt][j], f, -base));
+                // again: a scale that is NaN reaches the rows that see its block only
+                if (edge && 32 * tt + 16 * (j >> 3) + (j & 7) > mine) x[tt][j] = 0.0f;
+                sum += x[tt][j];
+            }
+        if (sum != 0.0f) l = fmaf(sum, __builtin_amdgcn_exp2f(-shift), l);
+    };
+
+    if (b0 < whole) {
+        store(0);
+        ks = ks_next;
+        vs = vs_next;
+    }
     __syncthreads();
-    float m = -INFINITY, l = 0.0f, o0 = 0.0f, o1 = 0.0f;
-    for (int p0 = 0; p0 < last; p0 += Q8_BLOCK) {
-        const bool in_tail = p0 == s.end / Q8_BLOCK * Q8_BLOCK;
-        const int p = p0 + lane;
-        const float x = p < last ? q8_key_dot(a, seq, kvh, p, in_tail, qs) * a.scale : -INFINITY;
-        const float top = fmaxf(m, wave_max(x));
-        const float base = top == -INFINITY ? 0.0f : top;
-        const float e = p < last ? expf(x - base) : 0.0f;
-        const float f = expf(m - base);
-        l = l * f + wave_sum(e);
-        o0 *= f;
-        o1 *= f;
-        m = top;
-        for (int i = 0; i < Q8_BLOCK && p0 + i < last; ++i) {
-            const float w = __shfl(e, i, T2H_WAVE);
-            o0 = fmaf(w, q8_v(a, seq, kvh, p0 + i, in_tail, 2 * lane), o0);
-            o1 = fmaf(w, q8_v(a, seq, kvh, p0 + i, in_tail, 2 * lane + 1), o1);
+    for (int b = b0; b < whole; ++b) {
+        const int buf = (b - b0) & 1;
+        if (b + 1 < whole) load(b + 1);
+        if (b * Q8_BLOCK <= wave_last) {
+            f32x16 x[2];
+            scores(buf, x);
+            if (vs > smax) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) o[i][j] *= smax / vs;
+                smax = vs;
+            }
+            // a block of zeros may have any scale: its scores or its values are zeros all the same
+            const float shift = vs == 0.0f ? 0.0f : __builtin_amdgcn_logf(vs * (DQ_P_SCALE / (smax > 0.0f ? smax : 1.0f)));
+            soften(x, b, (ks == 0.0f ? 1.0f : ks) * a.scale_log2, shift);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                f16x8 p;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) p[j] = (_Float16)x[i >> 1][8 * (i & 1) + j];
+#pragma unroll
+                for (int dt = 0; dt < 4; ++dt)
+                    o[dt] = mfma_f16(__builtin_bit_cast(f16x8, values[buf][cq_value_at(32 * dt + col, 2 * i + half)]), p, o[dt]);
+            }
+        }
+        if (b + 1 < whole) {
+            store(buf ^ 1);
+            ks = ks_next;
+            vs = vs_next;
+        }
+        __syncthreads();
+    }
+    if (has_tail) {
+        // bf16 rows as they are; weights in two bf16 terms
+        const size_t at = a.c.tail_at(seq, h);
+        const int live = s.end % Q8_BLOCK;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int n = tid + 256 * i;
+            keys[0][cq_key_at(n >> 4, n & 15)] = load_u4(a.c.kt + at + n * 8);
+            uint4 v = load_u4(a.c.vt + at + n * 8);
+            uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {  // nothing that lies behind the last token
+                if ((n & 7) * 8 + 2 * e >= live) w[e] = 0u;
+                else if ((n & 7) * 8 + 2 * e + 1 >= live) w[e] &= 0xffffu;
+            }
+            values[0][cq_value_at(n >> 3, n & 7)] = v;
+        }
+        __syncthreads();
+        if (tail_b * Q8_BLOCK <= wave_last) {
+            f32x16 x[2];
+            scores(0, x);
+            if (smax == 0.0f) smax = 1.0f;
+            soften(x, tail_b, a.scale_log2, __builtin_amdgcn_logf(DQ_P_SCALE / smax));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                bf16x8 ph, pl;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float p = x[i >> 1][8 * (i & 1) + j];
+                    ph[j] = (__bf16)p;
+                    pl[j] = (__bf16)(p - (float)ph[j]);
+                }
+#pragma unroll
+                for (int dt = 0; dt < 4; ++dt) {
+                    const bf16x8 v = as_bf16x8(values[0][cq_value_at(32 * dt + col, 2 * i + half)]);
+                    o[dt] = mfma_bf16(v, ph, o[dt]);
+                    o[dt] = mfma_bf16(v, pl, o[dt]);
+                }
+            }
         }
     }
-    const float inv = last > 0 ? 1.0f / l : 0.0f;
-    reinterpret_cast<uint32_t*>(a.out + at)[lane] = pack_bf16x2(o0 * inv, o1 * inv);
-    if (a.lse && lane == 0) a.lse[blockIdx.x] = m + logf(l);
+    l = xor_sum<32>(l);
+    // a lane's outputs: dims 32 dt + 8 (j / 4) + 4 half + j % 4 of its row; rows past the count are zeros
+    if (row >= (int)a.n * group) return;
+    if (row >= rows || smax == 0.0f) {
+        if (row >= rows) m = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) o[i][j] = 0.0f;
+    }
+    const float unit = smax * (1.0f / DQ_P_SCALE);
+    if (a.splits == 1) {
+        const float inv = l == 0.0f ? 0.0f : unit / l;
+        uint16_t* to = a.out + (((size_t)seq * a.n + t) * a.nh + h * group + g) * Q8_D + 4 * half;
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                *reinterpret_cast<uint2*>(to + 32 * dt + 8 * j) =
+                    make_uint2(pack_bf16x2(o[dt][4 * j] * inv, o[dt][4 * j + 1] * inv),
+                               pack_bf16x2(o[dt][4 * j + 2] * inv, o[dt][4 * j + 3] * inv));
+        if (a.lse && half == 0) a.lse[head_row + row] = m + log2f(l);
+        return;
+    }
+    const size_t part = (size_t)split * a.n_seq * a.c.nk * a.n * group + head_row + row;
+    float* to = a.part_o + part * Q8_D + 4 * half;
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<f32x4*>(to + 32 * dt + 8 * j) = f32x4{o[dt][4 * j] * unit, o[dt][4 * j + 1] * unit,
+                                                                    o[dt][4 * j + 2] * unit, o[dt][4 * j + 3] * unit};
+    if (half == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * part) = make_float2(m, l);
 }
 
-// weights_out[token] = weights_in (0 for a new token) + sum of p over the queries and the heads of the KV head
-template <bool F32>
-__global__ __launch_bounds__(64) void attn_q8_weights_kernel(const AttnQ8Args a) {
-    __shared__ float qs[Q8_D];
-    const int lane = threadIdx.x;
-    const uint32_t kvh = blockIdx.x % a.c.nk;
+// A row's parts joined: 8 rows a thread block, 32 lanes a row.
+__global__ __launch_bounds__(256) void attn_chunk_q8_merge_kernel(const ChunkQ8Args a) {
+    const uint64_t all = (uint64_t)a.n_seq * a.c.nk * a.n * a.group;
+    const uint64_t at = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (at >= all) return;
+    const int d = (threadIdx.x & 31) * 4;
+    const uint32_t row = (uint32_t)(at % ((uint64_t)a.n * a.group));
+    const uint64_t head = at / ((uint64_t)a.n * a.group);
+    const uint32_t h = (uint32_t)(head % a.c.nk), seq = (uint32_t)(head / a.c.nk);
+    const uint32_t t = row / a.group, g = row % a.group;
+    float M = -INFINITY, L = 0.0f;
+    for (uint32_t i = 0; i < a.splits; ++i) M = fmaxf(M, a.part_ml[2 * (i * all + at)]);
+    const float base = M == -INFINITY ? 0.0f : M;
+    f32x4 sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (uint32_t i = 0; i < a.splits; ++i) {
+        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (i * all + at));
+        const float f = __builtin_amdgcn_exp2f(ml.x - base);
+        L = fmaf(f, ml.y, L);
+        sum += *reinterpret_cast<const f32x4*>(a.part_o + (i * all + at) * Q8_D + d) * f;
+    }
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    *reinterpret_cast<uint2*>(a.out + (((size_t)seq * a.n + t) * a.nh + h * a.group + g) * Q8_D + d) =
+        make_uint2(pack_bf16x2(sum[0] * inv, sum[1] * inv), pack_bf16x2(sum[2] * inv, sum[3] * inv));
+    if (a.lse && d == 0) a.lse[at] = M + log2f(L);
+}
+
+// weights_out[token] = weights_in (0 for a new token) + sum of exp2(score - lse) over the rows of the KV head.  A wave takes
+// 64 tokens, one cache block, as the operand that stays in registers; the rows' queries stream past, the same for the
+// thread block's four waves.  Sums are in a fixed order.
+__global__ __launch_bounds__(256, 2) void attn_chunk_q8_weights_kernel(const ChunkQ8Args a) {
+    const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t h = blockIdx.x % a.c.nk;
     const uint32_t rest = blockIdx.x / a.c.nk;
-    const uint32_t b = rest % a.c.nb, seq = rest / a.c.nb;
+    const uint32_t per = (a.c.nb + 3) / 4;
+    const uint32_t seq = rest / per;
+    const int b = (int)(rest % per) * 4 + wave;
     const Q8Span s = q8_span(a.lengths, a.counts, seq, a.n, a.c.nb);
-    const int p0 = (int)b * Q8_BLOCK, p = p0 + lane;
-    if (p0 >= s.end) return;
-    const bool in_tail = p0 == s.end / Q8_BLOCK * Q8_BLOCK;
-    const int group = a.nh / a.c.nk;
-    const int count = a.counts ? min(a.counts[seq], (int)a.n) : (int)a.n;
-    const size_t wi = ((size_t)seq * a.c.nk + kvh) * a.c.nb * Q8_BLOCK + p;
-    float sum = 0.0f;
-    for (int t = 0; t < count; ++t) {
-        for (int g = 0; g < group; ++g) {
-            const size_t row = ((size_t)seq * a.n + t) * a.nh + kvh * group + g;
-            __syncthreads();
-            qs[lane] = q8_q(a, row * Q8_D + lane, F32);
-            qs[lane + 64] = q8_q(a, row * Q8_D + lane + 64, F32);
-            __syncthreads();
-            if (p < s.end && p <= a.lengths[seq] + t) sum += expf(q8_key_dot(a, seq, kvh, p, in_tail, qs) * a.scale - a.lse[row]);
-        }
+    if (b * Q8_BLOCK >= s.end) return;
+    const int len = min(a.lengths[seq], (int)(a.c.nb * Q8_BLOCK));
+    int count = a.counts ? a.counts[seq] : (int)a.n;
+    count = len < 0 || count < 0 ? 0 : (count < (int)a.n ? count : (int)a.n);
+    const int group = (int)a.group, rows = count * group;
+    const bool in_tail = s.end % Q8_BLOCK && b == s.end / Q8_BLOCK;
+    bf16x8 k[2][8];
+    float f = a.scale_log2;
+    if (in_tail) {
+        const uint16_t* p = a.c.kt + a.c.tail_at(seq, h) + 8 * half;
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) k[tt][i] = as_bf16x8(load_u4(p + (32 * tt + col) * Q8_D + 16 * i));
+    } else {
+        const int8_t* p = a.c.k + a.c.block_at(seq, (uint32_t)b, h) + 8 * half;
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint2 w = *reinterpret_cast<const uint2*>(p + (32 * tt + col) * Q8_D + 16 * i);
+                k[tt][i] = as_bf16x8(codes_bf16x8(w.x, w.y));
+            }
+        f *= a.c.ks[a.c.scale_at(seq, (uint32_t)b, h)];
     }
-    if (p < s.end) a.w_out[wi] = (p < s.len ? a.w_in[wi] : 0.0f) + sum;
+    float sum[2][16];
+#pragma unroll
+    for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) sum[tt][j] = 0.0f;
+    const float* lse = a.lse + ((size_t)seq * a.c.nk + h) * a.n * group;
+    // rows of queries that see the block's first token
+    const int t_first = b * Q8_BLOCK - len;
+    for (int row0 = t_first > 0 ? t_first * group / 32 * 32 : 0; row0 < rows; row0 += 32) {
+        const int row = row0 + col;
+        const int t = row / group, g = row - t * group;
+        const bool live = row < rows;
+        const uint16_t* qp = a.q + (((size_t)seq * a.n + (live ? t : 0)) * a.nh + h * group + (live ? g : 0)) * Q8_D + 8 * half;
+        const float sub = live ? lse[row] : INFINITY;
+        f32x16 x[2];
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) x[tt][j] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const bf16x8 q = as_bf16x8(load_u4(qp + 16 * i));
+            x[0] = mfma_bf16(k[0][i], q, x[0]);
+            x[1] = mfma_bf16(k[1][i], q, x[1]);
+        }
+        const int mine = len + t - b * Q8_BLOCK - 4 * half;  // tokens 32 tt + 8 (j / 4) + 4 half + j % 4
+        const bool edge = b * Q8_BLOCK + Q8_BLOCK - 1 > len + row0 / group;
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(x[tt][j], f, -sub));
+                sum[tt][j] += (!live || (edge && 32 * tt + 8 * (j >> 2) + (j & 3) > mine)) ? 0.0f : p;
+            }
+    }
+    // over the 32 rows that the lanes of a half hold
+#pragma unroll
+    for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            float v = sum[tt][j];
+            v += dpp_f32<0xB1>(v);
+            v += dpp_f32<0x4E>(v);
+            v += dpp_f32<0x141>(v);
+            v += dpp_f32<0x140>(v);
+            sum[tt][j] = xor_sum<16>(v);
+        }
+    if (col != 0) return;
+    const size_t at = ((size_t)seq * a.c.nk + h) * a.c.nb * Q8_BLOCK;
+#pragma unroll
+    for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const int p = b * Q8_BLOCK + 32 * tt + 8 * (j >> 2) + 4 * half + (j & 3);
+            if (p < s.end) a.w_out[at + p] = (p < s.len ? a.w_in[at + p] : 0.0f) + sum[tt][j];
+        }
 }
 
-template <bool F32>
-static int attn_q8_launch(const AttnQ8Args& a, void* stream) {
-    const uint64_t rows = (uint64_t)a.n_seq * a.n * a.nh, blocks = (uint64_t)a.n_seq * a.c.nb * a.c.nk;
-    if (rows > 0x7fffffffu || blocks > 0x7fffffffu) return T2H_ERR_SHAPE;
-    hipLaunchKernelGGL(attn_q8_kernel<F32>, dim3((uint32_t)rows), dim3(64), 0, reinterpret_cast<hipStream_t>(stream), a);
-    T2H_LAUNCH_CHECK();
-    if (a.w_out) {
-        hipLaunchKernelGGL(attn_q8_weights_kernel<F32>, dim3((uint32_t)blocks), dim3(64), 0, reinterpret_cast<hipStream_t>(stream), a);
-        T2H_LAUNCH_CHECK();
-    }
-    return T2H_OK;
+// Thread blocks that share a tile's keys: enough for two a CU, where a tile has at least 4 blocks of keys for each.
+static uint32_t cq_splits(uint32_t n, uint32_t n_seq, uint32_t nh, uint32_t nk, uint32_t nb) {
+    const uint64_t tiles = ((uint64_t)n * (nh / nk) + CQ_ROWS - 1) / CQ_ROWS;
+    const uint64_t grid = tiles * n_seq * nk;
+    const uint64_t want = grid ? (512 + grid - 1) / grid : 1, most = nb / 4;
+    return (uint32_t)(want < most ? (want ? want : 1) : (most ? most : 1));
 }
 
 }  // namespace t2h
@@ -753,14 +1059,17 @@ extern "C" int t2h_attn_decode_q8(const float* q, uint64_t q_row, const float* k
 
 extern "C" size_t t2h_flash_attn_prefill_q8_workspace_bytes(uint32_t n, uint32_t n_seq, uint32_t nh, uint32_t nk,
                                                             uint32_t s_cap, int weights) {
-    return (size_t)n_seq * n * nh * 4 + 256;
+    if (n_seq == 0 || nk == 0 || nh == 0 || nh % nk != 0 || nh / nk > Q8_MAX_GROUP || s_cap == 0 || s_cap % Q8_BLOCK != 0) return 0;
+    const size_t rows = (size_t)n_seq * nh * n;
+    const uint32_t splits = cq_splits(n, n_seq, nh, nk, s_cap / Q8_BLOCK);
+    return 16 + (weights ? rows * 4 : 0) + (splits > 1 ? splits * rows * (Q8_D + 2) * 4 : 0);
 }
 
 extern "C" int t2h_flash_attn_prefill_q8(const void* q, void* const* cache, uint32_t s_cap, const int32_t* lengths,
                                          const int32_t* counts, const float* weights, float* weights_out, void* out,
                                          uint32_t n, uint32_t n_seq, uint32_t nh, uint32_t nk, uint32_t d, float scale,
                                          void* workspace, size_t workspace_bytes, void* stream) {
-    AttnQ8Args a;
+    ChunkQ8Args a;
     if (!q || !lengths || !out || !workspace) return T2H_ERR_NULL;
     if ((weights == nullptr) != (weights_out == nullptr)) return T2H_ERR_NULL;
     if (const int e = q8_cache(cache, s_cap, n_seq, nh, nk, d, a.c)) return e;
@@ -769,9 +1078,8 @@ extern "C" int t2h_flash_attn_prefill_q8(const void* q, void* const* cache, uint
     if (workspace_bytes < t2h_flash_attn_prefill_q8_workspace_bytes(n, n_seq, nh, nk, s_cap, weights != nullptr))
         return T2H_ERR_WORKSPACE;
     if (n == 0) return T2H_OK;
-    a.q = q;
+    a.q = reinterpret_cast<const uint16_t*>(q);
     a.out = reinterpret_cast<uint16_t*>(out);
-    a.lse = reinterpret_cast<float*>(workspace);
     a.lengths = lengths;
     a.counts = counts;
     a.w_in = weights;
@@ -779,6 +1087,33 @@ extern "C" int t2h_flash_attn_prefill_q8(const void* q, void* const* cache, uint
     a.n = n;
     a.n_seq = n_seq;
     a.nh = nh;
-    a.scale = scale > 0.0f ? scale : 1.0f / sqrtf((float)Q8_D);
-    return attn_q8_launch<false>(a, stream);
+    a.group = nh / nk;
+    a.scale_log2 = 1.4426950408889634f * (scale > 0.0f ? scale : 1.0f / sqrtf((float)Q8_D));
+    const uint64_t rows = (uint64_t)n_seq * nh * n, tiles = ((uint64_t)n * a.group + CQ_ROWS - 1) / CQ_ROWS;
+    if (rows > 0x3fffffffu) return T2H_ERR_SHAPE;
+    a.splits = cq_splits(n, n_seq, nh, nk, a.c.nb);
+    a.tiles = (uint32_t)tiles;
+    float* at = reinterpret_cast<float*>(workspace);
+    a.part_o = a.part_ml = a.lse = nullptr;
+    if (a.splits > 1) {
+        a.part_o = at;
+        a.part_ml = at + a.splits * rows * Q8_D;
+        at += a.splits * rows * (Q8_D + 2);
+    }
+    if (weights) a.lse = at;
+    const uint64_t grid = tiles * n_seq * nk * a.splits, merge = (rows + 7) / 8;
+    const uint64_t wgrid = (uint64_t)n_seq * nk * ((a.c.nb + 3) / 4);
+    if (grid > 0x7fffffffu || wgrid > 0x7fffffffu) return T2H_ERR_SHAPE;
+    const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    hipLaunchKernelGGL(attn_chunk_q8_kernel, dim3((uint32_t)grid), dim3(CQ_WAVES * 64), 0, st, a);
+    T2H_LAUNCH_CHECK();
+    if (a.splits > 1) {
+        hipLaunchKernelGGL(attn_chunk_q8_merge_kernel, dim3((uint32_t)merge), dim3(256), 0, st, a);
+        T2H_LAUNCH_CHECK();
+    }
+    if (weights) {
+        hipLaunchKernelGGL(attn_chunk_q8_weights_kernel, dim3((uint32_t)wgrid), dim3(256), 0, st, a);
+        T2H_LAUNCH_CHECK();
+    }
+    return T2H_OK;
 }
