@@ -611,8 +611,8 @@ int t2h_qk_norm_rope_cache_q8(const float* q, uint64_t q_row, const float* k, ui
  * weights / weights_out (fp32 [n_seq, nk, s_cap], both or neither, the same or distinct): weights_out = weights + the
  * softmax weight that each cached token got, summed over the q heads of the KV head; a new token's begins at 0, and
  * elements behind the last token are left as they are.
- * workspace: t2h_attn_decode_q8_workspace_bytes() bytes, 16-byte aligned, no initialisation; calls that share one must not
- * overlap in time. */
+ * workspace: t2h_attn_decode_q8_workspace_bytes() bytes, 16-byte aligned, zero-filled once before its first use (calls
+ * leave it reusable); calls that share one must not overlap in time. */
 size_t t2h_attn_decode_q8_workspace_bytes(uint32_t n_seq, uint32_t nh, uint32_t nk, uint32_t d, uint32_t s_cap,
                                           int weights);
 int t2h_attn_decode_q8(const float* q, uint64_t q_row, const float* k_new, uint64_t k_row, const float* v_new,
@@ -622,7 +622,8 @@ int t2h_attn_decode_q8(const float* q, uint64_t q_row, const float* k_new, uint6
                        uint32_t d, void* workspace, size_t workspace_bytes, void* stream);
 /* Causal attention of a chunk that t2h_qk_norm_rope_cache_q8 has written, with the same lengths and counts: query t of
  * q bf16 [n_seq, n, nh, 128] sees tokens 0 .. length + t.  out as q (both 16-byte aligned); scale <= 0 means 1 / sqrt(128);
- * weights and workspace as above (the weights of all the chunk's queries). */
+ * weights as above, of all the chunk's queries.  workspace: 16-byte aligned, no initialisation; calls that share one must
+ * not overlap in time. */
 size_t t2h_flash_attn_prefill_q8_workspace_bytes(uint32_t n, uint32_t n_seq, uint32_t nh, uint32_t nk, uint32_t s_cap,
                                                  int weights);
 int t2h_flash_attn_prefill_q8(const void* q, void* const* cache, uint32_t s_cap, const int32_t* lengths,

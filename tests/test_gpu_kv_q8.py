@@ -277,7 +277,6 @@ def test_decode(device, nh, nk, lengths, s_cap, weights):
     w = torch.rand(n_seq, nk, s_cap, device=device) if weights else None
     w_out = torch.full_like(w, 0.25) if weights else None
     ws = K.attn_decode_q8_workspace(n_seq, nh, nk, D, s_cap, device, weights=weights)
-    ws.fill_(0xff)
     out = torch.full((n_seq, nh, D), math.nan, dtype=BF, device=device)
     K.attn_decode_q8(q, k, v, c, out, ints(lengths, device), ws, theta=1e6, rope_offsets=ints(offsets, device),
                      q_norm_weight=wq, k_norm_weight=wk, eps=EPS, weights=w, weights_out=w_out)

@@ -32,7 +32,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int DQ_WAVES = 4;
 constexpr int DQ_ROW = Q8_D + 4;          // fp32 row in LDS, padded
-constexpr uint32_t DQ_TARGET = 2048;      // thread blocks that a call is cut into, at most (+ one a sequence and head)
+constexpr int DQ_QROW = Q8_D + 8;         // fp16 row
 constexpr float DQ_P_SCALE = 4096.0f;
 
 struct DecodeQ8Args {
@@ -50,6 +50,7 @@ struct DecodeQ8Args {
     uint16_t* out;
     float* part_ml;  // [units][nk][group][2]: log2 maximum, sum
     float* part_o;   // [units][nk][group][128]
+    uint32_t* done;  // [n_seq][nk] units that have left their parts; zero between calls
     float* scores;   // [n_seq][nh][s_cap] log2 scores, or null
     uint32_t n_seq, nh, group, target, units;
     float eps, scale_log2;
@@ -83,14 +84,15 @@ __device__ __forceinline__ int dq_chunk(const DecodeQ8Args& a, uint32_t total) {
     return c <= 2 ? (c ? (int)c : 1) : (int)((c + DQ_WAVES - 1) / DQ_WAVES * DQ_WAVES);
 }
 
-// The sequence that unit `unit` belongs to (by_seq false), or sequence `unit` itself; false where there is none.
+// The sequence that unit `unit` belongs to (by_seq false), or sequence `unit` itself; false where there is none.  A
+// sequence without blocks has one unit, which writes its zeros.
 __device__ bool dq_find(const DecodeQ8Args& a, uint32_t unit, bool by_seq, DecodeUnit& u) {
     const uint32_t lane = threadIdx.x & 63;
     if (a.n_seq == 1) {
         u.blocks = dq_blocks(a, 0);
         u.chunk = dq_chunk(a, (uint32_t)u.blocks);
         u.seq = u.first = 0;
-        u.count = (uint32_t)((u.blocks + u.chunk - 1) / u.chunk);
+        u.count = u.blocks ? (uint32_t)((u.blocks + u.chunk - 1) / u.chunk) : 1u;
         u.len = a.lengths[0];
         return by_seq || unit < u.count;
     }
@@ -101,7 +103,8 @@ __device__ bool dq_find(const DecodeQ8Args& a, uint32_t unit, bool by_seq, Decod
     uint32_t before = 0;
     for (uint32_t base = 0; base < a.n_seq; base += 64) {
         const uint32_t i = base + lane;
-        const uint32_t mine = i < a.n_seq ? ((uint32_t)dq_blocks(a, i) + u.chunk - 1) / u.chunk : 0u;
+        const uint32_t n = i < a.n_seq ? (uint32_t)dq_blocks(a, i) : 0u;
+        const uint32_t mine = i < a.n_seq ? (n ? (n + u.chunk - 1) / u.chunk : 1u) : 0u;
         const uint32_t upto = before + wave_scan_u32(mine);
         const uint64_t hit = by_seq ? __ballot(i == unit) : __ballot(unit >= upto - mine && unit < upto);
         if (hit) {
@@ -136,9 +139,10 @@ __device__ __forceinline__ f16x8 codes_f16x8(uint32_t w0, uint32_t w1) {
 __device__ __forceinline__ bf16x8 as_bf16x8(uint4 v) { return __builtin_bit_cast(bf16x8, v); }
 
 // A block that its last token finishes, rounded by one wave from the tail's rows and that token: two passes over 32 KB,
-// once in 64 tokens.  The codes are in memory for the wave itself when this returns.
-__device__ __forceinline__ void dq_round(const KvQ8& c, uint32_t seq, uint32_t h, uint32_t b, const uint16_t* key,
-                                         const uint16_t* value) {
+// once in 64 tokens.  The codes are in memory for the wave itself when this returns the values' scale.
+__device__ __forceinline__ float dq_round(const KvQ8& c, uint32_t seq, uint32_t h, uint32_t b, const uint16_t* key,
+                                          const uint16_t* value) {
+    float s = 0.0f;
     const int lane = threadIdx.x & 63;
     const size_t tail = c.tail_at(seq, h), at = c.block_at(seq, b, h);
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -167,7 +171,7 @@ __device__ __forceinline__ void dq_round(const KvQ8& c, uint32_t seq, uint32_t h
             for (int i = 0; i < 8; ++i) top = max(top, max(w[i] << 16 & 0x7fffffffu, w[i] & 0x7fff0000u));
         }
         top = wave_max_u32(top);
-        float s, inv;
+        float inv;
         q8_scale(top, s, inv);
 #pragma unroll 2
         for (int n = 0; n < 8; ++n) {
@@ -183,15 +187,27 @@ __device__ __forceinline__ void dq_round(const KvQ8& c, uint32_t seq, uint32_t h
         if (lane == 0) (half == 0 ? c.ks : c.vs)[c.scale_at(seq, b, h)] = s;
     }
     __threadfence_block();  // other lanes of the wave read them
+    return s;
+}
+
+// Two floats past the caches that the chip's parts do not share.
+__device__ __forceinline__ void put_pair(float* p, float x, float y) {
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), (uint64_t)__float_as_uint(x) | (uint64_t)__float_as_uint(y) << 32,
+                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 get_pair(const float* p) {
+    const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
 }
 
 template <bool WEIGHTS>
 __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_decode_q8_kernel(const DecodeQ8Args a) {
-    __shared__ __align__(16) float qs[16][DQ_ROW];            // q of each head, its largest value in [1, 2)
+    __shared__ __align__(16) _Float16 qs[2][16][DQ_QROW];      // q's two terms, its largest value in [1, 2)
     __shared__ float qf[16];                                  // what that took off, with the softmax's scale and log2 e
     __shared__ __align__(16) uint16_t fresh[2][Q8_D];         // the new token's key and value
     __shared__ float wml[DQ_WAVES][16][2];
     __shared__ __align__(16) float wo[DQ_WAVES][16][DQ_ROW];
+    __shared__ uint32_t arrived;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t h = blockIdx.x % a.c.nk;
@@ -199,6 +215,11 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_decode_q8_kernel(const 
     DecodeUnit u;
     if (!dq_find(a, unit, false, u)) return;  // (every wave of a thread block finds the same)
     const int group = (int)a.group;
+    uint32_t* const out = reinterpret_cast<uint32_t*>(a.out + ((size_t)u.seq * a.nh + h * group) * Q8_D);
+    if (u.blocks == 0) {
+        for (int i = tid; i < group * (Q8_D / 2); i += DQ_WAVES * 64) out[i] = 0u;
+        return;
+    }
     const int b0 = (int)(unit - u.first) * u.chunk;
     const int b1 = b0 + u.chunk < u.blocks ? b0 + u.chunk : u.blocks;
     const int c = lane & 15, g4 = lane >> 4;
@@ -206,8 +227,45 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_decode_q8_kernel(const 
     const int new_b = has_new ? u.len / Q8_BLOCK : -1;  // the block of the new token, in bf16 unless the token finishes it
     const int r = u.len % Q8_BLOCK;
     const int tail_b = r == Q8_BLOCK - 1 ? -1 : new_b;
+    const bool writes = new_b >= b0 && new_b < b1 && (new_b - b0) % DQ_WAVES == wave;
+    const bool has_tail = writes && tail_b >= 0;
 
-    // 1. the first block's codes
+    // 1. the small operands (loads return in order: what is asked for after the codes would wait for them), then the first
+    // block's codes
+    const bool has_w = a.q_norm_w != nullptr;
+    float w0 = 1.0f, w1 = 1.0f, kw0 = 1.0f, kw1 = 1.0f;
+    if (has_w) {
+        w0 = a.q_norm_w[lane];
+        w1 = a.q_norm_w[lane + 64];
+    }
+    float x0[4], x1[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int g = wave + DQ_WAVES * i < group ? wave + DQ_WAVES * i : 0;
+        const float* x = a.q + u.seq * a.q_row + (size_t)(h * group + g) * Q8_D;
+        if (DQ_WAVES * i < group) {
+            x0[i] = x[lane];
+            x1[i] = x[lane + 64];
+        }
+    }
+    float kx0 = 0.0f, kx1 = 0.0f, vx0 = 0.0f, vx1 = 0.0f;
+    if (writes) {
+        const float* kx = a.k_new + u.seq * a.k_row + (size_t)h * Q8_D;
+        const float* vx = a.v_new + u.seq * a.v_row + (size_t)h * Q8_D;
+        kx0 = kx[lane];
+        kx1 = kx[lane + 64];
+        vx0 = vx[lane];
+        vx1 = vx[lane + 64];
+        if (has_w) {
+            kw0 = a.k_norm_w[lane];
+            kw1 = a.k_norm_w[lane + 64];
+        }
+    }
+    const int pos = u.len + (a.offsets ? a.offsets[u.seq] : 0);
+    // the largest value scale of the wave's blocks; a block that is only now rounded comes later
+    float smax = 0.0f;
+    for (int i = b0 + wave + DQ_WAVES * lane; i < b1; i += DQ_WAVES * 64)
+        if (i != new_b) smax = fmaxf(smax, a.c.vs[a.c.scale_at(u.seq, (uint32_t)i, h)]);
     const int krow = ((c >> 2) * 16 + (c & 3)) * Q8_D + g4 * 16;  // + t * 4 rows + j * 64
     const int vrow = c * Q8_BLOCK + g4 * 16;                      // + dt * 16 rows
     uint4 kr[4][2], vr[8];
@@ -227,72 +285,58 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_decode_q8_kernel(const 
         vs = a.c.vs[a.c.scale_at(u.seq, (uint32_t)b, h)];
     };
     int b = b0 + wave;
-    const bool writes = new_b >= b0 && new_b < b1 && (new_b - b0) % DQ_WAVES == wave;
-    const bool has_tail = writes && tail_b >= 0;
     if (b < b1 && b != new_b) {
         load_k(b);
         load_v(b);
     }
 
     // 2. q and the new token
-    const int pos = u.len + (a.offsets ? a.offsets[u.seq] : 0);
     float cs = 1.0f, sn = 0.0f;
     if (a.rope && (wave < group || writes)) rope_at(rope_turns(lane, a.log2_theta), pos, cs, sn);
-    const bool has_w = a.q_norm_w != nullptr;
-    for (int g = wave; g < group; g += DQ_WAVES) {
-        const float* x = a.q + u.seq * a.q_row + (size_t)(h * group + g) * Q8_D;
-        const float w0 = has_w ? a.q_norm_w[lane] : 1.0f, w1 = has_w ? a.q_norm_w[lane + 64] : 1.0f;
-        float r0, r1;
-        norm_rope_pair(x[lane], x[lane + 64], has_w, w0, w1, a.eps, cs, sn, a.rope != 0, r0, r1);
-        uint32_t e = wave_max_u32(max(abs_bits(r0), abs_bits(r1))) >> 23;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int g = wave + DQ_WAVES * i;
+        if (g >= group) break;
+        float y[2];
+        norm_rope_pair(x0[i], x1[i], has_w, w0, w1, a.eps, cs, sn, a.rope != 0, y[0], y[1]);
+        uint32_t e = wave_max_u32(max(abs_bits(y[0]), abs_bits(y[1]))) >> 23;
         e = e < 1 ? 1 : (e > 253 ? 253 : e);
         const float down = __uint_as_float((254u - e) << 23);
-        qs[g][lane] = r0 * down;
-        qs[g][lane + 64] = r1 * down;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const _Float16 hi = (_Float16)(y[n] * down);
+            qs[0][g][lane + 64 * n] = hi;
+            qs[1][g][lane + 64 * n] = (_Float16)(y[n] * down - (float)hi);
+        }
         if (lane == 0) qf[g] = __uint_as_float(e << 23) * a.scale_log2;
     }
     if (writes) {
-        const float* kx = a.k_new + u.seq * a.k_row + (size_t)h * Q8_D;
-        const float* vx = a.v_new + u.seq * a.v_row + (size_t)h * Q8_D;
-        const float w0 = has_w ? a.k_norm_w[lane] : 1.0f, w1 = has_w ? a.k_norm_w[lane + 64] : 1.0f;
-        float r0, r1;
-        norm_rope_pair(kx[lane], kx[lane + 64], has_w, w0, w1, a.eps, cs, sn, a.rope != 0, r0, r1);
-        const uint16_t kb[2] = {(uint16_t)f32_to_bf16_bits(r0), (uint16_t)f32_to_bf16_bits(r1)};
-        const uint16_t vb[2] = {(uint16_t)f32_to_bf16_bits(vx[lane]), (uint16_t)f32_to_bf16_bits(vx[lane + 64])};
+        float y[2];
+        norm_rope_pair(kx0, kx1, has_w, kw0, kw1, a.eps, cs, sn, a.rope != 0, y[0], y[1]);
+        const float v[2] = {vx0, vx1};
         const size_t tail = a.c.tail_at(u.seq, h);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            fresh[0][lane + 64 * i] = kb[i];
-            fresh[1][lane + 64 * i] = vb[i];
-            a.c.kt[tail + r * Q8_D + lane + 64 * i] = kb[i];
-            a.c.vt[tail + (lane + 64 * i) * Q8_BLOCK + r] = vb[i];
+            const uint16_t kb = (uint16_t)f32_to_bf16_bits(y[i]), vb = (uint16_t)f32_to_bf16_bits(v[i]);
+            fresh[0][lane + 64 * i] = kb;
+            fresh[1][lane + 64 * i] = vb;
+            a.c.kt[tail + r * Q8_D + lane + 64 * i] = kb;
+            a.c.vt[tail + (lane + 64 * i) * Q8_BLOCK + r] = vb;
         }
         if (tail_b < 0) {
-            dq_round(a.c, u.seq, h, (uint32_t)new_b, fresh[0], fresh[1]);
+            smax = fmaxf(smax, dq_round(a.c, u.seq, h, (uint32_t)new_b, fresh[0], fresh[1]));
             if (b == new_b) {
                 load_k(b);
                 load_v(b);
             }
         }
     }
-    // the largest value scale of the wave's blocks
-    float smax = 0.0f;
-    for (int i = b0 + wave + DQ_WAVES * lane; i < b1; i += DQ_WAVES * 64)
-        if (i != tail_b) smax = fmaxf(smax, a.c.vs[a.c.scale_at(u.seq, (uint32_t)i, h)]);
     __syncthreads();
-    f16x8 qh[2][2], ql[2][2];  // q's two terms at dims 64 j + 16 g4 + 8 i
-    const float qfac = c < group ? qf[c] : 0.0f;
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float x = c < group ? qs[c][64 * j + 16 * g4 + 8 * i + e] : 0.0f;
-                qh[j][i][e] = (_Float16)x;
-                ql[j][i][e] = (_Float16)(x - (float)qh[j][i][e]);
-            }
+    const float qfac = qf[c];  // lanes past the group hold what no one reads: a head is a column of the products
     smax = wave_max(smax);
+    auto query = [&](int term, int j, int i) {  // dims 64 j + 16 g4 + 8 i
+        return *reinterpret_cast<const f16x8*>(&qs[term][c][64 * j + 16 * g4 + 8 * i]);
+    };
 
     // 3. the wave's blocks
     float m = -INFINITY, l = 0.0f;
@@ -338,15 +382,17 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_decode_q8_kernel(const 
 #pragma unroll
         for (int t = 0; t < 4; ++t) x[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int j = 0; j < 2; ++j) {
+            const f16x8 h0 = query(0, j, 0), l0 = query(1, j, 0), h1 = query(0, j, 1), l1 = query(1, j, 1);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
+            for (int t = 0; t < 4; ++t) {
                 const f16x8 k0 = codes_f16x8(kr[t][j].x, kr[t][j].y), k1 = codes_f16x8(kr[t][j].z, kr[t][j].w);
-                x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qh[j][0], x[t], 0, 0, 0);
-                x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, ql[j][0], x[t], 0, 0, 0);
-                x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qh[j][1], x[t], 0, 0, 0);
-                x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, ql[j][1], x[t], 0, 0, 0);
+                x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, h0, x[t], 0, 0, 0);
+                x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, l0, x[t], 0, 0, 0);
+                x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, h1, x[t], 0, 0, 0);
+                x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, l1, x[t], 0, 0, 0);
             }
+        }
         const float fk = ks * qfac;
         const int next = b + DQ_WAVES;
         const bool more = next < b1 && next != tail_b;
@@ -377,10 +423,11 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_decode_q8_kernel(const 
         for (int n = 0; n < 4; ++n) {
             const int j = n >> 1, i = n & 1, d = 64 * j + 16 * g4 + 8 * i;
             __builtin_amdgcn_sched_barrier(0);
+            const f16x8 qhi = query(0, j, i), qlo = query(1, j, i);
             bf16x8 q3[3];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                float y = (float)qh[j][i][e] + (float)ql[j][i][e];
+                float y = (float)qhi[e] + (float)qlo[e];
 #pragma unroll
                 for (int z = 0; z < 3; ++z) {
                     q3[z][e] = (__bf16)y;
@@ -459,13 +506,68 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_decode_q8_kernel(const 
         const size_t part = ((size_t)unit * a.c.nk + h) * a.group + g;
         if (u.count == 1) {
             const float inv = 1.0f / L;
-            uint32_t* to = reinterpret_cast<uint32_t*>(a.out + ((size_t)u.seq * a.nh + h * group + g) * Q8_D + d);
-            to[0] = pack_bf16x2(sum[0] * inv, sum[1] * inv);
-            to[1] = pack_bf16x2(sum[2] * inv, sum[3] * inv);
+            out[(g * Q8_D + d) / 2] = pack_bf16x2(sum[0] * inv, sum[1] * inv);
+            out[(g * Q8_D + d) / 2 + 1] = pack_bf16x2(sum[2] * inv, sum[3] * inv);
         } else {
-            *reinterpret_cast<f32x4*>(a.part_o + part * Q8_D + d) = sum;
+            put_pair(a.part_o + part * Q8_D + d, sum[0], sum[1]);
+            put_pair(a.part_o + part * Q8_D + d + 2, sum[2], sum[3]);
         }
-        if (d == 0 && (WEIGHTS || u.count > 1)) *reinterpret_cast<float2*>(a.part_ml + 2 * part) = make_float2(M, L);
+        if (d == 0 && (WEIGHTS || u.count > 1)) put_pair(a.part_ml + 2 * part, M, L);
+    }
+    if (u.count == 1) return;
+
+    // 5. the last unit of a (sequence, head) to get here joins them.  Parts are written and read past the caches that the
+    // chip's parts do not share (agent scope), and are there before the count is raised.
+    __builtin_amdgcn_s_waitcnt(0);
+    asm volatile("" ::: "memory");
+    __syncthreads();
+    if (tid == 0) {
+        uint32_t* const done = a.done + (size_t)u.seq * a.c.nk + h;
+        arrived = __hip_atomic_fetch_add(done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u;
+        if (arrived == u.count) __hip_atomic_store(done, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (arrived != u.count) return;
+    // slices of the units, each a sum of its own in LDS
+    const int pieces = group * (Q8_D / 4);
+    const int slices = DQ_WAVES * 64 / pieces > 0 ? DQ_WAVES * 64 / pieces : 1;
+    for (int i = tid; i < pieces * slices; i += DQ_WAVES * 64) {
+        const int slice = i / pieces, g = i % pieces / (Q8_D / 4), d = i % (Q8_D / 4) * 4;
+        float M = -INFINITY, L = 0.0f;
+        f32x4 sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+        for (uint32_t n = (uint32_t)slice; n < u.count; n += (uint32_t)slices) {
+            const size_t part = ((size_t)(u.first + n) * a.c.nk + h) * a.group + g;
+            const float2 ml = get_pair(a.part_ml + 2 * part), lo = get_pair(a.part_o + part * Q8_D + d),
+                         hi = get_pair(a.part_o + part * Q8_D + d + 2);
+            const float now = fmaxf(M, ml.x), base = now == -INFINITY ? 0.0f : now;
+            const float keep = __builtin_amdgcn_exp2f(M - base), f = __builtin_amdgcn_exp2f(ml.x - base);
+            L = fmaf(L, keep, f * ml.y);
+            sum = sum * keep + f32x4{lo.x, lo.y, hi.x, hi.y} * f;
+            M = now;
+        }
+        const int at = slice * group + g;  // less than 16: 8 slices are of one head
+        *reinterpret_cast<f32x4*>(&wo[0][at][d]) = sum;
+        if (d == 0) {
+            wml[0][at][0] = M;
+            wml[0][at][1] = L;
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < pieces; i += DQ_WAVES * 64) {
+        const int g = i / (Q8_D / 4), d = i % (Q8_D / 4) * 4;
+        float M = -INFINITY, L = 0.0f;
+        for (int n = 0; n < slices; ++n) M = fmaxf(M, wml[0][n * group + g][0]);
+        const float base = M == -INFINITY ? 0.0f : M;
+        f32x4 sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int n = 0; n < slices; ++n) {
+            const float f = __builtin_amdgcn_exp2f(wml[0][n * group + g][0] - base);
+            L = fmaf(f, wml[0][n * group + g][1], L);
+            sum += *reinterpret_cast<const f32x4*>(&wo[0][n * group + g][d]) * f;
+        }
+        const float inv = 1.0f / L;
+        out[(g * Q8_D + d) / 2] = pack_bf16x2(sum[0] * inv, sum[1] * inv);
+        out[(g * Q8_D + d) / 2 + 1] = pack_bf16x2(sum[2] * inv, sum[3] * inv);
     }
 }
 
@@ -486,77 +588,48 @@ __device__ __forceinline__ void dq_total(const DecodeQ8Args& a, const DecodeUnit
 
 constexpr int DQ_SEGMENT = 1024;  // tokens of a thread block that adds up weights
 
-// Thread blocks [0, n_seq nh): a head's units joined.  Behind them, with weights: 1024 tokens of a (sequence, KV head),
-// exp2(score - log2 sum) over its heads.
-template <bool WEIGHTS>
-__global__ __launch_bounds__(256) void attn_decode_q8_merge_kernel(const DecodeQ8Args a) {
-    __shared__ __align__(16) float part[8][Q8_D];
+// weights_out[token] = weights_in (0 for the new token) + sum of exp2(score - log2 sum) over the heads of the KV head:
+// 1024 tokens of a (sequence, KV head) a thread block.
+__global__ __launch_bounds__(256) void attn_decode_q8_weights_kernel(const DecodeQ8Args a) {
     __shared__ float lse[16];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const uint32_t h = blockIdx.x % a.c.nk, rest = blockIdx.x / a.c.nk;
+    const uint32_t segments = (a.c.nb * Q8_BLOCK + DQ_SEGMENT - 1) / DQ_SEGMENT;
+    const uint32_t seq = rest / segments;
+    const int first = (int)(rest % segments) * DQ_SEGMENT, t0 = first + 4 * tid;
+    const int len = a.lengths[seq], cap = (int)(a.c.nb * Q8_BLOCK);
+    const int end = len < 0 ? 0 : (len < cap ? len + 1 : cap);
+    if (first >= end) return;
     DecodeUnit u;
-    if (blockIdx.x < a.n_seq * a.nh) {
-        const uint32_t seq = blockIdx.x / a.nh, head = blockIdx.x % a.nh;
-        const uint32_t h = head / a.group, g = head % a.group;
-        dq_find(a, seq, true, u);
-        uint32_t* out = reinterpret_cast<uint32_t*>(a.out + (size_t)blockIdx.x * Q8_D);
-        if (u.count == 0 && tid < 64) out[tid] = 0u;  // takes no part
-        if (u.count <= 1) return;
+    dq_find(a, seq, true, u);
+    for (uint32_t g = wave; g < a.group; g += 4) {
         float M, L;
         dq_total(a, u, h, g, M, L);
-        const float base = M == -INFINITY ? 0.0f : M;
-        const int slot = tid >> 5, d = (tid & 31) * 4;
-        f32x4 sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-        for (uint32_t i = (uint32_t)slot; i < u.count; i += 8) {
-            const size_t at = ((size_t)(u.first + i) * a.c.nk + h) * a.group + g;
-            sum += *reinterpret_cast<const f32x4*>(a.part_o + at * Q8_D + d) * __builtin_amdgcn_exp2f(a.part_ml[2 * at] - base);
-        }
-        *reinterpret_cast<f32x4*>(&part[slot][d]) = sum;
-        __syncthreads();
-        if (tid < 64) {
-            float s0 = 0.0f, s1 = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                s0 += part[i][2 * tid];
-                s1 += part[i][2 * tid + 1];
-            }
-            const float inv = 1.0f / L;
-            out[tid] = pack_bf16x2(s0 * inv, s1 * inv);
-        }
-        return;
+        if (lane == 0) lse[g] = M + log2f(L);
     }
-    if constexpr (WEIGHTS) {
-        const uint32_t i = blockIdx.x - a.n_seq * a.nh;
-        const uint32_t h = i % a.c.nk, rest = i / a.c.nk;
-        const uint32_t segments = (a.c.nb * Q8_BLOCK + DQ_SEGMENT - 1) / DQ_SEGMENT;
-        const uint32_t seq = rest / segments;
-        const int t0 = (int)(rest % segments) * DQ_SEGMENT + 4 * tid;
-        const int len = a.lengths[seq], cap = (int)(a.c.nb * Q8_BLOCK);
-        const int end = len < 0 ? 0 : (len < cap ? len + 1 : cap);
-        if ((int)(rest % segments) * DQ_SEGMENT >= end) return;
-        dq_find(a, seq, true, u);
-        for (uint32_t g = wave; g < a.group; g += 4) {
-            float M, L;
-            dq_total(a, u, h, g, M, L);
-            if (lane == 0) lse[g] = M + log2f(L);
-        }
-        __syncthreads();
-        if (t0 >= end) return;
-        f32x4 sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        for (uint32_t g = 0; g < a.group; ++g) {
-            const f32x4 s = *reinterpret_cast<const f32x4*>(a.scores + ((size_t)seq * a.nh + h * a.group + g) * cap + t0);
+    __syncthreads();
+    if (t0 >= end) return;
+    f32x4 sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t g = 0; g < a.group; ++g) {
+        const f32x4 s = *reinterpret_cast<const f32x4*>(a.scores + ((size_t)seq * a.nh + h * a.group + g) * cap + t0);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) sum[j] += __builtin_amdgcn_exp2f(s[j] - lse[g]);
-        }
-        const size_t at = ((size_t)seq * a.c.nk + h) * cap + t0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (t0 + j < end) a.w_out[at + j] = (t0 + j < len ? a.w_in[at + j] : 0.0f) + sum[j];
+        for (int j = 0; j < 4; ++j) sum[j] += __builtin_amdgcn_exp2f(s[j] - lse[g]);
     }
+    const size_t at = ((size_t)seq * a.c.nk + h) * cap + t0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (t0 + j < end) a.w_out[at + j] = (t0 + j < len ? a.w_in[at + j] : 0.0f) + sum[j];
+}
+
+// Thread blocks that a call is cut into (and one more a sequence and head): two a CU for one sequence, so that a head has
+// few parts to join, and four units a (sequence, head) where there are many, so that ragged lengths even out.
+static uint32_t dq_target(uint32_t n_seq, uint32_t nk) {
+    const uint64_t heads = (uint64_t)n_seq * nk;
+    return heads <= 128 ? 512u : (heads >= 1024 ? 4096u : (uint32_t)(4 * heads));
 }
 
 static uint32_t dq_units(uint32_t n_seq, uint32_t nk, uint32_t nb) {
-    const uint64_t a = (uint64_t)DQ_TARGET / nk + n_seq, b = (uint64_t)n_seq * nb;
+    const uint64_t a = (uint64_t)dq_target(n_seq, nk) / nk + n_seq, b = (uint64_t)n_seq * nb;
     return (uint32_t)(a < b ? a : b);
 }
 
@@ -997,7 +1070,7 @@ extern "C" size_t t2h_attn_decode_q8_workspace_bytes(uint32_t n_seq, uint32_t nh
         s_cap % Q8_BLOCK != 0)
         return 0;
     const size_t parts = (size_t)dq_units(n_seq, nk, s_cap / Q8_BLOCK) * nh;
-    return parts * (Q8_D + 2) * 4 + 16 + (weights ? (size_t)n_seq * nh * s_cap * 4 : 0);
+    return ((size_t)n_seq * nk * 4 + 15) / 16 * 16 + (parts * (Q8_D + 2) * 4 + 15) / 16 * 16 + (weights ? (size_t)n_seq * nh * s_cap * 4 : 0);
 }
 
 extern "C" int t2h_attn_decode_q8(const float* q, uint64_t q_row, const float* k_new, uint64_t k_row, const float* v_new,
@@ -1029,10 +1102,11 @@ extern "C" int t2h_attn_decode_q8(const float* q, uint64_t q_row, const float* k
     a.n_seq = n_seq;
     a.nh = nh;
     a.group = nh / nk;
-    a.target = DQ_TARGET;
+    a.target = dq_target(n_seq, nk);
     a.units = dq_units(n_seq, nk, a.c.nb);
     const size_t parts = (size_t)a.units * nh;
-    a.part_o = reinterpret_cast<float*>(workspace);
+    a.done = reinterpret_cast<uint32_t*>(workspace);
+    a.part_o = reinterpret_cast<float*>(workspace) + ((size_t)n_seq * nk + 3) / 4 * 4;
     a.part_ml = a.part_o + parts * Q8_D;
     a.scores = weights ? a.part_o + (parts * (Q8_D + 2) + 3) / 4 * 4 : nullptr;
     a.eps = eps;
@@ -1041,18 +1115,17 @@ extern "C" int t2h_attn_decode_q8(const float* q, uint64_t q_row, const float* k
     a.log2_theta = a.rope ? log2((double)theta) : 0.0;
     const uint64_t grid = (uint64_t)a.units * nk;
     const uint64_t segments = ((uint64_t)s_cap + DQ_SEGMENT - 1) / DQ_SEGMENT;
-    const uint64_t merge = (uint64_t)n_seq * nh + (weights ? (uint64_t)n_seq * nk * segments : 0);
-    if (grid > 0x7fffffffu || merge > 0x7fffffffu) return T2H_ERR_SHAPE;
+    const uint64_t wgrid = (uint64_t)n_seq * nk * segments;
+    if (grid > 0x7fffffffu || wgrid > 0x7fffffffu) return T2H_ERR_SHAPE;
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    if (weights) {
-        hipLaunchKernelGGL(attn_decode_q8_kernel<true>, dim3((uint32_t)grid), dim3(DQ_WAVES * 64), 0, st, a);
-        T2H_LAUNCH_CHECK();
-        hipLaunchKernelGGL(attn_decode_q8_merge_kernel<true>, dim3((uint32_t)merge), dim3(256), 0, st, a);
-    } else {
+    if (!weights) {
         hipLaunchKernelGGL(attn_decode_q8_kernel<false>, dim3((uint32_t)grid), dim3(DQ_WAVES * 64), 0, st, a);
         T2H_LAUNCH_CHECK();
-        hipLaunchKernelGGL(attn_decode_q8_merge_kernel<false>, dim3((uint32_t)merge), dim3(256), 0, st, a);
+        return T2H_OK;
     }
+    hipLaunchKernelGGL(attn_decode_q8_kernel<true>, dim3((uint32_t)grid), dim3(DQ_WAVES * 64), 0, st, a);
+    T2H_LAUNCH_CHECK();
+    hipLaunchKernelGGL(attn_decode_q8_weights_kernel, dim3((uint32_t)wgrid), dim3(256), 0, st, a);
     T2H_LAUNCH_CHECK();
     return T2H_OK;
 }

@@ -1633,21 +1633,11 @@ class KVCacheQ8:
             if tuple(t.shape) != shape or t.device != self.k.device:
                 raise ValueError(f"cache {name} must be {shape} on {self.k.device}, got {tuple(t.shape)} on {t.device}")
 
-    @property
-    def n_seq(self) -> int:
-        return self.k.shape[0]
-
-    @property
-    def s_cap(self) -> int:
-        return self.k.shape[1] * KV_Q8_BLOCK
-
-    @property
-    def nk(self) -> int:
-        return self.k.shape[2]
-
-    def _ptrs(self):
-        return _Ptr6(self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
-                     self.k_tail.data_ptr(), self.v_tail.data_ptr())
+        # what every call would ask the tensors for again
+        for name, value in (("n_seq", n_seq), ("s_cap", nb * KV_Q8_BLOCK), ("nk", nk), ("at", self.k.get_device()),
+                            ("ptrs", _Ptr6(*(t.data_ptr() for t in (self.k, self.v, self.k_scale, self.v_scale, self.k_tail,
+                                                                    self.v_tail))))):
+            object.__setattr__(self, name, value)
 
 
 def kv_cache_q8(n_seq: int, s_cap: int, nk: int, d: int, device) -> KVCacheQ8:
@@ -1667,24 +1657,26 @@ def kv_cache_q8(n_seq: int, s_cap: int, nk: int, d: int, device) -> KVCacheQ8:
                      zeros(n_seq, nk, d, KV_Q8_BLOCK, dtype=torch.bfloat16))
 
 
-def _q8_here(cache: KVCacheQ8, *tensors: tuple[str, torch.Tensor | None]) -> None:
+def _q8_here(cache: KVCacheQ8, names: str, *tensors: torch.Tensor | None) -> None:
     """Everything of a call is on the current device, on whose current stream it is launched."""
     if not isinstance(cache, KVCacheQ8):
         raise TypeError(f"cache must be a KVCacheQ8, got {type(cache).__name__}")
-    at = cache.k.get_device()
-    if at != torch.cuda.current_device():
+    at = cache.at
+    if at != torch._C._cuda_getDevice():
         raise ValueError(f"the cache is on cuda:{at}, the current device is cuda:{torch.cuda.current_device()}")
-    for name, t in tensors:
-        if t is not None and t.get_device() != at:
+    for i, t in enumerate(tensors):
+        if t is not None and not (isinstance(t, torch.Tensor) and t.get_device() == at):
+            name = names.split()[i]
+            if not isinstance(t, torch.Tensor):
+                raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
             raise ValueError(f"{name} is on {t.device}, the cache on cuda:{at}")
 
 
 def _q8_ints(t: torch.Tensor | None, name: str, n_seq: int) -> None:
-    if t is None:
+    if t is None or t.dtype is torch.int32 and t.numel() == n_seq and t.is_contiguous():
         return
     _check(t, name, torch.int32, align=4)
-    if t.numel() != n_seq:
-        raise ValueError(f"{name} must have one entry for each of {n_seq} sequences, got {tuple(t.shape)}")
+    raise ValueError(f"{name} must have one entry for each of {n_seq} sequences, got {tuple(t.shape)}")
 
 
 def _q8_heads(nh: int, nk: int) -> None:
@@ -1692,28 +1684,34 @@ def _q8_heads(nh: int, nk: int) -> None:
         raise ValueError(f"{nh} q heads over {nk} KV heads: 1 to {KV_Q8_MAX_GROUP} for each are built")
 
 
-def _q8_rows(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: KVCacheQ8, rows: int | None,
-             q_norm_weight: torch.Tensor | None, k_norm_weight: torch.Tensor | None) -> tuple[int, tuple[int, int, int]]:
+def _q8_rows(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: KVCacheQ8, rows: int,
+             q_norm_weight: torch.Tensor | None, k_norm_weight: torch.Tensor | None) -> tuple[int, int, int, int]:
     """q heads of fp32 [rows, heads * 128] column blocks, and their row strides."""
-    rows = int(q.shape[0]) if rows is None else rows
-    for t, name in ((q, "q"), (k, "k"), (v, "v")):
-        _check_strided(t, name, torch.float32)
-        if t.dim() != 2 or t.shape[0] != rows or t.shape[1] % 128:
-            raise ValueError(f"{name} must be fp32 [{rows}, heads * 128], got {tuple(t.shape)}")
-        if t.data_ptr() % 4 or (rows > 1 and t.stride(0) < t.shape[1]):
+    shape, width = q.shape, cache.nk * 128
+    q_width = shape[1] if len(shape) == 2 else 0
+    strides = []
+    for t, name, cols in ((q, "q", q_width), (k, "k", width), (v, "v", width)):
+        stride = t.stride()
+        if (t.dtype is not torch.float32 or t.shape != (rows, cols) or stride[1] != 1 or cols % 128
+                or stride[0] < cols and rows > 1):
+            _check_strided(t, name, torch.float32)
+            if t.dim() != 2 or t.shape[0] != rows or t.shape[1] % 128:
+                raise ValueError(f"{name} must be fp32 [{rows}, heads * 128], got {tuple(t.shape)}")
+            if t.shape[1] != cols:
+                raise ValueError(f"k and v must have the cache's {cache.nk} heads")
             raise ValueError(f"{name} must hold distinct rows")
-    nh = q.shape[1] // 128
-    if k.shape[1] != cache.nk * 128 or v.shape[1] != cache.nk * 128:
-        raise ValueError(f"k and v must have the cache's {cache.nk} heads")
+        strides.append(max(stride[0], cols))
+    nh = q_width // 128
     _q8_heads(nh, cache.nk)
-    if (q_norm_weight is None) != (k_norm_weight is None):
+    if q_norm_weight is None and k_norm_weight is None:
+        return nh, *strides
+    if q_norm_weight is None or k_norm_weight is None:
         raise ValueError("pass both q and k norm weights or neither")
     for t, name in ((q_norm_weight, "q_norm_weight"), (k_norm_weight, "k_norm_weight")):
-        if t is not None:
-            _check(t, name, torch.float32, align=4)
-            if t.numel() != 128:
-                raise ValueError(f"{name} must have 128 elements")
-    return nh, tuple(max(t.stride(0), t.shape[1]) for t in (q, k, v))
+        _check(t, name, torch.float32, align=4)
+        if t.numel() != 128:
+            raise ValueError(f"{name} must have 128 elements")
+    return nh, *strides
 
 
 def _q8_weights(cache: KVCacheQ8, weights: torch.Tensor | None,
@@ -1738,13 +1736,13 @@ def qk_norm_rope_cache_q8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_o
     [n_seq * n, nh, 128], k and v into the cache behind the ``lengths`` tokens that it holds.  q, k, v fp32
     [n_seq * n, heads * 128] with unit column stride.  ``counts``: new tokens of each sequence, its first rows (all n when
     None).  Token p stands at position p + rope_offsets.  ``lengths`` is not advanced."""
-    n_rows = int(q.shape[0]) if isinstance(q, torch.Tensor) and q.dim() else 0
-    _q8_here(cache, ("q", q), ("k", k), ("v", v), ("q_out", q_out), ("lengths", lengths), ("counts", counts),
-             ("rope_offsets", rope_offsets), ("q_norm_weight", q_norm_weight), ("k_norm_weight", k_norm_weight))
+    _q8_here(cache, "q k v q_out lengths counts rope_offsets q_norm_weight k_norm_weight", q, k, v, q_out, lengths, counts,
+             rope_offsets, q_norm_weight, k_norm_weight)
     n_seq = cache.n_seq
+    n_rows = q.shape[0] if q.dim() else 0
     if n_rows % n_seq:
         raise ValueError(f"{n_rows} rows do not split into {n_seq} sequences")
-    nh, (qr, kr, vr) = _q8_rows(q, k, v, cache, n_rows, q_norm_weight, k_norm_weight)
+    nh, qr, kr, vr = _q8_rows(q, k, v, cache, n_rows, q_norm_weight, k_norm_weight)
     _check(q_out, "q_out", torch.bfloat16, align=4)
     if q_out.numel() != n_rows * nh * 128:
         raise ValueError(f"q_out must hold [{n_rows}, {nh}, 128]")
@@ -1755,17 +1753,18 @@ def qk_norm_rope_cache_q8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_o
         return q_out
     call("t2h_qk_norm_rope_cache_q8", ptr(q), qr, ptr(k), kr, ptr(v), vr, ptr(q_norm_weight), ptr(k_norm_weight), eps,
          theta, ptr(lengths), ptr(counts), ptr(rope_offsets), n_rows // n_seq, n_seq, nh, cache.nk, 128, ptr(q_out),
-         cache._ptrs(), cache.s_cap, stream_handle())
+         cache.ptrs, cache.s_cap, stream_handle())
     return q_out
 
 
 def attn_decode_q8_workspace(n_seq: int, nh: int, nk: int, d: int, s_cap: int, device, *,
                              weights: bool = False) -> torch.Tensor:
-    """Workspace of :func:`attn_decode_q8` for such a cache; calls that share one must not overlap in time."""
+    """Zeroed workspace of :func:`attn_decode_q8` for such a cache; calls leave it reusable, and calls that share one must
+    not overlap in time."""
     n = int(_lib.lib().t2h_attn_decode_q8_workspace_bytes(n_seq, nh, nk, d, s_cap, int(weights)))
     if n == 0:
         raise ValueError(f"unsupported attention shape n_seq={n_seq} nh={nh} nk={nk} d={d} s_cap={s_cap}")
-    return torch.empty(n, dtype=torch.uint8, device=device)
+    return torch.zeros(n, dtype=torch.uint8, device=device)
 
 
 def attn_decode_q8(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, cache: KVCacheQ8, out: torch.Tensor,
@@ -1778,11 +1777,10 @@ def attn_decode_q8(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, ca
     behind the ``lengths`` cached tokens, then attention over them all; out bf16 [n_seq, nh, 128].  ``weights`` fp32
     [n_seq, nk, s_cap]: each cached token's softmax weight, summed over the KV head's q heads, is added (in place, or into
     ``weights_out``).  ``lengths`` is not advanced."""
-    _q8_here(cache, ("q", q), ("new_k", k_new), ("new_v", v_new), ("output", out), ("lengths", lengths),
-             ("workspace", workspace), ("rope_offsets", rope_offsets), ("q_norm_weight", q_norm_weight),
-             ("k_norm_weight", k_norm_weight), ("weights", weights), ("weights_out", weights_out))
+    _q8_here(cache, "q new_k new_v output lengths workspace rope_offsets q_norm_weight k_norm_weight weights weights_out", q,
+             k_new, v_new, out, lengths, workspace, rope_offsets, q_norm_weight, k_norm_weight, weights, weights_out)
     n_seq = cache.n_seq
-    nh, (qr, kr, vr) = _q8_rows(q, k_new, v_new, cache, n_seq, q_norm_weight, k_norm_weight)
+    nh, qr, kr, vr = _q8_rows(q, k_new, v_new, cache, n_seq, q_norm_weight, k_norm_weight)
     _check(out, "output", torch.bfloat16, align=4)
     if out.numel() != n_seq * nh * 128:
         raise ValueError(f"output must hold [{n_seq}, {nh}, 128]")
@@ -1791,7 +1789,7 @@ def attn_decode_q8(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, ca
     _check(workspace, "workspace", torch.uint8)
     weights_out = _q8_weights(cache, weights, weights_out)
     call("t2h_attn_decode_q8", ptr(q), qr, ptr(k_new), kr, ptr(v_new), vr, ptr(q_norm_weight), ptr(k_norm_weight), eps,
-         theta, ptr(lengths), ptr(rope_offsets), cache._ptrs(), cache.s_cap, ptr(weights), ptr(weights_out), ptr(out),
+         theta, ptr(lengths), ptr(rope_offsets), cache.ptrs, cache.s_cap, ptr(weights), ptr(weights_out), ptr(out),
          n_seq, nh, cache.nk, 128, ptr(workspace), workspace.numel(), stream_handle())
     return out
 
@@ -1802,8 +1800,7 @@ def flash_attn_prefill_q8(q: torch.Tensor, cache: KVCacheQ8, lengths: torch.Tens
     """Causal attention of a chunk's queries over the 8-bit cache that :func:`qk_norm_rope_cache_q8` wrote it into (the
     same ``lengths`` and ``counts``): query t of q bf16 [n_seq, n, nh, 128] sees tokens 0 .. length + t; rows past a
     count give zeros.  ``weights`` as in :func:`attn_decode_q8`, of all the chunk's queries."""
-    _q8_here(cache, ("q", q), ("lengths", lengths), ("output", out), ("counts", counts), ("weights", weights),
-             ("weights_out", weights_out))
+    _q8_here(cache, "q lengths output counts weights weights_out", q, lengths, out, counts, weights, weights_out)
     _check(q, "q", torch.bfloat16)
     if q.dim() != 4 or q.shape[0] != cache.n_seq or q.shape[3] != 128:
         raise ValueError(f"q must be bf16 [{cache.n_seq}, n, nh, 128], got {tuple(q.shape)}")
@@ -1822,7 +1819,7 @@ def flash_attn_prefill_q8(q: torch.Tensor, cache: KVCacheQ8, lengths: torch.Tens
     nbytes = int(_lib.lib().t2h_flash_attn_prefill_q8_workspace_bytes(n, n_seq, nh, cache.nk, cache.s_cap,
                                                                      int(weights is not None)))
     workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-    call("t2h_flash_attn_prefill_q8", ptr(q), cache._ptrs(), cache.s_cap, ptr(lengths), ptr(counts), ptr(weights),
+    call("t2h_flash_attn_prefill_q8", ptr(q), cache.ptrs, cache.s_cap, ptr(lengths), ptr(counts), ptr(weights),
          ptr(weights_out), ptr(out), n, n_seq, nh, cache.nk, 128, float(scale or 0.0), ptr(workspace), nbytes,
          stream_handle())
     return out
@@ -1832,7 +1829,7 @@ def kv_cache_q8_dequantize(cache: KVCacheQ8, lengths: torch.Tensor, k_out: torch
                            v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The cache's keys and values as bf16 [n_seq, s_cap, nk, 128], the layout of the other caches; zeros behind
     ``lengths``."""
-    _q8_here(cache, ("lengths", lengths), ("k_out", k_out), ("v_out", v_out))
+    _q8_here(cache, "lengths k_out v_out", lengths, k_out, v_out)
     _q8_ints(lengths, "lengths", cache.n_seq)
     shape = (cache.n_seq, cache.s_cap, cache.nk, 128)
     outs = []
@@ -1842,7 +1839,7 @@ def kv_cache_q8_dequantize(cache: KVCacheQ8, lengths: torch.Tensor, k_out: torch
         if tuple(t.shape) != shape:
             raise ValueError(f"{name} must be bf16 {shape}, got {tuple(t.shape)}")
         outs.append(t)
-    call("t2h_kv_cache_q8_dequantize", cache._ptrs(), cache.s_cap, ptr(lengths), cache.n_seq, cache.nk, 128, ptr(outs[0]),
+    call("t2h_kv_cache_q8_dequantize", cache.ptrs, cache.s_cap, ptr(lengths), cache.n_seq, cache.nk, 128, ptr(outs[0]),
          ptr(outs[1]), stream_handle())
     return outs[0], outs[1]
 
@@ -1857,8 +1854,8 @@ def kv_cache_q8_evict(cache: KVCacheQ8, lengths: torch.Tensor, weights: torch.Te
     -1) and the new lengths; ``lengths`` itself is not changed, so that every layer of a model can be evicted by it.
     A decode that goes on adds lengths - new lengths to its ``rope_offsets``."""
     dest = cache if out is None else out
-    _q8_here(cache, ("lengths", lengths), ("weights", weights), ("weights_out", weights_out))
-    _q8_here(dest)
+    _q8_here(cache, "lengths weights weights_out", lengths, weights, weights_out)
+    _q8_here(dest, "")
     n_seq, nk = cache.n_seq, cache.nk
     if dest.n_seq != n_seq or dest.nk != nk:
         raise ValueError(f"out must hold {n_seq} sequences of {nk} heads, got {dest.n_seq} of {dest.nk}")
@@ -1877,6 +1874,6 @@ def kv_cache_q8_evict(cache: KVCacheQ8, lengths: torch.Tensor, weights: torch.Te
             raise ValueError(f"{name} must be fp32 {(n_seq, nk, cap)}, got {tuple(t.shape)}")
     kept = torch.empty(n_seq, nk, KV_Q8_BLOCK * keep_blocks, dtype=torch.int32, device=cache.k.device)
     new = torch.empty_like(lengths)
-    call("t2h_kv_cache_q8_evict", cache._ptrs(), cache.s_cap, ptr(lengths), ptr(weights), keep_blocks, sink, recent, n_seq,
-         nk, 128, dest._ptrs(), dest.s_cap, ptr(weights_out), ptr(kept), ptr(new), stream_handle())
+    call("t2h_kv_cache_q8_evict", cache.ptrs, cache.s_cap, ptr(lengths), ptr(weights), keep_blocks, sink, recent, n_seq,
+         nk, 128, dest.ptrs, dest.s_cap, ptr(weights_out), ptr(kept), ptr(new), stream_handle())
     return kept, new
