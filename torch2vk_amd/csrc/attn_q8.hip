@@ -5,7 +5,6 @@
 
 #include "kv_q8.h"
 #include "kv_q8_args.h"
-#include "rope.h"
 
 namespace t2h {
 
@@ -23,16 +22,19 @@ namespace t2h {
 //   * codes become fp16 exactly (bytes beside 0x64 are 1024 + code + 128), scales multiply scores and weights in fp32;
 //   * q is split into two fp16 terms (22 bits), so that scores are as good as fp32's; weights are rounded once, to 11 bits,
 //     relative to the wave's largest value scale times 2^12 (they stay normal over scales 2^26 apart);
-//   * the unfinished block's bf16 rows go through the bf16 products, with q in three and weights in two bf16 terms.
-// The wave that holds the new token writes it, and first rounds its block if that is now whole.
+//   * the unfinished block's bf16 rows go through the bf16 products, a quarter a wave, q and weights in two bf16 terms.
+// The wave that holds the new token writes it; the four round its block if that is now whole, and then read it as codes.
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int DQ_WAVES = 4;
 constexpr int DQ_ROW = Q8_D + 4;          // fp32 row in LDS, padded
 constexpr int DQ_QROW = Q8_D + 8;         // fp16 row
+constexpr uint32_t DQ_SLOTS = 512;        // thread blocks that the chip holds at once
+constexpr uint32_t DQ_CHUNK_MAX = 64;     // blocks a unit, at most
 constexpr float DQ_P_SCALE = 4096.0f;
 
 struct DecodeQ8Args {
@@ -52,7 +54,7 @@ struct DecodeQ8Args {
     float* part_o;   // [units][nk][group][128]
     uint32_t* done;  // [n_seq][nk] units that have left their parts; zero between calls
     float* scores;   // [n_seq][nh][s_cap] log2 scores, or null
-    uint32_t n_seq, nh, group, target, units;
+    uint32_t n_seq, nh, group, units;
     float eps, scale_log2;
     double log2_theta;
     int rope;
@@ -78,10 +80,15 @@ __device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v) {
     return v;
 }
 
-// Blocks a unit: as many units as `target` thread blocks hold, in whole rounds of a thread block's waves.
-__device__ __forceinline__ int dq_chunk(const DecodeQ8Args& a, uint32_t total) {
-    const uint32_t c = (uint32_t)(((uint64_t)total * a.c.nk + a.target - 1) / a.target);
-    return c <= 2 ? (c ? (int)c : 1) : (int)((c + DQ_WAVES - 1) / DQ_WAVES * DQ_WAVES);
+// Blocks a unit, for the blocks of all sequences: 4 (one a wave) for short ones, then one thread block a CU until units have
+// 8, then two a CU, which the registers allow, until units have 64, where what a unit costs besides its blocks (3 to 4 us:
+// lengths, q, joining) no longer matters and ragged lengths want the chip refilled.  Measured (32 / 8 heads): 16000 tokens
+// 15.1 us in units of 8 against 18.3 of 4; 16 sequences of 100 to 8000 34.9 us of 16 against 43.7 of 32; 32 of 15000 to
+// 16200 184 us of 64, 193 of 32, 206 of 16.
+__host__ __device__ __forceinline__ uint32_t dq_chunk(uint64_t total, uint32_t nk) {
+    const uint64_t one = (total * nk + 255) / 256, two = (total * nk + DQ_SLOTS - 1) / DQ_SLOTS;
+    const uint64_t c = one <= 8 ? one : (two > 8 ? two : 8);
+    return c <= DQ_WAVES ? DQ_WAVES : c >= DQ_CHUNK_MAX ? DQ_CHUNK_MAX : (uint32_t)((c + DQ_WAVES - 1) / DQ_WAVES * DQ_WAVES);
 }
 
 // The sequence that unit `unit` belongs to (by_seq false), or sequence `unit` itself; false where there is none.  A
@@ -90,7 +97,7 @@ __device__ bool dq_find(const DecodeQ8Args& a, uint32_t unit, bool by_seq, Decod
     const uint32_t lane = threadIdx.x & 63;
     if (a.n_seq == 1) {
         u.blocks = dq_blocks(a, 0);
-        u.chunk = dq_chunk(a, (uint32_t)u.blocks);
+        u.chunk = (int)dq_chunk((uint64_t)u.blocks, a.c.nk);
         u.seq = u.first = 0;
         u.count = u.blocks ? (uint32_t)((u.blocks + u.chunk - 1) / u.chunk) : 1u;
         u.len = a.lengths[0];
@@ -99,7 +106,7 @@ __device__ bool dq_find(const DecodeQ8Args& a, uint32_t unit, bool by_seq, Decod
     uint32_t total = 0;
     for (uint32_t i = lane; i < a.n_seq; i += 64) total += (uint32_t)dq_blocks(a, i);
     total = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan_u32(total), 63);
-    u.chunk = dq_chunk(a, total);
+    u.chunk = (int)dq_chunk(total, a.c.nk);
     uint32_t before = 0;
     for (uint32_t base = 0; base < a.n_seq; base += 64) {
         const uint32_t i = base + lane;
@@ -138,56 +145,11 @@ __device__ __forceinline__ f16x8 codes_f16x8(uint32_t w0, uint32_t w1) {
 
 __device__ __forceinline__ bf16x8 as_bf16x8(uint4 v) { return __builtin_bit_cast(bf16x8, v); }
 
-// A block that its last token finishes, rounded by one wave from the tail's rows and that token: two passes over 32 KB,
-// once in 64 tokens.  The codes are in memory for the wave itself when this returns the values' scale.
-__device__ __forceinline__ float dq_round(const KvQ8& c, uint32_t seq, uint32_t h, uint32_t b, const uint16_t* key,
-                                          const uint16_t* value) {
-    float s = 0.0f;
-    const int lane = threadIdx.x & 63;
-    const size_t tail = c.tail_at(seq, h), at = c.block_at(seq, b, h);
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll 1
-    for (int half = 0; half < 2; ++half) {
-        const uint16_t* rows = (half == 0 ? c.kt : c.vt) + tail;
-        // 16 values of a row: the last token's are the last row of the keys, the last value of each row of the values
-        auto load = [&](int n, uint32_t (&w)[8]) {
-            const int i = (n * 64 + lane) * 16;
-            uint4 lo = load_u4(rows + i), hi = load_u4(rows + i + 8);
-            if (half == 0 && i / Q8_D == Q8_BLOCK - 1) {
-                lo = *reinterpret_cast<const uint4*>(key + i % Q8_D);
-                hi = *reinterpret_cast<const uint4*>(key + i % Q8_D + 8);
-            }
-            if (half == 1 && i % Q8_BLOCK == Q8_BLOCK - 16) hi.w = (hi.w & 0xffffu) | (uint32_t)value[i / Q8_BLOCK] << 16;
-            w[0] = lo.x, w[1] = lo.y, w[2] = lo.z, w[3] = lo.w, w[4] = hi.x, w[5] = hi.y, w[6] = hi.z, w[7] = hi.w;
-        };
-        uint32_t top = 0;
-#pragma unroll 2
-        for (int n = 0; n < 8; ++n) {
-            uint32_t w[8];
-            load(n, w);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) top = max(top, max(w[i] << 16 & 0x7fffffffu, w[i] & 0x7fff0000u));
-        }
-        top = wave_max_u32(top);
-        float inv;
-        q8_scale(top, s, inv);
-#pragma unroll 2
-        for (int n = 0; n < 8; ++n) {
-            uint32_t w[8], packed[4];
-            load(n, w);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                packed[i] = q8_pack4(__uint_as_float(w[2 * i] << 16), __uint_as_float(w[2 * i] & 0xffff0000u),
-                                     __uint_as_float(w[2 * i + 1] << 16), __uint_as_float(w[2 * i + 1] & 0xffff0000u), inv);
-            *reinterpret_cast<uint4*>((half == 0 ? c.k : c.v) + at + (n * 64 + lane) * 16) =
-                make_uint4(packed[0], packed[1], packed[2], packed[3]);
-        }
-        if (lane == 0) (half == 0 ? c.ks : c.vs)[c.scale_at(seq, b, h)] = s;
-    }
-    __threadfence_block();  // other lanes of the wave read them
-    return s;
+// A word of two bf16 values: the larger of their |x| as fp32 bits, and the codes of two words.
+__device__ __forceinline__ uint32_t bf16_abs_max(uint32_t w) { return max(w << 16 & 0x7fffffffu, w & 0x7fff0000u); }
+__device__ __forceinline__ uint32_t bf16_codes(uint32_t w0, uint32_t w1, float inv) {
+    return q8_pack4(__uint_as_float(w0 << 16), __uint_as_float(w0 & 0xffff0000u), __uint_as_float(w1 << 16),
+                    __uint_as_float(w1 & 0xffff0000u), inv);
 }
 
 // Two floats past the caches that the chip's parts do not share.
@@ -207,7 +169,7 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_decode_q8_kernel(const 
     __shared__ __align__(16) uint16_t fresh[2][Q8_D];         // the new token's key and value
     __shared__ float wml[DQ_WAVES][16][2];
     __shared__ __align__(16) float wo[DQ_WAVES][16][DQ_ROW];
-    __shared__ uint32_t arrived;
+    __shared__ uint32_t arrived, top[2][DQ_WAVES];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t h = blockIdx.x % a.c.nk;
@@ -227,8 +189,9 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_decode_q8_kernel(const 
     const int new_b = has_new ? u.len / Q8_BLOCK : -1;  // the block of the new token, in bf16 unless the token finishes it
     const int r = u.len % Q8_BLOCK;
     const int tail_b = r == Q8_BLOCK - 1 ? -1 : new_b;
-    const bool writes = new_b >= b0 && new_b < b1 && (new_b - b0) % DQ_WAVES == wave;
-    const bool has_tail = writes && tail_b >= 0;
+    const bool new_here = new_b >= b0 && new_b < b1;
+    const bool has_tail = tail_b >= b0 && tail_b < b1;
+    const bool writes = new_here && (new_b - b0) % DQ_WAVES == wave;
 
     // 1. the small operands (loads return in order: what is asked for after the codes would wait for them), then the first
     // block's codes
@@ -268,22 +231,31 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_decode_q8_kernel(const 
         if (i != new_b) smax = fmaxf(smax, a.c.vs[a.c.scale_at(u.seq, (uint32_t)i, h)]);
     const int krow = ((c >> 2) * 16 + (c & 3)) * Q8_D + g4 * 16;  // + t * 4 rows + j * 64
     const int vrow = c * Q8_BLOCK + g4 * 16;                      // + dt * 16 rows
-    uint4 kr[4][2], vr[8];
+    uint4 kr[8], vr[8];  // key tile t, dims 64 j ..: 2 t + j
     float ks = 0.0f, vs = 0.0f;
     auto load_k = [&](int b) {
         const int8_t* p = a.c.k + a.c.block_at(u.seq, (uint32_t)b, h) + krow;
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) kr[t][j] = load_nt_u4(p + t * 4 * Q8_D + j * 64);
+        for (int n = 0; n < 8; ++n) kr[n] = load_nt_u4(p + (n >> 1) * 4 * Q8_D + (n & 1) * 64);
         ks = a.c.ks[a.c.scale_at(u.seq, (uint32_t)b, h)];
     };
     auto load_v = [&](int b) {
         const int8_t* p = a.c.v + a.c.block_at(u.seq, (uint32_t)b, h) + vrow;
 #pragma unroll
-        for (int dt = 0; dt < 8; ++dt) vr[dt] = load_nt_u4(p + dt * 16 * Q8_BLOCK);
+        for (int n = 0; n < 8; ++n) vr[n] = load_nt_u4(p + n * 16 * Q8_BLOCK);
         vs = a.c.vs[a.c.scale_at(u.seq, (uint32_t)b, h)];
     };
+    // the tail's rows, a quarter a wave: token 16 (c / 4) + 4 wave + c % 4, dims 64 j + 16 g4 + 8 i; and the values of
+    // tokens 16 g4 + 4 wave .. of dim 16 n + c
+    const size_t tail = a.c.tail_at(u.seq, h);
+    uint4 tk[4];
+    uint2 tv[8];
+    if (new_here) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n) tk[n] = load_u4(a.c.kt + tail + krow + wave * 4 * Q8_D + 64 * (n >> 1) + 8 * (n & 1));
+#pragma unroll
+        for (int n = 0; n < 8; ++n) tv[n] = *reinterpret_cast<const uint2*>(a.c.vt + tail + vrow + n * 16 * Q8_BLOCK + 4 * wave);
+    }
     int b = b0 + wave;
     if (b < b1 && b != new_b) {
         load_k(b);
@@ -298,8 +270,8 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_decode_q8_kernel(const 
         const int g = wave + DQ_WAVES * i;
         if (g >= group) break;
         float y[2];
-        norm_rope_pair(x0[i], x1[i], has_w, w0, w1, a.eps, cs, sn, a.rope != 0, y[0], y[1]);
-        uint32_t e = wave_max_u32(max(abs_bits(y[0]), abs_bits(y[1]))) >> 23;
+        q8_norm_rope(x0[i], x1[i], has_w, w0, w1, a.eps, cs, sn, y[0], y[1]);
+        uint32_t e = __float_as_uint(wave_max(fmaxf(fabsf(y[0]), fabsf(y[1])))) >> 23;  // (a NaN stays one whatever e is)
         e = e < 1 ? 1 : (e > 253 ? 253 : e);
         const float down = __uint_as_float((254u - e) << 23);
 #pragma unroll
@@ -312,9 +284,8 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_decode_q8_kernel(const 
     }
     if (writes) {
         float y[2];
-        norm_rope_pair(kx0, kx1, has_w, kw0, kw1, a.eps, cs, sn, a.rope != 0, y[0], y[1]);
+        q8_norm_rope(kx0, kx1, has_w, kw0, kw1, a.eps, cs, sn, y[0], y[1]);
         const float v[2] = {vx0, vx1};
-        const size_t tail = a.c.tail_at(u.seq, h);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const uint16_t kb = (uint16_t)f32_to_bf16_bits(y[i]), vb = (uint16_t)f32_to_bf16_bits(v[i]);
@@ -323,15 +294,65 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_decode_q8_kernel(const 
             a.c.kt[tail + r * Q8_D + lane + 64 * i] = kb;
             a.c.vt[tail + (lane + 64 * i) * Q8_BLOCK + r] = vb;
         }
-        if (tail_b < 0) {
-            smax = fmaxf(smax, dq_round(a.c, u.seq, h, (uint32_t)new_b, fresh[0], fresh[1]));
+    }
+    __syncthreads();
+    if (new_here) {
+        // the new token among the tail's: its key a row, its value one of a word's two tokens (behind it: zeros)
+        if ((c >> 2) * 16 + wave * 4 + (c & 3) == r) {
+#pragma unroll
+            for (int n = 0; n < 4; ++n) tk[n] = *reinterpret_cast<const uint4*>(&fresh[0][64 * (n >> 1) + 16 * g4 + 8 * (n & 1)]);
+        }
+        const int ahead = r - 16 * g4 - 4 * wave;
+        const uint32_t old0 = ahead <= 0 ? 0u : ahead == 1 ? 0xffffu : 0xffffffffu;
+        const uint32_t old1 = ahead <= 2 ? 0u : ahead == 3 ? 0xffffu : 0xffffffffu;
+        const uint32_t new0 = ahead == 0 ? 0xffffu : ahead == 1 ? 0xffff0000u : 0u;
+        const uint32_t new1 = ahead == 2 ? 0xffffu : ahead == 3 ? 0xffff0000u : 0u;
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            const uint32_t vnew = fresh[1][16 * n + c] * 0x10001u;
+            tv[n] = make_uint2((tv[n].x & old0) | (vnew & new0), (tv[n].y & old1) | (vnew & new1));
+        }
+        if (!has_tail) {  // it finishes its block: rounded here, then read as codes
+            uint32_t kmax = 0, vmax = 0;
+#pragma unroll
+            for (int n = 0; n < 4; ++n) kmax = max(max(kmax, max(bf16_abs_max(tk[n].x), bf16_abs_max(tk[n].y))),
+                                                   max(bf16_abs_max(tk[n].z), bf16_abs_max(tk[n].w)));
+#pragma unroll
+            for (int n = 0; n < 8; ++n) vmax = max(vmax, max(bf16_abs_max(tv[n].x), bf16_abs_max(tv[n].y)));
+            kmax = wave_max_u32(kmax);
+            vmax = wave_max_u32(vmax);
+            if (lane == 0) {
+                top[0][wave] = kmax;
+                top[1][wave] = vmax;
+            }
+            __syncthreads();
+            float k_scale, v_scale, k_inv, v_inv;
+            q8_scale(max(max(top[0][0], top[0][1]), max(top[0][2], top[0][3])), k_scale, k_inv);
+            q8_scale(max(max(top[1][0], top[1][1]), max(top[1][2], top[1][3])), v_scale, v_inv);
+            const size_t at = a.c.block_at(u.seq, (uint32_t)new_b, h), scale_at = a.c.scale_at(u.seq, (uint32_t)new_b, h);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const uint4 x = tk[2 * j], y = tk[2 * j + 1];
+                *reinterpret_cast<uint4*>(a.c.k + at + krow + wave * 4 * Q8_D + 64 * j) =
+                    make_uint4(bf16_codes(x.x, x.y, k_inv), bf16_codes(x.z, x.w, k_inv), bf16_codes(y.x, y.y, k_inv),
+                               bf16_codes(y.z, y.w, k_inv));
+            }
+#pragma unroll
+            for (int n = 0; n < 8; ++n)
+                *reinterpret_cast<uint32_t*>(a.c.v + at + vrow + n * 16 * Q8_BLOCK + 4 * wave) = bf16_codes(tv[n].x, tv[n].y, v_inv);
+            if (tid == 0) {
+                a.c.ks[scale_at] = k_scale;
+                a.c.vs[scale_at] = v_scale;
+            }
+            __threadfence_block();
+            __syncthreads();
+            if (writes) smax = fmaxf(smax, v_scale);
             if (b == new_b) {
                 load_k(b);
                 load_v(b);
             }
         }
     }
-    __syncthreads();
     const float qfac = qf[c];  // lanes past the group hold what no one reads: a head is a column of the products
     smax = wave_max(smax);
     auto query = [&](int term, int j, int i) {  // dims 64 j + 16 g4 + 8 i
@@ -344,28 +365,30 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_decode_q8_kernel(const 
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt) o[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-    // scores of a block (x: dot products, to be multiplied by f) -> weights; a lane's tokens are 16 g4 + 4 t + i
-    auto soften = [&](f32x4 (&x)[4], float f, int b, int live) {
+    // scores of key tiles t0, t0 + 1, .. of a block (x: dot products, to be multiplied by f) -> weights; a lane's tokens are
+    // 16 g4 + 4 t + i
+    auto soften = [&](auto& x, int t0, float f, int b, int live) {
+        constexpr int N = sizeof(x) / sizeof(x[0]);
         float top = -INFINITY;
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < N; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 x[t][i] *= f;
-                if (live < Q8_BLOCK && 16 * g4 + 4 * t + i >= live) x[t][i] = -INFINITY;
+                if (live < Q8_BLOCK && 16 * g4 + 4 * (t0 + t) + i >= live) x[t][i] = -INFINITY;
                 top = fmaxf(top, x[t][i]);
             }
         if (WEIGHTS && c < group) {
-            float* to = a.scores + ((size_t)u.seq * a.nh + h * group + c) * a.c.nb * Q8_BLOCK + b * Q8_BLOCK + 16 * g4;
+            float* to = a.scores + ((size_t)u.seq * a.nh + h * group + c) * a.c.nb * Q8_BLOCK + b * Q8_BLOCK + 16 * g4 + 4 * t0;
 #pragma unroll
-            for (int t = 0; t < 4; ++t) *reinterpret_cast<f32x4*>(to + 4 * t) = x[t];
+            for (int t = 0; t < N; ++t) *reinterpret_cast<f32x4*>(to + 4 * t) = x[t];
         }
         top = fmaxf(m, xor_max<32>(xor_max<16>(top)));
         const float base = top == -INFINITY ? 0.0f : top;
         const float keep = __builtin_amdgcn_exp2f(m - base);
         float sum = 0.0f;
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < N; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 x[t][i] = __builtin_amdgcn_exp2f(x[t][i] - base);
@@ -386,7 +409,8 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_decode_q8_kernel(const 
             const f16x8 h0 = query(0, j, 0), l0 = query(1, j, 0), h1 = query(0, j, 1), l1 = query(1, j, 1);
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-                const f16x8 k0 = codes_f16x8(kr[t][j].x, kr[t][j].y), k1 = codes_f16x8(kr[t][j].z, kr[t][j].w);
+                const uint4 kk = kr[2 * t + j];
+                const f16x8 k0 = codes_f16x8(kk.x, kk.y), k1 = codes_f16x8(kk.z, kk.w);
                 x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, h0, x[t], 0, 0, 0);
                 x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, l0, x[t], 0, 0, 0);
                 x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, h1, x[t], 0, 0, 0);
@@ -397,7 +421,7 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_decode_q8_kernel(const 
         const int next = b + DQ_WAVES;
         const bool more = next < b1 && next != tail_b;
         if (more) load_k(next);
-        soften(x, fk, b, Q8_BLOCK);
+        soften(x, 0, fk, b, Q8_BLOCK);
         const float fv = vs * (DQ_P_SCALE / (smax > 0.0f ? smax : 1.0f));
         f16x8 p[2];
 #pragma unroll
@@ -412,70 +436,38 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_decode_q8_kernel(const 
         if (more) load_v(next);
     }
 
-    if (has_tail) {  // the unfinished block, the wave's last
-        f32x4 x[4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) x[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        const size_t tail = a.c.tail_at(u.seq, h);
-        // a scheduling fence a step: the compiler would have all rows in flight at once, which the loop's other path
-        // has no registers for
+    if (has_tail) {  // tile `wave` of the unfinished block
+        f32x4 x[1] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
-            const int j = n >> 1, i = n & 1, d = 64 * j + 16 * g4 + 8 * i;
-            __builtin_amdgcn_sched_barrier(0);
-            const f16x8 qhi = query(0, j, i), qlo = query(1, j, i);
-            bf16x8 q3[3];
+            const int j = n >> 1, i = n & 1;
+            const f16x8 hi = query(0, j, i), lo = query(1, j, i);
+            bf16x8 q2[2];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                float y = (float)qhi[e] + (float)qlo[e];
-#pragma unroll
-                for (int z = 0; z < 3; ++z) {
-                    q3[z][e] = (__bf16)y;
-                    y -= (float)q3[z][e];
-                }
+                const float y = (float)hi[e] + (float)lo[e];
+                q2[0][e] = (__bf16)y;
+                q2[1][e] = (__bf16)(y - (float)q2[0][e]);
             }
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const int token = (c >> 2) * 16 + t * 4 + (c & 3);
-                uint4 kk = load_u4(a.c.kt + tail + token * Q8_D + d);
-                if (token == r) kk = *reinterpret_cast<const uint4*>(&fresh[0][d]);
-#pragma unroll
-                for (int z = 0; z < 3; ++z)
-                    x[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(kk), q3[z], x[t], 0, 0, 0);
-            }
+            const bf16x8 kk = as_bf16x8(tk[n]);
+            x[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kk, q2[0], x[0], 0, 0, 0);
+            x[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kk, q2[1], x[0], 0, 0, 0);
         }
-        __builtin_amdgcn_sched_barrier(0);
-        soften(x, qfac, tail_b, r + 1);
+        soften(x, wave, qfac, tail_b, r + 1);
         const float f_unit = DQ_P_SCALE / (smax > 0.0f ? smax : 1.0f);
-        bf16x8 ph[2], pl[2];
+        bf16x4 ph, pl;
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float p = x[2 * s + e / 4][e % 4] * f_unit;
-                ph[s][e] = (__bf16)p;
-                pl[s][e] = (__bf16)(p - (float)ph[s][e]);
-            }
+        for (int e = 0; e < 4; ++e) {
+            const float p = x[0][e] * f_unit;
+            ph[e] = (__bf16)p;
+            pl[e] = (__bf16)(p - (float)ph[e]);
+        }
 #pragma unroll
         for (int dt = 0; dt < 8; ++dt) {
-            __builtin_amdgcn_sched_barrier(0);
-            const int d = 16 * dt + c;
-            const uint16_t* vp = a.c.vt + tail + d * Q8_BLOCK + 16 * g4;
-            const uint32_t vnew = fresh[1][d];
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                uint4 vv = load_u4(vp + 8 * s);
-                uint32_t* w = reinterpret_cast<uint32_t*>(&vv);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {  // tokens 16 g4 + 8 s + 2 e and the next: the new one, and none behind it
-                    const int first = 16 * g4 + 8 * s + 2 * e;
-                    if (first == r) w[e] = vnew;
-                    if (first + 1 == r) w[e] = (w[e] & 0xffffu) | vnew << 16;
-                    if (first > r) w[e] = 0u;
-                }
-                o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(vv), ph[s], o[dt], 0, 0, 0);
-                o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(vv), pl[s], o[dt], 0, 0, 0);
-            }
+            o[dt] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(t2h_v4i16, tv[dt]), __builtin_bit_cast(t2h_v4i16, ph),
+                                                              o[dt], 0, 0, 0);
+            o[dt] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(t2h_v4i16, tv[dt]), __builtin_bit_cast(t2h_v4i16, pl),
+                                                              o[dt], 0, 0, 0);
         }
     }
 
@@ -491,7 +483,7 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_decode_q8_kernel(const 
         }
     }
     __syncthreads();
-    const int waves = b1 - b0 < DQ_WAVES ? b1 - b0 : DQ_WAVES;
+    const int waves = !has_tail && b1 - b0 < DQ_WAVES ? b1 - b0 : DQ_WAVES;
     for (int i = tid; i < group * (Q8_D / 4); i += DQ_WAVES * 64) {
         const int g = i / (Q8_D / 4), d = i % (Q8_D / 4) * 4;
         float M = -INFINITY, L = 0.0f;
@@ -531,20 +523,30 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_decode_q8_kernel(const 
     // slices of the units, each a sum of its own in LDS
     const int pieces = group * (Q8_D / 4);
     const int slices = DQ_WAVES * 64 / pieces > 0 ? DQ_WAVES * 64 / pieces : 1;
+    constexpr int BATCH = 16;  // parts of a slice in flight
     for (int i = tid; i < pieces * slices; i += DQ_WAVES * 64) {
         const int slice = i / pieces, g = i % pieces / (Q8_D / 4), d = i % (Q8_D / 4) * 4;
         float M = -INFINITY, L = 0.0f;
         f32x4 sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-        for (uint32_t n = (uint32_t)slice; n < u.count; n += (uint32_t)slices) {
-            const size_t part = ((size_t)(u.first + n) * a.c.nk + h) * a.group + g;
-            const float2 ml = get_pair(a.part_ml + 2 * part), lo = get_pair(a.part_o + part * Q8_D + d),
-                         hi = get_pair(a.part_o + part * Q8_D + d + 2);
-            const float now = fmaxf(M, ml.x), base = now == -INFINITY ? 0.0f : now;
-            const float keep = __builtin_amdgcn_exp2f(M - base), f = __builtin_amdgcn_exp2f(ml.x - base);
-            L = fmaf(L, keep, f * ml.y);
-            sum = sum * keep + f32x4{lo.x, lo.y, hi.x, hi.y} * f;
-            M = now;
+        for (uint32_t n0 = (uint32_t)slice; n0 < u.count; n0 += (uint32_t)slices * BATCH) {
+            float2 ml[BATCH], lo[BATCH], hi[BATCH];
+#pragma unroll
+            for (int e = 0; e < BATCH; ++e) {
+                const uint32_t n = n0 + (uint32_t)(slices * e);
+                const size_t part = ((size_t)(u.first + (n < u.count ? n : n0)) * a.c.nk + h) * a.group + g;
+                ml[e] = get_pair(a.part_ml + 2 * part);
+                lo[e] = get_pair(a.part_o + part * Q8_D + d);
+                hi[e] = get_pair(a.part_o + part * Q8_D + d + 2);
+            }
+#pragma unroll
+            for (int e = 0; e < BATCH; ++e) {
+                if (n0 + (uint32_t)(slices * e) >= u.count) break;
+                const float now = fmaxf(M, ml[e].x), base = now == -INFINITY ? 0.0f : now;
+                const float keep = __builtin_amdgcn_exp2f(M - base), f = __builtin_amdgcn_exp2f(ml[e].x - base);
+                L = fmaf(L, keep, f * ml[e].y);
+                sum = sum * keep + f32x4{lo[e].x, lo[e].y, hi[e].x, hi[e].y} * f;
+                M = now;
+            }
         }
         const int at = slice * group + g;  // less than 16: 8 slices are of one head
         *reinterpret_cast<f32x4*>(&wo[0][at][d]) = sum;
@@ -621,16 +623,12 @@ __global__ __launch_bounds__(256) void attn_decode_q8_weights_kernel(const Decod
         if (t0 + j < end) a.w_out[at + j] = (t0 + j < len ? a.w_in[at + j] : 0.0f) + sum[j];
 }
 
-// Thread blocks that a call is cut into (and one more a sequence and head): two a CU for one sequence, so that a head has
-// few parts to join, and four units a (sequence, head) where there are many, so that ragged lengths even out.
-static uint32_t dq_target(uint32_t n_seq, uint32_t nk) {
-    const uint64_t heads = (uint64_t)n_seq * nk;
-    return heads <= 128 ? 512u : (heads >= 1024 ? 4096u : (uint32_t)(4 * heads));
-}
-
+// Units that sequences of any lengths can have: sum of ceil(blocks / chunk) <= total / chunk + n_seq, and total / chunk is at
+// most that of the largest total or the slots' share, as the chunk grows with the total in between.
 static uint32_t dq_units(uint32_t n_seq, uint32_t nk, uint32_t nb) {
-    const uint64_t a = (uint64_t)dq_target(n_seq, nk) / nk + n_seq, b = (uint64_t)n_seq * nb;
-    return (uint32_t)(a < b ? a : b);
+    const uint64_t most = (uint64_t)n_seq * nb, slots = DQ_SLOTS / nk, full = most / DQ_CHUNK_MAX;
+    const uint64_t units = (slots > full ? slots : full) + n_seq;
+    return (uint32_t)(units < most ? units : most);
 }
 
 // ------------------------------------------------------------------------------------------------------ chunks --
@@ -1102,7 +1100,6 @@ extern "C" int t2h_attn_decode_q8(const float* q, uint64_t q_row, const float* k
     a.n_seq = n_seq;
     a.nh = nh;
     a.group = nh / nk;
-    a.target = dq_target(n_seq, nk);
     a.units = dq_units(n_seq, nk, a.c.nb);
     const size_t parts = (size_t)a.units * nh;
     a.done = reinterpret_cast<uint32_t*>(workspace);

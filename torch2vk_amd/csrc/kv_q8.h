@@ -101,6 +101,18 @@ __device__ __forceinline__ double rope_turns(int lane, double log2_theta) {
     return exp2(-(double)lane * log2_theta * (1.0 / 64.0)) * 0.15915494309189535;
 }
 
+// One wave's head: RMSNorm (with has_w) of lane's dims lane and lane + 64, then the rotation by (cs, sn), (1, 0) for none.
+__device__ __forceinline__ void q8_norm_rope(float x0, float x1, bool has_w, float w0, float w1, float eps, float cs, float sn,
+                                             float& r0, float& r1) {
+    if (has_w) {
+        const float inv = __builtin_amdgcn_rsqf(wave_sum(x0 * x0 + x1 * x1) * (1.0f / Q8_D) + eps);
+        x0 *= inv * w0;
+        x1 *= inv * w1;
+    }
+    r0 = x0 * cs - x1 * sn;
+    r1 = x1 * cs + x0 * sn;
+}
+
 __device__ __forceinline__ void rope_at(double turns, int pos, float& cs, float& sn) {
     const double t = (double)pos * turns;
     sincospif(2.0f * (float)(t - floor(t)), &sn, &cs);

@@ -3,7 +3,6 @@
 
 #include "kv_q8.h"
 #include "kv_q8_args.h"
-#include "rope.h"
 
 namespace t2h {
 
@@ -32,7 +31,6 @@ struct Q8WriteArgs {
     uint32_t kv_blocks;  // cache blocks that n tokens can touch
     uint32_t kv_grid;    // kv_blocks * nk * n_seq
     uint16_t* q_out;
-    float* q_f32;  // or q in fp32
     KvQ8 c;
 };
 
@@ -50,7 +48,6 @@ __device__ __forceinline__ void q8_write_q(const Q8WriteArgs& a, uint64_t unit) 
     const int len = a.lengths[seq];
     const int count = a.counts ? a.counts[seq] : (int)a.n;
     if (len < 0 || (int)t >= count) {  // padding
-        if (a.q_f32) return;
         for (uint32_t j = 0; j < heads; ++j) reinterpret_cast<uint32_t*>(out + j * Q8_D)[lane] = 0u;
         return;
     }
@@ -70,12 +67,7 @@ __device__ __forceinline__ void q8_write_q(const Q8WriteArgs& a, uint64_t unit) 
     for (int j = 0; j < Q8W_HEADS; ++j) {
         if (j >= (int)heads) break;
         float r0, r1;
-        norm_rope_pair(x0[j], x1[j], has_w, w0, w1, a.eps, cs, sn, a.rope != 0, r0, r1);
-        if (a.q_f32) {
-            a.q_f32[(row * a.nh + h0 + j) * Q8_D + lane] = r0;
-            a.q_f32[(row * a.nh + h0 + j) * Q8_D + lane + 64] = r1;
-            continue;
-        }
+        q8_norm_rope(x0[j], x1[j], has_w, w0, w1, a.eps, cs, sn, r0, r1);
         out[j * Q8_D + lane] = (uint16_t)f32_to_bf16_bits(r0);
         out[j * Q8_D + lane + 64] = (uint16_t)f32_to_bf16_bits(r1);
     }
@@ -117,7 +109,7 @@ __device__ __forceinline__ void q8_write_block(const Q8WriteArgs& a, uint32_t se
         if (p >= s.len && p < s.end) {
             float cs = 1.0f, sn = 0.0f, r0, r1;
             if (a.rope) rope_at(turns, p + off, cs, sn);
-            norm_rope_pair(k0[i], k1[i], has_w, w0, w1, a.eps, cs, sn, a.rope != 0, r0, r1);
+            q8_norm_rope(k0[i], k1[i], has_w, w0, w1, a.eps, cs, sn, r0, r1);
             k0[i] = bf16_bits_to_f32(f32_to_bf16_bits(r0));
             k1[i] = bf16_bits_to_f32(f32_to_bf16_bits(r1));
             v0[i] = bf16_bits_to_f32(f32_to_bf16_bits(v0[i]));
@@ -469,10 +461,15 @@ __global__ __launch_bounds__(256) void q8_evict_move_kernel(const Q8EvictArgs a)
     }
 }
 
-int q8_write_launch(const float* q, uint64_t q_row, const float* k, uint64_t k_row, const float* v, uint64_t v_row,
-                    const float* q_norm_w, const float* k_norm_w, float eps, float theta, const int32_t* lengths,
-                    const int32_t* counts, const int32_t* rope_offsets, uint32_t n, uint32_t n_seq, uint32_t nh,
-                    uint32_t nk, uint32_t d, void* q_out, bool q_f32, void* const* cache, uint32_t s_cap, void* stream) {
+}  // namespace t2h
+
+using namespace t2h;
+
+extern "C" int t2h_qk_norm_rope_cache_q8(const float* q, uint64_t q_row, const float* k, uint64_t k_row, const float* v,
+                                         uint64_t v_row, const float* q_norm_w, const float* k_norm_w, float eps,
+                                         float theta, const int32_t* lengths, const int32_t* counts,
+                                         const int32_t* rope_offsets, uint32_t n, uint32_t n_seq, uint32_t nh, uint32_t nk,
+                                         uint32_t d, void* q_out, void* const* cache, uint32_t s_cap, void* stream) {
     Q8WriteArgs a;
     if (!q || !k || !v || !lengths || !q_out) return T2H_ERR_NULL;
     if ((q_norm_w == nullptr) != (k_norm_w == nullptr)) return T2H_ERR_NULL;
@@ -504,24 +501,10 @@ int q8_write_launch(const float* q, uint64_t q_row, const float* k, uint64_t k_r
     a.kv_blocks = (uint32_t)kv_blocks;
     a.kv_grid = (uint32_t)kv_grid;
     a.q_out = reinterpret_cast<uint16_t*>(q_out);
-    a.q_f32 = q_f32 ? reinterpret_cast<float*>(q_out) : nullptr;
     hipLaunchKernelGGL(q8_write_kernel, dim3((uint32_t)(kv_grid + (units + 3) / 4)), dim3(256), 0,
                        reinterpret_cast<hipStream_t>(stream), a);
     T2H_LAUNCH_CHECK();
     return T2H_OK;
-}
-
-}  // namespace t2h
-
-using namespace t2h;
-
-extern "C" int t2h_qk_norm_rope_cache_q8(const float* q, uint64_t q_row, const float* k, uint64_t k_row, const float* v,
-                                         uint64_t v_row, const float* q_norm_w, const float* k_norm_w, float eps,
-                                         float theta, const int32_t* lengths, const int32_t* counts,
-                                         const int32_t* rope_offsets, uint32_t n, uint32_t n_seq, uint32_t nh, uint32_t nk,
-                                         uint32_t d, void* q_out, void* const* cache, uint32_t s_cap, void* stream) {
-    return q8_write_launch(q, q_row, k, k_row, v, v_row, q_norm_w, k_norm_w, eps, theta, lengths, counts, rope_offsets, n,
-                           n_seq, nh, nk, d, q_out, false, cache, s_cap, stream);
 }
 
 extern "C" int t2h_kv_cache_q8_dequantize(void* const* cache, uint32_t s_cap, const int32_t* lengths, uint32_t n_seq,

@@ -30,9 +30,4 @@ static inline int q8_cache(void* const* cache, uint32_t s_cap, uint32_t n_seq, u
     return T2H_OK;
 }
 
-int q8_write_launch(const float* q, uint64_t q_row, const float* k, uint64_t k_row, const float* v, uint64_t v_row,
-                    const float* q_norm_w, const float* k_norm_w, float eps, float theta, const int32_t* lengths,
-                    const int32_t* counts, const int32_t* rope_offsets, uint32_t n, uint32_t n_seq, uint32_t nh,
-                    uint32_t nk, uint32_t d, void* q_out, bool q_f32, void* const* cache, uint32_t s_cap, void* stream);
-
 }  // namespace t2h
