@@ -630,7 +630,7 @@ int t2h_flash_attn_prefill_q8(const void* q, void* const* cache, uint32_t s_cap,
                               const int32_t* counts, const float* weights, float* weights_out, void* out, uint32_t n,
                               uint32_t n_seq, uint32_t nh, uint32_t nk, uint32_t d, float scale, void* workspace,
                               size_t workspace_bytes, void* stream);
-/* The cache as bf16 rows [n_seq, s_cap, nk, 128], the layout of the other caches, zeros behind each length. */
+/* The cache as bf16 rows [n_seq, s_cap, nk, 128] (16-byte aligned), the layout of the other caches, zeros behind each length. */
 int t2h_kv_cache_q8_dequantize(void* const* cache, uint32_t s_cap, const int32_t* lengths, uint32_t n_seq, uint32_t nk,
                                uint32_t d, void* k_out, void* v_out, void* stream);
 /* Eviction by accumulated weight (weights fp32 [n_seq, nk, s_cap]): of a sequence's F whole blocks of tokens each KV head

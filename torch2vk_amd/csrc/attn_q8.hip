@@ -145,8 +145,7 @@ __device__ __forceinline__ f16x8 codes_f16x8(uint32_t w0, uint32_t w1) {
 
 __device__ __forceinline__ bf16x8 as_bf16x8(uint4 v) { return __builtin_bit_cast(bf16x8, v); }
 
-// A word of two bf16 values: the larger of their |x| as fp32 bits, and the codes of two words.
-__device__ __forceinline__ uint32_t bf16_abs_max(uint32_t w) { return max(w << 16 & 0x7fffffffu, w & 0x7fff0000u); }
+// The codes of four bf16 values.
 __device__ __forceinline__ uint32_t bf16_codes(uint32_t w0, uint32_t w1, float inv) {
     return q8_pack4(__uint_as_float(w0 << 16), __uint_as_float(w0 & 0xffff0000u), __uint_as_float(w1 << 16),
                     __uint_as_float(w1 & 0xffff0000u), inv);

@@ -62,6 +62,9 @@ __device__ __forceinline__ Q8Span q8_span(const int32_t* lengths, const int32_t*
 // Bits of |x|, which order as the values do and put infinities and NaN on top.
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
+// The larger |x| of two bf16 values, as fp32 bits.
+__device__ __forceinline__ uint32_t bf16_abs_max(uint32_t w) { return max(w << 16 & 0x7fffffffu, w & 0x7fff0000u); }
+
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) {

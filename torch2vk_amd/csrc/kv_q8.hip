@@ -74,65 +74,60 @@ __device__ __forceinline__ void q8_write_q(const Q8WriteArgs& a, uint64_t unit) 
 }
 
 // One cache block of one head: tokens 64 b + 16 wave + i in wave `wave`, row i; a lane holds key dims lane and lane + 64
-// and value dims 2 lane and 2 lane + 1.
+// and value dims 2 lane and 2 lane + 1, as bf16 pairs.
 __device__ __forceinline__ void q8_write_block(const Q8WriteArgs& a, uint32_t seq, uint32_t h, Q8Span s, int b,
                                                uint32_t* kbytes, uint32_t* red) {
     constexpr int ROWS = Q8_BLOCK / 4;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int p0 = b * Q8_BLOCK + wave * ROWS;
     const bool whole = (b + 1) * Q8_BLOCK <= s.end;
     const bool has_w = a.k_norm_w != nullptr;
     const float w0 = has_w ? a.k_norm_w[lane] : 1.0f, w1 = has_w ? a.k_norm_w[lane + 64] : 1.0f;
     const size_t tail = a.c.tail_at(seq, h);
-    const int base = a.lengths[seq];  // token p is row p - base of the chunk
     const int off = a.offsets ? a.offsets[seq] : 0;
+    const size_t row0 = (size_t)seq * a.n + (size_t)((int64_t)p0 - a.lengths[seq]);  // of token p0, if that is new
+    const float* kx = a.k + row0 * a.k_row + (size_t)h * Q8_D + lane;
+    const float* vx = a.v + row0 * a.v_row + (size_t)h * Q8_D + 2 * lane;
     float k0[ROWS], k1[ROWS], v0[ROWS], v1[ROWS];
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
-        const int p = p0 + i;
         k0[i] = k1[i] = v0[i] = v1[i] = 0.0f;
-        if (p >= s.len && p < s.end) {
-            const size_t row = (size_t)seq * a.n + (size_t)(p - base);
-            const float* kx = a.k + row * a.k_row + (size_t)h * Q8_D;
-            const float* vx = a.v + row * a.v_row + (size_t)h * Q8_D;
-            k0[i] = kx[lane];
-            k1[i] = kx[lane + 64];
-            v0[i] = vx[2 * lane];
-            v1[i] = vx[2 * lane + 1];
+        if (p0 + i >= s.len && p0 + i < s.end) {
+            k0[i] = kx[i * a.k_row];
+            k1[i] = kx[i * a.k_row + 64];
+            v0[i] = vx[i * a.v_row];
+            v1[i] = vx[i * a.v_row + 1];
         }
     }
     const double turns = a.rope ? rope_turns(lane, a.log2_theta) : 0.0;
-    uint32_t kmax = 0, vmax = 0;
+    uint32_t kk[ROWS], vv[ROWS], kmax = 0, vmax = 0;
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
-        const int p = p0 + i;
+        __builtin_amdgcn_sched_barrier(0);  // a row at a time: 16 angles at once would take every register
+        const int p = p0 + i, r = wave * ROWS + i;
+        kk[i] = vv[i] = 0;
         if (p >= s.len && p < s.end) {
             float cs = 1.0f, sn = 0.0f, r0, r1;
             if (a.rope) rope_at(turns, p + off, cs, sn);
             q8_norm_rope(k0[i], k1[i], has_w, w0, w1, a.eps, cs, sn, r0, r1);
-            k0[i] = bf16_bits_to_f32(f32_to_bf16_bits(r0));
-            k1[i] = bf16_bits_to_f32(f32_to_bf16_bits(r1));
-            v0[i] = bf16_bits_to_f32(f32_to_bf16_bits(v0[i]));
-            v1[i] = bf16_bits_to_f32(f32_to_bf16_bits(v1[i]));
+            kk[i] = pack_bf16x2(r0, r1);
+            vv[i] = pack_bf16x2(v0[i], v1[i]);
         } else if (whole) {  // a token of the tail that this chunk completes
-            const int r = wave * ROWS + i;
-            k0[i] = bf16_bits_to_f32(a.c.kt[tail + r * Q8_D + lane]);
-            k1[i] = bf16_bits_to_f32(a.c.kt[tail + r * Q8_D + lane + 64]);
-            v0[i] = bf16_bits_to_f32(a.c.vt[tail + (2 * lane) * Q8_BLOCK + r]);
-            v1[i] = bf16_bits_to_f32(a.c.vt[tail + (2 * lane + 1) * Q8_BLOCK + r]);
+            kk[i] = (uint32_t)a.c.kt[tail + r * Q8_D + lane] | (uint32_t)a.c.kt[tail + r * Q8_D + lane + 64] << 16;
+            vv[i] = (uint32_t)a.c.vt[tail + (2 * lane) * Q8_BLOCK + r] | (uint32_t)a.c.vt[tail + (2 * lane + 1) * Q8_BLOCK + r] << 16;
         }
-        kmax = max(kmax, max(abs_bits(k0[i]), abs_bits(k1[i])));
-        vmax = max(vmax, max(abs_bits(v0[i]), abs_bits(v1[i])));
+        kmax = max(kmax, bf16_abs_max(kk[i]));
+        vmax = max(vmax, bf16_abs_max(vv[i]));
     }
     if (!whole) {
 #pragma unroll
         for (int i = 0; i < ROWS; ++i) {
             const int p = p0 + i, r = wave * ROWS + i;
             if (p < s.len || p >= s.end) continue;
-            a.c.kt[tail + r * Q8_D + lane] = (uint16_t)f32_to_bf16_bits(k0[i]);
-            a.c.kt[tail + r * Q8_D + lane + 64] = (uint16_t)f32_to_bf16_bits(k1[i]);
-            a.c.vt[tail + (2 * lane) * Q8_BLOCK + r] = (uint16_t)f32_to_bf16_bits(v0[i]);
-            a.c.vt[tail + (2 * lane + 1) * Q8_BLOCK + r] = (uint16_t)f32_to_bf16_bits(v1[i]);
+            a.c.kt[tail + r * Q8_D + lane] = (uint16_t)kk[i];
+            a.c.kt[tail + r * Q8_D + lane + 64] = (uint16_t)(kk[i] >> 16);
+            a.c.vt[tail + (2 * lane) * Q8_BLOCK + r] = (uint16_t)vv[i];
+            a.c.vt[tail + (2 * lane + 1) * Q8_BLOCK + r] = (uint16_t)(vv[i] >> 16);
         }
         return;
     }
@@ -147,25 +142,24 @@ __device__ __forceinline__ void q8_write_block(const Q8WriteArgs& a, uint32_t se
     q8_scale(max(max(red[0], red[1]), max(red[2], red[3])), ks, kinv);
     q8_scale(max(max(red[4], red[5]), max(red[6], red[7])), vs, vinv);
     // keys: bytes through LDS, so that they leave as 16-byte stores
-    uint8_t* kb = reinterpret_cast<uint8_t*>(kbytes);
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-        kb[(wave * ROWS + i) * Q8_D + lane] = (uint8_t)q8_code(k0[i], kinv);
-        kb[(wave * ROWS + i) * Q8_D + lane + 64] = (uint8_t)q8_code(k1[i], kinv);
-    }
+    uint8_t* kb = reinterpret_cast<uint8_t*>(kbytes) + wave * ROWS * Q8_D + lane;
     const size_t at = a.c.block_at(seq, (uint32_t)b, h);
-    uint4 lo, hi;
-    lo.x = q8_pack4(v0[0], v0[1], v0[2], v0[3], vinv);
-    lo.y = q8_pack4(v0[4], v0[5], v0[6], v0[7], vinv);
-    lo.z = q8_pack4(v0[8], v0[9], v0[10], v0[11], vinv);
-    lo.w = q8_pack4(v0[12], v0[13], v0[14], v0[15], vinv);
-    hi.x = q8_pack4(v1[0], v1[1], v1[2], v1[3], vinv);
-    hi.y = q8_pack4(v1[4], v1[5], v1[6], v1[7], vinv);
-    hi.z = q8_pack4(v1[8], v1[9], v1[10], v1[11], vinv);
-    hi.w = q8_pack4(v1[12], v1[13], v1[14], v1[15], vinv);
+    uint32_t lo[4], hi[4];
+#pragma unroll
+    for (int i = 0; i < ROWS; i += 4) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            kb[(i + e) * Q8_D] = (uint8_t)q8_code(__uint_as_float(kk[i + e] << 16), kinv);
+            kb[(i + e) * Q8_D + 64] = (uint8_t)q8_code(__uint_as_float(kk[i + e] & 0xffff0000u), kinv);
+        }
+        lo[i / 4] = q8_pack4(__uint_as_float(vv[i] << 16), __uint_as_float(vv[i + 1] << 16), __uint_as_float(vv[i + 2] << 16),
+                             __uint_as_float(vv[i + 3] << 16), vinv);
+        hi[i / 4] = q8_pack4(__uint_as_float(vv[i] & 0xffff0000u), __uint_as_float(vv[i + 1] & 0xffff0000u),
+                             __uint_as_float(vv[i + 2] & 0xffff0000u), __uint_as_float(vv[i + 3] & 0xffff0000u), vinv);
+    }
     int8_t* vb = a.c.v + at + (size_t)(2 * lane) * Q8_BLOCK + wave * ROWS;
-    *reinterpret_cast<uint4*>(vb) = lo;
-    *reinterpret_cast<uint4*>(vb + Q8_BLOCK) = hi;
+    *reinterpret_cast<uint4*>(vb) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    *reinterpret_cast<uint4*>(vb + Q8_BLOCK) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
     __syncthreads();
     uint4* kout = reinterpret_cast<uint4*>(a.c.k + at);
 #pragma unroll
@@ -214,6 +208,12 @@ struct Q8ReadArgs {
     uint16_t* v_out;
 };
 
+// Eight codes times a scale as bf16.
+__device__ __forceinline__ uint4 q8_rows(uint32_t w0, uint32_t w1, float s) {
+    return make_uint4(pack_bf16x2(q8_value(w0, 0) * s, q8_value(w0, 1) * s), pack_bf16x2(q8_value(w0, 2) * s, q8_value(w0, 3) * s),
+                      pack_bf16x2(q8_value(w1, 0) * s, q8_value(w1, 1) * s), pack_bf16x2(q8_value(w1, 2) * s, q8_value(w1, 3) * s));
+}
+
 __global__ __launch_bounds__(256) void q8_read_kernel(const Q8ReadArgs a) {
     __shared__ uint32_t vb[Q8_D][Q8_BLOCK / 4 + 1];
     const uint32_t h = blockIdx.x % a.c.nk;
@@ -222,32 +222,53 @@ __global__ __launch_bounds__(256) void q8_read_kernel(const Q8ReadArgs a) {
     const int cap = (int)(a.c.nb * Q8_BLOCK);
     const int given = a.lengths[seq];
     const int len = given < 0 ? 0 : (given < cap ? given : cap);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int tid = threadIdx.x;
     const int p0 = (int)b * Q8_BLOCK;
     const bool whole = p0 + Q8_BLOCK <= len;
     const size_t at = a.c.block_at(seq, b, h), tail = a.c.tail_at(seq, h);
-    float ks = 0.0f, vs = 0.0f;
+    const size_t out = (((size_t)seq * cap + p0) * a.c.nk + h) * Q8_D, step = (size_t)a.c.nk * Q8_D;  // token p0; a token
     if (whole) {
-        ks = a.c.ks[a.c.scale_at(seq, b, h)];
-        vs = a.c.vs[a.c.scale_at(seq, b, h)];
-        const uint32_t* v = reinterpret_cast<const uint32_t*>(a.c.v + at);
-        for (int i = threadIdx.x; i < Q8_BYTES / 4; i += 256) vb[i / 16][i % 16] = v[i];
+        // keys: 16 codes of a row a thread, twice
+        uint4 kc[2], vc[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            kc[i] = load_u4(a.c.k + at + (tid + 256 * i) * 16);
+            vc[i] = load_u4(a.c.v + at + (tid + 256 * i) * 16);
+        }
+        const float ks = a.c.ks[a.c.scale_at(seq, b, h)], vs = a.c.vs[a.c.scale_at(seq, b, h)];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int n = tid + 256 * i;
+            uint32_t* row = &vb[n >> 2][4 * (n & 3)];
+            row[0] = vc[i].x, row[1] = vc[i].y, row[2] = vc[i].z, row[3] = vc[i].w;
+            uint4* to = reinterpret_cast<uint4*>(a.k_out + out + (n >> 3) * step + 16 * (n & 7));
+            to[0] = q8_rows(kc[i].x, kc[i].y, ks);
+            to[1] = q8_rows(kc[i].z, kc[i].w, ks);
+        }
+        __syncthreads();
+        // values: 4 tokens of 8 dims a thread, transposed in registers
+        const int d = (tid & 15) * 8, quad = tid >> 4;
+        uint32_t w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = vb[d + j][quad];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            uint32_t o[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] = pack_bf16x2(q8_value(w[2 * j], t) * vs, q8_value(w[2 * j + 1], t) * vs);
+            *reinterpret_cast<uint4*>(a.v_out + out + (4 * quad + t) * step + d) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+        return;
     }
-    __syncthreads();
+    const int lane = tid & 63, wave = tid >> 6;
     for (int i = wave; i < Q8_BLOCK; i += 4) {
-        const int p = p0 + i;
         uint32_t kk = 0, vv = 0;  // dims 2 lane, 2 lane + 1
-        if (whole) {
-            const uint32_t two = reinterpret_cast<const uint16_t*>(a.c.k + at + i * Q8_D)[lane];
-            kk = pack_bf16x2(q8_value(two, 0) * ks, q8_value(two, 1) * ks);
-            vv = pack_bf16x2(q8_value(vb[2 * lane][i / 4], i % 4) * vs, q8_value(vb[2 * lane + 1][i / 4], i % 4) * vs);
-        } else if (p < len) {
+        if (p0 + i < len) {
             kk = reinterpret_cast<const uint32_t*>(a.c.kt + tail + i * Q8_D)[lane];
             vv = (uint32_t)a.c.vt[tail + (2 * lane) * Q8_BLOCK + i] | (uint32_t)a.c.vt[tail + (2 * lane + 1) * Q8_BLOCK + i] << 16;
         }
-        const size_t row = (((size_t)seq * cap + p) * a.c.nk + h) * Q8_D;
-        reinterpret_cast<uint32_t*>(a.k_out + row)[lane] = kk;
-        reinterpret_cast<uint32_t*>(a.v_out + row)[lane] = vv;
+        reinterpret_cast<uint32_t*>(a.k_out + out + i * step)[lane] = kk;
+        reinterpret_cast<uint32_t*>(a.v_out + out + i * step)[lane] = vv;
     }
 }
 
@@ -512,7 +533,7 @@ extern "C" int t2h_kv_cache_q8_dequantize(void* const* cache, uint32_t s_cap, co
     Q8ReadArgs a;
     if (!lengths || !k_out || !v_out) return T2H_ERR_NULL;
     if (const int e = q8_cache(cache, s_cap, n_seq, nk, nk, d, a.c)) return e;
-    if ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 3) return T2H_ERR_ALIGN;
+    if ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15) return T2H_ERR_ALIGN;
     a.lengths = lengths;
     a.k_out = reinterpret_cast<uint16_t*>(k_out);
     a.v_out = reinterpret_cast<uint16_t*>(v_out);
