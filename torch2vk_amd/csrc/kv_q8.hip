@@ -306,6 +306,7 @@ __device__ __forceinline__ uint32_t evict_key(const float* w, int t, int full, c
 
 constexpr int EV_THREADS = 1024;
 constexpr int EV_WAVES = EV_THREADS / 64;
+constexpr int EV_BATCH = 16;  // keys a lane holds
 
 __global__ __launch_bounds__(EV_THREADS) void q8_evict_select_kernel(const Q8EvictArgs a) {
     __shared__ uint32_t hist[2048];
@@ -323,16 +324,33 @@ __global__ __launch_bounds__(EV_THREADS) void q8_evict_select_kernel(const Q8Evi
     if (stay == full) return;
     const float* w = a.w_in + (size_t)blockIdx.x * a.c.nb * Q8_BLOCK;
 
-    uint32_t prefix = 0, need = (uint32_t)stay;  // of the tokens whose key begins with prefix, `need` stay
+    // each wave takes a run of tokens, EV_BATCH rows of 64 at a time in registers; up to 16384 tokens are loaded once
+    const int per = ((full + EV_WAVES - 1) / EV_WAVES + 63) / 64 * 64;
+    const int t0 = wave * per + lane, t1 = wave * per + per < full ? wave * per + per : full;
+    const bool once = per <= EV_BATCH * 64;
+    uint32_t key[EV_BATCH];
+    auto load = [&](int base) {
 #pragma unroll
+        for (int e = 0; e < EV_BATCH; ++e) {
+            const int t = t0 + base + 64 * e;
+            key[e] = t < t1 ? evict_key(w, t, full, a) : 0u;
+        }
+    };
+    load(0);
+    uint32_t prefix = 0, need = (uint32_t)stay;  // of the tokens whose key begins with prefix, `need` stay
+#pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
-        const uint32_t mask = pass == 0 ? 0u : ~0u << (shift + bits);
+        const uint32_t mask = pass == 0 ? 0u : ~0u << (shift + bits), digits = (1u << bits) - 1u;
         for (int i = tid; i < 2048; i += EV_THREADS) hist[i] = 0;
         __syncthreads();
-        for (int t = tid; t < full; t += EV_THREADS) {
-            const uint32_t key = evict_key(w, t, full, a);
-            if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & ((1u << bits) - 1u)], 1u);
+        for (int base = 0; base < per; base += EV_BATCH * 64) {
+            if (!once) load(base);
+#pragma unroll
+            for (int e = 0; e < EV_BATCH; ++e) {
+                if (base + 64 * e >= per) break;
+                if (t0 + base + 64 * e < t1 && (key[e] & mask) == prefix) atomicAdd(&hist[(key[e] >> shift) & digits], 1u);
+            }
         }
         __syncthreads();
         // bins from the top: thread i holds bins 2047 - 2 i and 2046 - 2 i
@@ -346,7 +364,8 @@ __global__ __launch_bounds__(EV_THREADS) void q8_evict_select_kernel(const Q8Evi
         if (lane == 63) wsum[wave][0] = run;
         __syncthreads();
         uint32_t before = run - c0 - c1;
-        for (int i = 0; i < wave; ++i) before += wsum[i][0];
+#pragma unroll
+        for (int i = 0; i < EV_WAVES; ++i) before += i < wave ? wsum[i][0] : 0u;
         if (before < need && need <= before + c0) {
             found[0] = 2047u - 2u * (uint32_t)tid;
             found[1] = need - before;
@@ -358,35 +377,44 @@ __global__ __launch_bounds__(EV_THREADS) void q8_evict_select_kernel(const Q8Evi
         prefix |= found[0] << shift;
         need = found[1];
     }
-    // prefix is the smallest key that stays, and `need` of the tokens that have it; each wave takes a run of tokens
-    const int per = ((full + EV_WAVES - 1) / EV_WAVES + 63) / 64 * 64;
-    const int t0 = wave * per, t1 = t0 + per < full ? t0 + per : full;
+    // prefix is the smallest key that stays, and `need` of the tokens that have it
     uint32_t above = 0, equal = 0;
-    for (int t = t0; t < t1; t += 64) {
-        const uint32_t key = t + lane < t1 ? evict_key(w, t + lane, full, a) : 0u;
-        above += __popcll(__ballot(t + lane < t1 && key > prefix));
-        equal += __popcll(__ballot(t + lane < t1 && key == prefix));
+    for (int base = 0; base < per; base += EV_BATCH * 64) {
+        if (!once) load(base);
+#pragma unroll
+        for (int e = 0; e < EV_BATCH; ++e) {
+            if (base + 64 * e >= per) break;
+            const bool in = t0 + base + 64 * e < t1;
+            above += __popcll(__ballot(in && key[e] > prefix));
+            equal += __popcll(__ballot(in && key[e] == prefix));
+        }
     }
+    __syncthreads();
     if (lane == 0) {
         wsum[wave][0] = above;
         wsum[wave][1] = equal;
     }
     __syncthreads();
     above = equal = 0;
-    for (int i = 0; i < wave; ++i) {
-        above += wsum[i][0];
-        equal += wsum[i][1];
+#pragma unroll
+    for (int i = 0; i < EV_WAVES; ++i) {
+        above += i < wave ? wsum[i][0] : 0u;
+        equal += i < wave ? wsum[i][1] : 0u;
     }
     const uint64_t below = (1ull << lane) - 1;
-    for (int t = t0; t < t1; t += 64) {
-        const bool in = t + lane < t1;
-        const uint32_t key = in ? evict_key(w, t + lane, full, a) : 0u;
-        const uint64_t ma = __ballot(in && key > prefix), me = __ballot(in && key == prefix);
-        const uint32_t a0 = above + __popcll(ma & below), e0 = equal + __popcll(me & below);
-        const bool stays = in && (key > prefix || (key == prefix && e0 < need));
-        if (stays) kept[a0 + (e0 < need ? e0 : need)] = t + lane;
-        above += __popcll(ma);
-        equal += __popcll(me);
+    for (int base = 0; base < per; base += EV_BATCH * 64) {
+        if (!once) load(base);
+#pragma unroll
+        for (int e = 0; e < EV_BATCH; ++e) {
+            if (base + 64 * e >= per) break;
+            const int t = t0 + base + 64 * e;
+            const bool in = t < t1;
+            const uint64_t ma = __ballot(in && key[e] > prefix), me = __ballot(in && key[e] == prefix);
+            const uint32_t a0 = above + __popcll(ma & below), e0 = equal + __popcll(me & below);
+            if (in && (key[e] > prefix || (key[e] == prefix && e0 < need))) kept[a0 + (e0 < need ? e0 : need)] = t;
+            above += __popcll(ma);
+            equal += __popcll(me);
+        }
     }
 }
 
