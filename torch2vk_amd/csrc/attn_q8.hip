@@ -641,14 +641,14 @@ static uint32_t dq_units(uint32_t n_seq, uint32_t nk, uint32_t nb) {
 //     exchange a step for the row's maximum, none between the products (the key rows are taken in the order that makes a
 //     lane's scores the tokens of its operand of the second one);
 //   * scales go into the exponent: p of a block is exp2(s * ks + log2(vs / largest vs so far) - max); the accumulators follow a
-//     maximum only when it has grown by more than 2^3.
+//     maximum only when it has grown by more than 2^2, and a scale when it has more than doubled.
 // Where there are few rows the keys are split over thread blocks, and a second kernel joins the parts.
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int CQ_WAVES = 4;
 constexpr int CQ_ROWS = 32 * CQ_WAVES;  // rows a thread block
-constexpr float CQ_SLACK = 3.0f;        // log2 that a row's weights may pass 1 by: 2^12 * 2^3 is in fp16's range
+constexpr float CQ_SLACK = 2.0f;        // log2 that a row's weights may pass 1 by: 2^12 * 2^2 * 2 is in fp16's range
 
 struct ChunkQ8Args {
     KvQ8 c;
@@ -749,7 +749,7 @@ __global__ __launch_bounds__(CQ_WAVES * 64, 2) void attn_chunk_q8_kernel(const C
 #pragma unroll
     for (int i = 0; i < 8; ++i) q[i] = load_u4(qp + 16 * i);
     float m = -INFINITY, l = 0.0f;
-    float smax = 0.0f;  // the largest value scale so far: the accumulators are in units of smax / 2^12
+    float smax = 0.0f;  // the largest value scale so far, or half of it: the accumulators are in units of smax / 2^12
     f32x16 o[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -769,8 +769,8 @@ __global__ __launch_bounds__(CQ_WAVES * 64, 2) void attn_chunk_q8_kernel(const C
         }
     };
     // scores -> weights, times 2^shift where they are used and summed without it; a lane's scores j of tile tt are the
-    // tokens 32 tt + 16 (j / 8) + 8 half + j % 8
-    auto soften = [&](f32x16 (&x)[2], int b, float f, float shift) {
+    // tokens 32 tt + 16 (j / 8) + 8 half + j % 8.  unit: what the accumulators' unit is to be multiplied by (1: as it is).
+    auto soften = [&](f32x16 (&x)[2], int b, float f, float shift, float unit) {
         const bool edge = b * Q8_BLOCK + Q8_BLOCK - 1 > wave_first;
         const int mine = last - b * Q8_BLOCK - 8 * half;
         if (edge) {
@@ -788,27 +788,35 @@ __global__ __launch_bounds__(CQ_WAVES * 64, 2) void attn_chunk_q8_kernel(const C
             for (int j = 0; j < 16; ++j) top = fmaxf(top, x[tt][j]);
         top = xor_max<32>(top);
         top = top == -INFINITY ? top : top * f;
-        if (__any(top > m + CQ_SLACK)) {
+        if (unit != 1.0f || __any(top > m + CQ_SLACK)) {
             const float now = fmaxf(m, top);
             const float keep = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - now);
             l *= keep;
             m = now;
+            const float turn = keep * unit;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int j = 0; j < 16; ++j) o[i][j] *= keep;
+                for (int j = 0; j < 16; ++j) o[i][j] *= turn;
         }
         const float base = (m == -INFINITY ? 0.0f : m) - shift;
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) x[tt][j] = __builtin_amdgcn_exp2f(fmaf(x[tt][j], f, -base));
+        if (edge) {  // again: a scale that is NaN reaches the rows that see its block only
+            asm volatile("");  // (a branch: selects would cost every block what few need)
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    if (32 * tt + 16 * (j >> 3) + (j & 7) > mine) x[tt][j] = 0.0f;
+        }
         float sum = 0.0f;
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                x[tt][j] = __builtin_amdgcn_exp2f(fmaf(x[tt][j], f, -base));
-                // again: a scale that is NaN reaches the rows that see its block only
-                if (edge && 32 * tt + 16 * (j >> 3) + (j & 7) > mine) x[tt][j] = 0.0f;
-                sum += x[tt][j];
-            }
+            for (int j = 0; j < 16; ++j) sum += x[tt][j];
         if (sum != 0.0f) l = fmaf(sum, __builtin_amdgcn_exp2f(-shift), l);
     };
 
@@ -824,16 +832,14 @@ __global__ __launch_bounds__(CQ_WAVES * 64, 2) void attn_chunk_q8_kernel(const C
         if (b * Q8_BLOCK <= wave_last) {
             f32x16 x[2];
             scores(buf, x);
-            if (vs > smax) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) o[i][j] *= smax / vs;
+            float unit = 1.0f;
+            if (vs > 2.0f * smax) {  // up to twice the unit's scale is in fp16's range too
+                unit = smax / vs;
                 smax = vs;
             }
             // a block of zeros may have any scale: its scores or its values are zeros all the same
             const float shift = vs == 0.0f ? 0.0f : __builtin_amdgcn_logf(vs * (DQ_P_SCALE / (smax > 0.0f ? smax : 1.0f)));
-            soften(x, b, (ks == 0.0f ? 1.0f : ks) * a.scale_log2, shift);
+            soften(x, b, (ks == 0.0f ? 1.0f : ks) * a.scale_log2, shift, unit);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 f16x8 p;
@@ -873,7 +879,7 @@ __global__ __launch_bounds__(CQ_WAVES * 64, 2) void attn_chunk_q8_kernel(const C
             f32x16 x[2];
             scores(0, x);
             if (smax == 0.0f) smax = 1.0f;
-            soften(x, tail_b, a.scale_log2, __builtin_amdgcn_logf(DQ_P_SCALE / smax));
+            soften(x, tail_b, a.scale_log2, __builtin_amdgcn_logf(DQ_P_SCALE / smax), 1.0f);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 bf16x8 ph, pl;
