@@ -633,8 +633,8 @@ static uint32_t dq_units(uint32_t n_seq, uint32_t nk, uint32_t nb) {
 // ------------------------------------------------------------------------------------------------------ chunks --
 //
 // Bound by the matrix cores and, as much, by the softmax's and the conversion's vector instructions.  The queries of a KV
-// head's q heads are rows of one matrix (row = t * group + g), so a key tile serves them all; a thread block takes 128 rows,
-// a wave 32, and walks the cache a block of 64 tokens at a time:
+// head's q heads are rows of one matrix (row = t * group + g), so a key tile serves them all; a wave takes
+// 32 rows, a thread block 4 or 8 waves, and walks the cache a block of 64 tokens at a time:
 //   * a block's codes go to registers one step ahead, become bf16 keys and fp16 values (both exact) and go to the other of
 //     two LDS buffers: one barrier a step;
 //   * S^T = K . Q^T and O^T = V^T . P^T (32 x 32 x 16), so that a lane has 32 of a row's 64 scores in registers: one
@@ -646,8 +646,7 @@ static uint32_t dq_units(uint32_t n_seq, uint32_t nk, uint32_t nb) {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-constexpr int CQ_WAVES = 4;
-constexpr int CQ_ROWS = 32 * CQ_WAVES;  // rows a thread block
+constexpr uint32_t CQ_WIDE_GRID = 512;
 constexpr float CQ_SLACK = 2.0f;        // log2 that a row's weights may pass 1 by: 2^12 * 2^2 * 2 is in fp16's range
 
 struct ChunkQ8Args {
@@ -683,7 +682,9 @@ __device__ __forceinline__ uint4 codes_bf16x8(uint32_t w0, uint32_t w1) {
 __device__ __forceinline__ int cq_key_at(int token, int chunk) { return token * 16 + (chunk ^ (token & 15)); }
 __device__ __forceinline__ int cq_value_at(int d, int chunk) { return d * 8 + (chunk ^ (d & 7)); }
 
-__global__ __launch_bounds__(CQ_WAVES * 64, 2) void attn_chunk_q8_kernel(const ChunkQ8Args a) {
+template <int WAVES>
+__global__ __launch_bounds__(WAVES * 64, 2) void attn_chunk_q8_kernel(const ChunkQ8Args a) {
+    constexpr int ROWS = 32 * WAVES, THREADS = 64 * WAVES, PIECES = Q8_BYTES / 16 / THREADS;
     __shared__ __align__(16) uint4 keys[2][Q8_BLOCK * 16];
     __shared__ __align__(16) uint4 values[2][Q8_D * 8];
     const int tid = threadIdx.x, lane = tid & 63;
@@ -704,38 +705,38 @@ __global__ __launch_bounds__(CQ_WAVES * 64, 2) void attn_chunk_q8_kernel(const C
     const size_t head_row = ((size_t)seq * a.c.nk + h) * a.n * group;  // of row 0 in lse and the parts
 
     // rows of this wave: row0 + lane % 32; `last` is the last token that the lane's row sees
-    const int row0 = tile * CQ_ROWS + wave * 32;
+    const int row0 = tile * ROWS + wave * 32;
     const int row = row0 + col;
     const int t = row / group, g = row - t * group;
     const int last = row < rows ? (len + t < s.end ? len + t : s.end - 1) : -1;
     const int wave_top = row0 + 31 < rows ? row0 + 31 : rows - 1;  // its last live row, below row0 if it has none
     const int wave_last = wave_top >= row0 ? (len + wave_top / group < s.end ? len + wave_top / group : s.end - 1) : -1;
     const int wave_first = row0 < rows ? (len + row0 / group < s.end ? len + row0 / group : s.end - 1) : -1;
-    const int top_row = (tile + 1) * CQ_ROWS < rows ? (tile + 1) * CQ_ROWS - 1 : rows - 1;
-    const int tile_last = tile * CQ_ROWS < rows ? (len + top_row / group < s.end ? len + top_row / group : s.end - 1) : -1;
+    const int top_row = (tile + 1) * ROWS < rows ? (tile + 1) * ROWS - 1 : rows - 1;
+    const int tile_last = tile * ROWS < rows ? (len + top_row / group < s.end ? len + top_row / group : s.end - 1) : -1;
     const int blocks = tile_last >= 0 ? tile_last / Q8_BLOCK + 1 : 0;
     const int b0 = (int)((int64_t)blocks * split / a.splits), b1 = (int)((int64_t)blocks * (split + 1) / a.splits);
     const int tail_b = s.end % Q8_BLOCK ? s.end / Q8_BLOCK : -1;  // held in bf16
     const bool has_tail = tail_b >= b0 && tail_b < b1;
     const int whole = has_tail ? b1 - 1 : b1;
 
-    // a block's codes: 16-byte pieces tid and tid + 256, of a token (8 pieces) and of a value's dim (4)
-    uint4 kc[2], vc[2];
+    // a block's codes: 16-byte pieces tid, tid + THREADS .., of a token (8 pieces) and of a value's dim (4)
+    uint4 kc[PIECES], vc[PIECES];
     float ks = 0.0f, vs = 0.0f, ks_next = 0.0f, vs_next = 0.0f;
     auto load = [&](int b) {
         const size_t at = a.c.block_at(seq, (uint32_t)b, h);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            kc[i] = load_u4(a.c.k + at + (tid + 256 * i) * 16);
-            vc[i] = load_u4(a.c.v + at + (tid + 256 * i) * 16);
+        for (int i = 0; i < PIECES; ++i) {
+            kc[i] = load_u4(a.c.k + at + (tid + THREADS * i) * 16);
+            vc[i] = load_u4(a.c.v + at + (tid + THREADS * i) * 16);
         }
         ks_next = a.c.ks[a.c.scale_at(seq, (uint32_t)b, h)];
         vs_next = a.c.vs[a.c.scale_at(seq, (uint32_t)b, h)];
     };
     auto store = [&](int buf) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int n = tid + 256 * i;
+        for (int i = 0; i < PIECES; ++i) {
+            const int n = tid + THREADS * i;
             keys[buf][cq_key_at(n >> 3, 2 * (n & 7))] = codes_bf16x8(kc[i].x, kc[i].y);
             keys[buf][cq_key_at(n >> 3, 2 * (n & 7) + 1)] = codes_bf16x8(kc[i].z, kc[i].w);
             values[buf][cq_value_at(n >> 2, 2 * (n & 3))] = __builtin_bit_cast(uint4, codes_f16x8(vc[i].x, vc[i].y));
@@ -862,8 +863,8 @@ __global__ __launch_bounds__(CQ_WAVES * 64, 2) void attn_chunk_q8_kernel(const C
         const size_t at = a.c.tail_at(seq, h);
         const int live = s.end % Q8_BLOCK;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int n = tid + 256 * i;
+        for (int i = 0; i < 2 * PIECES; ++i) {
+            const int n = tid + THREADS * i;
             keys[0][cq_key_at(n >> 4, n & 15)] = load_u4(a.c.kt + at + n * 8);
             uint4 v = load_u4(a.c.vt + at + n * 8);
             uint32_t* w = reinterpret_cast<uint32_t*>(&v);
@@ -1055,9 +1056,14 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_q8_weights_kernel(const Chu
         }
 }
 
+// Waves a thread block: 8 share a block's conversion to 16 bits where that leaves a thread block for every CU and more.
+static uint32_t cq_waves(uint32_t n, uint32_t n_seq, uint32_t nh, uint32_t nk) {
+    return ((uint64_t)n * (nh / nk) + 255) / 256 * n_seq * nk >= CQ_WIDE_GRID ? 8 : 4;
+}
+
 // Thread blocks that share a tile's keys: enough for two a CU, where a tile has at least 4 blocks of keys for each.
 static uint32_t cq_splits(uint32_t n, uint32_t n_seq, uint32_t nh, uint32_t nk, uint32_t nb) {
-    const uint64_t tiles = ((uint64_t)n * (nh / nk) + CQ_ROWS - 1) / CQ_ROWS;
+    const uint64_t rows = 32 * cq_waves(n, n_seq, nh, nk), tiles = ((uint64_t)n * (nh / nk) + rows - 1) / rows;
     const uint64_t grid = tiles * n_seq * nk;
     const uint64_t want = grid ? (512 + grid - 1) / grid : 1, most = nb / 4;
     return (uint32_t)(want < most ? (want ? want : 1) : (most ? most : 1));
@@ -1164,7 +1170,8 @@ extern "C" int t2h_flash_attn_prefill_q8(const void* q, void* const* cache, uint
     a.nh = nh;
     a.group = nh / nk;
     a.scale_log2 = 1.4426950408889634f * (scale > 0.0f ? scale : 1.0f / sqrtf((float)Q8_D));
-    const uint64_t rows = (uint64_t)n_seq * nh * n, tiles = ((uint64_t)n * a.group + CQ_ROWS - 1) / CQ_ROWS;
+    const uint64_t rows = (uint64_t)n_seq * nh * n, tile_rows = 32 * cq_waves(n, n_seq, nh, nk),
+                   tiles = ((uint64_t)n * a.group + tile_rows - 1) / tile_rows;
     if (rows > 0x3fffffffu) return T2H_ERR_SHAPE;
     a.splits = cq_splits(n, n_seq, nh, nk, a.c.nb);
     a.tiles = (uint32_t)tiles;
@@ -1180,7 +1187,10 @@ extern "C" int t2h_flash_attn_prefill_q8(const void* q, void* const* cache, uint
     const uint64_t wgrid = (uint64_t)n_seq * nk * ((a.c.nb + 3) / 4);
     if (grid > 0x7fffffffu || wgrid > 0x7fffffffu) return T2H_ERR_SHAPE;
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    hipLaunchKernelGGL(attn_chunk_q8_kernel, dim3((uint32_t)grid), dim3(CQ_WAVES * 64), 0, st, a);
+    if (tile_rows == 256)
+        hipLaunchKernelGGL(attn_chunk_q8_kernel<8>, dim3((uint32_t)grid), dim3(512), 0, st, a);
+    else
+        hipLaunchKernelGGL(attn_chunk_q8_kernel<4>, dim3((uint32_t)grid), dim3(256), 0, st, a);
     T2H_LAUNCH_CHECK();
     if (a.splits > 1) {
         hipLaunchKernelGGL(attn_chunk_q8_merge_kernel, dim3((uint32_t)merge), dim3(256), 0, st, a);
