@@ -690,13 +690,19 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_chunk_q8_kernel(const Chun
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31, half = lane >> 5;
+    // The longest tiles first; in every other round of 256 thread blocks, one a CU, from the shortest up, so that the CUs of
+    // a grid of two or three rounds get long and short ones alike.  An XCD (of 8, in turn) keeps its share of the heads.
     uint32_t rest = blockIdx.x;
+    if (rest / 256 & 1) {
+        const uint32_t left = gridDim.x - rest / 256 * 256, size = left < 256 ? left / 8 * 8 : 256;
+        if (rest % 256 < size) rest = rest / 256 * 256 + (size - 8 - rest % 256 / 8 * 8) + rest % 8;
+    }
     const uint32_t h = rest % a.c.nk;  // neighbours work on different heads: with 8 of them an XCD's L2 holds one head's keys
     rest /= a.c.nk;
     const uint32_t split = rest % a.splits;
     rest /= a.splits;
     const uint32_t seq = rest % a.n_seq;
-    const int tile = (int)(a.tiles - 1 - rest / a.n_seq);  // the longest first
+    const int tile = (int)(a.tiles - 1 - rest / a.n_seq);
     const Q8Span s = q8_span(a.lengths, a.counts, seq, a.n, a.c.nb);
     const int len = min(a.lengths[seq], (int)(a.c.nb * Q8_BLOCK));
     int count = a.counts ? a.counts[seq] : (int)a.n;
@@ -944,16 +950,27 @@ __global__ __launch_bounds__(256) void attn_chunk_q8_merge_kernel(const ChunkQ8A
     const uint64_t head = at / ((uint64_t)a.n * a.group);
     const uint32_t h = (uint32_t)(head % a.c.nk), seq = (uint32_t)(head / a.c.nk);
     const uint32_t t = row / a.group, g = row % a.group;
+    constexpr uint32_t BATCH = 8;  // parts in flight
     float M = -INFINITY, L = 0.0f;
-    for (uint32_t i = 0; i < a.splits; ++i) M = fmaxf(M, a.part_ml[2 * (i * all + at)]);
-    const float base = M == -INFINITY ? 0.0f : M;
     f32x4 sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-    for (uint32_t i = 0; i < a.splits; ++i) {
-        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (i * all + at));
-        const float f = __builtin_amdgcn_exp2f(ml.x - base);
-        L = fmaf(f, ml.y, L);
-        sum += *reinterpret_cast<const f32x4*>(a.part_o + (i * all + at) * Q8_D + d) * f;
+    for (uint32_t i0 = 0; i0 < a.splits; i0 += BATCH) {
+        float2 ml[BATCH];
+        f32x4 part[BATCH];
+#pragma unroll
+        for (uint32_t e = 0; e < BATCH; ++e) {
+            const uint64_t i = (i0 + e < a.splits ? i0 + e : i0) * all + at;
+            ml[e] = *reinterpret_cast<const float2*>(a.part_ml + 2 * i);
+            part[e] = *reinterpret_cast<const f32x4*>(a.part_o + i * Q8_D + d);
+        }
+#pragma unroll
+        for (uint32_t e = 0; e < BATCH; ++e) {
+            if (i0 + e >= a.splits) break;
+            const float now = fmaxf(M, ml[e].x), base = now == -INFINITY ? 0.0f : now;
+            const float keep = __builtin_amdgcn_exp2f(M - base), f = __builtin_amdgcn_exp2f(ml[e].x - base);
+            L = fmaf(L, keep, f * ml[e].y);
+            sum = sum * keep + part[e] * f;
+            M = now;
+        }
     }
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
     *reinterpret_cast<uint2*>(a.out + (((size_t)seq * a.n + t) * a.nh + h * a.group + g) * Q8_D + d) =
@@ -962,23 +979,45 @@ __global__ __launch_bounds__(256) void attn_chunk_q8_merge_kernel(const ChunkQ8A
 }
 
 // weights_out[token] = weights_in (0 for a new token) + sum of exp2(score - lse) over the rows of the KV head.  A wave takes
-// 64 tokens, one cache block, as the operand that stays in registers; the rows' queries stream past, the same for the
-// thread block's four waves.  Sums are in a fixed order.
+// 64 tokens, one cache block, as the operand that stays in registers; the rows' queries pass through LDS, 64 at a time and
+// the next 64 on their way, the same for the thread block's four waves.  Sums are in a fixed order.  Bound by the
+// exponentials, a quarter of a vector instruction's rate.
 __global__ __launch_bounds__(256, 2) void attn_chunk_q8_weights_kernel(const ChunkQ8Args a) {
-    const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    constexpr int STEP = 64;  // rows
+    __shared__ __align__(16) uint4 queries[2][STEP * 16];
+    const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t h = blockIdx.x % a.c.nk;
     const uint32_t rest = blockIdx.x / a.c.nk;
     const uint32_t per = (a.c.nb + 3) / 4;
     const uint32_t seq = rest / per;
-    const int b = (int)(rest % per) * 4 + wave;
+    const int first_b = (int)(rest % per) * 4, b = first_b + wave;
     const Q8Span s = q8_span(a.lengths, a.counts, seq, a.n, a.c.nb);
-    if (b * Q8_BLOCK >= s.end) return;
+    if (first_b * Q8_BLOCK >= s.end) return;
     const int len = min(a.lengths[seq], (int)(a.c.nb * Q8_BLOCK));
     int count = a.counts ? a.counts[seq] : (int)a.n;
     count = len < 0 || count < 0 ? 0 : (count < (int)a.n ? count : (int)a.n);
     const int group = (int)a.group, rows = count * group;
+    const bool mine = b * Q8_BLOCK < s.end;
     const bool in_tail = s.end % Q8_BLOCK && b == s.end / Q8_BLOCK;
+    // from the first row that sees the thread block's first token
+    const int t_first = first_b * Q8_BLOCK - len;
+    const int row_first = t_first > 0 ? t_first * group / STEP * STEP : 0;
+    uint4 next[4];
+    auto load = [&](int row0) {  // 16 bytes of a row: piece tid % 16 of rows tid / 16, + 16 ..
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = row0 + (tid >> 4) + 16 * i;
+            const int t = row / group, g = row - t * group;
+            const size_t at = (((size_t)seq * a.n + (row < rows ? t : 0)) * a.nh + h * group + (row < rows ? g : 0)) * Q8_D;
+            next[i] = load_u4(a.q + at + 8 * (tid & 15));
+        }
+    };
+    auto store = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) queries[buf][cq_key_at((tid >> 4) + 16 * i, tid & 15)] = next[i];
+    };
+    load(row_first);
     bf16x8 k[2][8];
     float f = a.scale_log2;
     if (in_tail) {
@@ -988,7 +1027,8 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_q8_weights_kernel(const Chu
 #pragma unroll
             for (int i = 0; i < 8; ++i) k[tt][i] = as_bf16x8(load_u4(p + (32 * tt + col) * Q8_D + 16 * i));
     } else {
-        const int8_t* p = a.c.k + a.c.block_at(seq, (uint32_t)b, h) + 8 * half;
+        const int from = mine ? b : first_b;  // (a wave without a block helps with the queries)
+        const int8_t* p = a.c.k + a.c.block_at(seq, (uint32_t)from, h) + 8 * half;
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
@@ -996,7 +1036,7 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_q8_weights_kernel(const Chu
                 const uint2 w = *reinterpret_cast<const uint2*>(p + (32 * tt + col) * Q8_D + 16 * i);
                 k[tt][i] = as_bf16x8(codes_bf16x8(w.x, w.y));
             }
-        f *= a.c.ks[a.c.scale_at(seq, (uint32_t)b, h)];
+        f *= a.c.ks[a.c.scale_at(seq, (uint32_t)from, h)];
     }
     float sum[2][16];
 #pragma unroll
@@ -1004,35 +1044,48 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_q8_weights_kernel(const Chu
 #pragma unroll
         for (int j = 0; j < 16; ++j) sum[tt][j] = 0.0f;
     const float* lse = a.lse + ((size_t)seq * a.c.nk + h) * a.n * group;
-    // rows of queries that see the block's first token
-    const int t_first = b * Q8_BLOCK - len;
-    for (int row0 = t_first > 0 ? t_first * group / 32 * 32 : 0; row0 < rows; row0 += 32) {
-        const int row = row0 + col;
-        const int t = row / group, g = row - t * group;
-        const bool live = row < rows;
-        const uint16_t* qp = a.q + (((size_t)seq * a.n + (live ? t : 0)) * a.nh + h * group + (live ? g : 0)) * Q8_D + 8 * half;
-        const float sub = live ? lse[row] : INFINITY;
-        f32x16 x[2];
+    store(0);
+    __syncthreads();
+    for (int row0 = row_first; row0 < rows; row0 += STEP) {
+        const int buf = (row0 - row_first) / STEP & 1;
+        if (row0 + STEP < rows) load(row0 + STEP);
+        if (mine) {
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
+            for (int r = 0; r < 2; ++r) {
+                const int row = row0 + 32 * r + col, t = row / group;
+                const float sub = row < rows ? lse[row] : INFINITY;  // a row that is not there weighs nothing
+                f32x16 x[2];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) x[tt][j] = 0.0f;
+                for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const bf16x8 q = as_bf16x8(load_u4(qp + 16 * i));
-            x[0] = mfma_bf16(k[0][i], q, x[0]);
-            x[1] = mfma_bf16(k[1][i], q, x[1]);
-        }
-        const int mine = len + t - b * Q8_BLOCK - 4 * half;  // tokens 32 tt + 8 (j / 4) + 4 half + j % 4
-        const bool edge = b * Q8_BLOCK + Q8_BLOCK - 1 > len + row0 / group;
+                    for (int j = 0; j < 16; ++j) x[tt][j] = 0.0f;
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
+                for (int i = 0; i < 8; ++i) {
+                    const bf16x8 q = as_bf16x8(queries[buf][cq_key_at(32 * r + col, 2 * i + half)]);
+                    x[0] = mfma_bf16(k[0][i], q, x[0]);
+                    x[1] = mfma_bf16(k[1][i], q, x[1]);
+                }
+                if (b * Q8_BLOCK + Q8_BLOCK - 1 > len + (row0 + 32 * r) / group) {
+                    const int seen = len + t - b * Q8_BLOCK - 4 * half;  // tokens 32 tt + 8 (j / 4) + 4 half + j % 4
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const float p = __builtin_amdgcn_exp2f(fmaf(x[tt][j], f, -sub));
-                sum[tt][j] += (!live || (edge && 32 * tt + 8 * (j >> 2) + (j & 3) > mine)) ? 0.0f : p;
+                    for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            const float p = __builtin_amdgcn_exp2f(fmaf(x[tt][j], f, -sub));
+                            sum[tt][j] += row >= rows || 32 * tt + 8 * (j >> 2) + (j & 3) > seen ? 0.0f : p;
+                        }
+                } else {
+#pragma unroll
+                    for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) sum[tt][j] += __builtin_amdgcn_exp2f(fmaf(x[tt][j], f, -sub));
+                }
             }
+        }
+        if (row0 + STEP < rows) store(buf ^ 1);
+        __syncthreads();
     }
+    if (!mine) return;
     // over the 32 rows that the lanes of a half hold
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt)
@@ -1061,11 +1114,14 @@ static uint32_t cq_waves(uint32_t n, uint32_t n_seq, uint32_t nh, uint32_t nk) {
     return ((uint64_t)n * (nh / nk) + 255) / 256 * n_seq * nk >= CQ_WIDE_GRID ? 8 : 4;
 }
 
-// Thread blocks that share a tile's keys: enough for two a CU, where a tile has at least 4 blocks of keys for each.
+// Thread blocks that share a tile's keys: two a CU where there are not as many tiles, each with 4 blocks of keys or more of
+// those that a row of the chunk's middle sees in a full cache.  Measured (us, 32 / 8 heads but for the last): 1901 tokens,
+// 480 tiles: 58 whole, 64 in two parts; 700, 176 tiles: 25 whole, 30 in two; 2 x 5 tokens at 4000: 20 in 16 parts, 24 in 8
+// and in 32; 2048 of 16 / 8 heads, 256 tiles: 48 in two, 58 whole.
 static uint32_t cq_splits(uint32_t n, uint32_t n_seq, uint32_t nh, uint32_t nk, uint32_t nb) {
     const uint64_t rows = 32 * cq_waves(n, n_seq, nh, nk), tiles = ((uint64_t)n * (nh / nk) + rows - 1) / rows;
     const uint64_t grid = tiles * n_seq * nk;
-    const uint64_t want = grid ? (512 + grid - 1) / grid : 1, most = nb / 4;
+    const uint64_t want = grid ? 512 / grid : 1, skip = n / (2 * Q8_BLOCK), most = nb > skip ? (nb - skip) / 4 : 0;
     return (uint32_t)(want < most ? (want ? want : 1) : (most ? most : 1));
 }
 

@@ -35,6 +35,7 @@ struct Q8WriteArgs {
 };
 
 constexpr int Q8W_HEADS = 8;  // q heads a wave
+constexpr int Q8W_WAVES = 8;  // a thread block
 
 __device__ __forceinline__ void q8_write_q(const Q8WriteArgs& a, uint64_t unit) {
     const int lane = threadIdx.x & 63;
@@ -73,11 +74,11 @@ __device__ __forceinline__ void q8_write_q(const Q8WriteArgs& a, uint64_t unit) 
     }
 }
 
-// One cache block of one head: tokens 64 b + 16 wave + i in wave `wave`, row i; a lane holds key dims lane and lane + 64
+// One cache block of one head: tokens 64 b + 8 wave + i in wave `wave`, row i; a lane holds key dims lane and lane + 64
 // and value dims 2 lane and 2 lane + 1, as bf16 pairs.
 __device__ __forceinline__ void q8_write_block(const Q8WriteArgs& a, uint32_t seq, uint32_t h, Q8Span s, int b,
                                                uint32_t* kbytes, uint32_t* red) {
-    constexpr int ROWS = Q8_BLOCK / 4;
+    constexpr int ROWS = Q8_BLOCK / Q8W_WAVES;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int p0 = b * Q8_BLOCK + wave * ROWS;
     const bool whole = (b + 1) * Q8_BLOCK <= s.end;
@@ -135,16 +136,20 @@ __device__ __forceinline__ void q8_write_block(const Q8WriteArgs& a, uint32_t se
     vmax = wave_max_u32(vmax);
     if (lane == 0) {
         red[wave] = kmax;
-        red[4 + wave] = vmax;
+        red[Q8W_WAVES + wave] = vmax;
     }
     __syncthreads();
+    for (int i = 0; i < Q8W_WAVES; ++i) {
+        kmax = max(kmax, red[i]);
+        vmax = max(vmax, red[Q8W_WAVES + i]);
+    }
     float ks, kinv, vs, vinv;
-    q8_scale(max(max(red[0], red[1]), max(red[2], red[3])), ks, kinv);
-    q8_scale(max(max(red[4], red[5]), max(red[6], red[7])), vs, vinv);
+    q8_scale(kmax, ks, kinv);
+    q8_scale(vmax, vs, vinv);
     // keys: bytes through LDS, so that they leave as 16-byte stores
     uint8_t* kb = reinterpret_cast<uint8_t*>(kbytes) + wave * ROWS * Q8_D + lane;
     const size_t at = a.c.block_at(seq, (uint32_t)b, h);
-    uint32_t lo[4], hi[4];
+    uint32_t lo[ROWS / 4], hi[ROWS / 4];
 #pragma unroll
     for (int i = 0; i < ROWS; i += 4) {
 #pragma unroll
@@ -158,23 +163,21 @@ __device__ __forceinline__ void q8_write_block(const Q8WriteArgs& a, uint32_t se
                              __uint_as_float(vv[i + 2] & 0xffff0000u), __uint_as_float(vv[i + 3] & 0xffff0000u), vinv);
     }
     int8_t* vb = a.c.v + at + (size_t)(2 * lane) * Q8_BLOCK + wave * ROWS;
-    *reinterpret_cast<uint4*>(vb) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-    *reinterpret_cast<uint4*>(vb + Q8_BLOCK) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    *reinterpret_cast<uint2*>(vb) = make_uint2(lo[0], lo[1]);
+    *reinterpret_cast<uint2*>(vb + Q8_BLOCK) = make_uint2(hi[0], hi[1]);
     __syncthreads();
-    uint4* kout = reinterpret_cast<uint4*>(a.c.k + at);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) kout[threadIdx.x + 256 * i] = reinterpret_cast<const uint4*>(kbytes)[threadIdx.x + 256 * i];
+    reinterpret_cast<uint4*>(a.c.k + at)[threadIdx.x] = reinterpret_cast<const uint4*>(kbytes)[threadIdx.x];
     if (threadIdx.x == 0) {
         a.c.ks[a.c.scale_at(seq, (uint32_t)b, h)] = ks;
         a.c.vs[a.c.scale_at(seq, (uint32_t)b, h)] = vs;
     }
 }
 
-__global__ __launch_bounds__(256) void q8_write_kernel(const Q8WriteArgs a) {
+__global__ __launch_bounds__(Q8W_WAVES * 64) void q8_write_kernel(const Q8WriteArgs a) {
     __shared__ __align__(16) uint32_t kbytes[Q8_BYTES / 4];
-    __shared__ uint32_t red[8];
+    __shared__ uint32_t red[2 * Q8W_WAVES];
     if (blockIdx.x >= a.kv_grid) {
-        q8_write_q(a, (uint64_t)(blockIdx.x - a.kv_grid) * 4 + (threadIdx.x >> 6));
+        q8_write_q(a, (uint64_t)(blockIdx.x - a.kv_grid) * Q8W_WAVES + (threadIdx.x >> 6));
         return;
     }
     const uint32_t h = blockIdx.x % a.c.nk;
@@ -529,7 +532,7 @@ extern "C" int t2h_qk_norm_rope_cache_q8(const float* q, uint64_t q_row, const f
     const uint64_t kv_blocks = ((uint64_t)n + 2 * Q8_BLOCK - 2) / Q8_BLOCK;
     const uint64_t kv_grid = kv_blocks * nk * n_seq;
     const uint64_t units = (uint64_t)n_seq * n * ((nh + Q8W_HEADS - 1) / Q8W_HEADS);
-    if (n > 0x3fffffffu || kv_grid + (units + 3) / 4 > 0x7fffffffu) return T2H_ERR_SHAPE;
+    if (n > 0x3fffffffu || kv_grid + (units + Q8W_WAVES - 1) / Q8W_WAVES > 0x7fffffffu) return T2H_ERR_SHAPE;
     a.q = q;
     a.k = k;
     a.v = v;
@@ -550,7 +553,7 @@ extern "C" int t2h_qk_norm_rope_cache_q8(const float* q, uint64_t q_row, const f
     a.kv_blocks = (uint32_t)kv_blocks;
     a.kv_grid = (uint32_t)kv_grid;
     a.q_out = reinterpret_cast<uint16_t*>(q_out);
-    hipLaunchKernelGGL(q8_write_kernel, dim3((uint32_t)(kv_grid + (units + 3) / 4)), dim3(256), 0,
+    hipLaunchKernelGGL(q8_write_kernel, dim3((uint32_t)(kv_grid + (units + Q8W_WAVES - 1) / Q8W_WAVES)), dim3(Q8W_WAVES * 64), 0,
                        reinterpret_cast<hipStream_t>(stream), a);
     T2H_LAUNCH_CHECK();
     return T2H_OK;
