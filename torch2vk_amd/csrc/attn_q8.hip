@@ -717,7 +717,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_chunk_q8_kernel(const Chun
     const int last = row < rows ? (len + t < s.end ? len + t : s.end - 1) : -1;
     const int wave_top = row0 + 31 < rows ? row0 + 31 : rows - 1;  // its last live row, below row0 if it has none
     const int wave_last = wave_top >= row0 ? (len + wave_top / group < s.end ? len + wave_top / group : s.end - 1) : -1;
-    const int wave_first = row0 < rows ? (len + row0 / group < s.end ? len + row0 / group : s.end - 1) : -1;
+    // (a wave without rows takes all of every block for seen, and what it computes for nothing)
+    const int wave_first = row0 < rows ? (len + row0 / group < s.end ? len + row0 / group : s.end - 1) : 0x7fffffff;
     const int top_row = (tile + 1) * ROWS < rows ? (tile + 1) * ROWS - 1 : rows - 1;
     const int tile_last = tile * ROWS < rows ? (len + top_row / group < s.end ? len + top_row / group : s.end - 1) : -1;
     const int blocks = tile_last >= 0 ? tile_last / Q8_BLOCK + 1 : 0;
@@ -739,15 +740,15 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_chunk_q8_kernel(const Chun
         ks_next = a.c.ks[a.c.scale_at(seq, (uint32_t)b, h)];
         vs_next = a.c.vs[a.c.scale_at(seq, (uint32_t)b, h)];
     };
-    auto store = [&](int buf) {
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-            const int n = tid + THREADS * i;
-            keys[buf][cq_key_at(n >> 3, 2 * (n & 7))] = codes_bf16x8(kc[i].x, kc[i].y);
-            keys[buf][cq_key_at(n >> 3, 2 * (n & 7) + 1)] = codes_bf16x8(kc[i].z, kc[i].w);
-            values[buf][cq_value_at(n >> 2, 2 * (n & 3))] = __builtin_bit_cast(uint4, codes_f16x8(vc[i].x, vc[i].y));
-            values[buf][cq_value_at(n >> 2, 2 * (n & 3) + 1)] = __builtin_bit_cast(uint4, codes_f16x8(vc[i].z, vc[i].w));
-        }
+    // 16 bytes of LDS at a time: 0, 1: keys of piece 0, then its values, then those of piece 1
+    auto store = [&](int buf, int e) {
+        const int i = e >> 2, n = tid + THREADS * i;
+        const uint32_t lo = e & 1 ? (e & 2 ? vc[i].z : kc[i].z) : (e & 2 ? vc[i].x : kc[i].x);
+        const uint32_t hi = e & 1 ? (e & 2 ? vc[i].w : kc[i].w) : (e & 2 ? vc[i].y : kc[i].y);
+        if (e & 2)
+            values[buf][cq_value_at(n >> 2, 2 * (n & 3) + (e & 1))] = __builtin_bit_cast(uint4, codes_f16x8(lo, hi));
+        else
+            keys[buf][cq_key_at(n >> 3, 2 * (n & 7) + (e & 1))] = codes_bf16x8(lo, hi);
     };
     if (b0 < whole) load(b0);
     // the row's query
@@ -775,17 +776,24 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_chunk_q8_kernel(const Chun
                 x[tt] = mfma_bf16(as_bf16x8(keys[buf][cq_key_at(32 * tt + key_row, 2 * i + half)]), as_bf16x8(q[i]), x[tt]);
         }
     };
-    // scores -> weights, times 2^shift where they are used and summed without it; a lane's scores j of tile tt are the
-    // tokens 32 tt + 16 (j / 8) + 8 half + j % 8.  unit: what the accumulators' unit is to be multiplied by (1: as it is).
-    auto soften = [&](f32x16 (&x)[2], int b, float f, float shift, float unit) {
-        const bool edge = b * Q8_BLOCK + Q8_BLOCK - 1 > wave_first;
-        const int mine = last - b * Q8_BLOCK - 8 * half;
-        if (edge) {
+    // What comes before the weights: rows that do not see all of the block, and the row's maximum, which the accumulators
+    // follow.  A lane's scores j of tile tt are the tokens 32 tt + 16 (j / 8) + 8 half + j % 8; f is their factor, 2^shift
+    // the weights', unit what the accumulators' unit is to be multiplied by (1: as it is).
+    auto ready = [&](f32x16 (&x)[2], int b, float& f, float& shift, float unit) {
+        if (b * Q8_BLOCK + Q8_BLOCK - 1 > wave_first) {
+            const int mine = last - b * Q8_BLOCK - 8 * half;
+            const bool broken = f != f || shift != shift;  // a scale that is NaN reaches the rows that see its block only
 #pragma unroll
             for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
-                for (int j = 0; j < 16; ++j)
+                for (int j = 0; j < 16; ++j) {
+                    if (broken) x[tt][j] = __uint_as_float(0x7fc00000u);
                     if (32 * tt + 16 * (j >> 3) + (j & 7) > mine) x[tt][j] = -INFINITY;
+                }
+            if (broken) {
+                f = 1.0f;
+                shift = 0.0f;
+            }
         }
         // the maximum before the factor: ks and the scale are not negative
         float top = -INFINITY;
@@ -806,62 +814,88 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_chunk_q8_kernel(const Chun
 #pragma unroll
                 for (int j = 0; j < 16; ++j) o[i][j] *= turn;
         }
-        const float base = (m == -INFINITY ? 0.0f : m) - shift;
+    };
+    // weights j0 .. j1 - 1 of the 8 that a lane has of 16 tokens, and their sum
+    auto weigh = [&](f32x16 (&x)[2], int i, int j0, int j1, float f, float base, float& sum, float (&w)[8]) {
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-            for (int j = 0; j < 16; ++j) x[tt][j] = __builtin_amdgcn_exp2f(fmaf(x[tt][j], f, -base));
-        if (edge) {  // again: a scale that is NaN reaches the rows that see its block only
-            asm volatile("");  // (a branch: selects would cost every block what few need)
-#pragma unroll
-            for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-                for (int j = 0; j < 16; ++j)
-                    if (32 * tt + 16 * (j >> 3) + (j & 7) > mine) x[tt][j] = 0.0f;
+        for (int j = 0; j < 8; ++j) {
+            if (j < j0 || j >= j1) continue;
+            w[j] = __builtin_amdgcn_exp2f(fmaf(x[i >> 1][8 * (i & 1) + j], f, -base));
+            sum += w[j];
         }
-        float sum = 0.0f;
-#pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-            for (int j = 0; j < 16; ++j) sum += x[tt][j];
-        if (sum != 0.0f) l = fmaf(sum, __builtin_amdgcn_exp2f(-shift), l);
     };
 
+    // A step, in the order that it is issued in: block b's scores, a product for each of two tiles at a time and 8 codes of
+    // block b + 1 between them (they came during the step before and go to the other buffer); then 8 weights of a lane's at a
+    // time, two of them between two products of the 8 before.  Left to itself the compiler puts the products of a step in a
+    // row, which leaves the vector unit idle, or all operands in flight, for which there are no registers.
     if (b0 < whole) {
-        store(0);
+#pragma unroll
+        for (int e = 0; e < 4 * PIECES; ++e) store(0, e);
         ks = ks_next;
         vs = vs_next;
+        if (b0 + 1 < whole) load(b0 + 1);
     }
     __syncthreads();
     for (int b = b0; b < whole; ++b) {
         const int buf = (b - b0) & 1;
-        if (b + 1 < whole) load(b + 1);
-        if (b * Q8_BLOCK <= wave_last) {
-            f32x16 x[2];
-            scores(buf, x);
-            float unit = 1.0f;
-            if (vs > 2.0f * smax) {  // up to twice the unit's scale is in fp16's range too
-                unit = smax / vs;
-                smax = vs;
+        f32x16 x[2];
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) x[tt][j] = 0.0f;
+        uint4 kf[3][2];  // operands two steps ahead
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt) kf[i][tt] = keys[buf][cq_key_at(32 * tt + key_row, 2 * i + half)];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (i < 6) {
+#pragma unroll
+                for (int tt = 0; tt < 2; ++tt) kf[(i + 2) % 3][tt] = keys[buf][cq_key_at(32 * tt + key_row, 2 * (i + 2) + half)];
             }
-            // a block of zeros may have any scale: its scores or its values are zeros all the same
-            const float shift = vs == 0.0f ? 0.0f : __builtin_amdgcn_logf(vs * (DQ_P_SCALE / (smax > 0.0f ? smax : 1.0f)));
-            soften(x, b, (ks == 0.0f ? 1.0f : ks) * a.scale_log2, shift, unit);
+            x[0] = mfma_bf16(as_bf16x8(kf[i % 3][0]), as_bf16x8(q[i]), x[0]);
+            x[1] = mfma_bf16(as_bf16x8(kf[i % 3][1]), as_bf16x8(q[i]), x[1]);
+            if (PIECES == 2 || i % 2 == 0) store(buf ^ 1, PIECES == 2 ? i : i / 2);  // (behind the last block: what no one reads)
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        const float kf_scale = ks, vf_scale = vs;
+        ks = ks_next;
+        vs = vs_next;
+        if (b + 2 < whole) load(b + 2);
+        float unit = 1.0f;
+        if (vf_scale > 2.0f * smax) {  // up to twice the unit's scale is in fp16's range too
+            unit = smax / vf_scale;
+            smax = vf_scale;
+        }
+        // a block of zeros may have any scale: its scores or its values are zeros all the same
+        float shift = vf_scale == 0.0f ? 0.0f : __builtin_amdgcn_logf(vf_scale * (DQ_P_SCALE / (smax > 0.0f ? smax : 1.0f)));
+        float f = (kf_scale == 0.0f ? 1.0f : kf_scale) * a.scale_log2;
+        ready(x, b, f, shift, unit);
+        const float base = (m == -INFINITY ? 0.0f : m) - shift;
+        float sum = 0.0f;
+        uint4 vf[3];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                f16x8 p;
+        for (int i = 0; i < 2; ++i) vf[i] = values[buf][cq_value_at(32 * i + col, half)];
+        float w[8];
+        weigh(x, 0, 0, 8, f, base, sum, w);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) p[j] = (_Float16)x[i >> 1][8 * (i & 1) + j];
+        for (int i = 0; i < 4; ++i) {
+            f16x8 p;
 #pragma unroll
-                for (int dt = 0; dt < 4; ++dt)
-                    o[dt] = mfma_f16(__builtin_bit_cast(f16x8, values[buf][cq_value_at(32 * dt + col, 2 * i + half)]), p, o[dt]);
+            for (int j = 0; j < 8; ++j) p[j] = (_Float16)w[j];
+#pragma unroll
+            for (int dt = 0; dt < 4; ++dt) {
+                const int n = 4 * i + dt;
+                __builtin_amdgcn_sched_barrier(0);
+                if (n < 14) vf[(n + 2) % 3] = values[buf][cq_value_at(32 * ((n + 2) & 3) + col, 2 * ((n + 2) >> 2) + half)];
+                o[dt] = mfma_f16(__builtin_bit_cast(f16x8, vf[n % 3]), p, o[dt]);
+                if (i < 3) weigh(x, i + 1, 2 * dt, 2 * dt + 2, f, base, sum, w);
             }
         }
-        if (b + 1 < whole) {
-            store(buf ^ 1);
-            ks = ks_next;
-            vs = vs_next;
-        }
+        l = fmaf(sum, __builtin_amdgcn_exp2f(-shift), l);
         __syncthreads();
     }
     if (has_tail) {
@@ -886,15 +920,19 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_chunk_q8_kernel(const Chun
             f32x16 x[2];
             scores(0, x);
             if (smax == 0.0f) smax = 1.0f;
-            soften(x, tail_b, a.scale_log2, __builtin_amdgcn_logf(DQ_P_SCALE / smax), 1.0f);
+            float f = a.scale_log2, shift = __builtin_amdgcn_logf(DQ_P_SCALE / smax);
+            ready(x, tail_b, f, shift, 1.0f);
+            const float base = (m == -INFINITY ? 0.0f : m) - shift;
+            float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
+                float w[8];
+                weigh(x, i, 0, 8, f, base, sum, w);
                 bf16x8 ph, pl;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const float p = x[i >> 1][8 * (i & 1) + j];
-                    ph[j] = (__bf16)p;
-                    pl[j] = (__bf16)(p - (float)ph[j]);
+                    ph[j] = (__bf16)w[j];
+                    pl[j] = (__bf16)(w[j] - (float)ph[j]);
                 }
 #pragma unroll
                 for (int dt = 0; dt < 4; ++dt) {
@@ -903,6 +941,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_chunk_q8_kernel(const Chun
                     o[dt] = mfma_bf16(v, pl, o[dt]);
                 }
             }
+            l = fmaf(sum, __builtin_amdgcn_exp2f(-shift), l);
         }
     }
     l = xor_sum<32>(l);
