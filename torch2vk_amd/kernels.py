@@ -1661,22 +1661,67 @@ def _q8_here(cache: KVCacheQ8, names: str, *tensors: torch.Tensor | None) -> Non
     """Everything of a call is on the current device, on whose current stream it is launched."""
     if not isinstance(cache, KVCacheQ8):
         raise TypeError(f"cache must be a KVCacheQ8, got {type(cache).__name__}")
-    at = cache.at
-    if at != torch._C._cuda_getDevice():
-        raise ValueError(f"the cache is on cuda:{at}, the current device is cuda:{torch.cuda.current_device()}")
-    for i, t in enumerate(tensors):
-        if t is not None and not (isinstance(t, torch.Tensor) and t.get_device() == at):
-            name = names.split()[i]
-            if not isinstance(t, torch.Tensor):
-                raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
-            raise ValueError(f"{name} is on {t.device}, the cache on cuda:{at}")
+    if cache.at != torch._C._cuda_getDevice():
+        raise ValueError(f"the cache is on cuda:{cache.at}, the current device is cuda:{torch.cuda.current_device()}")
+    for name, t in zip(names.split(), tensors):
+        if t is not None and not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+        if t is not None and t.get_device() != cache.at:
+            raise ValueError(f"{name} is on {t.device}, the cache on cuda:{cache.at}")
 
 
-def _q8_ints(t: torch.Tensor | None, name: str, n_seq: int) -> None:
-    if t is None or t.dtype is torch.int32 and t.numel() == n_seq and t.is_contiguous():
-        return
-    _check(t, name, torch.int32, align=4)
-    raise ValueError(f"{name} must have one entry for each of {n_seq} sequences, got {tuple(t.shape)}")
+def _q8_plain(t: torch.Tensor | None, dtype: torch.dtype, n: int, at: int) -> bool:
+    """A contiguous tensor of n elements on device ``at``, or none."""
+    return t is None or t.dtype is dtype and t.numel() == n and t.get_device() == at and t.is_contiguous()
+
+
+def _q8_columns(t: torch.Tensor, rows: int, width: int, at: int) -> int:
+    """The row stride of fp32 [rows, width] column blocks on device ``at`` with distinct rows, or 0."""
+    if t.dtype is torch.float32 and t.get_device() == at and t.shape == (rows, width):
+        row, one = t.stride()
+        if one == 1 and (row >= width or rows <= 1):
+            return row if row > width else width
+    return 0
+
+
+# What the fast checks of a call refuse is looked at again here, and named.
+
+
+def _q8_refuse_ints(n_seq: int, **tensors: torch.Tensor | None) -> None:
+    for name, t in tensors.items():
+        if t is not None:
+            _check(t, name, torch.int32, align=4)
+            if t.numel() != n_seq:
+                raise ValueError(f"{name} must have one entry for each of {n_seq} sequences, got {tuple(t.shape)}")
+
+
+def _q8_refuse_rows(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: KVCacheQ8, rows: int,
+                    q_norm_weight: torch.Tensor | None, k_norm_weight: torch.Tensor | None) -> None:
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        _check_strided(t, name, torch.float32)
+        if t.dim() != 2 or t.shape[0] != rows or t.shape[1] % 128:
+            raise ValueError(f"{name} must be fp32 [{rows}, heads * 128], got {tuple(t.shape)}")
+        if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+            raise ValueError(f"{name} must hold distinct rows")
+    if k.shape[1] != cache.nk * 128 or v.shape[1] != cache.nk * 128:
+        raise ValueError(f"k and v must have the cache's {cache.nk} heads")
+    if (q_norm_weight is None) != (k_norm_weight is None):
+        raise ValueError("pass both q and k norm weights or neither")
+    for t, name in ((q_norm_weight, "q_norm_weight"), (k_norm_weight, "k_norm_weight")):
+        if t is not None:
+            _check(t, name, torch.float32, align=4)
+            if t.numel() != 128:
+                raise ValueError(f"{name} must have 128 elements")
+
+
+def _q8_refuse_weights(cache: KVCacheQ8, weights: torch.Tensor | None, weights_out: torch.Tensor | None) -> None:
+    if weights is None and weights_out is not None:
+        raise ValueError("weights_out needs weights")
+    for t, name in ((weights, "weights"), (weights_out, "weights_out")):
+        if t is not None:
+            _check(t, name, torch.float32, align=4)
+            if tuple(t.shape) != (cache.n_seq, cache.nk, cache.s_cap):
+                raise ValueError(f"{name} must be fp32 {(cache.n_seq, cache.nk, cache.s_cap)}, got {tuple(t.shape)}")
 
 
 def _q8_heads(nh: int, nk: int) -> None:
@@ -1684,48 +1729,13 @@ def _q8_heads(nh: int, nk: int) -> None:
         raise ValueError(f"{nh} q heads over {nk} KV heads: 1 to {KV_Q8_MAX_GROUP} for each are built")
 
 
-def _q8_rows(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: KVCacheQ8, rows: int,
-             q_norm_weight: torch.Tensor | None, k_norm_weight: torch.Tensor | None) -> tuple[int, int, int, int]:
-    """q heads of fp32 [rows, heads * 128] column blocks, and their row strides."""
-    shape, width = q.shape, cache.nk * 128
-    q_width = shape[1] if len(shape) == 2 else 0
-    strides = []
-    for t, name, cols in ((q, "q", q_width), (k, "k", width), (v, "v", width)):
-        stride = t.stride()
-        if (t.dtype is not torch.float32 or t.shape != (rows, cols) or stride[1] != 1 or cols % 128
-                or stride[0] < cols and rows > 1):
-            _check_strided(t, name, torch.float32)
-            if t.dim() != 2 or t.shape[0] != rows or t.shape[1] % 128:
-                raise ValueError(f"{name} must be fp32 [{rows}, heads * 128], got {tuple(t.shape)}")
-            if t.shape[1] != cols:
-                raise ValueError(f"k and v must have the cache's {cache.nk} heads")
-            raise ValueError(f"{name} must hold distinct rows")
-        strides.append(max(stride[0], cols))
-    nh = q_width // 128
-    _q8_heads(nh, cache.nk)
-    if q_norm_weight is None and k_norm_weight is None:
-        return nh, *strides
-    if q_norm_weight is None or k_norm_weight is None:
-        raise ValueError("pass both q and k norm weights or neither")
-    for t, name in ((q_norm_weight, "q_norm_weight"), (k_norm_weight, "k_norm_weight")):
-        _check(t, name, torch.float32, align=4)
-        if t.numel() != 128:
-            raise ValueError(f"{name} must have 128 elements")
-    return nh, *strides
-
-
-def _q8_weights(cache: KVCacheQ8, weights: torch.Tensor | None,
-                weights_out: torch.Tensor | None) -> torch.Tensor | None:
+def _q8_weights_ok(cache: KVCacheQ8, weights: torch.Tensor | None, weights_out: torch.Tensor | None) -> bool:
     if weights is None:
-        if weights_out is not None:
-            raise ValueError("weights_out needs weights")
-        return None
-    out = weights if weights_out is None else weights_out
-    for t, name in ((weights, "weights"), (out, "weights_out")):
-        _check(t, name, torch.float32, align=4)
-        if tuple(t.shape) != (cache.n_seq, cache.nk, cache.s_cap):
-            raise ValueError(f"{name} must be fp32 {(cache.n_seq, cache.nk, cache.s_cap)}, got {tuple(t.shape)}")
-    return out
+        return weights_out is None
+    shape = (cache.n_seq, cache.nk, cache.s_cap)
+    return (weights.shape == shape and _q8_plain(weights, torch.float32, weights.numel(), cache.at)
+            and (weights_out is None or weights_out.shape == shape
+                 and _q8_plain(weights_out, torch.float32, weights_out.numel(), cache.at)))
 
 
 def qk_norm_rope_cache_q8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_out: torch.Tensor, cache: KVCacheQ8,
@@ -1736,24 +1746,37 @@ def qk_norm_rope_cache_q8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_o
     [n_seq * n, nh, 128], k and v into the cache behind the ``lengths`` tokens that it holds.  q, k, v fp32
     [n_seq * n, heads * 128] with unit column stride.  ``counts``: new tokens of each sequence, its first rows (all n when
     None).  Token p stands at position p + rope_offsets.  ``lengths`` is not advanced."""
-    _q8_here(cache, "q k v q_out lengths counts rope_offsets q_norm_weight k_norm_weight", q, k, v, q_out, lengths, counts,
-             rope_offsets, q_norm_weight, k_norm_weight)
-    n_seq = cache.n_seq
-    n_rows = q.shape[0] if q.dim() else 0
-    if n_rows % n_seq:
-        raise ValueError(f"{n_rows} rows do not split into {n_seq} sequences")
-    nh, qr, kr, vr = _q8_rows(q, k, v, cache, n_rows, q_norm_weight, k_norm_weight)
-    _check(q_out, "q_out", torch.bfloat16, align=4)
-    if q_out.numel() != n_rows * nh * 128:
-        raise ValueError(f"q_out must hold [{n_rows}, {nh}, 128]")
-    _q8_ints(lengths, "lengths", n_seq)
-    _q8_ints(counts, "counts", n_seq)
-    _q8_ints(rope_offsets, "rope_offsets", n_seq)
-    if n_rows == 0:
+    try:
+        n_seq, nk, at = cache.n_seq, cache.nk, cache.at
+        rows, width = q.shape
+        qr, kr, vr = _q8_columns(q, rows, width, at), _q8_columns(k, rows, nk * 128, at), _q8_columns(v, rows, nk * 128, at)
+        ok = (at == torch._C._cuda_getDevice() and qr and kr and vr and width % 128 == 0 and rows % n_seq == 0
+              and _q8_plain(q_out, torch.bfloat16, rows * width, at) and q_out is not None
+              and lengths is not None and _q8_plain(lengths, torch.int32, n_seq, at)
+              and _q8_plain(counts, torch.int32, n_seq, at) and _q8_plain(rope_offsets, torch.int32, n_seq, at)
+              and _q8_plain(q_norm_weight, torch.float32, 128, at) and _q8_plain(k_norm_weight, torch.float32, 128, at)
+              and (q_norm_weight is None) == (k_norm_weight is None))
+    except (AttributeError, ValueError):
+        ok = False
+    if not ok:
+        _q8_here(cache, "q k v q_out lengths counts rope_offsets q_norm_weight k_norm_weight", q, k, v, q_out, lengths,
+                 counts, rope_offsets, q_norm_weight, k_norm_weight)
+        rows = q.shape[0] if q.dim() else 0
+        if rows % cache.n_seq:
+            raise ValueError(f"{rows} rows do not split into {cache.n_seq} sequences")
+        _q8_refuse_rows(q, k, v, cache, rows, q_norm_weight, k_norm_weight)
+        _check(q_out, "q_out", torch.bfloat16, align=4)
+        if q_out.numel() != q.numel():
+            raise ValueError(f"q_out must hold [{rows}, {q.shape[1] // 128}, 128]")
+        _check(lengths, "lengths", torch.int32, align=4)
+        _q8_refuse_ints(cache.n_seq, lengths=lengths, counts=counts, rope_offsets=rope_offsets)
+        raise ValueError("the tensors of a call must be on one device")
+    _q8_heads(width // 128, nk)
+    if rows == 0:
         return q_out
-    call("t2h_qk_norm_rope_cache_q8", ptr(q), qr, ptr(k), kr, ptr(v), vr, ptr(q_norm_weight), ptr(k_norm_weight), eps,
-         theta, ptr(lengths), ptr(counts), ptr(rope_offsets), n_rows // n_seq, n_seq, nh, cache.nk, 128, ptr(q_out),
-         cache.ptrs, cache.s_cap, stream_handle())
+    call("t2h_qk_norm_rope_cache_q8", q.data_ptr(), qr, k.data_ptr(), kr, v.data_ptr(), vr, ptr(q_norm_weight),
+         ptr(k_norm_weight), eps, theta, lengths.data_ptr(), ptr(counts), ptr(rope_offsets), rows // n_seq, n_seq,
+         width // 128, nk, 128, q_out.data_ptr(), cache.ptrs, cache.s_cap, stream_handle())
     return q_out
 
 
@@ -1777,20 +1800,37 @@ def attn_decode_q8(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, ca
     behind the ``lengths`` cached tokens, then attention over them all; out bf16 [n_seq, nh, 128].  ``weights`` fp32
     [n_seq, nk, s_cap]: each cached token's softmax weight, summed over the KV head's q heads, is added (in place, or into
     ``weights_out``).  ``lengths`` is not advanced."""
-    _q8_here(cache, "q new_k new_v output lengths workspace rope_offsets q_norm_weight k_norm_weight weights weights_out", q,
-             k_new, v_new, out, lengths, workspace, rope_offsets, q_norm_weight, k_norm_weight, weights, weights_out)
-    n_seq = cache.n_seq
-    nh, qr, kr, vr = _q8_rows(q, k_new, v_new, cache, n_seq, q_norm_weight, k_norm_weight)
-    _check(out, "output", torch.bfloat16, align=4)
-    if out.numel() != n_seq * nh * 128:
-        raise ValueError(f"output must hold [{n_seq}, {nh}, 128]")
-    _q8_ints(lengths, "lengths", n_seq)
-    _q8_ints(rope_offsets, "rope_offsets", n_seq)
-    _check(workspace, "workspace", torch.uint8)
-    weights_out = _q8_weights(cache, weights, weights_out)
-    call("t2h_attn_decode_q8", ptr(q), qr, ptr(k_new), kr, ptr(v_new), vr, ptr(q_norm_weight), ptr(k_norm_weight), eps,
-         theta, ptr(lengths), ptr(rope_offsets), cache.ptrs, cache.s_cap, ptr(weights), ptr(weights_out), ptr(out),
-         n_seq, nh, cache.nk, 128, ptr(workspace), workspace.numel(), stream_handle())
+    try:
+        n_seq, nk, at = cache.n_seq, cache.nk, cache.at
+        width = q.shape[1]
+        qr = _q8_columns(q, n_seq, width, at)
+        kr, vr = _q8_columns(k_new, n_seq, nk * 128, at), _q8_columns(v_new, n_seq, nk * 128, at)
+        ok = (at == torch._C._cuda_getDevice() and qr and kr and vr and width % 128 == 0
+              and out is not None and _q8_plain(out, torch.bfloat16, n_seq * width, at)
+              and lengths is not None and _q8_plain(lengths, torch.int32, n_seq, at)
+              and workspace.dtype is torch.uint8 and workspace.get_device() == at and workspace.is_contiguous()
+              and _q8_plain(rope_offsets, torch.int32, n_seq, at)
+              and _q8_plain(q_norm_weight, torch.float32, 128, at) and _q8_plain(k_norm_weight, torch.float32, 128, at)
+              and (q_norm_weight is None) == (k_norm_weight is None) and _q8_weights_ok(cache, weights, weights_out))
+    except (AttributeError, IndexError):
+        ok = False
+    if not ok:
+        _q8_here(cache, "q new_k new_v output lengths workspace rope_offsets q_norm_weight k_norm_weight weights weights_out",
+                 q, k_new, v_new, out, lengths, workspace, rope_offsets, q_norm_weight, k_norm_weight, weights, weights_out)
+        _q8_refuse_rows(q, k_new, v_new, cache, cache.n_seq, q_norm_weight, k_norm_weight)
+        _check(out, "output", torch.bfloat16, align=4)
+        if out.numel() != q.numel():
+            raise ValueError(f"output must hold [{cache.n_seq}, {q.shape[1] // 128}, 128]")
+        _check(lengths, "lengths", torch.int32, align=4)
+        _q8_refuse_ints(cache.n_seq, lengths=lengths, rope_offsets=rope_offsets)
+        _check(workspace, "workspace", torch.uint8)
+        _q8_refuse_weights(cache, weights, weights_out)
+        raise ValueError("the tensors of a call must be on one device")
+    _q8_heads(width // 128, nk)
+    call("t2h_attn_decode_q8", q.data_ptr(), qr, k_new.data_ptr(), kr, v_new.data_ptr(), vr, ptr(q_norm_weight),
+         ptr(k_norm_weight), eps, theta, lengths.data_ptr(), ptr(rope_offsets), cache.ptrs, cache.s_cap, ptr(weights),
+         ptr(weights if weights_out is None else weights_out), out.data_ptr(), n_seq, width // 128, nk, 128,
+         workspace.data_ptr(), workspace.numel(), stream_handle())
     return out
 
 
@@ -1800,28 +1840,35 @@ def flash_attn_prefill_q8(q: torch.Tensor, cache: KVCacheQ8, lengths: torch.Tens
     """Causal attention of a chunk's queries over the 8-bit cache that :func:`qk_norm_rope_cache_q8` wrote it into (the
     same ``lengths`` and ``counts``): query t of q bf16 [n_seq, n, nh, 128] sees tokens 0 .. length + t; rows past a
     count give zeros.  ``weights`` as in :func:`attn_decode_q8`, of all the chunk's queries."""
-    _q8_here(cache, "q lengths output counts weights weights_out", q, lengths, out, counts, weights, weights_out)
-    _check(q, "q", torch.bfloat16)
-    if q.dim() != 4 or q.shape[0] != cache.n_seq or q.shape[3] != 128:
-        raise ValueError(f"q must be bf16 [{cache.n_seq}, n, nh, 128], got {tuple(q.shape)}")
-    n_seq, n, nh, _ = q.shape
-    _q8_heads(nh, cache.nk)
-    _q8_ints(lengths, "lengths", n_seq)
-    _q8_ints(counts, "counts", n_seq)
-    weights_out = _q8_weights(cache, weights, weights_out)
+    try:
+        n_seq, nk, at = cache.n_seq, cache.nk, cache.at
+        b, n, nh, d = q.shape
+        ok = (at == torch._C._cuda_getDevice() and b == n_seq and d == 128 and _q8_plain(q, torch.bfloat16, q.numel(), at)
+              and lengths is not None and _q8_plain(lengths, torch.int32, n_seq, at)
+              and _q8_plain(counts, torch.int32, n_seq, at) and _q8_weights_ok(cache, weights, weights_out)
+              and (out is None or out.shape == q.shape and _q8_plain(out, torch.bfloat16, q.numel(), at)))
+    except (AttributeError, ValueError):
+        ok = False
+    if not ok:
+        _q8_here(cache, "q lengths output counts weights weights_out", q, lengths, out, counts, weights, weights_out)
+        _check(q, "q", torch.bfloat16)
+        if q.dim() != 4 or q.shape[0] != cache.n_seq or q.shape[3] != 128:
+            raise ValueError(f"q must be bf16 [{cache.n_seq}, n, nh, 128], got {tuple(q.shape)}")
+        _check(lengths, "lengths", torch.int32, align=4)
+        _q8_refuse_ints(cache.n_seq, lengths=lengths, counts=counts)
+        _q8_refuse_weights(cache, weights, weights_out)
+        _check(out, "output", torch.bfloat16)
+        raise ValueError(f"output must be {tuple(q.shape)}, got {tuple(out.shape)}")
+    _q8_heads(nh, nk)
     if out is None:
         out = torch.empty_like(q)
-    _check(out, "output", torch.bfloat16)
-    if out.shape != q.shape:
-        raise ValueError(f"output must be {tuple(q.shape)}, got {tuple(out.shape)}")
     if n == 0:
         return out
-    nbytes = int(_lib.lib().t2h_flash_attn_prefill_q8_workspace_bytes(n, n_seq, nh, cache.nk, cache.s_cap,
-                                                                     int(weights is not None)))
+    nbytes = _lib.lib().t2h_flash_attn_prefill_q8_workspace_bytes(n, n_seq, nh, nk, cache.s_cap, int(weights is not None))
     workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-    call("t2h_flash_attn_prefill_q8", ptr(q), cache.ptrs, cache.s_cap, ptr(lengths), ptr(counts), ptr(weights),
-         ptr(weights_out), ptr(out), n, n_seq, nh, cache.nk, 128, float(scale or 0.0), ptr(workspace), nbytes,
-         stream_handle())
+    call("t2h_flash_attn_prefill_q8", q.data_ptr(), cache.ptrs, cache.s_cap, lengths.data_ptr(), ptr(counts), ptr(weights),
+         ptr(weights if weights_out is None else weights_out), out.data_ptr(), n, n_seq, nh, nk, 128, scale or 0.0,
+         workspace.data_ptr(), nbytes, stream_handle())
     return out
 
 
@@ -1830,18 +1877,22 @@ def kv_cache_q8_dequantize(cache: KVCacheQ8, lengths: torch.Tensor, k_out: torch
     """The cache's keys and values as bf16 [n_seq, s_cap, nk, 128], the layout of the other caches; zeros behind
     ``lengths``."""
     _q8_here(cache, "lengths k_out v_out", lengths, k_out, v_out)
-    _q8_ints(lengths, "lengths", cache.n_seq)
+    if lengths is None or not _q8_plain(lengths, torch.int32, cache.n_seq, cache.at):
+        _check(lengths, "lengths", torch.int32, align=4)
+        _q8_refuse_ints(cache.n_seq, lengths=lengths)
     shape = (cache.n_seq, cache.s_cap, cache.nk, 128)
-    outs = []
     for t, name in ((k_out, "k_out"), (v_out, "v_out")):
-        t = torch.empty(shape, dtype=torch.bfloat16, device=cache.k.device) if t is None else t
-        _check(t, name, torch.bfloat16)
-        if tuple(t.shape) != shape:
-            raise ValueError(f"{name} must be bf16 {shape}, got {tuple(t.shape)}")
-        outs.append(t)
-    call("t2h_kv_cache_q8_dequantize", cache.ptrs, cache.s_cap, ptr(lengths), cache.n_seq, cache.nk, 128, ptr(outs[0]),
-         ptr(outs[1]), stream_handle())
-    return outs[0], outs[1]
+        if t is not None:
+            _check(t, name, torch.bfloat16)
+            if tuple(t.shape) != shape:
+                raise ValueError(f"{name} must be bf16 {shape}, got {tuple(t.shape)}")
+    if k_out is None:
+        k_out = torch.empty(shape, dtype=torch.bfloat16, device=cache.k.device)
+    if v_out is None:
+        v_out = torch.empty(shape, dtype=torch.bfloat16, device=cache.k.device)
+    call("t2h_kv_cache_q8_dequantize", cache.ptrs, cache.s_cap, lengths.data_ptr(), cache.n_seq, cache.nk, 128,
+         k_out.data_ptr(), v_out.data_ptr(), stream_handle())
+    return k_out, v_out
 
 
 def kv_cache_q8_evict(cache: KVCacheQ8, lengths: torch.Tensor, weights: torch.Tensor, keep_blocks: int, *, sink: int = 0,
@@ -1867,7 +1918,8 @@ def kv_cache_q8_evict(cache: KVCacheQ8, lengths: torch.Tensor, weights: torch.Te
         raise ValueError(f"out holds {dest.s_cap} tokens, {KV_Q8_BLOCK * (keep_blocks + 1)} may stay")
     if weights_out is None:
         weights_out = weights
-    _q8_ints(lengths, "lengths", n_seq)
+    _check(lengths, "lengths", torch.int32, align=4)
+    _q8_refuse_ints(n_seq, lengths=lengths)
     for t, name, cap in ((weights, "weights", cache.s_cap), (weights_out, "weights_out", dest.s_cap)):
         _check(t, name, torch.float32, align=4)
         if tuple(t.shape) != (n_seq, nk, cap):
