@@ -218,6 +218,8 @@ def bind_model_tensors(decoder) -> ModelTensors:
     """Build the decode tensor sets over a Qwen3Decoder's weights, caches, residual stream and token state, and
     make them the ones the run_* functions use (the reference's model_tensors())."""
     global _MODEL
+    if decoder.kv_bits != 16:
+        raise NotImplementedError("the named operators read a bf16 KV cache")
     c = decoder.config
     dev = decoder.device
     bf, f32 = torch.bfloat16, torch.float32

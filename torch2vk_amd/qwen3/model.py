@@ -58,14 +58,26 @@ class Qwen3Decoder:
     for all of them (t2h_qwen3_decode_layers: the 8B and 0.6B shapes with Q4_K weights, v and down Q4_K or
     Q6_K as the uniform and Q4_K_M policies give them), or one launch per op (run_decode_layer, every shape and
     weight mix).  None (the default) picks the persistent kernel when it
-    applies: on MI355X it saves the launch and ramp of ~250 kernels per token."""
+    applies: on MI355X it saves the launch and ramp of ~250 kernels per token.
+
+    ``kv_bits`` 8 holds the KV cache in 8 bits (kernels.KVCacheQ8, one a layer): half the bytes an attention reads, for
+    contexts where those are most of a step; the layers run one launch per op.  Such a cache goes on from its length only:
+    ``start`` of a prefill is 0 or the tokens it holds, and step_logits and forward_masked are refused.  With
+    ``kv_weights`` it also keeps each token's accumulated attention weight, by which ``evict_cache`` cuts it down."""
 
     PREFILL_GRAPHS = 4  # captured prefill graphs kept (prefill_graphed)
 
     def __init__(self, weights: Qwen3Weights, *, max_positions: int, max_new_tokens: int, device=None,
                  persistent: bool | None = None,
-                 kv_cache: tuple[torch.Tensor, torch.Tensor] | None = None) -> None:
+                 kv_cache: tuple[torch.Tensor, torch.Tensor] | None = None, kv_bits: int = 16,
+                 kv_weights: bool = False) -> None:
         c = weights.config
+        if kv_bits not in (8, 16):
+            raise ValueError(f"kv_bits must be 8 or 16, got {kv_bits}")
+        if kv_weights and kv_bits != 8:
+            raise ValueError("kv_weights are kept for an 8-bit cache")
+        if kv_bits == 8 and (persistent or kv_cache is not None):
+            raise NotImplementedError("an 8-bit KV cache is the decoder's own and has no persistent kernel")
         self.config: Qwen3Config = c
         self.weights = weights
         self.types = dict(weights.types)
@@ -74,7 +86,17 @@ class Qwen3Decoder:
         self.device = dev
         self.max_positions = max_positions
         bf, f32 = torch.bfloat16, torch.float32
-        if kv_cache is None:
+        self.kv_bits = kv_bits
+        self.kv_weights: list[torch.Tensor] | None = None
+        if kv_bits == 8:
+            self.k_cache = self.v_cache = None
+            self.kv = [kernels.kv_cache_q8(1, max_positions, c.kv_heads, c.head_dim, dev) for _ in range(c.layers)]
+            self.rope_offset = torch.zeros(1, dtype=torch.int32, device=dev)  # tokens evicted: position - place in the cache
+            self.chunk_start = torch.zeros(1, dtype=torch.int32, device=dev)
+            if kv_weights:
+                self.kv_weights = [torch.zeros(1, c.kv_heads, self.kv[0].s_cap, dtype=f32, device=dev)
+                                   for _ in range(c.layers)]
+        elif kv_cache is None:
             self.k_cache = torch.zeros(c.layers, max_positions, c.kv_heads, c.head_dim, dtype=bf, device=dev)
             self.v_cache = torch.zeros_like(self.k_cache)
         else:
@@ -92,7 +114,11 @@ class Qwen3Decoder:
         self.v = torch.zeros(c.kv_dim, dtype=f32, device=dev)
         self.attn = torch.zeros(c.q_dim, dtype=bf, device=dev)
         self.act = torch.zeros(c.mlp, dtype=bf, device=dev)
-        self.attn_ws = kernels.attn_decode_workspace(c.heads, c.kv_heads, c.head_dim, max_positions, dev)
+        if kv_bits == 8:
+            self.attn_ws = kernels.attn_decode_q8_workspace(1, c.heads, c.kv_heads, c.head_dim, self.kv[0].s_cap, dev,
+                                                            weights=kv_weights)
+        else:
+            self.attn_ws = kernels.attn_decode_workspace(c.heads, c.kv_heads, c.head_dim, max_positions, dev)
         self.partial_scores = torch.zeros(LM_HEAD_PARTIALS, dtype=f32, device=dev)
         self.partial_tokens = torch.zeros(LM_HEAD_PARTIALS, dtype=torch.int32, device=dev)
         self.next_token = torch.zeros(1, 1, dtype=torch.int64, device=dev)
@@ -119,6 +145,8 @@ class Qwen3Decoder:
 
     def _persistent_unsupported(self) -> str | None:
         c = self.config
+        if self.kv_bits == 8:
+            return "8-bit KV cache"
         if not kernels.decode_layers_supported(c.hidden, c.mlp, c.heads, c.kv_heads, c.head_dim):
             return f"shape hidden={c.hidden} mlp={c.mlp} heads={c.heads}/{c.kv_heads} d={c.head_dim} not built"
         if self.max_positions > 8192:
@@ -157,6 +185,8 @@ class Qwen3Decoder:
         self.stopped.zero_()
         self.done.zero_()
         self.generated.fill_(-1)
+        if self.kv_bits == 8 and position == 0:
+            self.rope_offset.zero_()
         if token is not None:
             self.next_token.fill_(token)
 
@@ -203,6 +233,12 @@ class Qwen3Decoder:
 
     def _attention(self, layer_idx: int) -> None:
         c, p = self.config, f"layers.{layer_idx}."
+        if self.kv_bits == 8:
+            kernels.attn_decode_q8(self.q.view(1, -1), self.k.view(1, -1), self.v.view(1, -1), self.kv[layer_idx], self.attn,
+                                   self.position, self.attn_ws, theta=c.rope_theta, rope_offsets=self.rope_offset,
+                                   q_norm_weight=self._n(p + "q_norm"), k_norm_weight=self._n(p + "k_norm"), eps=c.rms_eps,
+                                   weights=None if self.kv_weights is None else self.kv_weights[layer_idx])
+            return
         kernels.attn_decode(self.q, self.k, self.v, self.k_cache[layer_idx], self.v_cache[layer_idx], self.attn,
                             self.position, self.attn_ws, q_norm_weight=self._n(p + "q_norm"),
                             k_norm_weight=self._n(p + "k_norm"), theta=c.rope_theta, eps=c.rms_eps)
@@ -257,6 +293,8 @@ class Qwen3Decoder:
         restored afterwards, so a finished generation can be re-examined step by step."""
         if (token is None) == (embed is None):
             raise ValueError("pass token or embed")
+        if self.kv_bits == 8:
+            raise NotImplementedError("an 8-bit KV cache goes on from its length only")
         if not 0 <= position < self.max_positions:
             raise ValueError(f"position {position} outside the KV capacity {self.max_positions}")
         saved = [t.clone() for t in (self.position, self.next_token, self.h, self.k_cache[:, position],
@@ -330,12 +368,15 @@ class Qwen3Decoder:
         return self._graphs[steps]
 
     def _save_state(self):
-        return [t.clone() for t in (self.position, self.length, self.stopped, self.done, self.next_token,
-                                    self.generated)]
+        return [t.clone() for t in self._state()]
+
+    def _state(self) -> list[torch.Tensor]:
+        """What a step changes and a repeated one would change again (not the cache rows, which it writes anew)."""
+        return [self.position, self.length, self.stopped, self.done, self.next_token, self.generated,
+                *(self.kv_weights or ())]
 
     def _restore_state(self, saved) -> None:
-        for dst, src in zip((self.position, self.length, self.stopped, self.done, self.next_token, self.generated),
-                            saved):
+        for dst, src in zip(self._state(), saved):
             dst.copy_(src)
 
     def run_steps(self, n: int, steps_per_graph: int = 8, use_graph: bool = True) -> None:
@@ -398,16 +439,21 @@ class Qwen3Decoder:
             q, k, v = (kernels.quantized_linear(x, self._w(p + nm), t[p + nm], out_dtype=torch.float32)
                        for nm in ("q", "k", "v"))
         qb = torch.empty(n, c.heads, c.head_dim, dtype=torch.bfloat16, device=self.device)
-        kernels.qk_norm_rope_cache(q, k, v, qb, self.k_cache[i], self.v_cache[i], start,
-                                   q_norm_weight=self._n(p + "q_norm"), k_norm_weight=self._n(p + "k_norm"),
-                                   theta=c.rope_theta, eps=c.rms_eps)
-        keys = self.k_cache[i, :start + n].unsqueeze(0)
-        vals = self.v_cache[i, :start + n].unsqueeze(0)
-        if mask is None:
-            attn = kernels.flash_attn_prefill(qb.unsqueeze(0), keys, vals, causal=True, causal_offset=start)
+        norms = dict(q_norm_weight=self._n(p + "q_norm"), k_norm_weight=self._n(p + "k_norm"), theta=c.rope_theta,
+                     eps=c.rms_eps)
+        if self.kv_bits == 8:  # at chunk_start, which holds ``start``
+            kernels.qk_norm_rope_cache_q8(q, k, v, qb, self.kv[i], self.chunk_start, rope_offsets=self.rope_offset, **norms)
+            attn = kernels.flash_attn_prefill_q8(qb.unsqueeze(0), self.kv[i], self.chunk_start,
+                                                 weights=None if self.kv_weights is None else self.kv_weights[i])
         else:
-            attn = kernels.flash_attn_prefill(qb.unsqueeze(0), keys, vals, causal=False, mask=mask,
-                                              mask_tiles=mask_tiles)
+            kernels.qk_norm_rope_cache(q, k, v, qb, self.k_cache[i], self.v_cache[i], start, **norms)
+            keys = self.k_cache[i, :start + n].unsqueeze(0)
+            vals = self.v_cache[i, :start + n].unsqueeze(0)
+            if mask is None:
+                attn = kernels.flash_attn_prefill(qb.unsqueeze(0), keys, vals, causal=True, causal_offset=start)
+            else:
+                attn = kernels.flash_attn_prefill(qb.unsqueeze(0), keys, vals, causal=False, mask=mask,
+                                                  mask_tiles=mask_tiles)
         kernels.quantized_linear(attn.view(n, c.q_dim), self._w(p + "o"), t[p + "o"], out=h, residual=h)
         x = kernels.rms_norm(h, self._n(p + "post_norm"), out=x, eps=c.rms_eps)
         if t[p + "gate"] == t[p + "up"] and n > kernels.GEMV_MAX_ROWS:
@@ -426,6 +472,8 @@ class Qwen3Decoder:
         of every position -> fp32 [T, hidden].  The layers' K/V go to rows 0..T-1 of the KV cache.  The same
         kernels as the chunked prefill: matrix-core GEMMs of each weight's type and masked flash attention."""
         c = self.config
+        if self.kv_bits == 8:
+            raise NotImplementedError("masked attention reads a bf16 KV cache")
         e = embeds.to(device=self.device, dtype=torch.float32).reshape(-1, c.hidden)
         t_len = e.shape[0]
         if t_len > self.max_positions:
@@ -464,6 +512,8 @@ class Qwen3Decoder:
         self.reset(position=start)
         for c0 in range(0, total, chunk):
             h = e[c0:c0 + chunk].clone()
+            if self.kv_bits == 8:
+                self.chunk_start.fill_(start + c0)
             for i in range(c.layers):
                 self._prefill_layer(i, h, start + c0)
         self.h.copy_(h[-1])
@@ -526,6 +576,21 @@ class Qwen3Decoder:
                 self.position.add_(1)
         self.run_lm_head_select()
         self.run_token_store(advance=True)
+
+    def evict_cache(self, keep_blocks: int, *, sink: int = 4, recent: int = 64) -> list[torch.Tensor]:
+        """Between two steps: every layer's KV heads keep 64 * keep_blocks of their whole blocks' tokens, the first
+        ``sink``, the last ``recent`` and those of most accumulated attention weight (kernels.kv_cache_q8_evict), in place, so
+        that captured graphs go on.  The positions of the tokens that follow stay what they would have been.  Returns each
+        layer's kept tokens, int32 [1, kv_heads, 64 * keep_blocks] of places in the cache before, -1 behind them."""
+        if self.kv_weights is None:
+            raise ValueError("eviction goes by accumulated weights: kv_bits=8, kv_weights=True")
+        kept, lengths = [], self.position
+        for cache, w in zip(self.kv, self.kv_weights):
+            k, lengths = kernels.kv_cache_q8_evict(cache, self.position, w, keep_blocks, sink=sink, recent=recent)
+            kept.append(k)
+        self.rope_offset += self.position - lengths
+        self.position.copy_(lengths)
+        return kept
 
     def _check_budget(self, prompt_len: int, max_new_tokens: int) -> None:
         if max_new_tokens > self.generated.numel():
