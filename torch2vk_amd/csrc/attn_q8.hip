@@ -60,15 +60,22 @@ struct DecodeQ8Args {
     int rope;
 };
 
+// What units are found from: the lengths before a call of up to n new tokens a sequence.
+struct UnitsOf {
+    const int32_t* lengths;
+    const int32_t* counts;
+    uint32_t n, n_seq, nb, nk;
+
+    __device__ __forceinline__ int blocks(uint32_t seq) const {
+        if (counts && counts[seq] <= 0) return 0;
+        return (q8_span(lengths, counts, seq, n, nb).end + Q8_BLOCK - 1) / Q8_BLOCK;
+    }
+};
+
 struct DecodeUnit {
     uint32_t seq, first, count;  // the sequence, its first unit and how many it has
     int chunk, blocks, len;      // blocks a unit, the sequence's blocks and its length before the call
 };
-
-__device__ __forceinline__ int dq_blocks(const DecodeQ8Args& a, uint32_t seq) {
-    const int len = a.lengths[seq];
-    return len < 0 ? 0 : len >= (int)(a.c.nb * Q8_BLOCK) ? (int)a.c.nb : len / Q8_BLOCK + 1;
-}
 
 __device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v) {
     const int lane = threadIdx.x & 63;
@@ -93,24 +100,24 @@ __host__ __device__ __forceinline__ uint32_t dq_chunk(uint64_t total, uint32_t n
 
 // The sequence that unit `unit` belongs to (by_seq false), or sequence `unit` itself; false where there is none.  A
 // sequence without blocks has one unit, which writes its zeros.
-__device__ bool dq_find(const DecodeQ8Args& a, uint32_t unit, bool by_seq, DecodeUnit& u) {
+__device__ bool dq_find(const UnitsOf& a, uint32_t unit, bool by_seq, DecodeUnit& u) {
     const uint32_t lane = threadIdx.x & 63;
     if (a.n_seq == 1) {
-        u.blocks = dq_blocks(a, 0);
-        u.chunk = (int)dq_chunk((uint64_t)u.blocks, a.c.nk);
+        u.blocks = a.blocks(0);
+        u.chunk = (int)dq_chunk((uint64_t)u.blocks, a.nk);
         u.seq = u.first = 0;
         u.count = u.blocks ? (uint32_t)((u.blocks + u.chunk - 1) / u.chunk) : 1u;
         u.len = a.lengths[0];
         return by_seq || unit < u.count;
     }
     uint32_t total = 0;
-    for (uint32_t i = lane; i < a.n_seq; i += 64) total += (uint32_t)dq_blocks(a, i);
+    for (uint32_t i = lane; i < a.n_seq; i += 64) total += (uint32_t)a.blocks(i);
     total = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan_u32(total), 63);
-    u.chunk = (int)dq_chunk(total, a.c.nk);
+    u.chunk = (int)dq_chunk(total, a.nk);
     uint32_t before = 0;
     for (uint32_t base = 0; base < a.n_seq; base += 64) {
         const uint32_t i = base + lane;
-        const uint32_t n = i < a.n_seq ? (uint32_t)dq_blocks(a, i) : 0u;
+        const uint32_t n = i < a.n_seq ? (uint32_t)a.blocks(i) : 0u;
         const uint32_t mine = i < a.n_seq ? (n ? (n + u.chunk - 1) / u.chunk : 1u) : 0u;
         const uint32_t upto = before + wave_scan_u32(mine);
         const uint64_t hit = by_seq ? __ballot(i == unit) : __ballot(unit >= upto - mine && unit < upto);
@@ -119,7 +126,7 @@ __device__ bool dq_find(const DecodeQ8Args& a, uint32_t unit, bool by_seq, Decod
             u.seq = base + at;
             u.count = (uint32_t)__builtin_amdgcn_readlane((int)mine, at);
             u.first = (uint32_t)__builtin_amdgcn_readlane((int)(upto - mine), at);
-            u.blocks = dq_blocks(a, u.seq);
+            u.blocks = a.blocks(u.seq);
             u.len = a.lengths[u.seq];
             return true;
         }
@@ -174,7 +181,7 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_decode_q8_kernel(const 
     const uint32_t h = blockIdx.x % a.c.nk;
     const uint32_t unit = blockIdx.x / a.c.nk;
     DecodeUnit u;
-    if (!dq_find(a, unit, false, u)) return;  // (every wave of a thread block finds the same)
+    if (!dq_find({a.lengths, nullptr, 1, a.n_seq, a.c.nb, a.c.nk}, unit, false, u)) return;  // (every wave of a thread block finds the same)
     const int group = (int)a.group;
     uint32_t* const out = reinterpret_cast<uint32_t*>(a.out + ((size_t)u.seq * a.nh + h * group) * Q8_D);
     if (u.blocks == 0) {
@@ -602,7 +609,7 @@ __global__ __launch_bounds__(256) void attn_decode_q8_weights_kernel(const Decod
     const int end = len < 0 ? 0 : (len < cap ? len + 1 : cap);
     if (first >= end) return;
     DecodeUnit u;
-    dq_find(a, seq, true, u);
+    dq_find({a.lengths, nullptr, 1, a.n_seq, a.c.nb, a.c.nk}, seq, true, u);
     for (uint32_t g = wave; g < a.group; g += 4) {
         float M, L;
         dq_total(a, u, h, g, M, L);
@@ -1003,7 +1010,7 @@ __global__ __launch_bounds__(256) void attn_chunk_q8_merge_kernel(const ChunkQ8A
         }
 #pragma unroll
         for (uint32_t e = 0; e < BATCH; ++e) {
-            if (i0 + e >= a.splits) break;
+            if (i0 + e >= a.splits) ml[e].x = -INFINITY;
             const float now = fmaxf(M, ml[e].x), base = now == -INFINITY ? 0.0f : now;
             const float keep = __builtin_amdgcn_exp2f(M - base), f = __builtin_amdgcn_exp2f(ml[e].x - base);
             L = fmaf(L, keep, f * ml[e].y);
@@ -1148,6 +1155,301 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_q8_weights_kernel(const Chu
         }
 }
 
+// ---------------------------------------------------------------------------------------------------- few rows --
+//
+// Up to 32 rows of a KV head (a few drafted tokens): bound by memory like a single token, and read like one, in units of
+// blocks that a wave takes whole; the rows are the columns of one or two 16 x 16 x 32 products, each with its own last
+// token.  Their queries are bf16 already, so fp16 holds them in one term.  A second kernel joins a sequence's units.
+template <int CT>
+__global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_rows_q8_kernel(const ChunkQ8Args a) {
+    constexpr int COLS = 16 * CT;
+    // the queries (fp16 with the largest value in [1, 2), and bf16 as they came), then the waves' outputs
+    __shared__ __align__(16) float room[DQ_WAVES * COLS * DQ_ROW];
+    __shared__ float qf[COLS], wml[DQ_WAVES][COLS][2];
+    _Float16* const qs = reinterpret_cast<_Float16*>(room);
+    uint16_t* const qb = reinterpret_cast<uint16_t*>(room) + COLS * DQ_QROW;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t h = blockIdx.x % a.c.nk, unit = blockIdx.x / a.c.nk;
+    DecodeUnit u;
+    if (!dq_find({a.lengths, a.counts, a.n, a.n_seq, a.c.nb, a.c.nk}, unit, false, u)) return;
+    const int group = (int)a.group, rows = (int)a.n * group;
+    const Q8Span s = q8_span(a.lengths, a.counts, u.seq, a.n, a.c.nb);
+    int count = a.counts ? a.counts[u.seq] : (int)a.n;
+    count = u.blocks == 0 ? 0 : (count < (int)a.n ? count : (int)a.n);
+    const int b0 = (int)(unit - u.first) * u.chunk;
+    const int b1 = b0 + u.chunk < u.blocks ? b0 + u.chunk : u.blocks;
+    const int c = lane & 15, g4 = lane >> 4;
+    const int tail_b = s.end % Q8_BLOCK ? s.end / Q8_BLOCK : -1;
+    const bool has_tail = tail_b >= b0 && tail_b < b1;
+    const int len = min(u.len, (int)(a.c.nb * Q8_BLOCK));
+    auto row_at = [&](int row) {  // row t * group + g in q and out
+        return (((size_t)u.seq * a.n + row / group) * a.nh + h * group + row % group) * Q8_D;
+    };
+    uint32_t qw[COLS / DQ_WAVES];
+#pragma unroll
+    for (int i = 0; i < COLS / DQ_WAVES; ++i) {
+        const int row = wave + DQ_WAVES * i;
+        qw[i] = row < count * group ? reinterpret_cast<const uint32_t*>(a.q + row_at(row))[lane] : 0u;
+    }
+    float smax = 0.0f;
+    for (int i = b0 + wave + DQ_WAVES * lane; i < b1; i += DQ_WAVES * 64)
+        if (i != tail_b) smax = fmaxf(smax, a.c.vs[a.c.scale_at(u.seq, (uint32_t)i, h)]);
+    const int krow = ((c >> 2) * 16 + (c & 3)) * Q8_D + g4 * 16;
+    const int vrow = c * Q8_BLOCK + g4 * 16;
+    uint4 kr[8], vr[8];
+    float ks = 0.0f, vs = 0.0f;
+    auto load_k = [&](int b) {
+        const int8_t* p = a.c.k + a.c.block_at(u.seq, (uint32_t)b, h) + krow;
+#pragma unroll
+        for (int n = 0; n < 8; ++n) kr[n] = load_nt_u4(p + (n >> 1) * 4 * Q8_D + (n & 1) * 64);
+        ks = a.c.ks[a.c.scale_at(u.seq, (uint32_t)b, h)];
+    };
+    auto load_v = [&](int b) {
+        const int8_t* p = a.c.v + a.c.block_at(u.seq, (uint32_t)b, h) + vrow;
+#pragma unroll
+        for (int n = 0; n < 8; ++n) vr[n] = load_nt_u4(p + n * 16 * Q8_BLOCK);
+        vs = a.c.vs[a.c.scale_at(u.seq, (uint32_t)b, h)];
+    };
+    int b = b0 + wave;
+    if (b < b1 && b != tail_b) {
+        load_k(b);
+        load_v(b);
+    }
+#pragma unroll
+    for (int i = 0; i < COLS / DQ_WAVES; ++i) {  // dims 2 lane, 2 lane + 1
+        const int row = wave + DQ_WAVES * i;
+        const float x = __uint_as_float(qw[i] << 16), y = __uint_as_float(qw[i] & 0xffff0000u);
+        uint32_t e = __float_as_uint(wave_max(fmaxf(fabsf(x), fabsf(y)))) >> 23;
+        e = e < 1 ? 1 : (e > 253 ? 253 : e);
+        const float down = __uint_as_float((254u - e) << 23);
+        const f16x2_t two = {(_Float16)(x * down), (_Float16)(y * down)};
+        *reinterpret_cast<f16x2_t*>(qs + row * DQ_QROW + 2 * lane) = two;
+        *reinterpret_cast<uint32_t*>(qb + row * DQ_QROW + 2 * lane) = qw[i];
+        if (lane == 0) qf[row] = __uint_as_float(e << 23) * a.scale_log2;
+    }
+    __syncthreads();
+    smax = wave_max(smax);
+    float m[CT], l[CT], qfac[CT];
+    int last[CT];  // the last token that the column sees
+    f32x4 o[CT][8];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+        const int row = 16 * ct + c;
+        m[ct] = -INFINITY;
+        l[ct] = 0.0f;
+        qfac[ct] = qf[row];
+        last[ct] = row < count * group ? min(len + row / group, s.end - 1) : -1;
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) o[ct][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    const int first = count > 0 ? min(len, s.end - 1) : -1;  // what every row sees
+
+    // scores of key tiles t0 .. of a block -> weights; tokens 16 g4 + 4 t + i
+    auto soften = [&](auto& x, int ct, int t0, float f, int b) {
+        constexpr int N = sizeof(x) / sizeof(x[0]);
+        const int mine = last[ct] - b * Q8_BLOCK;
+        float top = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < N; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[t][i] = 16 * g4 + 4 * (t0 + t) + i > mine ? -INFINITY : x[t][i] * f;
+                top = fmaxf(top, x[t][i]);
+            }
+        top = fmaxf(m[ct], xor_max<32>(xor_max<16>(top)));
+        const float base = top == -INFINITY ? 0.0f : top;
+        const float keep = __builtin_amdgcn_exp2f(m[ct] - base);
+        float sum = 0.0f;
+#pragma unroll
+        for (int t = 0; t < N; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[t][i] = __builtin_amdgcn_exp2f(x[t][i] - base);
+                sum += x[t][i];
+            }
+        l[ct] = fmaf(l[ct], keep, sum);
+        m[ct] = top;
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) o[ct][dt] *= keep;
+    };
+
+    for (; b < b1 && b != tail_b; b += DQ_WAVES) {
+        f32x4 x[CT][4];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) x[ct][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            f16x8 q[CT][2];
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    q[ct][i] = *reinterpret_cast<const f16x8*>(qs + (16 * ct + c) * DQ_QROW + 64 * j + 16 * g4 + 8 * i);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const uint4 kk = kr[2 * t + j];
+                const f16x8 k0 = codes_f16x8(kk.x, kk.y), k1 = codes_f16x8(kk.z, kk.w);
+#pragma unroll
+                for (int ct = 0; ct < CT; ++ct) {
+                    x[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q[ct][0], x[ct][t], 0, 0, 0);
+                    x[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, q[ct][1], x[ct][t], 0, 0, 0);
+                }
+            }
+        }
+        const float fk = ks;
+        const int next = b + DQ_WAVES;
+        const bool more = next < b1 && next != tail_b;
+        if (more) load_k(next);
+        const float fv = vs * (DQ_P_SCALE / (smax > 0.0f ? smax : 1.0f));
+        const bool edge = b * Q8_BLOCK + Q8_BLOCK - 1 > first;
+        f16x8 p[CT][2];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+            soften(x[ct], ct, 0, fk * qfac[ct], b);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                float w = x[ct][e / 4][e % 4] * fv;
+                if (edge && x[ct][e / 4][e % 4] == 0.0f) w = 0.0f;  // (where the block is broken and the row does not see it)
+                p[ct][e / 8][e % 8] = (_Float16)w;
+            }
+        }
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) {
+            const f16x8 v0 = codes_f16x8(vr[dt].x, vr[dt].y), v1 = codes_f16x8(vr[dt].z, vr[dt].w);
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+                o[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, p[ct][0], o[ct][dt], 0, 0, 0);
+                o[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, p[ct][1], o[ct][dt], 0, 0, 0);
+            }
+        }
+        if (more) load_v(next);
+    }
+    if (has_tail) {  // tile `wave` of the unfinished block, as in the kernel of one token
+        const size_t tail = a.c.tail_at(u.seq, h);
+        const int ahead = s.end % Q8_BLOCK - 16 * g4 - 4 * wave;  // of a lane's 4 value tokens, those that there are
+        const uint32_t live0 = ahead <= 0 ? 0u : ahead == 1 ? 0xffffu : 0xffffffffu;
+        const uint32_t live1 = ahead <= 2 ? 0u : ahead == 3 ? 0xffffu : 0xffffffffu;
+        uint4 tk[4];
+        uint2 tv[8];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) tk[n] = load_u4(a.c.kt + tail + krow + wave * 4 * Q8_D + 64 * (n >> 1) + 8 * (n & 1));
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            tv[n] = *reinterpret_cast<const uint2*>(a.c.vt + tail + vrow + n * 16 * Q8_BLOCK + 4 * wave);
+            tv[n] = make_uint2(tv[n].x & live0, tv[n].y & live1);
+        }
+        const float f_unit = DQ_P_SCALE / (smax > 0.0f ? smax : 1.0f);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+            f32x4 x[1] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+                x[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                    as_bf16x8(tk[n]),
+                    as_bf16x8(*reinterpret_cast<const uint4*>(qb + (16 * ct + c) * DQ_QROW + 64 * (n >> 1) + 16 * g4 + 8 * (n & 1))),
+                    x[0], 0, 0, 0);
+            soften(x, ct, wave, a.scale_log2, tail_b);
+            bf16x4 ph, pl;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float p = x[0][e] * f_unit;
+                ph[e] = (__bf16)p;
+                pl[e] = (__bf16)(p - (float)ph[e]);
+            }
+#pragma unroll
+            for (int dt = 0; dt < 8; ++dt) {
+                const t2h_v4i16 v = __builtin_bit_cast(t2h_v4i16, tv[dt]);
+                o[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(v, __builtin_bit_cast(t2h_v4i16, ph), o[ct][dt], 0, 0, 0);
+                o[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(v, __builtin_bit_cast(t2h_v4i16, pl), o[ct][dt], 0, 0, 0);
+            }
+        }
+    }
+
+    // the waves' states joined
+    const float unscale = (smax > 0.0f ? smax : 1.0f) * (1.0f / DQ_P_SCALE);
+    __syncthreads();
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+        const float sum = xor_sum<32>(xor_sum<16>(l[ct]));
+        const int row = 16 * ct + c;
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt)
+            *reinterpret_cast<f32x4*>(room + (wave * COLS + row) * DQ_ROW + 16 * dt + 4 * g4) = o[ct][dt] * unscale;
+        if (g4 == 0) {
+            wml[wave][row][0] = m[ct];
+            wml[wave][row][1] = sum;
+        }
+    }
+    __syncthreads();
+    const int waves = !has_tail && b1 - b0 < DQ_WAVES ? b1 - b0 : DQ_WAVES;
+    for (int i = tid; i < rows * (Q8_D / 4); i += DQ_WAVES * 64) {
+        const int row = i / (Q8_D / 4), d = i % (Q8_D / 4) * 4;
+        float M = -INFINITY, L = 0.0f;
+        for (int w = 0; w < waves; ++w) M = fmaxf(M, wml[w][row][0]);
+        const float base = M == -INFINITY ? 0.0f : M;
+        f32x4 sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int w = 0; w < waves; ++w) {
+            const float f = __builtin_amdgcn_exp2f(wml[w][row][0] - base);
+            L = fmaf(f, wml[w][row][1], L);
+            sum += *reinterpret_cast<const f32x4*>(room + (w * COLS + row) * DQ_ROW + d) * f;
+        }
+        if (u.count == 1) {
+            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+            *reinterpret_cast<uint2*>(a.out + row_at(row) + d) =
+                make_uint2(pack_bf16x2(sum[0] * inv, sum[1] * inv), pack_bf16x2(sum[2] * inv, sum[3] * inv));
+            if (a.lse && d == 0) a.lse[((size_t)u.seq * a.c.nk + h) * rows + row] = M + log2f(L);
+        } else {
+            const size_t part = ((size_t)unit * a.c.nk + h) * rows + row;
+            *reinterpret_cast<f32x4*>(a.part_o + part * Q8_D + d) = sum;
+            if (d == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * part) = make_float2(M, L);
+        }
+    }
+}
+
+// The units of a (sequence, KV head) joined, 8 rows a thread block, 32 lanes a row.
+__global__ __launch_bounds__(256) void attn_rows_q8_merge_kernel(const ChunkQ8Args a) {
+    const uint32_t rows = a.n * a.group, per = (rows + 7) / 8;
+    const uint32_t h = blockIdx.x % a.c.nk, rest = blockIdx.x / a.c.nk;
+    const uint32_t row = rest % per * 8 + (threadIdx.x >> 5), seq = rest / per;
+    DecodeUnit u;
+    dq_find({a.lengths, a.counts, a.n, a.n_seq, a.c.nb, a.c.nk}, seq, true, u);
+    if (u.count <= 1 || row >= rows) return;
+    const int d = (threadIdx.x & 31) * 4;
+    constexpr uint32_t BATCH = 16;  // parts in flight
+    float M = -INFINITY, L = 0.0f;
+    f32x4 sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t i0 = 0; i0 < u.count; i0 += BATCH) {
+        float2 ml[BATCH];
+        f32x4 part[BATCH];
+#pragma unroll
+        for (uint32_t e = 0; e < BATCH; ++e) {
+            const size_t at = ((size_t)(u.first + (i0 + e < u.count ? i0 + e : i0)) * a.c.nk + h) * rows + row;
+            ml[e] = *reinterpret_cast<const float2*>(a.part_ml + 2 * at);
+            part[e] = *reinterpret_cast<const f32x4*>(a.part_o + at * Q8_D + d);
+        }
+#pragma unroll
+        for (uint32_t e = 0; e < BATCH; ++e) {
+            if (i0 + e >= u.count) ml[e].x = -INFINITY;
+            const float now = fmaxf(M, ml[e].x), base = now == -INFINITY ? 0.0f : now;
+            const float keep = __builtin_amdgcn_exp2f(M - base), f = __builtin_amdgcn_exp2f(ml[e].x - base);
+            L = fmaf(L, keep, f * ml[e].y);
+            sum = sum * keep + part[e] * f;
+            M = now;
+        }
+    }
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    const uint32_t t = row / a.group, g = row % a.group;
+    *reinterpret_cast<uint2*>(a.out + (((size_t)seq * a.n + t) * a.nh + h * a.group + g) * Q8_D + d) =
+        make_uint2(pack_bf16x2(sum[0] * inv, sum[1] * inv), pack_bf16x2(sum[2] * inv, sum[3] * inv));
+    if (a.lse && d == 0) a.lse[((size_t)seq * a.c.nk + h) * rows + row] = M + log2f(L);
+}
+
+// Whether a KV head's rows are columns of the products of single tokens: up to two tiles of 16.
+static bool cq_few(uint32_t n, uint32_t nh, uint32_t nk) { return (uint64_t)n * (nh / nk) <= 32; }
+
 // Waves a thread block: 8 share a block's conversion to 16 bits where that leaves a thread block for every CU and more.
 static uint32_t cq_waves(uint32_t n, uint32_t n_seq, uint32_t nh, uint32_t nk) {
     return ((uint64_t)n * (nh / nk) + 255) / 256 * n_seq * nk >= CQ_WIDE_GRID ? 8 : 4;
@@ -1237,6 +1539,7 @@ extern "C" size_t t2h_flash_attn_prefill_q8_workspace_bytes(uint32_t n, uint32_t
                                                             uint32_t s_cap, int weights) {
     if (n_seq == 0 || nk == 0 || nh == 0 || nh % nk != 0 || nh / nk > Q8_MAX_GROUP || s_cap == 0 || s_cap % Q8_BLOCK != 0) return 0;
     const size_t rows = (size_t)n_seq * nh * n;
+    if (cq_few(n, nh, nk)) return 16 + (weights ? rows * 4 : 0) + (size_t)dq_units(n_seq, nk, s_cap / Q8_BLOCK) * nh * n * (Q8_D + 2) * 4;
     const uint32_t splits = cq_splits(n, n_seq, nh, nk, s_cap / Q8_BLOCK);
     return 16 + (weights ? rows * 4 : 0) + (splits > 1 ? splits * rows * (Q8_D + 2) * 4 : 0);
 }
@@ -1268,26 +1571,37 @@ extern "C" int t2h_flash_attn_prefill_q8(const void* q, void* const* cache, uint
     const uint64_t rows = (uint64_t)n_seq * nh * n, tile_rows = 32 * cq_waves(n, n_seq, nh, nk),
                    tiles = ((uint64_t)n * a.group + tile_rows - 1) / tile_rows;
     if (rows > 0x3fffffffu) return T2H_ERR_SHAPE;
-    a.splits = cq_splits(n, n_seq, nh, nk, a.c.nb);
+    const bool few = cq_few(n, nh, nk);
+    const uint32_t units = dq_units(n_seq, nk, a.c.nb);
+    a.splits = few ? 1 : cq_splits(n, n_seq, nh, nk, a.c.nb);
     a.tiles = (uint32_t)tiles;
     float* at = reinterpret_cast<float*>(workspace);
     a.part_o = a.part_ml = a.lse = nullptr;
-    if (a.splits > 1) {
+    if (few || a.splits > 1) {
+        const uint64_t parts = few ? (uint64_t)units * nh * n : a.splits * rows;
         a.part_o = at;
-        a.part_ml = at + a.splits * rows * Q8_D;
-        at += a.splits * rows * (Q8_D + 2);
+        a.part_ml = at + parts * Q8_D;
+        at += parts * (Q8_D + 2);
     }
     if (weights) a.lse = at;
-    const uint64_t grid = tiles * n_seq * nk * a.splits, merge = (rows + 7) / 8;
+    const uint64_t grid = few ? (uint64_t)units * nk : tiles * n_seq * nk * a.splits;
+    const uint64_t merge = few ? ((uint64_t)n * a.group + 7) / 8 * n_seq * nk : (rows + 7) / 8;
     const uint64_t wgrid = (uint64_t)n_seq * nk * ((a.c.nb + 3) / 4);
-    if (grid > 0x7fffffffu || wgrid > 0x7fffffffu) return T2H_ERR_SHAPE;
+    if (grid > 0x7fffffffu || merge > 0x7fffffffu || wgrid > 0x7fffffffu) return T2H_ERR_SHAPE;
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    if (tile_rows == 256)
+    if (few && n * a.group <= 16)
+        hipLaunchKernelGGL(attn_rows_q8_kernel<1>, dim3((uint32_t)grid), dim3(DQ_WAVES * 64), 0, st, a);
+    else if (few)
+        hipLaunchKernelGGL(attn_rows_q8_kernel<2>, dim3((uint32_t)grid), dim3(DQ_WAVES * 64), 0, st, a);
+    else if (tile_rows == 256)
         hipLaunchKernelGGL(attn_chunk_q8_kernel<8>, dim3((uint32_t)grid), dim3(512), 0, st, a);
     else
         hipLaunchKernelGGL(attn_chunk_q8_kernel<4>, dim3((uint32_t)grid), dim3(256), 0, st, a);
     T2H_LAUNCH_CHECK();
-    if (a.splits > 1) {
+    if (few) {
+        hipLaunchKernelGGL(attn_rows_q8_merge_kernel, dim3((uint32_t)merge), dim3(256), 0, st, a);
+        T2H_LAUNCH_CHECK();
+    } else if (a.splits > 1) {
         hipLaunchKernelGGL(attn_chunk_q8_merge_kernel, dim3((uint32_t)merge), dim3(256), 0, st, a);
         T2H_LAUNCH_CHECK();
     }
