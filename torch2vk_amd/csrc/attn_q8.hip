@@ -254,14 +254,29 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_decode_q8_kernel(const 
     // the tail's rows, a quarter a wave: token 16 (c / 4) + 4 wave + c % 4, dims 64 j + 16 g4 + 8 i; and the values of
     // tokens 16 g4 + 4 wave .. of dim 16 n + c
     const size_t tail = a.c.tail_at(u.seq, h);
-    uint4 tk[4];
-    uint2 tv[8];
-    if (new_here) {
+    auto load_tail = [&](uint4 (&tk)[4], uint2 (&tv)[8]) {
 #pragma unroll
         for (int n = 0; n < 4; ++n) tk[n] = load_u4(a.c.kt + tail + krow + wave * 4 * Q8_D + 64 * (n >> 1) + 8 * (n & 1));
 #pragma unroll
         for (int n = 0; n < 8; ++n) tv[n] = *reinterpret_cast<const uint2*>(a.c.vt + tail + vrow + n * 16 * Q8_BLOCK + 4 * wave);
-    }
+    };
+    // the new token among them: its key a row, its value one of a word's two tokens (behind it: zeros)
+    auto put_new = [&](uint4 (&tk)[4], uint2 (&tv)[8]) {
+        if ((c >> 2) * 16 + wave * 4 + (c & 3) == r) {
+#pragma unroll
+            for (int n = 0; n < 4; ++n) tk[n] = *reinterpret_cast<const uint4*>(&fresh[0][64 * (n >> 1) + 16 * g4 + 8 * (n & 1)]);
+        }
+        const int ahead = r - 16 * g4 - 4 * wave;
+        const uint32_t old0 = ahead <= 0 ? 0u : ahead == 1 ? 0xffffu : 0xffffffffu;
+        const uint32_t old1 = ahead <= 2 ? 0u : ahead == 3 ? 0xffffu : 0xffffffffu;
+        const uint32_t new0 = ahead == 0 ? 0xffffu : ahead == 1 ? 0xffff0000u : 0u;
+        const uint32_t new1 = ahead == 2 ? 0xffffu : ahead == 3 ? 0xffff0000u : 0u;
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            const uint32_t vnew = fresh[1][16 * n + c] * 0x10001u;
+            tv[n] = make_uint2((tv[n].x & old0) | (vnew & new0), (tv[n].y & old1) | (vnew & new1));
+        }
+    };
     int b = b0 + wave;
     if (b < b1 && b != new_b) {
         load_k(b);
@@ -303,22 +318,11 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_decode_q8_kernel(const 
     }
     __syncthreads();
     if (new_here) {
-        // the new token among the tail's: its key a row, its value one of a word's two tokens (behind it: zeros)
-        if ((c >> 2) * 16 + wave * 4 + (c & 3) == r) {
-#pragma unroll
-            for (int n = 0; n < 4; ++n) tk[n] = *reinterpret_cast<const uint4*>(&fresh[0][64 * (n >> 1) + 16 * g4 + 8 * (n & 1)]);
-        }
-        const int ahead = r - 16 * g4 - 4 * wave;
-        const uint32_t old0 = ahead <= 0 ? 0u : ahead == 1 ? 0xffffu : 0xffffffffu;
-        const uint32_t old1 = ahead <= 2 ? 0u : ahead == 3 ? 0xffffu : 0xffffffffu;
-        const uint32_t new0 = ahead == 0 ? 0xffffu : ahead == 1 ? 0xffff0000u : 0u;
-        const uint32_t new1 = ahead == 2 ? 0xffffu : ahead == 3 ? 0xffff0000u : 0u;
-#pragma unroll
-        for (int n = 0; n < 8; ++n) {
-            const uint32_t vnew = fresh[1][16 * n + c] * 0x10001u;
-            tv[n] = make_uint2((tv[n].x & old0) | (vnew & new0), (tv[n].y & old1) | (vnew & new1));
-        }
-        if (!has_tail) {  // it finishes its block: rounded here, then read as codes
+        if (!has_tail) {  // the new token finishes its block: rounded here, then read as codes
+            uint4 tk[4];
+            uint2 tv[8];
+            load_tail(tk, tv);
+            put_new(tk, tv);
             uint32_t kmax = 0, vmax = 0;
 #pragma unroll
             for (int n = 0; n < 4; ++n) kmax = max(max(kmax, max(bf16_abs_max(tk[n].x), bf16_abs_max(tk[n].y))),
@@ -415,6 +419,7 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_decode_q8_kernel(const 
             const f16x8 h0 = query(0, j, 0), l0 = query(1, j, 0), h1 = query(0, j, 1), l1 = query(1, j, 1);
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
+                __builtin_amdgcn_sched_barrier(0);
                 const uint4 kk = kr[2 * t + j];
                 const f16x8 k0 = codes_f16x8(kk.x, kk.y), k1 = codes_f16x8(kk.z, kk.w);
                 x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, h0, x[t], 0, 0, 0);
@@ -436,6 +441,7 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_decode_q8_kernel(const 
             for (int e = 0; e < 8; ++e) p[s][e] = (_Float16)(x[2 * s + e / 4][e % 4] * fv);
 #pragma unroll
         for (int dt = 0; dt < 8; ++dt) {
+            __builtin_amdgcn_sched_barrier(0);
             o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16x8(vr[dt].x, vr[dt].y), p[0], o[dt], 0, 0, 0);
             o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16x8(vr[dt].z, vr[dt].w), p[1], o[dt], 0, 0, 0);
         }
@@ -443,6 +449,10 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_decode_q8_kernel(const 
     }
 
     if (has_tail) {  // tile `wave` of the unfinished block
+        uint4 tk[4];
+        uint2 tv[8];
+        load_tail(tk, tv);
+        put_new(tk, tv);
         f32x4 x[1] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
