@@ -612,7 +612,7 @@ int t2h_qk_norm_rope_cache_q8(const float* q, uint64_t q_row, const float* k, ui
  * softmax weight that each cached token got, summed over the q heads of the KV head; a new token's begins at 0, and
  * elements behind the last token are left as they are.
  * workspace: t2h_attn_decode_q8_workspace_bytes() bytes, 16-byte aligned, zero-filled once before its first use (calls
- * leave it reusable); calls that share one must not overlap in time. */
+ * leave it reusable, for other shapes too up to n_seq * nk = 16384); calls that share one must not overlap in time. */
 size_t t2h_attn_decode_q8_workspace_bytes(uint32_t n_seq, uint32_t nh, uint32_t nk, uint32_t d, uint32_t s_cap,
                                           int weights);
 int t2h_attn_decode_q8(const float* q, uint64_t q_row, const float* k_new, uint64_t k_row, const float* v_new,

@@ -166,7 +166,7 @@ def test_kv_q8_argument_validation(lib):
         q=fake, c=c, cap=128, ln=fake, ct=None, w=None, wo=None, out=fake, n=4, s=1, nh=4, nk=2, d=128, scale=0.0, ws=fake,
         nb=1 << 20, st=None), **m}.values())
     evict = lambda **m: lib.t2h_kv_cache_q8_evict(*{**dict(  # noqa: E731
-        c=c, cap=128, ln=fake, w=fake, keep=1, sink=0, recent=0, s=1, nk=2, d=128, o=c, ocap=128, wo=fake, kept=fake, lo=fake,
+        c=c, cap=128, ln=fake, w=fake, keep=1, sink=0, recent=0, s=1, nk=2, d=128, o=c, ocap=128, wo=fake, kept=fake, lo=0x5000,
         st=None), **m}.values())
     read = lambda **m: lib.t2h_kv_cache_q8_dequantize(*{**dict(  # noqa: E731
         c=c, cap=128, ln=fake, s=1, nk=2, d=128, k=fake, v=fake, st=None), **m}.values())
@@ -202,4 +202,4 @@ def test_kv_q8_argument_validation(lib):
     other = six(*[0x2000] * 6)
     assert evict(o=other, ocap=64, wo=0x3000) == 2
     assert evict(ocap=192) == 2 and evict(o=other, ocap=192) == 2
-    assert evict(o=None) == 1
+    assert evict(o=None) == 1 and evict(lo=fake) == 5

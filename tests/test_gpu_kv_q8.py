@@ -392,6 +392,25 @@ def test_decode_replayed_from_a_graph(device):
     assert torch.equal(runs[0][2].k, runs[1][2].k) and torch.equal(runs[0][2].v, runs[1][2].v)
 
 
+def test_decode_of_several_shapes_in_one_workspace(device):
+    """Calls of different batches, heads and capacities in turn, in one workspace: each as with its own."""
+    shapes = [(1, 8, 8, 3000), (40, 8, 1, 2000), (3, 32, 8, 900), (1, 16, 1, 3000), (40, 8, 1, 2000)]
+    ws = max((K.attn_decode_q8_workspace(n, nh, nk, D, 3008, device, weights=True) for n, nh, nk, _ in shapes), key=len)
+    for rnd, (n, nh, nk, length) in enumerate(shapes):
+        lengths = [max(1, length - 61 * i) for i in range(n)]
+        c = filled(n, 3008, nk, lengths, device, 30 + rnd)
+        (q, k, v), wq, wk = inputs(n, nh, nk, device, 40 + rnd)
+        outs = []
+        for own in (False, True):
+            out = torch.empty(n, nh, D, dtype=BF, device=device)
+            w = torch.zeros(n, nk, 3008, device=device)
+            K.attn_decode_q8(q, k, v, copy_of(c), out, ints(lengths, device),
+                             K.attn_decode_q8_workspace(n, nh, nk, D, 3008, device, weights=True) if own else ws, theta=1e6,
+                             q_norm_weight=wq, k_norm_weight=wk, weights=w)
+            outs.append((out, w))
+        assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
+
+
 # ---------------------------------------------------------------------------------------------------- chunks
 
 

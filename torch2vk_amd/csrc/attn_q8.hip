@@ -639,6 +639,13 @@ __global__ __launch_bounds__(256) void attn_decode_q8_weights_kernel(const Decod
         if (t0 + j < end) a.w_out[at + j] = (t0 + j < len ? a.w_in[at + j] : 0.0f) + sum[j];
 }
 
+// Counters at the start of the workspace, as many for every shape (of up to 16384 sequences times KV heads), so that calls of
+// several shapes may share one: another shape's parts never lie where counters are.
+static size_t dq_counters(uint32_t n_seq, uint32_t nk) {
+    const size_t heads = (size_t)n_seq * nk;
+    return heads <= 16384 ? 16384 : (heads + 3) / 4 * 4;
+}
+
 // Units that sequences of any lengths can have: sum of ceil(blocks / chunk) <= total / chunk + n_seq, and total / chunk is at
 // most that of the largest total or the slots' share, as the chunk grows with the total in between.
 static uint32_t dq_units(uint32_t n_seq, uint32_t nk, uint32_t nb) {
@@ -1486,7 +1493,7 @@ extern "C" size_t t2h_attn_decode_q8_workspace_bytes(uint32_t n_seq, uint32_t nh
         s_cap % Q8_BLOCK != 0)
         return 0;
     const size_t parts = (size_t)dq_units(n_seq, nk, s_cap / Q8_BLOCK) * nh;
-    return ((size_t)n_seq * nk * 4 + 15) / 16 * 16 + (parts * (Q8_D + 2) * 4 + 15) / 16 * 16 + (weights ? (size_t)n_seq * nh * s_cap * 4 : 0);
+    return dq_counters(n_seq, nk) * 4 + (parts * (Q8_D + 2) * 4 + 15) / 16 * 16 + (weights ? (size_t)n_seq * nh * s_cap * 4 : 0);
 }
 
 extern "C" int t2h_attn_decode_q8(const float* q, uint64_t q_row, const float* k_new, uint64_t k_row, const float* v_new,
@@ -1521,7 +1528,7 @@ extern "C" int t2h_attn_decode_q8(const float* q, uint64_t q_row, const float* k
     a.units = dq_units(n_seq, nk, a.c.nb);
     const size_t parts = (size_t)a.units * nh;
     a.done = reinterpret_cast<uint32_t*>(workspace);
-    a.part_o = reinterpret_cast<float*>(workspace) + ((size_t)n_seq * nk + 3) / 4 * 4;
+    a.part_o = reinterpret_cast<float*>(workspace) + dq_counters(n_seq, nk);
     a.part_ml = a.part_o + parts * Q8_D;
     a.scores = weights ? a.part_o + (parts * (Q8_D + 2) + 3) / 4 * 4 : nullptr;
     a.eps = eps;

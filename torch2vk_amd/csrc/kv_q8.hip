@@ -583,7 +583,7 @@ extern "C" int t2h_kv_cache_q8_evict(void* const* cache, uint32_t s_cap, const i
     if (!lengths || !weights || !weights_out || !kept || !lengths_out) return T2H_ERR_NULL;
     if (const int e = q8_cache(cache, s_cap, n_seq, nk, nk, d, a.c)) return e;
     if (const int e = q8_cache(cache_out, s_cap_out, n_seq, nk, nk, d, a.o)) return e;
-    if (keep_blocks == 0 || keep_blocks > 0x1000000u) return T2H_ERR_ARG;
+    if (keep_blocks == 0 || keep_blocks > 0x1000000u || lengths_out == lengths) return T2H_ERR_ARG;
     if ((uint64_t)sink + recent > (uint64_t)keep_blocks * Q8_BLOCK) return T2H_ERR_ARG;
     // a cache of the output's capacity holds what stays and a tail
     if ((uint64_t)s_cap_out < s_cap && s_cap_out < ((uint64_t)keep_blocks + 1) * Q8_BLOCK) return T2H_ERR_SHAPE;
