@@ -492,9 +492,15 @@ __global__ __launch_bounds__(256) void q8_evict_move_kernel(const Q8EvictArgs a)
             __syncthreads();
             q8_scale(max(max(red[0], red[1]), max(red[2], red[3])), s, inv);
             if (all) s = f;
+            // a dim's 4 tokens leave as one word: byte stores would take a cycle of the address unit for each lane
             int8_t* dst = a.o.v + to + (size_t)wave * 32 * Q8_BLOCK + lane;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) dst[i * Q8_BLOCK] = all ? x[i] : (int8_t)q8_code((float)x[i] * f, inv);
+            for (int i = 0; i < 32; ++i) {
+                int w = (all ? (int)x[i] : q8_code((float)x[i] * f, inv)) & 255;
+                w |= __builtin_amdgcn_update_dpp(0, w, 0xB1, 0xf, 0xf, true) << 8;   // lane ^ 1
+                w |= __builtin_amdgcn_update_dpp(0, w, 0x4E, 0xf, 0xf, true) << 16;  // lane ^ 2
+                if ((lane & 3) == 0) *reinterpret_cast<int*>(dst + i * Q8_BLOCK) = w;
+            }
         }
         if (tid == 0) (values ? a.o.vs : a.o.ks)[a.o.scale_at(seq, (uint32_t)b, h)] = s;
     }
