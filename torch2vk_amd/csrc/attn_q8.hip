@@ -701,12 +701,9 @@ __device__ __forceinline__ uint4 codes_bf16x8(uint32_t w0, uint32_t w1) {
                       pack_bf16x2(q8_value(w1, 0), q8_value(w1, 1)), pack_bf16x2(q8_value(w1, 2), q8_value(w1, 3)));
 }
 
-// LDS places of 16 bytes: keys [64][128], queries [64][128] and values [128][64], 2 bytes each, chunks of a row permuted by the
-// row so that 8 lanes of an operand's read, which are rows, meet different banks.  Key rows are read in the order of
-// cq_swap: bits 2 and 3 of the lane change places.
-__device__ __forceinline__ int cq_swap(int row) { return (row & ~12) | (row & 8) >> 1 | (row & 4) << 1; }
-__device__ __forceinline__ int cq_key_at(int token, int chunk) { return token * 16 + (chunk ^ (cq_swap(token) & 15)); }
-__device__ __forceinline__ int cq_query_at(int row, int chunk) { return row * 16 + (chunk ^ (row & 15)); }
+// LDS places of 16 bytes: keys [64][128] and values [128][64], 2 bytes each, chunks of a row permuted by the row so that
+// the lanes of an operand's read, which are rows, meet different banks.
+__device__ __forceinline__ int cq_key_at(int token, int chunk) { return token * 16 + (chunk ^ (token & 15)); }
 __device__ __forceinline__ int cq_value_at(int d, int chunk) { return d * 8 + (chunk ^ (d & 7)); }
 
 template <int WAVES>
@@ -790,7 +787,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_chunk_q8_kernel(const Chun
     for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < 16; ++j) o[i][j] = 0.0f;
-    const int key_row = cq_swap(col);
+    const int key_row = (col & 19) | (col & 8) >> 1 | (col & 4) << 1;  // of operand row `col`: bits 2 and 3 change places
 
     // one block from LDS; f: the scores' factor, shift: log2 of the weights' (both of the whole block)
     auto scores = [&](int buf, f32x16 (&x)[2]) {
@@ -1081,7 +1078,7 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_q8_weights_kernel(const Chu
     };
     auto store = [&](int buf) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) queries[buf][cq_query_at((tid >> 4) + 16 * i, tid & 15)] = next[i];
+        for (int i = 0; i < 4; ++i) queries[buf][cq_key_at((tid >> 4) + 16 * i, tid & 15)] = next[i];
     };
     load(row_first);
     bf16x8 k[2][8];
@@ -1127,7 +1124,7 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_q8_weights_kernel(const Chu
                     for (int j = 0; j < 16; ++j) x[tt][j] = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const bf16x8 q = as_bf16x8(queries[buf][cq_query_at(32 * r + col, 2 * i + half)]);
+                    const bf16x8 q = as_bf16x8(queries[buf][cq_key_at(32 * r + col, 2 * i + half)]);
                     x[0] = mfma_bf16(k[0][i], q, x[0]);
                     x[1] = mfma_bf16(k[1][i], q, x[1]);
                 }
