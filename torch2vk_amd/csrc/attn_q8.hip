@@ -704,7 +704,7 @@ __device__ __forceinline__ uint4 codes_bf16x8(uint32_t w0, uint32_t w1) {
 // LDS places of 16 bytes: keys [64][128] and values [128][64], 2 bytes each, chunks of a row permuted by the row so that
 // the lanes of an operand's read, which are rows, meet different banks.
 __device__ __forceinline__ int cq_key_at(int token, int chunk) { return token * 16 + (chunk ^ (token & 15)); }
-__device__ __forceinline__ int cq_value_at(int d, int chunk) { return d * 8 + (chunk ^ (d & 7)); }
+__device__ __forceinline__ int cq_value_at(int d, int chunk) { return d * 8 + (chunk ^ (d >> 1 & 7)); }
 
 template <int WAVES>
 __global__ __launch_bounds__(WAVES * 64, 2) void attn_chunk_q8_kernel(const ChunkQ8Args a) {
