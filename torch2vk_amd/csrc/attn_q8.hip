@@ -2,6 +2,7 @@
 // or a chunk of tokens, and the attention weight that each cached token got.  One pass over the keys with the running
 // maximum and sum of the softmax, both in fp32, scores in log2 units.
 #include <math.h>
+#include <type_traits>
 
 #include "kv_q8.h"
 #include "kv_q8_args.h"
@@ -782,6 +783,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_chunk_q8_kernel(const Chun
     for (int i = 0; i < 8; ++i) q[i] = load_u4(qp + 16 * i);
     float m = -INFINITY, l = 0.0f;
     float smax = 0.0f;  // the largest value scale so far, or half of it: the accumulators are in units of smax / 2^12
+    float to_unit = DQ_P_SCALE;
     f32x16 o[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -861,8 +863,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_chunk_q8_kernel(const Chun
         if (b0 + 1 < whole) load(b0 + 1);
     }
     __syncthreads();
-    for (int b = b0; b < whole; ++b) {
-        const int buf = (b - b0) & 1;
+    auto step = [&](int b, auto which) {
+        constexpr int buf = decltype(which)::value;
         f32x16 x[2];
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt)
@@ -893,9 +895,10 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_chunk_q8_kernel(const Chun
         if (vf_scale > 2.0f * smax) {  // up to twice the unit's scale is in fp16's range too
             unit = smax / vf_scale;
             smax = vf_scale;
+            to_unit = DQ_P_SCALE / smax;
         }
         // a block of zeros may have any scale: its scores or its values are zeros all the same
-        float shift = vf_scale == 0.0f ? 0.0f : __builtin_amdgcn_logf(vf_scale * (DQ_P_SCALE / (smax > 0.0f ? smax : 1.0f)));
+        float shift = vf_scale == 0.0f ? 0.0f : __builtin_amdgcn_logf(vf_scale * to_unit);
         float f = (kf_scale == 0.0f ? 1.0f : kf_scale) * a.scale_log2;
         ready(x, b, f, shift, unit);
         const float base = (m == -INFINITY ? 0.0f : m) - shift;
@@ -921,6 +924,10 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_chunk_q8_kernel(const Chun
         }
         l = fmaf(sum, __builtin_amdgcn_exp2f(-shift), l);
         __syncthreads();
+    };
+    for (int b = b0; b < whole; b += 2) {
+        step(b, std::integral_constant<int, 0>{});
+        if (b + 1 < whole) step(b + 1, std::integral_constant<int, 1>{});
     }
     if (has_tail) {
         // bf16 rows as they are; weights in two bf16 terms
@@ -1067,13 +1074,33 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_q8_weights_kernel(const Chu
     const int t_first = first_b * Q8_BLOCK - len;
     const int row_first = t_first > 0 ? t_first * group / STEP * STEP : 0;
     uint4 next[4];
-    auto load = [&](int row0) {  // 16 bytes of a row: piece tid % 16 of rows tid / 16, + 16 ..
+    float sub[2], sub_next[2];  // rows lane % 32 and 32 + lane % 32; one that is not there weighs nothing
+    const float* lse = a.lse + ((size_t)seq * a.c.nk + h) * a.n * group;
+    // 16 bytes of a row: piece tid % 16 of rows tid / 16, + 16 ..; their heads and places in q, from STEP rows to the next
+    // without a division
+    int g_at[4];
+    uint32_t q_at[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = row_first + (tid >> 4) + 16 * i, t = row / group;
+        g_at[i] = row - t * group;
+        q_at[i] = (uint32_t)t * a.nh + (uint32_t)g_at[i];
+    }
+    const int g_step = STEP % group;
+    const uint32_t q_step = (uint32_t)(STEP / group) * a.nh + (uint32_t)g_step, q_wrap = a.nh - a.group;
+    const uint16_t* const q_from = a.q + ((size_t)seq * a.n * a.nh + h * group) * Q8_D + 8 * (tid & 15);
+    auto load = [&](int row0) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int row = row0 + (tid >> 4) + 16 * i;
-            const int t = row / group, g = row - t * group;
-            const size_t at = (((size_t)seq * a.n + (row < rows ? t : 0)) * a.nh + h * group + (row < rows ? g : 0)) * Q8_D;
-            next[i] = load_u4(a.q + at + 8 * (tid & 15));
+            next[i] = load_u4(q_from + (size_t)(row0 + (tid >> 4) + 16 * i < rows ? q_at[i] : 0u) * Q8_D);
+            g_at[i] += g_step;
+            q_at[i] += q_step + (g_at[i] >= group ? q_wrap : 0u);
+            g_at[i] -= g_at[i] >= group ? group : 0;
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int row = row0 + 32 * r + col;
+            sub_next[r] = row < rows ? lse[row] : INFINITY;
         }
     };
     auto store = [&](int buf) {
@@ -1106,17 +1133,17 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_q8_weights_kernel(const Chu
     for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
         for (int j = 0; j < 16; ++j) sum[tt][j] = 0.0f;
-    const float* lse = a.lse + ((size_t)seq * a.c.nk + h) * a.n * group;
     store(0);
     __syncthreads();
     for (int row0 = row_first; row0 < rows; row0 += STEP) {
         const int buf = (row0 - row_first) / STEP & 1;
+        sub[0] = sub_next[0];
+        sub[1] = sub_next[1];
         if (row0 + STEP < rows) load(row0 + STEP);
         if (mine) {
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                const int row = row0 + 32 * r + col, t = row / group;
-                const float sub = row < rows ? lse[row] : INFINITY;  // a row that is not there weighs nothing
+                const int row = row0 + 32 * r + col;
                 f32x16 x[2];
 #pragma unroll
                 for (int tt = 0; tt < 2; ++tt)
@@ -1129,19 +1156,19 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_q8_weights_kernel(const Chu
                     x[1] = mfma_bf16(k[1][i], q, x[1]);
                 }
                 if (b * Q8_BLOCK + Q8_BLOCK - 1 > len + (row0 + 32 * r) / group) {
-                    const int seen = len + t - b * Q8_BLOCK - 4 * half;  // tokens 32 tt + 8 (j / 4) + 4 half + j % 4
+                    const int seen = len + row / group - b * Q8_BLOCK - 4 * half;  // tokens 32 tt + 8 (j / 4) + 4 half + j % 4
 #pragma unroll
                     for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
                         for (int j = 0; j < 16; ++j) {
-                            const float p = __builtin_amdgcn_exp2f(fmaf(x[tt][j], f, -sub));
+                            const float p = __builtin_amdgcn_exp2f(fmaf(x[tt][j], f, -sub[r]));
                             sum[tt][j] += row >= rows || 32 * tt + 8 * (j >> 2) + (j & 3) > seen ? 0.0f : p;
                         }
                 } else {
 #pragma unroll
                     for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) sum[tt][j] += __builtin_amdgcn_exp2f(fmaf(x[tt][j], f, -sub));
+                        for (int j = 0; j < 16; ++j) sum[tt][j] += __builtin_amdgcn_exp2f(fmaf(x[tt][j], f, -sub[r]));
                 }
             }
         }
@@ -1149,7 +1176,11 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_q8_weights_kernel(const Chu
         __syncthreads();
     }
     if (!mine) return;
-    // over the 32 rows that the lanes of a half hold
+    // over the 32 rows that the lanes of a half hold; a lane writes one token
+    const int p = b * Q8_BLOCK + 32 * (col >> 4) + 8 * (col >> 2 & 3) + 4 * half + (col & 3);
+    const size_t at = ((size_t)seq * a.c.nk + h) * a.c.nb * Q8_BLOCK + p;
+    const float before = p < s.len ? a.w_in[at] : 0.0f;
+    float total = 0.0f;
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
@@ -1159,17 +1190,10 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_q8_weights_kernel(const Chu
             v += dpp_f32<0x4E>(v);
             v += dpp_f32<0x141>(v);
             v += dpp_f32<0x140>(v);
-            sum[tt][j] = xor_sum<16>(v);
+            v = xor_sum<16>(v);
+            if (col == 16 * tt + j) total = v;
         }
-    if (col != 0) return;
-    const size_t at = ((size_t)seq * a.c.nk + h) * a.c.nb * Q8_BLOCK;
-#pragma unroll
-    for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            const int p = b * Q8_BLOCK + 32 * tt + 8 * (j >> 2) + 4 * half + (j & 3);
-            if (p < s.end) a.w_out[at + p] = (p < s.len ? a.w_in[at + p] : 0.0f) + sum[tt][j];
-        }
+    if (p < s.end) a.w_out[at] = before + total;
 }
 
 // ---------------------------------------------------------------------------------------------------- few rows --
