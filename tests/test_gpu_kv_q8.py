@@ -421,7 +421,9 @@ def test_decode_of_several_shapes_in_one_workspace(device):
     (16, 8, 512, [700], None, 1280, True), (12, 4, 3, [5000], None, 5056, True), (32, 8, 129, [190], None, 256, False),
     (8, 4, 40, [230, 250], None, 256, True), (4, 4, 700, [0], None, 704, False), (16, 2, 2, [20000], None, 20032, True),
     (3, 3, 1, [8191], None, 8192, False), (8, 2, 1300, [900], None, 2240, True), (32, 8, 5, [3990, 61, 0], [5, 4, 2], 4032, True),
-    (8, 8, 32, [100, 33, -1, 160], [28, 32, 5, 32], 192, True), (4, 1, 8, [30000, 120], None, 30016, True)])
+    (8, 8, 32, [100, 33, -1, 160], [28, 32, 5, 32], 192, True), (4, 1, 8, [30000, 120], None, 30016, True),
+    (12, 2, 400, [5, -1, 130], [400, 7, 333], 576, True), (16, 1, 256, [0, 100, 60], [256, 1, 0], 384, True),
+    (14, 2, 700, [300], [650], 960, True)])
 def test_chunk(device, nh, nk, n, lengths, counts, s_cap, weights):
     """A chunk written and attended to, against the definition over what the cache then holds; tokens past the capacity are
     dropped."""

@@ -685,7 +685,8 @@ struct ChunkQ8Args {
     const int32_t* counts;
     const float* w_in;
     float* w_out;
-    uint32_t n, n_seq, nh, group, tiles, splits;
+    float* w_part;      // [w_splits][n_seq][nk][s_cap] sums, or null
+    uint32_t n, n_seq, nh, group, tiles, splits, w_splits;
     float scale_log2;
 };
 
@@ -1058,7 +1059,9 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_q8_weights_kernel(const Chu
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t h = blockIdx.x % a.c.nk;
-    const uint32_t rest = blockIdx.x / a.c.nk;
+    uint32_t rest = blockIdx.x / a.c.nk;
+    const uint32_t split = rest % a.w_splits;
+    rest /= a.w_splits;
     const uint32_t per = (a.c.nb + 3) / 4;
     const uint32_t seq = rest / per;
     const int first_b = (int)(rest % per) * 4, b = first_b + wave;
@@ -1070,9 +1073,11 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_q8_weights_kernel(const Chu
     const int group = (int)a.group, rows = count * group;
     const bool mine = b * Q8_BLOCK < s.end;
     const bool in_tail = s.end % Q8_BLOCK && b == s.end / Q8_BLOCK;
-    // from the first row that sees the thread block's first token
+    // from the first row that sees the thread block's first token, a share of the steps
     const int t_first = first_b * Q8_BLOCK - len;
-    const int row_first = t_first > 0 ? t_first * group / STEP * STEP : 0;
+    const int step0 = t_first > 0 ? (int)((int64_t)t_first * group / STEP) : 0, steps = (rows + STEP - 1) / STEP - step0;
+    const int row_first = (step0 + (int)((int64_t)steps * split / a.w_splits)) * STEP;
+    const int row_end = min(rows, (step0 + (int)((int64_t)steps * (split + 1) / a.w_splits)) * STEP);
     uint4 next[4];
     float sub[2], sub_next[2];  // rows lane % 32 and 32 + lane % 32; one that is not there weighs nothing
     const float* lse = a.lse + ((size_t)seq * a.c.nk + h) * a.n * group;
@@ -1135,11 +1140,11 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_q8_weights_kernel(const Chu
         for (int j = 0; j < 16; ++j) sum[tt][j] = 0.0f;
     store(0);
     __syncthreads();
-    for (int row0 = row_first; row0 < rows; row0 += STEP) {
+    for (int row0 = row_first; row0 < row_end; row0 += STEP) {
         const int buf = (row0 - row_first) / STEP & 1;
         sub[0] = sub_next[0];
         sub[1] = sub_next[1];
-        if (row0 + STEP < rows) load(row0 + STEP);
+        if (row0 + STEP < row_end) load(row0 + STEP);
         if (mine) {
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
@@ -1172,14 +1177,14 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_q8_weights_kernel(const Chu
                 }
             }
         }
-        if (row0 + STEP < rows) store(buf ^ 1);
+        if (row0 + STEP < row_end) store(buf ^ 1);
         __syncthreads();
     }
     if (!mine) return;
     // over the 32 rows that the lanes of a half hold; a lane writes one token
     const int p = b * Q8_BLOCK + 32 * (col >> 4) + 8 * (col >> 2 & 3) + 4 * half + (col & 3);
-    const size_t at = ((size_t)seq * a.c.nk + h) * a.c.nb * Q8_BLOCK + p;
-    const float before = p < s.len ? a.w_in[at] : 0.0f;
+    const size_t all = (size_t)a.n_seq * a.c.nk * a.c.nb * Q8_BLOCK, at = ((size_t)seq * a.c.nk + h) * a.c.nb * Q8_BLOCK + p;
+    const float before = a.w_splits == 1 && p < s.len ? a.w_in[at] : 0.0f;
     float total = 0.0f;
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt)
@@ -1193,7 +1198,27 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_q8_weights_kernel(const Chu
             v = xor_sum<16>(v);
             if (col == 16 * tt + j) total = v;
         }
-    if (p < s.end) a.w_out[at] = before + total;
+    if (p >= s.end) return;
+    if (a.w_splits == 1)
+        a.w_out[at] = before + total;
+    else
+        a.w_part[split * all + at] = total;
+}
+
+// The shares added up, in their order: 4 tokens a thread.
+__global__ __launch_bounds__(256) void attn_chunk_q8_weights_merge_kernel(const ChunkQ8Args a) {
+    const uint32_t cap = a.c.nb * Q8_BLOCK;
+    const size_t all = (size_t)a.n_seq * a.c.nk * cap, at = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (at >= all) return;
+    const uint32_t seq = (uint32_t)(at / ((size_t)a.c.nk * cap));
+    const int p = (int)(at % cap);
+    const Q8Span s = q8_span(a.lengths, a.counts, seq, a.n, a.c.nb);
+    if (p >= s.end) return;
+    f32x4 sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t i = 0; i < a.w_splits; ++i) sum += *reinterpret_cast<const f32x4*>(a.w_part + i * all + at);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (p + j < s.end) a.w_out[at + j] = (p + j < s.len ? a.w_in[at + j] : 0.0f) + sum[j];
 }
 
 // ---------------------------------------------------------------------------------------------------- few rows --
@@ -1507,6 +1532,20 @@ static uint32_t cq_splits(uint32_t n, uint32_t n_seq, uint32_t nh, uint32_t nk, 
     return (uint32_t)(want < most ? (want ? want : 1) : (most ? most : 1));
 }
 
+// Thread blocks that share the rows of a chunk's weights where there are few tokens: two rounds of the chip (for a causal
+// chunk's share of the pairs), 512 rows each or more.  Measured (us, 32 / 8 heads): 2048 tokens at 0: 38 in rounds of 1024
+// thread blocks, 48 of 512, 196 unshared; 2 x 300 of 40 / 8 heads at 3000: 37 of 512 rows or more, 41 of 256, 45 unshared.
+static uint32_t cq_weight_splits(uint32_t n, uint32_t n_seq, uint32_t nh, uint32_t nk, uint32_t nb) {
+    const uint64_t grid = ((uint64_t)nb + 3) / 4 * n_seq * nk, want = 1024 / grid, most = (uint64_t)n * (nh / nk) / 512;
+    return (uint32_t)(want < most ? (want ? want : 1) : (most ? most : 1));
+}
+
+// fp32 values of a chunk's weights: each row's softmax and the shares
+static size_t cq_weight_values(uint32_t n, uint32_t n_seq, uint32_t nh, uint32_t nk, uint32_t s_cap) {
+    const uint32_t splits = cq_weight_splits(n, n_seq, nh, nk, s_cap / Q8_BLOCK);
+    return (size_t)n_seq * nh * n + (splits > 1 ? (size_t)splits * n_seq * nk * s_cap : 0);
+}
+
 }  // namespace t2h
 
 using namespace t2h;
@@ -1580,9 +1619,10 @@ extern "C" size_t t2h_flash_attn_prefill_q8_workspace_bytes(uint32_t n, uint32_t
                                                             uint32_t s_cap, int weights) {
     if (n_seq == 0 || nk == 0 || nh == 0 || nh % nk != 0 || nh / nk > Q8_MAX_GROUP || s_cap == 0 || s_cap % Q8_BLOCK != 0) return 0;
     const size_t rows = (size_t)n_seq * nh * n;
-    if (cq_few(n, nh, nk)) return 16 + (weights ? rows * 4 : 0) + (size_t)dq_units(n_seq, nk, s_cap / Q8_BLOCK) * nh * n * (Q8_D + 2) * 4;
+    const size_t sums = weights ? cq_weight_values(n, n_seq, nh, nk, s_cap) * 4 : 0;
+    if (cq_few(n, nh, nk)) return 16 + sums + (size_t)dq_units(n_seq, nk, s_cap / Q8_BLOCK) * nh * n * (Q8_D + 2) * 4;
     const uint32_t splits = cq_splits(n, n_seq, nh, nk, s_cap / Q8_BLOCK);
-    return 16 + (weights ? rows * 4 : 0) + (splits > 1 ? splits * rows * (Q8_D + 2) * 4 : 0);
+    return 16 + sums + (splits > 1 ? splits * rows * (Q8_D + 2) * 4 : 0);
 }
 
 extern "C" int t2h_flash_attn_prefill_q8(const void* q, void* const* cache, uint32_t s_cap, const int32_t* lengths,
@@ -1617,7 +1657,12 @@ extern "C" int t2h_flash_attn_prefill_q8(const void* q, void* const* cache, uint
     a.splits = few ? 1 : cq_splits(n, n_seq, nh, nk, a.c.nb);
     a.tiles = (uint32_t)tiles;
     float* at = reinterpret_cast<float*>(workspace);
-    a.part_o = a.part_ml = a.lse = nullptr;
+    a.part_o = a.part_ml = a.lse = a.w_part = nullptr;
+    a.w_splits = weights ? cq_weight_splits(n, n_seq, nh, nk, a.c.nb) : 1;
+    if (a.w_splits > 1) {
+        a.w_part = at;
+        at += (size_t)a.w_splits * n_seq * nk * s_cap;
+    }
     if (few || a.splits > 1) {
         const uint64_t parts = few ? (uint64_t)units * nh * n : a.splits * rows;
         a.part_o = at;
@@ -1627,7 +1672,7 @@ extern "C" int t2h_flash_attn_prefill_q8(const void* q, void* const* cache, uint
     if (weights) a.lse = at;
     const uint64_t grid = few ? (uint64_t)units * nk : tiles * n_seq * nk * a.splits;
     const uint64_t merge = few ? ((uint64_t)n * a.group + 7) / 8 * n_seq * nk : (rows + 7) / 8;
-    const uint64_t wgrid = (uint64_t)n_seq * nk * ((a.c.nb + 3) / 4);
+    const uint64_t wgrid = (uint64_t)n_seq * nk * ((a.c.nb + 3) / 4) * a.w_splits;
     if (grid > 0x7fffffffu || merge > 0x7fffffffu || wgrid > 0x7fffffffu) return T2H_ERR_SHAPE;
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     if (few && n * a.group <= 16)
@@ -1649,6 +1694,11 @@ extern "C" int t2h_flash_attn_prefill_q8(const void* q, void* const* cache, uint
     if (weights) {
         hipLaunchKernelGGL(attn_chunk_q8_weights_kernel, dim3((uint32_t)wgrid), dim3(256), 0, st, a);
         T2H_LAUNCH_CHECK();
+        if (a.w_splits > 1) {
+            const uint64_t sums = ((uint64_t)n_seq * nk * s_cap + 1023) / 1024;
+            hipLaunchKernelGGL(attn_chunk_q8_weights_merge_kernel, dim3((uint32_t)sums), dim3(256), 0, st, a);
+            T2H_LAUNCH_CHECK();
+        }
     }
     return T2H_OK;
 }
