@@ -25,6 +25,10 @@ namespace t2h {
 //     relative to the wave's largest value scale times 2^12 (they stay normal over scales 2^26 apart);
 //   * the unfinished block's bf16 rows go through the bf16 products, a quarter a wave, q and weights in two bf16 terms.
 // The wave that holds the new token writes it; the four round its block if that is now whole, and then read it as codes.
+// Measured (32 / 8 heads): 32 sequences of 15000 to 16200 tokens 188 us, 5.5 TB/s of the cache's bytes, each read once; one of
+// 4096 tokens 11.2 us, of 200 8.0 us, where the chain of lengths, q, codes, products and join is what is left (an empty launch
+// takes 1.7).  Two waves a SIMD (184 registers hold a block's codes while the next one's are on their way): at three, with the
+// loads later, the long case took 10 % more.
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -608,7 +612,9 @@ __device__ __forceinline__ void dq_total(const DecodeQ8Args& a, const DecodeUnit
 constexpr int DQ_SEGMENT = 1024;  // tokens of a thread block that adds up weights
 
 // weights_out[token] = weights_in (0 for the new token) + sum of exp2(score - log2 sum) over the heads of the KV head:
-// 1024 tokens of a (sequence, KV head) a thread block.
+// 1024 tokens of a (sequence, KV head) a thread block.  A second kernel, because a token's weight needs the sum over all units:
+// the scores pass through memory (4 bytes a head and token beside the cache's 256 a KV head and token).  6.3 us for 16
+// sequences of 100 to 8000 tokens, beside the attention's 34.6.
 __global__ __launch_bounds__(256) void attn_decode_q8_weights_kernel(const DecodeQ8Args a) {
     __shared__ float lse[16];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -668,6 +674,13 @@ static uint32_t dq_units(uint32_t n_seq, uint32_t nk, uint32_t nb) {
 //   * scales go into the exponent: p of a block is exp2(s * ks + log2(vs / largest vs so far) - max); the accumulators follow a
 //     maximum only when it has grown by more than 2^2, and a scale when it has more than doubled.
 // Where there are few rows the keys are split over thread blocks, and a second kernel joins the parts.
+//
+// Measured (32 / 8 heads): 8 x 2048 tokens 320 us, 860 TFLOP/s of the pairs that are seen; a prompt of 16000 1060, where a bf16
+// product of 8192^3 reaches 1197; 1901 tokens 48 us; 4 x 512 of 16 / 8 heads at 7000 148 us, 820.  At 8 x 2048 the matrix cores
+// are busy for 39 % of the time and the vector units for 50 %: about 205 vector instructions and 32 products a step, half of the
+// former the softmax's, a fifth the conversion's.  What took vector instructions out of the step paid (320 us; 337 with LDS
+// addresses that depend on the buffer and a division a step); what let the two units overlap otherwise did not: a third buffer
+// with half of the waves a phase behind, raised priority around the products, fewer LDS conflicts (22 -> 9 million cycles).
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
@@ -703,8 +716,8 @@ __device__ __forceinline__ uint4 codes_bf16x8(uint32_t w0, uint32_t w1) {
                       pack_bf16x2(q8_value(w1, 0), q8_value(w1, 1)), pack_bf16x2(q8_value(w1, 2), q8_value(w1, 3)));
 }
 
-// LDS places of 16 bytes: keys [64][128] and values [128][64], 2 bytes each, chunks of a row permuted by the row so that
-// the lanes of an operand's read, which are rows, meet different banks.
+// LDS places of 16 bytes: keys and queries [64][128] and values [128][64], 2 bytes each, chunks of a row permuted by the row
+// (two rows of values fill the banks once) so that the lanes of an operand's read, which are rows, meet different banks.
 __device__ __forceinline__ int cq_key_at(int token, int chunk) { return token * 16 + (chunk ^ (token & 15)); }
 __device__ __forceinline__ int cq_value_at(int d, int chunk) { return d * 8 + (chunk ^ (d >> 1 & 7)); }
 
@@ -1011,7 +1024,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_chunk_q8_kernel(const Chun
     if (half == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * part) = make_float2(m, l);
 }
 
-// A row's parts joined: 8 rows a thread block, 32 lanes a row.
+// A row's parts joined: 8 rows a thread block, 32 lanes a row.  Bound by memory: 12 us for the 2 parts of 4 x 512 x 16 rows.
 __global__ __launch_bounds__(256) void attn_chunk_q8_merge_kernel(const ChunkQ8Args a) {
     const uint64_t all = (uint64_t)a.n_seq * a.c.nk * a.n * a.group;
     const uint64_t at = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -1051,8 +1064,10 @@ __global__ __launch_bounds__(256) void attn_chunk_q8_merge_kernel(const ChunkQ8A
 
 // weights_out[token] = weights_in (0 for a new token) + sum of exp2(score - lse) over the rows of the KV head.  A wave takes
 // 64 tokens, one cache block, as the operand that stays in registers; the rows' queries pass through LDS, 64 at a time and
-// the next 64 on their way, the same for the thread block's four waves.  Sums are in a fixed order.  Bound by the
-// exponentials, a quarter of a vector instruction's rate.
+// the next 64 on their way, the same for the thread block's four waves.  Sums are in a fixed order.  Bound by the products and
+// the three vector instructions a pair (scale, exponential, sum), which overlap little: 73 us for 4 x 512 tokens of 16 / 8
+// heads at 7000 (61 GFLOP, 237 million pairs).  Products of one half with the other half's exponentials between them took 5 %
+// more: with both halves' scores the registers do not hold the keys.
 __global__ __launch_bounds__(256, 2) void attn_chunk_q8_weights_kernel(const ChunkQ8Args a) {
     constexpr int STEP = 64;  // rows
     __shared__ __align__(16) uint4 queries[2][STEP * 16];
@@ -1226,6 +1241,7 @@ __global__ __launch_bounds__(256) void attn_chunk_q8_weights_merge_kernel(const 
 // Up to 32 rows of a KV head (a few drafted tokens): bound by memory like a single token, and read like one, in units of
 // blocks that a wave takes whole; the rows are the columns of one or two 16 x 16 x 32 products, each with its own last
 // token.  Their queries are bf16 already, so fp16 holds them in one term.  A second kernel joins a sequence's units.
+// Measured (32 / 8 heads): 2 x 5 tokens at 4000 14.2 us, 1 at 8000 and its join 12.7.
 template <int CT>
 __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_rows_q8_kernel(const ChunkQ8Args a) {
     constexpr int COLS = 16 * CT;
@@ -1475,7 +1491,7 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_rows_q8_kernel(const Ch
     }
 }
 
-// The units of a (sequence, KV head) joined, 8 rows a thread block, 32 lanes a row.
+// The units of a (sequence, KV head) joined, 8 rows a thread block, 32 lanes a row: 5 us for 2 x 5 tokens at 4000, latency.
 __global__ __launch_bounds__(256) void attn_rows_q8_merge_kernel(const ChunkQ8Args a) {
     const uint32_t rows = a.n * a.group, per = (rows + 7) / 8;
     const uint32_t h = blockIdx.x % a.c.nk, rest = blockIdx.x / a.c.nk;
@@ -1513,10 +1529,13 @@ __global__ __launch_bounds__(256) void attn_rows_q8_merge_kernel(const ChunkQ8Ar
     if (a.lse && d == 0) a.lse[((size_t)seq * a.c.nk + h) * rows + row] = M + log2f(L);
 }
 
-// Whether a KV head's rows are columns of the products of single tokens: up to two tiles of 16.
+// Whether a KV head's rows are columns of the products of single tokens: up to two tiles of 16 (three would not leave the
+// registers a block's codes).  Measured against the kernel of 32-row waves (32 / 8 heads): 1 token at 8000 12.7 us for 25.3,
+// 2 x 5 at 4000 17.7 for 19.9, 8 at 8000 17.7.
 static bool cq_few(uint32_t n, uint32_t nh, uint32_t nk) { return (uint64_t)n * (nh / nk) <= 32; }
 
-// Waves a thread block: 8 share a block's conversion to 16 bits where that leaves a thread block for every CU and more.
+// Waves a thread block: 8 share a block's conversion to 16 bits where that leaves two thread blocks for every CU.  Measured (32 /
+// 8 heads): 16000 tokens 942 TFLOP/s of 8, 912 of 4; 1901 tokens, 240 and 480 thread blocks, 78 us of 8, 68 of 4.
 static uint32_t cq_waves(uint32_t n, uint32_t n_seq, uint32_t nh, uint32_t nk) {
     return ((uint64_t)n * (nh / nk) + 255) / 256 * n_seq * nk >= CQ_WIDE_GRID ? 8 : 4;
 }

@@ -12,7 +12,9 @@ namespace t2h {
 // q and k; q goes out in bf16, k and v go to the cache.  Bound by memory: a token's q, k and v are read once in fp32.
 // One launch holds two kinds of blocks: those of q (a wave takes 8 heads of a token), and one for each (sequence, cache
 // block that the chunk touches, KV head), which holds the 64 tokens in registers because a finished block's scale needs
-// all of them before the first is rounded.
+// all of them before the first is rounded.  Measured: 8 ragged prompts of 900 to 2048 tokens, 32 / 8 heads, 95 us for
+// 446 MB, 4.7 TB/s (a large copy reaches 4.8); 512 tokens of 16 / 8 heads 8.1 us, the latency of a block's rows, angles and
+// scale in turn.
 
 struct Q8WriteArgs {
     const float* q;
@@ -202,7 +204,8 @@ __global__ __launch_bounds__(Q8W_WAVES * 64) void q8_write_kernel(const Q8WriteA
 // ------------------------------------------------------------------------------------------------- read back --
 //
 // The cache's values as the token-major bf16 rows [n_seq][s_cap][nk][128] of the framework's other caches, code times
-// scale rounded once; zeros from the length on.  Bound by the bf16 rows that it writes.
+// scale rounded once; zeros from the length on.  Bound by the bf16 rows that it writes: 38 us for 8
+// sequences of 4096 tokens and a tail, 8 heads: 67 MB read and 137 written, 5.4 TB/s.
 
 struct Q8ReadArgs {
     KvQ8 c;
@@ -282,6 +285,11 @@ __global__ __launch_bounds__(256) void q8_read_kernel(const Q8ReadArgs a) {
 // The choice is a radix selection of the last weight that stays, 11 + 11 + 10 bits of an order-preserving key, each
 // digit one pass over the weights and a histogram in LDS; then ballots give each token its place.  A second kernel moves
 // the tokens: block by block it gathers 64 of them, finds their new scale and rounds them again.
+//
+// Measured: 8 sequences of 9000 to 16300 tokens, 8 heads, brought to 64 blocks: selection 23 us, one thread block a head, bound
+// by the chain of three digits (the keys stay in registers up to 16384 tokens; more are read again for every pass: 60000 tokens
+// 95 us); moving 57 us, 145 MB read and 70 written, 3.8 TB/s.  A token's values are a byte of each of its block's 128 rows, so
+// that all rows of a block with any token that stays are read, while its keys are 128 bytes in a row.
 
 struct Q8EvictArgs {
     KvQ8 c, o;
