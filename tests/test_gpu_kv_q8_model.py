@@ -68,6 +68,25 @@ def test_graphs_replay_the_eager_steps(weights):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("more", [20, 90])
+def test_a_graphed_prompt_behind_another(weights, more):
+    """The warm-up that a captured prefill begins with leaves the unfinished block and the weights of the tokens before it as
+    they were."""
+    g = torch.Generator().manual_seed(5)
+    first, then = torch.randint(0, 1000, (100,), generator=g), torch.randint(0, 1000, (more,), generator=g)
+    runs = []
+    for graphs in (False, True):
+        d = decoder(weights, kv_bits=8, kv_weights=True)
+        d.prefill_chunked(first)
+        (d.prefill_graphed if graphs else d.prefill_chunked)(then, start=100, chunk=64)
+        n = int(d.position)
+        assert n == 100 + more
+        runs.append((d.generated.clone(), torch.stack(d.kv_weights)[..., :n], *K.kv_cache_q8_dequantize(d.kv[0], d.position),
+                     *K.kv_cache_q8_dequantize(d.kv[1], d.position)))
+    for a, b in zip(*runs):
+        assert torch.equal(a, b)
+
+
 def test_eviction_in_the_loop(weights):
     """A prompt, steps, an eviction and steps from the same graph: weights count every query once, positions go on, and the
     kept tokens' keys are the old ones to half a code."""

@@ -541,11 +541,14 @@ class Qwen3Decoder:
             while len(self._prefill_graphs) >= self.PREFILL_GRAPHS:
                 self._prefill_graphs.pop(next(iter(self._prefill_graphs)))
             buf = ids.clone()
+            saved = [(t, t.clone()) for t in self._behind(start)]
             side = torch.cuda.Stream(device=self.device)
             side.wait_stream(torch.cuda.current_stream(self.device))
             with torch.cuda.stream(side):
                 self.prefill_chunked(buf, start=start, chunk=chunk)  # warm-up launch outside capture
             torch.cuda.current_stream(self.device).wait_stream(side)
+            for t, was in saved:
+                t.copy_(was)
             g = torch.cuda.CUDAGraph()
             with torch.cuda.graph(g):
                 self.prefill_chunked(buf, start=start, chunk=chunk)
@@ -553,6 +556,13 @@ class Qwen3Decoder:
         g, buf = self._prefill_graphs[key]
         buf.copy_(ids)
         g.replay()
+
+    def _behind(self, start: int) -> list[torch.Tensor]:
+        """What a prefill from ``start`` changes of the tokens before it: in an 8-bit cache it takes over the unfinished
+        block's rows and adds to their weights."""
+        if self.kv_bits != 8 or start == 0:
+            return []
+        return [t for c in self.kv for t in (c.k_tail, c.v_tail)] + list(self.kv_weights or ())
 
     def clear_prefill_graphs(self) -> None:
         """Drop every captured prefill graph and its memory pool."""
