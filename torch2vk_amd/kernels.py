@@ -1876,20 +1876,28 @@ def kv_cache_q8_dequantize(cache: KVCacheQ8, lengths: torch.Tensor, k_out: torch
                            v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The cache's keys and values as bf16 [n_seq, s_cap, nk, 128], the layout of the other caches; zeros behind
     ``lengths``."""
-    _q8_here(cache, "lengths k_out v_out", lengths, k_out, v_out)
-    if lengths is None or not _q8_plain(lengths, torch.int32, cache.n_seq, cache.at):
+    try:
+        n_seq, at = cache.n_seq, cache.at
+        shape = (n_seq, cache.s_cap, cache.nk, 128)
+        ok = at == torch._C._cuda_getDevice() and lengths is not None and _q8_plain(lengths, torch.int32, n_seq, at)
+        for t in (k_out, v_out):
+            ok = ok and (t is None or t.shape == shape and _q8_plain(t, torch.bfloat16, t.numel(), at))
+    except AttributeError:
+        ok = False
+    if not ok:
+        _q8_here(cache, "lengths k_out v_out", lengths, k_out, v_out)
         _check(lengths, "lengths", torch.int32, align=4)
         _q8_refuse_ints(cache.n_seq, lengths=lengths)
-    shape = (cache.n_seq, cache.s_cap, cache.nk, 128)
-    for t, name in ((k_out, "k_out"), (v_out, "v_out")):
-        if t is not None:
-            _check(t, name, torch.bfloat16)
-            if tuple(t.shape) != shape:
-                raise ValueError(f"{name} must be bf16 {shape}, got {tuple(t.shape)}")
+        for t, name in ((k_out, "k_out"), (v_out, "v_out")):
+            if t is not None:
+                _check(t, name, torch.bfloat16)
+                if tuple(t.shape) != shape:
+                    raise ValueError(f"{name} must be bf16 {shape}, got {tuple(t.shape)}")
+        raise ValueError("the tensors of a call must be on one device")
     if k_out is None:
-        k_out = torch.empty(shape, dtype=torch.bfloat16, device=cache.k.device)
+        k_out = torch.empty(shape, dtype=torch.bfloat16, device=lengths.device)
     if v_out is None:
-        v_out = torch.empty(shape, dtype=torch.bfloat16, device=cache.k.device)
+        v_out = torch.empty(shape, dtype=torch.bfloat16, device=lengths.device)
     call("t2h_kv_cache_q8_dequantize", cache.ptrs, cache.s_cap, lengths.data_ptr(), cache.n_seq, cache.nk, 128,
          k_out.data_ptr(), v_out.data_ptr(), stream_handle())
     return k_out, v_out
@@ -1905,9 +1913,26 @@ def kv_cache_q8_evict(cache: KVCacheQ8, lengths: torch.Tensor, weights: torch.Te
     -1) and the new lengths; ``lengths`` itself is not changed, so that every layer of a model can be evicted by it.
     A decode that goes on adds lengths - new lengths to its ``rope_offsets``."""
     dest = cache if out is None else out
-    _q8_here(cache, "lengths weights weights_out", lengths, weights, weights_out)
-    _q8_here(dest, "")
-    n_seq, nk = cache.n_seq, cache.nk
+    if weights_out is None:
+        weights_out = weights
+    try:
+        n_seq, nk, at = cache.n_seq, cache.nk, cache.at
+        ok = (at == torch._C._cuda_getDevice() and dest.at == at and lengths is not None
+              and _q8_plain(lengths, torch.int32, n_seq, at) and weights.shape == (n_seq, nk, cache.s_cap)
+              and _q8_plain(weights, torch.float32, weights.numel(), at) and weights_out.shape == (n_seq, nk, dest.s_cap)
+              and _q8_plain(weights_out, torch.float32, weights_out.numel(), at))
+    except AttributeError:
+        ok = False
+    if not ok:
+        _q8_here(cache, "lengths weights weights_out", lengths, weights, weights_out)
+        _q8_here(dest, "")
+        _check(lengths, "lengths", torch.int32, align=4)
+        _q8_refuse_ints(n_seq, lengths=lengths)
+        for t, name, cap in ((weights, "weights", cache.s_cap), (weights_out, "weights_out", dest.s_cap)):
+            _check(t, name, torch.float32, align=4)
+            if tuple(t.shape) != (n_seq, nk, cap):
+                raise ValueError(f"{name} must be fp32 {(n_seq, nk, cap)}, got {tuple(t.shape)}")
+        raise ValueError("the tensors of a call must be on one device")
     if dest.n_seq != n_seq or dest.nk != nk:
         raise ValueError(f"out must hold {n_seq} sequences of {nk} heads, got {dest.n_seq} of {dest.nk}")
     if keep_blocks < 1:
@@ -1916,16 +1941,8 @@ def kv_cache_q8_evict(cache: KVCacheQ8, lengths: torch.Tensor, weights: torch.Te
         raise ValueError(f"sink + recent must be 0 to {KV_Q8_BLOCK * keep_blocks}, got {sink} + {recent}")
     if dest.s_cap < min(cache.s_cap, KV_Q8_BLOCK * (keep_blocks + 1)):
         raise ValueError(f"out holds {dest.s_cap} tokens, {KV_Q8_BLOCK * (keep_blocks + 1)} may stay")
-    if weights_out is None:
-        weights_out = weights
-    _check(lengths, "lengths", torch.int32, align=4)
-    _q8_refuse_ints(n_seq, lengths=lengths)
-    for t, name, cap in ((weights, "weights", cache.s_cap), (weights_out, "weights_out", dest.s_cap)):
-        _check(t, name, torch.float32, align=4)
-        if tuple(t.shape) != (n_seq, nk, cap):
-            raise ValueError(f"{name} must be fp32 {(n_seq, nk, cap)}, got {tuple(t.shape)}")
-    kept = torch.empty(n_seq, nk, KV_Q8_BLOCK * keep_blocks, dtype=torch.int32, device=cache.k.device)
+    kept = torch.empty(n_seq, nk, KV_Q8_BLOCK * keep_blocks, dtype=torch.int32, device=lengths.device)
     new = torch.empty_like(lengths)
-    call("t2h_kv_cache_q8_evict", cache.ptrs, cache.s_cap, ptr(lengths), ptr(weights), keep_blocks, sink, recent, n_seq,
-         nk, 128, dest.ptrs, dest.s_cap, ptr(weights_out), ptr(kept), ptr(new), stream_handle())
+    call("t2h_kv_cache_q8_evict", cache.ptrs, cache.s_cap, lengths.data_ptr(), weights.data_ptr(), keep_blocks, sink, recent,
+         n_seq, nk, 128, dest.ptrs, dest.s_cap, weights_out.data_ptr(), kept.data_ptr(), new.data_ptr(), stream_handle())
     return kept, new
