@@ -266,7 +266,8 @@ def test_blocks_of_zeros_tiny_and_broken_values(device):
     (8, 1, [62, 63, 64, 65, 127, 128, 190], 192, True), (16, 1, [-1, 5, 192, 500, 191], 192, True),
     (6, 2, [300, 17], 448, True), (5, 1, [1000], 1024, False), (16, 8, [200], 2048, False), (32, 8, [4100], 8192, True),
     (12, 4, [0, 9000, 3, 500, 20000], 20032, True), (8, 8, [700, 64, 1, 129], 768, False),
-    (8, 2, list(range(0, 4000, 57)), 4032, True), (20, 4, [70000], 70016, True)])
+    (8, 2, list(range(0, 4000, 57)), 4032, True), (20, 4, [70000], 70016, True),
+    (4, 2, list(range(3000, -100, -20)), 3008, True)])
 def test_decode(device, nh, nk, lengths, s_cap, weights):
     print("decode", nh, nk, lengths[:8], s_cap, weights, flush=True)
     n_seq, group = len(lengths), nh // nk

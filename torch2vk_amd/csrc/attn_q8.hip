@@ -25,7 +25,7 @@ namespace t2h {
 //     relative to the wave's largest value scale times 2^12 (they stay normal over scales 2^26 apart);
 //   * the unfinished block's bf16 rows go through the bf16 products, a quarter a wave, q and weights in two bf16 terms.
 // The wave that holds the new token writes it; the four round its block if that is now whole, and then read it as codes.
-// Measured (32 / 8 heads): 32 sequences of 15000 to 16200 tokens 188 us, 5.5 TB/s of the cache's bytes, each read once; one of
+// Measured (32 / 8 heads): 32 sequences of 15000 to 16200 tokens 181 us, 5.6 TB/s of the cache's bytes, each read once; one of
 // 4096 tokens 11.2 us, of 200 8.0 us, where the chain of lengths, q, codes, products and join is what is left (an empty launch
 // takes 1.7).  Two waves a SIMD (184 registers hold a block's codes while the next one's are on their way): at three, with the
 // loads later, the long case took 10 % more.
@@ -39,7 +39,7 @@ constexpr int DQ_WAVES = 4;
 constexpr int DQ_ROW = Q8_D + 4;          // fp32 row in LDS, padded
 constexpr int DQ_QROW = Q8_D + 8;         // fp16 row
 constexpr uint32_t DQ_SLOTS = 512;        // thread blocks that the chip holds at once
-constexpr uint32_t DQ_CHUNK_MAX = 64;     // blocks a unit, at most
+constexpr uint32_t DQ_CHUNK_MAX = 32;     // blocks a unit, at most
 constexpr float DQ_P_SCALE = 4096.0f;
 
 struct DecodeQ8Args {
@@ -78,39 +78,43 @@ struct UnitsOf {
 };
 
 struct DecodeUnit {
-    uint32_t seq, first, count;  // the sequence, its first unit and how many it has
+    uint32_t seq, first, count;  // the sequence, where its parts begin and how many units it has
+    int part;                    // the unit among them
     int chunk, blocks, len;      // blocks a unit, the sequence's blocks and its length before the call
 };
 
+// Sums over the lanes up to each: within rows of 16, then over the rows.
 __device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const uint32_t o = (uint32_t)__shfl_up((int)v, off, T2H_WAVE);
-        if (lane >= off) v += o;
-    }
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);  // 1 lane up
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);  // a row's last lane to the odd rows
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);  // lane 31 to the upper half
     return v;
 }
 
 // Blocks a unit, for the blocks of all sequences: 4 (one a wave) for short ones, then one thread block a CU until units have
-// 8, then two a CU, which the registers allow, until units have 64, where what a unit costs besides its blocks (3 to 4 us:
-// lengths, q, joining) no longer matters and ragged lengths want the chip refilled.  Measured (32 / 8 heads): 16000 tokens
-// 15.1 us in units of 8 against 18.3 of 4; 16 sequences of 100 to 8000 34.9 us of 16 against 43.7 of 32; 32 of 15000 to
-// 16200 184 us of 64, 193 of 32, 206 of 16.
-__host__ __device__ __forceinline__ uint32_t dq_chunk(uint64_t total, uint32_t nk) {
-    const uint64_t one = (total * nk + 255) / 256, two = (total * nk + DQ_SLOTS - 1) / DQ_SLOTS;
+// 8, then two a CU, which the registers allow, or one where the sequences' heads alone are that many, until units have 32,
+// where what a unit costs besides its blocks (3 to 4 us: lengths, q, joining) no longer matters and ragged lengths want the chip
+// refilled.  Measured (us, 32 / 8 heads but for the third): 1 of 16000 15.1 in units of 8, 18.3 of 4; 16 of 100 to 8000 39 of
+// 20, 44 of 12, 46 of 32; 128 of 300 to 1200, 4 KV heads, 32 at one a CU, 38 at two; 64 of 100 to 16000 209 of up to 32, 219 of 64.
+__device__ __forceinline__ uint32_t dq_chunk(uint64_t total, uint32_t n_seq, uint32_t nk) {
+    const uint64_t one = (total * nk + 255) / 256, two = (total * nk * (n_seq * nk >= DQ_SLOTS / 2 ? 2 : 1) + DQ_SLOTS - 1) / DQ_SLOTS;
     const uint64_t c = one <= 8 ? one : (two > 8 ? two : 8);
     return c <= DQ_WAVES ? DQ_WAVES : c >= DQ_CHUNK_MAX ? DQ_CHUNK_MAX : (uint32_t)((c + DQ_WAVES - 1) / DQ_WAVES * DQ_WAVES);
 }
 
-// The sequence that unit `unit` belongs to (by_seq false), or sequence `unit` itself; false where there is none.  A
-// sequence without blocks has one unit, which writes its zeros.
+// The unit `unit` (by_seq false), or sequence `unit`; false where there is none.  Units of a whole chunk come first, the
+// sequences' last, shorter ones behind them, so that what the chip ends with is short (64 sequences of 100 to 16000
+// tokens: 219 us, 240 sequence by sequence).  A sequence without blocks has one unit, which writes its zeros.
 __device__ bool dq_find(const UnitsOf& a, uint32_t unit, bool by_seq, DecodeUnit& u) {
     const uint32_t lane = threadIdx.x & 63;
     if (a.n_seq == 1) {
         u.blocks = a.blocks(0);
-        u.chunk = (int)dq_chunk((uint64_t)u.blocks, a.nk);
+        u.chunk = (int)dq_chunk((uint64_t)u.blocks, 1, a.nk);
         u.seq = u.first = 0;
+        u.part = (int)unit;
         u.count = u.blocks ? (uint32_t)((u.blocks + u.chunk - 1) / u.chunk) : 1u;
         u.len = a.lengths[0];
         return by_seq || unit < u.count;
@@ -118,24 +122,35 @@ __device__ bool dq_find(const UnitsOf& a, uint32_t unit, bool by_seq, DecodeUnit
     uint32_t total = 0;
     for (uint32_t i = lane; i < a.n_seq; i += 64) total += (uint32_t)a.blocks(i);
     total = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan_u32(total), 63);
-    u.chunk = (int)dq_chunk(total, a.nk);
-    uint32_t before = 0;
+    u.chunk = (int)dq_chunk(total, a.n_seq, a.nk);
+    uint32_t fulls = 0;  // units of a whole chunk
+    if (!by_seq) {
+        for (uint32_t i = lane; i < a.n_seq; i += 64) fulls += (uint32_t)a.blocks(i) / (uint32_t)u.chunk;
+        fulls = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan_u32(fulls), 63);
+    }
+    uint32_t before = 0, fulls_before = 0;
     for (uint32_t base = 0; base < a.n_seq; base += 64) {
         const uint32_t i = base + lane;
-        const uint32_t n = i < a.n_seq ? (uint32_t)a.blocks(i) : 0u;
+        const uint32_t n = i < a.n_seq ? (uint32_t)a.blocks(i) : 0u, full = n / (uint32_t)u.chunk;
         const uint32_t mine = i < a.n_seq ? (n ? (n + u.chunk - 1) / u.chunk : 1u) : 0u;
-        const uint32_t upto = before + wave_scan_u32(mine);
-        const uint64_t hit = by_seq ? __ballot(i == unit) : __ballot(unit >= upto - mine && unit < upto);
+        const uint32_t upto = before + wave_scan_u32(mine), fulls_upto = fulls_before + wave_scan_u32(full);
+        const uint32_t rest_upto = upto - fulls_upto;  // units of less than a chunk, up to one a sequence
+        const bool is_full = unit < fulls;
+        const uint64_t hit = by_seq    ? __ballot(i == unit)
+                             : is_full ? __ballot(unit >= fulls_upto - full && unit < fulls_upto)
+                                       : __ballot(mine > full && unit - fulls == rest_upto - 1);
         if (hit) {
             const int at = __builtin_ctzll(hit);
             u.seq = base + at;
             u.count = (uint32_t)__builtin_amdgcn_readlane((int)mine, at);
             u.first = (uint32_t)__builtin_amdgcn_readlane((int)(upto - mine), at);
+            u.part = is_full ? (int)(unit - (uint32_t)__builtin_amdgcn_readlane((int)(fulls_upto - full), at)) : (int)u.count - 1;
             u.blocks = a.blocks(u.seq);
             u.len = a.lengths[u.seq];
             return true;
         }
         before = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+        fulls_before = (uint32_t)__builtin_amdgcn_readlane((int)fulls_upto, 63);
     }
     return false;
 }
@@ -193,7 +208,7 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_decode_q8_kernel(const 
         for (int i = tid; i < group * (Q8_D / 2); i += DQ_WAVES * 64) out[i] = 0u;
         return;
     }
-    const int b0 = (int)(unit - u.first) * u.chunk;
+    const int b0 = u.part * u.chunk;
     const int b1 = b0 + u.chunk < u.blocks ? b0 + u.chunk : u.blocks;
     const int c = lane & 15, g4 = lane >> 4;
     const bool has_new = u.len < (int)(a.c.nb * Q8_BLOCK);
@@ -516,7 +531,7 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_decode_q8_kernel(const 
             L = fmaf(f, wml[w][g][1], L);
             sum += *reinterpret_cast<const f32x4*>(&wo[w][g][d]) * f;
         }
-        const size_t part = ((size_t)unit * a.c.nk + h) * a.group + g;
+        const size_t part = ((size_t)(u.first + (uint32_t)u.part) * a.c.nk + h) * a.group + g;
         if (u.count == 1) {
             const float inv = 1.0f / L;
             out[(g * Q8_D + d) / 2] = pack_bf16x2(sum[0] * inv, sum[1] * inv);
@@ -1259,7 +1274,7 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_rows_q8_kernel(const Ch
     const Q8Span s = q8_span(a.lengths, a.counts, u.seq, a.n, a.c.nb);
     int count = a.counts ? a.counts[u.seq] : (int)a.n;
     count = u.blocks == 0 ? 0 : (count < (int)a.n ? count : (int)a.n);
-    const int b0 = (int)(unit - u.first) * u.chunk;
+    const int b0 = u.part * u.chunk;
     const int b1 = b0 + u.chunk < u.blocks ? b0 + u.chunk : u.blocks;
     const int c = lane & 15, g4 = lane >> 4;
     const int tail_b = s.end % Q8_BLOCK ? s.end / Q8_BLOCK : -1;
@@ -1484,7 +1499,7 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_rows_q8_kernel(const Ch
                 make_uint2(pack_bf16x2(sum[0] * inv, sum[1] * inv), pack_bf16x2(sum[2] * inv, sum[3] * inv));
             if (a.lse && d == 0) a.lse[((size_t)u.seq * a.c.nk + h) * rows + row] = M + log2f(L);
         } else {
-            const size_t part = ((size_t)unit * a.c.nk + h) * rows + row;
+            const size_t part = ((size_t)(u.first + (uint32_t)u.part) * a.c.nk + h) * rows + row;
             *reinterpret_cast<f32x4*>(a.part_o + part * Q8_D + d) = sum;
             if (d == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * part) = make_float2(M, L);
         }
