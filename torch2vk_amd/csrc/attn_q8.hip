@@ -83,17 +83,6 @@ struct DecodeUnit {
     int chunk, blocks, len;      // blocks a unit, the sequence's blocks and its length before the call
 };
 
-// Sums over the lanes up to each: within rows of 16, then over the rows.
-__device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v) {
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);  // 1 lane up
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);  // a row's last lane to the odd rows
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);  // lane 31 to the upper half
-    return v;
-}
-
 // Blocks a unit, for the blocks of all sequences: 4 (one a wave) for short ones, then one thread block a CU until units have
 // 8, then two a CU, which the registers allow, or one where the sequences' heads alone are that many, until units have 32,
 // where what a unit costs besides its blocks (3 to 4 us: lengths, q, joining) no longer matters and ragged lengths want the chip

@@ -74,6 +74,17 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
     return v;
 }
 
+// Sums over the lanes up to each: within rows of 16, then over the rows.
+__device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v) {
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);  // 1 lane up
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);  // a row's last lane to the odd rows
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);  // lane 31 to the upper half
+    return v;
+}
+
 // A block's scale and the factor that its values are multiplied by before rounding, from the bits of its max|x|.
 // Values under 1.3e-28 are held as zeros; a block with a NaN or an infinity has a NaN scale, so that whoever reads it
 // sees NaN and not numbers.

@@ -366,12 +366,7 @@ __global__ __launch_bounds__(EV_THREADS) void q8_evict_select_kernel(const Q8Evi
         __syncthreads();
         // bins from the top: thread i holds bins 2047 - 2 i and 2046 - 2 i
         const uint32_t c0 = hist[2047 - 2 * tid], c1 = hist[2046 - 2 * tid];
-        uint32_t run = c0 + c1;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const uint32_t o = (uint32_t)__shfl_up((int)run, off, T2H_WAVE);
-            if (lane >= off) run += o;
-        }
+        const uint32_t run = wave_scan_u32(c0 + c1);
         if (lane == 63) wsum[wave][0] = run;
         __syncthreads();
         uint32_t before = run - c0 - c1;
