@@ -503,7 +503,8 @@ def evicted(c, i, w, length, keep, sink, recent):
 @pytest.mark.parametrize("nk,lengths,s_cap,keep,sink,recent,kind", [
     (2, [130], 192, 1, 0, 0, "random"), (1, [64, 63, 0, -1], 128, 1, 0, 0, "random"), (2, [500, 300, 700], 704, 4, 4, 64, "ties"),
     (8, [4100], 4160, 32, 4, 128, "random"), (2, [640], 640, 3, 100, 92, "random"), (1, [5000], 5056, 1, 0, 64, "zeros"),
-    (2, [1000], 1024, 7, 1, 30, "special"), (2, [20000, 9000], 20032, 150, 4, 1000, "ties")])
+    (2, [1000], 1024, 7, 1, 30, "special"), (2, [20000, 9000], 20032, 150, 4, 1000, "ties"),
+    (1, [70000, 60000], 70016, 300, 4, 500, "special")])
 @pytest.mark.parametrize("in_place", [False, True])
 def test_evict(device, nk, lengths, s_cap, keep, sink, recent, kind, in_place):
     print("evict", nk, lengths, keep, sink, recent, kind, in_place, flush=True)

@@ -317,8 +317,9 @@ __device__ __forceinline__ uint32_t evict_key(const float* w, int t, int full, c
 
 constexpr int EV_THREADS = 1024;
 constexpr int EV_WAVES = EV_THREADS / 64;
-constexpr int EV_BATCH = 16;  // keys a lane holds
+constexpr int EV_SMALL = 16384;  // tokens that 16 keys a lane hold; 64 hold 65536, the most that the registers of 16 waves do
 
+template <int EV_BATCH>
 __global__ __launch_bounds__(EV_THREADS) void q8_evict_select_kernel(const Q8EvictArgs a) {
     __shared__ uint32_t hist[2048];
     __shared__ uint32_t wsum[EV_WAVES][2];
@@ -335,7 +336,7 @@ __global__ __launch_bounds__(EV_THREADS) void q8_evict_select_kernel(const Q8Evi
     if (stay == full) return;
     const float* w = a.w_in + (size_t)blockIdx.x * a.c.nb * Q8_BLOCK;
 
-    // each wave takes a run of tokens, EV_BATCH rows of 64 at a time in registers; up to 16384 tokens are loaded once
+    // each wave takes a run of tokens, EV_BATCH rows of 64 at a time in registers; up to 1024 EV_BATCH tokens are loaded once
     const int per = ((full + EV_WAVES - 1) / EV_WAVES + 63) / 64 * 64;
     const int t0 = wave * per + lane, t1 = wave * per + per < full ? wave * per + per : full;
     const bool once = per <= EV_BATCH * 64;
@@ -427,7 +428,7 @@ __global__ __launch_bounds__(EV_THREADS) void q8_evict_select_kernel(const Q8Evi
 // Keys (blockIdx.y 0, with the weights) or values (1) of one head: output blocks job, job + jobs, ...  Where the output
 // is the input's own cache one thread block walks a head's blocks in order: token i of the output comes from a token
 // j >= i, so block b is read before it is overwritten, and no later block needs what it overwrites.
-__global__ __launch_bounds__(256) void q8_evict_move_kernel(const Q8EvictArgs a) {
+__global__ __launch_bounds__(256, 7) void q8_evict_move_kernel(const Q8EvictArgs a) {
     __shared__ int from[Q8_BLOCK];
     __shared__ float fs[Q8_BLOCK];
     __shared__ uint32_t red[4];
@@ -467,6 +468,8 @@ __global__ __launch_bounds__(256) void q8_evict_move_kernel(const Q8EvictArgs a)
             uint32_t* u = reinterpret_cast<uint32_t*>(x);
 #pragma unroll
             for (int i = 0; i < 32; ++i) top = max(top, abs_bits(q8_value(u[i / 4], i % 4) * f));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(u[i]));
             const float wt = tid < Q8_BLOCK ? w_in[from[tid]] : 0.0f;
             top = wave_max_u32(top);
             if (lane == 0) red[wave] = top;
@@ -485,11 +488,19 @@ __global__ __launch_bounds__(256) void q8_evict_move_kernel(const Q8EvictArgs a)
             const int t = from[lane];
             const float f = fs[lane];
             const int8_t* src = a.c.v + a.c.block_at(seq, (uint32_t)t / Q8_BLOCK, h) + (size_t)wave * 32 * Q8_BLOCK + t % Q8_BLOCK;
-            int8_t x[32];
+            uint32_t u[8];  // 4 dims a word: the kernel waits for memory, and more registers would be fewer waves that do
+            {
+                uint8_t x[32];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] = src[i * Q8_BLOCK];
+                for (int i = 0; i < 32; ++i) x[i] = (uint8_t)src[i * Q8_BLOCK];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) top = max(top, abs_bits((float)x[i] * f));
+                for (int i = 0; i < 8; ++i)
+                    u[i] = (uint32_t)x[4 * i] | (uint32_t)x[4 * i + 1] << 8 | (uint32_t)x[4 * i + 2] << 16 | (uint32_t)x[4 * i + 3] << 24;
+            }
+#pragma unroll
+            for (int i = 0; i < 32; ++i) top = max(top, abs_bits(q8_value(u[i / 4], i % 4) * f));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(u[i]));  // (unpacked again below, not kept)
             top = wave_max_u32(top);
             if (lane == 0) red[wave] = top;
             __syncthreads();
@@ -499,7 +510,7 @@ __global__ __launch_bounds__(256) void q8_evict_move_kernel(const Q8EvictArgs a)
             int8_t* dst = a.o.v + to + (size_t)wave * 32 * Q8_BLOCK + lane;
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
-                int w = (all ? (int)x[i] : q8_code((float)x[i] * f, inv)) & 255;
+                int w = (all ? (int)(u[i / 4] >> (8 * (i % 4))) : q8_code(q8_value(u[i / 4], i % 4) * f, inv)) & 255;
                 w |= __builtin_amdgcn_update_dpp(0, w, 0xB1, 0xf, 0xf, true) << 8;   // lane ^ 1
                 w |= __builtin_amdgcn_update_dpp(0, w, 0x4E, 0xf, 0xf, true) << 16;  // lane ^ 2
                 if ((lane & 3) == 0) *reinterpret_cast<int*>(dst + i * Q8_BLOCK) = w;
@@ -613,7 +624,10 @@ extern "C" int t2h_kv_cache_q8_evict(void* const* cache, uint32_t s_cap, const i
     a.jobs = same || weights == weights_out ? 1 : most;
     const uint64_t grid = (uint64_t)n_seq * a.jobs * nk;
     if (grid > 0x7fffffffu) return T2H_ERR_SHAPE;
-    hipLaunchKernelGGL(q8_evict_select_kernel, dim3(n_seq * nk), dim3(EV_THREADS), 0, reinterpret_cast<hipStream_t>(stream), a);
+    if (s_cap <= EV_SMALL)
+        hipLaunchKernelGGL(q8_evict_select_kernel<16>, dim3(n_seq * nk), dim3(EV_THREADS), 0, reinterpret_cast<hipStream_t>(stream), a);
+    else
+        hipLaunchKernelGGL(q8_evict_select_kernel<64>, dim3(n_seq * nk), dim3(EV_THREADS), 0, reinterpret_cast<hipStream_t>(stream), a);
     T2H_LAUNCH_CHECK();
     hipLaunchKernelGGL(q8_evict_move_kernel, dim3((uint32_t)grid, 2), dim3(256), 0, reinterpret_cast<hipStream_t>(stream), a);
     T2H_LAUNCH_CHECK();
