@@ -287,9 +287,11 @@ __global__ __launch_bounds__(256) void q8_read_kernel(const Q8ReadArgs a) {
 // the tokens: block by block it gathers 64 of them, finds their new scale and rounds them again.
 //
 // Measured: 8 sequences of 9000 to 16300 tokens, 8 heads, brought to 64 blocks: selection 23 us, one thread block a head, bound
-// by the chain of three digits (the keys stay in registers up to 16384 tokens; more are read again for every pass: 60000 tokens
-// 95 us); moving 57 us, 145 MB read and 70 written, 3.8 TB/s.  A token's values are a byte of each of its block's 128 rows, so
-// that all rows of a block with any token that stays are read, while its keys are 128 bytes in a row.
+// by the chain of three digits and by what one CU issues (60000 tokens, both kernels: 73 us with the keys in registers, 112 with
+// keys read again for every pass); moving 56 us, 145 MB read and 70 written, 3.8 TB/s.  A token's values are a byte of each of
+// its block's 128 rows, so that all rows of a block with any token that stays are read, while its keys are 128 bytes in a row.
+// Taking those rows through LDS whole, with loads straight into it, was 4 % faster where all of a large batch's blocks lie
+// close (32 of 16000: 365 us for 379) and 4 % slower at 8 sequences; through registers it was slower throughout.
 
 struct Q8EvictArgs {
     KvQ8 c, o;
