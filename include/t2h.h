@@ -640,11 +640,13 @@ int t2h_kv_cache_q8_dequantize(void* const* cache, uint32_t s_cap, const int32_t
  * -1.  lengths_out [n_seq] (not lengths itself): the lengths after it; rope_offsets grow by what a length lost.
  * weights_out [n_seq, nk, s_cap_out]: the weights of what stays (elements behind it are left).
  * cache_out and weights_out are the inputs themselves, or distinct and of a capacity s_cap_out >= 64 (keep_blocks + 1) or
- * >= s_cap. */
+ * >= s_cap.  workspace: needed where either is the input itself, 16-byte aligned, no initialisation; calls that share one must
+ * not overlap in time. */
+size_t t2h_kv_cache_q8_evict_workspace_bytes(uint32_t keep_blocks, uint32_t n_seq, uint32_t nk, uint32_t s_cap);
 int t2h_kv_cache_q8_evict(void* const* cache, uint32_t s_cap, const int32_t* lengths, const float* weights,
                           uint32_t keep_blocks, uint32_t sink, uint32_t recent, uint32_t n_seq, uint32_t nk, uint32_t d,
                           void* const* cache_out, uint32_t s_cap_out, float* weights_out, int32_t* kept,
-                          int32_t* lengths_out, void* stream);
+                          int32_t* lengths_out, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

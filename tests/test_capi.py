@@ -167,7 +167,7 @@ def test_kv_q8_argument_validation(lib):
         nb=1 << 20, st=None), **m}.values())
     evict = lambda **m: lib.t2h_kv_cache_q8_evict(*{**dict(  # noqa: E731
         c=c, cap=128, ln=fake, w=fake, keep=1, sink=0, recent=0, s=1, nk=2, d=128, o=c, ocap=128, wo=fake, kept=fake, lo=0x5000,
-        st=None), **m}.values())
+        ws=fake, nb=1 << 20, st=None), **m}.values())
     read = lambda **m: lib.t2h_kv_cache_q8_dequantize(*{**dict(  # noqa: E731
         c=c, cap=128, ln=fake, s=1, nk=2, d=128, k=fake, v=fake, st=None), **m}.values())
     for fn in (write, decode, chunk, evict, read):
@@ -203,3 +203,4 @@ def test_kv_q8_argument_validation(lib):
     assert evict(o=other, ocap=64, wo=0x3000) == 2
     assert evict(ocap=192) == 2 and evict(o=other, ocap=192) == 2
     assert evict(o=None) == 1 and evict(lo=fake) == 5
+    assert evict(ws=None) == 1 and evict(ws=0x1008) == 7 and evict(nb=8) == 6 and evict(o=other, nb=8) == 6

@@ -560,6 +560,46 @@ def test_evict(device, nk, lengths, s_cap, keep, sink, recent, kind, in_place):
             assert (w_out[i, :, at.shape[1]:] == -7).all()
 
 
+@pytest.mark.parametrize("in_cache,in_weights", [(True, False), (False, True), (True, True)])
+def test_evict_half_in_place(device, in_cache, in_weights):
+    """The cache's blocks, the weights or both in their own memory: what an eviction into other memory gives, in a captured
+    graph too; elements behind what stays are left."""
+    lengths, nk, s_cap, keep = [700, 130, 0, -1, 256, 63], 3, 704, 3
+    c = filled(len(lengths), s_cap, nk, lengths, device, 33)
+    w, lens = torch.rand(len(lengths), nk, s_cap, device=device), ints(lengths, device)
+    ref, ref_w = K.kv_cache_q8(len(lengths), s_cap, nk, D, device), torch.full_like(w, -7.0)
+    ref_kept, ref_new = K.kv_cache_q8_evict(c, lens, w, keep, sink=2, recent=9, out=ref, weights_out=ref_w)
+
+    def check(dest, w_out, kept, new, old_w):
+        assert torch.equal(kept, ref_kept) and torch.equal(new, ref_new)
+        for i in range(len(lengths)):
+            end = max(0, int(new[i]))
+            for name in ("k", "v", "k_scale", "v_scale"):
+                assert torch.equal(getattr(dest, name)[i, :end // B], getattr(ref, name)[i, :end // B]), name
+            assert torch.equal(dest.k_tail[i].nan_to_num(), ref.k_tail[i].nan_to_num())
+            assert torch.equal(dest.v_tail[i].nan_to_num(), ref.v_tail[i].nan_to_num())
+            assert torch.equal(w_out[i, :, :end], ref_w[i, :, :end]) and torch.equal(w_out[i, :, end:], old_w[i, :, end:])
+
+    for graph in (False, True):
+        mine, w_mine = copy_of(c), w.clone()
+        dest = mine if in_cache else K.kv_cache_q8(len(lengths), s_cap, nk, D, device)
+        w_out = w_mine if in_weights else torch.full_like(w, -7.0)
+        old_w = w_out.clone()
+        run = lambda: K.kv_cache_q8_evict(mine, lens, w_mine, keep, sink=2, recent=9, out=dest, weights_out=w_out)  # noqa: E731
+        if not graph:
+            check(dest, w_out, *run(), old_w)
+            continue
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            kept, new = run()
+        for _ in range(3):
+            for name in PARTS:
+                getattr(mine, name).copy_(getattr(c, name))
+            w_mine.copy_(w)
+            g.replay()
+            check(dest, w_out, kept, new, old_w)
+
+
 # ------------------------------------------------------------------------------------------------- read back
 
 

@@ -133,7 +133,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "t2h_flash_attn_prefill_q8_workspace_bytes": (_sz, [_u32] * 5 + [_i32]),
     "t2h_flash_attn_prefill_q8": (_i32, [_vp, _vp, _u32, _vp, _vp, _vp, _vp, _vp] + [_u32] * 5 + [_f32, _vp, _sz, _vp]),
     "t2h_kv_cache_q8_dequantize": (_i32, [_vp, _u32, _vp, _u32, _u32, _u32, _vp, _vp, _vp]),
-    "t2h_kv_cache_q8_evict": (_i32, [_vp, _u32, _vp, _vp] + [_u32] * 6 + [_vp, _u32, _vp, _vp, _vp, _vp]),
+    "t2h_kv_cache_q8_evict_workspace_bytes": (_sz, [_u32] * 4),
+    "t2h_kv_cache_q8_evict": (_i32, [_vp, _u32, _vp, _vp] + [_u32] * 6 + [_vp, _u32, _vp, _vp, _vp, _vp, _sz, _vp]),
 }
 
 

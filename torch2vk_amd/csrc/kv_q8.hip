@@ -294,14 +294,17 @@ __global__ __launch_bounds__(256) void q8_read_kernel(const Q8ReadArgs a) {
 // close (32 of 16000: 365 us for 379) and 4 % slower at 8 sequences; through registers it was slower throughout.
 
 struct Q8EvictArgs {
-    KvQ8 c, o;
+    KvQ8 c, o;  // from, to
     const int32_t* lengths;
     const float* w_in;
     float* w_out;
     int32_t* kept;  // [n_seq][nk][64 keep]
     int32_t* lengths_out;
     uint32_t keep, sink, recent;
-    uint32_t jobs;  // thread blocks that share a head's output blocks (1 where output and input are the same cache)
+    uint32_t most;   // output blocks that a head can have
+    int same;        // output and input are one cache: o is the workspace
+    float* w_back;   // where weights_out and weights are one: they, w_out being the workspace
+    size_t w_row;    // of a head in w_out
 };
 
 __device__ __forceinline__ int q8_length(const int32_t* lengths, uint32_t seq, uint32_t nb) {
@@ -427,32 +430,40 @@ __global__ __launch_bounds__(EV_THREADS) void q8_evict_select_kernel(const Q8Evi
     }
 }
 
-// Keys (blockIdx.y 0, with the weights) or values (1) of one head: output blocks job, job + jobs, ...  Where the output
-// is the input's own cache one thread block walks a head's blocks in order: token i of the output comes from a token
-// j >= i, so block b is read before it is overwritten, and no later block needs what it overwrites.
+// Keys (blockIdx.y 0, with the weights) or values (1): one output block of one head.  Where the output is the input's own
+// memory, what is written here lies in the workspace and the kernel below brings it back, so that all blocks are made at once:
+// a thread block that walks a head's blocks in order needs no second memory, but takes 115 us for 32 blocks of 8 heads, 20 here.
 __global__ __launch_bounds__(256, 7) void q8_evict_move_kernel(const Q8EvictArgs a) {
     __shared__ int from[Q8_BLOCK];
     __shared__ float fs[Q8_BLOCK];
     __shared__ uint32_t red[4];
     const uint32_t h = blockIdx.x % a.c.nk;
     const uint32_t rest = blockIdx.x / a.c.nk;
-    const uint32_t job = rest % a.jobs, seq = rest / a.jobs;
+    const int b = (int)(rest % a.most);
+    const uint32_t seq = rest / a.most;
     const bool values = blockIdx.y != 0;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int len = q8_length(a.lengths, seq, a.c.nb);
     const int blocks = len / Q8_BLOCK;
     const int stay = blocks < (int)a.keep ? blocks : (int)a.keep;
-    const bool in_place = a.c.k == a.o.k;
     const size_t head = (size_t)seq * a.c.nk + h;
-    const int32_t* kept = a.kept + head * a.keep * Q8_BLOCK;
     const float* w_in = a.w_in + head * a.c.nb * Q8_BLOCK;
-    float* w_out = a.w_out + head * a.o.nb * Q8_BLOCK;
+    float* w_out = a.w_out + head * a.w_row;
     const bool all = stay == blocks;  // nothing leaves: blocks are copied as they are
-    if (in_place && all && a.w_in == a.w_out) return;
-    for (int b = (int)job; b < stay; b += (int)a.jobs) {
-        __syncthreads();
+    const bool move = !(all && a.same);
+    if (!values) {
+        if (b < stay && tid < Q8_BLOCK) w_out[b * Q8_BLOCK + tid] = w_in[a.kept[(head * a.keep + b) * Q8_BLOCK + tid]];
+        const int r = len - blocks * Q8_BLOCK;
+        if (b == 0 && tid < r) w_out[stay * Q8_BLOCK + tid] = w_in[blocks * Q8_BLOCK + tid];
+    }
+    if (b == 0 && !a.same) {  // the tail's rows
+        const uint4* src = reinterpret_cast<const uint4*>((values ? a.c.vt : a.c.kt) + a.c.tail_at(seq, h));
+        uint4* dst = reinterpret_cast<uint4*>((values ? a.o.vt : a.o.kt) + a.o.tail_at(seq, h));
+        for (int i = tid; i < Q8_BYTES * 2 / 16; i += 256) dst[i] = src[i];
+    }
+    if (b < stay && move) {
         if (tid < Q8_BLOCK) {
-            const int t = kept[b * Q8_BLOCK + tid];
+            const int t = a.kept[(head * a.keep + b) * Q8_BLOCK + tid];
             from[tid] = t;
             fs[tid] = (values ? a.c.vs : a.c.ks)[a.c.scale_at(seq, (uint32_t)t / Q8_BLOCK, h)];
         }
@@ -472,7 +483,6 @@ __global__ __launch_bounds__(256, 7) void q8_evict_move_kernel(const Q8EvictArgs
             for (int i = 0; i < 32; ++i) top = max(top, abs_bits(q8_value(u[i / 4], i % 4) * f));
 #pragma unroll
             for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(u[i]));
-            const float wt = tid < Q8_BLOCK ? w_in[from[tid]] : 0.0f;
             top = wave_max_u32(top);
             if (lane == 0) red[wave] = top;
             __syncthreads();
@@ -484,7 +494,6 @@ __global__ __launch_bounds__(256, 7) void q8_evict_move_kernel(const Q8EvictArgs
             uint4* dst = reinterpret_cast<uint4*>(a.o.k + to + r * Q8_D + part * 32);
             dst[0] = x[0];
             dst[1] = x[1];
-            if (tid < Q8_BLOCK) w_out[b * Q8_BLOCK + tid] = wt;
         } else {
             // a lane is a token, a wave 32 dims: 64 tokens of a dim are a few short runs of bytes
             const int t = from[lane];
@@ -520,18 +529,37 @@ __global__ __launch_bounds__(256, 7) void q8_evict_move_kernel(const Q8EvictArgs
         }
         if (tid == 0) (values ? a.o.vs : a.o.ks)[a.o.scale_at(seq, (uint32_t)b, h)] = s;
     }
-    if (job != 0) return;
-    // the tail's tokens: their rows where the output is another cache, and their weights
-    if (!in_place) {
-        const uint4* src = reinterpret_cast<const uint4*>((values ? a.c.vt : a.c.kt) + a.c.tail_at(seq, h));
-        uint4* dst = reinterpret_cast<uint4*>((values ? a.o.vt : a.o.kt) + a.o.tail_at(seq, h));
-        for (int i = tid; i < Q8_BYTES * 2 / 16; i += 256) dst[i] = src[i];
+}
+
+// An output block of one head, and its weights, from the workspace to where they belong.
+__global__ __launch_bounds__(256) void q8_evict_back_kernel(const Q8EvictArgs a) {
+    const uint32_t h = blockIdx.x % a.c.nk;
+    const uint32_t rest = blockIdx.x / a.c.nk;
+    const int b = (int)(rest % a.most);
+    const uint32_t seq = rest / a.most;
+    const int tid = threadIdx.x;
+    const int len = q8_length(a.lengths, seq, a.c.nb);
+    const int blocks = len / Q8_BLOCK;
+    if (blocks <= (int)a.keep) return;  // nothing has left
+    const int stay = (int)a.keep;
+    const size_t head = (size_t)seq * a.c.nk + h;
+    if (a.same) {
+        const size_t at = a.o.block_at(seq, (uint32_t)b, h), to = a.c.block_at(seq, (uint32_t)b, h);
+        uint4 x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = load_u4((i < 2 ? a.o.k : a.o.v) + at + ((i & 1) * 256 + tid) * 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>((i < 2 ? a.c.k : a.c.v) + to + ((i & 1) * 256 + tid) * 16) = x[i];
+        if (tid == 0) {
+            a.c.ks[a.c.scale_at(seq, (uint32_t)b, h)] = a.o.ks[a.o.scale_at(seq, (uint32_t)b, h)];
+            a.c.vs[a.c.scale_at(seq, (uint32_t)b, h)] = a.o.vs[a.o.scale_at(seq, (uint32_t)b, h)];
+        }
     }
-    if (!values) {
-        const int r = len - blocks * Q8_BLOCK;
-        const float wt = tid < r ? w_in[blocks * Q8_BLOCK + tid] : 0.0f;
-        __syncthreads();
-        if (tid < r) w_out[stay * Q8_BLOCK + tid] = wt;
+    if (a.w_back) {
+        const float* w = a.w_out + head * a.w_row;
+        float* to = a.w_back + head * a.c.nb * Q8_BLOCK;
+        if (tid < Q8_BLOCK) to[b * Q8_BLOCK + tid] = w[b * Q8_BLOCK + tid];
+        if (b == 0 && tid < len - blocks * Q8_BLOCK) to[stay * Q8_BLOCK + tid] = w[stay * Q8_BLOCK + tid];
     }
 }
 
@@ -597,10 +625,28 @@ extern "C" int t2h_kv_cache_q8_dequantize(void* const* cache, uint32_t s_cap, co
     return T2H_OK;
 }
 
+// Bytes of the parts of an eviction's workspace: codes, scales, weights.
+struct Q8EvictRoom {
+    size_t codes, scales, weights;
+    Q8EvictRoom(uint32_t keep, uint32_t n_seq, uint32_t nk, uint32_t s_cap) {
+        const size_t most = keep < s_cap / Q8_BLOCK ? keep : s_cap / Q8_BLOCK, heads = (size_t)n_seq * nk;
+        codes = heads * most * Q8_BYTES;
+        scales = (heads * most * 4 + 15) / 16 * 16;
+        weights = heads * (most + 1) * Q8_BLOCK * 4;
+    }
+};
+
+extern "C" size_t t2h_kv_cache_q8_evict_workspace_bytes(uint32_t keep_blocks, uint32_t n_seq, uint32_t nk, uint32_t s_cap) {
+    if (keep_blocks == 0 || n_seq == 0 || nk == 0 || s_cap == 0 || s_cap % Q8_BLOCK != 0) return 0;
+    const Q8EvictRoom room(keep_blocks, n_seq, nk, s_cap);
+    return 2 * room.codes + 2 * room.scales + room.weights;
+}
+
 extern "C" int t2h_kv_cache_q8_evict(void* const* cache, uint32_t s_cap, const int32_t* lengths, const float* weights,
                                      uint32_t keep_blocks, uint32_t sink, uint32_t recent, uint32_t n_seq, uint32_t nk,
                                      uint32_t d, void* const* cache_out, uint32_t s_cap_out, float* weights_out,
-                                     int32_t* kept, int32_t* lengths_out, void* stream) {
+                                     int32_t* kept, int32_t* lengths_out, void* workspace, size_t workspace_bytes,
+                                     void* stream) {
     Q8EvictArgs a;
     if (!lengths || !weights || !weights_out || !kept || !lengths_out) return T2H_ERR_NULL;
     if (const int e = q8_cache(cache, s_cap, n_seq, nk, nk, d, a.c)) return e;
@@ -613,7 +659,11 @@ extern "C" int t2h_kv_cache_q8_evict(void* const* cache, uint32_t s_cap, const i
     if (same != (a.c.v == a.o.v) || same != (a.c.ks == a.o.ks) || same != (a.c.vs == a.o.vs) ||
         same != (a.c.kt == a.o.kt) || same != (a.c.vt == a.o.vt))
         return T2H_ERR_ARG;
-    if ((same || weights == weights_out) && s_cap != s_cap_out) return T2H_ERR_SHAPE;
+    const bool in_place = same || weights == weights_out;
+    if (in_place && s_cap != s_cap_out) return T2H_ERR_SHAPE;
+    if (in_place && !workspace) return T2H_ERR_NULL;
+    if (in_place && (reinterpret_cast<uintptr_t>(workspace) & 15)) return T2H_ERR_ALIGN;
+    if (in_place && workspace_bytes < t2h_kv_cache_q8_evict_workspace_bytes(keep_blocks, n_seq, nk, s_cap)) return T2H_ERR_WORKSPACE;
     a.lengths = lengths;
     a.w_in = weights;
     a.w_out = weights_out;
@@ -622,9 +672,25 @@ extern "C" int t2h_kv_cache_q8_evict(void* const* cache, uint32_t s_cap, const i
     a.keep = keep_blocks;
     a.sink = sink;
     a.recent = recent;
-    const uint32_t most = keep_blocks < a.c.nb ? keep_blocks : a.c.nb;
-    a.jobs = same || weights == weights_out ? 1 : most;
-    const uint64_t grid = (uint64_t)n_seq * a.jobs * nk;
+    a.most = keep_blocks < a.c.nb ? keep_blocks : a.c.nb;
+    a.same = same;
+    a.w_back = nullptr;
+    a.w_row = (size_t)s_cap_out;
+    const Q8EvictRoom room(keep_blocks, n_seq, nk, s_cap);
+    int8_t* const at = reinterpret_cast<int8_t*>(workspace);
+    if (same) {
+        a.o.k = at;
+        a.o.v = at + room.codes;
+        a.o.ks = reinterpret_cast<float*>(at + 2 * room.codes);
+        a.o.vs = reinterpret_cast<float*>(at + 2 * room.codes + room.scales);
+        a.o.nb = a.most;
+    }
+    if (weights == weights_out) {
+        a.w_back = weights_out;
+        a.w_out = reinterpret_cast<float*>(at + 2 * room.codes + 2 * room.scales);
+        a.w_row = ((size_t)a.most + 1) * Q8_BLOCK;
+    }
+    const uint64_t grid = (uint64_t)n_seq * a.most * nk;
     if (grid > 0x7fffffffu) return T2H_ERR_SHAPE;
     if (s_cap <= EV_SMALL)
         hipLaunchKernelGGL(q8_evict_select_kernel<16>, dim3(n_seq * nk), dim3(EV_THREADS), 0, reinterpret_cast<hipStream_t>(stream), a);
@@ -633,5 +699,9 @@ extern "C" int t2h_kv_cache_q8_evict(void* const* cache, uint32_t s_cap, const i
     T2H_LAUNCH_CHECK();
     hipLaunchKernelGGL(q8_evict_move_kernel, dim3((uint32_t)grid, 2), dim3(256), 0, reinterpret_cast<hipStream_t>(stream), a);
     T2H_LAUNCH_CHECK();
+    if (in_place) {
+        hipLaunchKernelGGL(q8_evict_back_kernel, dim3((uint32_t)grid), dim3(256), 0, reinterpret_cast<hipStream_t>(stream), a);
+        T2H_LAUNCH_CHECK();
+    }
     return T2H_OK;
 }

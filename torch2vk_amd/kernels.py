@@ -1943,6 +1943,12 @@ def kv_cache_q8_evict(cache: KVCacheQ8, lengths: torch.Tensor, weights: torch.Te
         raise ValueError(f"out holds {dest.s_cap} tokens, {KV_Q8_BLOCK * (keep_blocks + 1)} may stay")
     kept = torch.empty(n_seq, nk, KV_Q8_BLOCK * keep_blocks, dtype=torch.int32, device=lengths.device)
     new = torch.empty_like(lengths)
+    room, nbytes = None, 0
+    if dest.k.data_ptr() == cache.k.data_ptr() or weights_out.data_ptr() == weights.data_ptr():
+        nbytes = _lib.lib().t2h_kv_cache_q8_evict_workspace_bytes(keep_blocks, n_seq, nk, cache.s_cap)
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=lengths.device)
+        room = workspace.data_ptr()
     call("t2h_kv_cache_q8_evict", cache.ptrs, cache.s_cap, lengths.data_ptr(), weights.data_ptr(), keep_blocks, sink, recent,
-         n_seq, nk, 128, dest.ptrs, dest.s_cap, weights_out.data_ptr(), kept.data_ptr(), new.data_ptr(), stream_handle())
+         n_seq, nk, 128, dest.ptrs, dest.s_cap, weights_out.data_ptr(), kept.data_ptr(), new.data_ptr(), room, nbytes,
+         stream_handle())
     return kept, new
