@@ -89,7 +89,8 @@ struct DecodeUnit {
 // refilled.  Measured (us, 32 / 8 heads but for the third): 1 of 16000 15.1 in units of 8, 18.3 of 4; 16 of 100 to 8000 39 of
 // 20, 44 of 12, 46 of 32; 128 of 300 to 1200, 4 KV heads, 32 at one a CU, 38 at two; 64 of 100 to 16000 209 of up to 32, 219 of 64.
 __device__ __forceinline__ uint32_t dq_chunk(uint64_t total, uint32_t n_seq, uint32_t nk) {
-    const uint64_t one = (total * nk + 255) / 256, two = (total * nk * (n_seq * nk >= DQ_SLOTS / 2 ? 2 : 1) + DQ_SLOTS - 1) / DQ_SLOTS;
+    const uint64_t blocks = total * nk, one = (blocks + 255) / 256;
+    const uint64_t two = (blocks * (n_seq * nk >= DQ_SLOTS / 2 ? 2 : 1) + DQ_SLOTS - 1) / DQ_SLOTS;
     const uint64_t c = one <= 8 ? one : (two > 8 ? two : 8);
     return c <= DQ_WAVES ? DQ_WAVES : c >= DQ_CHUNK_MAX ? DQ_CHUNK_MAX : (uint32_t)((c + DQ_WAVES - 1) / DQ_WAVES * DQ_WAVES);
 }
@@ -190,7 +191,8 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_decode_q8_kernel(const 
     const uint32_t h = blockIdx.x % a.c.nk;
     const uint32_t unit = blockIdx.x / a.c.nk;
     DecodeUnit u;
-    if (!dq_find({a.lengths, nullptr, 1, a.n_seq, a.c.nb, a.c.nk}, unit, false, u)) return;  // (every wave of a thread block finds the same)
+    // (every wave of a thread block finds the same)
+    if (!dq_find({a.lengths, nullptr, 1, a.n_seq, a.c.nb, a.c.nk}, unit, false, u)) return;
     const int group = (int)a.group;
     uint32_t* const out = reinterpret_cast<uint32_t*>(a.out + ((size_t)u.seq * a.nh + h * group) * Q8_D);
     if (u.blocks == 0) {
@@ -796,7 +798,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_chunk_q8_kernel(const Chun
     if (b0 < whole) load(b0);
     // the row's query
     uint4 q[8];
-    const uint16_t* qp = a.q + (((size_t)seq * a.n + (row < rows ? t : 0)) * a.nh + h * group + (row < rows ? g : 0)) * Q8_D + 8 * half;
+    const size_t q_at = ((size_t)seq * a.n + (row < rows ? t : 0)) * a.nh + h * group + (row < rows ? g : 0);
+    const uint16_t* qp = a.q + q_at * Q8_D + 8 * half;
 #pragma unroll
     for (int i = 0; i < 8; ++i) q[i] = load_u4(qp + 16 * i);
     float m = -INFINITY, l = 0.0f;

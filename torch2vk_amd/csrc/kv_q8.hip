@@ -490,7 +490,8 @@ __global__ __launch_bounds__(256, 7) void q8_evict_move_kernel(const Q8EvictArgs
             if (all) s = f;
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                if (!all) u[i] = q8_pack4(q8_value(u[i], 0) * f, q8_value(u[i], 1) * f, q8_value(u[i], 2) * f, q8_value(u[i], 3) * f, inv);
+                if (!all)
+                    u[i] = q8_pack4(q8_value(u[i], 0) * f, q8_value(u[i], 1) * f, q8_value(u[i], 2) * f, q8_value(u[i], 3) * f, inv);
             uint4* dst = reinterpret_cast<uint4*>(a.o.k + to + r * Q8_D + part * 32);
             dst[0] = x[0];
             dst[1] = x[1];
@@ -506,7 +507,8 @@ __global__ __launch_bounds__(256, 7) void q8_evict_move_kernel(const Q8EvictArgs
                 for (int i = 0; i < 32; ++i) x[i] = (uint8_t)src[i * Q8_BLOCK];
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    u[i] = (uint32_t)x[4 * i] | (uint32_t)x[4 * i + 1] << 8 | (uint32_t)x[4 * i + 2] << 16 | (uint32_t)x[4 * i + 3] << 24;
+                    u[i] = (uint32_t)x[4 * i] | (uint32_t)x[4 * i + 1] << 8 | (uint32_t)x[4 * i + 2] << 16 |
+                           (uint32_t)x[4 * i + 3] << 24;
             }
 #pragma unroll
             for (int i = 0; i < 32; ++i) top = max(top, abs_bits(q8_value(u[i / 4], i % 4) * f));
@@ -663,7 +665,8 @@ extern "C" int t2h_kv_cache_q8_evict(void* const* cache, uint32_t s_cap, const i
     if (in_place && s_cap != s_cap_out) return T2H_ERR_SHAPE;
     if (in_place && !workspace) return T2H_ERR_NULL;
     if (in_place && (reinterpret_cast<uintptr_t>(workspace) & 15)) return T2H_ERR_ALIGN;
-    if (in_place && workspace_bytes < t2h_kv_cache_q8_evict_workspace_bytes(keep_blocks, n_seq, nk, s_cap)) return T2H_ERR_WORKSPACE;
+    if (in_place && workspace_bytes < t2h_kv_cache_q8_evict_workspace_bytes(keep_blocks, n_seq, nk, s_cap))
+        return T2H_ERR_WORKSPACE;
     a.lengths = lengths;
     a.w_in = weights;
     a.w_out = weights_out;
