@@ -667,61 +667,56 @@ def test_prompt_decode_evict_decode(device):
 
 def test_the_far_end_of_a_large_cache(device):
     """The last of 40 sequences in a cache of 5 GB of codes each for keys and values, past 32 bits: every operator gives it
-    what a cache of its own does."""
+    what it gives it in a cache of less capacity."""
     nh, nk, n_seq, s_cap, length = 16, 8, 40, 131072, 6000
-    one, big = filled(1, 8192, nk, [length], device, 31), K.kv_cache_q8(n_seq, s_cap, nk, D, device)
+    lens = ints([-1] * (n_seq - 1) + [length], device)
+    low, big = filled(n_seq, 8192, nk, lens.tolist(), device, 31), K.kv_cache_q8(n_seq, s_cap, nk, D, device)
     for name in PARTS:
-        part = getattr(one, name)[0]
+        part = getattr(low, name)[-1]
         getattr(big, name)[-1, :part.shape[0]] = part
-    lens1, lens = ints([length], device), ints([-1] * (n_seq - 1) + [length], device)
-    w1, w = torch.rand(1, nk, 8192, device=device), torch.zeros(n_seq, nk, s_cap, device=device)
-    w[-1, :, :8192] = w1
+    w_low, w = torch.rand(n_seq, nk, 8192, device=device), torch.zeros(n_seq, nk, s_cap, device=device)
+    w[..., :8192] = w_low
 
     def same(what):
         for name in PARTS:
-            part = getattr(one, name)[0]
+            part = getattr(low, name)[-1]
             assert torch.equal(getattr(big, name)[-1, :part.shape[0]].nan_to_num(), part.nan_to_num()), f"{what}: {name}"
-        assert torch.equal(w[-1, :, :8192], w1[0]), f"{what}: weights"
+        assert torch.equal(w[..., :8192], w_low), f"{what}: weights"
 
     n = 300
-    (q, k, v), wq, wk = inputs(n, nh, nk, device, 32)
+    rows, wq, wk = inputs(n_seq * n, nh, nk, device, 32)
     norms = dict(theta=1e6, q_norm_weight=wq, k_norm_weight=wk)
-    pad = torch.nn.functional.pad
-    qs, ks, vs = (pad(t, (0, 0, (n_seq - 1) * n, 0)) for t in (q, k, v))
-    out1, out = torch.empty(1, n, nh, D, dtype=BF, device=device), torch.empty(n_seq, n, nh, D, dtype=BF, device=device)
-    K.qk_norm_rope_cache_q8(q, k, v, out1, one, lens1, **norms)
-    K.qk_norm_rope_cache_q8(qs, ks, vs, out, big, lens, **norms)
-    assert torch.equal(out[-1], out1[0]) and not out[:-1].any()
+    outs = [torch.empty(n_seq, n, nh, D, dtype=BF, device=device) for _ in range(2)]
+    for c, out in zip((low, big), outs):
+        K.qk_norm_rope_cache_q8(*rows, out, c, lens, **norms)
+    assert torch.equal(*outs) and not outs[1][:-1].any()
     same("chunk write")
-    got = K.flash_attn_prefill_q8(out, big, lens, weights=w)
-    K.flash_attn_prefill_q8(out1, one, lens1, weights=w1)
-    kc, vc = rows_of(one, 0, length + n)
-    ref, mass_v, _, mass_qk = attention(out1[0].to(F64), kc, vc, length + torch.arange(n, device=device))
+    got = K.flash_attn_prefill_q8(outs[1], big, lens, weights=w)
+    K.flash_attn_prefill_q8(outs[0], low, lens, weights=w_low)
+    kc, vc = rows_of(low, n_seq - 1, length + n)
+    ref, mass_v, _, mass_qk = attention(outs[0][-1].to(F64), kc, vc, length + torch.arange(n, device=device))
     check_out(got[-1], ref, mass_v, mass_qk, "chunk")
     assert not got[:-1].any()
-    assert within(w[-1, :, :length + n], w1[0, :, :length + n], 1e-4 * (1 + w1[0, :, :length + n]))  # other splits, other sums
-    w[-1, :, :8192] = w1
-    lens1 += n
+    end = length + n
+    assert within(w[-1, :, :end], w_low[-1, :, :end], 1e-4 * (1 + w_low[-1, :, :end]))  # other splits, other sums
+    w[..., :8192] = w_low
     lens[-1] += n
-    few = out1[:, :2].contiguous()
-    got = K.flash_attn_prefill_q8(pad(few, (0, 0, 0, 0, 0, 0, n_seq - 1, 0)), big, lens - 2)
-    assert torch.equal(got[-1:], K.flash_attn_prefill_q8(few, one, lens1 - 2)), "a few tokens"
-    step1, step = torch.empty(1, nh, D, dtype=BF, device=device), torch.empty(n_seq, nh, D, dtype=BF, device=device)
+    few = [K.flash_attn_prefill_q8(outs[0][:, :2].contiguous(), c, lens - 2) for c in (low, big)]
+    assert torch.equal(*few), "a few tokens"
+    steps = [torch.empty(n_seq, nh, D, dtype=BF, device=device) for _ in range(2)]
+    spaces = [K.attn_decode_q8_workspace(n_seq, nh, nk, D, c.s_cap, device, weights=True) for c in (low, big)]
     for j in range(70):  # over a block's end
-        K.attn_decode_q8(q[j:j + 1], k[j:j + 1], v[j:j + 1], one, step1, lens1,
-                         K.attn_decode_q8_workspace(1, nh, nk, D, 8192, device, weights=True), weights=w1, **norms)
-        if j == 0:
-            ws = K.attn_decode_q8_workspace(n_seq, nh, nk, D, s_cap, device, weights=True)
-        K.attn_decode_q8(*(pad(t[j:j + 1], (0, 0, n_seq - 1, 0)) for t in (q, k, v)), big, step, lens, ws, weights=w, **norms)
-        assert torch.equal(step[-1:], step1), f"step {j}"
-        lens1 += 1
+        q, k, v = (t[j * n_seq:(j + 1) * n_seq] for t in rows)
+        for c, step, ws, weights in zip((low, big), steps, spaces, (w_low, w)):
+            K.attn_decode_q8(q, k, v, c, step, lens, ws, weights=weights, **norms)
+        assert torch.equal(*steps), f"step {j}"
         lens[-1] += 1
     same("steps")
-    (kept1, new1), (kept, new) = K.kv_cache_q8_evict(one, lens1, w1, 30), K.kv_cache_q8_evict(big, lens, w, 30)
-    assert torch.equal(kept[-1], kept1[0]) and torch.equal(new[-1:], new1) and bool((new[:-1] == -1).all())
+    (kept_low, new_low), (kept, new) = (K.kv_cache_q8_evict(c, lens, x, 30) for c, x in ((low, w_low), (big, w)))
+    assert torch.equal(kept, kept_low) and torch.equal(new, new_low) and bool((new[:-1] == -1).all())
     same("eviction")
-    for a, b in zip(K.kv_cache_q8_dequantize(big, new), K.kv_cache_q8_dequantize(one, new1)):
-        assert torch.equal(a[-1, :8192], b[0]) and not a[-1, 8192:].any() and not a[0].any()
+    for a, b in zip(K.kv_cache_q8_dequantize(big, new), K.kv_cache_q8_dequantize(low, new)):
+        assert torch.equal(a[-1, :8192], b[-1]) and not a[-1, 8192:].any() and not a[0].any()
 
 
 # -------------------------------------------------------------------------------------------------- refusals

@@ -83,15 +83,21 @@ struct DecodeUnit {
     int chunk, blocks, len;      // blocks a unit, the sequence's blocks and its length before the call
 };
 
-// Blocks a unit, for the blocks of all sequences: 4 (one a wave) for short ones, then one thread block a CU until units have
-// 8, then two a CU, which the registers allow, or one where the sequences' heads alone are that many, until units have 32,
-// where what a unit costs besides its blocks (3 to 4 us: lengths, q, joining) no longer matters and ragged lengths want the chip
-// refilled.  Measured (us, 32 / 8 heads but for the third): 1 of 16000 15.1 in units of 8, 18.3 of 4; 16 of 100 to 8000 39 of
-// 20, 44 of 12, 46 of 32; 128 of 300 to 1200, 4 KV heads, 32 at one a CU, 38 at two; 64 of 100 to 16000 209 of up to 32, 219 of 64.
+// Blocks a unit, for the blocks of all sequences: 4 (one a wave) where that makes a sequence one unit, which needs no join, or
+// its units many; 1 or 2 between, as a CU takes a block in no less than 0.5 us and the chip is far from full.  Then one thread
+// block a CU until units have 8, then two a CU, which the registers allow, or one where the sequences' heads alone are that many,
+// until units have 32, where what a unit costs besides its blocks (3 to 4 us: lengths, q, joining) no longer matters and ragged
+// lengths want the chip refilled.  Measured (us, 32 / 8 heads but for the sixth): 200 tokens 8.4 in units of 4, 9.0 of 1; 500 11.4
+// and 9.1; 2000 11.5 of 4, 10.4 of 2, 11.8 of 1; 16000 15.1 of 8, 18.3 of 4; 16 sequences of 100 to 8000 39 of 20, 44 of 12, 46 of
+// 32; 128 of 300 to 1200, 4 KV heads, 32 at one a CU, 38 at two; 64 of 100 to 16000 209 of up to 32, 219 of 64.
 __device__ __forceinline__ uint32_t dq_chunk(uint64_t total, uint32_t n_seq, uint32_t nk) {
     const uint64_t blocks = total * nk, one = (blocks + 255) / 256;
     const uint64_t two = (blocks * (n_seq * nk >= DQ_SLOTS / 2 ? 2 : 1) + DQ_SLOTS - 1) / DQ_SLOTS;
     const uint64_t c = one <= 8 ? one : (two > 8 ? two : 8);
+    if (c <= 2 && total > (uint64_t)n_seq * DQ_WAVES) {
+        if (c < 2 && total <= (uint64_t)n_seq * 16) return 1;
+        if (total <= (uint64_t)n_seq * 32) return 2;
+    }
     return c <= DQ_WAVES ? DQ_WAVES : c >= DQ_CHUNK_MAX ? DQ_CHUNK_MAX : (uint32_t)((c + DQ_WAVES - 1) / DQ_WAVES * DQ_WAVES);
 }
 
