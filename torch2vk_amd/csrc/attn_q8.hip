@@ -637,6 +637,19 @@ __global__ __launch_bounds__(256) void attn_decode_q8_weights_kernel(const Decod
     const int len = a.lengths[seq], cap = (int)(a.c.nb * Q8_BLOCK);
     const int end = len < 0 ? 0 : (len < cap ? len + 1 : cap);
     if (first >= end) return;
+    // what does not wait for the sums is asked for before them
+    const float* const scores = a.scores + ((size_t)seq * a.nh + h * a.group) * cap + t0;
+    const size_t at = ((size_t)seq * a.c.nk + h) * cap + t0;
+    constexpr uint32_t AHEAD = 4;
+    f32x4 early[AHEAD];
+    float before[4];
+    if (t0 < end) {
+#pragma unroll
+        for (uint32_t g = 0; g < AHEAD; ++g)
+            if (g < a.group) early[g] = *reinterpret_cast<const f32x4*>(scores + (size_t)g * cap);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) before[j] = t0 + j < len ? a.w_in[at + j] : 0.0f;
+    }
     DecodeUnit u;
     dq_find({a.lengths, nullptr, 1, a.n_seq, a.c.nb, a.c.nk}, seq, true, u);
     for (uint32_t g = wave; g < a.group; g += 4) {
@@ -647,15 +660,17 @@ __global__ __launch_bounds__(256) void attn_decode_q8_weights_kernel(const Decod
     __syncthreads();
     if (t0 >= end) return;
     f32x4 sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t g = 0; g < a.group; ++g) {
-        const f32x4 s = *reinterpret_cast<const f32x4*>(a.scores + ((size_t)seq * a.nh + h * a.group + g) * cap + t0);
+    auto add = [&](f32x4 s, uint32_t g) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) sum[j] += __builtin_amdgcn_exp2f(s[j] - lse[g]);
-    }
-    const size_t at = ((size_t)seq * a.c.nk + h) * cap + t0;
+    };
+#pragma unroll
+    for (uint32_t g = 0; g < AHEAD; ++g)
+        if (g < a.group) add(early[g], g);
+    for (uint32_t g = AHEAD; g < a.group; ++g) add(*reinterpret_cast<const f32x4*>(scores + (size_t)g * cap), g);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-        if (t0 + j < end) a.w_out[at + j] = (t0 + j < len ? a.w_in[at + j] : 0.0f) + sum[j];
+        if (t0 + j < end) a.w_out[at + j] = before[j] + sum[j];
 }
 
 // Counters at the start of the workspace, as many for every shape (of up to 16384 sequences times KV heads), so that calls of
