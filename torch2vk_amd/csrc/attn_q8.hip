@@ -1580,11 +1580,16 @@ static uint32_t cq_splits(uint32_t n, uint32_t n_seq, uint32_t nh, uint32_t nk, 
 }
 
 // Thread blocks that share the rows of a chunk's weights where there are few tokens: two rounds of the chip (for a causal
-// chunk's share of the pairs), 512 rows each or more.  Measured (us, 32 / 8 heads): 2048 tokens at 0: 38 in rounds of 1024
-// thread blocks, 48 of 512, 196 unshared; 2 x 300 of 40 / 8 heads at 3000: 37 of 512 rows or more, 41 of 256, 45 unshared.
+// chunk's share of the pairs) of 512 rows each or more, or one round of 128 or more.  Measured (us, 32 / 8 heads but for the
+// last two): 2048 tokens at 0: 38 in rounds of 1024 thread blocks, 48 of 512, 196 unshared; 142 tokens at 4: 14 of 128 rows, 18
+// of 256, 24 unshared; 2 x 300 of 40 / 8 at 3000: 37 of 512 rows in two rounds, 41 of 256; 300 of 16 / 2 at 2000: 18 of 128 rows
+// in one round, 22 of 64, 26 of 512.
 static uint32_t cq_weight_splits(uint32_t n, uint32_t n_seq, uint32_t nh, uint32_t nk, uint32_t nb) {
-    const uint64_t grid = ((uint64_t)nb + 3) / 4 * n_seq * nk, want = 1024 / grid, most = (uint64_t)n * (nh / nk) / 512;
-    return (uint32_t)(want < most ? (want ? want : 1) : (most ? most : 1));
+    const uint64_t grid = ((uint64_t)nb + 3) / 4 * n_seq * nk, rows = (uint64_t)n * (nh / nk);
+    const uint64_t large = 1024 / grid < rows / 512 ? 1024 / grid : rows / 512;
+    const uint64_t small = 512 / grid < rows / 128 ? 512 / grid : rows / 128;
+    const uint64_t splits = large > small ? large : small;
+    return (uint32_t)(splits ? splits : 1);
 }
 
 // fp32 values of a chunk's weights: each row's softmax and the shares
