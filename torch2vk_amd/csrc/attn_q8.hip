@@ -1568,14 +1568,17 @@ static uint32_t cq_waves(uint32_t n, uint32_t n_seq, uint32_t nh, uint32_t nk) {
     return ((uint64_t)n * (nh / nk) + 255) / 256 * n_seq * nk >= CQ_WIDE_GRID ? 8 : 4;
 }
 
-// Thread blocks that share a tile's keys: two a CU where there are not as many tiles, each with 4 blocks of keys or more of
-// those that a row of the chunk's middle sees in a full cache.  Measured (us, 32 / 8 heads but for the last): 1901 tokens,
-// 480 tiles: 58 whole, 64 in two parts; 700, 176 tiles: 25 whole, 30 in two; 2 x 5 tokens at 4000: 20 in 16 parts, 24 in 8
-// and in 32; 2048 of 16 / 8 heads, 256 tiles: 48 in two, 58 whole.
+// Thread blocks that share a tile's keys, in a full cache each with 4 blocks of keys or more of those that a row of the chunk's
+// middle sees: one a CU where there are not as many tiles; two a CU where that leaves each 8 blocks or more, 32 where it is what
+// brings the join with it.  Measured (us, 32 / 8 heads unless named; one a CU, two): 100 tokens at 3000 24, 28; 64 at 8000 26, 30;
+// 256 at 16000 89, 87; 512 at 8000 94, 87; and where one a CU is whole: 1000 at 0 26, 33; 2 x 512 at 2000 53, 59, at 4000 89, 90;
+// 4 x 512 of 16 / 8 heads at 7000 150, 142; 2048 of 16 / 8 at 2048 79, 72.  1901 tokens, 480 tiles: 58 whole, 64 in two parts.
 static uint32_t cq_splits(uint32_t n, uint32_t n_seq, uint32_t nh, uint32_t nk, uint32_t nb) {
     const uint64_t rows = 32 * cq_waves(n, n_seq, nh, nk), tiles = ((uint64_t)n * (nh / nk) + rows - 1) / rows;
-    const uint64_t grid = tiles * n_seq * nk;
-    const uint64_t want = grid ? 512 / grid : 1, skip = n / (2 * Q8_BLOCK), most = nb > skip ? (nb - skip) / 4 : 0;
+    const uint64_t grid = tiles * n_seq * nk, skip = n / (2 * Q8_BLOCK), most = nb > skip ? (nb - skip) / 4 : 0;
+    if (grid == 0) return 1;
+    const uint64_t one = 256 / grid, two = 512 / grid;
+    const uint64_t want = two && nb / two >= (one > 1 ? 8 : 32) ? two : one;
     return (uint32_t)(want < most ? (want ? want : 1) : (most ? most : 1));
 }
 
