@@ -587,7 +587,8 @@ int t2h_slice_last_token(const float* x, void* out, int out_dtype, uint32_t b, u
  * A whole block's values are code * scale, scale = max|x| / 127 over its bf16 values x, code = x / scale rounded once, ties
  * to even.  The tokens of a sequence's last, unfinished block are bf16 rows in the tail and are rounded when the block's
  * last token arrives, so that the cache depends on the tokens and not on the chunks they came in.  A block of values under
- * 1.3e-28 is held as zeros; one with a NaN or an infinity reads as NaN.
+ * 1.3e-28 is held as zeros; one with a NaN or an infinity reads as NaN.  Such a value in the tail makes what sees its token
+ * not finite: the scores if it is a key's, the output in its dimension if it is a value's.
  * lengths (device int32 [n_seq]): the tokens that each sequence holds before the call; calls do not advance them, so that
  * the layers of a step share them.  A negative length: the sequence takes no part, its outputs are zeros.  Tokens past s_cap
  * are dropped: they are not written, and their queries see the s_cap cached ones.  A sequence goes on from its length

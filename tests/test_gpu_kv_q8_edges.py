@@ -1,0 +1,62 @@
+"""The 8-bit KV cache where values are not finite, lie far apart or belong to no row: against the definition in 64 bits over
+what the cache holds (the plain forms and tolerances of test_gpu_kv_q8.py)."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from tests.test_gpu_kv_q8 import (B, BF, D, F64, HALF_BF16, attention, check_out, check_weights, copy_of, filled, inputs, ints,
+                                  rows_of)
+from torch2vk_amd import kernels as K
+
+pytestmark = pytest.mark.gpu
+
+
+def chunk_rows(shape, device, seed):
+    gen = torch.Generator(device=device)
+    gen.manual_seed(seed)
+    return torch.randn(shape, generator=gen, device=device).to(BF)
+
+
+def check_rows(got, q, k, v, last, what):
+    """Rows got [t, nh, D] of queries q fp64 that see keys 0 .. last[t]: test_gpu_kv_q8.check_out's tolerance with the largest
+    |v| that the row itself sees in the place of the sequence's (2^-37 of it for each key, times the 2^10 of check_out)."""
+    ref, _, p, mass_qk = attention(q, k, v, last)
+    size = v.abs().repeat_interleave(q.shape[1] // k.shape[0], 0)
+    top = size.amax(-1).cummax(-1).values[:, last].T[..., None]
+    mass_v = torch.einsum("hts,hsd->thd", p, size) + 2.0 ** -27 * k.shape[1] * top
+    tol = HALF_BF16 * 1.01 * ref.abs() + (2.0 ** -10 + 2.0 ** -17 * mass_qk) * mass_v + 1e-38
+    bad = ~((got.to(F64) - ref).abs() <= tol)
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, first {bad.nonzero()[0].tolist()}"
+
+
+# ------------------------------------------------------------------- the unfinished block's values, not finite
+
+
+@pytest.mark.parametrize("nh,nk,n,end,s_cap", [
+    (4, 2, 5, 100, 128), (8, 2, 8, 1030, 1088), (4, 2, 5, 4098, 4160),  # few rows: a tile, two, several units
+    (4, 2, 200, 230, 256), (6, 2, 100, 300, 8192), (3, 1, 130, 130, 192)])  # tiles, and their keys split
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_a_broken_value_of_the_tail_reaches_the_rows_that_see_it(device, nh, nk, n, end, s_cap, value):
+    """A NaN or an infinity in the unfinished block's values: its dimension of the rows that see its token is not finite, and
+    every other output is what it is without it, rows of earlier blocks and earlier tokens among them."""
+    print("tail", nh, nk, n, end, s_cap, value, flush=True)
+    length = end - n
+    c = filled(1, s_cap, nk, [end], device, 50)
+    bad = {(end - 1, 0, 5), (end - 1, nk - 1, 70), (max(length, end // B * B), 0, 127)}
+    for token, head, dim in bad:
+        c.v_tail[0, head, dim, token % B] = value
+    q = chunk_rows((1, n, nh, D), device, 51)
+    out = K.flash_attn_prefill_q8(q, c, ints([length], device))[0]
+    k, v = rows_of(c, 0, end)
+    last = length + torch.arange(n, device=device)
+    broken = torch.zeros(n, nh, D, dtype=torch.bool, device=device)
+    for token, head, dim in bad:
+        broken[token - length:, head * (nh // nk):(head + 1) * (nh // nk), dim] = True
+    assert not torch.isfinite(out[broken]).any()
+    assert torch.isfinite(out[~broken]).all(), f"{int((~torch.isfinite(out) & ~broken).sum())} outputs that do not see it"
+    ref, mass_v, _, mass_qk = attention(q[0].to(F64), k, v.nan_to_num(0.0, 0.0, 0.0), last)
+    check_out(torch.where(broken, 0.0, out.float()), torch.where(broken, 0.0, ref), mass_v, mass_qk, "the others")

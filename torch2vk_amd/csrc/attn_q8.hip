@@ -174,6 +174,14 @@ __device__ __forceinline__ uint32_t bf16_codes(uint32_t w0, uint32_t w1, float i
                     __uint_as_float(w1 & 0xffff0000u), inv);
 }
 
+// Whether the low or the high one of two bf16 values is a NaN or an infinity, which becomes 0.
+__device__ __forceinline__ bool bf16_drop_broken(uint32_t& w, int high) {
+    const uint32_t mask = high ? 0xffff0000u : 0xffffu;
+    if ((w & mask & 0x7f807f80u) != (mask & 0x7f807f80u)) return false;
+    w &= ~mask;
+    return true;
+}
+
 // Two floats past the caches that the chip's parts do not share.
 __device__ __forceinline__ void put_pair(float* p, float x, float y) {
     __hip_atomic_store(reinterpret_cast<uint64_t*>(p), (uint64_t)__float_as_uint(x) | (uint64_t)__float_as_uint(y) << 32,
@@ -975,6 +983,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_chunk_q8_kernel(const Chun
         // bf16 rows as they are; weights in two bf16 terms
         const size_t at = a.c.tail_at(seq, h);
         const int live = s.end % Q8_BLOCK;
+        int* const broken_from = reinterpret_cast<int*>(values[1]);  // [128]; no one reads that buffer any more
 #pragma unroll
         for (int i = 0; i < 2 * PIECES; ++i) {
             const int n = tid + THREADS * i;
@@ -986,6 +995,17 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_chunk_q8_kernel(const Chun
                 if ((n & 7) * 8 + 2 * e >= live) w[e] = 0u;
                 else if ((n & 7) * 8 + 2 * e + 1 >= live) w[e] &= 0xffffu;
             }
+            // A NaN or an infinity would make the products of rows that do not see its token NaN too (0 times it): they take it
+            // for 0, and the first such token of a dim is noted.
+            int first = Q8_BLOCK;
+            if (__any(max(max(bf16_abs_max(v.x), bf16_abs_max(v.y)), max(bf16_abs_max(v.z), bf16_abs_max(v.w))) >= 0x7f800000u)) {
+#pragma unroll
+                for (int e = 7; e >= 0; --e)
+                    if (bf16_drop_broken(w[e >> 1], e & 1)) first = (n & 7) * 8 + e;
+#pragma unroll
+                for (int off = 1; off < 8; off <<= 1) first = min(first, __shfl_xor(first, off));  // the dim's 8 lanes
+            }
+            if ((n & 7) == 0) broken_from[n >> 3] = first;
             values[0][cq_value_at(n >> 3, n & 7)] = v;
         }
         __syncthreads();
@@ -995,6 +1015,14 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_chunk_q8_kernel(const Chun
             if (smax == 0.0f) smax = 1.0f;
             float f = a.scale_log2, shift = __builtin_amdgcn_logf(DQ_P_SCALE / smax);
             ready(x, tail_b, f, shift, 1.0f);
+            if (__any(min(broken_from[lane], broken_from[lane + 64]) < Q8_BLOCK)) {
+                const int mine = last - tail_b * Q8_BLOCK;
+#pragma unroll
+                for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        if (broken_from[32 * dt + 8 * (j >> 2) + 4 * half + (j & 3)] <= mine) o[dt][j] = __uint_as_float(0x7fc00000u);
+            }
             const float base = (m == -INFINITY ? 0.0f : m) - shift;
             float sum = 0.0f;
 #pragma unroll
@@ -1450,6 +1478,29 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_rows_q8_kernel(const Ch
         for (int n = 0; n < 8; ++n) {
             tv[n] = *reinterpret_cast<const uint2*>(a.c.vt + tail + vrow + n * 16 * Q8_BLOCK + 4 * wave);
             tv[n] = make_uint2(tv[n].x & live0, tv[n].y & live1);
+        }
+        // A NaN or an infinity would make the outputs of rows that do not see its token NaN too (0 times it): it is taken for 0,
+        // and the rows that see it become NaN in its dim.
+        uint32_t largest = 0;
+#pragma unroll
+        for (int n = 0; n < 8; ++n) largest = max(largest, max(bf16_abs_max(tv[n].x), bf16_abs_max(tv[n].y)));
+        if (__any(largest >= 0x7f800000u)) {
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                int first = Q8_BLOCK;  // of dim 16 n + c
+#pragma unroll
+                for (int e = 3; e >= 0; --e)
+                    if (bf16_drop_broken(e < 2 ? tv[n].x : tv[n].y, e & 1)) first = 16 * g4 + 4 * wave + e;
+                first = min(first, __shfl_xor(first, 16));
+                first = min(first, __shfl_xor(first, 32));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int from = __shfl(first, 4 * g4 + i);
+#pragma unroll
+                    for (int ct = 0; ct < CT; ++ct)
+                        if (from <= last[ct] - tail_b * Q8_BLOCK) o[ct][n][i] = __uint_as_float(0x7fc00000u);
+                }
+            }
         }
         const float f_unit = DQ_P_SCALE / (smax > 0.0f ? smax : 1.0f);
 #pragma unroll
