@@ -60,3 +60,19 @@ def test_a_broken_value_of_the_tail_reaches_the_rows_that_see_it(device, nh, nk,
     assert torch.isfinite(out[~broken]).all(), f"{int((~torch.isfinite(out) & ~broken).sum())} outputs that do not see it"
     ref, mass_v, _, mass_qk = attention(q[0].to(F64), k, v.nan_to_num(0.0, 0.0, 0.0), last)
     check_out(torch.where(broken, 0.0, out.float()), torch.where(broken, 0.0, ref), mass_v, mass_qk, "the others")
+
+
+# -------------------------------------------------------------------------------------- rows past a count
+
+
+@pytest.mark.parametrize("nh,nk,n,length,count,s_cap", [(4, 2, 5, 100, 3, 192), (8, 2, 8, 200, 1, 256), (4, 2, 6, 5000, 4, 5056),
+                                                        (4, 2, 90, 200, 40, 320)])
+@pytest.mark.parametrize("part", ["k_scale", "v_scale"])
+def test_rows_past_a_count_are_zeros_beside_a_broken_block(device, nh, nk, n, length, count, s_cap, part):
+    c = filled(1, s_cap, nk, [length + count], device, 52)
+    getattr(c, part)[0, 0, 0] = math.nan
+    q = chunk_rows((1, n, nh, D), device, 53)
+    out = K.flash_attn_prefill_q8(q, c, ints([length], device), torch.full_like(q, 7.0), counts=ints([count], device))[0]
+    group = nh // nk
+    assert out[:count, :group].isnan().all() and torch.isfinite(out[:count, group:]).all()
+    assert torch.equal(out[count:], torch.zeros_like(out[count:]))

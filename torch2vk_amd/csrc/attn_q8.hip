@@ -1558,6 +1558,7 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_rows_q8_kernel(const Ch
             sum += *reinterpret_cast<const f32x4*>(room + (w * COLS + row) * DQ_ROW + d) * f;
         }
         if (u.count == 1) {
+            if (L == 0.0f) sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};  // a row past the count: 0 times a broken block's scale is NaN
             const float inv = L == 0.0f ? 0.0f : 1.0f / L;
             *reinterpret_cast<uint2*>(a.out + row_at(row) + d) =
                 make_uint2(pack_bf16x2(sum[0] * inv, sum[1] * inv), pack_bf16x2(sum[2] * inv, sum[3] * inv));
@@ -1601,6 +1602,7 @@ __global__ __launch_bounds__(256) void attn_rows_q8_merge_kernel(const ChunkQ8Ar
             M = now;
         }
     }
+    if (L == 0.0f) sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};  // (as above)
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
     const uint32_t t = row / a.group, g = row % a.group;
     *reinterpret_cast<uint2*>(a.out + (((size_t)seq * a.n + t) * a.nh + h * a.group + g) * Q8_D + d) =
