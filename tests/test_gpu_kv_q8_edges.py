@@ -76,3 +76,31 @@ def test_rows_past_a_count_are_zeros_beside_a_broken_block(device, nh, nk, n, le
     group = nh // nk
     assert out[:count, :group].isnan().all() and torch.isfinite(out[:count, group:]).all()
     assert torch.equal(out[count:], torch.zeros_like(out[count:]))
+
+
+# --------------------------------------------------------------------------- value scales that lie far apart
+
+
+@pytest.mark.parametrize("low,high", [(-90, 50), (-99, 100), (-60, 0)])
+@pytest.mark.parametrize("order", ["low first", "high first", "between"])
+@pytest.mark.parametrize("n,s_cap", [(250, 256), (250, 4096)])
+def test_chunk_of_value_scales_far_apart(device, low, high, order, n, s_cap):
+    """Whole blocks whose value scales are 2^60 to 2^199 apart: every output is finite, rows that see the small ones only are
+    as good as among small ones (a tile of 128 tokens holds rows of two blocks), and the weights, which no value has part
+    in, are what they are."""
+    nh, nk = 2, 2
+    c = filled(1, s_cap, nk, [n], device, 54)
+    at = {"low first": [low, high, high], "high first": [high, low, low], "between": [low, high, low]}[order]
+    for b, e in enumerate(at):
+        c.v_scale[0, b] = 2.0 ** e
+    c.v_tail.mul_(2.0 ** low)
+    q = chunk_rows((1, n, nh, D), device, 55)
+    w = torch.rand(1, nk, s_cap, device=device)
+    w_out = torch.full_like(w, 0.25)
+    out = K.flash_attn_prefill_q8(q, c, ints([0], device), weights=w, weights_out=w_out)[0]
+    assert torch.isfinite(out).all() and torch.isfinite(w_out).all()
+    k, v = rows_of(c, 0, n)
+    last = torch.arange(n, device=device)
+    check_rows(out, q[0].to(F64), k, v, last, f"{order} 2^{low} 2^{high}")
+    _, _, p, mass_qk = attention(q[0].to(F64), k, v, last)
+    check_weights(w_out[0], torch.full_like(w[0], 0.25), p, 0, nh // nk, mass_qk, "weights")

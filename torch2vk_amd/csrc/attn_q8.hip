@@ -706,8 +706,9 @@ static uint32_t dq_units(uint32_t n_seq, uint32_t nk, uint32_t nb) {
 //   * S^T = K . Q^T and O^T = V^T . P^T (32 x 32 x 16), so that a lane has 32 of a row's 64 scores in registers: one
 //     exchange a step for the row's maximum, none between the products (the key rows are taken in the order that makes a
 //     lane's scores the tokens of its operand of the second one);
-//   * scales go into the exponent: p of a block is exp2(s * ks + log2(vs / largest vs so far) - max); the accumulators follow a
-//     maximum only when it has grown by more than 2^2, and a scale when it has more than doubled.
+//   * scales go into the exponent: p of a block is exp2(s * ks + log2(vs / largest vs so far) - max), rounded once to fp16's 11
+//     bits; the accumulators follow a maximum only when it has grown by more than 2^2, and a scale when it has more than
+//     doubled, and then only in the rows that see its block.
 // Where there are few rows the keys are split over thread blocks, and a second kernel joins the parts.
 //
 // Measured (32 / 8 heads): 8 x 2048 tokens 320 us, 860 TFLOP/s of the pairs that are seen; a prompt of 16000 1060, where a bf16
@@ -720,6 +721,7 @@ static uint32_t dq_units(uint32_t n_seq, uint32_t nk, uint32_t nb) {
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr uint32_t CQ_WIDE_GRID = 512;
+constexpr float CQ_SHIFT_LEAST = -60.0f;
 constexpr float CQ_SLACK = 2.0f;        // log2 that a row's weights may pass 1 by: 2^12 * 2^2 * 2 is in fp16's range
 
 struct ChunkQ8Args {
@@ -833,6 +835,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_chunk_q8_kernel(const Chun
     for (int i = 0; i < 8; ++i) q[i] = load_u4(qp + 16 * i);
     float m = -INFINITY, l = 0.0f;
     float smax = 0.0f;  // the largest value scale so far, or half of it: the accumulators are in units of smax / 2^12
+    float own = 0.0f;   // the same of the blocks that the row sees, which its accumulators stay in
     float to_unit = DQ_P_SCALE;
     f32x16 o[4];
 #pragma unroll
@@ -884,7 +887,9 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_chunk_q8_kernel(const Chun
             const float keep = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - now);
             l *= keep;
             m = now;
-            const float turn = keep * unit;
+            const bool sees = last >= b * Q8_BLOCK;
+            const float turn = sees ? keep * unit : keep;
+            if (sees) own = smax;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -949,6 +954,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_chunk_q8_kernel(const Chun
         }
         // a block of zeros may have any scale: its scores or its values are zeros all the same
         float shift = vf_scale == 0.0f ? 0.0f : __builtin_amdgcn_logf(vf_scale * to_unit);
+        // Weights under 2^-25 of a unit are 0 in fp16 already; further down their fp32 sum would go the same way.
+        if (shift < CQ_SHIFT_LEAST) shift = CQ_SHIFT_LEAST;
         float f = (kf_scale == 0.0f ? 1.0f : kf_scale) * a.scale_log2;
         ready(x, b, f, shift, unit);
         const float base = (m == -INFINITY ? 0.0f : m) - shift;
@@ -1015,6 +1022,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_chunk_q8_kernel(const Chun
             if (smax == 0.0f) smax = 1.0f;
             float f = a.scale_log2, shift = __builtin_amdgcn_logf(DQ_P_SCALE / smax);
             ready(x, tail_b, f, shift, 1.0f);
+            if (tail_b * Q8_BLOCK <= last) own = smax;
             if (__any(min(broken_from[lane], broken_from[lane + 64]) < Q8_BLOCK)) {
                 const int mine = last - tail_b * Q8_BLOCK;
 #pragma unroll
@@ -1048,14 +1056,14 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_chunk_q8_kernel(const Chun
     l = xor_sum<32>(l);
     // a lane's outputs: dims 32 dt + 8 (j / 4) + 4 half + j % 4 of its row; rows past the count are zeros
     if (row >= (int)a.n * group) return;
-    if (row >= rows || smax == 0.0f) {
+    if (row >= rows || own == 0.0f) {
         if (row >= rows) m = -INFINITY, l = 0.0f;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int j = 0; j < 16; ++j) o[i][j] = 0.0f;
     }
-    const float unit = smax * (1.0f / DQ_P_SCALE);
+    const float unit = own * (1.0f / DQ_P_SCALE);
     if (a.splits == 1) {
         const float inv = l == 0.0f ? 0.0f : unit / l;
         uint16_t* to = a.out + (((size_t)seq * a.n + t) * a.nh + h * group + g) * Q8_D + 4 * half;
