@@ -104,3 +104,27 @@ def test_chunk_of_value_scales_far_apart(device, low, high, order, n, s_cap):
     check_rows(out, q[0].to(F64), k, v, last, f"{order} 2^{low} 2^{high}")
     _, _, p, mass_qk = attention(q[0].to(F64), k, v, last)
     check_weights(w_out[0], torch.full_like(w[0], 0.25), p, 0, nh // nk, mass_qk, "weights")
+
+
+@pytest.mark.parametrize("e_block,e_tail", [(0, 115), (-85, 60), (-85, 115), (100, -90)])
+@pytest.mark.parametrize("n", [0, 5, 150])  # a single token's kernel, few rows, tiles
+@pytest.mark.parametrize("length", [10, 420])
+def test_tail_values_far_from_the_blocks(device, e_block, e_tail, n, length):
+    """The unfinished block's values 2^115 to 2^200 over or under those of the blocks, and no blocks."""
+    nh, nk, s_cap = 4, 2, 640
+    c = filled(1, s_cap, nk, [length + n], device, 56)
+    c.v_scale.mul_(2.0 ** e_block)
+    c.v_tail.mul_(2.0 ** e_tail)
+    if n == 0:
+        (q, k_new, v_new), _, _ = inputs(1, nh, nk, device, 57, 1.0)
+        out = torch.empty(1, nh, D, dtype=BF, device=device)
+        K.attn_decode_q8(q, k_new, v_new * 2.0 ** e_tail, c, out, ints([length], device),
+                         K.attn_decode_q8_workspace(1, nh, nk, D, s_cap, device), theta=0.0)
+        q, last = q.reshape(1, nh, D), torch.tensor([length], device=device)
+        k, v = rows_of(c, 0, length + 1)
+    else:
+        q = chunk_rows((n, nh, D), device, 58)
+        out = K.flash_attn_prefill_q8(q[None], c, ints([length], device))[0]
+        last = length + torch.arange(n, device=device)
+        k, v = rows_of(c, 0, length + n)
+    check_rows(out, q.to(F64), k, v, last, f"blocks 2^{e_block}, tail 2^{e_tail}")

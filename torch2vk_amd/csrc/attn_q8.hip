@@ -23,7 +23,8 @@ namespace t2h {
 //   * codes become fp16 exactly (bytes beside 0x64 are 1024 + code + 128), scales multiply scores and weights in fp32;
 //   * q is split into two fp16 terms (22 bits), so that scores are as good as fp32's; weights are rounded once, to 11 bits,
 //     relative to the wave's largest value scale times 2^12 (they stay normal over scales 2^26 apart);
-//   * the unfinished block's bf16 rows go through the bf16 products, a quarter a wave, q and weights in two bf16 terms.
+//   * the unfinished block's bf16 rows go through the bf16 products, a quarter a wave, q and weights in two bf16 terms, their
+//     values as they are.
 // The wave that holds the new token writes it; the four round its block if that is now whole, and then read it as codes.
 // Measured (32 / 8 heads): 32 sequences of 15000 to 16200 tokens 181 us, 5.6 TB/s of the cache's bytes, each read once; one of
 // 4096 tokens 11.2 us, of 200 8.0 us, where the chain of lengths, q, codes, products and join is what is left (an empty launch
@@ -473,6 +474,7 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_decode_q8_kernel(const 
         if (more) load_v(next);
     }
 
+    float unscale = (smax > 0.0f ? smax : 1.0f) * (1.0f / DQ_P_SCALE);  // the unit that the accumulators are in
     if (has_tail) {  // tile `wave` of the unfinished block
         uint4 tk[4];
         uint2 tv[8];
@@ -495,14 +497,16 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_decode_q8_kernel(const 
             x[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kk, q2[1], x[0], 0, 0, 0);
         }
         soften(x, wave, qfac, tail_b, r + 1);
-        const float f_unit = DQ_P_SCALE / (smax > 0.0f ? smax : 1.0f);
+        // the values as they are: in the blocks' unit, which they may be any number of times, products could leave fp32's range
         bf16x4 ph, pl;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float p = x[0][e] * f_unit;
-            ph[e] = (__bf16)p;
-            pl[e] = (__bf16)(p - (float)ph[e]);
+            ph[e] = (__bf16)x[0][e];
+            pl[e] = (__bf16)(x[0][e] - (float)ph[e]);
         }
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) o[dt] *= unscale;
+        unscale = 1.0f;
 #pragma unroll
         for (int dt = 0; dt < 8; ++dt) {
             o[dt] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(t2h_v4i16, tv[dt]), __builtin_bit_cast(t2h_v4i16, ph),
@@ -513,7 +517,6 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_decode_q8_kernel(const 
     }
 
     // 4. the waves' states joined; one unit: the output itself, more: the unit's part of it
-    const float unscale = (smax > 0.0f ? smax : 1.0f) * (1.0f / DQ_P_SCALE);
     l = xor_sum<32>(xor_sum<16>(l));
     if (c < group) {
 #pragma unroll
@@ -991,11 +994,17 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_chunk_q8_kernel(const Chun
         const size_t at = a.c.tail_at(seq, h);
         const int live = s.end % Q8_BLOCK;
         int* const broken_from = reinterpret_cast<int*>(values[1]);  // [128]; no one reads that buffer any more
+        uint4 vt[2 * PIECES];
 #pragma unroll
         for (int i = 0; i < 2 * PIECES; ++i) {
             const int n = tid + THREADS * i;
             keys[0][cq_key_at(n >> 4, n & 15)] = load_u4(a.c.kt + at + n * 8);
-            uint4 v = load_u4(a.c.vt + at + n * 8);
+            vt[i] = load_u4(a.c.vt + at + n * 8);
+        }
+#pragma unroll
+        for (int i = 0; i < 2 * PIECES; ++i) {
+            const int n = tid + THREADS * i;
+            uint4 v = vt[i];
             uint32_t* w = reinterpret_cast<uint32_t*>(&v);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {  // nothing that lies behind the last token
@@ -1017,12 +1026,16 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_chunk_q8_kernel(const Chun
         }
         __syncthreads();
         if (tail_b * Q8_BLOCK <= wave_last) {
+            // the values as they are: in the blocks' unit, which they may be any number of times, products could leave fp32's range
+#pragma unroll
+            for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) o[dt][j] *= own * (1.0f / DQ_P_SCALE);
+            own = smax = DQ_P_SCALE;
             f32x16 x[2];
             scores(0, x);
-            if (smax == 0.0f) smax = 1.0f;
-            float f = a.scale_log2, shift = __builtin_amdgcn_logf(DQ_P_SCALE / smax);
+            float f = a.scale_log2, shift = 0.0f;
             ready(x, tail_b, f, shift, 1.0f);
-            if (tail_b * Q8_BLOCK <= last) own = smax;
             if (__any(min(broken_from[lane], broken_from[lane + 64]) < Q8_BLOCK)) {
                 const int mine = last - tail_b * Q8_BLOCK;
 #pragma unroll
@@ -1031,7 +1044,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_chunk_q8_kernel(const Chun
                     for (int j = 0; j < 16; ++j)
                         if (broken_from[32 * dt + 8 * (j >> 2) + 4 * half + (j & 3)] <= mine) o[dt][j] = __uint_as_float(0x7fc00000u);
             }
-            const float base = (m == -INFINITY ? 0.0f : m) - shift;
+            const float base = m == -INFINITY ? 0.0f : m;
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -1050,7 +1063,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_chunk_q8_kernel(const Chun
                     o[dt] = mfma_bf16(v, pl, o[dt]);
                 }
             }
-            l = fmaf(sum, __builtin_amdgcn_exp2f(-shift), l);
+            l += sum;
         }
     }
     l = xor_sum<32>(l);
@@ -1473,6 +1486,7 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_rows_q8_kernel(const Ch
         }
         if (more) load_v(next);
     }
+    float unscale = (smax > 0.0f ? smax : 1.0f) * (1.0f / DQ_P_SCALE);
     if (has_tail) {  // tile `wave` of the unfinished block, as in the kernel of one token
         const size_t tail = a.c.tail_at(u.seq, h);
         const int ahead = s.end % Q8_BLOCK - 16 * g4 - 4 * wave;  // of a lane's 4 value tokens, those that there are
@@ -1487,30 +1501,6 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_rows_q8_kernel(const Ch
             tv[n] = *reinterpret_cast<const uint2*>(a.c.vt + tail + vrow + n * 16 * Q8_BLOCK + 4 * wave);
             tv[n] = make_uint2(tv[n].x & live0, tv[n].y & live1);
         }
-        // A NaN or an infinity would make the outputs of rows that do not see its token NaN too (0 times it): it is taken for 0,
-        // and the rows that see it become NaN in its dim.
-        uint32_t largest = 0;
-#pragma unroll
-        for (int n = 0; n < 8; ++n) largest = max(largest, max(bf16_abs_max(tv[n].x), bf16_abs_max(tv[n].y)));
-        if (__any(largest >= 0x7f800000u)) {
-#pragma unroll
-            for (int n = 0; n < 8; ++n) {
-                int first = Q8_BLOCK;  // of dim 16 n + c
-#pragma unroll
-                for (int e = 3; e >= 0; --e)
-                    if (bf16_drop_broken(e < 2 ? tv[n].x : tv[n].y, e & 1)) first = 16 * g4 + 4 * wave + e;
-                first = min(first, __shfl_xor(first, 16));
-                first = min(first, __shfl_xor(first, 32));
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int from = __shfl(first, 4 * g4 + i);
-#pragma unroll
-                    for (int ct = 0; ct < CT; ++ct)
-                        if (from <= last[ct] - tail_b * Q8_BLOCK) o[ct][n][i] = __uint_as_float(0x7fc00000u);
-                }
-            }
-        }
-        const float f_unit = DQ_P_SCALE / (smax > 0.0f ? smax : 1.0f);
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
             f32x4 x[1] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
@@ -1521,13 +1511,37 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_rows_q8_kernel(const Ch
                     as_bf16x8(*reinterpret_cast<const uint4*>(qb + (16 * ct + c) * DQ_QROW + 64 * (n >> 1) + 16 * g4 + 8 * (n & 1))),
                     x[0], 0, 0, 0);
             soften(x, ct, wave, a.scale_log2, tail_b);
+            // A NaN or an infinity would make the outputs of rows that do not see its token NaN too (0 times it): it is taken for 0,
+            // and the rows that see it become NaN in its dim.
+            uint32_t largest = 0;  // (here, where the values have come)
+#pragma unroll
+            for (int n = 0; n < 8; ++n) largest = max(largest, max(bf16_abs_max(tv[n].x), bf16_abs_max(tv[n].y)));
+            if (ct == 0 && __any(largest >= 0x7f800000u)) {
+#pragma unroll
+                for (int n = 0; n < 8; ++n) {
+                    int first = Q8_BLOCK;  // of dim 16 n + c
+#pragma unroll
+                    for (int e = 3; e >= 0; --e)
+                        if (bf16_drop_broken(e < 2 ? tv[n].x : tv[n].y, e & 1)) first = 16 * g4 + 4 * wave + e;
+                    first = min(first, __shfl_xor(first, 16));
+                    first = min(first, __shfl_xor(first, 32));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int from = __shfl(first, 4 * g4 + i);
+#pragma unroll
+                        for (int cc = 0; cc < CT; ++cc)
+                            if (from <= last[cc] - tail_b * Q8_BLOCK) o[cc][n][i] = __uint_as_float(0x7fc00000u);
+                    }
+                }
+            }
             bf16x4 ph, pl;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float p = x[0][e] * f_unit;
-                ph[e] = (__bf16)p;
-                pl[e] = (__bf16)(p - (float)ph[e]);
+                ph[e] = (__bf16)x[0][e];
+                pl[e] = (__bf16)(x[0][e] - (float)ph[e]);
             }
+#pragma unroll
+            for (int dt = 0; dt < 8; ++dt) o[ct][dt] *= unscale;
 #pragma unroll
             for (int dt = 0; dt < 8; ++dt) {
                 const t2h_v4i16 v = __builtin_bit_cast(t2h_v4i16, tv[dt]);
@@ -1535,10 +1549,10 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_rows_q8_kernel(const Ch
                 o[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(v, __builtin_bit_cast(t2h_v4i16, pl), o[ct][dt], 0, 0, 0);
             }
         }
+        unscale = 1.0f;
     }
 
     // the waves' states joined
-    const float unscale = (smax > 0.0f ? smax : 1.0f) * (1.0f / DQ_P_SCALE);
     __syncthreads();
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
