@@ -128,3 +128,32 @@ def test_tail_values_far_from_the_blocks(device, e_block, e_tail, n, length):
         last = length + torch.arange(n, device=device)
         k, v = rows_of(c, 0, length + n)
     check_rows(out, q.to(F64), k, v, last, f"blocks 2^{e_block}, tail 2^{e_tail}")
+
+
+# ------------------------------------------------------------------------------------------ a chunk's weights
+
+
+@pytest.mark.parametrize("nh,nk,n,length,s_cap", [(4, 2, 200, 0, 256), (4, 2, 200, 70, 320), (4, 2, 5, 300, 320),
+                                                  (4, 2, 100, 150, 8192)])
+def test_weights_beside_a_block_of_broken_values(device, nh, nk, n, length, s_cap):
+    """The weights are the softmax of the scores: a NaN among the values, which makes the outputs that see it NaN, has no part
+    in them."""
+    end = length + n
+    c = filled(1, s_cap, nk, [end], device, 59)
+    q = chunk_rows((1, n, nh, D), device, 60)
+    w = torch.rand(1, nk, s_cap, device=device)
+    want = torch.full_like(w, 0.25)
+    K.flash_attn_prefill_q8(q, c, ints([length], device), weights=w, weights_out=want)
+    assert torch.isfinite(want).all()
+    c.v_scale[0, 1, 0] = math.nan
+    got = torch.full_like(w, 0.25)
+    out = K.flash_attn_prefill_q8(q, c, ints([length], device), weights=w, weights_out=got)[0]
+    sees = length + torch.arange(n, device=device) >= B
+    assert out[sees][:, :nh // nk].isnan().all() and torch.isfinite(out[:, nh // nk:]).all()
+    assert torch.isfinite(out[~sees]).all()
+    k, v = rows_of(c, 0, end)
+    assert torch.isfinite(got).all()
+    _, _, p, mass_qk = attention(q[0].to(F64), k, torch.zeros_like(v), length + torch.arange(n, device=device))
+    prior = torch.full_like(w[0], 0.25)
+    prior[:, :length] = w[0, :, :length]
+    check_weights(got[0], prior, p, length, nh // nk, mass_qk, "weights")

@@ -859,12 +859,12 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_chunk_q8_kernel(const Chun
         }
     };
     // What comes before the weights: rows that do not see all of the block, and the row's maximum, which the accumulators
-    // follow.  A lane's scores j of tile tt are the tokens 32 tt + 16 (j / 8) + 8 half + j % 8; f is their factor, 2^shift
-    // the weights', unit what the accumulators' unit is to be multiplied by (1: as it is).
-    auto ready = [&](f32x16 (&x)[2], int b, float& f, float& shift, float unit) {
+    // follow.  A lane's scores j of tile tt are the tokens 32 tt + 16 (j / 8) + 8 half + j % 8; f is their factor, unit what the
+    // accumulators' unit is to be multiplied by (1: as it is).
+    auto ready = [&](f32x16 (&x)[2], int b, float& f, float unit) {
         if (b * Q8_BLOCK + Q8_BLOCK - 1 > wave_first) {
             const int mine = last - b * Q8_BLOCK - 8 * half;
-            const bool broken = f != f || shift != shift;  // a scale that is NaN reaches the rows that see its block only
+            const bool broken = f != f;  // a scale that is NaN reaches the rows that see its block only
 #pragma unroll
             for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
@@ -872,10 +872,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_chunk_q8_kernel(const Chun
                     if (broken) x[tt][j] = __uint_as_float(0x7fc00000u);
                     if (32 * tt + 16 * (j >> 3) + (j & 7) > mine) x[tt][j] = -INFINITY;
                 }
-            if (broken) {
-                f = 1.0f;
-                shift = 0.0f;
-            }
+            if (broken) f = 1.0f;
         }
         // the maximum before the factor: ks and the scale are not negative
         float top = -INFINITY;
@@ -950,17 +947,19 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_chunk_q8_kernel(const Chun
         vs = vs_next;
         if (b + 2 < whole) load(b + 2);
         float unit = 1.0f;
-        if (vf_scale > 2.0f * smax) {  // up to twice the unit's scale is in fp16's range too
-            unit = smax / vf_scale;
-            smax = vf_scale;
-            to_unit = DQ_P_SCALE / smax;
+        if (!(vf_scale <= 2.0f * smax)) {  // up to twice the unit's scale is in fp16's range too
+            unit = smax / vf_scale;        // NaN: so become the outputs of the rows that see the block, but not their sums
+            if (vf_scale == vf_scale) {
+                smax = vf_scale;
+                to_unit = DQ_P_SCALE / smax;
+            }
         }
         // a block of zeros may have any scale: its scores or its values are zeros all the same
-        float shift = vf_scale == 0.0f ? 0.0f : __builtin_amdgcn_logf(vf_scale * to_unit);
+        float shift = vf_scale > 0.0f ? __builtin_amdgcn_logf(vf_scale * to_unit) : 0.0f;
         // Weights under 2^-25 of a unit are 0 in fp16 already; further down their fp32 sum would go the same way.
         if (shift < CQ_SHIFT_LEAST) shift = CQ_SHIFT_LEAST;
         float f = (kf_scale == 0.0f ? 1.0f : kf_scale) * a.scale_log2;
-        ready(x, b, f, shift, unit);
+        ready(x, b, f, unit);
         const float base = (m == -INFINITY ? 0.0f : m) - shift;
         float sum = 0.0f;
         uint4 vf[3];
@@ -1034,8 +1033,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_chunk_q8_kernel(const Chun
             own = smax = DQ_P_SCALE;
             f32x16 x[2];
             scores(0, x);
-            float f = a.scale_log2, shift = 0.0f;
-            ready(x, tail_b, f, shift, 1.0f);
+            float f = a.scale_log2;
+            ready(x, tail_b, f, 1.0f);
             if (__any(min(broken_from[lane], broken_from[lane + 64]) < Q8_BLOCK)) {
                 const int mine = last - tail_b * Q8_BLOCK;
 #pragma unroll
@@ -1069,8 +1068,9 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_chunk_q8_kernel(const Chun
     l = xor_sum<32>(l);
     // a lane's outputs: dims 32 dt + 8 (j / 4) + 4 half + j % 4 of its row; rows past the count are zeros
     if (row >= (int)a.n * group) return;
-    if (row >= rows || own == 0.0f) {
-        if (row >= rows) m = -INFINITY, l = 0.0f;
+    if (row >= rows) {
+        m = -INFINITY;
+        l = 0.0f;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
