@@ -157,3 +157,21 @@ def test_weights_beside_a_block_of_broken_values(device, nh, nk, n, length, s_ca
     prior = torch.full_like(w[0], 0.25)
     prior[:, :length] = w[0, :, :length]
     check_weights(got[0], prior, p, length, nh // nk, mass_qk, "weights")
+
+
+def test_a_first_query_of_nan_adds_to_what_it_sees(device):
+    """A first query of NaN makes the weights of the first token NaN, which it sees, and no others, whatever rows the last
+    step of the chunk's queries does not fill."""
+    n, s_cap = 200, 256
+    c = filled(1, s_cap, 1, [n], device, 61)
+    q = chunk_rows((1, n, 1, D), device, 62)
+    k, v = rows_of(c, 0, n)
+    _, _, p, mass_qk = attention(q[0].to(F64), k, v, torch.arange(n, device=device))
+    q[0, 0] = math.nan
+    w = torch.full((1, 1, s_cap), 0.25, device=device)
+    out = K.flash_attn_prefill_q8(q, c, ints([0], device), weights=w)[0]
+    assert out[0].isnan().all() and torch.isfinite(out[1:]).all()
+    assert w[0, 0, 0].isnan()
+    assert torch.isfinite(w[0, 0, 1:]).all()
+    w[0, 0, 0] = p[0, :, 0].sum()
+    check_weights(w[0], torch.full_like(w[0], 0.25), p, 0, 1, mass_qk, "weights")

@@ -1183,13 +1183,15 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_q8_weights_kernel(const Chu
         g_at[i] = row - t * group;
         q_at[i] = (uint32_t)t * a.nh + (uint32_t)g_at[i];
     }
+    // (in the place of a row that is not there the last one, which sees every token: a NaN of it is in every sum already)
+    const uint32_t q_last = rows > 0 ? (uint32_t)((rows - 1) / group) * a.nh + (uint32_t)((rows - 1) % group) : 0u;
     const int g_step = STEP % group;
     const uint32_t q_step = (uint32_t)(STEP / group) * a.nh + (uint32_t)g_step, q_wrap = a.nh - a.group;
     const uint16_t* const q_from = a.q + ((size_t)seq * a.n * a.nh + h * group) * Q8_D + 8 * (tid & 15);
     auto load = [&](int row0) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            next[i] = load_u4(q_from + (size_t)(row0 + (tid >> 4) + 16 * i < rows ? q_at[i] : 0u) * Q8_D);
+            next[i] = load_u4(q_from + (size_t)(row0 + (tid >> 4) + 16 * i < rows ? q_at[i] : q_last) * Q8_D);
             g_at[i] += g_step;
             q_at[i] += q_step + (g_at[i] >= group ? q_wrap : 0u);
             g_at[i] -= g_at[i] >= group ? group : 0;
