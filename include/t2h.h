@@ -624,7 +624,7 @@ int t2h_attn_decode_q8(const float* q, uint64_t q_row, const float* k_new, uint6
 /* Causal attention of a chunk that t2h_qk_norm_rope_cache_q8 has written, with the same lengths and counts: query t of
  * q bf16 [n_seq, n, nh, 128] sees tokens 0 .. length + t.  out as q (both 16-byte aligned); scale <= 0 means 1 / sqrt(128);
  * weights as above, of all the chunk's queries.  workspace: 16-byte aligned, no initialisation; calls that share one must
- * not overlap in time. */
+ * not overlap in time.  n = 0 (q, out and workspace may be NULL): weights_out = weights. */
 size_t t2h_flash_attn_prefill_q8_workspace_bytes(uint32_t n, uint32_t n_seq, uint32_t nh, uint32_t nk, uint32_t s_cap,
                                                  int weights);
 int t2h_flash_attn_prefill_q8(const void* q, void* const* cache, uint32_t s_cap, const int32_t* lengths,

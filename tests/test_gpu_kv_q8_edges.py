@@ -175,3 +175,19 @@ def test_a_first_query_of_nan_adds_to_what_it_sees(device):
     assert torch.isfinite(w[0, 0, 1:]).all()
     w[0, 0, 0] = p[0, :, 0].sum()
     check_weights(w[0], torch.full_like(w[0], 0.25), p, 0, 1, mass_qk, "weights")
+
+
+@pytest.mark.parametrize("counts", [None, [0, 0, 0]])
+def test_weights_of_a_chunk_without_tokens(device, counts):
+    """No new token: weights_out holds the cached tokens' weights as they were."""
+    lengths, nk, s_cap = [100, -1, 500], 2, 256
+    c = filled(3, s_cap, nk, lengths, device, 63)
+    w = torch.rand(3, nk, s_cap, device=device)
+    w_out = torch.full_like(w, -7.0)
+    q = torch.zeros(3, 0 if counts is None else 4, 4, D, dtype=BF, device=device)
+    out = K.flash_attn_prefill_q8(q, c, ints(lengths, device), weights=w, weights_out=w_out,
+                                  counts=None if counts is None else ints(counts, device))
+    assert not out.any()
+    for i, length in enumerate(lengths):
+        end = max(0, min(length, s_cap))
+        assert torch.equal(w_out[i, :, :end], w[i, :, :end]) and bool((w_out[i, :, end:] == -7).all())

@@ -1762,14 +1762,13 @@ extern "C" int t2h_flash_attn_prefill_q8(const void* q, void* const* cache, uint
                                          uint32_t n, uint32_t n_seq, uint32_t nh, uint32_t nk, uint32_t d, float scale,
                                          void* workspace, size_t workspace_bytes, void* stream) {
     ChunkQ8Args a;
-    if (!q || !lengths || !out || !workspace) return T2H_ERR_NULL;
+    if (!lengths || (n && (!q || !out || !workspace))) return T2H_ERR_NULL;
     if ((weights == nullptr) != (weights_out == nullptr)) return T2H_ERR_NULL;
     if (const int e = q8_cache(cache, s_cap, n_seq, nh, nk, d, a.c)) return e;
     if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) & 15)
         return T2H_ERR_ALIGN;
-    if (workspace_bytes < t2h_flash_attn_prefill_q8_workspace_bytes(n, n_seq, nh, nk, s_cap, weights != nullptr))
+    if (n && workspace_bytes < t2h_flash_attn_prefill_q8_workspace_bytes(n, n_seq, nh, nk, s_cap, weights != nullptr))
         return T2H_ERR_WORKSPACE;
-    if (n == 0) return T2H_OK;
     a.q = reinterpret_cast<const uint16_t*>(q);
     a.out = reinterpret_cast<uint16_t*>(out);
     a.lengths = lengths;
@@ -1778,6 +1777,17 @@ extern "C" int t2h_flash_attn_prefill_q8(const void* q, void* const* cache, uint
     a.w_out = weights_out;
     a.n = n;
     a.n_seq = n_seq;
+    const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    const uint64_t sums = ((uint64_t)n_seq * nk * s_cap + 1023) / 1024;
+    if (sums > 0x7fffffffu) return T2H_ERR_SHAPE;
+    if (n == 0) {  // no shares: the cached tokens' weights as they are
+        if (weights == weights_out) return T2H_OK;
+        a.w_part = nullptr;
+        a.w_splits = 0;
+        hipLaunchKernelGGL(attn_chunk_q8_weights_merge_kernel, dim3((uint32_t)sums), dim3(256), 0, st, a);
+        T2H_LAUNCH_CHECK();
+        return T2H_OK;
+    }
     a.nh = nh;
     a.group = nh / nk;
     a.scale_log2 = 1.4426950408889634f * (scale > 0.0f ? scale : 1.0f / sqrtf((float)Q8_D));
@@ -1806,7 +1816,6 @@ extern "C" int t2h_flash_attn_prefill_q8(const void* q, void* const* cache, uint
     const uint64_t merge = few ? ((uint64_t)n * a.group + 7) / 8 * n_seq * nk : (rows + 7) / 8;
     const uint64_t wgrid = (uint64_t)n_seq * nk * ((a.c.nb + 3) / 4) * a.w_splits;
     if (grid > 0x7fffffffu || merge > 0x7fffffffu || wgrid > 0x7fffffffu) return T2H_ERR_SHAPE;
-    const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     if (few && n * a.group <= 16)
         hipLaunchKernelGGL(attn_rows_q8_kernel<1>, dim3((uint32_t)grid), dim3(DQ_WAVES * 64), 0, st, a);
     else if (few)
@@ -1827,7 +1836,6 @@ extern "C" int t2h_flash_attn_prefill_q8(const void* q, void* const* cache, uint
         hipLaunchKernelGGL(attn_chunk_q8_weights_kernel, dim3((uint32_t)wgrid), dim3(256), 0, st, a);
         T2H_LAUNCH_CHECK();
         if (a.w_splits > 1) {
-            const uint64_t sums = ((uint64_t)n_seq * nk * s_cap + 1023) / 1024;
             hipLaunchKernelGGL(attn_chunk_q8_weights_merge_kernel, dim3((uint32_t)sums), dim3(256), 0, st, a);
             T2H_LAUNCH_CHECK();
         }

@@ -1862,7 +1862,7 @@ def flash_attn_prefill_q8(q: torch.Tensor, cache: KVCacheQ8, lengths: torch.Tens
     _q8_heads(nh, nk)
     if out is None:
         out = torch.empty_like(q)
-    if n == 0:
+    if n == 0 and weights_out is None:
         return out
     nbytes = _lib.lib().t2h_flash_attn_prefill_q8_workspace_bytes(n, n_seq, nh, nk, cache.s_cap, int(weights is not None))
     workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
