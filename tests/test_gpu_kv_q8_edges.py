@@ -191,3 +191,41 @@ def test_weights_of_a_chunk_without_tokens(device, counts):
     for i, length in enumerate(lengths):
         end = max(0, min(length, s_cap))
         assert torch.equal(w_out[i, :, :end], w[i, :, :end]) and bool((w_out[i, :, end:] == -7).all())
+
+
+# ----------------------------------------------------------------------- queries of very different elements
+
+
+@pytest.mark.parametrize("small", [-10, -16, -20])
+@pytest.mark.parametrize("n", [0, 3])  # a single token's kernel, few rows
+def test_small_elements_of_a_query_keep_their_precision(device, n, small):
+    """A query's elements 2^10 to 2^20 under its largest, whose keys are zeros, so that the small ones alone make the scores:
+    these are within 2^-18 of sum |q k| all the same."""
+    nh, nk, length, s_cap = 4, 2, 400, 448
+    c = filled(1, s_cap, nk, [length + n], device, 64, 1.0)
+    c.k[..., :D // 2] = 0
+    c.k_tail[..., :D // 2] = 0
+    c.k_scale.mul_(2.0 ** -small)
+    c.k_tail.mul_(2.0 ** -small)
+    (q, k_new, v_new), _, _ = inputs(max(1, n), nh, nk, device, 65, 1.0)
+    q = q.reshape(-1, nh, D).clone()
+    q[..., D // 2:] *= 2.0 ** small
+    if n == 0:
+        k_new = k_new.reshape(1, nk, D).clone()
+        k_new[..., :D // 2] = 0
+        out = torch.empty(1, nh, D, dtype=BF, device=device)
+        K.attn_decode_q8(q.reshape(1, -1), (k_new * 2.0 ** -small).reshape(1, -1), v_new, c, out, ints([length], device),
+                         K.attn_decode_q8_workspace(1, nh, nk, D, s_cap, device), theta=0.0)
+        last = torch.tensor([length], device=device)
+    else:
+        q = q.to(BF)
+        out = K.flash_attn_prefill_q8(q[None], c, ints([length], device))[0]
+        last = length + torch.arange(n, device=device)
+    w = torch.zeros(1, nk, s_cap, device=device)
+    k, v = rows_of(c, 0, int(last[-1]) + 1)
+    ref, mass_v, p, mass_qk = attention(q.to(F64), k, v, last)
+    check_out(out, ref, mass_v, mass_qk, f"2^{small}")
+    if n:  # the weights say what the scores are, to check_weights' tolerance
+        K.flash_attn_prefill_q8(q[None], c, ints([length], device), weights=w)
+        assert torch.isfinite(w).all()
+        check_weights(w[0], torch.zeros_like(w[0]), p, length, nh // nk, mass_qk, f"2^{small}")

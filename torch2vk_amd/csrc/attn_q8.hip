@@ -21,7 +21,8 @@ namespace t2h {
 //     the softmax's weights go from one product into the other in registers, and a softmax over tokens needs two
 //     exchanges between lanes a block;
 //   * codes become fp16 exactly (bytes beside 0x64 are 1024 + code + 128), scales multiply scores and weights in fp32;
-//   * q is split into two fp16 terms (22 bits), so that scores are as good as fp32's; weights are rounded once, to 11 bits,
+//   * q is split into two fp16 terms (22 bits of elements down to 2^-16 of the largest, 18 at 2^-20), so that scores are about as
+//     good as fp32's; weights are rounded once, to 11 bits,
 //     relative to the wave's largest value scale times 2^12 (they stay normal over scales 2^26 apart);
 //   * the unfinished block's bf16 rows go through the bf16 products, a quarter a wave, q and weights in two bf16 terms, their
 //     values as they are.
@@ -193,9 +194,19 @@ __device__ __forceinline__ float2 get_pair(const float* p) {
     return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
 }
 
+// A query in fp16: its largest value is brought to [2^13, 2^14) by a power of two.  Its products with codes stay in fp32's range
+// and what fp16 holds least, 2^-24, is 2^-37 of that value or less: near 1 it would be 2^-24 of it, and an element 2^-18 of the
+// largest, whose keys may be the larger by as much, would have lost all but 7 bits.
+__device__ __forceinline__ uint32_t q_exponent(float largest) {
+    const uint32_t e = __float_as_uint(largest) >> 23;
+    return e < 14 ? 14 : (e > 253 ? 253 : e);
+}
+__device__ __forceinline__ float q_to_fp16(uint32_t e) { return __uint_as_float((267u - e) << 23); }
+__device__ __forceinline__ float q_from_fp16(uint32_t e) { return __uint_as_float((e - 13u) << 23); }
+
 template <bool WEIGHTS>
 __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_decode_q8_kernel(const DecodeQ8Args a) {
-    __shared__ __align__(16) _Float16 qs[2][16][DQ_QROW];      // q's two terms, its largest value in [1, 2)
+    __shared__ __align__(16) _Float16 qs[2][16][DQ_QROW];      // q's two terms (q_to_fp16)
     __shared__ float qf[16];                                  // what that took off, with the softmax's scale and log2 e
     __shared__ __align__(16) uint16_t fresh[2][Q8_D];         // the new token's key and value
     __shared__ float wml[DQ_WAVES][16][2];
@@ -318,16 +329,15 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_decode_q8_kernel(const 
         if (g >= group) break;
         float y[2];
         q8_norm_rope(x0[i], x1[i], has_w, w0, w1, a.eps, cs, sn, y[0], y[1]);
-        uint32_t e = __float_as_uint(wave_max(fmaxf(fabsf(y[0]), fabsf(y[1])))) >> 23;  // (a NaN stays one whatever e is)
-        e = e < 1 ? 1 : (e > 253 ? 253 : e);
-        const float down = __uint_as_float((254u - e) << 23);
+        const uint32_t e = q_exponent(wave_max(fmaxf(fabsf(y[0]), fabsf(y[1]))));  // (a NaN stays one whatever e is)
+        const float down = q_to_fp16(e);
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
             const _Float16 hi = (_Float16)(y[n] * down);
             qs[0][g][lane + 64 * n] = hi;
             qs[1][g][lane + 64 * n] = (_Float16)(y[n] * down - (float)hi);
         }
-        if (lane == 0) qf[g] = __uint_as_float(e << 23) * a.scale_log2;
+        if (lane == 0) qf[g] = q_from_fp16(e) * a.scale_log2;
     }
     if (writes) {
         float y[2];
@@ -1319,12 +1329,13 @@ __global__ __launch_bounds__(256) void attn_chunk_q8_weights_merge_kernel(const 
 //
 // Up to 32 rows of a KV head (a few drafted tokens): bound by memory like a single token, and read like one, in units of
 // blocks that a wave takes whole; the rows are the columns of one or two 16 x 16 x 32 products, each with its own last
-// token.  Their queries are bf16 already, so fp16 holds them in one term.  A second kernel joins a sequence's units.
+// token.  Their queries are bf16 already, so fp16 holds them in one term: elements down to 2^-30 of the largest exactly.  A
+// second kernel joins a sequence's units.
 // Measured (32 / 8 heads): 2 x 5 tokens at 4000 14.2 us, 1 at 8000 and its join 12.7.
 template <int CT>
 __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_rows_q8_kernel(const ChunkQ8Args a) {
     constexpr int COLS = 16 * CT;
-    // the queries (fp16 with the largest value in [1, 2), and bf16 as they came), then the waves' outputs
+    // the queries (fp16 by q_to_fp16, and bf16 as they came), then the waves' outputs
     __shared__ __align__(16) float room[DQ_WAVES * COLS * DQ_ROW];
     __shared__ float qf[COLS], wml[DQ_WAVES][COLS][2];
     _Float16* const qs = reinterpret_cast<_Float16*>(room);
@@ -1381,13 +1392,12 @@ __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_rows_q8_kernel(const Ch
     for (int i = 0; i < COLS / DQ_WAVES; ++i) {  // dims 2 lane, 2 lane + 1
         const int row = wave + DQ_WAVES * i;
         const float x = __uint_as_float(qw[i] << 16), y = __uint_as_float(qw[i] & 0xffff0000u);
-        uint32_t e = __float_as_uint(wave_max(fmaxf(fabsf(x), fabsf(y)))) >> 23;
-        e = e < 1 ? 1 : (e > 253 ? 253 : e);
-        const float down = __uint_as_float((254u - e) << 23);
+        const uint32_t e = q_exponent(wave_max(fmaxf(fabsf(x), fabsf(y))));
+        const float down = q_to_fp16(e);
         const f16x2_t two = {(_Float16)(x * down), (_Float16)(y * down)};
         *reinterpret_cast<f16x2_t*>(qs + row * DQ_QROW + 2 * lane) = two;
         *reinterpret_cast<uint32_t*>(qb + row * DQ_QROW + 2 * lane) = qw[i];
-        if (lane == 0) qf[row] = __uint_as_float(e << 23) * a.scale_log2;
+        if (lane == 0) qf[row] = q_from_fp16(e) * a.scale_log2;
     }
     __syncthreads();
     smax = wave_max(smax);
