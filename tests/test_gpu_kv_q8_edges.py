@@ -229,3 +229,21 @@ def test_small_elements_of_a_query_keep_their_precision(device, n, small):
         K.flash_attn_prefill_q8(q[None], c, ints([length], device), weights=w)
         assert torch.isfinite(w).all()
         check_weights(w[0], torch.zeros_like(w[0]), p, length, nh // nk, mass_qk, f"2^{small}")
+
+
+# ------------------------------------------------------------------------------------------------- eviction
+
+
+def test_eviction_leaves_a_sequence_that_takes_no_part(device):
+    """A negative length: nothing of that sequence in the other cache or the other weights is written."""
+    lengths, nk, keep = [300, -1, 130], 2, 2
+    c = filled(3, 320, nk, lengths, device, 66)
+    w = torch.rand(3, nk, 320, device=device)
+    dest = filled(3, 320, nk, [0, 200, 0], device, 67)
+    w_out = torch.full_like(w, -7.0)
+    before = copy_of(dest)
+    _, new = K.kv_cache_q8_evict(c, ints(lengths, device), w, keep, out=dest, weights_out=w_out)
+    assert new.tolist() == [128 + 44, -1, 130]
+    for name in ("k", "v", "k_scale", "v_scale", "k_tail", "v_tail"):
+        assert torch.equal(getattr(dest, name)[1].nan_to_num(-3.0), getattr(before, name)[1].nan_to_num(-3.0)), name
+    assert bool((w_out[1] == -7).all())

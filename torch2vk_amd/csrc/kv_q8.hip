@@ -456,7 +456,7 @@ __global__ __launch_bounds__(256, 7) void q8_evict_move_kernel(const Q8EvictArgs
         const int r = len - blocks * Q8_BLOCK;
         if (b == 0 && tid < r) w_out[stay * Q8_BLOCK + tid] = w_in[blocks * Q8_BLOCK + tid];
     }
-    if (b == 0 && !a.same) {  // the tail's rows
+    if (b == 0 && !a.same && a.lengths[seq] >= 0) {  // the tail's rows
         const uint4* src = reinterpret_cast<const uint4*>((values ? a.c.vt : a.c.kt) + a.c.tail_at(seq, h));
         uint4* dst = reinterpret_cast<uint4*>((values ? a.o.vt : a.o.kt) + a.o.tail_at(seq, h));
         for (int i = tid; i < Q8_BYTES * 2 / 16; i += 256) dst[i] = src[i];
