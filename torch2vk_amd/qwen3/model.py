@@ -62,7 +62,8 @@ class Qwen3Decoder:
 
     ``kv_bits`` 8 holds the KV cache in 8 bits (kernels.KVCacheQ8, one a layer): half the bytes an attention reads, for
     contexts where those are most of a step; the layers run one launch per op.  Such a cache goes on from its length only:
-    ``start`` of a prefill is 0 or the tokens it holds, and step_logits and forward_masked are refused.  With
+    ``start`` of a prefill is 0 or the tokens it holds (``position``, which is read back to see), a ``cache_position`` one of
+    these or the next, and step_logits and forward_masked are refused.  With
     ``kv_weights`` it also keeps each token's accumulated attention weight, by which ``evict_cache`` cuts it down."""
 
     PREFILL_GRAPHS = 4  # captured prefill graphs kept (prefill_graphed)
@@ -179,7 +180,18 @@ class Qwen3Decoder:
 
     # ----------------------------------------------------------- state --
 
+    def _goes_on(self, place: int, *places: int) -> None:
+        """An 8-bit cache holds the rows of its last, unfinished block only: at an earlier place others' would be taken for
+        those of the tokens before it.  ``places``: further ones from the tokens held.  Not looked at under capture."""
+        if self.kv_bits != 8 or place == 0 or torch.cuda.is_current_stream_capturing():
+            return
+        held = int(self.position)
+        if place - held not in (0, *places):
+            raise ValueError(f"an 8-bit KV cache goes on from its length: it holds {held} tokens, not {place} (a caller that has "
+                             "put others in place writes position)")
+
     def reset(self, position: int = 0, token: int | None = None) -> None:
+        self._goes_on(position)
         self.position.fill_(position)
         self.length.zero_()
         self.stopped.zero_()
@@ -212,7 +224,10 @@ class Qwen3Decoder:
         (run_decode_layer, src/models/optimized_qwen3/dispatch/decode_layer.py:131-136).
         A Python ``cache_position`` is written to the device counter first."""
         if cache_position is not None:
+            self._goes_on(cache_position, 1)
             self.position.fill_(cache_position)
+            if self.kv_bits == 8 and cache_position == 0:
+                self.rope_offset.zero_()
         p = f"layers.{layer_idx}."
         self._qkv(layer_idx)
         self._attention(layer_idx)
@@ -533,6 +548,7 @@ class Qwen3Decoder:
         ids = prompt_ids.to(device=self.device, dtype=torch.int64).view(-1)
         if ids.numel() == 0:
             raise ValueError("empty prompt")
+        self._goes_on(start)
         # stop_on_eos is read on the host when the token store is launched, so the capture freezes it
         key = (ids.numel(), start, chunk, bool(self.stop_on_eos))
         if key in self._prefill_graphs:
