@@ -73,3 +73,18 @@ def test_layers_at_the_places_that_follow(weights):  # noqa: F811
     other.run_decode_embed()
     other.run_decode_layer(0, cache_position=17)
     assert int(other.position) == 17
+
+
+@pytest.mark.parametrize("keep,more,recent", [(1, {}, 60), (1, dict(sink=0), 64), (2, {}, 64), (1, dict(sink=64), 0)])
+def test_default_recent_tokens_fit_the_budget(weights, keep, more, recent):  # noqa: F811
+    """evict_cache's defaults: the last 64 tokens, or as many as the first ones leave of the budget."""
+    d = decoder(weights, kv_bits=8, kv_weights=True)
+    d.prefill_chunked(prompt(200, 8))
+    kept = d.evict_cache(keep, **more)
+    assert int(d.position) == 64 * keep + 8
+    for layer in kept:
+        for row in layer[0].tolist():
+            assert row[:more.get("sink", 4)] == list(range(more.get("sink", 4)))
+            assert row[len(row) - recent:] == list(range(192 - recent, 192))
+    with pytest.raises(ValueError):
+        decoder(weights, kv_bits=8, kv_weights=True).evict_cache(1, sink=4, recent=64)

@@ -603,13 +603,16 @@ class Qwen3Decoder:
         self.run_lm_head_select()
         self.run_token_store(advance=True)
 
-    def evict_cache(self, keep_blocks: int, *, sink: int = 4, recent: int = 64) -> list[torch.Tensor]:
+    def evict_cache(self, keep_blocks: int, *, sink: int = 4, recent: int | None = None) -> list[torch.Tensor]:
         """Between two steps: every layer's KV heads keep 64 * keep_blocks of their whole blocks' tokens, the first
-        ``sink``, the last ``recent`` and those of most accumulated attention weight (kernels.kv_cache_q8_evict), in place, so
-        that captured graphs go on.  The positions of the tokens that follow stay what they would have been.  Returns each
-        layer's kept tokens, int32 [1, kv_heads, 64 * keep_blocks] of places in the cache before, -1 behind them."""
+        ``sink``, the last ``recent`` (None: 64, or what the first ones leave of the budget) and those of most accumulated
+        attention weight (kernels.kv_cache_q8_evict), in place, so that captured graphs go on.  The positions of the tokens
+        that follow stay what they would have been.  Returns each layer's kept tokens, int32 [1, kv_heads, 64 * keep_blocks]
+        of places in the cache before, -1 behind them."""
         if self.kv_weights is None:
             raise ValueError("eviction goes by accumulated weights: kv_bits=8, kv_weights=True")
+        if recent is None:
+            recent = max(0, min(64, kernels.KV_Q8_BLOCK * keep_blocks - sink))
         kept, lengths = [], self.position
         for cache, w in zip(self.kv, self.kv_weights):
             k, lengths = kernels.kv_cache_q8_evict(cache, self.position, w, keep_blocks, sink=sink, recent=recent)
