@@ -247,3 +247,89 @@ def test_eviction_leaves_a_sequence_that_takes_no_part(device):
     for name in ("k", "v", "k_scale", "v_scale", "k_tail", "v_tail"):
         assert torch.equal(getattr(dest, name)[1].nan_to_num(-3.0), getattr(before, name)[1].nan_to_num(-3.0)), name
     assert bool((w_out[1] == -7).all())
+
+
+def ranked(w, full, stay, sink, recent):
+    """Kept tokens of one head by the definition: the first and the last, then NaN, then by weight, -0 as 0, ties to the
+    earliest."""
+    def key(t):
+        x = w[t]
+        if t < sink or t >= full - recent:
+            return (0, 0.0, t)
+        return (1, 0.0, t) if math.isnan(x) else (2, -x + 0.0, t)
+
+    return sorted(sorted(range(full), key=key)[:stay])
+
+
+@pytest.mark.parametrize("inside", ["nan", "inf", "positive", "zeros", "negative", "-inf"])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_eviction_whose_cut_lies_among_special_weights(device, inside, in_place):
+    """Weights of six kinds, of which 128 tokens stay: the last that stays is one of the kind named.  NaN ranks above
+    infinity, and 0 and -0 are one weight."""
+    nk, length, keep, s_cap = 2, 520, 2, 576
+    full, sink, recent = 512, 3, 5
+    gen = torch.Generator().manual_seed(68)
+    kinds = ["nan", "inf", "positive", "zeros", "negative", "-inf"]
+    at = kinds.index(inside)
+    w = torch.zeros(1, nk, s_cap)
+    for h in range(nk):
+        # 120 of the sink, recent and all kinds above in sum; the rest of the kind named, and 60 of each below
+        counts = [0] * 6
+        for i in range(at):
+            counts[i] = 110 // at
+        for i in range(at + 1, 6):
+            counts[i] = 30
+        counts[at] = full - sink - recent - sum(counts)
+        values = []
+        for kind, count in zip(kinds, counts):
+            x = torch.rand(count, generator=gen) + 0.5
+            values.append({"nan": torch.full((count,), math.nan), "inf": torch.full((count,), math.inf), "positive": x,
+                           "zeros": torch.where(x > 1, 0.0, -0.0), "negative": -x, "-inf": torch.full((count,), -math.inf)}[kind])
+        x = torch.cat(values)
+        w[0, h, sink:full - recent] = x[torch.randperm(len(x), generator=gen)]
+    w = w.to(device)
+    host = w.cpu()
+    c = filled(1, s_cap, nk, [length], device, 69)
+    more = {} if in_place else dict(out=K.kv_cache_q8(1, s_cap, nk, D, device), weights_out=torch.zeros_like(w))
+    kept, new = K.kv_cache_q8_evict(c, ints([length], device), w, keep, sink=sink, recent=recent, **more)
+    assert int(new) == keep * B + length - full
+    for h in range(nk):
+        row = host[0, h].tolist()
+        want = ranked(row, full, keep * B, sink, recent)
+        assert kept[0, h].tolist() == want
+        rest = set(range(sink, full - recent)) - set(want)
+        same = {"nan": math.isnan, "inf": lambda x: x == math.inf, "positive": lambda x: 0 < x < math.inf,
+                "zeros": lambda x: x == 0, "negative": lambda x: -math.inf < x < 0, "-inf": lambda x: x == -math.inf}[inside]
+        assert any(same(row[t]) for t in want) and any(same(row[t]) for t in rest)  # the cut is inside
+
+
+# -------------------------------------------------------------------------------------- many wide tiles
+
+
+def test_many_ragged_tiles_of_a_group_that_does_not_divide_them(device):
+    """Over 512 tiles of 256 rows in thread blocks of 8 waves, in rounds of 256 of them of which every other runs from the
+    shortest up, a last one that is no multiple of 8 among them; with counts, lengths and a sequence that takes no part."""
+    nh, nk, n = 21, 7, 930  # 2790 rows: 11 tiles a head and sequence, 11 * 7 * 11 = 3 * 256 + 79 of them
+    lengths = [0, 70, 3, 128, -1, 64, 200, 1, 0, 31, 65]
+    counts = [930, 900, 1, 930, 930, 0, 700, 929, 930, 500, 257]
+    s_cap = 1024
+    c = filled(11, s_cap, nk, [max(0, x) + y if x >= 0 else 0 for x, y in zip(lengths, counts)], device, 70)
+    q = chunk_rows((11, n, nh, D), device, 71)
+    w = torch.rand(11, nk, s_cap, device=device)
+    w_out = torch.full_like(w, 0.25)
+    out = K.flash_attn_prefill_q8(q, c, ints(lengths, device), torch.full_like(q, math.nan), counts=ints(counts, device),
+                                  weights=w, weights_out=w_out)
+    for i, length in enumerate(lengths):
+        count = counts[i] if length >= 0 else 0
+        assert torch.equal(out[i, count:], torch.zeros_like(out[i, count:]))
+        if count == 0:
+            continue
+        end = min(length + count, s_cap)
+        k, v = rows_of(c, i, end)
+        last = (length + torch.arange(count, device=device)).clamp(max=end - 1)
+        ref, mass_v, p, mass_qk = attention(q[i, :count].to(F64), k, v, last)
+        check_out(out[i, :count], ref, mass_v, mass_qk, f"sequence {i}")
+        assert torch.isfinite(w_out[i]).all()
+        prior = torch.full_like(w[i], 0.25)
+        prior[:, :length] = w[i, :, :length]
+        check_weights(w_out[i], prior, p, length, nh // nk, mass_qk, f"weights of sequence {i}")
