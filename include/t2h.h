@@ -596,6 +596,8 @@ int t2h_slice_last_token(const float* x, void* out, int out_dtype, uint32_t b, u
  * counts (device int32 [n_seq], or NULL for n each): new tokens of each sequence, the first of its n rows; outputs of the
  * rows behind them are zeros.
  * rope_offsets (device int32 [n_seq], or NULL): position of a token = its place in the cache + offset, as after an eviction.
+ * Scores, softmax sums and kept weights are fp32; the softmax weights of whole blocks are rounded to fp16's 11 bits before the
+ * product with the values.  Accumulated weights have no part of the values: one that is not finite leaves them as they are.
  * nh / nk is a whole number up to 16. */
 #define T2H_KV_Q8_BLOCK 64
 

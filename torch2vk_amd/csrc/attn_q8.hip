@@ -647,7 +647,7 @@ constexpr int DQ_SEGMENT = 1024;  // tokens of a thread block that adds up weigh
 // weights_out[token] = weights_in (0 for the new token) + sum of exp2(score - log2 sum) over the heads of the KV head:
 // 1024 tokens of a (sequence, KV head) a thread block.  A second kernel, because a token's weight needs the sum over all units:
 // the scores pass through memory (4 bytes a head and token beside the cache's 256 a KV head and token).  6.3 us for 16
-// sequences of 100 to 8000 tokens, beside the attention's 34.6.
+// sequences of 100 to 8000 tokens, beside the attention's 35.
 __global__ __launch_bounds__(256) void attn_decode_q8_weights_kernel(const DecodeQ8Args a) {
     __shared__ float lse[16];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -724,12 +724,13 @@ static uint32_t dq_units(uint32_t n_seq, uint32_t nk, uint32_t nb) {
 //     doubled, and then only in the rows that see its block.
 // Where there are few rows the keys are split over thread blocks, and a second kernel joins the parts.
 //
-// Measured (32 / 8 heads): 8 x 2048 tokens 320 us, 860 TFLOP/s of the pairs that are seen; a prompt of 16000 1060, where a bf16
-// product of 8192^3 reaches 1197; 1901 tokens 48 us; 4 x 512 of 16 / 8 heads at 7000 148 us, 820.  At 8 x 2048 the matrix cores
-// are busy for 39 % of the time and the vector units for 50 %: about 205 vector instructions and 32 products a step, half of the
-// former the softmax's, a fifth the conversion's.  What took vector instructions out of the step paid (320 us; 337 with LDS
-// addresses that depend on the buffer and a division a step); what let the two units overlap otherwise did not: a third buffer
-// with half of the waves a phase behind, raised priority around the products, fewer LDS conflicts (22 -> 9 million cycles).
+// Measured (32 / 8 heads): 8 x 2048 tokens 318 us, 865 TFLOP/s of the pairs that are seen; a prompt of 16000 1958 us, 1071, where
+// a bf16 product of 8192^3 reaches 1197; 1901 tokens 47 us; 4 x 512 of 16 / 8 heads at 7000 144 us, 845, with the join.  At 8 x
+// 2048 the matrix cores are busy for 38 % of the time and the vector units for 50 %: about 208 vector instructions and 32 products
+// a step, half of the former the softmax's, a fifth the conversion's.  What took vector instructions out of the step paid (318 us;
+// 337 with LDS addresses that depend on the buffer and a division a step); what let the two units overlap otherwise did not: a
+// third buffer with half of the waves a phase behind, raised priority around the products, fewer LDS conflicts (22 -> 9 million
+// cycles).
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
@@ -1152,8 +1153,8 @@ __global__ __launch_bounds__(256) void attn_chunk_q8_merge_kernel(const ChunkQ8A
 // weights_out[token] = weights_in (0 for a new token) + sum of exp2(score - lse) over the rows of the KV head.  A wave takes
 // 64 tokens, one cache block, as the operand that stays in registers; the rows' queries pass through LDS, 64 at a time and
 // the next 64 on their way, the same for the thread block's four waves.  Sums are in a fixed order.  Bound by the products and
-// the three vector instructions a pair (scale, exponential, sum), which overlap little: 73 us for 4 x 512 tokens of 16 / 8
-// heads at 7000 (61 GFLOP, 237 million pairs).  Products of one half with the other half's exponentials between them took 5 %
+// the three vector instructions a pair (scale, exponential, sum), which overlap little: 80 to 87 us for 4 x 512 tokens of 16 / 8
+// heads at 7000 (61 GFLOP, 238 million pairs).  Products of one half with the other half's exponentials between them took 5 %
 // more: with both halves' scores the registers do not hold the keys.
 __global__ __launch_bounds__(256, 2) void attn_chunk_q8_weights_kernel(const ChunkQ8Args a) {
     constexpr int STEP = 64;  // rows
@@ -1331,7 +1332,7 @@ __global__ __launch_bounds__(256) void attn_chunk_q8_weights_merge_kernel(const 
 // blocks that a wave takes whole; the rows are the columns of one or two 16 x 16 x 32 products, each with its own last
 // token.  Their queries are bf16 already, so fp16 holds them in one term: elements down to 2^-30 of the largest exactly.  A
 // second kernel joins a sequence's units.
-// Measured (32 / 8 heads): 2 x 5 tokens at 4000 14.2 us, 1 at 8000 and its join 12.7.
+// Measured (32 / 8 heads): 2 x 5 tokens at 4000 12.8 us and 4.6 the join (17.1 both, 27 with weights), 1 at 8000 and its join 12.2.
 template <int CT>
 __global__ __launch_bounds__(DQ_WAVES * 64, 2) void attn_rows_q8_kernel(const ChunkQ8Args a) {
     constexpr int COLS = 16 * CT;
@@ -1645,21 +1646,25 @@ __global__ __launch_bounds__(256) void attn_rows_q8_merge_kernel(const ChunkQ8Ar
 }
 
 // Whether a KV head's rows are columns of the products of single tokens: up to two tiles of 16 (three would not leave the
-// registers a block's codes).  Measured against the kernel of 32-row waves (32 / 8 heads): 1 token at 8000 12.7 us for 25.3,
-// 2 x 5 at 4000 17.7 for 19.9, 8 at 8000 17.7.
+// registers a block's codes).  Measured against the kernel of 32-row waves (us a call, 32 / 8 heads): 1 token at 8000 12.2, 16.9;
+// 8 at 8000 17.1, 17.9; 4 x 8 at 16000 37, 42; 16 x 5 at 4000 39, 42; 16 x 8 at 8000 62, 78; 32 x 5 at 8000 115, 161; but 5 at
+// 1000 12.4, 12.1; 2 x 5 at 4000 17.1, 15.4; 2 x 8 at 4000 17.9, 15.5; 8 x 5 at 2000 21.0, 19.1, where the join's launch is 5 us.
 static bool cq_few(uint32_t n, uint32_t nh, uint32_t nk) { return (uint64_t)n * (nh / nk) <= 32; }
 
-// Waves a thread block: 8 share a block's conversion to 16 bits where that leaves two thread blocks for every CU.  Measured (32 /
-// 8 heads): 16000 tokens 942 TFLOP/s of 8, 912 of 4; 1901 tokens, 240 and 480 thread blocks, 78 us of 8, 68 of 4.
+// Waves a thread block: 8 share a block's conversion to 16 bits where that leaves two thread blocks for every CU.  Measured (us of
+// 8 and of 4, 32 / 8 heads): 16000 tokens 1958, 2068; 8 x 2048 318, 318; 1901, 240 and 480 thread blocks, 56, 47; 1500 45, 38; at
+// the border, 512 thread blocks, where those of 8 are one uneven round: 4096 tokens 169, 159; 2 x 2048 94, 87.
 static uint32_t cq_waves(uint32_t n, uint32_t n_seq, uint32_t nh, uint32_t nk) {
     return ((uint64_t)n * (nh / nk) + 255) / 256 * n_seq * nk >= CQ_WIDE_GRID ? 8 : 4;
 }
 
 // Thread blocks that share a tile's keys, in a full cache each with 4 blocks of keys or more of those that a row of the chunk's
 // middle sees: one a CU where there are not as many tiles; two a CU where that leaves each 8 blocks or more, 32 where it is what
-// brings the join with it.  Measured (us, 32 / 8 heads unless named; one a CU, two): 100 tokens at 3000 24, 28; 64 at 8000 26, 30;
-// 256 at 16000 89, 87; 512 at 8000 94, 87; and where one a CU is whole: 1000 at 0 26, 33; 2 x 512 at 2000 53, 59, at 4000 89, 90;
-// 4 x 512 of 16 / 8 heads at 7000 150, 142; 2048 of 16 / 8 at 2048 79, 72.  1901 tokens, 480 tiles: 58 whole, 64 in two parts.
+// brings the join with it.  Measured (us, 32 / 8 heads unless named; one a CU, two): 100 tokens at 3000 24, 26; 64 at 8000 25, 29;
+// 256 at 16000 89, 85; 512 at 8000 95, 87; and where one a CU is whole: 1000 at 0 26, 34; 2 x 512 at 2000 54, 59, at 4000 92, 93;
+// 4 x 512 of 16 / 8 heads at 7000 147, 144; 2048 of 16 / 8 at 2048 81, 73.
+// What the cache holds is not known here, its capacity stands for it: 100 tokens at 0 take 9 us at a capacity of 192 and 22 at 8192,
+// where the keys have 16 parts of which 14 are empty.
 static uint32_t cq_splits(uint32_t n, uint32_t n_seq, uint32_t nh, uint32_t nk, uint32_t nb) {
     const uint64_t rows = 32 * cq_waves(n, n_seq, nh, nk), tiles = ((uint64_t)n * (nh / nk) + rows - 1) / rows;
     const uint64_t grid = tiles * n_seq * nk, skip = n / (2 * Q8_BLOCK), most = nb > skip ? (nb - skip) / 4 : 0;
@@ -1673,7 +1678,8 @@ static uint32_t cq_splits(uint32_t n, uint32_t n_seq, uint32_t nh, uint32_t nk, 
 // chunk's share of the pairs) of 512 rows each or more, or one round of 128 or more.  Measured (us, 32 / 8 heads but for the
 // last two): 2048 tokens at 0: 38 in rounds of 1024 thread blocks, 48 of 512, 196 unshared; 142 tokens at 4: 14 of 128 rows, 18
 // of 256, 24 unshared; 2 x 300 of 40 / 8 at 3000: 37 of 512 rows in two rounds, 41 of 256; 300 of 16 / 2 at 2000: 18 of 128 rows
-// in one round, 22 of 64, 26 of 512.
+// in one round, 22 of 64, 26 of 512.  Here too the capacity stands for what the cache holds: 2048 tokens at 0, with their
+// attention, 89 us at a capacity of 2112, 116 at 8192, 159 at 16384 and 243 from 32768 on, where nothing is shared.
 static uint32_t cq_weight_splits(uint32_t n, uint32_t n_seq, uint32_t nh, uint32_t nk, uint32_t nb) {
     const uint64_t grid = ((uint64_t)nb + 3) / 4 * n_seq * nk, rows = (uint64_t)n * (nh / nk);
     const uint64_t large = 1024 / grid < rows / 512 ? 1024 / grid : rows / 512;

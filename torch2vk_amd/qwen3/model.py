@@ -61,10 +61,11 @@ class Qwen3Decoder:
     applies: on MI355X it saves the launch and ramp of ~250 kernels per token.
 
     ``kv_bits`` 8 holds the KV cache in 8 bits (kernels.KVCacheQ8, one a layer): half the bytes an attention reads, for
-    contexts where those are most of a step; the layers run one launch per op.  Such a cache goes on from its length only:
-    ``start`` of a prefill is 0 or the tokens it holds (``position``, which is read back to see), a ``cache_position`` one of
-    these or the next, and step_logits and forward_masked are refused.  With
-    ``kv_weights`` it also keeps each token's accumulated attention weight, by which ``evict_cache`` cuts it down."""
+    contexts where those are most of a step; the layers run one launch per op, which up to 8192 positions is slower than the
+    persistent kernel over a bf16 cache.  Such a cache goes on from its length only: ``start`` of a prefill is 0 or the
+    tokens it holds (``position``, which is read back to see), a ``cache_position`` one of these or the next, and step_logits
+    and forward_masked are refused.  With ``kv_weights`` it also keeps each token's accumulated attention weight, by which
+    ``evict_cache`` cuts it down."""
 
     PREFILL_GRAPHS = 4  # captured prefill graphs kept (prefill_graphed)
 
