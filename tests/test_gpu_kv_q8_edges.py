@@ -333,3 +333,56 @@ def test_many_ragged_tiles_of_a_group_that_does_not_divide_them(device):
         prior = torch.full_like(w[i], 0.25)
         prior[:, :length] = w[i, :, :length]
         check_weights(w_out[i], prior, p, length, nh // nk, mass_qk, f"weights of sequence {i}")
+
+
+def test_a_broken_tail_in_wide_tiles(device):
+    """As in tiles of 4 waves: a NaN and an infinity among the unfinished block's values in thread blocks of 8."""
+    nh, nk, n, n_seq, s_cap = 8, 8, 1000, 16, 1088  # 4 tiles of 256 rows a head and sequence, 512 of them
+    lengths = [7 * i for i in range(n_seq)]
+    ends = [n + x for x in lengths]
+    c = filled(n_seq, s_cap, nk, [min(x, s_cap) for x in ends], device, 72)
+    q = chunk_rows((n_seq, n, nh, D), device, 73)
+    bad = {(3, 2, 11, math.nan), (5, 7, 127, math.inf), (5, 7, 0, -math.inf)}  # sequence, head, dim of its last token
+    for i, h, d, value in bad:
+        assert ends[i] < s_cap and ends[i] % B
+        c.v_tail[i, h, d, (ends[i] - 1) % B] = value
+    out = K.flash_attn_prefill_q8(q, c, ints(lengths, device))
+    broken = torch.zeros_like(out, dtype=torch.bool)
+    for i, h, d, _ in bad:
+        broken[i, -1, h, d] = True
+    assert torch.equal(~torch.isfinite(out), broken)
+    for i in (0, 3, 5, 15):
+        end = min(ends[i], s_cap)
+        k, v = rows_of(c, i, end)
+        last = (lengths[i] + torch.arange(n, device=device)).clamp(max=end - 1)
+        ref, mass_v, _, mass_qk = attention(q[i].to(F64), k, v.nan_to_num(0.0, 0.0, 0.0), last)
+        keep = ~broken[i]
+        check_out(torch.where(keep, out[i].float(), 0.0), torch.where(keep, ref, 0.0), mass_v, mass_qk, f"sequence {i}")
+
+
+# --------------------------------------------------------------------------------------- behind a full cache
+
+
+@pytest.mark.parametrize("n", [3, 90])  # few rows, tiles
+def test_chunk_behind_a_full_cache(device, n):
+    """Lengths at and past the capacity: every query sees all cached tokens, whose weights grow; nothing is written."""
+    nh, nk, s_cap, lengths = 4, 2, 256, [256, 300, 255]
+    c = filled(3, s_cap, nk, lengths, device, 74)
+    (q, k_new, v_new), _, _ = inputs(3 * n, nh, nk, device, 75)
+    before = copy_of(c)
+    q_out = torch.empty(3, n, nh, D, dtype=BF, device=device)
+    K.qk_norm_rope_cache_q8(q, k_new, v_new, q_out, c, ints(lengths, device), theta=1e6)
+    for name in ("k", "v", "k_scale", "v_scale"):
+        assert torch.equal(getattr(c, name)[:2], getattr(before, name)[:2])
+    w = torch.rand(3, nk, s_cap, device=device)
+    w_out = torch.full_like(w, 0.25)
+    out = K.flash_attn_prefill_q8(q_out, c, ints(lengths, device), weights=w, weights_out=w_out)
+    for i, length in enumerate(lengths):
+        k, v = rows_of(c, i, s_cap)
+        last = (length + torch.arange(n, device=device)).clamp(max=s_cap - 1)
+        ref, mass_v, p, mass_qk = attention(q_out[i].to(F64), k, v, last)
+        check_out(out[i], ref, mass_v, mass_qk, f"sequence {i}")
+        assert torch.isfinite(w_out[i]).all()
+        prior = w[i].clone()
+        prior[:, min(length, s_cap):] = 0.25
+        check_weights(w_out[i], prior, p, min(length, s_cap), nh // nk, mass_qk, f"weights of sequence {i}")
