@@ -651,6 +651,64 @@ int t2h_kv_cache_q8_evict(void* const* cache, uint32_t s_cap, const int32_t* len
                           void* const* cache_out, uint32_t s_cap_out, float* weights_out, int32_t* kept,
                           int32_t* lengths_out, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------- trees of drafted tokens --- */
+/* One step over several drafted tokens of each sequence: n <= T2H_TREE_MAX_NODES rows a sequence, the nodes of a tree.
+ * parents (device int32 [n_seq][n], or NULL for chains: i - 1): node i hangs on the earlier node parents[i], or on the cached
+ * tokens (-1).  counts (device int32 [n_seq], or NULL for n each): nodes of each sequence, the first of its n rows.  A node
+ * with a parent outside [-1, i), and all that hang on it, are no nodes.  No counterpart in the reference, which decodes one
+ * token a step (src/models/optimized_qwen3/run.py:142-172). */
+#define T2H_TREE_MAX_NODES 64
+
+/* Attention of a tree's nodes over a bf16 cache.  q fp32 [n_seq * n, q_row], k_new and v_new likewise, head h at columns
+ * 128 h: per-head RMSNorm of q and k (q_norm_w / k_norm_w, both or neither) and rotate-half RoPE (theta <= 0: none; angles in
+ * fp64) at position length + the number of the node's ancestors; k and v -> slots length + i of k_cache and v_cache, bf16
+ * [n_seq][s_cap][nk][128] with k_seq and v_seq elements from one sequence to the next; then out bf16 [n_seq][n][nh][128] =
+ * softmax(q . k / sqrt(128)) . v over the `lengths` cached tokens (device int32 [n_seq]), the node's ancestors and itself.
+ * Rows that are no nodes give zeros and leave their slots; nodes without a slot (length + i >= s_cap) and those of a
+ * sequence whose length lies outside [0, s_cap] are none.  lengths is not advanced.  Values that are not finite reach the rows
+ * that see their token only.  d = 128, nh / nk a whole number up to 16; caches, out and workspace 16-byte aligned, k_seq and
+ * v_seq multiples of 8.
+ * workspace: t2h_attn_tree_workspace_bytes() bytes, zero-filled once before its first use (calls leave it reusable, for other
+ * shapes too up to n_seq * nk = 16384); calls that share one must not overlap in time. */
+size_t t2h_attn_tree_workspace_bytes(uint32_t n_seq, uint32_t n, uint32_t nh, uint32_t nk, uint32_t d, uint32_t s_cap);
+int t2h_attn_tree(const float* q, uint64_t q_row, const float* k_new, uint64_t k_row, const float* v_new, uint64_t v_row,
+                  const float* q_norm_w, const float* k_norm_w, float eps, float theta, const int32_t* lengths,
+                  const int32_t* parents, const int32_t* counts, void* k_cache, uint64_t k_seq, void* v_cache, uint64_t v_seq,
+                  uint32_t s_cap, void* out, uint32_t n, uint32_t n_seq, uint32_t nh, uint32_t nk, uint32_t d,
+                  void* workspace, size_t workspace_bytes, void* stream);
+
+/* Which drafted tokens the target's probabilities accept, and the token that follows them.  Node 0 is a token that stands
+ * already; tokens (int64 [n_seq][n]) are the nodes', logits [n_seq * n] rows of `vocab` values (fp32 or bf16: dtype), row_stride
+ * elements apart, the target's after each node.  The walk begins at node 0.  With w = exp(logit / temperature - the row's
+ * maximum) of the row it stands at and S their sum, it asks the node's children in their order: child c with token x is accepted
+ * if uniforms[c] S < w(x), and then the walk stands at c; if not, w(x) leaves the row and S.  Where no child is accepted,
+ * the next token is the first one up to which the row's sum exceeds uniforms[0] S.  So the tokens are distributed as the
+ * target's own whatever was drafted.
+ * draft (NULL, or rows as logits', [n_seq * (n - 1)], draft_stride apart; parents NULL): the drafts were drawn: row i is
+ * what token i + 1 was drawn from, at the same temperature.  With p and q the two rows' probabilities, x is accepted if
+ * uniforms[i + 1] q(x) < p(x); if not, the next token is drawn from max(p - q, 0).
+ * temperatures (device fp32 [n_seq], or NULL for `temperature`): one that is not positive is greedy: the child whose token is
+ * the row's largest logit (the lowest index of equals), and that token follows.  uniforms (fp32 [n_seq][n]) may be NULL where
+ * `temperature` is not positive and temperatures is NULL; numbers outside [0, 1) count as the nearest in it, NaN as 0.
+ * A logit of -infinity or NaN has no probability; infinite ones share it.  Sums are kept in 64 bits.
+ * path int32 [n_seq][n]: the nodes that the walk stood at, node 0 first, then -1; kept [n_seq]: how many (0 where a sequence has
+ * no nodes); next_token int64 [n_seq]: -1 where there are no nodes or no token has any probability.
+ * workspace: t2h_tree_verify_workspace_bytes() bytes, 16-byte aligned, zero-filled once before its first use (calls leave it
+ * reusable, for other shapes too up to n_seq = 16384); calls that share one must not overlap in time. */
+size_t t2h_tree_verify_workspace_bytes(uint32_t n_seq, uint32_t n, uint32_t vocab, int drawn);
+int t2h_tree_verify(const void* logits, uint64_t row_stride, const void* draft, uint64_t draft_stride, int dtype,
+                    const int64_t* tokens, const int32_t* parents, const int32_t* counts, const float* uniforms,
+                    float temperature, const float* temperatures, int32_t* path, int32_t* kept, int64_t* next_token,
+                    uint32_t n, uint32_t n_seq, uint32_t vocab, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The K and V rows of a path to where the cache goes on, in all layers: slot length + path[j] -> slot length + j for j < kept.
+ * Caches bf16 [layers][n_seq][s_cap][nk][128] with k_layer / v_layer elements from one layer to the next and k_seq / v_seq from
+ * one sequence to the next (multiples of 8; 16-byte aligned).  An entry below its own place, outside [0, n) or past the capacity
+ * leaves its row as it is.  lengths is not advanced. */
+int t2h_tree_keep(void* k_cache, uint64_t k_layer, uint64_t k_seq, void* v_cache, uint64_t v_layer, uint64_t v_seq,
+                  uint32_t layers, uint32_t s_cap, const int32_t* path, const int32_t* kept, const int32_t* lengths, uint32_t n,
+                  uint32_t n_seq, uint32_t nk, uint32_t d, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -135,6 +135,13 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "t2h_kv_cache_q8_dequantize": (_i32, [_vp, _u32, _vp, _u32, _u32, _u32, _vp, _vp, _vp]),
     "t2h_kv_cache_q8_evict_workspace_bytes": (_sz, [_u32] * 4),
     "t2h_kv_cache_q8_evict": (_i32, [_vp, _u32, _vp, _vp] + [_u32] * 6 + [_vp, _u32, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "t2h_attn_tree_workspace_bytes": (_sz, [_u32] * 6),
+    "t2h_attn_tree": (_i32, [_vp, _u64, _vp, _u64, _vp, _u64, _vp, _vp, _f32, _f32, _vp, _vp, _vp, _vp, _u64, _vp, _u64, _u32,
+                             _vp] + [_u32] * 5 + [_vp, _sz, _vp]),
+    "t2h_tree_verify_workspace_bytes": (_sz, [_u32] * 3 + [_i32]),
+    "t2h_tree_verify": (_i32, [_vp, _u64, _vp, _u64, _i32, _vp, _vp, _vp, _vp, _f32, _vp, _vp, _vp, _vp] + [_u32] * 3
+                        + [_vp, _sz, _vp]),
+    "t2h_tree_keep": (_i32, [_vp, _u64, _u64, _vp, _u64, _u64, _u32, _u32, _vp, _vp, _vp] + [_u32] * 4 + [_vp]),
 }
 
 

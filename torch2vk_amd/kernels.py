@@ -1952,3 +1952,274 @@ def kv_cache_q8_evict(cache: KVCacheQ8, lengths: torch.Tensor, weights: torch.Te
          n_seq, nk, 128, dest.ptrs, dest.s_cap, weights_out.data_ptr(), kept.data_ptr(), new.data_ptr(), room, nbytes,
          stream_handle())
     return kept, new
+
+
+# ------------------------------------------------- trees of drafted tokens --
+
+TREE_MAX_NODES = 64  # drafted tokens a sequence and step, the token they follow among them
+
+
+def _tree_here(at: int, needed: dict[str, torch.Tensor], **tensors: torch.Tensor | None) -> None:
+    """Everything of a call is on the current device, on whose current stream it is launched."""
+    for name, t in (needed | {name: t for name, t in tensors.items() if t is not None}).items():
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+        if t.get_device() != at:
+            raise ValueError(f"{name} is on {t.device}, the current device is cuda:{at}")
+
+
+def _tree_refuse_nodes(n_seq: int, n: int, parents: torch.Tensor | None, counts: torch.Tensor | None) -> None:
+    if n > TREE_MAX_NODES:
+        raise ValueError(f"a tree has up to {TREE_MAX_NODES} nodes, got {n}")
+    for name, t, shape in (("parents", parents, (n_seq, n)), ("counts", counts, (n_seq,))):
+        if t is not None:
+            _check(t, name, torch.int32, align=4)
+            if t.numel() != n_seq * (n if name == "parents" else 1):
+                raise ValueError(f"{name} must be int32 {shape}, got {tuple(t.shape)}")
+
+
+def _tree_cache_ok(t: torch.Tensor, dims: int, at: int) -> bool:
+    """A bf16 cache [.., s_cap, nk, 128] of ``dims`` dimensions whose last three are contiguous and whose rows are distinct."""
+    if t.dtype is not torch.bfloat16 or t.get_device() != at or t.dim() != dims:
+        return False
+    shape, stride = t.shape, t.stride()
+    row = shape[-2] * 128
+    if (shape[-1] != 128 or stride[-1] != 1 or (shape[-2] > 1 and stride[-2] != 128) or (shape[-3] > 1 and stride[-3] != row)
+            or t.data_ptr() % 16 or t.numel() == 0):
+        return False
+    least = shape[-3] * row
+    outer = sorted((stride[i], shape[i]) for i in range(dims - 3) if shape[i] > 1)  # layers in sequences, or sequences in layers
+    for step, size in outer:
+        if step < least or step % 8:
+            return False
+        least = step * size
+    return True
+
+
+def _tree_refuse_cache(dims: int, **caches: torch.Tensor) -> None:
+    form = "[layers, n_seq, s_cap, nk, 128]" if dims == 5 else "[n_seq, s_cap, nk, 128]"
+    for name, t in caches.items():
+        if t.dtype != torch.bfloat16:
+            raise TypeError(f"{name} dtype {t.dtype}, expected {torch.bfloat16}")
+        if t.dim() != dims or t.shape[-1] != 128 or t.numel() == 0:
+            raise ValueError(f"{name} must be bf16 {form}, got {tuple(t.shape)}")
+        if not _tree_cache_ok(t, dims, t.get_device()):
+            raise ValueError(f"{name} must hold contiguous sequences [s_cap, nk, 128] at distinct, 16-byte aligned places")
+    k, v = caches.values()
+    if k.shape != v.shape:
+        raise ValueError(f"k_cache and v_cache must have the same shape, got {tuple(k.shape)} and {tuple(v.shape)}")
+
+
+def attn_tree_workspace(n_seq: int, n: int, nh: int, nk: int, d: int, s_cap: int, device) -> torch.Tensor:
+    """Zeroed workspace of :func:`attn_tree` for such calls; calls leave it reusable, and calls that share one must not overlap
+    in time."""
+    nbytes = int(_lib.lib().t2h_attn_tree_workspace_bytes(n_seq, n, nh, nk, d, s_cap))
+    if nbytes == 0:
+        raise ValueError(f"unsupported tree attention shape n_seq={n_seq} n={n} nh={nh} nk={nk} d={d} s_cap={s_cap}")
+    return torch.zeros(nbytes, dtype=torch.uint8, device=device)
+
+
+def attn_tree(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+              out: torch.Tensor, lengths: torch.Tensor, workspace: torch.Tensor, *, theta: float,
+              parents: torch.Tensor | None = None, counts: torch.Tensor | None = None,
+              q_norm_weight: torch.Tensor | None = None, k_norm_weight: torch.Tensor | None = None,
+              eps: float = RMS_EPS) -> torch.Tensor:
+    """:func:`attn_decode` for a tree of drafted tokens of each sequence: q fp32 [n_seq * n, nh * 128], k_new / v_new fp32
+    [n_seq * n, nk * 128] (row strides are free) are the rows of n nodes a sequence.  q and k are normalised and rotated for
+    position length + the number of the node's ancestors (``theta`` 0: not rotated), node i's k and v go to slot length + i of
+    the bf16 caches [n_seq, s_cap, nk, 128], and each node attends to the ``lengths`` cached tokens, its ancestors and itself;
+    out bf16 [n_seq, n, nh, 128].  ``parents`` int32 [n_seq, n]: the earlier node that a node hangs on, -1 for the cached
+    tokens (None: a chain).  ``counts``: nodes of each sequence, its first rows (all n when None); rows that are no nodes, or
+    have no slot, give zeros and write nothing.  ``lengths`` is not advanced."""
+    try:
+        at = torch._C._cuda_getDevice()
+        n_seq, s_cap, nk, _ = k_cache.shape
+        rows, width = q.shape
+        qr, kr, vr = _q8_columns(q, rows, width, at), _q8_columns(k_new, rows, nk * 128, at), _q8_columns(v_new, rows, nk * 128, at)
+        ok = (_tree_cache_ok(k_cache, 4, at) and _tree_cache_ok(v_cache, 4, at) and v_cache.shape == k_cache.shape
+              and qr and kr and vr and width % 128 == 0 and rows % n_seq == 0 and rows <= n_seq * TREE_MAX_NODES
+              and _q8_plain(out, torch.bfloat16, rows * width, at) and out is not None and out.data_ptr() % 16 == 0
+              and lengths is not None and _q8_plain(lengths, torch.int32, n_seq, at)
+              and _q8_plain(parents, torch.int32, rows, at) and _q8_plain(counts, torch.int32, n_seq, at)
+              and workspace.dtype is torch.uint8 and workspace.get_device() == at and workspace.is_contiguous()
+              and _q8_plain(q_norm_weight, torch.float32, 128, at) and _q8_plain(k_norm_weight, torch.float32, 128, at)
+              and (q_norm_weight is None) == (k_norm_weight is None))
+    except (AttributeError, ValueError, IndexError):
+        ok = False
+    if not ok:  # named here
+        at = torch.cuda.current_device()
+        _tree_here(at, dict(q=q, k_new=k_new, v_new=v_new, k_cache=k_cache, v_cache=v_cache, output=out, lengths=lengths,
+                            workspace=workspace), parents=parents, counts=counts, q_norm_weight=q_norm_weight,
+                   k_norm_weight=k_norm_weight)
+        _tree_refuse_cache(4, k_cache=k_cache, v_cache=v_cache)
+        n_seq, nk = int(k_cache.shape[0]), int(k_cache.shape[2])
+        rows = int(q.shape[0]) if q.dim() else 0
+        if rows % n_seq:
+            raise ValueError(f"{rows} rows do not split into {n_seq} sequences")
+        for t, name in ((q, "q"), (k_new, "k_new"), (v_new, "v_new")):
+            _check_strided(t, name, torch.float32)
+            if t.dim() != 2 or t.shape[0] != rows or t.shape[1] % 128:
+                raise ValueError(f"{name} must be fp32 [{rows}, heads * 128], got {tuple(t.shape)}")
+            if rows > 1 and t.stride(0) < t.shape[1]:
+                raise ValueError(f"{name} must hold distinct rows")
+        if k_new.shape[1] != nk * 128 or v_new.shape[1] != nk * 128:
+            raise ValueError(f"k_new and v_new must have the cache's {nk} heads")
+        _tree_refuse_nodes(n_seq, rows // n_seq, parents, counts)
+        _check(out, "output", torch.bfloat16)
+        if out.numel() != q.numel():
+            raise ValueError(f"output must hold [{n_seq}, {rows // n_seq}, {q.shape[1] // 128}, 128]")
+        _check(lengths, "lengths", torch.int32, align=4)
+        if lengths.numel() != n_seq:
+            raise ValueError(f"lengths must have one entry for each of {n_seq} sequences, got {tuple(lengths.shape)}")
+        _check(workspace, "workspace", torch.uint8)
+        if (q_norm_weight is None) != (k_norm_weight is None):
+            raise ValueError("pass both q and k norm weights or neither")
+        for t, name in ((q_norm_weight, "q_norm_weight"), (k_norm_weight, "k_norm_weight")):
+            if t is not None:
+                _check(t, name, torch.float32, align=4)
+                if t.numel() != 128:
+                    raise ValueError(f"{name} must have 128 elements")
+        raise ValueError("unsupported tensors for tree attention")
+    _q8_heads(width // 128, nk)
+    if rows == 0:
+        return out
+    call("t2h_attn_tree", q.data_ptr(), qr, k_new.data_ptr(), kr, v_new.data_ptr(), vr, ptr(q_norm_weight), ptr(k_norm_weight),
+         eps, theta, lengths.data_ptr(), ptr(parents), ptr(counts), k_cache.data_ptr(), k_cache.stride(0), v_cache.data_ptr(),
+         v_cache.stride(0), s_cap, out.data_ptr(), rows // n_seq, n_seq, width // 128, nk, 128, workspace.data_ptr(),
+         workspace.numel(), stream_handle())
+    return out
+
+
+def tree_verify_workspace(n_seq: int, n: int, vocab: int, device, *, drawn: bool = False) -> torch.Tensor:
+    """Zeroed workspace of :func:`tree_verify` for such calls (``drawn``: with draft logits); calls leave it reusable, and calls
+    that share one must not overlap in time."""
+    nbytes = int(_lib.lib().t2h_tree_verify_workspace_bytes(n_seq, n, vocab, int(drawn)))
+    if nbytes == 0:
+        raise ValueError(f"unsupported verification shape n_seq={n_seq} n={n} vocab={vocab}")
+    return torch.zeros(nbytes, dtype=torch.uint8, device=device)
+
+
+def _logit_rows(t: torch.Tensor, n_seq: int, n: int, vocab: int, dtype: torch.dtype, at: int) -> int:
+    """The row stride of logits [n_seq, n, vocab] on device ``at`` whose n_seq * n distinct rows are evenly spaced, or 0."""
+    if t.dtype is dtype and t.get_device() == at and t.shape == (n_seq, n, vocab):
+        seq, row, one = t.stride()
+        if n == 1:
+            row = seq if n_seq > 1 else vocab
+        if (one == 1 or vocab == 1) and row >= vocab and (n_seq == 1 or seq == n * row):
+            return row
+        if n == 0:
+            return vocab
+    return 0
+
+
+def tree_verify(logits: torch.Tensor, tokens: torch.Tensor, workspace: torch.Tensor, *,
+                temperature: float | torch.Tensor = 0.0, uniforms: torch.Tensor | None = None,
+                parents: torch.Tensor | None = None, counts: torch.Tensor | None = None,
+                draft_logits: torch.Tensor | None = None, path: torch.Tensor | None = None, kept: torch.Tensor | None = None,
+                next_token: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Which drafted tokens the target's probabilities accept, and the token that follows them (include/t2h.h, "trees of drafted
+    tokens"): ``logits`` fp32 or bf16 [n_seq, n, vocab] (a free row stride), the target's after each node; ``tokens`` int64
+    [n_seq, n], the nodes', of which the first stands already.  ``temperature`` 0 is greedy; a tensor fp32 [n_seq] has one for
+    each sequence.  ``uniforms`` fp32 [n_seq, n] in [0, 1): one for each drafted token, the first for the token that follows.
+    With n = 1 this samples a token.  ``draft_logits`` [n_seq, n - 1, vocab] of the type of ``logits``: a chain whose token
+    i + 1 was drawn from row i at the same temperature.  Returns path int32 [n_seq, n] (the accepted nodes, the first node
+    among them, then -1), kept int32 [n_seq] (how many) and next_token int64 [n_seq]."""
+    try:
+        at = torch._C._cuda_getDevice()
+        n_seq, n, vocab = logits.shape
+        dtype = logits.dtype
+        row = _logit_rows(logits, n_seq, n, vocab, dtype, at)
+        draft_row = 0 if draft_logits is None else _logit_rows(draft_logits, n_seq, n - 1, vocab, dtype, at)
+        by_seq = isinstance(temperature, torch.Tensor)
+        ok = (row and dtype in _OUT_DTYPES and 0 < n <= TREE_MAX_NODES and n_seq > 0 and vocab > 0
+              and (draft_logits is None or draft_row and parents is None)
+              and tokens.dtype is torch.int64 and tokens.shape == (n_seq, n) and tokens.get_device() == at and tokens.is_contiguous()
+              and workspace.dtype is torch.uint8 and workspace.get_device() == at and workspace.is_contiguous()
+              and (_q8_plain(temperature, torch.float32, n_seq, at) if by_seq else 0.0 <= temperature < float("inf"))
+              and (uniforms is not None and _q8_plain(uniforms, torch.float32, n_seq * n, at)
+                   or uniforms is None and not by_seq and temperature == 0)
+              and _q8_plain(parents, torch.int32, n_seq * n, at) and _q8_plain(counts, torch.int32, n_seq, at)
+              and _q8_plain(path, torch.int32, n_seq * n, at) and _q8_plain(kept, torch.int32, n_seq, at)
+              and _q8_plain(next_token, torch.int64, n_seq, at))
+    except (AttributeError, ValueError, TypeError, IndexError):
+        ok = False
+    if not ok:  # named here
+        at = torch.cuda.current_device()
+        _tree_here(at, dict(logits=logits, tokens=tokens, workspace=workspace), uniforms=uniforms, parents=parents,
+                   counts=counts, draft_logits=draft_logits, path=path, kept=kept, next_token=next_token)
+        if logits.dim() != 3 or logits.numel() == 0:
+            raise ValueError(f"logits must be [n_seq, n, vocab], got {tuple(logits.shape)}")
+        n_seq, n, vocab = (int(x) for x in logits.shape)
+        _tree_refuse_nodes(n_seq, n, parents, counts)
+        if draft_logits is not None and parents is not None:
+            raise ValueError("drawn drafts are a chain: pass draft_logits or parents")
+        for t, name, m in ((logits, "logits", n), (draft_logits, "draft_logits", n - 1)):
+            if t is None:
+                continue
+            if t.dtype not in _OUT_DTYPES or t.dtype != logits.dtype:
+                raise TypeError(f"{name} dtype {t.dtype}: fp32 or bf16, one for both")
+            if not _logit_rows(t, n_seq, m, vocab, logits.dtype, at):
+                raise ValueError(f"{name} must be [{n_seq}, {m}, {vocab}] with evenly spaced rows, got {tuple(t.shape)} with "
+                                 f"strides {t.stride()}")
+        if isinstance(temperature, torch.Tensor):
+            _check(temperature, "temperature", torch.float32, align=4)
+            _tree_here(at, dict(temperature=temperature))
+            if temperature.numel() != n_seq:
+                raise ValueError(f"temperature must have one entry for each of {n_seq} sequences")
+        elif not 0.0 <= temperature < float("inf"):
+            raise ValueError(f"temperature must be finite and not negative, got {temperature}")
+        for t, name, dt, shape in ((tokens, "tokens", torch.int64, (n_seq, n)), (uniforms, "uniforms", torch.float32, (n_seq, n)),
+                                   (path, "path", torch.int32, (n_seq, n)), (kept, "kept", torch.int32, (n_seq,)),
+                                   (next_token, "next_token", torch.int64, (n_seq,))):
+            if t is None and name == "uniforms":
+                raise ValueError("sampling needs uniforms")
+            if t is not None:
+                _check(t, name, dt, align=8 if dt == torch.int64 else 4)
+                if tuple(t.shape) != shape:
+                    raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
+        _check(workspace, "workspace", torch.uint8)
+        raise ValueError("unsupported tensors for a verification")
+    if path is None:
+        path = torch.empty(n_seq, n, dtype=torch.int32, device=logits.device)
+    if kept is None:
+        kept = torch.empty(n_seq, dtype=torch.int32, device=logits.device)
+    if next_token is None:
+        next_token = torch.empty(n_seq, dtype=torch.int64, device=logits.device)
+    call("t2h_tree_verify", logits.data_ptr(), row, ptr(draft_logits) if n > 1 else None, draft_row, _OUT_DTYPES[dtype],
+         tokens.data_ptr(), ptr(parents), ptr(counts), ptr(uniforms), 0.0 if by_seq else temperature,
+         temperature.data_ptr() if by_seq else None, path.data_ptr(), kept.data_ptr(), next_token.data_ptr(), n, n_seq, vocab,
+         workspace.data_ptr(), workspace.numel(), stream_handle())
+    return path, kept, next_token
+
+
+def tree_keep(k_cache: torch.Tensor, v_cache: torch.Tensor, path: torch.Tensor, kept: torch.Tensor,
+              lengths: torch.Tensor) -> None:
+    """After :func:`tree_verify`: the K and V rows of the accepted nodes from slots length + path[j] to slots length + j, j < kept,
+    of every layer's cache, bf16 [layers, n_seq, s_cap, nk, 128] (layer and sequence strides are free).  path int32 [n_seq, n],
+    kept and ``lengths`` int32 [n_seq], as before the step; ``lengths`` is not advanced."""
+    try:
+        at = torch._C._cuda_getDevice()
+        layers, n_seq, s_cap, nk, _ = k_cache.shape
+        n = path.shape[1]
+        ok = (_tree_cache_ok(k_cache, 5, at) and _tree_cache_ok(v_cache, 5, at) and v_cache.shape == k_cache.shape
+              and path.shape == (n_seq, n) and 0 < n <= TREE_MAX_NODES and _q8_plain(path, torch.int32, n_seq * n, at)
+              and kept is not None and lengths is not None and _q8_plain(kept, torch.int32, n_seq, at)
+              and _q8_plain(lengths, torch.int32, n_seq, at))
+    except (AttributeError, ValueError, IndexError):
+        ok = False
+    if not ok:  # named here
+        at = torch.cuda.current_device()
+        _tree_here(at, dict(k_cache=k_cache, v_cache=v_cache, path=path, kept=kept, lengths=lengths))
+        _tree_refuse_cache(5, k_cache=k_cache, v_cache=v_cache)
+        n_seq = int(k_cache.shape[1])
+        _check(path, "path", torch.int32, align=4)
+        if path.dim() != 2 or path.shape[0] != n_seq or not 0 < path.shape[1] <= TREE_MAX_NODES:
+            raise ValueError(f"path must be int32 [{n_seq}, up to {TREE_MAX_NODES}], got {tuple(path.shape)}")
+        for name, t in (("kept", kept), ("lengths", lengths)):
+            _check(t, name, torch.int32, align=4)
+            if t.numel() != n_seq:
+                raise ValueError(f"{name} must have one entry for each of {n_seq} sequences, got {tuple(t.shape)}")
+        raise ValueError("unsupported tensors for a path")
+    ks, vs = k_cache.stride(), v_cache.stride()
+    call("t2h_tree_keep", k_cache.data_ptr(), ks[0], ks[1], v_cache.data_ptr(), vs[0], vs[1], layers, s_cap, path.data_ptr(),
+         kept.data_ptr(), lengths.data_ptr(), n, n_seq, nk, 128, stream_handle())
