@@ -246,6 +246,24 @@ def test_what_is_not_finite_reaches_the_rows_that_see_it(device, bad, n):
             assert c.out[hit].isnan().all()  # the norm of a row with an infinity or a NaN leaves NaN
 
 
+@pytest.mark.parametrize("length", [230, 255, 256, 480])
+def test_what_is_not_finite_in_trees_that_lie_across_units(device, length):
+    parents = [-1, 0, 0] + [(i - 1) // 2 for i in range(3, 64)]
+    clean, c = (Call(device, 1, 64, 16, 1, [length], 600, parents=parents, seed=18) for _ in range(2))
+    for node, bad in ((1, math.inf), (2, -math.inf), (40, math.nan), (63, math.inf)):
+        c.v[node, 64 + node] = bad
+    clean.run()
+    c.run()
+    for t in range(64):
+        line = lineage(parents, t)
+        for node, bad in ((1, math.inf), (2, -math.inf), (40, math.nan), (63, math.inf)):
+            got = c.out[0, t, :, 64 + node].float()
+            if node in line:
+                assert got.isnan().all() if math.isnan(bad) else (got == bad).all(), (t, node)
+                c.out[0, t, :, 64 + node] = clean.out[0, t, :, 64 + node]
+    assert torch.equal(c.out, clean.out)
+
+
 def test_an_infinity_of_each_sign_on_one_path_is_a_nan(device):
     c = Call(device, 1, 5, 8, 8, [40], 64, parents=[-1, 0, 0, 1, 2], seed=13)
     c.v[1, 5], c.v[2, 5], c.v[3, 5] = math.inf, math.inf, -math.inf

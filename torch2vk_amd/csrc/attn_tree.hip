@@ -3,12 +3,28 @@
 #include <math.h>
 
 #include "kv_q8.h"
+#include "lds_dma.h"
 #include "tree.h"
 
 namespace t2h {
 
+typedef __bf16 ta_bf16x8 __attribute__((ext_vector_type(8)));
+typedef float ta_f32x16 __attribute__((ext_vector_type(16)));
+typedef float ta_f32x4 __attribute__((ext_vector_type(4)));
+
 constexpr int TA_D = 128;
 constexpr int TA_MAX_GROUP = 16;
+constexpr int TA_ROW_BYTES = TA_D * 2;
+constexpr float TA_RESCALE = 8.0f;  // log2 headroom of the lazily updated running maximum
+
+// What a thread block of the attention works on: tiles [tile0, tile1) of a sequence's tokens.
+struct TreeUnit {
+    int seq;  // -1: none
+    int tile0, tile1;
+    int slot;        // where its part goes, -1: it is the sequence's only one
+    int len, count;  // cached tokens, nodes
+    int pad0, pad1;
+};
 
 struct TreeAttnArgs {
     const float* q;
@@ -28,114 +44,534 @@ struct TreeAttnArgs {
     size_t k_seq, v_seq;
     uint32_t s_cap, n, n_seq, nh, nk, group;
     uint16_t* out;
-    float* qs;       // [n_seq][n][nh][128] rotated queries
-    uint64_t* line;  // [n_seq][n] sets of seen nodes
+    // workspace
+    uint16_t* qh;      // [n_seq][nk][n * group][128] rotated queries, and what their rounding to bf16 left
+    uint16_t* ql;
+    uint64_t* line;    // [n_seq][n] sets of seen nodes
+    uint16_t* vt;      // [n_seq][nk][n + 1][128] the nodes' values; zeros where there is none or it is not finite
+    uint32_t* broken;  // [n_seq][nk] whether a node's value is not finite
+    uint64_t* which;   // [n_seq][nk][128][3] then: the nodes whose value in a dim is NaN, infinite, -infinite
+    TreeUnit* units;   // [n_units]
+    int2* of_seq;      // [n_seq] first part, parts
+    float* part_ml;    // [n_units * nk][rows][2] log2 maximum, sum
+    float* part_o;     // [n_units * nk][rows][128]
+    uint32_t n_units, row_tiles, rows;  // rows: of a KV head, in whole tiles
+    uint32_t slots;    // units a KV head that fill the chip
+    uint32_t keys, least;  // tokens a tile; the least tiles a unit
+    uint32_t kv_blocks, q_blocks;
 };
 
-constexpr int TP_HEADS = 4;  // heads a wave
+// ------------------------------------------------------------------------------------------ before the attention --
+//
+// One launch of three kinds of thread blocks: the units' table, the nodes' K and V rows of a (sequence, KV head), and the
+// queries.
 
-// One wave: heads TP_HEADS * part .. of a node's row, q's, then k's, then v's.
-__global__ __launch_bounds__(256) void tree_rows_kernel(const TreeAttnArgs a) {
-    const int lane = threadIdx.x & 63;
-    const uint32_t heads = a.nh + 2 * a.nk, parts = (heads + TP_HEADS - 1) / TP_HEADS;
-    const uint64_t unit = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (unit >= (uint64_t)a.n_seq * a.n * parts) return;
-    const uint32_t row = (uint32_t)(unit / parts), h0 = (uint32_t)(unit % parts) * TP_HEADS;
-    const uint32_t seq = row / a.n, i = row % a.n;
+constexpr int TP_HEADS = 4;  // q heads a wave
+
+__device__ void tree_table(const TreeAttnArgs& a) {
+    const uint32_t lane = threadIdx.x;
+    if (lane >= 64) return;
+    auto tiles_of = [&](uint32_t i, int& len, int& count) {
+        len = a.lengths[i];
+        count = tree_count_at(a.counts, i, a.n, len, a.s_cap);
+        return count > 0 ? ((uint32_t)(len + count) + a.keys - 1) / a.keys : 0u;
+    };
+    uint32_t total = 0;
+    int len, count;
+    for (uint32_t i = lane; i < a.n_seq; i += 64) total += tiles_of(i, len, count);
+    total = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan_u32(total), 63);
+    uint32_t chunk = (total + a.slots - 1) / a.slots;
+    chunk = chunk > a.least ? chunk : a.least;
+    uint32_t fulls = 0;
+    for (uint32_t i = lane; i < a.n_seq; i += 64) fulls += tiles_of(i, len, count) / chunk;
+    fulls = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan_u32(fulls), 63);
+    uint32_t full_at = 0, rest_at = fulls, part_at = 0;
+    for (uint32_t base = 0; base < a.n_seq; base += 64) {
+        const uint32_t i = base + lane;
+        uint32_t tiles = 0;
+        len = count = 0;
+        if (i < a.n_seq) tiles = tiles_of(i, len, count);
+        const uint32_t full = tiles / chunk, rest = i < a.n_seq && (tiles % chunk || tiles == 0) ? 1u : 0u;
+        const uint32_t full_up = wave_scan_u32(full), rest_up = wave_scan_u32(rest);
+        if (i < a.n_seq) {
+            const uint32_t first = part_at + full_up - full + rest_up - rest, parts = full + rest;
+            a.of_seq[i] = make_int2((int)first, (int)parts);
+            TreeUnit u;
+            u.seq = (int)i;
+            u.len = len;
+            u.count = count;
+            u.pad0 = u.pad1 = 0;
+            for (uint32_t p = 0; p < parts; ++p) {
+                u.tile0 = (int)(p * chunk);
+                u.tile1 = (int)min(p * chunk + chunk, tiles);
+                u.slot = parts == 1 ? -1 : (int)(first + p);
+                a.units[p < full ? full_at + full_up - full + p : rest_at + rest_up - rest] = u;
+            }
+        }
+        full_at += (uint32_t)__builtin_amdgcn_readlane((int)full_up, 63);
+        rest_at += (uint32_t)__builtin_amdgcn_readlane((int)rest_up, 63);
+        part_at += (uint32_t)__builtin_amdgcn_readlane((int)(full_up + rest_up), 63);
+    }
+    for (uint32_t u = rest_at + lane; u < a.n_units; u += 64) a.units[u].seq = -1;
+}
+
+__device__ __forceinline__ uint64_t readlane64(uint64_t x, int lane) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)x, lane);
+}
+
+__device__ void tree_kv_rows(const TreeAttnArgs& a, uint32_t block) {
+    __shared__ uint64_t found[4][TA_D][3];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t seq = block / a.nk, h = block % a.nk;
     const int len = a.lengths[seq];
     const int count = tree_count_at(a.counts, seq, a.n, len, a.s_cap);
     const uint64_t lines = tree_lineage(a.parents, seq, a.n, count);
-    const uint64_t line = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(lines >> 32), (int)i) << 32 |
-                          (uint32_t)__builtin_amdgcn_readlane((int)lines, (int)i);
+    const bool has_w = a.k_norm_w != nullptr;
+    const float w0 = has_w ? a.k_norm_w[lane] : 1.0f, w1 = has_w ? a.k_norm_w[lane + 64] : 1.0f;
+    const double turns = a.rope ? rope_turns(lane, a.log2_theta) : 0.0;
+    uint32_t* const vt = reinterpret_cast<uint32_t*>(a.vt + (size_t)block * (a.n + 1) * TA_D);
+    uint64_t bad[2][3] = {{0, 0, 0}, {0, 0, 0}};
+    if (wave == 3) vt[a.n * 64 + lane] = 0u;
+    for (int i = wave; i < (int)a.n; i += 4) {
+        const uint64_t line = readlane64(lines, i);
+        if (line == 0) {
+            vt[i * 64 + lane] = 0u;
+            continue;
+        }
+        const size_t row = (size_t)seq * a.n + i, slot = ((size_t)len + i) * a.nk + h;
+        const float* kx = a.k_new + row * a.k_row + (size_t)h * TA_D + lane;
+        const float* vx = a.v_new + row * a.v_row + (size_t)h * TA_D + 2 * lane;
+        const float k0 = kx[0], k1 = kx[64], v0 = vx[0], v1 = vx[1];
+        float cs = 1.0f, sn = 0.0f, r0, r1;
+        if (a.rope) rope_at(turns, len + __popcll(line) - 1, cs, sn);
+        q8_norm_rope(k0, k1, has_w, w0, w1, a.eps, cs, sn, r0, r1);
+        uint16_t* const y = a.k_cache + seq * a.k_seq + slot * TA_D + lane;
+        y[0] = (uint16_t)f32_to_bf16_bits(r0);
+        y[64] = (uint16_t)f32_to_bf16_bits(r1);
+        uint32_t v = pack_bf16x2(v0, v1);
+        reinterpret_cast<uint32_t*>(a.v_cache + seq * a.v_seq + slot * TA_D)[lane] = v;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const uint32_t x = v >> (16 * e) & 0xffffu;
+            if ((x & 0x7f80u) == 0x7f80u) {
+                bad[e][x & 0x7fu ? 0 : x >> 15 ? 2 : 1] |= 1ull << i;
+                v &= e ? 0xffffu : 0xffff0000u;
+            }
+        }
+        vt[i * 64 + lane] = v;
+    }
+    const bool any = (bad[0][0] | bad[0][1] | bad[0][2] | bad[1][0] | bad[1][1] | bad[1][2]) != 0;
+    const int all = __syncthreads_or(any);
+    if (threadIdx.x == 0) a.broken[block] = all ? 1u : 0u;
+    if (!all) return;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int k = 0; k < 3; ++k) found[wave][2 * lane + e][k] = bad[e][k];
+    __syncthreads();
+    for (int i = threadIdx.x; i < TA_D * 3; i += 256) {
+        const int d = i / 3, k = i % 3;
+        a.which[(size_t)block * TA_D * 3 + i] = found[0][d][k] | found[1][d][k] | found[2][d][k] | found[3][d][k];
+    }
+}
+
+__device__ void tree_q_rows(const TreeAttnArgs& a, uint64_t unit) {
+    const int lane = threadIdx.x & 63;
+    const uint32_t parts = (a.nh + TP_HEADS - 1) / TP_HEADS;
+    if (unit >= (uint64_t)a.n_seq * a.n * parts) return;
+    const uint32_t row = (uint32_t)(unit / parts), h0 = (uint32_t)(unit % parts) * TP_HEADS;
+    const uint32_t seq = row / a.n, i = row % a.n;
+    float x0[TP_HEADS], x1[TP_HEADS];
+#pragma unroll
+    for (int j = 0; j < TP_HEADS; ++j) {
+        const uint32_t h = h0 + j < a.nh ? h0 + j : h0;
+        const float* x = a.q + row * a.q_row + (size_t)h * TA_D;
+        x0[j] = x[lane];
+        x1[j] = x[lane + 64];
+    }
+    const int len = a.lengths[seq];
+    const int count = tree_count_at(a.counts, seq, a.n, len, a.s_cap);
+    const uint64_t line = readlane64(tree_lineage(a.parents, seq, a.n, count), (int)i);
     if (h0 == 0 && lane == 0) a.line[row] = line;
-    if (line == 0) return;
+    if (line == 0) return;  // what lies in the workspace stays: it reaches no output
     float cs = 1.0f, sn = 0.0f;
     if (a.rope) rope_at(rope_turns(lane, a.log2_theta), len + __popcll(line) - 1, cs, sn);
     const bool has_w = a.q_norm_w != nullptr;
-    for (uint32_t h = h0; h < h0 + TP_HEADS && h < heads; ++h) {
-        const size_t slot = (size_t)len + i;
-        if (h < a.nh) {
-            const float* x = a.q + row * a.q_row + (size_t)h * TA_D;
-            float r0, r1;
-            q8_norm_rope(x[lane], x[lane + 64], has_w, has_w ? a.q_norm_w[lane] : 1.0f, has_w ? a.q_norm_w[lane + 64] : 1.0f,
-                         a.eps, cs, sn, r0, r1);
-            float* y = a.qs + ((size_t)row * a.nh + h) * TA_D;
-            y[lane] = r0;
-            y[lane + 64] = r1;
-        } else if (h < a.nh + a.nk) {
-            const uint32_t kh = h - a.nh;
-            const float* x = a.k_new + row * a.k_row + (size_t)kh * TA_D;
-            float r0, r1;
-            q8_norm_rope(x[lane], x[lane + 64], has_w, has_w ? a.k_norm_w[lane] : 1.0f, has_w ? a.k_norm_w[lane + 64] : 1.0f,
-                         a.eps, cs, sn, r0, r1);
-            uint16_t* y = a.k_cache + seq * a.k_seq + (slot * a.nk + kh) * TA_D;
-            y[lane] = (uint16_t)f32_to_bf16_bits(r0);
-            y[lane + 64] = (uint16_t)f32_to_bf16_bits(r1);
-        } else {
-            const uint32_t vh = h - a.nh - a.nk;
-            const float* x = a.v_new + row * a.v_row + (size_t)vh * TA_D;
-            uint16_t* y = a.v_cache + seq * a.v_seq + (slot * a.nk + vh) * TA_D;
-            y[lane] = (uint16_t)f32_to_bf16_bits(x[lane]);
-            y[lane + 64] = (uint16_t)f32_to_bf16_bits(x[lane + 64]);
+    const float w0 = has_w ? a.q_norm_w[lane] : 1.0f, w1 = has_w ? a.q_norm_w[lane + 64] : 1.0f;
+#pragma unroll
+    for (int j = 0; j < TP_HEADS; ++j) {
+        const uint32_t h = h0 + j;
+        if (h >= a.nh) break;
+        float r[2];
+        q8_norm_rope(x0[j], x1[j], has_w, w0, w1, a.eps, cs, sn, r[0], r[1]);
+        const size_t at = (((size_t)seq * a.nk + h / a.group) * a.n * a.group + i * a.group + h % a.group) * TA_D + lane;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const uint32_t hi = f32_to_bf16_bits(r[e]);
+            a.qh[at + 64 * e] = (uint16_t)hi;
+            a.ql[at + 64 * e] = (uint16_t)f32_to_bf16_bits(r[e] - bf16_bits_to_f32(hi));
         }
     }
 }
 
-// One wave a (node, head): 64 keys at a time, a lane a key for the scores and two dims for the sum.
-__global__ __launch_bounds__(64) void tree_attn_kernel(const TreeAttnArgs a) {
-    __shared__ float qs[TA_D];
-    const int lane = threadIdx.x;
-    const uint32_t h = blockIdx.x % a.nh, row = blockIdx.x / a.nh, seq = row / a.n;
-    uint32_t* const out = reinterpret_cast<uint32_t*>(a.out + ((size_t)row * a.nh + h) * TA_D);
-    const uint64_t line = a.line[row];
-    if (line == 0) {
+__global__ __launch_bounds__(256) void tree_rows_kernel(const TreeAttnArgs a) {
+    if (blockIdx.x == 0) return tree_table(a);
+    if (blockIdx.x <= a.kv_blocks) return tree_kv_rows(a, blockIdx.x - 1);
+    tree_q_rows(a, (uint64_t)(blockIdx.x - 1 - a.kv_blocks) * 4 + (threadIdx.x >> 6));
+}
+
+// ----------------------------------------------------------------------------------------------- the attention --
+//
+// A thread block takes a unit's tiles of one KV head and the rows (node, q head) of that head, NWR waves of 32 rows by NWK waves
+// of 32 keys.  Tiles go straight from the cache into LDS, STAGES of them in turn.
+//   * S^T = K . Q^T on v_mfma_f32_32x32x16_bf16, q in two bf16 terms: a lane then holds 16 scores of one row, and their
+//     weights, packed to bf16, are the B operand of
+//   * O^T += V^T . P^T, whose A operand the transposing LDS read hands out.
+// 16-byte pieces of a row lie in LDS at their place XOR f(row), so that neither product's reads meet in a bank: f is the
+// row's low four bits for keys (16 rows, one piece each) and twice two of them for values (4 rows, 4 pieces each).
+
+template <int NWR, int NWK, int STAGES>
+struct TreeShape {
+    static constexpr int WAVES = NWR * NWK, KEYS = 32 * NWK, PER = 16 / NWR;  // loads of 1 KiB a wave and tile
+    static constexpr int STAGE = KEYS * 2 * TA_ROW_BYTES;
+    static constexpr int OROW = TA_D + 4;  // fp32 row of the join, padded
+    static constexpr int JOIN = WAVES * 32 * OROW * 4;
+    static constexpr int LDS = STAGES * STAGE > JOIN ? STAGES * STAGE : JOIN;
+};
+
+template <int NWR, int NWK, int STAGES>
+__global__ __launch_bounds__(NWR * NWK * 64) __attribute__((amdgpu_waves_per_eu(1, NWR * NWK / 4)))
+void tree_attn_kernel(const TreeAttnArgs a) {
+    using S = TreeShape<NWR, NWK, STAGES>;
+    constexpr bool OWN = NWR == 1;  // a wave reads only what it has loaded itself
+    __shared__ __align__(1024) uint8_t lds[S::LDS];
+    __shared__ float wml[S::WAVES][32][2];
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave % NWR, wk = wave / NWR;
+    // the row tiles of a unit one after another on one of the 8 XCDs
+    uint32_t rt = 0, uh = blockIdx.x;
+    if (a.row_tiles > 1) {
+        const uint32_t per = a.n_units * a.nk;
+        if (per % 8 == 0) {
+            const uint32_t j = blockIdx.x / 8;
+            rt = j % a.row_tiles;
+            uh = j / a.row_tiles * 8 + blockIdx.x % 8;
+        } else {
+            rt = blockIdx.x / per;
+            uh = blockIdx.x % per;
+        }
+    }
+    const uint32_t unit = uh / a.nk, h = uh % a.nk;
+    const TreeUnit u = a.units[unit];
+    if (u.seq < 0) return;
+    const int group = (int)a.group, len = u.len, rows = u.count * group;  // the sequence's rows of this head
+    const int r0 = (int)rt * NWR * 32;
+    const size_t head = (size_t)u.seq * a.nk + h;
+    const int tiles = rows > r0 ? u.tile1 - u.tile0 : 0;
+    const uint16_t* const kb = a.k_cache + u.seq * a.k_seq + (size_t)h * TA_D;
+    const uint16_t* const vb = a.v_cache + u.seq * a.v_seq + (size_t)h * TA_D;
+    const uint16_t* const vt = a.vt + head * (a.n + 1) * TA_D;
+    const size_t step = (size_t)a.nk * TA_D;  // elements from a token to the next
+
+    // loads of this wave: pieces of rows 4 q + lane / 16, q = q0 ..
+    const uint32_t base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)&lds[0]);
+    constexpr int HALF = S::PER / 2;
+    const int q0 = wave * HALF;
+    const int lr = lane >> 4, lp = lane & 15;
+    const int kcol = 8 * (lp ^ lr), vcol = 8 * (lp ^ (lr << 2));  // a key's piece also goes by the row's next two bits: 4 (q % 4)
+    auto load = [&](int it) {
+        const int t0 = (u.tile0 + it) * S::KEYS;
+        const uint32_t at = base + (uint32_t)(it % STAGES) * S::STAGE;
+        if (t0 + S::KEYS <= len) {
+            const uint16_t* const kp = kb + (size_t)(t0 + lr) * step;
+            const uint16_t* const vp = vb + (size_t)(t0 + lr) * step + vcol;
+#pragma unroll
+            for (int i = 0; i < HALF; ++i) {
+                const int q = q0 + i;
+                lds_dma16(kp + (size_t)(4 * q) * step + (kcol ^ (32 * (q & 3))), at + q * 1024);
+            }
+#pragma unroll
+            for (int i = 0; i < HALF; ++i) {
+                const int q = q0 + i;
+                lds_dma16(vp + (size_t)(4 * q) * step, at + S::KEYS * TA_ROW_BYTES + q * 1024);
+            }
+        } else {
+            // the tile of the last cached tokens or of nodes: their values come from the copy without what is not finite, and what
+            // lies behind them is its row of zeros (keys there: any row of the cache, the scores are masked)
+#pragma unroll
+            for (int i = 0; i < HALF; ++i) {
+                const int q = q0 + i, t = min(t0 + 4 * q + lr, (int)a.s_cap - 1);
+                lds_dma16(kb + (size_t)t * step + (kcol ^ (32 * (q & 3))), at + q * 1024);
+            }
+#pragma unroll
+            for (int i = 0; i < HALF; ++i) {
+                const int q = q0 + i, t = t0 + 4 * q + lr;
+                const uint16_t* const p = t < len ? vb + (size_t)t * step : vt + (size_t)min(t - len, (int)a.n) * TA_D;
+                lds_dma16(p + vcol, at + S::KEYS * TA_ROW_BYTES + q * 1024);
+            }
+        }
+    };
+
+    ta_f32x16 o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[i][e] = 0.0f;
+    float m_run = -INFINITY, l_part = 0.0f;
+    const int row = r0 + 32 * wr + (lane & 31);  // this lane's
+    const bool busy = r0 + 32 * wr < rows;       // whether this wave has any
+    if (tiles > 0) {
+        load(0);
+        const int qr = row < rows ? row : rows - 1;
+        const uint16_t* const qhp = a.qh + (head * a.n * group + qr) * TA_D + 8 * half;
+        const uint16_t* const qlp = a.ql + (head * a.n * group + qr) * TA_D + 8 * half;
+        ta_bf16x8 qh[8], ql[8];
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+            qh[s] = *reinterpret_cast<const ta_bf16x8*>(qhp + 16 * s);
+            ql[s] = *reinterpret_cast<const ta_bf16x8*>(qlp + 16 * s);
+        }
+        const uint64_t line = a.line[(size_t)u.seq * a.n + qr / group];
+        // (the compiler does not count the loads into LDS: everything that it counts has landed before the loop)
+        wait_vm<0>();
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int i = 1; i < STAGES - 1; ++i)
+            if (i < tiles) load(i);
+
+        // where this lane reads: a key's row and pieces, a value's 8 bytes in 4 rows (and 8 rows on)
+        const int krow = 32 * wk + (lane & 31), n16 = lane & 15;
+        const uint32_t ka = (uint32_t)krow * TA_ROW_BYTES;
+        const int vr = 32 * wk + 4 * half + (n16 >> 2), vpiece = 2 * ((lane >> 4) & 1) + ((n16 & 3) >> 1);
+        const uint32_t va = S::KEYS * TA_ROW_BYTES + (uint32_t)vr * TA_ROW_BYTES + 8 * (n16 & 1);
+        for (int it = 0; it < tiles; ++it) {
+            if constexpr (OWN) {
+                if (it + 1 < tiles) {
+                    load(it + 1);
+                    wait_vm<S::PER>();
+                } else {
+                    wait_vm<0>();
+                }
+                asm volatile("" ::: "memory");
+            } else {
+                const int left = tiles - 1 - it;
+                if (left >= STAGES - 2) wait_vm<S::PER * (STAGES - 2)>();
+                else wait_vm<0>();
+                wait_lgkm0();
+                wave_barrier();
+                if (it + STAGES - 1 < tiles) load(it + STAGES - 1);
+            }
+            if (busy) {
+                const uint8_t* const stage = &lds[(it % STAGES) * S::STAGE];
+                ta_f32x16 s;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[e] = 0.0f;
+#pragma unroll
+                for (int st = 0; st < 8; ++st) {
+                    const ta_bf16x8 kf =
+                        *reinterpret_cast<const ta_bf16x8*>(stage + ka + (((2 * st + half) ^ (krow & 15)) << 4));
+                    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qh[st], s, 0, 0, 0);
+                    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, ql[st], s, 0, 0, 0);
+                }
+                const int t0 = (u.tile0 + it) * S::KEYS + 32 * wk;
+                if (t0 + 32 > len) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int j = t0 + 8 * (e >> 2) + 4 * half + (e & 3) - len;
+                        const bool seen = j < 0 || (j < TREE_MAX && (line >> (j & 63) & 1));
+                        s[e] = seen ? s[e] : -INFINITY;
+                    }
+                }
+                float mt = -INFINITY;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[e]);
+                mt = xor_max<32>(mt * a.scale_log2);
+                const bool grow = mt > m_run + TA_RESCALE;
+                const float m_new = grow ? mt : m_run;
+                const float alpha = grow ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
+                const float msub = m_new == -INFINITY ? 0.0f : m_new;
+                m_run = m_new;
+                uint32_t pk[8];
+                float lsum = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 16; e += 2) {
+                    const float p0 = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2, -msub));
+                    const float p1 = __builtin_amdgcn_exp2f(fmaf(s[e + 1], a.scale_log2, -msub));
+                    lsum += p0 + p1;
+                    pk[e / 2] = pack_bf16x2(p0, p1);
+                }
+                l_part = fmaf(l_part, alpha, lsum);
+                if (__builtin_amdgcn_ballot_w64(grow) != 0) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[i][e] *= alpha;
+                }
+#pragma unroll
+                for (int stp = 0; stp < 2; ++stp) {
+                    const ta_bf16x8 pf = __builtin_bit_cast(
+                        ta_bf16x8, make_uint4(pk[4 * stp], pk[4 * stp + 1], pk[4 * stp + 2], pk[4 * stp + 3]));
+                    const uint8_t* const v = stage + va + 16 * stp * TA_ROW_BYTES;
+#pragma unroll
+                    for (int db = 0; db < 4; ++db) {
+                        const uint32_t at = (uint32_t)((4 * db + vpiece) ^ ((vr & 3) << 2)) << 4;
+                        const uint2 x = lds_read_tr16_b64(reinterpret_cast<const uint16_t*>(v + at));
+                        const uint2 y = lds_read_tr16_b64(reinterpret_cast<const uint16_t*>(v + at + 8 * TA_ROW_BYTES));
+                        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                            __builtin_bit_cast(ta_bf16x8, make_uint4(x.x, x.y, y.x, y.y)), pf, o[db], 0, 0, 0);
+                    }
+                }
+            }
+            if constexpr (OWN) {  // the buffer is read before it is loaded again
+                wait_lgkm0();
+                asm volatile("" ::: "memory");
+            }
+        }
+    }
+
+    // join the waves of the same rows
+    const float l = xor_sum<32>(l_part);
+    wait_lgkm0();
+    __syncthreads();
+    float* const os = reinterpret_cast<float*>(lds);
+    if (half == 0) {
+        wml[wave][lane][0] = m_run;
+        wml[wave][lane][1] = l;
+    }
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<ta_f32x4*>(os + (wave * 32 + (lane & 31)) * S::OROW + 32 * db + 8 * g + 4 * half) =
+                ta_f32x4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
+    __syncthreads();
+    const bool whole = u.slot < 0;
+    // values that are not finite were zeros in the products; they come to the rows that see them here, in the nodes' own unit
+    const int node0 = max(u.tile0 * S::KEYS - len, 0), node1 = min(u.tile1 * S::KEYS - len, TREE_MAX);
+    const bool broken = a.broken[head] != 0 && node1 > node0;
+    const uint64_t here = broken ? (~0ull >> (TREE_MAX - (node1 - node0))) << node0 : 0;
+    const int all = (int)a.n * group;  // rows of the output, nodes or not
+    for (int i = tid; i < NWR * 32 * 32; i += S::WAVES * 64) {
+        const int r = i >> 5, d = (i & 31) * 4, at = r0 + r;
+        if (at >= (whole ? all : rows)) break;
+        float M = -INFINITY, L = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NWK; ++w) M = fmaxf(M, wml[w * NWR + (r >> 5)][r & 31][0]);
+        const float msub = M == -INFINITY ? 0.0f : M;
+        ta_f32x4 sum = ta_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < NWK; ++w) {
+            const int from = w * NWR + (r >> 5);
+            const float f = __builtin_amdgcn_exp2f(wml[from][r & 31][0] - msub);
+            L = fmaf(f, wml[from][r & 31][1], L);
+            sum += *reinterpret_cast<const ta_f32x4*>(os + (from * 32 + (r & 31)) * S::OROW + d) * f;
+        }
+        const int node = at / group;
+        const uint64_t line = a.line[(size_t)u.seq * a.n + node];
+        if (broken) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint64_t* const w = a.which + (head * TA_D + d + e) * 3;
+                if (line & here & w[0]) sum[e] += __uint_as_float(0x7fc00000u);
+                if (line & here & w[1]) sum[e] += INFINITY;
+                if (line & here & w[2]) sum[e] -= INFINITY;
+            }
+        }
+        if (whole) {
+            const float inv = line ? 1.0f / L : 0.0f;
+            uint2 y = make_uint2(0u, 0u);
+            if (line) y = make_uint2(pack_bf16x2(sum[0] * inv, sum[1] * inv), pack_bf16x2(sum[2] * inv, sum[3] * inv));
+            *reinterpret_cast<uint2*>(a.out + (((size_t)u.seq * a.n + node) * a.nh + h * group + at % group) * TA_D + d) = y;
+        } else {
+            const size_t part = ((size_t)u.slot * a.nk + h) * a.rows + at;
+            *reinterpret_cast<ta_f32x4*>(a.part_o + part * TA_D + d) = sum;
+            if (d == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * part) = make_float2(M, L);
+        }
+    }
+}
+
+// Joins the units of a sequence, a wave a row.
+constexpr int TJ_BATCH = 8;
+
+__global__ __launch_bounds__(256) void tree_join_kernel(const TreeAttnArgs a) {
+    const int lane = threadIdx.x & 63;
+    const uint32_t unit = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (unit >= a.n_seq * a.n * a.nh) return;
+    const uint32_t seq = unit / (a.n * a.nh), i = unit / a.nh % a.n, head = unit % a.nh, h = head / a.group;
+    const int2 parts = a.of_seq[seq];
+    if (parts.y <= 1) return;
+    uint32_t* const out = reinterpret_cast<uint32_t*>(a.out + ((size_t)unit) * TA_D);
+    if (a.line[(size_t)seq * a.n + i] == 0) {
         out[lane] = 0u;
         return;
     }
-    const float* q = a.qs + ((size_t)row * a.nh + h) * TA_D;
-    qs[lane] = q[lane];
-    qs[lane + 64] = q[lane + 64];
-    __syncthreads();
-    const int len = a.lengths[seq], end = len + 64 - __builtin_clzll(line);
-    const uint16_t* const kb = a.k_cache + seq * a.k_seq + (size_t)(h / a.group) * TA_D;
-    const uint16_t* const vb = a.v_cache + seq * a.v_seq + (size_t)(h / a.group) * TA_D;
-    float m = -INFINITY, l = 0.0f, o0 = 0.0f, o1 = 0.0f;
-    for (int t0 = 0; t0 < end; t0 += 64) {
-        const int t = t0 + lane;
-        const bool seen = t < len || (t < end && (line >> (t - len) & 1));
-        float s = -INFINITY;
-        if (seen) {
-            const uint4* k = reinterpret_cast<const uint4*>(kb + (size_t)t * a.nk * TA_D);
-            s = 0.0f;
-            for (int c = 0; c < TA_D / 8; ++c) {
-                const uint4 w = k[c];
-                const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+    const size_t r = (size_t)i * a.group + head % a.group;
+    float M = -INFINITY, L = 0.0f, o0 = 0.0f, o1 = 0.0f;
+    for (int p0 = 0; p0 < parts.y; p0 += TJ_BATCH) {
+        float2 ml[TJ_BATCH], x[TJ_BATCH];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    s = fmaf(qs[8 * c + 2 * j], __uint_as_float(x[j] << 16), s);
-                    s = fmaf(qs[8 * c + 2 * j + 1], __uint_as_float(x[j] & 0xffff0000u), s);
-                }
-            }
-            s *= a.scale_log2;
+        for (int p = 0; p < TJ_BATCH; ++p) {
+            const size_t at = ((size_t)(parts.x + min(p0 + p, parts.y - 1)) * a.nk + h) * a.rows + r;
+            ml[p] = *reinterpret_cast<const float2*>(a.part_ml + 2 * at);
+            x[p] = *reinterpret_cast<const float2*>(a.part_o + at * TA_D + 2 * lane);
         }
-        const float now = fmaxf(m, wave_max(s)), base = now == -INFINITY ? 0.0f : now;
-        const float keep = __builtin_amdgcn_exp2f(m - base);
-        const float p = seen ? __builtin_amdgcn_exp2f(s - base) : 0.0f;
-        m = now;
-        l = fmaf(l, keep, wave_sum(p));
-        o0 *= keep;
-        o1 *= keep;
-        uint64_t todo = __ballot(seen);
-        while (todo) {
-            const int j = __builtin_ctzll(todo);
-            todo &= todo - 1;
-            const float pj = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(p), j));
-            const uint32_t v = reinterpret_cast<const uint32_t*>(vb + (size_t)(t0 + j) * a.nk * TA_D)[lane];
-            o0 = fmaf(pj, __uint_as_float(v << 16), o0);
-            o1 = fmaf(pj, __uint_as_float(v & 0xffff0000u), o1);
+#pragma unroll
+        for (int p = 0; p < TJ_BATCH; ++p) {
+            if (p0 + p >= parts.y) break;
+            const float now = fmaxf(M, ml[p].x), msub = now == -INFINITY ? 0.0f : now;
+            const float keep = __builtin_amdgcn_exp2f(M - msub), f = __builtin_amdgcn_exp2f(ml[p].x - msub);
+            L = fmaf(L, keep, f * ml[p].y);
+            o0 = fmaf(o0, keep, x[p].x * f);
+            o1 = fmaf(o1, keep, x[p].y * f);
+            M = now;
         }
     }
-    out[lane] = pack_bf16x2(o0 / l, o1 / l);
+    out[lane] = pack_bf16x2(o0 / L, o1 / L);
+}
+
+// ------------------------------------------------------------------------------------------------------ launch --
+
+// Rows of a KV head that one thread block takes: 32, 64, 128 or 256, for more of them several.
+static uint32_t ta_tile_rows(uint32_t rows) { return rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256; }
+
+struct TreeSizes {
+    uint32_t tile_rows, row_tiles, rows, keys, least, slots, units;
+    size_t qh, ql, line, vt, broken, which, table, of_seq, part_ml, part_o, end;
+};
+
+constexpr uint32_t TA_CUS = 256;
+
+static TreeSizes ta_sizes(uint32_t n_seq, uint32_t n, uint32_t nh, uint32_t nk, uint32_t s_cap) {
+    TreeSizes s;
+    const uint32_t rows = n * (nh / nk);
+    s.tile_rows = ta_tile_rows(rows);
+    s.row_tiles = (rows + s.tile_rows - 1) / s.tile_rows;
+    s.rows = s.row_tiles * s.tile_rows;
+    s.keys = s.tile_rows <= 64 ? 128 : s.tile_rows == 128 ? 64 : 32;
+    s.least = s.tile_rows <= 64 ? 1 : s.tile_rows == 128 ? 4 : 8;
+    s.slots = TA_CUS / (nk * s.row_tiles) > 1 ? TA_CUS / (nk * s.row_tiles) : 1;
+    const uint64_t most = (uint64_t)n_seq * ((s_cap + s.keys - 1) / s.keys), some = (uint64_t)s.slots + n_seq;
+    s.units = (uint32_t)(most < some ? most : some);
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += (bytes + 255) / 256 * 256;
+        return here;
+    };
+    const size_t q = (size_t)n_seq * n * nh * TA_D * 2, heads = (size_t)n_seq * nk, parts = (size_t)s.units * nk * s.rows;
+    s.qh = take(q);
+    s.ql = take(q);
+    s.line = take((size_t)n_seq * n * 8);
+    s.vt = take(heads * (n + 1) * TA_D * 2);
+    s.broken = take(heads * 4);
+    s.which = take(heads * TA_D * 24);
+    s.table = take((size_t)s.units * sizeof(TreeUnit));
+    s.of_seq = take((size_t)n_seq * 8);
+    s.part_ml = take(parts * 8);
+    s.part_o = take(parts * TA_D * 4);
+    s.end = at;
+    return s;
 }
 
 }  // namespace t2h
@@ -149,7 +585,7 @@ static bool ta_shape(uint32_t n_seq, uint32_t n, uint32_t nh, uint32_t nk, uint3
 extern "C" size_t t2h_attn_tree_workspace_bytes(uint32_t n_seq, uint32_t n, uint32_t nh, uint32_t nk, uint32_t d,
                                                 uint32_t s_cap) {
     if (!ta_shape(n_seq, n, nh, nk, s_cap) || n == 0 || nh / nk > TA_MAX_GROUP || d != TA_D) return 0;
-    return (size_t)n_seq * n * (8 + (size_t)nh * TA_D * 4);
+    return ta_sizes(n_seq, n, nh, nk, s_cap).end;
 }
 
 extern "C" int t2h_attn_tree(const float* q, uint64_t q_row, const float* k_new, uint64_t k_row, const float* v_new,
@@ -170,7 +606,8 @@ extern "C" int t2h_attn_tree(const float* q, uint64_t q_row, const float* k_new,
          reinterpret_cast<uintptr_t>(workspace) | (n_seq > 1 ? (k_seq | v_seq) * 2 : 0)) & 15)
         return T2H_ERR_ALIGN;
     if (n == 0) return T2H_OK;
-    if (workspace_bytes < t2h_attn_tree_workspace_bytes(n_seq, n, nh, nk, d, s_cap)) return T2H_ERR_WORKSPACE;
+    const TreeSizes s = ta_sizes(n_seq, n, nh, nk, s_cap);
+    if (workspace_bytes < s.end) return T2H_ERR_WORKSPACE;
     TreeAttnArgs a;
     a.q = q;
     a.k_new = k_new;
@@ -198,15 +635,40 @@ extern "C" int t2h_attn_tree(const float* q, uint64_t q_row, const float* k_new,
     a.nk = nk;
     a.group = nh / nk;
     a.out = reinterpret_cast<uint16_t*>(out);
-    const uint64_t rows = (uint64_t)n_seq * n;
-    a.qs = reinterpret_cast<float*>(workspace);
-    a.line = reinterpret_cast<uint64_t*>(a.qs + rows * nh * TA_D);
-    const uint64_t waves = rows * ((nh + 2 * nk + TP_HEADS - 1) / TP_HEADS);
-    if (waves > 0x7fffffffu || rows * nh > 0x7fffffffu) return T2H_ERR_SHAPE;
+    uint8_t* const ws = reinterpret_cast<uint8_t*>(workspace);
+    a.qh = reinterpret_cast<uint16_t*>(ws + s.qh);
+    a.ql = reinterpret_cast<uint16_t*>(ws + s.ql);
+    a.line = reinterpret_cast<uint64_t*>(ws + s.line);
+    a.vt = reinterpret_cast<uint16_t*>(ws + s.vt);
+    a.broken = reinterpret_cast<uint32_t*>(ws + s.broken);
+    a.which = reinterpret_cast<uint64_t*>(ws + s.which);
+    a.units = reinterpret_cast<TreeUnit*>(ws + s.table);
+    a.of_seq = reinterpret_cast<int2*>(ws + s.of_seq);
+    a.part_ml = reinterpret_cast<float*>(ws + s.part_ml);
+    a.part_o = reinterpret_cast<float*>(ws + s.part_o);
+    a.n_units = s.units;
+    a.row_tiles = s.row_tiles;
+    a.rows = s.rows;
+    a.slots = s.slots;
+    a.keys = s.keys;
+    a.least = s.least;
+    const uint64_t waves = (uint64_t)n_seq * n * ((nh + TP_HEADS - 1) / TP_HEADS), kv = (uint64_t)n_seq * nk;
+    const uint64_t grid = (uint64_t)s.units * nk * s.row_tiles, joins = ((uint64_t)n_seq * n * nh + 3) / 4;
+    if (kv + waves > 0x3fffffffu || grid > 0x7fffffffu || joins > 0x3fffffffu) return T2H_ERR_SHAPE;
+    a.kv_blocks = (uint32_t)kv;
+    a.q_blocks = (uint32_t)((waves + 3) / 4);
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    hipLaunchKernelGGL(tree_rows_kernel, dim3((uint32_t)((waves + 3) / 4)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(tree_rows_kernel, dim3(1 + a.kv_blocks + a.q_blocks), dim3(256), 0, st, a);
     T2H_LAUNCH_CHECK();
-    hipLaunchKernelGGL(tree_attn_kernel, dim3((uint32_t)(rows * nh)), dim3(64), 0, st, a);
+    const dim3 g((uint32_t)grid);
+    if (s.tile_rows == 32) hipLaunchKernelGGL((tree_attn_kernel<1, 4, 2>), g, dim3(256), 0, st, a);
+    else if (s.tile_rows == 64) hipLaunchKernelGGL((tree_attn_kernel<2, 4, 2>), g, dim3(512), 0, st, a);
+    else if (s.tile_rows == 128) hipLaunchKernelGGL((tree_attn_kernel<4, 2, 4>), g, dim3(512), 0, st, a);
+    else hipLaunchKernelGGL((tree_attn_kernel<8, 1, 8>), g, dim3(512), 0, st, a);
     T2H_LAUNCH_CHECK();
+    if (s.units > n_seq) {
+        hipLaunchKernelGGL(tree_join_kernel, dim3((uint32_t)joins), dim3(256), 0, st, a);
+        T2H_LAUNCH_CHECK();
+    }
     return T2H_OK;
 }
