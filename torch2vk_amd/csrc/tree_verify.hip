@@ -10,11 +10,15 @@ namespace t2h {
 // ------------------------------------------------------------------------------------------------ verification --
 //
 // Two launches.  The first reads every node's row of logits once, a wave a piece of E * 64 of them, and leaves the piece's largest
-// logit and the sum of exp((l - largest) / T).  The second joins a row's pieces, walks down the tree, and draws the token that
-// follows from the row where the walk ended: the piece in which the running sum passes the border, then its logits once more.
-// Where drafts were drawn it reads that row of both models again for max(p - q, 0), in thread blocks of their own.
-// Sums and exponentials are in 64 bits, relative errors of 10^-14: the borders between the tokens of a large vocabulary lie
-// 10^-5 of the sum apart, and 32 bits would draw its neighbour for a token now and then.
+// logit and the sum of exp((l - largest) / T), or where that logit is.  In the second every thread block joins the rows' pieces
+// and walks down the tree; then its waves sum their segments of the row where the walk ended, and the last thread block of a
+// sequence to get there draws the next token: the segment in which the running sum passes the border, then its logits.
+// The borders between the tokens of a large vocabulary lie 10^-5 of the sum apart: that row's sums and exponentials are in 64
+// bits (relative errors of 10^-12), since 32 would now and then draw a token's neighbour.  A child's acceptance compares one
+// probability with one number, where 32-bit exponentials and 64-bit sums (10^-7) decide as well.
+// Where drafts are drawn the next token's mass is max(p - q, 0) = max(w / Z - v / Y, 0), and Z and Y are known to 10^-7 only when
+// the second pass begins.  That is enough to tell which tokens have any (the others' share is 10^-7 of theirs); the sums of
+// their w and v, and of all w and v, are kept apart, and the last thread block has Z and Y in 64 bits.
 
 struct VerifyArgs {
     const void* logits;
@@ -30,253 +34,298 @@ struct VerifyArgs {
     int32_t* kept;
     int64_t* next_token;
     uint32_t n, n_seq, vocab;
-    uint32_t pieces;   // of a row
-    double* part_sum;  // [rows][pieces], the draft's rows behind the target's
-    uint2* part_top;   // bits of the largest logit; its index where the sequence is greedy
-    uint32_t chunks;   // thread blocks that read a sequence's last row again
-    uint32_t* done;    // [n_seq] of those that have left their sums; zero between calls
-    double* left;      // [n_seq][chunks] sums of max(p - q, 0)
+    uint32_t pieces;  // of a row
+    uint2* part;      // [rows][pieces], the draft's rows behind the target's: bits of the largest logit; of the sum, or its index
+    uint32_t chunks;  // thread blocks a sequence in the second launch, of per_block segments
+    uint32_t per_block;
+    uint32_t* done;   // [n_seq] of those that have left their sums; zero between calls
+    double* left;     // [n_seq][segments][4] sums of the row where the walk ended
 };
 
 constexpr int V_TABLE = 32;
 
-// 2^(j / 32), by the first lanes of a thread block.
-__device__ __forceinline__ void exp_table(double* table) {
-    if (threadIdx.x < V_TABLE) table[threadIdx.x] = exp2((double)threadIdx.x / V_TABLE);
-}
+// 2^(j / 32)
+__device__ const double V_POWERS[V_TABLE] = {
+    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237,
+    1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
+    1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
+    1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
+    1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228,
+    1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.645755478153965,
+    1.681792830507429, 1.718619298122478, 1.7562521603732995, 1.7947090750031072,
+    1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002,
+};
 
-// exp(x) of x = y ln 2 / 32, y <= 0: 2^(j / 32) from the table, and the Taylor series of what is left, |z| <= ln 2 / 64, up to
-// z^5 (the next term is 2 10^-15).  Under 2^-1000 it is 0.
-__device__ __forceinline__ double exp_steps(double y, const double* table) {
-    constexpr double C = 0.02166084939249829;  // ln 2 / 32
+// exp(y ln 2 / 32) of N numbers y <= 0: 2^(j / 32) from the table, and the Taylor series of what is left, |z| <= ln 2 / 64, up to
+// z^4 (the next term is 10^-12).  What is less than 2^-1000, and NaN, gives 0.
+template <int N>
+__device__ __forceinline__ void exp_steps(double (&y)[N], const double* table) {
+    constexpr double C = 0.02166084939249829;     // ln 2 / 32
     constexpr double MAGIC = 6755399441055744.0;  // 1.5 2^52: a sum with it is rounded to a whole number, in its low word
-    y = fmax(y, -33000.0);
-    const double z = y + MAGIC, r = y - (z - MAGIC);
-    const int steps = (int)__double2loint(z), e = steps >> 5;
-    double p = C * C * C * C * C / 120.0;
-    p = fma(p, r, C * C * C * C / 24.0);
-    p = fma(p, r, C * C * C / 6.0);
-    p = fma(p, r, C * C / 2.0);
-    p = fma(p, r, C);
-    p = fma(p, r, 1.0);
-    p *= table[steps & (V_TABLE - 1)];
-    const double w = __hiloint2double(__double2hiint(p) + (e << 20), __double2loint(p));
-    return e < -1000 ? 0.0 : w;
+    int steps[N];
+    double power[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        y[e] = fmax(y[e], -32001.0);
+        const double z = y[e] + MAGIC;
+        y[e] -= z - MAGIC;
+        steps[e] = (int)__double2loint(z);
+        power[e] = table[steps[e] & (V_TABLE - 1)];
+    }
+    __builtin_amdgcn_sched_barrier(0);  // (the table's reads all on their way)
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        const double r = y[e];
+        double p = fma(C * C * C * C / 24.0, r, C * C * C / 6.0);
+        p = fma(p, r, C * C / 2.0);
+        p = fma(p, r, C);
+        p = fma(p, r, 1.0) * power[e];
+        y[e] = steps[e] <= -32000 ? 0.0 : __hiloint2double(__double2hiint(p) + ((steps[e] >> 5) << 20), __double2loint(p));
+    }
 }
 
-// exp((x - top) / T) with steps = 32 / (T ln 2); infinite logits share the probability.  x is not NaN.
-__device__ __forceinline__ double verify_weight(float x, float top, double steps, const double* table) {
-    if (top == INFINITY) return x == INFINITY ? 1.0 : 0.0;
-    if (x == -INFINITY) return 0.0;
-    return exp_steps(((double)x - (double)top) * steps, table);
-}
-
-__device__ __forceinline__ double verify_steps(const VerifyArgs& a, uint32_t seq) {  // 0: greedy
+__device__ __forceinline__ float verify_temperature(const VerifyArgs& a, uint32_t seq) {  // 0: greedy
     const float t = a.temperatures ? a.temperatures[seq] : a.temperature;
-    return t > 0.0f ? 46.16624130844683 / (double)t : 0.0;
+    return t > 0.0f ? t : 0.0f;
 }
+__device__ __forceinline__ double verify_steps(float t) { return 46.16624130844683 / (double)t; }
+__device__ __forceinline__ float verify_factor(float t) { return fminf(1.4426950408889634f / t, 3.4e38f); }
 
-// A logit as it counts: NaN as -infinity.
 template <bool BF16>
 __device__ __forceinline__ float verify_logit(const void* base, size_t at) {
-    const float x = BF16 ? bf16_bits_to_f32(static_cast<const uint16_t*>(base)[at]) : static_cast<const float*>(base)[at];
-    return fmaxf(x, -INFINITY);
+    return BF16 ? bf16_bits_to_f32(static_cast<const uint16_t*>(base)[at]) : static_cast<const float*>(base)[at];
 }
 
-__device__ __forceinline__ double wave_sum_f64(double v) {
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_f64(double v) {
+    return __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, ROWS, 0xf, false),
+                            __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ double readlane_f64(double x, int lane) {
+    return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(x), lane), __builtin_amdgcn_readlane(__double2loint(x), lane));
+}
+
+// Sums over the lanes up to each: within rows of 16, then over the rows.
+__device__ __forceinline__ double wave_scan_f64(double v) {
+    v += dpp_f64<0x111, 0xf>(v);  // 1 lane up
+    v += dpp_f64<0x112, 0xf>(v);
+    v += dpp_f64<0x114, 0xf>(v);
+    v += dpp_f64<0x118, 0xf>(v);
+    v += dpp_f64<0x142, 0xa>(v);  // a row's last lane to the odd rows
+    v += dpp_f64<0x143, 0xc>(v);  // lane 31 to the upper half
+    return v;
+}
+__device__ __forceinline__ double wave_sum_f64(double v) { return readlane_f64(wave_scan_f64(v), 63); }
+__device__ __forceinline__ uint32_t wave_min_u32(uint32_t v) {
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
+    for (int off = 32; off > 0; off >>= 1) v = min(v, (uint32_t)__shfl_xor((int)v, off));
     return v;
 }
 
 template <bool BF16, int E>
 __global__ __launch_bounds__(256) void verify_rows_kernel(const VerifyArgs a) {
     constexpr int PER = BF16 ? 8 : 4, LOADS = E / PER;  // logits a load of 16 bytes
-    __shared__ double table[V_TABLE];
-    exp_table(table);
-    __syncthreads();
     const int lane = threadIdx.x & 63;
     const uint32_t unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t r = unit / a.pieces, piece = unit % a.pieces, rows = a.n_seq * a.n;
     const bool draft = r >= rows;
     if (r >= rows + (a.draft ? a.n_seq * (a.n - 1) : 0)) return;
     const uint32_t per = draft ? a.n - 1 : a.n, row = draft ? r - rows : r, seq = row / per;
-    if ((int)(row % per) >= tree_count(a.counts, seq, a.n) - (draft ? 1 : 0)) return;
     const uint8_t* const base = draft ? static_cast<const uint8_t*>(a.draft) + (size_t)row * a.draft_stride * (BF16 ? 2 : 4)
                                       : static_cast<const uint8_t*>(a.logits) + (size_t)row * a.row_stride * (BF16 ? 2 : 4);
+    if ((int)(row % per) >= tree_count(a.counts, seq, a.n) - (draft ? 1 : 0)) return;
+    const float t = verify_temperature(a, seq);
     const uint32_t first = piece * (E * 64) + lane * PER;
     float x[E];
+    if ((piece + 1) * (E * 64) <= a.vocab) {
+        uint4 w[LOADS];
 #pragma unroll
-    for (int v = 0; v < LOADS; ++v) {
-        const uint32_t at = first + v * (64 * PER);
-        if (at + PER <= a.vocab) {
-            const uint4 w = load_u4_ua(base + (size_t)at * (BF16 ? 2 : 4));
-            const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+        for (int v = 0; v < LOADS; ++v) w[v] = load_u4_ua(base + (size_t)(first + v * (64 * PER)) * (BF16 ? 2 : 4));
+#pragma unroll
+        for (int v = 0; v < LOADS; ++v) {
+            const uint32_t words[4] = {w[v].x, w[v].y, w[v].z, w[v].w};
 #pragma unroll
             for (int e = 0; e < PER; ++e)
                 x[v * PER + e] = BF16 ? __uint_as_float(e & 1 ? words[e / 2] & 0xffff0000u : words[e / 2] << 16) : __uint_as_float(words[e & 3]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < PER; ++e) x[v * PER + e] = at + e < a.vocab ? verify_logit<BF16>(base, at + e) : -INFINITY;
         }
-    }
-    float top = -INFINITY;
+    } else {
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        x[e] = fmaxf(x[e], -INFINITY);
-        top = fmaxf(top, x[e]);
+        for (int e = 0; e < E; ++e) {
+            const uint32_t at = first + (e / PER) * (64 * PER) + e % PER;
+            x[e] = verify_logit<BF16>(base, min(at, a.vocab - 1));  // (no load waits for another)
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (first + (e / PER) * (64 * PER) + e % PER >= a.vocab) x[e] = -INFINITY;
     }
+    float top = -INFINITY;  // (of a NaN and a number the number)
+#pragma unroll
+    for (int e = 0; e < E; ++e) top = fmaxf(top, x[e]);
     top = wave_max(top);
-    const double steps = verify_steps(a, seq);
-    const size_t part = (size_t)r * a.pieces + piece;
-    if (steps == 0.0) {
-        uint32_t best = 0xffffffffu;
+    uint32_t second;
+    if (t == 0.0f) {
+        second = 0xffffffffu;
 #pragma unroll
         for (int e = E - 1; e >= 0; --e)
-            if (x[e] == top) best = first + (e / PER) * (64 * PER) + e % PER;
+            if (x[e] == top) second = first + (e / PER) * (64 * PER) + e % PER;
+        second = wave_min_u32(second);
+    } else {
+        float sum = 0.0f;  // up to 64 terms a lane: as good as its terms
+        if (top == INFINITY) {
 #pragma unroll
-        for (int off = 32; off > 0; off >>= 1) best = min(best, (uint32_t)__shfl_xor((int)best, off));
-        if (lane == 0) a.part_top[part] = make_uint2(__float_as_uint(top), best);
-        return;
-    }
-    double sum = 0.0;
-    if (top == INFINITY) {
+            for (int e = 0; e < E; ++e) sum += x[e] == INFINITY ? 1.0f : 0.0f;
+        } else if (top > -INFINITY) {
+            const float c = verify_factor(t);
 #pragma unroll
-        for (int e = 0; e < E; ++e) sum += x[e] == INFINITY ? 1.0 : 0.0;
-    } else if (top > -INFINITY) {
-        const double dtop = (double)top;
-#pragma unroll
-        for (int e = 0; e < E; ++e) sum += exp_steps(((double)x[e] - dtop) * steps, table);
+            for (int e = 0; e < E; ++e) sum += __builtin_amdgcn_exp2f(fmaxf((x[e] - top) * c, -200.0f));
+        }
+        second = __float_as_uint(wave_sum(sum));
     }
-    sum = wave_sum_f64(sum);
-    if (lane == 0) {
-        a.part_top[part] = make_uint2(__float_as_uint(top), 0u);
-        a.part_sum[part] = sum;
-    }
+    if (lane == 0) a.part[(size_t)r * a.pieces + piece] = make_uint2(__float_as_uint(top), second);
 }
 
 constexpr int VF_WAVES = 16, VF_THREADS = VF_WAVES * 64;
-
-__device__ __forceinline__ double shfl_up_f64(double v, int by) { return __shfl_up(v, by); }
-
-// Sums over a thread block's threads up to each; `room` holds VF_WAVES doubles and is free again after the next barrier.
-__device__ __forceinline__ double block_scan(double v, double* room) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const double o = shfl_up_f64(v, off);
-        if (lane >= off) v += o;
-    }
-    if (lane == 63) room[wave] = v;
-    __syncthreads();
-    double before = 0.0;
-    for (int w = 0; w < wave; ++w) before += room[w];
-    return before + v;
-}
+constexpr int VF_EACH = 8;                        // logits a lane
+constexpr uint32_t VF_SEGMENT = 64 * VF_EACH;     // a wave
 
 struct VerifyState {
     float top[2 * TREE_MAX];   // the rows' largest logits, the draft's behind the target's
     double sum[2 * TREE_MAX];  // and sums
     int64_t best[TREE_MAX];
-    int64_t gone[TREE_MAX];    // tokens that the walk rejected where it ended
+    int gone[TREE_MAX];        // tokens that the walk rejected where it ended
     int n_gone, cur, kept;
-    double scan[2][VF_WAVES];
-    uint32_t hit[2], last[2];
-    double fresh[TREE_MAX];    // masses of the pieces that lost them, read anew
-    double before, border, total;
-    uint32_t arrived;
+    double u;                  // the number that draws the next token
 };
 
-__device__ __forceinline__ double readlane_f64(double x, int lane) {
-    return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(x), lane), __builtin_amdgcn_readlane(__double2loint(x), lane));
-}
 __device__ __forceinline__ int64_t readlane_i64(int64_t x, int lane) {
     return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32 |
                      (uint32_t)__builtin_amdgcn_readlane((int)x, lane));
 }
 
-// A row's largest logit and sum (or its index) from its pieces, in every lane of a wave.
-__device__ __forceinline__ void verify_join(const VerifyArgs& a, size_t row, double steps, const double* table, float& top,
-                                            double& sum, uint32_t& best) {
-    const int lane = threadIdx.x & 63;
-    const uint2* const tops = a.part_top + row * a.pieces;
-    top = -INFINITY;
-    for (uint32_t i = lane; i < a.pieces; i += 64) top = fmaxf(top, __uint_as_float(tops[i].x));
-    top = wave_max(top);
-    sum = 0.0;
-    best = 0xffffffffu;
-    for (uint32_t i = lane; i < a.pieces; i += 64) {
-        const uint2 t = tops[i];
-        const float x = __uint_as_float(t.x);
-        if (steps == 0.0) {
-            if (x == top) best = min(best, t.y);
-        } else {
-            sum += a.part_sum[row * a.pieces + i] * verify_weight(x, top, steps, table);
-        }
-    }
-    if (steps == 0.0) {
+// Rows' largest logits and sums, or those logits' indexes, from their pieces: a wave two rows at a time.
+__device__ __forceinline__ void verify_join(const VerifyArgs& a, uint32_t seq, int count, int rows, float t, VerifyState& st) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    constexpr int AHEAD = 3;  // 64 pieces each: those of 151936 logits, where they are small
+    const float c = t > 0.0f ? verify_factor(t) : 0.0f;
+    for (int i0 = wave; i0 < rows; i0 += 2 * VF_WAVES) {
+        uint2 p[2][AHEAD];
+        const uint2* part[2];
 #pragma unroll
-        for (int off = 32; off > 0; off >>= 1) best = min(best, (uint32_t)__shfl_xor((int)best, off));
-    } else {
-        sum = wave_sum_f64(sum);
+        for (int k = 0; k < 2; ++k) {
+            const int i = min(i0 + k * VF_WAVES, rows - 1);
+            const size_t row = i < count ? (size_t)seq * a.n + i : (size_t)a.n_seq * a.n + (size_t)seq * (a.n - 1) + (i - count);
+            part[k] = a.part + row * a.pieces;
+#pragma unroll
+            for (int g = 0; g < AHEAD; ++g) p[k][g] = part[k][min((uint32_t)(lane + 64 * g), a.pieces - 1)];
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int i = i0 + k * VF_WAVES;
+            if (i >= rows) break;
+            float top = -INFINITY;
+#pragma unroll
+            for (int g = 0; g < AHEAD; ++g) top = fmaxf(top, __uint_as_float(p[k][g].x));
+            for (uint32_t q = lane + 64 * AHEAD; q < a.pieces; q += 64) top = fmaxf(top, __uint_as_float(part[k][q].x));
+            top = wave_max(top);
+            double sum = 0.0;
+            uint32_t best = 0xffffffffu;
+            auto add = [&](uint2 q, bool in) {
+                const float x = __uint_as_float(q.x);
+                if (t == 0.0f) {
+                    if (x == top) best = min(best, q.y);  // (a piece twice is no harm here)
+                } else {
+                    const float w = top == INFINITY ? (x == INFINITY ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(fmaxf((x - top) * c, -200.0f));
+                    sum += in && x > -INFINITY ? (double)(__uint_as_float(q.y) * w) : 0.0;
+                }
+            };
+#pragma unroll
+            for (int g = 0; g < AHEAD; ++g) add(p[k][g], (uint32_t)(lane + 64 * g) < a.pieces);
+            for (uint32_t q = lane + 64 * AHEAD; q < a.pieces; q += 64) add(part[k][q], true);
+            if (t == 0.0f) best = wave_min_u32(best);
+            else sum = wave_sum_f64(sum);
+            if (lane == 0) {
+                const int to = i < count ? i : TREE_MAX + i - count;
+                st.top[to] = top;
+                st.sum[to] = sum;
+                if (i < count) st.best[i] = top == -INFINITY ? -1 : (int64_t)best;
+            }
+        }
     }
 }
 
-__device__ __forceinline__ double verify_uniform(const VerifyArgs& a, uint32_t seq, int c) {
-    return (double)fminf(fmaxf(a.uniforms[(size_t)seq * a.n + c], 0.0f), 0.99999994f);  // NaN as 0
+// A node as a lane of the walking wave sees it, with the logits of its token after its parent.
+struct VerifyNode {
+    int up;
+    int64_t token;
+    float x, y, u;
+};
+
+template <bool BF16, bool DRAWN>
+__device__ __forceinline__ VerifyNode verify_node(const VerifyArgs& a, uint32_t seq, int count, float t) {
+    const int lane = threadIdx.x & 63;
+    VerifyNode v = {lane - 1, -1, -INFINITY, -INFINITY, 0.0f};
+    if (lane >= count) return v;
+    const size_t at = (size_t)seq * a.n + lane;
+    v.token = a.tokens[at];
+    if (a.parents) v.up = a.parents[at];
+    if (t == 0.0f) return v;
+    v.u = fminf(fmaxf(a.uniforms[at], 0.0f), 0.99999994f);  // NaN as 0
+    if (v.up >= 0 && v.up < lane && v.token >= 0 && v.token < (int64_t)a.vocab) {
+        v.x = verify_logit<BF16>(a.logits, ((size_t)seq * a.n + v.up) * a.row_stride + v.token);
+        if (DRAWN) v.y = verify_logit<BF16>(a.draft, ((size_t)seq * (a.n - 1) + v.up) * a.draft_stride + v.token);
+    }
+    return v;
+}
+
+// exp((x - top) / T) in 32 bits, as the sums have it.
+__device__ __forceinline__ double verify_share(float x, float top, double sum, float c) {
+    if (!(x > -INFINITY) || !(sum > 0.0)) return 0.0;
+    return (double)(top == INFINITY ? (x == INFINITY ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(fmaxf((x - top) * c, -200.0f)));
 }
 
 // One wave walks down a sequence's tree.
-template <bool BF16, bool DRAWN>
-__device__ void verify_walk(const VerifyArgs& a, uint32_t seq, int count, double steps, const double* table, VerifyState& st,
-                            bool writes) {
+template <bool DRAWN>
+__device__ __forceinline__ void verify_walk(const VerifyArgs& a, uint32_t seq, int count, float t, const VerifyNode& v,
+                                            VerifyState& st, bool writes) {
     const int lane = threadIdx.x & 63;
-    int up = lane - 1;
-    int64_t token = -1;
-    double w = 0.0, q = 0.0, u = 0.0;
-    if (lane < count) {
-        if (a.parents) up = a.parents[(size_t)seq * a.n + lane];
-        token = a.tokens[(size_t)seq * a.n + lane];
-        if (lane > 0 && up >= 0 && up < lane && token >= 0 && token < (int64_t)a.vocab && steps != 0.0) {
-            const size_t row = (size_t)seq * a.n + up;
-            w = verify_weight(verify_logit<BF16>(a.logits, row * a.row_stride + token), st.top[up], steps, table);
-            if (DRAWN) {
-                const size_t draft = (size_t)seq * (a.n - 1) + up;
-                const double z = st.sum[up], zq = st.sum[TREE_MAX + up];
-                w = z > 0.0 ? w / z : 0.0;
-                q = verify_weight(verify_logit<BF16>(a.draft, draft * a.draft_stride + token), st.top[TREE_MAX + up], steps, table);
-                q = zq > 0.0 ? q / zq : 0.0;
-            }
+    double w = 0.0, q = 0.0;  // drawn: both times the sums, u q Y^-1 < p Z^-1 as u q Z < p Y
+    if (t > 0.0f && v.up >= 0 && v.up < lane && lane < count) {
+        const float c = verify_factor(t);
+        w = verify_share(v.x, st.top[v.up], st.sum[v.up], c);
+        if (DRAWN) {
+            const double z = st.sum[v.up], y = st.sum[TREE_MAX + v.up];
+            q = verify_share(v.y, st.top[TREE_MAX + v.up], y, c) * (z > 0.0 ? z : 1.0);
+            w *= y > 0.0 ? y : 1.0;
         }
-        if (steps != 0.0) u = verify_uniform(a, seq, lane);
     }
     int cur = 0, kept = count > 0 ? 1 : 0, mine = lane == 0 && kept ? 0 : -1;  // lane j: the path's entry j
     uint64_t gone = 0;
-    double rest = count > 0 && steps != 0.0 ? st.sum[0] : 0.0;
+    double rest = kept && t > 0.0f ? st.sum[0] : 0.0;
     for (bool more = kept != 0; more;) {
         more = false;
-        uint64_t children = __ballot(lane > cur && lane < count && up == cur);
+        uint64_t children = __ballot(lane > cur && lane < count && v.up == cur);
         while (children) {
             const int c = __builtin_ctzll(children);
             children &= children - 1;
-            const int64_t x = readlane_i64(token, c);
+            const int64_t x = readlane_i64(v.token, c);
+            const double u = (double)__int_as_float(__builtin_amdgcn_readlane(__float_as_int(v.u), c));
             bool yes;
             double wc = 0.0;
-            if (steps == 0.0) {
+            if (t == 0.0f) {
                 yes = st.best[cur] >= 0 && x == st.best[cur];
             } else if (DRAWN) {
-                yes = readlane_f64(u, c) * readlane_f64(q, c) < readlane_f64(w, c);
+                yes = u * readlane_f64(q, c) < readlane_f64(w, c);
             } else {
-                const bool again = __ballot((gone >> lane & 1) && token == x) != 0;
+                const bool again = __ballot((gone >> lane & 1) && v.token == x) != 0;
                 wc = again ? 0.0 : readlane_f64(w, c);
-                yes = readlane_f64(u, c) * rest < wc;
+                yes = u * rest < wc;
             }
             if (yes) {
                 if (lane == kept) mine = c;
                 ++kept;
                 cur = c;
                 gone = 0;
-                rest = steps != 0.0 ? st.sum[cur] : 0.0;
+                rest = t > 0.0f ? st.sum[cur] : 0.0;
                 more = true;
                 break;
             }
@@ -288,209 +337,220 @@ __device__ void verify_walk(const VerifyArgs& a, uint32_t seq, int count, double
         if (lane < (int)a.n) a.path[(size_t)seq * a.n + lane] = mine;
         if (lane == 0) a.kept[seq] = kept;
     }
-    if (gone >> lane & 1) st.gone[__popcll(gone & ((1ull << lane) - 1))] = token;
+    if (gone >> lane & 1) st.gone[__popcll(gone & ((1ull << lane) - 1))] = v.token >= 0 && v.token < (int64_t)a.vocab ? (int)v.token : -1;
     if (lane == 0) {
         st.cur = cur;
         st.kept = kept;
         st.n_gone = DRAWN ? 0 : __popcll(gone);
-        st.total = rest;
+        st.u = (double)v.u;
     }
 }
 
-template <bool BF16, int E, bool DRAWN>
+__device__ __forceinline__ void put_f64(double* p, double x) {
+    __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ double get_f64(const double* p) {
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+template <bool BF16, bool DRAWN>
 __global__ __launch_bounds__(VF_THREADS) void verify_finish_kernel(const VerifyArgs a) {
     __shared__ double table[V_TABLE];
     __shared__ VerifyState st;
-    const uint32_t seq = DRAWN ? blockIdx.x / a.chunks : blockIdx.x, chunk = DRAWN ? blockIdx.x % a.chunks : 0;
+    const uint32_t seq = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int count = tree_count(a.counts, seq, a.n);
-    const double steps = verify_steps(a, seq);
-    const uint32_t row0 = seq * a.n, rows = a.n_seq * a.n;
-    exp_table(table);
+    const float t = verify_temperature(a, seq);
+    if (chunk != 0 && (count == 0 || t == 0.0f)) return;
+    VerifyNode node;
+    if (wave == 0) node = verify_node<BF16, DRAWN>(a, seq, count, t);
+    if (tid >= VF_THREADS - V_TABLE) table[tid - (VF_THREADS - V_TABLE)] = V_POWERS[tid - (VF_THREADS - V_TABLE)];
+    verify_join(a, seq, count, DRAWN && count > 0 ? 2 * count - 1 : count, t, st);
     __syncthreads();
-    for (int i = wave; i < (DRAWN ? 2 * count - 1 : count); i += VF_WAVES) {
-        const bool draft = i >= count;
-        const int node = draft ? i - count : i;
-        float top;
-        double sum;
-        uint32_t best;
-        verify_join(a, draft ? (size_t)rows + (size_t)seq * (a.n - 1) + node : (size_t)row0 + node, steps, table, top, sum, best);
-        if (lane == 0) {
-            st.top[draft ? TREE_MAX + node : node] = top;
-            st.sum[draft ? TREE_MAX + node : node] = sum;
-            if (!draft) st.best[node] = top == -INFINITY ? -1 : (int64_t)best;
-        }
-    }
-    __syncthreads();
-    if (wave == 0) verify_walk<BF16, DRAWN>(a, seq, count, steps, table, st, chunk == 0);
-    if (tid == 0) {
-        st.hit[0] = st.hit[1] = 0xffffffffu;
-        st.last[0] = st.last[1] = 0;
-        st.before = 0.0;
-    }
+    if (wave == 0) verify_walk<DRAWN>(a, seq, count, t, node, st, chunk == 0);
     __syncthreads();
     const int cur = st.cur;
-    if (st.kept == 0 || steps == 0.0) {
-        if (chunk == 0 && tid == 0) a.next_token[seq] = st.kept == 0 ? -1 : st.best[cur];
+    if (st.kept == 0 || t == 0.0f) {
+        if (tid == 0) a.next_token[seq] = st.kept == 0 ? -1 : st.best[cur];
         return;
     }
+    // the row where the walk ended, and the draft's there if its token was drawn and rejected
+    const double steps = verify_steps(t);
     const float top = st.top[cur];
-    const size_t row = (size_t)(row0 + cur), logits = row * a.row_stride;
-    // the mass that token x has in the row where the walk ended
-    auto mass = [&](uint32_t x) {
-        if (x >= a.vocab) return 0.0;
-        for (int j = 0; j < st.n_gone; ++j)
-            if (st.gone[j] == (int64_t)x) return 0.0;
-        return verify_weight(verify_logit<BF16>(a.logits, logits + x), top, steps, table);
-    };
-
-    if (DRAWN && cur < count - 1) {
-        // max(p - q, 0), a chunk a thread block
-        const float qtop = st.top[TREE_MAX + cur];
-        const double z = st.sum[cur], zq = st.sum[TREE_MAX + cur], iz = z > 0.0 ? 1.0 / z : 0.0, izq = zq > 0.0 ? 1.0 / zq : 0.0;
-        const size_t draft = ((size_t)seq * (a.n - 1) + cur) * a.draft_stride;
-        auto more = [&](uint32_t x) {
-            if (x >= a.vocab) return 0.0;
-            const double p = verify_weight(verify_logit<BF16>(a.logits, logits + x), top, steps, table) * iz;
-            const double q = verify_weight(verify_logit<BF16>(a.draft, draft + x), qtop, steps, table) * izq;
-            return p > q ? p - q : 0.0;
-        };
-        constexpr int EACH = 8;
-        constexpr uint32_t CHUNK = VF_THREADS * EACH;
-        double sum = 0.0;
+    const size_t logits = ((size_t)seq * a.n + cur) * a.row_stride;
+    const int gone = lane < st.n_gone ? st.gone[lane] : -1;
+    const bool residual = DRAWN && cur < count - 1;
+    const void* const draft = residual  // (or a row that is not looked at)
+                                  ? static_cast<const uint8_t*>(a.draft) + ((size_t)seq * (a.n - 1) + cur) * a.draft_stride * (BF16 ? 2 : 4)
+                                  : static_cast<const uint8_t*>(a.logits) + logits * (BF16 ? 2 : 4);
+    const float qtop = residual ? st.top[TREE_MAX + cur] : 0.0f;
+    auto weigh = [&](const float (&x)[VF_EACH], float top, double (&w)[VF_EACH]) {
+        if (top == INFINITY) {  // infinite logits share the probability
 #pragma unroll
-        for (int e = 0; e < EACH; ++e) sum += more(chunk * CHUNK + e * VF_THREADS + tid);
-        const double upto = block_scan(sum, st.scan[0]);
-        if (tid == VF_THREADS - 1)
-            __hip_atomic_store(&a.left[(size_t)seq * a.chunks + chunk], upto, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        // the last thread block of a sequence to get here draws.  A sum is there before the count is raised.
-        __builtin_amdgcn_s_waitcnt(0);
-        asm volatile("" ::: "memory");
-        __syncthreads();
-        if (tid == 0) {
-            st.arrived = __hip_atomic_fetch_add(&a.done[seq], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u;
-            if (st.arrived == a.chunks) __hip_atomic_store(&a.done[seq], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            for (int e = 0; e < VF_EACH; ++e) w[e] = x[e] == INFINITY ? 1.0 : 0.0;
+        } else {
+#pragma unroll
+            for (int e = 0; e < VF_EACH; ++e) w[e] = ((double)x[e] - (double)top) * steps;
+            exp_steps(w, table);
         }
-        __syncthreads();
-        if (st.arrived != a.chunks) return;
-        if (tid == 0) {
-            double total = 0.0;
-            for (uint32_t c = 0; c < a.chunks; ++c)
-                total += __hip_atomic_load(&a.left[(size_t)seq * a.chunks + c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            const double border = verify_uniform(a, seq, 0) * total;
-            double before = 0.0;
-            uint32_t at = 0;
-            for (uint32_t c = 0; c < a.chunks; ++c) {
-                const double x = __hip_atomic_load(&a.left[(size_t)seq * a.chunks + c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                if (x <= 0.0) continue;
-                at = c;
-                if (before + x > border) break;
-                before += x;
-            }
-            st.total = total;
-            st.before = before;
-            st.border = border;
-            st.cur = (int)at;
-        }
-        __syncthreads();
-        if (st.total > 0.0) {
-            const uint32_t at = (uint32_t)st.cur * CHUNK;
-            for (int e = 0; e < EACH; ++e) {
-                const uint32_t x = at + e * VF_THREADS + tid;
-                const double v = more(x);
-                const double to = st.before + block_scan(v, st.scan[e & 1]);
-                if (v > 0.0) {
-                    atomicMax(&st.last[0], x);
-                    if (to > st.border) atomicMin(&st.hit[0], x);
-                }
-                __syncthreads();
-                if (tid == VF_THREADS - 1) st.before = to;
-                __syncthreads();
-                if (st.hit[0] != 0xffffffffu) break;
-            }
-            if (tid == 0) a.next_token[seq] = st.hit[0] != 0xffffffffu ? st.hit[0] : st.last[0];
-            return;
-        }
-        // nothing is left of the target's row beside the draft's: the row itself
-        __syncthreads();
-        if (tid == 0) st.before = 0.0;
-        __syncthreads();
-    } else if (DRAWN && chunk != 0) {
-        return;
-    }
-
-    // 1. the pieces' masses: a piece that lost tokens is read anew where little is left of the row, so that no difference of two
-    // near numbers is drawn from
-    const double whole = st.sum[cur];
-    const bool little = st.n_gone > 0 && st.total < whole * (1.0 / 1024.0);
-    constexpr uint32_t PIECE = E * 64;
-    if (little)
-        for (int j = 0; j < st.n_gone; ++j) {
-            const int64_t x = st.gone[j];
-            double m = 0.0;
-            if (x >= 0 && x < (int64_t)a.vocab)
-                for (uint32_t i = tid; i < PIECE; i += VF_THREADS) m += mass((uint32_t)x / PIECE * PIECE + i);
-            const double upto = block_scan(m, st.scan[j & 1]);
-            if (tid == VF_THREADS - 1) st.fresh[j] = upto;
-            __syncthreads();
-        }
-    auto piece_mass = [&](uint32_t i) {
-        if (i >= a.pieces) return 0.0;
-        const float t = __uint_as_float(a.part_top[row * a.pieces + i].x);
-        double m = a.part_sum[row * a.pieces + i] * verify_weight(t, top, steps, table);
-        for (int j = 0; j < st.n_gone; ++j) {
-            const int64_t x = st.gone[j];
-            if (x < 0 || x >= (int64_t)a.vocab || (uint32_t)x / PIECE != i) continue;
-            if (little) return st.fresh[j];
-            bool first = true;
-            for (int k = 0; k < j; ++k) first = first && st.gone[k] != x;
-            if (first) m -= verify_weight(verify_logit<BF16>(a.logits, logits + (size_t)x), top, steps, table);
-        }
-        return m > 0.0 ? m : 0.0;
     };
-    double total = 0.0;
-    for (uint32_t i0 = 0; i0 < a.pieces; i0 += VF_THREADS) total += piece_mass(i0 + tid);
-    const double sums = block_scan(total, st.scan[0]);
-    if (tid == VF_THREADS - 1) {
-        st.total = sums;
-        st.border = verify_uniform(a, seq, 0) * sums;
+    // of segment s: exp((l - top) / T) of the target (without what the walk rejected) and of the draft, lane's tokens 64 e + lane
+    auto segment = [&](uint32_t s, double (&w)[VF_EACH], double (&v)[VF_EACH]) {
+        const uint32_t x0 = s * VF_SEGMENT + lane;
+        float x[VF_EACH], y[VF_EACH];
+#pragma unroll
+        for (int e = 0; e < VF_EACH; ++e) {  // (no load waits for another)
+            const uint32_t at = min(x0 + 64 * e, a.vocab - 1);
+            x[e] = verify_logit<BF16>(a.logits, logits + at);
+            if (DRAWN) y[e] = verify_logit<BF16>(draft, at);
+        }
+#pragma unroll
+        for (int e = 0; e < VF_EACH; ++e)
+            if (x0 + 64 * e >= a.vocab) x[e] = y[e] = -INFINITY;
+        weigh(x, top, w);
+        if (DRAWN) {
+            if (residual) weigh(y, qtop, v);
+        } else {
+            for (uint64_t here = __ballot(gone >= 0 && (uint32_t)gone / VF_SEGMENT == s); here; here &= here - 1) {
+                const int g = __builtin_amdgcn_readlane(gone, __builtin_ctzll(here)) - (int)x0;
+#pragma unroll
+                for (int e = 0; e < VF_EACH; ++e)
+                    if (g == 64 * e) w[e] = 0.0;
+            }
+        }
+    };
+    double w[VF_EACH], v[VF_EACH];
+    const double near = residual && st.sum[TREE_MAX + cur] > 0.0 ? st.sum[cur] / st.sum[TREE_MAX + cur] : 0.0;  // Z / Y to 10^-7
+    const uint32_t segments = (a.vocab + VF_SEGMENT - 1) / VF_SEGMENT;
+    double* const left = a.left + (size_t)seq * segments * 4;
+    for (uint32_t s = chunk * a.per_block + wave; s < min((chunk + 1) * a.per_block, segments); s += VF_WAVES) {
+        double sum = 0.0, others = 0.0, all = 0.0, all_others = 0.0;
+        segment(s, w, v);
+        if (residual) {
+#pragma unroll
+            for (int e = 0; e < VF_EACH; ++e) {
+                const bool some = w[e] > near * v[e];
+                sum += some ? w[e] : 0.0;
+                others += some ? v[e] : 0.0;
+                all += w[e];
+                all_others += v[e];
+            }
+            others = wave_sum_f64(others);
+            all = wave_sum_f64(all);
+            all_others = wave_sum_f64(all_others);
+        } else {
+#pragma unroll
+            for (int e = 0; e < VF_EACH; ++e) sum += w[e];
+        }
+        sum = wave_sum_f64(sum);
+        if (lane == 0) {
+            put_f64(left + 4 * s, sum);
+            if (residual) {
+                put_f64(left + 4 * s + 1, others);
+                put_f64(left + 4 * s + 2, all);
+                put_f64(left + 4 * s + 3, all_others);
+            }
+        }
     }
+    // the last thread block of a sequence to get here draws.  The sums are there before the count is raised.
+    __builtin_amdgcn_s_waitcnt(0);
+    asm volatile("" ::: "memory");
     __syncthreads();
-    if (!(st.total > 0.0)) {
-        if (tid == 0) a.next_token[seq] = -1;
+    if (wave != 0) return;
+    uint32_t arrived = 0;
+    if (lane == 0) {
+        arrived = __hip_atomic_fetch_add(&a.done[seq], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u;
+        if (arrived == a.chunks) __hip_atomic_store(&a.done[seq], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    if ((uint32_t)__builtin_amdgcn_readfirstlane((int)arrived) != a.chunks) return;
+
+    // 64 * GROUPS segments at a time, lane's are 64 apart
+    constexpr int GROUPS = 5;  // those of 151936 tokens
+    auto get = [&](uint32_t s0, int k, double (&x)[GROUPS]) {
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) x[g] = get_f64(left + 4 * (size_t)min(s0 + 64 * g + lane, segments - 1) + k);
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g)
+            if (s0 + 64 * g + lane >= segments) x[g] = 0.0;
+    };
+    bool both = residual;
+    double ratio = 0.0, total = 0.0;
+    if (residual) {
+        double z = 0.0, y = 0.0;
+        for (uint32_t s0 = 0; s0 < segments; s0 += 64 * GROUPS) {
+            double p[GROUPS], q[GROUPS];
+            get(s0, 2, p);
+            get(s0, 3, q);
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) {
+                z += p[g];
+                y += q[g];
+            }
+        }
+        z = wave_sum_f64(z);
+        y = wave_sum_f64(y);
+        ratio = y > 0.0 ? z / y : 0.0;
+    }
+    double m[GROUPS];
+    auto masses = [&](uint32_t s0) {
+        get(s0, residual && !both ? 2 : 0, m);
+        if (both) {
+            double q[GROUPS];
+            get(s0, 1, q);
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) m[g] = m[g] > ratio * q[g] ? m[g] - ratio * q[g] : 0.0;
+        }
+    };
+    for (;;) {
+        for (uint32_t s0 = 0; s0 < segments; s0 += 64 * GROUPS) {
+            masses(s0);
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) total += m[g];
+        }
+        total = wave_sum_f64(total);
+        if (total > 0.0 || !both) break;
+        both = false;  // nothing is left of the target's row beside the draft's: the row itself
+    }
+    if (!(total > 0.0)) {
+        if (lane == 0) a.next_token[seq] = -1;
         return;
     }
-    // 2. the piece, 3. the token
-    for (uint32_t i0 = 0; i0 < a.pieces; i0 += VF_THREADS) {
-        const double m = piece_mass(i0 + tid), upto = st.before + block_scan(m, st.scan[1]);
-        if (m > 0.0) {
-            atomicMax(&st.last[0], i0 + tid);
-            if (upto > st.border) atomicMin(&st.hit[0], i0 + tid);
+    const double border = st.u * total;
+    double before = 0.0;
+    uint32_t at = 0;
+    bool past = false;  // rounding may leave nothing past the border: then the last segment, and token, with any mass
+    for (uint32_t s0 = 0; s0 < segments && !past; s0 += 64 * GROUPS) {
+        if (segments > 64 * GROUPS) masses(s0);
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+            const double upto = before + wave_scan_f64(m[g]);
+            const uint64_t some = __ballot(m[g] > 0.0), over = __ballot(m[g] > 0.0 && upto > border);
+            if (past) continue;
+            past = over != 0;
+            if (past) {
+                const int hit = __builtin_ctzll(over);
+                at = s0 + 64 * g + hit;
+                before = readlane_f64(upto - m[g], hit);
+            } else {
+                if (some) at = s0 + 64 * g + 63 - __builtin_clzll(some);
+                before = readlane_f64(upto, 63);
+            }
         }
-        __syncthreads();
-        const uint32_t hit = st.hit[0];
-        if (hit == i0 + tid) st.before = upto - m;
-        if (hit == 0xffffffffu && tid == VF_THREADS - 1) st.before = upto;
-        __syncthreads();
-        if (hit != 0xffffffffu) break;
     }
-    const bool found = st.hit[0] != 0xffffffffu;
-    const uint32_t at = (found ? st.hit[0] : st.last[0]) * PIECE;
-    if (!found && tid == 0) st.border = INFINITY;  // rounding: the last token that has any
-    __syncthreads();
-    for (uint32_t x0 = at; x0 < at + PIECE; x0 += VF_THREADS) {
-        const uint32_t x = x0 + tid;
-        const double v = x < at + PIECE ? mass(x) : 0.0, upto = st.before + block_scan(v, st.scan[0]);
-        if (v > 0.0) {
-            atomicMax(&st.last[1], x);
-            if (upto > st.border) atomicMin(&st.hit[1], x);
-        }
-        __syncthreads();
-        if (tid == VF_THREADS - 1) st.before = upto;
-        __syncthreads();
-        if (st.hit[1] != 0xffffffffu) break;
+    segment(at, w, v);
+    int64_t choice = -1;
+    bool done = false;
+#pragma unroll
+    for (int e = 0; e < VF_EACH; ++e) {
+        double x = w[e];
+        if (both) x = x > ratio * v[e] ? x - ratio * v[e] : 0.0;
+        const double upto = before + wave_scan_f64(x);
+        const uint64_t some = __ballot(x > 0.0), over = past ? __ballot(x > 0.0 && upto > border) : 0;
+        if (!done && some) choice = (int64_t)at * VF_SEGMENT + 64 * e + (over ? __builtin_ctzll(over) : 63 - __builtin_clzll(some));
+        done = done || over != 0;
+        before = readlane_f64(upto, 63);
     }
-    if (tid == 0) a.next_token[seq] = st.hit[1] != 0xffffffffu ? st.hit[1] : st.last[1];
+    if (lane == 0) a.next_token[seq] = choice;
 }
 
 struct KeepArgs {
@@ -550,9 +610,9 @@ __global__ __launch_bounds__(KEEP_THREADS) void tree_keep_kernel(const KeepArgs 
 static uint32_t verify_each(uint64_t rows, uint32_t vocab) { return rows * ((vocab + 1023) / 1024) <= 12288 ? 16 : 64; }
 
 struct VerifySizes {
-    uint32_t each, pieces, chunks;
+    uint32_t each, pieces, chunks, per_block;
     uint64_t rows;
-    size_t done, top, sum, left, end;
+    size_t done, part, left, end;
 };
 
 static VerifySizes verify_sizes(uint32_t n_seq, uint32_t n, uint32_t vocab, bool drawn) {
@@ -560,12 +620,15 @@ static VerifySizes verify_sizes(uint32_t n_seq, uint32_t n, uint32_t vocab, bool
     s.rows = (uint64_t)n_seq * n + (drawn ? (uint64_t)n_seq * (n - 1) : 0);
     s.each = verify_each(s.rows, vocab);
     s.pieces = (vocab + s.each * 64 - 1) / (s.each * 64);
-    s.chunks = drawn ? (vocab + VF_THREADS * 8 - 1) / (VF_THREADS * 8) : 1;
+    // a segment a wave, more of them where the sequences' thread blocks would be more than the chip's CUs
+    const uint64_t segments = (vocab + VF_SEGMENT - 1) / VF_SEGMENT, blocks = (segments + VF_WAVES - 1) / VF_WAVES;
+    const uint64_t turns = (n_seq * blocks + 255) / 256 < blocks ? (n_seq * blocks + 255) / 256 : blocks;
+    s.per_block = (uint32_t)turns * VF_WAVES;
+    s.chunks = (uint32_t)((segments + s.per_block - 1) / s.per_block);
     s.done = 0;  // as many for every shape of up to 16384 sequences, so that calls of several shapes may share them
-    s.top = ((size_t)(n_seq > 16384 ? n_seq : 16384) * 4 + 15) / 16 * 16;
-    s.sum = s.top + (size_t)s.rows * s.pieces * 8;
-    s.left = s.sum + (size_t)s.rows * s.pieces * 8;
-    s.end = s.left + (drawn ? (size_t)n_seq * s.chunks * 8 : 0);
+    s.part = ((size_t)(n_seq > 16384 ? n_seq : 16384) * 4 + 15) / 16 * 16;
+    s.left = s.part + (size_t)s.rows * s.pieces * 8;
+    s.end = s.left + (size_t)n_seq * segments * 32;
     return s;
 }
 
@@ -616,30 +679,27 @@ extern "C" int t2h_tree_verify(const void* logits, uint64_t row_stride, const vo
     a.vocab = vocab;
     a.pieces = s.pieces;
     a.chunks = s.chunks;
+    a.per_block = s.per_block;
     uint8_t* const ws = reinterpret_cast<uint8_t*>(workspace);
     a.done = reinterpret_cast<uint32_t*>(ws + s.done);
-    a.part_top = reinterpret_cast<uint2*>(ws + s.top);
-    a.part_sum = reinterpret_cast<double*>(ws + s.sum);
+    a.part = reinterpret_cast<uint2*>(ws + s.part);
     a.left = reinterpret_cast<double*>(ws + s.left);
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    auto launch = [&](auto bf16, auto each) {
-        constexpr bool BF16 = decltype(bf16)::value;
-        constexpr int E = decltype(each)::value;
-        hipLaunchKernelGGL((verify_rows_kernel<BF16, E>), dim3((uint32_t)grid), dim3(256), 0, st, a);
-        if (drawn)
-            hipLaunchKernelGGL((verify_finish_kernel<BF16, E, true>), dim3((uint32_t)finish), dim3(VF_THREADS), 0, st, a);
-        else
-            hipLaunchKernelGGL((verify_finish_kernel<BF16, E, false>), dim3((uint32_t)finish), dim3(VF_THREADS), 0, st, a);
+    auto launch = [&](auto bf16, auto each, auto with_draft) {
+        constexpr bool BF16 = decltype(bf16)::value, DRAWN = decltype(with_draft)::value;
+        hipLaunchKernelGGL((verify_rows_kernel<BF16, decltype(each)::value>), dim3((uint32_t)grid), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((verify_finish_kernel<BF16, DRAWN>), dim3((uint32_t)finish), dim3(VF_THREADS), 0, st, a);
     };
-    using std::integral_constant;
-    const bool bf16 = dtype == T2H_DTYPE_BF16;
-    if (s.each == 16) {
-        if (bf16) launch(integral_constant<bool, true>{}, integral_constant<int, 16>{});
-        else launch(integral_constant<bool, false>{}, integral_constant<int, 16>{});
-    } else {
-        if (bf16) launch(integral_constant<bool, true>{}, integral_constant<int, 64>{});
-        else launch(integral_constant<bool, false>{}, integral_constant<int, 64>{});
-    }
+    auto with_each = [&](auto bf16, auto with_draft) {
+        if (s.each == 16) launch(bf16, std::integral_constant<int, 16>{}, with_draft);
+        else launch(bf16, std::integral_constant<int, 64>{}, with_draft);
+    };
+    auto with_type = [&](auto with_draft) {
+        if (dtype == T2H_DTYPE_BF16) with_each(std::true_type{}, with_draft);
+        else with_each(std::false_type{}, with_draft);
+    };
+    if (drawn) with_type(std::true_type{});
+    else with_type(std::false_type{});
     T2H_LAUNCH_CHECK();
     return T2H_OK;
 }
