@@ -15,15 +15,15 @@ typedef float ta_f32x4 __attribute__((ext_vector_type(4)));
 constexpr int TA_D = 128;
 constexpr int TA_MAX_GROUP = 16;
 constexpr int TA_ROW_BYTES = TA_D * 2;
+constexpr int TP_NODES = 16, TP_GROUPS = TREE_MAX / TP_NODES;  // nodes of a thread block that writes K and V rows
 constexpr float TA_RESCALE = 8.0f;  // log2 headroom of the lazily updated running maximum
 
 // What a thread block of the attention works on: tiles [tile0, tile1) of a sequence's tokens.
 struct TreeUnit {
     int seq;  // -1: none
     int tile0, tile1;
-    int slot;        // where its part goes, -1: it is the sequence's only one
-    int len, count;  // cached tokens, nodes
-    int pad0, pad1;
+    int len, count;          // cached tokens, nodes
+    int first, parts, part;  // where the sequence's parts begin, how many they are, and which this is
 };
 
 struct TreeAttnArgs {
@@ -49,15 +49,16 @@ struct TreeAttnArgs {
     uint16_t* ql;
     uint64_t* line;    // [n_seq][n] sets of seen nodes
     uint16_t* vt;      // [n_seq][nk][n + 1][128] the nodes' values; zeros where there is none or it is not finite
-    uint32_t* broken;  // [n_seq][nk] whether a node's value is not finite
-    uint64_t* which;   // [n_seq][nk][128][3] then: the nodes whose value in a dim is NaN, infinite, -infinite
+    uint32_t* broken;  // [n_seq][nk][TP_GROUPS] whether a value of 16 nodes is not finite
+    uint64_t* which;   // [n_seq][nk][TP_GROUPS][128][3] then: the nodes whose value in a dim is NaN, infinite, -infinite
+    uint32_t* done;    // [n_seq][nk] units that have left their parts; zero between calls
     TreeUnit* units;   // [n_units]
     int2* of_seq;      // [n_seq] first part, parts
     float* part_ml;    // [n_units * nk][rows][2] log2 maximum, sum
     float* part_o;     // [n_units * nk][rows][128]
     uint32_t n_units, row_tiles, rows;  // rows: of a KV head, in whole tiles
     uint32_t slots;    // units a KV head that fill the chip
-    uint32_t keys, least;  // tokens a tile; the least tiles a unit
+    uint32_t keys, least, extra;  // tokens a tile; the least tiles a unit; what a unit costs besides, in tiles
     uint32_t kv_blocks, q_blocks;
 };
 
@@ -68,29 +69,64 @@ struct TreeAttnArgs {
 
 constexpr int TP_HEADS = 4;  // q heads a wave
 
+// Tiles that a sequence's cached tokens and nodes fill; none where there are no nodes.
+__device__ __forceinline__ uint32_t tree_tiles(const TreeAttnArgs& a, uint32_t i, int& len, int& count) {
+    len = a.lengths[i];
+    count = tree_count_at(a.counts, i, a.n, len, a.s_cap);
+    if (count == 0) len = 0;
+    return count > 0 ? ((uint32_t)(len + count) + a.keys - 1) / a.keys : 0u;
+}
+
+__device__ __forceinline__ uint32_t wave_total_u32(uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)wave_scan_u32(v), 63); }
+
+// Tiles a unit: the fewest that leave no more units than `turns` times what the chip holds at once, for the number of turns that
+// ends first; a unit costs a.extra tiles' time besides its own.  Where the sequences alone are more than that, what would be
+// one turn's share.  `mine`: tiles of sequence `lane`, the others' are looked up.
+__device__ uint32_t tree_chunk(const TreeAttnArgs& a, uint32_t mine) {
+    const uint32_t lane = threadIdx.x & 63;
+    int len, count;
+    uint32_t total = lane < a.n_seq ? mine : 0;
+    for (uint32_t i = lane + 64; i < a.n_seq; i += 64) total += tree_tiles(a, i, len, count);
+    total = wave_total_u32(total);
+    uint32_t chunk = (total + a.slots - 1) / a.slots, best = 0xffffffffu;
+    for (uint32_t turns = (a.n_seq + a.slots - 1) / a.slots; turns <= 4; ++turns) {
+        const uint32_t most = turns * a.slots;
+        uint32_t c = (total + most - 1) / most;
+        c = c > a.least ? c : a.least;
+        for (;;) {
+            uint32_t units = lane < a.n_seq ? (mine ? (mine + c - 1) / c : 1u) : 0u;
+            for (uint32_t i = lane + 64; i < a.n_seq; i += 64) {
+                const uint32_t t = tree_tiles(a, i, len, count);
+                units += t ? (t + c - 1) / c : 1u;
+            }
+            units = wave_total_u32(units);
+            if (units <= most) break;
+            c += c * (units - most) / units + 1;  // (there is such a c: every sequence one unit)
+        }
+        if (turns * (c + a.extra) < best) {
+            best = turns * (c + a.extra);
+            chunk = c;
+        }
+        if (c == a.least) break;
+    }
+    return chunk > a.least ? chunk : a.least;
+}
+
+// Units of a whole chunk come first, the sequences' last, shorter ones behind them, so that what the chip ends with is short.
 __device__ void tree_table(const TreeAttnArgs& a) {
     const uint32_t lane = threadIdx.x;
     if (lane >= 64) return;
-    auto tiles_of = [&](uint32_t i, int& len, int& count) {
-        len = a.lengths[i];
-        count = tree_count_at(a.counts, i, a.n, len, a.s_cap);
-        return count > 0 ? ((uint32_t)(len + count) + a.keys - 1) / a.keys : 0u;
-    };
-    uint32_t total = 0;
-    int len, count;
-    for (uint32_t i = lane; i < a.n_seq; i += 64) total += tiles_of(i, len, count);
-    total = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan_u32(total), 63);
-    uint32_t chunk = (total + a.slots - 1) / a.slots;
-    chunk = chunk > a.least ? chunk : a.least;
+    int len = 0, count = 0;
+    const uint32_t chunk = tree_chunk(a, lane < a.n_seq ? tree_tiles(a, lane, len, count) : 0u);
     uint32_t fulls = 0;
-    for (uint32_t i = lane; i < a.n_seq; i += 64) fulls += tiles_of(i, len, count) / chunk;
-    fulls = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan_u32(fulls), 63);
+    for (uint32_t i = lane; i < a.n_seq; i += 64) fulls += tree_tiles(a, i, len, count) / chunk;
+    fulls = wave_total_u32(fulls);
     uint32_t full_at = 0, rest_at = fulls, part_at = 0;
     for (uint32_t base = 0; base < a.n_seq; base += 64) {
         const uint32_t i = base + lane;
         uint32_t tiles = 0;
         len = count = 0;
-        if (i < a.n_seq) tiles = tiles_of(i, len, count);
+        if (i < a.n_seq) tiles = tree_tiles(a, i, len, count);
         const uint32_t full = tiles / chunk, rest = i < a.n_seq && (tiles % chunk || tiles == 0) ? 1u : 0u;
         const uint32_t full_up = wave_scan_u32(full), rest_up = wave_scan_u32(rest);
         if (i < a.n_seq) {
@@ -100,11 +136,12 @@ __device__ void tree_table(const TreeAttnArgs& a) {
             u.seq = (int)i;
             u.len = len;
             u.count = count;
-            u.pad0 = u.pad1 = 0;
+            u.first = (int)first;
+            u.parts = (int)parts;
             for (uint32_t p = 0; p < parts; ++p) {
                 u.tile0 = (int)(p * chunk);
                 u.tile1 = (int)min(p * chunk + chunk, tiles);
-                u.slot = parts == 1 ? -1 : (int)(first + p);
+                u.part = (int)p;
                 a.units[p < full ? full_at + full_up - full + p : rest_at + rest_up - rest] = u;
             }
         }
@@ -115,55 +152,126 @@ __device__ void tree_table(const TreeAttnArgs& a) {
     for (uint32_t u = rest_at + lane; u < a.n_units; u += 64) a.units[u].seq = -1;
 }
 
+// The same unit by its number, worked out by one wave.
+__device__ bool tree_find(const TreeAttnArgs& a, uint32_t unit, TreeUnit& u) {
+    const uint32_t lane = threadIdx.x & 63;
+    if (a.n_seq == 1) {
+        const uint32_t tiles = tree_tiles(a, 0, u.len, u.count);
+        const uint32_t share = (tiles + a.slots - 1) / a.slots, chunk = share > a.least ? share : a.least;
+        u.seq = u.first = 0;
+        u.part = (int)unit;
+        u.parts = tiles ? (int)((tiles + chunk - 1) / chunk) : 1;
+        u.tile0 = (int)(unit * chunk);
+        u.tile1 = (int)min(unit * chunk + chunk, tiles);
+        return (int)unit < u.parts;
+    }
+    int len = 0, count = 0;
+    const uint32_t mine = lane < a.n_seq ? tree_tiles(a, lane, len, count) : 0u;
+    const uint32_t chunk = tree_chunk(a, mine);
+    uint32_t fulls = lane < a.n_seq ? mine / chunk : 0u;
+    int l, c;
+    for (uint32_t i = lane + 64; i < a.n_seq; i += 64) fulls += tree_tiles(a, i, l, c) / chunk;
+    fulls = wave_total_u32(fulls);
+    uint32_t full_at = 0, rest_at = 0;
+    for (uint32_t base = 0; base < a.n_seq; base += 64) {
+        const uint32_t i = base + lane;
+        uint32_t tiles = mine;
+        if (base) tiles = i < a.n_seq ? tree_tiles(a, i, len, count) : 0u;
+        const uint32_t full = tiles / chunk, rest = i < a.n_seq && (tiles % chunk || tiles == 0) ? 1u : 0u;
+        const uint32_t full_up = full_at + wave_scan_u32(full), rest_up = rest_at + wave_scan_u32(rest);
+        const bool whole = unit < fulls;
+        const uint64_t hit = whole ? __ballot(unit >= full_up - full && unit < full_up) : __ballot(rest && unit - fulls == rest_up - 1);
+        if (hit) {
+            const int at = __builtin_ctzll(hit);
+            u.seq = (int)base + at;
+            u.len = __builtin_amdgcn_readlane(len, at);
+            u.count = __builtin_amdgcn_readlane(count, at);
+            const uint32_t first = (uint32_t)__builtin_amdgcn_readlane((int)(full_up - full), at),
+                           n_full = (uint32_t)__builtin_amdgcn_readlane((int)full, at),
+                           n_rest = (uint32_t)__builtin_amdgcn_readlane((int)rest, at),
+                           all = (uint32_t)__builtin_amdgcn_readlane((int)tiles, at);
+            u.first = (int)(first + (uint32_t)__builtin_amdgcn_readlane((int)(rest_up - rest), at));
+            u.parts = (int)(n_full + n_rest);
+            u.part = (int)(whole ? unit - first : n_full);
+            u.tile0 = u.part * (int)chunk;
+            u.tile1 = (int)min((uint32_t)u.tile0 + chunk, all);
+            return true;
+        }
+        full_at = (uint32_t)__builtin_amdgcn_readlane((int)full_up, 63);
+        rest_at = (uint32_t)__builtin_amdgcn_readlane((int)rest_up, 63);
+    }
+    return false;
+}
+
 __device__ __forceinline__ uint64_t readlane64(uint64_t x, int lane) {
     return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32 |
            (uint32_t)__builtin_amdgcn_readlane((int)x, lane);
 }
 
+// Which nodes' bf16 values, two a lane, are NaN, infinite, -infinite; those become zeros.
+__device__ __forceinline__ void tree_take_broken(uint32_t& v, int node, uint64_t (&bad)[2][3]) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const uint32_t x = v >> (16 * e) & 0xffffu;
+        if ((x & 0x7f80u) == 0x7f80u) {
+            bad[e][x & 0x7fu ? 0 : x >> 15 ? 2 : 1] |= 1ull << node;
+            v &= e ? 0xffffu : 0xffff0000u;
+        }
+    }
+}
+
+// 16 nodes of a (sequence, KV head), four a wave.
 __device__ void tree_kv_rows(const TreeAttnArgs& a, uint32_t block) {
     __shared__ uint64_t found[4][TA_D][3];
+    constexpr int EACH = TP_NODES / 4;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t seq = block / a.nk, h = block % a.nk;
+    const uint32_t groups = (a.n + TP_NODES - 1) / TP_NODES, group = block % groups, head = block / groups;
+    const uint32_t seq = head / a.nk, h = head % a.nk;
+    const int i0 = (int)group * TP_NODES + wave * EACH;
+    float k0[EACH], k1[EACH], v0[EACH], v1[EACH];
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+        const size_t row = (size_t)seq * a.n + min(i0 + e, (int)a.n - 1);
+        const float* kx = a.k_new + row * a.k_row + (size_t)h * TA_D + lane;
+        const float* vx = a.v_new + row * a.v_row + (size_t)h * TA_D + 2 * lane;
+        k0[e] = kx[0];
+        k1[e] = kx[64];
+        v0[e] = vx[0];
+        v1[e] = vx[1];
+    }
     const int len = a.lengths[seq];
     const int count = tree_count_at(a.counts, seq, a.n, len, a.s_cap);
     const uint64_t lines = tree_lineage(a.parents, seq, a.n, count);
     const bool has_w = a.k_norm_w != nullptr;
     const float w0 = has_w ? a.k_norm_w[lane] : 1.0f, w1 = has_w ? a.k_norm_w[lane + 64] : 1.0f;
     const double turns = a.rope ? rope_turns(lane, a.log2_theta) : 0.0;
-    uint32_t* const vt = reinterpret_cast<uint32_t*>(a.vt + (size_t)block * (a.n + 1) * TA_D);
+    uint32_t* const vt = reinterpret_cast<uint32_t*>(a.vt + (size_t)head * (a.n + 1) * TA_D);
     uint64_t bad[2][3] = {{0, 0, 0}, {0, 0, 0}};
-    if (wave == 3) vt[a.n * 64 + lane] = 0u;
-    for (int i = wave; i < (int)a.n; i += 4) {
+    if (group == 0 && wave == 3) vt[a.n * 64 + lane] = 0u;
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+        const int i = i0 + e;
+        if (i >= (int)a.n) break;
         const uint64_t line = readlane64(lines, i);
         if (line == 0) {
             vt[i * 64 + lane] = 0u;
             continue;
         }
-        const size_t row = (size_t)seq * a.n + i, slot = ((size_t)len + i) * a.nk + h;
-        const float* kx = a.k_new + row * a.k_row + (size_t)h * TA_D + lane;
-        const float* vx = a.v_new + row * a.v_row + (size_t)h * TA_D + 2 * lane;
-        const float k0 = kx[0], k1 = kx[64], v0 = vx[0], v1 = vx[1];
+        const size_t slot = ((size_t)len + i) * a.nk + h;
         float cs = 1.0f, sn = 0.0f, r0, r1;
         if (a.rope) rope_at(turns, len + __popcll(line) - 1, cs, sn);
-        q8_norm_rope(k0, k1, has_w, w0, w1, a.eps, cs, sn, r0, r1);
+        q8_norm_rope(k0[e], k1[e], has_w, w0, w1, a.eps, cs, sn, r0, r1);
         uint16_t* const y = a.k_cache + seq * a.k_seq + slot * TA_D + lane;
         y[0] = (uint16_t)f32_to_bf16_bits(r0);
         y[64] = (uint16_t)f32_to_bf16_bits(r1);
-        uint32_t v = pack_bf16x2(v0, v1);
+        uint32_t v = pack_bf16x2(v0[e], v1[e]);
         reinterpret_cast<uint32_t*>(a.v_cache + seq * a.v_seq + slot * TA_D)[lane] = v;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const uint32_t x = v >> (16 * e) & 0xffffu;
-            if ((x & 0x7f80u) == 0x7f80u) {
-                bad[e][x & 0x7fu ? 0 : x >> 15 ? 2 : 1] |= 1ull << i;
-                v &= e ? 0xffffu : 0xffff0000u;
-            }
-        }
+        tree_take_broken(v, i, bad);
         vt[i * 64 + lane] = v;
     }
     const bool any = (bad[0][0] | bad[0][1] | bad[0][2] | bad[1][0] | bad[1][1] | bad[1][2]) != 0;
     const int all = __syncthreads_or(any);
-    if (threadIdx.x == 0) a.broken[block] = all ? 1u : 0u;
+    if (threadIdx.x == 0) a.broken[head * TP_GROUPS + group] = all ? 1u : 0u;
     if (!all) return;
 #pragma unroll
     for (int e = 0; e < 2; ++e)
@@ -172,7 +280,7 @@ __device__ void tree_kv_rows(const TreeAttnArgs& a, uint32_t block) {
     __syncthreads();
     for (int i = threadIdx.x; i < TA_D * 3; i += 256) {
         const int d = i / 3, k = i % 3;
-        a.which[(size_t)block * TA_D * 3 + i] = found[0][d][k] | found[1][d][k] | found[2][d][k] | found[3][d][k];
+        a.which[((size_t)head * TP_GROUPS + group) * TA_D * 3 + i] = found[0][d][k] | found[1][d][k] | found[2][d][k] | found[3][d][k];
     }
 }
 
@@ -231,6 +339,14 @@ __global__ __launch_bounds__(256) void tree_rows_kernel(const TreeAttnArgs a) {
 // 16-byte pieces of a row lie in LDS at their place XOR f(row), so that neither product's reads meet in a bank: f is the
 // row's low four bits for keys (16 rows, one piece each) and twice two of them for values (4 rows, 4 pieces each).
 
+// A sum with the values that were zeros in the products.
+__device__ __forceinline__ float tree_put_broken(float x, uint64_t nan, uint64_t inf, uint64_t minus) {
+    if (nan) x += __uint_as_float(0x7fc00000u);
+    if (inf) x += INFINITY;
+    if (minus) x -= INFINITY;
+    return x;
+}
+
 template <int NWR, int NWK, int STAGES>
 struct TreeShape {
     static constexpr int WAVES = NWR * NWK, KEYS = 32 * NWK, PER = 16 / NWR;  // loads of 1 KiB a wave and tile
@@ -244,7 +360,6 @@ template <int NWR, int NWK, int STAGES>
 __global__ __launch_bounds__(NWR * NWK * 64) __attribute__((amdgpu_waves_per_eu(1, NWR * NWK / 4)))
 void tree_attn_kernel(const TreeAttnArgs a) {
     using S = TreeShape<NWR, NWK, STAGES>;
-    constexpr bool OWN = NWR == 1;  // a wave reads only what it has loaded itself
     __shared__ __align__(1024) uint8_t lds[S::LDS];
     __shared__ float wml[S::WAVES][32][2];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
@@ -346,22 +461,12 @@ void tree_attn_kernel(const TreeAttnArgs a) {
         const int vr = 32 * wk + 4 * half + (n16 >> 2), vpiece = 2 * ((lane >> 4) & 1) + ((n16 & 3) >> 1);
         const uint32_t va = S::KEYS * TA_ROW_BYTES + (uint32_t)vr * TA_ROW_BYTES + 8 * (n16 & 1);
         for (int it = 0; it < tiles; ++it) {
-            if constexpr (OWN) {
-                if (it + 1 < tiles) {
-                    load(it + 1);
-                    wait_vm<S::PER>();
-                } else {
-                    wait_vm<0>();
-                }
-                asm volatile("" ::: "memory");
-            } else {
-                const int left = tiles - 1 - it;
-                if (left >= STAGES - 2) wait_vm<S::PER * (STAGES - 2)>();
-                else wait_vm<0>();
-                wait_lgkm0();
-                wave_barrier();
-                if (it + STAGES - 1 < tiles) load(it + STAGES - 1);
-            }
+            const int left = tiles - 1 - it;
+            if (left >= STAGES - 2) wait_vm<S::PER * (STAGES - 2)>();
+            else wait_vm<0>();
+            wait_lgkm0();
+            wave_barrier();
+            if (it + STAGES - 1 < tiles) load(it + STAGES - 1);
             if (busy) {
                 const uint8_t* const stage = &lds[(it % STAGES) * S::STAGE];
                 ta_f32x16 s;
@@ -423,10 +528,6 @@ void tree_attn_kernel(const TreeAttnArgs a) {
                     }
                 }
             }
-            if constexpr (OWN) {  // the buffer is read before it is loaded again
-                wait_lgkm0();
-                asm volatile("" ::: "memory");
-            }
         }
     }
 
@@ -446,10 +547,12 @@ void tree_attn_kernel(const TreeAttnArgs a) {
             *reinterpret_cast<ta_f32x4*>(os + (wave * 32 + (lane & 31)) * S::OROW + 32 * db + 8 * g + 4 * half) =
                 ta_f32x4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
     __syncthreads();
-    const bool whole = u.slot < 0;
+    const bool whole = u.parts == 1;
     // values that are not finite were zeros in the products; they come to the rows that see them here, in the nodes' own unit
     const int node0 = max(u.tile0 * S::KEYS - len, 0), node1 = min(u.tile1 * S::KEYS - len, TREE_MAX);
-    const bool broken = a.broken[head] != 0 && node1 > node0;
+    uint32_t broken = 0;  // groups of nodes
+    if (node1 > node0)
+        for (uint32_t g = 0; g < (a.n + TP_NODES - 1) / TP_NODES; ++g) broken |= (a.broken[head * TP_GROUPS + g] & 1u) << g;
     const uint64_t here = broken ? (~0ull >> (TREE_MAX - (node1 - node0))) << node0 : 0;
     const int all = (int)a.n * group;  // rows of the output, nodes or not
     for (int i = tid; i < NWR * 32 * 32; i += S::WAVES * 64) {
@@ -469,14 +572,10 @@ void tree_attn_kernel(const TreeAttnArgs a) {
         }
         const int node = at / group;
         const uint64_t line = a.line[(size_t)u.seq * a.n + node];
-        if (broken) {
+        for (uint32_t rest = broken; rest; rest &= rest - 1) {
+            const uint64_t* const w = a.which + ((head * TP_GROUPS + __builtin_ctz(rest)) * TA_D + d) * 3;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint64_t* const w = a.which + (head * TA_D + d + e) * 3;
-                if (line & here & w[0]) sum[e] += __uint_as_float(0x7fc00000u);
-                if (line & here & w[1]) sum[e] += INFINITY;
-                if (line & here & w[2]) sum[e] -= INFINITY;
-            }
+            for (int e = 0; e < 4; ++e) sum[e] = tree_put_broken(sum[e], line & here & w[3 * e], line & here & w[3 * e + 1], line & here & w[3 * e + 2]);
         }
         if (whole) {
             const float inv = line ? 1.0f / L : 0.0f;
@@ -484,15 +583,15 @@ void tree_attn_kernel(const TreeAttnArgs a) {
             if (line) y = make_uint2(pack_bf16x2(sum[0] * inv, sum[1] * inv), pack_bf16x2(sum[2] * inv, sum[3] * inv));
             *reinterpret_cast<uint2*>(a.out + (((size_t)u.seq * a.n + node) * a.nh + h * group + at % group) * TA_D + d) = y;
         } else {
-            const size_t part = ((size_t)u.slot * a.nk + h) * a.rows + at;
+            const size_t part = ((size_t)(u.first + u.part) * a.nk + h) * a.rows + at;
             *reinterpret_cast<ta_f32x4*>(a.part_o + part * TA_D + d) = sum;
             if (d == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * part) = make_float2(M, L);
         }
     }
 }
 
-// Joins the units of a sequence, a wave a row.
-constexpr int TJ_BATCH = 8;
+// Joins the units of a sequence, a wave a row: a lane holds a unit's maximum and sum, and two dims.
+constexpr int TJ_BATCH = 16;
 
 __global__ __launch_bounds__(256) void tree_join_kernel(const TreeAttnArgs a) {
     const int lane = threadIdx.x & 63;
@@ -500,34 +599,449 @@ __global__ __launch_bounds__(256) void tree_join_kernel(const TreeAttnArgs a) {
     if (unit >= a.n_seq * a.n * a.nh) return;
     const uint32_t seq = unit / (a.n * a.nh), i = unit / a.nh % a.n, head = unit % a.nh, h = head / a.group;
     const int2 parts = a.of_seq[seq];
+    const uint64_t line = a.line[(size_t)seq * a.n + i];
     if (parts.y <= 1) return;
     uint32_t* const out = reinterpret_cast<uint32_t*>(a.out + ((size_t)unit) * TA_D);
-    if (a.line[(size_t)seq * a.n + i] == 0) {
+    if (line == 0) {
         out[lane] = 0u;
         return;
     }
     const size_t r = (size_t)i * a.group + head % a.group;
+    auto at = [&](int p) { return ((size_t)(parts.x + min(p, parts.y - 1)) * a.nk + h) * a.rows + r; };
     float M = -INFINITY, L = 0.0f, o0 = 0.0f, o1 = 0.0f;
-    for (int p0 = 0; p0 < parts.y; p0 += TJ_BATCH) {
-        float2 ml[TJ_BATCH], x[TJ_BATCH];
+    for (int p0 = 0; p0 < parts.y; p0 += 64) {
+        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * at(p0 + lane));
+        float2 x[TJ_BATCH];
+        auto load = [&](int p) {
 #pragma unroll
-        for (int p = 0; p < TJ_BATCH; ++p) {
-            const size_t at = ((size_t)(parts.x + min(p0 + p, parts.y - 1)) * a.nk + h) * a.rows + r;
-            ml[p] = *reinterpret_cast<const float2*>(a.part_ml + 2 * at);
-            x[p] = *reinterpret_cast<const float2*>(a.part_o + at * TA_D + 2 * lane);
-        }
+            for (int e = 0; e < TJ_BATCH; ++e) x[e] = *reinterpret_cast<const float2*>(a.part_o + at(p + e) * TA_D + 2 * lane);
+        };
+        load(p0);
+        const float m = p0 + lane < parts.y ? ml.x : -INFINITY;
+        const float now = fmaxf(M, wave_max(m)), msub = now == -INFINITY ? 0.0f : now;
+        const float keep = __builtin_amdgcn_exp2f(M - msub), f = p0 + lane < parts.y ? __builtin_amdgcn_exp2f(m - msub) : 0.0f;
+        L = fmaf(L, keep, wave_sum(p0 + lane < parts.y ? f * ml.y : 0.0f));
+        o0 *= keep;
+        o1 *= keep;
+        M = now;
+        const int end = min(parts.y - p0, 64);
+        for (int p = 0; p < end; p += TJ_BATCH) {
+            if (p) load(p0 + p);
 #pragma unroll
-        for (int p = 0; p < TJ_BATCH; ++p) {
-            if (p0 + p >= parts.y) break;
-            const float now = fmaxf(M, ml[p].x), msub = now == -INFINITY ? 0.0f : now;
-            const float keep = __builtin_amdgcn_exp2f(M - msub), f = __builtin_amdgcn_exp2f(ml[p].x - msub);
-            L = fmaf(L, keep, f * ml[p].y);
-            o0 = fmaf(o0, keep, x[p].x * f);
-            o1 = fmaf(o1, keep, x[p].y * f);
-            M = now;
+            for (int e = 0; e < TJ_BATCH; ++e) {
+                if (p + e >= end) break;
+                const float fe = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), (p + e) & 63));
+                o0 = fmaf(x[e].x, fe, o0);
+                o1 = fmaf(x[e].y, fe, o1);
+            }
         }
     }
     out[lane] = pack_bf16x2(o0 / L, o1 / L);
+}
+
+// ------------------------------------------------------------------------------------- the attention of few rows --
+//
+// Up to 32 rows a KV head: all in one launch.  Every thread block norms and rotates the head's queries itself, while its first
+// tiles are on their way, and finds its unit in the lengths; the one that holds the nodes also brings their K and V into the
+// cache and reads them from LDS.  4 waves, 32 keys each, that wait for nothing but their own loads in the loop.  The last unit
+// of a (sequence, KV head) to leave its part joins them: parts go past the caches that the chip's parts do not share (agent
+// scope), and are there before the count is raised.
+
+constexpr int TF_WAVES = 4, TF_ROWS = 32;
+constexpr int TF_EACH = TF_ROWS / TF_WAVES;  // rows, and nodes, a wave
+constexpr int TF_QROW = TA_D + 8;            // bf16 row of queries in LDS, padded
+
+typedef uint32_t ta_u32x4 __attribute__((ext_vector_type(4)));
+constexpr int TF_AGENT = 16;  // cache policy of buffer loads and stores: agent scope
+
+__global__ __launch_bounds__(TF_WAVES * 64) __attribute__((amdgpu_waves_per_eu(1, 1))) void tree_few_kernel(const TreeAttnArgs a) {
+    using S = TreeShape<1, TF_WAVES, 2>;
+    __shared__ __align__(1024) uint8_t lds[S::LDS];
+    __shared__ __align__(16) uint8_t fresh[2][(TF_ROWS + 1) * TA_ROW_BYTES];  // the nodes' keys and values, and a row of zeros
+    __shared__ float wml[TF_WAVES][32][2];
+    __shared__ uint32_t found[TA_D][3], arrived;
+    // before the loop the second stage holds the queries' two terms and the nodes' angles
+    uint16_t* const qs = reinterpret_cast<uint16_t*>(lds + S::STAGE);
+    float2* const angles = reinterpret_cast<float2*>(lds + S::STAGE + 2 * TF_ROWS * TF_QROW * 2);
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t unit = blockIdx.x / a.nk, h = blockIdx.x % a.nk;
+    const int group = (int)a.group, all = (int)a.n * group;  // rows of the head, nodes or not
+    TreeUnit u;
+    float x0[TF_EACH], x1[TF_EACH];
+    auto load_q = [&](uint32_t seq) {
+#pragma unroll
+        for (int e = 0; e < TF_EACH; ++e) {
+            const int r = min(wave + TF_WAVES * e, all - 1);
+            const float* x = a.q + ((size_t)seq * a.n + r / group) * a.q_row + (size_t)(h * group + r % group) * TA_D + lane;
+            x0[e] = x[0];
+            x1[e] = x[64];
+        }
+    };
+    if (a.n_seq == 1) load_q(0);  // (they do not wait for the lengths)
+    if (!tree_find(a, unit, u)) return;  // every wave of the thread block finds the same
+    const uint32_t seq = (uint32_t)u.seq;
+    if (a.n_seq != 1) load_q(seq);
+    const int len = u.len, count = u.count, rows = count * group, tiles = u.tile1 - u.tile0;
+    const size_t head = (size_t)seq * a.nk + h;
+    const bool has_nodes = u.tile1 * S::KEYS > len && count > 0;
+    const uint16_t* const kb = a.k_cache + seq * a.k_seq + (size_t)h * TA_D;
+    const uint16_t* const vb = a.v_cache + seq * a.v_seq + (size_t)h * TA_D;
+    const size_t step = (size_t)a.nk * TA_D;
+    const bool has_w = a.q_norm_w != nullptr;
+    const float qw0 = has_w ? a.q_norm_w[lane] : 1.0f, qw1 = has_w ? a.q_norm_w[lane + 64] : 1.0f;
+    float k0[TF_EACH], k1[TF_EACH], v0[TF_EACH], v1[TF_EACH], kw0 = 1.0f, kw1 = 1.0f;
+    if (has_nodes) {
+#pragma unroll
+        for (int e = 0; e < TF_EACH; ++e) {
+            const size_t row = (size_t)seq * a.n + min(wave + TF_WAVES * e, (int)a.n - 1);
+            const float* kx = a.k_new + row * a.k_row + (size_t)h * TA_D + lane;
+            const float* vx = a.v_new + row * a.v_row + (size_t)h * TA_D + 2 * lane;
+            k0[e] = kx[0];
+            k1[e] = kx[64];
+            v0[e] = vx[0];
+            v1[e] = vx[1];
+        }
+        if (has_w) {
+            kw0 = a.k_norm_w[lane];
+            kw1 = a.k_norm_w[lane + 64];
+        }
+    }
+    const uint64_t lines = tree_lineage(a.parents, seq, a.n, count);
+
+    const uint32_t base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)&lds[0]);
+    constexpr int HALF = S::PER / 2;  // loads of 4 rows: a wave's 32 keys, and values
+    const int q0 = wave * HALF, lr = lane >> 4, lp = lane & 15;
+    const int kcol = 8 * (lp ^ lr), vcol = 8 * (lp ^ (lr << 2));
+    auto load = [&](int it) {
+        const int t0 = (u.tile0 + it) * S::KEYS + 4 * q0 + lr;
+        const uint32_t at = base + (uint32_t)(it & 1) * S::STAGE + q0 * 1024;
+        if ((u.tile0 + it) * S::KEYS + 4 * (q0 + HALF) <= len) {
+            const uint16_t* const kp = kb + (size_t)t0 * step;
+            const uint16_t* const vp = vb + (size_t)t0 * step + vcol;
+#pragma unroll
+            for (int i = 0; i < HALF; ++i) lds_dma16(kp + (size_t)(4 * i) * step + (kcol ^ (32 * (i & 3))), at + i * 1024);
+#pragma unroll
+            for (int i = 0; i < HALF; ++i) lds_dma16(vp + (size_t)(4 * i) * step, at + S::KEYS * TA_ROW_BYTES + i * 1024);
+        } else {  // rows from the length on are read from `fresh`: here the last slot's stand for them
+#pragma unroll
+            for (int i = 0; i < HALF; ++i) {
+                const int t = min(t0 + 4 * i, (int)a.s_cap - 1);
+                lds_dma16(kb + (size_t)t * step + (kcol ^ (32 * (i & 3))), at + i * 1024);
+            }
+#pragma unroll
+            for (int i = 0; i < HALF; ++i) {
+                const int t = min(t0 + 4 * i, (int)a.s_cap - 1);
+                lds_dma16(vb + (size_t)t * step + vcol, at + S::KEYS * TA_ROW_BYTES + i * 1024);
+            }
+        }
+    };
+    if (tiles > 0) load(0);
+
+    // the nodes' angles, then the rows
+    if (a.rope && tiles > 0) {
+        const double turns = rope_turns(lane, a.log2_theta);
+        for (int i = wave; i < count; i += TF_WAVES) {
+            float cs, sn;
+            rope_at(turns, len + __popcll(readlane64(lines, i)) - 1, cs, sn);
+            angles[i * 64 + lane] = make_float2(cs, sn);
+        }
+    }
+    for (int i = tid; i < TA_D * 3; i += TF_WAVES * 64) found[i / 3][i % 3] = 0u;
+    __syncthreads();
+    uint64_t bad[2][3] = {{0, 0, 0}, {0, 0, 0}};
+    if (tiles > 0) {
+#pragma unroll
+        for (int e = 0; e < TF_EACH; ++e) {
+            const int r = wave + TF_WAVES * e;
+            if (r >= rows) break;
+            const float2 angle = a.rope ? angles[r / group * 64 + lane] : make_float2(1.0f, 0.0f);
+            float y[2];
+            q8_norm_rope(x0[e], x1[e], has_w, qw0, qw1, a.eps, angle.x, angle.y, y[0], y[1]);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const uint32_t hi = f32_to_bf16_bits(y[k]);
+                qs[r * TF_QROW + lane + 64 * k] = (uint16_t)hi;
+                qs[(TF_ROWS + r) * TF_QROW + lane + 64 * k] = (uint16_t)f32_to_bf16_bits(y[k] - bf16_bits_to_f32(hi));
+            }
+        }
+        if (has_nodes) {
+            // pieces of a row lie where a tile's row of that number has them; rows that are no nodes are zeros
+            auto key_at = [&](int i, int d) { return i * TA_D + ((d >> 3 ^ (i & 15)) << 3 | (d & 7)); };
+            uint16_t* const fk = reinterpret_cast<uint16_t*>(fresh[0]);
+            uint32_t* const fv = reinterpret_cast<uint32_t*>(fresh[1]);
+#pragma unroll
+            for (int e = 0; e < TF_EACH; ++e) {
+                const int i = wave + TF_WAVES * e;
+                if (i >= (int)a.n) break;
+                const uint64_t line = readlane64(lines, i);
+                uint32_t v = 0;
+                float r0 = 0.0f, r1 = 0.0f;
+                if (line) {
+                    const float2 angle = a.rope ? angles[i * 64 + lane] : make_float2(1.0f, 0.0f);
+                    q8_norm_rope(k0[e], k1[e], has_w, kw0, kw1, a.eps, angle.x, angle.y, r0, r1);
+                    v = pack_bf16x2(v0[e], v1[e]);
+                    // (where the nodes lie across two units both have them; one writes)
+                    if (len + i >= u.tile0 * S::KEYS && len + i < u.tile1 * S::KEYS) {
+                        const size_t slot = ((size_t)len + i) * step + (size_t)h * TA_D;
+                        uint16_t* const y = a.k_cache + seq * a.k_seq + slot + lane;
+                        y[0] = (uint16_t)f32_to_bf16_bits(r0);
+                        y[64] = (uint16_t)f32_to_bf16_bits(r1);
+                        reinterpret_cast<uint32_t*>(a.v_cache + seq * a.v_seq + slot)[lane] = v;
+                    }
+                    tree_take_broken(v, i, bad);
+                }
+                fk[key_at(i, lane)] = (uint16_t)f32_to_bf16_bits(r0);
+                fk[key_at(i, lane + 64)] = (uint16_t)f32_to_bf16_bits(r1);
+                fv[i * 64 + ((lane >> 2 ^ (i & 3) << 2) << 2 | (lane & 3))] = v;
+            }
+            if (wave == 0) fv[a.n * 64 + lane] = 0u;
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int k = 0; k < 3; ++k)
+                    if (bad[e][k]) atomicOr(&found[2 * lane + e][k], (uint32_t)bad[e][k]);
+        }
+    }
+    const int broken = __syncthreads_or((bad[0][0] | bad[0][1] | bad[0][2] | bad[1][0] | bad[1][1] | bad[1][2]) != 0);
+
+    ta_f32x16 o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[i][e] = 0.0f;
+    float m_run = -INFINITY, l_part = 0.0f;
+    if (tiles > 0) {
+        ta_bf16x8 qh[8], ql[8];
+        const int r = min(lane & 31, rows - 1);
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+            qh[s] = *reinterpret_cast<const ta_bf16x8*>(qs + r * TF_QROW + 16 * s + 8 * half);
+            ql[s] = *reinterpret_cast<const ta_bf16x8*>(qs + (TF_ROWS + r) * TF_QROW + 16 * s + 8 * half);
+        }
+        const uint32_t line = (uint32_t)__shfl((int)lines, r / group);  // up to 32 nodes
+        // every load that the compiler counts has landed, and the second stage is free
+        wait_vm<0>();
+        wait_lgkm0();
+        __syncthreads();
+        const int krow = 32 * wave + (lane & 31), n16 = lane & 15;
+        const int vr = 4 * half + (n16 >> 2), vpiece = 2 * ((lane >> 4) & 1) + ((n16 & 3) >> 1);
+        const uint32_t fresh_at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)&fresh[0][0]);
+        for (int it = 0; it < tiles; ++it) {
+            const int t0 = (u.tile0 + it) * S::KEYS + 32 * wave;
+            if (it + 1 < tiles) {
+                load(it + 1);
+                wait_vm<S::PER>();
+            } else {
+                wait_vm<0>();
+            }
+            asm volatile("" ::: "memory");
+            if (t0 >= len + count) continue;  // behind the nodes: nothing
+            const bool edge = t0 + 32 > len;
+            const uint32_t stage = base + (uint32_t)(it & 1) * S::STAGE;
+            // where this lane reads: a key's row, and four values' rows, of the tile or of the nodes
+            uint32_t ka = stage + (uint32_t)krow * TA_ROW_BYTES, kf = (uint32_t)krow & 15, va[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) va[i] = stage + S::KEYS * TA_ROW_BYTES + (uint32_t)(32 * wave + vr + 8 * i) * TA_ROW_BYTES;
+            uint32_t vf[4] = {(uint32_t)vr & 3, (uint32_t)vr & 3, (uint32_t)vr & 3, (uint32_t)vr & 3};
+            if (edge) {
+                const int jk = t0 + (lane & 31) - len;
+                if (jk >= 0) {
+                    ka = fresh_at + (uint32_t)min(jk, (int)a.n) * TA_ROW_BYTES;
+                    kf = (uint32_t)min(jk, (int)a.n) & 15;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int jv = t0 + vr + 8 * i - len;
+                    if (jv >= 0) {
+                        va[i] = fresh_at + (TF_ROWS + 1) * TA_ROW_BYTES + (uint32_t)min(jv, (int)a.n) * TA_ROW_BYTES;
+                        vf[i] = (uint32_t)min(jv, (int)a.n) & 3;
+                    }
+                }
+            }
+            typedef __attribute__((address_space(3))) uint8_t lds_u8;
+            ta_f32x16 s;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] = 0.0f;
+#pragma unroll
+            for (int st = 0; st < 8; ++st) {
+                const ta_bf16x8 kr = *(const __attribute__((address_space(3))) ta_bf16x8*)(lds_u8*)(uintptr_t)(ka + (((2 * st + half) ^ kf) << 4));
+                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kr, qh[st], s, 0, 0, 0);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kr, ql[st], s, 0, 0, 0);
+            }
+            if (edge) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int j = t0 + 8 * (e >> 2) + 4 * half + (e & 3) - len;
+                    const bool seen = j < 0 || (j < 32 && (line >> (j & 31) & 1));
+                    s[e] = seen ? s[e] : -INFINITY;
+                }
+            }
+            float mt = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[e]);
+            mt = xor_max<32>(mt * a.scale_log2);
+            const bool grow = mt > m_run + TA_RESCALE;
+            const float m_new = grow ? mt : m_run;
+            const float alpha = grow ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
+            const float msub = m_new == -INFINITY ? 0.0f : m_new;
+            m_run = m_new;
+            uint32_t pk[8];
+            float lsum = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+                const float p0 = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2, -msub));
+                const float p1 = __builtin_amdgcn_exp2f(fmaf(s[e + 1], a.scale_log2, -msub));
+                lsum += p0 + p1;
+                pk[e / 2] = pack_bf16x2(p0, p1);
+            }
+            l_part = fmaf(l_part, alpha, lsum);
+            if (__builtin_amdgcn_ballot_w64(grow) != 0) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[i][e] *= alpha;
+            }
+#pragma unroll
+            for (int stp = 0; stp < 2; ++stp) {
+                const ta_bf16x8 pf =
+                    __builtin_bit_cast(ta_bf16x8, make_uint4(pk[4 * stp], pk[4 * stp + 1], pk[4 * stp + 2], pk[4 * stp + 3]));
+#pragma unroll
+                for (int db = 0; db < 4; ++db) {
+                    auto value = [&](int i) {
+                        const uint32_t at = va[i] + (((uint32_t)(4 * db + vpiece) ^ (vf[i] << 2)) << 4) + 8 * (n16 & 1);
+                        return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) t2h_v4i16*)(lds_u8*)(uintptr_t)at));
+                    };
+                    const uint2 x = value(2 * stp), y = value(2 * stp + 1);
+                    o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(ta_bf16x8, make_uint4(x.x, x.y, y.x, y.y)), pf, o[db], 0, 0, 0);
+                }
+            }
+            wait_lgkm0();  // the buffer is read before it is loaded again
+            asm volatile("" ::: "memory");
+        }
+    }
+
+    // join the waves
+    const float l = xor_sum<32>(l_part);
+    wait_vm<0>();
+    wait_lgkm0();
+    __syncthreads();
+    float* const os = reinterpret_cast<float*>(lds);
+    if (half == 0) {
+        wml[wave][lane][0] = m_run;
+        wml[wave][lane][1] = l;
+    }
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<ta_f32x4*>(os + (wave * 32 + (lane & 31)) * S::OROW + 32 * db + 8 * g + 4 * half) =
+                ta_f32x4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
+    __syncthreads();
+    const bool whole = u.parts == 1;
+    const int node0 = max(u.tile0 * S::KEYS - len, 0), node1 = min(u.tile1 * S::KEYS - len, 32);
+    const uint32_t here = broken && node1 > node0 ? (~0u >> (32 - (node1 - node0))) << node0 : 0;
+    auto put = [&](int r, int d, ta_f32x4 sum, float L, bool node) {
+        uint2 y = make_uint2(0u, 0u);
+        if (node) {
+            const float inv = 1.0f / L;
+            y = make_uint2(pack_bf16x2(sum[0] * inv, sum[1] * inv), pack_bf16x2(sum[2] * inv, sum[3] * inv));
+        }
+        *reinterpret_cast<uint2*>(a.out + (((size_t)seq * a.n + r / group) * a.nh + h * group + r % group) * TA_D + d) = y;
+    };
+    // this (sequence, head)'s parts: maxima and sums, then rows
+    const size_t part_bytes = (size_t)TF_ROWS * (TA_D + 4) * 4;
+    uint8_t* const parts = reinterpret_cast<uint8_t*>(a.part_o) + ((size_t)u.first * a.nk + (size_t)h * u.parts) * part_bytes;
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(parts, 0, (int)min((size_t)u.parts * part_bytes, (size_t)0x7fffffff), 0x00027000);
+    for (int i = tid; i < TF_ROWS * 32; i += TF_WAVES * 64) {
+        const int r = i >> 5, d = (i & 31) * 4;
+        if (r >= (whole ? all : rows)) break;
+        float M = -INFINITY, L = 0.0f;
+#pragma unroll
+        for (int w = 0; w < TF_WAVES; ++w) M = fmaxf(M, wml[w][r][0]);
+        const float msub = M == -INFINITY ? 0.0f : M;
+        ta_f32x4 sum = ta_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < TF_WAVES; ++w) {
+            const float f = __builtin_amdgcn_exp2f(wml[w][r][0] - msub);
+            L = fmaf(f, wml[w][r][1], L);
+            sum += *reinterpret_cast<const ta_f32x4*>(os + (w * 32 + r) * S::OROW + d) * f;
+        }
+        const uint32_t line = (uint32_t)__shfl((int)lines, r / group);
+        if (line & here) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                sum[e] = tree_put_broken(sum[e], line & here & found[d + e][0], line & here & found[d + e][1], line & here & found[d + e][2]);
+        }
+        if (whole) {
+            put(r, d, sum, L, line != 0);
+        } else {
+            const int at = u.part * (int)part_bytes + r * (TA_D + 4) * 4;
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(ta_u32x4, sum), rsrc, at + 16 + d * 4, 0, TF_AGENT);
+            if (d == 0) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(ta_u32x4, ta_f32x4{M, L, 0.0f, 0.0f}), rsrc, at, 0, TF_AGENT);
+        }
+    }
+    if (whole) return;
+    __builtin_amdgcn_s_waitcnt(0);
+    asm volatile("" ::: "memory");
+    __syncthreads();
+    if (tid == 0) {
+        arrived = __hip_atomic_fetch_add(&a.done[head], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u;
+        if (arrived == (uint32_t)u.parts) __hip_atomic_store(&a.done[head], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (arrived != (uint32_t)u.parts) return;
+    // slices of the parts, where rows are few; 8 parts of a slice on their way at a time
+    const int pieces = rows * 32, slices = TF_WAVES * 64 / pieces > 0 ? TF_WAVES * 64 / pieces : 1;
+    constexpr int BATCH = 8;
+    for (int i = tid; i < pieces * slices; i += TF_WAVES * 64) {
+        const int slice = i / pieces, r = i % pieces / 32, d = i % 32 * 4;
+        float M = -INFINITY, L = 0.0f;
+        ta_f32x4 sum = ta_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int n0 = slice; n0 < u.parts; n0 += slices * BATCH) {
+            ta_u32x4 ml[BATCH], x[BATCH];
+#pragma unroll
+            for (int e = 0; e < BATCH; ++e) {
+                const int at = min(n0 + slices * e, u.parts - 1) * (int)part_bytes + r * (TA_D + 4) * 4;
+                ml[e] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, 0, TF_AGENT);
+                x[e] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, at + 16 + d * 4, 0, TF_AGENT);
+            }
+#pragma unroll
+            for (int e = 0; e < BATCH; ++e) {
+                if (n0 + slices * e >= u.parts) break;
+                const ta_f32x4 q = __builtin_bit_cast(ta_f32x4, ml[e]);
+                const float now = fmaxf(M, q[0]), msub = now == -INFINITY ? 0.0f : now;
+                const float keep = __builtin_amdgcn_exp2f(M - msub), f = __builtin_amdgcn_exp2f(q[0] - msub);
+                L = fmaf(L, keep, f * q[1]);
+                sum = sum * keep + __builtin_bit_cast(ta_f32x4, x[e]) * f;
+                M = now;
+            }
+        }
+        if (slices == 1) {
+            put(r, d, sum, L, (uint32_t)__shfl((int)lines, r / group) != 0);
+        } else {
+            *reinterpret_cast<ta_f32x4*>(os + (slice * 32 + r) * S::OROW + d) = sum;  // (up to 8 slices of up to 4 rows)
+            if (d == 0) {
+                wml[slice & 3][(slice >> 2) * 16 + r][0] = M;
+                wml[slice & 3][(slice >> 2) * 16 + r][1] = L;
+            }
+        }
+    }
+    __syncthreads();
+    if (slices > 1 && tid < pieces) {
+        const int r = tid / 32, d = tid % 32 * 4;
+        float M = -INFINITY, L = 0.0f;
+        for (int n = 0; n < slices; ++n) M = fmaxf(M, wml[n & 3][(n >> 2) * 16 + r][0]);
+        const float msub = M == -INFINITY ? 0.0f : M;
+        ta_f32x4 sum = ta_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int n = 0; n < slices; ++n) {
+            const float f = __builtin_amdgcn_exp2f(wml[n & 3][(n >> 2) * 16 + r][0] - msub);
+            L = fmaf(f, wml[n & 3][(n >> 2) * 16 + r][1], L);
+            sum += *reinterpret_cast<const ta_f32x4*>(os + (n * 32 + r) * S::OROW + d) * f;
+        }
+        put(r, d, sum, L, (uint32_t)__shfl((int)lines, r / group) != 0);
+    }
+    // rows that are no nodes
+    for (int i = rows * 32 + tid; i < all * 32; i += TF_WAVES * 64) put(i / 32, i % 32 * 4, ta_f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 1.0f, false);
 }
 
 // ------------------------------------------------------------------------------------------------------ launch --
@@ -536,36 +1050,44 @@ __global__ __launch_bounds__(256) void tree_join_kernel(const TreeAttnArgs a) {
 static uint32_t ta_tile_rows(uint32_t rows) { return rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256; }
 
 struct TreeSizes {
-    uint32_t tile_rows, row_tiles, rows, keys, least, slots, units;
-    size_t qh, ql, line, vt, broken, which, table, of_seq, part_ml, part_o, end;
+    uint32_t tile_rows, row_tiles, rows, keys, least, extra, slots, units;
+    size_t done, qh, ql, line, vt, broken, which, table, of_seq, part_ml, part_o, end;
 };
 
 constexpr uint32_t TA_CUS = 256;
 
 static TreeSizes ta_sizes(uint32_t n_seq, uint32_t n, uint32_t nh, uint32_t nk, uint32_t s_cap) {
-    TreeSizes s;
+    TreeSizes s = {};
     const uint32_t rows = n * (nh / nk);
     s.tile_rows = ta_tile_rows(rows);
     s.row_tiles = (rows + s.tile_rows - 1) / s.tile_rows;
     s.rows = s.row_tiles * s.tile_rows;
     s.keys = s.tile_rows <= 64 ? 128 : s.tile_rows == 128 ? 64 : 32;
     s.least = s.tile_rows <= 64 ? 1 : s.tile_rows == 128 ? 4 : 8;
+    s.extra = s.tile_rows <= 64 ? 2 : s.tile_rows == 128 ? 4 : 6;
     s.slots = TA_CUS / (nk * s.row_tiles) > 1 ? TA_CUS / (nk * s.row_tiles) : 1;
-    const uint64_t most = (uint64_t)n_seq * ((s_cap + s.keys - 1) / s.keys), some = (uint64_t)s.slots + n_seq;
+    const uint64_t most = (uint64_t)n_seq * ((s_cap + s.keys - 1) / s.keys), some = (uint64_t)4 * s.slots + n_seq;
     s.units = (uint32_t)(most < some ? most : some);
     size_t at = 0;
+    const size_t counters = (size_t)n_seq * nk;  // first, and as many for every shape up to 16384 of them: calls may share a workspace
     auto take = [&](size_t bytes) {
         const size_t here = at;
         at += (bytes + 255) / 256 * 256;
         return here;
     };
     const size_t q = (size_t)n_seq * n * nh * TA_D * 2, heads = (size_t)n_seq * nk, parts = (size_t)s.units * nk * s.rows;
+    s.done = take((counters > 16384 ? counters : 16384) * 4);
+    if (s.tile_rows == 32) {  // one launch
+        s.part_o = take(parts * (TA_D + 4) * 4);
+        s.end = at;
+        return s;
+    }
     s.qh = take(q);
     s.ql = take(q);
     s.line = take((size_t)n_seq * n * 8);
     s.vt = take(heads * (n + 1) * TA_D * 2);
-    s.broken = take(heads * 4);
-    s.which = take(heads * TA_D * 24);
+    s.broken = take(heads * TP_GROUPS * 4);
+    s.which = take(heads * TP_GROUPS * TA_D * 24);
     s.table = take((size_t)s.units * sizeof(TreeUnit));
     s.of_seq = take((size_t)n_seq * 8);
     s.part_ml = take(parts * 8);
@@ -636,6 +1158,7 @@ extern "C" int t2h_attn_tree(const float* q, uint64_t q_row, const float* k_new,
     a.group = nh / nk;
     a.out = reinterpret_cast<uint16_t*>(out);
     uint8_t* const ws = reinterpret_cast<uint8_t*>(workspace);
+    a.done = reinterpret_cast<uint32_t*>(ws + s.done);
     a.qh = reinterpret_cast<uint16_t*>(ws + s.qh);
     a.ql = reinterpret_cast<uint16_t*>(ws + s.ql);
     a.line = reinterpret_cast<uint64_t*>(ws + s.line);
@@ -652,17 +1175,22 @@ extern "C" int t2h_attn_tree(const float* q, uint64_t q_row, const float* k_new,
     a.slots = s.slots;
     a.keys = s.keys;
     a.least = s.least;
-    const uint64_t waves = (uint64_t)n_seq * n * ((nh + TP_HEADS - 1) / TP_HEADS), kv = (uint64_t)n_seq * nk;
+    a.extra = s.extra;
+    const uint64_t waves = (uint64_t)n_seq * n * ((nh + TP_HEADS - 1) / TP_HEADS), kv = (uint64_t)n_seq * nk * ((n + TP_NODES - 1) / TP_NODES);
     const uint64_t grid = (uint64_t)s.units * nk * s.row_tiles, joins = ((uint64_t)n_seq * n * nh + 3) / 4;
     if (kv + waves > 0x3fffffffu || grid > 0x7fffffffu || joins > 0x3fffffffu) return T2H_ERR_SHAPE;
     a.kv_blocks = (uint32_t)kv;
     a.q_blocks = (uint32_t)((waves + 3) / 4);
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    const dim3 g((uint32_t)grid);
+    if (s.tile_rows == 32) {
+        hipLaunchKernelGGL(tree_few_kernel, g, dim3(TF_WAVES * 64), 0, st, a);
+        T2H_LAUNCH_CHECK();
+        return T2H_OK;
+    }
     hipLaunchKernelGGL(tree_rows_kernel, dim3(1 + a.kv_blocks + a.q_blocks), dim3(256), 0, st, a);
     T2H_LAUNCH_CHECK();
-    const dim3 g((uint32_t)grid);
-    if (s.tile_rows == 32) hipLaunchKernelGGL((tree_attn_kernel<1, 4, 2>), g, dim3(256), 0, st, a);
-    else if (s.tile_rows == 64) hipLaunchKernelGGL((tree_attn_kernel<2, 4, 2>), g, dim3(512), 0, st, a);
+    if (s.tile_rows == 64) hipLaunchKernelGGL((tree_attn_kernel<2, 4, 2>), g, dim3(512), 0, st, a);
     else if (s.tile_rows == 128) hipLaunchKernelGGL((tree_attn_kernel<4, 2, 4>), g, dim3(512), 0, st, a);
     else hipLaunchKernelGGL((tree_attn_kernel<8, 1, 8>), g, dim3(512), 0, st, a);
     T2H_LAUNCH_CHECK();
