@@ -13,6 +13,7 @@ typedef float ta_f32x16 __attribute__((ext_vector_type(16)));
 typedef float ta_f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int TA_D = 128;
+constexpr uint32_t TA_CUS = 256;
 constexpr int TA_MAX_GROUP = 16;
 constexpr int TA_ROW_BYTES = TA_D * 2;
 constexpr int TP_NODES = 16, TP_GROUPS = TREE_MAX / TP_NODES;  // nodes of a thread block that writes K and V rows
@@ -57,8 +58,8 @@ struct TreeAttnArgs {
     float* part_ml;    // [n_units * nk][rows][2] log2 maximum, sum
     float* part_o;     // [n_units * nk][rows][128]
     uint32_t n_units, row_tiles, rows;  // rows: of a KV head, in whole tiles
-    uint32_t slots;    // units a KV head that fill the chip
-    uint32_t keys, least, extra;  // tokens a tile; the least tiles a unit; what a unit costs besides, in tiles
+    uint32_t keys, least;               // tokens a tile; the least tiles a unit
+    float us_turn, us_tile, us_shared, us_join;  // what tree_chunk goes by
     uint32_t kv_blocks, q_blocks;
 };
 
@@ -79,37 +80,42 @@ __device__ __forceinline__ uint32_t tree_tiles(const TreeAttnArgs& a, uint32_t i
 
 __device__ __forceinline__ uint32_t wave_total_u32(uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)wave_scan_u32(v), 63); }
 
-// Tiles a unit: the fewest that leave no more units than `turns` times what the chip holds at once, for the number of turns that
-// ends first; a unit costs a.extra tiles' time besides its own.  Where the sequences alone are more than that, what would be
-// one turn's share.  `mine`: tiles of sequence `lane`, the others' are looked up.
+__device__ __forceinline__ uint32_t div_up(uint32_t x, uint32_t by) {  // x < 2^24
+    uint32_t q = (uint32_t)((float)(x + by - 1) * __builtin_amdgcn_rcpf((float)by));
+    const int r = (int)(x + by - 1 - q * by);
+    q = r < 0 ? q - 1 : q;
+    return r >= (int)by ? q + 1 : q;
+}
+
+// Tiles a unit.  Each lane weighs the longest sequence in another number of units, by what a turn of the chip costs besides tiles,
+// what a tile costs where its thread block is alone and what it costs where all are bound by memory, and a join.
+// `mine`: tiles of sequence `lane`, the others' are looked up.
 __device__ uint32_t tree_chunk(const TreeAttnArgs& a, uint32_t mine) {
     const uint32_t lane = threadIdx.x & 63;
     int len, count;
-    uint32_t total = lane < a.n_seq ? mine : 0;
-    for (uint32_t i = lane + 64; i < a.n_seq; i += 64) total += tree_tiles(a, i, len, count);
-    total = wave_total_u32(total);
-    uint32_t chunk = (total + a.slots - 1) / a.slots, best = 0xffffffffu;
-    for (uint32_t turns = (a.n_seq + a.slots - 1) / a.slots; turns <= 4; ++turns) {
-        const uint32_t most = turns * a.slots;
-        uint32_t c = (total + most - 1) / most;
-        c = c > a.least ? c : a.least;
-        for (;;) {
-            uint32_t units = lane < a.n_seq ? (mine ? (mine + c - 1) / c : 1u) : 0u;
-            for (uint32_t i = lane + 64; i < a.n_seq; i += 64) {
-                const uint32_t t = tree_tiles(a, i, len, count);
-                units += t ? (t + c - 1) / c : 1u;
-            }
-            units = wave_total_u32(units);
-            if (units <= most) break;
-            c += c * (units - most) / units + 1;  // (there is such a c: every sequence one unit)
-        }
-        if (turns * (c + a.extra) < best) {
-            best = turns * (c + a.extra);
-            chunk = c;
-        }
-        if (c == a.least) break;
+    uint32_t total = lane < a.n_seq ? mine : 0, most = total;
+    for (uint32_t i = lane + 64; i < a.n_seq; i += 64) {
+        const uint32_t t = tree_tiles(a, i, len, count);
+        total += t;
+        most = most > t ? most : t;
     }
-    return chunk > a.least ? chunk : a.least;
+    total = wave_total_u32(total);
+    most = wave_max_u32(most);
+    if (most == 0) return 1;
+    uint32_t c = div_up(most, lane < 32 ? lane + 1 : 32 + (lane - 31) * 7);
+    c = c > a.least ? c : a.least;
+    uint32_t units = 0;
+    for (uint32_t i = 0; i < a.n_seq; ++i) {
+        const uint32_t t = i < 64 ? (uint32_t)__builtin_amdgcn_readlane((int)mine, (int)i) : tree_tiles(a, i, len, count);
+        units += t > c ? div_up(t, c) : 1u;
+    }
+    const float blocks = (float)(a.nk * a.row_tiles) * (1.0f / TA_CUS), turns = ceilf((float)units * blocks);
+    const float alone = turns * (a.us_turn + (float)min(c, most) * a.us_tile), together = a.us_turn + (float)total * blocks * a.us_shared;
+    float cost = fmaxf(alone, together) + (c < most ? a.us_join : 0.0f);
+    if (units > a.n_units) cost = INFINITY;
+    const uint64_t best = __ballot(cost == -wave_max(-cost));
+    const uint32_t chunk = (uint32_t)__builtin_amdgcn_readlane((int)c, __builtin_ctzll(best));
+    return chunk;  // (one unit a sequence is never too many)
 }
 
 // Units of a whole chunk come first, the sequences' last, shorter ones behind them, so that what the chip ends with is short.
@@ -157,7 +163,7 @@ __device__ bool tree_find(const TreeAttnArgs& a, uint32_t unit, TreeUnit& u) {
     const uint32_t lane = threadIdx.x & 63;
     if (a.n_seq == 1) {
         const uint32_t tiles = tree_tiles(a, 0, u.len, u.count);
-        const uint32_t share = (tiles + a.slots - 1) / a.slots, chunk = share > a.least ? share : a.least;
+        const uint32_t chunk = tree_chunk(a, tiles);
         u.seq = u.first = 0;
         u.part = (int)unit;
         u.parts = tiles ? (int)((tiles + chunk - 1) / chunk) : 1;
@@ -201,6 +207,13 @@ __device__ bool tree_find(const TreeAttnArgs& a, uint32_t unit, TreeUnit& u) {
         rest_at = (uint32_t)__builtin_amdgcn_readlane((int)rest_up, 63);
     }
     return false;
+}
+
+// Which of 32 tokens a row sees, from the one `at` places behind the cached ones: those before are seen, nodes by their set.
+__device__ __forceinline__ uint32_t tree_seen(uint64_t line, int at) {
+    const uint32_t nodes = at < 64 ? (uint32_t)(line >> (at & 63)) : 0u;
+    const uint32_t before = at > -32 ? ((uint32_t)line << (-at & 31)) | ((1u << (-at & 31)) - 1u) : 0xffffffffu;
+    return at >= 0 ? nodes : before;
 }
 
 __device__ __forceinline__ uint64_t readlane64(uint64_t x, int lane) {
@@ -474,19 +487,15 @@ void tree_attn_kernel(const TreeAttnArgs a) {
                 for (int e = 0; e < 16; ++e) s[e] = 0.0f;
 #pragma unroll
                 for (int st = 0; st < 8; ++st) {
-                    const ta_bf16x8 kf =
-                        *reinterpret_cast<const ta_bf16x8*>(stage + ka + (((2 * st + half) ^ (krow & 15)) << 4));
+                    const ta_bf16x8 kf = *reinterpret_cast<const ta_bf16x8*>(stage + ka + (((2 * st + half) ^ (krow & 15)) << 4));
                     s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qh[st], s, 0, 0, 0);
                     s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, ql[st], s, 0, 0, 0);
                 }
                 const int t0 = (u.tile0 + it) * S::KEYS + 32 * wk;
                 if (t0 + 32 > len) {
+                    const uint32_t seen = tree_seen(line, t0 + 4 * half - len);
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const int j = t0 + 8 * (e >> 2) + 4 * half + (e & 3) - len;
-                        const bool seen = j < 0 || (j < TREE_MAX && (line >> (j & 63) & 1));
-                        s[e] = seen ? s[e] : -INFINITY;
-                    }
+                    for (int e = 0; e < 16; ++e) s[e] = seen & 1u << (8 * (e >> 2) + (e & 3)) ? s[e] : -INFINITY;
                 }
                 float mt = -INFINITY;
 #pragma unroll
@@ -515,8 +524,8 @@ void tree_attn_kernel(const TreeAttnArgs a) {
                 }
 #pragma unroll
                 for (int stp = 0; stp < 2; ++stp) {
-                    const ta_bf16x8 pf = __builtin_bit_cast(
-                        ta_bf16x8, make_uint4(pk[4 * stp], pk[4 * stp + 1], pk[4 * stp + 2], pk[4 * stp + 3]));
+                    const ta_bf16x8 pf =
+                        __builtin_bit_cast(ta_bf16x8, make_uint4(pk[4 * stp], pk[4 * stp + 1], pk[4 * stp + 2], pk[4 * stp + 3]));
                     const uint8_t* const v = stage + va + 16 * stp * TA_ROW_BYTES;
 #pragma unroll
                     for (int db = 0; db < 4; ++db) {
@@ -590,8 +599,24 @@ void tree_attn_kernel(const TreeAttnArgs a) {
     }
 }
 
-// Joins the units of a sequence, a wave a row: a lane holds a unit's maximum and sum, and two dims.
+// Joins the units of a sequence, a wave a row: a lane holds a unit's maximum and sum, and four dims of every other unit's row.
+// All of up to 32 units are on their way at once.
 constexpr int TJ_BATCH = 16;
+
+template <int N>
+__device__ __forceinline__ void tree_join_rows(const float* part_o, size_t first, size_t step, int p0, int parts, float f, ta_f32x4& o) {
+    const int lane = threadIdx.x & 63, half = lane >> 5, d = (lane & 31) * 4;
+    ta_f32x4 x[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] = *reinterpret_cast<const ta_f32x4*>(part_o + (first + min(p0 + 2 * e + half, parts - 1) * step) * TA_D + d);
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        const float f0 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), (p0 + 2 * e) & 63)),
+                    f1 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), (p0 + 2 * e + 1) & 63));
+        const bool in = p0 + 2 * e + half < parts;
+        if (in) o += x[e] * (half ? f1 : f0);
+    }
+}
 
 __global__ __launch_bounds__(256) void tree_join_kernel(const TreeAttnArgs a) {
     const int lane = threadIdx.x & 63;
@@ -601,98 +626,129 @@ __global__ __launch_bounds__(256) void tree_join_kernel(const TreeAttnArgs a) {
     const int2 parts = a.of_seq[seq];
     const uint64_t line = a.line[(size_t)seq * a.n + i];
     if (parts.y <= 1) return;
-    uint32_t* const out = reinterpret_cast<uint32_t*>(a.out + ((size_t)unit) * TA_D);
     if (line == 0) {
-        out[lane] = 0u;
+        reinterpret_cast<uint32_t*>(a.out + (size_t)unit * TA_D)[lane] = 0u;
         return;
     }
-    const size_t r = (size_t)i * a.group + head % a.group;
-    auto at = [&](int p) { return ((size_t)(parts.x + min(p, parts.y - 1)) * a.nk + h) * a.rows + r; };
-    float M = -INFINITY, L = 0.0f, o0 = 0.0f, o1 = 0.0f;
+    const size_t first = ((size_t)parts.x * a.nk + h) * a.rows + (size_t)i * a.group + head % a.group, step = (size_t)a.nk * a.rows;
+    float M = -INFINITY, L = 0.0f;
+    ta_f32x4 o = ta_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     for (int p0 = 0; p0 < parts.y; p0 += 64) {
-        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * at(p0 + lane));
-        float2 x[TJ_BATCH];
-        auto load = [&](int p) {
-#pragma unroll
-            for (int e = 0; e < TJ_BATCH; ++e) x[e] = *reinterpret_cast<const float2*>(a.part_o + at(p + e) * TA_D + 2 * lane);
-        };
-        load(p0);
-        const float m = p0 + lane < parts.y ? ml.x : -INFINITY;
+        const bool in = p0 + lane < parts.y;
+        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (first + min(p0 + lane, parts.y - 1) * step));
+        const float m = in ? ml.x : -INFINITY;
         const float now = fmaxf(M, wave_max(m)), msub = now == -INFINITY ? 0.0f : now;
-        const float keep = __builtin_amdgcn_exp2f(M - msub), f = p0 + lane < parts.y ? __builtin_amdgcn_exp2f(m - msub) : 0.0f;
-        L = fmaf(L, keep, wave_sum(p0 + lane < parts.y ? f * ml.y : 0.0f));
-        o0 *= keep;
-        o1 *= keep;
+        const float keep = __builtin_amdgcn_exp2f(M - msub), f = in ? __builtin_amdgcn_exp2f(m - msub) : 0.0f;
+        L = fmaf(L, keep, wave_sum(in ? f * ml.y : 0.0f));
+        o *= keep;
         M = now;
-        const int end = min(parts.y - p0, 64);
-        for (int p = 0; p < end; p += TJ_BATCH) {
-            if (p) load(p0 + p);
-#pragma unroll
-            for (int e = 0; e < TJ_BATCH; ++e) {
-                if (p + e >= end) break;
-                const float fe = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), (p + e) & 63));
-                o0 = fmaf(x[e].x, fe, o0);
-                o1 = fmaf(x[e].y, fe, o1);
-            }
+        if (parts.y <= 8) {
+            tree_join_rows<4>(a.part_o, first, step, 0, parts.y, f, o);
+        } else {
+            for (int p = p0; p < min(p0 + 64, parts.y); p += 2 * TJ_BATCH) tree_join_rows<TJ_BATCH>(a.part_o, first, step, p, parts.y, f, o);
         }
     }
-    out[lane] = pack_bf16x2(o0 / L, o1 / L);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = xor_sum<32>(o[e]) / L;
+    if (lane < 32)
+        *reinterpret_cast<uint2*>(a.out + (size_t)unit * TA_D + lane * 4) = make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
 }
 
 // ------------------------------------------------------------------------------------- the attention of few rows --
 //
 // Up to 32 rows a KV head: all in one launch.  Every thread block norms and rotates the head's queries itself, while its first
 // tiles are on their way, and finds its unit in the lengths; the one that holds the nodes also brings their K and V into the
-// cache and reads them from LDS.  4 waves, 32 keys each, that wait for nothing but their own loads in the loop.  The last unit
-// of a (sequence, KV head) to leave its part joins them: parts go past the caches that the chip's parts do not share (agent
-// scope), and are there before the count is raised.
+// cache and reads them from LDS.  8 waves, 16 keys each, that wait for nothing but their own loads in the loop: two waves a SIMD
+// hide each other's latency.  Both products on v_mfma_f32_16x16x32_bf16 and _16x16x16_, CB blocks of 16 rows as their columns:
+// S^T's accumulators hold 4 keys a lane, which are the operand of the second product, and a transposing LDS read hands out 4
+// keys of a dim.
+// The last unit of a (sequence, KV head) to leave its part joins them: parts go past the caches that the chip's parts do not
+// share (agent scope), and are there before the count is raised.
 
-constexpr int TF_WAVES = 4, TF_ROWS = 32;
-constexpr int TF_EACH = TF_ROWS / TF_WAVES;  // rows, and nodes, a wave
-constexpr int TF_QROW = TA_D + 8;            // bf16 row of queries in LDS, padded
+constexpr int TF_WAVES = 8, TF_KEYS = 16 * TF_WAVES;
+constexpr int TF_QROW = TA_D + 8;  // bf16 row of queries in LDS, padded
+constexpr int TF_OROW = TA_D + 4;  // fp32 row of the join, padded
+constexpr int TF_STAGE = TF_KEYS * 2 * TA_ROW_BYTES;
+constexpr int TF_PART = (TA_D + 4) * 4;  // bytes of a row's part: maximum, sum, nothing, then the row
 
 typedef uint32_t ta_u32x4 __attribute__((ext_vector_type(4)));
+typedef short ta_s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) uint8_t ta_lds;
 constexpr int TF_AGENT = 16;  // cache policy of buffer loads and stores: agent scope
 
-__global__ __launch_bounds__(TF_WAVES * 64) __attribute__((amdgpu_waves_per_eu(1, 1))) void tree_few_kernel(const TreeAttnArgs a) {
-    using S = TreeShape<1, TF_WAVES, 2>;
-    __shared__ __align__(1024) uint8_t lds[S::LDS];
-    __shared__ __align__(16) uint8_t fresh[2][(TF_ROWS + 1) * TA_ROW_BYTES];  // the nodes' keys and values, and a row of zeros
-    __shared__ float wml[TF_WAVES][32][2];
+template <int CB>
+__global__ __launch_bounds__(TF_WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void tree_few_kernel(const TreeAttnArgs a) {
+    constexpr int ROWS = 16 * CB, EACH = ROWS / TF_WAVES;  // rows, and most nodes, of a wave
+    constexpr int QS = 2 * ROWS * TF_QROW * 2, ANGLES = ROWS * 64 * 8;
+    constexpr bool APART = CB == 1;  // the queries' two terms and the nodes' angles have room of their own, or before the loop the
+                                     // second stage's, which is then loaded later
+    static_assert(TF_WAVES * ROWS * TF_OROW * 4 <= 2 * TF_STAGE + 4096 * CB, "the join's rows fit the stages");
+    constexpr int LDS = TF_WAVES * ROWS * TF_OROW * 4 > 2 * TF_STAGE ? TF_WAVES * ROWS * TF_OROW * 4 : 2 * TF_STAGE;
+    __shared__ __align__(1024) uint8_t lds[LDS];
+    __shared__ __align__(16) uint8_t own[APART ? QS + ANGLES : 16];
+    __shared__ __align__(16) uint8_t fresh[2][(ROWS + 1) * TA_ROW_BYTES];  // the nodes' keys and values, and a row of zeros
+    __shared__ float wml[TF_WAVES][ROWS][2];
     __shared__ uint32_t found[TA_D][3], arrived;
-    // before the loop the second stage holds the queries' two terms and the nodes' angles
-    uint16_t* const qs = reinterpret_cast<uint16_t*>(lds + S::STAGE);
-    float2* const angles = reinterpret_cast<float2*>(lds + S::STAGE + 2 * TF_ROWS * TF_QROW * 2);
-    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    uint16_t* const qs = reinterpret_cast<uint16_t*>(APART ? own : lds + TF_STAGE);
+    float2* const angles = reinterpret_cast<float2*>((APART ? own : lds + TF_STAGE) + QS);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t unit = blockIdx.x / a.nk, h = blockIdx.x % a.nk;
     const int group = (int)a.group, all = (int)a.n * group;  // rows of the head, nodes or not
     TreeUnit u;
-    float x0[TF_EACH], x1[TF_EACH];
-    auto load_q = [&](uint32_t seq) {
-#pragma unroll
-        for (int e = 0; e < TF_EACH; ++e) {
-            const int r = min(wave + TF_WAVES * e, all - 1);
-            const float* x = a.q + ((size_t)seq * a.n + r / group) * a.q_row + (size_t)(h * group + r % group) * TA_D + lane;
-            x0[e] = x[0];
-            x1[e] = x[64];
-        }
-    };
-    if (a.n_seq == 1) load_q(0);  // (they do not wait for the lengths)
     if (!tree_find(a, unit, u)) return;  // every wave of the thread block finds the same
+    u.seq = __builtin_amdgcn_readfirstlane(u.seq);
+    u.tile0 = __builtin_amdgcn_readfirstlane(u.tile0);
+    u.tile1 = __builtin_amdgcn_readfirstlane(u.tile1);
+    u.first = __builtin_amdgcn_readfirstlane(u.first);
+    u.parts = __builtin_amdgcn_readfirstlane(u.parts);
+    u.part = __builtin_amdgcn_readfirstlane(u.part);
     const uint32_t seq = (uint32_t)u.seq;
-    if (a.n_seq != 1) load_q(seq);
-    const int len = u.len, count = u.count, rows = count * group, tiles = u.tile1 - u.tile0;
+    const int len = __builtin_amdgcn_readfirstlane(u.len), count = __builtin_amdgcn_readfirstlane(u.count);
+    const int rows = count * group, tiles = u.tile1 - u.tile0;
     const size_t head = (size_t)seq * a.nk + h;
-    const bool has_nodes = u.tile1 * S::KEYS > len && count > 0;
+    const bool has_nodes = u.tile1 * TF_KEYS > len && count > 0;
     const uint16_t* const kb = a.k_cache + seq * a.k_seq + (size_t)h * TA_D;
     const uint16_t* const vb = a.v_cache + seq * a.v_seq + (size_t)h * TA_D;
     const size_t step = (size_t)a.nk * TA_D;
+
+    // the wave's 16 keys and values of a tile, 4 rows a load; 16-byte pieces lie at their place XOR f(row): a key's row's four
+    // bits, twice three of a value's row
+    const uint32_t base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(ta_lds*)&lds[0]);
+    const int lr = lane >> 4, lp = lane & 15;
+    const int kcol = 8 * (lp ^ lr), vcol = 8 * (lp ^ (lr << 1));
+    auto load = [&](int it) {
+        const int first = (u.tile0 + it) * TF_KEYS + 16 * wave, t0 = first + lr;
+        const uint32_t at = __builtin_amdgcn_readfirstlane(base + (uint32_t)(it & 1) * TF_STAGE + wave * 16 * TA_ROW_BYTES);
+        if (first + 16 <= len) {
+            const uint16_t* const kp = kb + (size_t)t0 * step;
+            const uint16_t* const vp = vb + (size_t)t0 * step;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) lds_dma16(kp + (size_t)(4 * i) * step + (kcol ^ (32 * i)), at + i * 1024);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) lds_dma16(vp + (size_t)(4 * i) * step + (vcol ^ (64 * (i & 1))), at + TF_KEYS * TA_ROW_BYTES + i * 1024);
+        } else {  // rows from the length on are read from `fresh`: here the last slot's stand for them
+#pragma unroll
+            for (int i = 0; i < 4; ++i) lds_dma16(kb + (size_t)min(t0 + 4 * i, (int)a.s_cap - 1) * step + (kcol ^ (32 * i)), at + i * 1024);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                lds_dma16(vb + (size_t)min(t0 + 4 * i, (int)a.s_cap - 1) * step + (vcol ^ (64 * (i & 1))), at + TF_KEYS * TA_ROW_BYTES + i * 1024);
+        }
+    };
+    // the loads that the prologue waits for, then the tiles'
+    float x0[EACH], x1[EACH];
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+        const int r = min(wave + TF_WAVES * e, all - 1);
+        const float* x = a.q + ((size_t)seq * a.n + r / group) * a.q_row + (size_t)(h * group + r % group) * TA_D + lane;
+        x0[e] = x[0];
+        x1[e] = x[64];
+    }
     const bool has_w = a.q_norm_w != nullptr;
     const float qw0 = has_w ? a.q_norm_w[lane] : 1.0f, qw1 = has_w ? a.q_norm_w[lane + 64] : 1.0f;
-    float k0[TF_EACH], k1[TF_EACH], v0[TF_EACH], v1[TF_EACH], kw0 = 1.0f, kw1 = 1.0f;
+    float k0[EACH], k1[EACH], v0[EACH], v1[EACH], kw0 = 1.0f, kw1 = 1.0f;
     if (has_nodes) {
 #pragma unroll
-        for (int e = 0; e < TF_EACH; ++e) {
+        for (int e = 0; e < EACH; ++e) {
             const size_t row = (size_t)seq * a.n + min(wave + TF_WAVES * e, (int)a.n - 1);
             const float* kx = a.k_new + row * a.k_row + (size_t)h * TA_D + lane;
             const float* vx = a.v_new + row * a.v_row + (size_t)h * TA_D + 2 * lane;
@@ -707,35 +763,8 @@ __global__ __launch_bounds__(TF_WAVES * 64) __attribute__((amdgpu_waves_per_eu(1
         }
     }
     const uint64_t lines = tree_lineage(a.parents, seq, a.n, count);
-
-    const uint32_t base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)&lds[0]);
-    constexpr int HALF = S::PER / 2;  // loads of 4 rows: a wave's 32 keys, and values
-    const int q0 = wave * HALF, lr = lane >> 4, lp = lane & 15;
-    const int kcol = 8 * (lp ^ lr), vcol = 8 * (lp ^ (lr << 2));
-    auto load = [&](int it) {
-        const int t0 = (u.tile0 + it) * S::KEYS + 4 * q0 + lr;
-        const uint32_t at = base + (uint32_t)(it & 1) * S::STAGE + q0 * 1024;
-        if ((u.tile0 + it) * S::KEYS + 4 * (q0 + HALF) <= len) {
-            const uint16_t* const kp = kb + (size_t)t0 * step;
-            const uint16_t* const vp = vb + (size_t)t0 * step + vcol;
-#pragma unroll
-            for (int i = 0; i < HALF; ++i) lds_dma16(kp + (size_t)(4 * i) * step + (kcol ^ (32 * (i & 3))), at + i * 1024);
-#pragma unroll
-            for (int i = 0; i < HALF; ++i) lds_dma16(vp + (size_t)(4 * i) * step, at + S::KEYS * TA_ROW_BYTES + i * 1024);
-        } else {  // rows from the length on are read from `fresh`: here the last slot's stand for them
-#pragma unroll
-            for (int i = 0; i < HALF; ++i) {
-                const int t = min(t0 + 4 * i, (int)a.s_cap - 1);
-                lds_dma16(kb + (size_t)t * step + (kcol ^ (32 * (i & 3))), at + i * 1024);
-            }
-#pragma unroll
-            for (int i = 0; i < HALF; ++i) {
-                const int t = min(t0 + 4 * i, (int)a.s_cap - 1);
-                lds_dma16(vb + (size_t)t * step + vcol, at + S::KEYS * TA_ROW_BYTES + i * 1024);
-            }
-        }
-    };
     if (tiles > 0) load(0);
+    if (APART && tiles > 1) load(1);
 
     // the nodes' angles, then the rows
     if (a.rope && tiles > 0) {
@@ -746,12 +775,13 @@ __global__ __launch_bounds__(TF_WAVES * 64) __attribute__((amdgpu_waves_per_eu(1
             angles[i * 64 + lane] = make_float2(cs, sn);
         }
     }
-    for (int i = tid; i < TA_D * 3; i += TF_WAVES * 64) found[i / 3][i % 3] = 0u;
+    if (has_nodes)
+        for (int i = tid; i < TA_D * 3; i += TF_WAVES * 64) found[i / 3][i % 3] = 0u;
     __syncthreads();
     uint64_t bad[2][3] = {{0, 0, 0}, {0, 0, 0}};
     if (tiles > 0) {
 #pragma unroll
-        for (int e = 0; e < TF_EACH; ++e) {
+        for (int e = 0; e < EACH; ++e) {
             const int r = wave + TF_WAVES * e;
             if (r >= rows) break;
             const float2 angle = a.rope ? angles[r / group * 64 + lane] : make_float2(1.0f, 0.0f);
@@ -761,7 +791,7 @@ __global__ __launch_bounds__(TF_WAVES * 64) __attribute__((amdgpu_waves_per_eu(1
             for (int k = 0; k < 2; ++k) {
                 const uint32_t hi = f32_to_bf16_bits(y[k]);
                 qs[r * TF_QROW + lane + 64 * k] = (uint16_t)hi;
-                qs[(TF_ROWS + r) * TF_QROW + lane + 64 * k] = (uint16_t)f32_to_bf16_bits(y[k] - bf16_bits_to_f32(hi));
+                qs[(ROWS + r) * TF_QROW + lane + 64 * k] = (uint16_t)f32_to_bf16_bits(y[k] - bf16_bits_to_f32(hi));
             }
         }
         if (has_nodes) {
@@ -770,18 +800,17 @@ __global__ __launch_bounds__(TF_WAVES * 64) __attribute__((amdgpu_waves_per_eu(1
             uint16_t* const fk = reinterpret_cast<uint16_t*>(fresh[0]);
             uint32_t* const fv = reinterpret_cast<uint32_t*>(fresh[1]);
 #pragma unroll
-            for (int e = 0; e < TF_EACH; ++e) {
+            for (int e = 0; e < EACH; ++e) {
                 const int i = wave + TF_WAVES * e;
                 if (i >= (int)a.n) break;
-                const uint64_t line = readlane64(lines, i);
                 uint32_t v = 0;
                 float r0 = 0.0f, r1 = 0.0f;
-                if (line) {
+                if (readlane64(lines, i)) {
                     const float2 angle = a.rope ? angles[i * 64 + lane] : make_float2(1.0f, 0.0f);
                     q8_norm_rope(k0[e], k1[e], has_w, kw0, kw1, a.eps, angle.x, angle.y, r0, r1);
                     v = pack_bf16x2(v0[e], v1[e]);
                     // (where the nodes lie across two units both have them; one writes)
-                    if (len + i >= u.tile0 * S::KEYS && len + i < u.tile1 * S::KEYS) {
+                    if (len + i >= u.tile0 * TF_KEYS && len + i < u.tile1 * TF_KEYS) {
                         const size_t slot = ((size_t)len + i) * step + (size_t)h * TA_D;
                         uint16_t* const y = a.k_cache + seq * a.k_seq + slot + lane;
                         y[0] = (uint16_t)f32_to_bf16_bits(r0);
@@ -792,7 +821,7 @@ __global__ __launch_bounds__(TF_WAVES * 64) __attribute__((amdgpu_waves_per_eu(1
                 }
                 fk[key_at(i, lane)] = (uint16_t)f32_to_bf16_bits(r0);
                 fk[key_at(i, lane + 64)] = (uint16_t)f32_to_bf16_bits(r1);
-                fv[i * 64 + ((lane >> 2 ^ (i & 3) << 2) << 2 | (lane & 3))] = v;
+                fv[i * 64 + ((lane >> 2 ^ (i & 7) << 1) << 2 | (lane & 3))] = v;
             }
             if (wave == 0) fv[a.n * 64 + lane] = 0u;
 #pragma unroll
@@ -804,141 +833,127 @@ __global__ __launch_bounds__(TF_WAVES * 64) __attribute__((amdgpu_waves_per_eu(1
     }
     const int broken = __syncthreads_or((bad[0][0] | bad[0][1] | bad[0][2] | bad[1][0] | bad[1][1] | bad[1][2]) != 0);
 
-    ta_f32x16 o[4];
+    ta_f32x4 o[CB][8];
+    float m_run[CB], l_part[CB];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int b = 0; b < CB; ++b) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) o[i][e] = 0.0f;
-    float m_run = -INFINITY, l_part = 0.0f;
+        for (int i = 0; i < 8; ++i) o[b][i] = ta_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        m_run[b] = -INFINITY;
+        l_part[b] = 0.0f;
+    }
     if (tiles > 0) {
-        ta_bf16x8 qh[8], ql[8];
-        const int r = min(lane & 31, rows - 1);
+        // dims 32 s + 8 (lane / 16) .. of row 16 b + lane % 16
+        ta_bf16x8 qh[CB][4], ql[CB][4];
+        uint32_t line[CB];
 #pragma unroll
-        for (int s = 0; s < 8; ++s) {
-            qh[s] = *reinterpret_cast<const ta_bf16x8*>(qs + r * TF_QROW + 16 * s + 8 * half);
-            ql[s] = *reinterpret_cast<const ta_bf16x8*>(qs + (TF_ROWS + r) * TF_QROW + 16 * s + 8 * half);
+        for (int b = 0; b < CB; ++b) {
+            const int r = min(16 * b + lp, rows - 1);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                qh[b][s] = *reinterpret_cast<const ta_bf16x8*>(qs + r * TF_QROW + 32 * s + 8 * lr);
+                ql[b][s] = *reinterpret_cast<const ta_bf16x8*>(qs + (ROWS + r) * TF_QROW + 32 * s + 8 * lr);
+            }
+            line[b] = (uint32_t)__shfl((int)lines, r / group);  // up to 32 nodes
         }
-        const uint32_t line = (uint32_t)__shfl((int)lines, r / group);  // up to 32 nodes
-        // every load that the compiler counts has landed, and the second stage is free
+        // every load that the compiler counts has landed; the second stage is free
         wait_vm<0>();
         wait_lgkm0();
-        __syncthreads();
-        const int krow = 32 * wave + (lane & 31), n16 = lane & 15;
-        const int vr = 4 * half + (n16 >> 2), vpiece = 2 * ((lane >> 4) & 1) + ((n16 & 3) >> 1);
-        const uint32_t fresh_at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)&fresh[0][0]);
+        asm volatile("" ::: "memory");
+        if (!APART) {
+            __syncthreads();
+            if (tiles > 1) load(1);
+        }
+        const int vj = 4 * lr + (lp >> 2), vpiece = (lp & 3) >> 1;
+        const uint32_t fresh_at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(ta_lds*)&fresh[0][0]);
         for (int it = 0; it < tiles; ++it) {
-            const int t0 = (u.tile0 + it) * S::KEYS + 32 * wave;
-            if (it + 1 < tiles) {
-                load(it + 1);
-                wait_vm<S::PER>();
-            } else {
-                wait_vm<0>();
-            }
+            const int t0 = (u.tile0 + it) * TF_KEYS + 16 * wave;
+            if (it + 1 < tiles) wait_vm<8>();
+            else wait_vm<0>();
             asm volatile("" ::: "memory");
-            if (t0 >= len + count) continue;  // behind the nodes: nothing
-            const bool edge = t0 + 32 > len;
-            const uint32_t stage = base + (uint32_t)(it & 1) * S::STAGE;
-            // where this lane reads: a key's row, and four values' rows, of the tile or of the nodes
-            uint32_t ka = stage + (uint32_t)krow * TA_ROW_BYTES, kf = (uint32_t)krow & 15, va[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) va[i] = stage + S::KEYS * TA_ROW_BYTES + (uint32_t)(32 * wave + vr + 8 * i) * TA_ROW_BYTES;
-            uint32_t vf[4] = {(uint32_t)vr & 3, (uint32_t)vr & 3, (uint32_t)vr & 3, (uint32_t)vr & 3};
-            if (edge) {
-                const int jk = t0 + (lane & 31) - len;
-                if (jk >= 0) {
-                    ka = fresh_at + (uint32_t)min(jk, (int)a.n) * TA_ROW_BYTES;
-                    kf = (uint32_t)min(jk, (int)a.n) & 15;
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int jv = t0 + vr + 8 * i - len;
+            if (t0 < len + count) {
+                const bool edge = t0 + 16 > len;
+                const uint32_t stage = base + (uint32_t)(it & 1) * TF_STAGE + wave * 16 * TA_ROW_BYTES;
+                // where this lane reads: a key's row and a value's, of the tile or of the nodes
+                uint32_t ka = stage + (uint32_t)lp * TA_ROW_BYTES, kf = (uint32_t)lp;
+                uint32_t va = stage + TF_KEYS * TA_ROW_BYTES + (uint32_t)vj * TA_ROW_BYTES, vf = (uint32_t)vj & 7;
+                if (edge) {
+                    const int jk = min(t0 + lp - len, (int)a.n), jv = min(t0 + vj - len, (int)a.n);
+                    if (jk >= 0) {
+                        ka = fresh_at + (uint32_t)jk * TA_ROW_BYTES;
+                        kf = (uint32_t)jk & 15;
+                    }
                     if (jv >= 0) {
-                        va[i] = fresh_at + (TF_ROWS + 1) * TA_ROW_BYTES + (uint32_t)min(jv, (int)a.n) * TA_ROW_BYTES;
-                        vf[i] = (uint32_t)min(jv, (int)a.n) & 3;
+                        va = fresh_at + (uint32_t)(ROWS + 1 + jv) * TA_ROW_BYTES;
+                        vf = (uint32_t)jv & 7;
                     }
                 }
-            }
-            typedef __attribute__((address_space(3))) uint8_t lds_u8;
-            ta_f32x16 s;
+                ta_bf16x8 kr[4];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) s[e] = 0.0f;
+                for (int s = 0; s < 4; ++s) kr[s] = *(const __attribute__((address_space(3))) ta_bf16x8*)(ta_lds*)(uintptr_t)(ka + (((4 * s + lr) ^ kf) << 4));
+                uint2 vr[8];
 #pragma unroll
-            for (int st = 0; st < 8; ++st) {
-                const ta_bf16x8 kr = *(const __attribute__((address_space(3))) ta_bf16x8*)(lds_u8*)(uintptr_t)(ka + (((2 * st + half) ^ kf) << 4));
-                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kr, qh[st], s, 0, 0, 0);
-                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kr, ql[st], s, 0, 0, 0);
-            }
-            if (edge) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int j = t0 + 8 * (e >> 2) + 4 * half + (e & 3) - len;
-                    const bool seen = j < 0 || (j < 32 && (line >> (j & 31) & 1));
-                    s[e] = seen ? s[e] : -INFINITY;
+                for (int d = 0; d < 8; ++d) {
+                    const uint32_t at = va + (((uint32_t)(2 * d + vpiece) ^ (vf << 1)) << 4) + 8 * (lp & 1);
+                    vr[d] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) t2h_v4i16*)(ta_lds*)(uintptr_t)at));
                 }
-            }
-            float mt = -INFINITY;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[e]);
-            mt = xor_max<32>(mt * a.scale_log2);
-            const bool grow = mt > m_run + TA_RESCALE;
-            const float m_new = grow ? mt : m_run;
-            const float alpha = grow ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
-            const float msub = m_new == -INFINITY ? 0.0f : m_new;
-            m_run = m_new;
-            uint32_t pk[8];
-            float lsum = 0.0f;
+                for (int b = 0; b < CB; ++b) {
+                    ta_f32x4 sh = ta_f32x4{0.0f, 0.0f, 0.0f, 0.0f}, sl = sh;
 #pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-                const float p0 = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2, -msub));
-                const float p1 = __builtin_amdgcn_exp2f(fmaf(s[e + 1], a.scale_log2, -msub));
-                lsum += p0 + p1;
-                pk[e / 2] = pack_bf16x2(p0, p1);
-            }
-            l_part = fmaf(l_part, alpha, lsum);
-            if (__builtin_amdgcn_ballot_w64(grow) != 0) {
+                    for (int s = 0; s < 4; ++s) {
+                        sh = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kr[s], qh[b][s], sh, 0, 0, 0);
+                        sl = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kr[s], ql[b][s], sl, 0, 0, 0);
+                    }
+                    sh += sl;
+                    if (edge) {
+                        const uint32_t seen = tree_seen(line[b], t0 + 4 * lr - len);
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                        for (int e = 0; e < 4; ++e) sh[e] = seen & 1u << e ? sh[e] : -INFINITY;
+                    }
+                    float mt = fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3])) * a.scale_log2;
+                    mt = xor_max<32>(xor_max<16>(mt));
+                    const bool grow = mt > m_run[b] + TA_RESCALE;
+                    const float m_new = grow ? mt : m_run[b], alpha = grow ? __builtin_amdgcn_exp2f(m_run[b] - m_new) : 1.0f;
+                    const float msub = m_new == -INFINITY ? 0.0f : m_new;
+                    m_run[b] = m_new;
+                    float pe[4];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) o[i][e] *= alpha;
-            }
+                    for (int e = 0; e < 4; ++e) pe[e] = __builtin_amdgcn_exp2f(fmaf(sh[e], a.scale_log2, -msub));
+                    l_part[b] = fmaf(l_part[b], alpha, (pe[0] + pe[1]) + (pe[2] + pe[3]));
+                    if (__builtin_amdgcn_ballot_w64(grow) != 0) {
 #pragma unroll
-            for (int stp = 0; stp < 2; ++stp) {
-                const ta_bf16x8 pf =
-                    __builtin_bit_cast(ta_bf16x8, make_uint4(pk[4 * stp], pk[4 * stp + 1], pk[4 * stp + 2], pk[4 * stp + 3]));
+                        for (int i = 0; i < 8; ++i) o[b][i] *= alpha;
+                    }
+                    const ta_s16x4 pf = __builtin_bit_cast(ta_s16x4, make_uint2(pack_bf16x2(pe[0], pe[1]), pack_bf16x2(pe[2], pe[3])));
 #pragma unroll
-                for (int db = 0; db < 4; ++db) {
-                    auto value = [&](int i) {
-                        const uint32_t at = va[i] + (((uint32_t)(4 * db + vpiece) ^ (vf[i] << 2)) << 4) + 8 * (n16 & 1);
-                        return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) t2h_v4i16*)(lds_u8*)(uintptr_t)at));
-                    };
-                    const uint2 x = value(2 * stp), y = value(2 * stp + 1);
-                    o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(ta_bf16x8, make_uint4(x.x, x.y, y.x, y.y)), pf, o[db], 0, 0, 0);
+                    for (int d = 0; d < 8; ++d)
+                        o[b][d] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(ta_s16x4, vr[d]), pf, o[b][d], 0, 0, 0);
                 }
             }
             wait_lgkm0();  // the buffer is read before it is loaded again
             asm volatile("" ::: "memory");
+            if (it + 2 < tiles) load(it + 2);
         }
     }
 
-    // join the waves
-    const float l = xor_sum<32>(l_part);
-    wait_vm<0>();
+    // join the waves: lane holds dims 16 d + 4 (lane / 16) .. of row 16 b + lane % 16
     wait_lgkm0();
     __syncthreads();
     float* const os = reinterpret_cast<float*>(lds);
-    if (half == 0) {
-        wml[wave][lane][0] = m_run;
-        wml[wave][lane][1] = l;
+#pragma unroll
+    for (int b = 0; b < CB; ++b) {
+        const float l = xor_sum<32>(xor_sum<16>(l_part[b]));
+        if (lr == 0) {
+            wml[wave][16 * b + lp][0] = m_run[b];
+            wml[wave][16 * b + lp][1] = l;
+        }
+#pragma unroll
+        for (int d = 0; d < 8; ++d) *reinterpret_cast<ta_f32x4*>(os + (wave * ROWS + 16 * b + lp) * TF_OROW + 16 * d + 4 * lr) = o[b][d];
     }
-#pragma unroll
-    for (int db = 0; db < 4; ++db)
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-            *reinterpret_cast<ta_f32x4*>(os + (wave * 32 + (lane & 31)) * S::OROW + 32 * db + 8 * g + 4 * half) =
-                ta_f32x4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
     __syncthreads();
     const bool whole = u.parts == 1;
-    const int node0 = max(u.tile0 * S::KEYS - len, 0), node1 = min(u.tile1 * S::KEYS - len, 32);
+    const int node0 = max(u.tile0 * TF_KEYS - len, 0), node1 = min(u.tile1 * TF_KEYS - len, 32);
     const uint32_t here = broken && node1 > node0 ? (~0u >> (32 - (node1 - node0))) << node0 : 0;
     auto put = [&](int r, int d, ta_f32x4 sum, float L, bool node) {
         uint2 y = make_uint2(0u, 0u);
@@ -948,11 +963,11 @@ __global__ __launch_bounds__(TF_WAVES * 64) __attribute__((amdgpu_waves_per_eu(1
         }
         *reinterpret_cast<uint2*>(a.out + (((size_t)seq * a.n + r / group) * a.nh + h * group + r % group) * TA_D + d) = y;
     };
-    // this (sequence, head)'s parts: maxima and sums, then rows
-    const size_t part_bytes = (size_t)TF_ROWS * (TA_D + 4) * 4;
-    uint8_t* const parts = reinterpret_cast<uint8_t*>(a.part_o) + ((size_t)u.first * a.nk + (size_t)h * u.parts) * part_bytes;
-    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(parts, 0, (int)min((size_t)u.parts * part_bytes, (size_t)0x7fffffff), 0x00027000);
-    for (int i = tid; i < TF_ROWS * 32; i += TF_WAVES * 64) {
+    // this (sequence, head)'s parts, rows of ROWS each
+    constexpr int PART = ROWS * TF_PART;
+    uint8_t* const parts = reinterpret_cast<uint8_t*>(a.part_o) + ((size_t)u.first * a.nk + (size_t)h * u.parts) * PART;
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(parts, 0, u.parts * PART, 0x00027000);
+    for (int i = tid; i < ROWS * 32; i += TF_WAVES * 64) {
         const int r = i >> 5, d = (i & 31) * 4;
         if (r >= (whole ? all : rows)) break;
         float M = -INFINITY, L = 0.0f;
@@ -964,9 +979,9 @@ __global__ __launch_bounds__(TF_WAVES * 64) __attribute__((amdgpu_waves_per_eu(1
         for (int w = 0; w < TF_WAVES; ++w) {
             const float f = __builtin_amdgcn_exp2f(wml[w][r][0] - msub);
             L = fmaf(f, wml[w][r][1], L);
-            sum += *reinterpret_cast<const ta_f32x4*>(os + (w * 32 + r) * S::OROW + d) * f;
+            sum += *reinterpret_cast<const ta_f32x4*>(os + (w * ROWS + r) * TF_OROW + d) * f;
         }
-        const uint32_t line = (uint32_t)__shfl((int)lines, r / group);
+        const uint32_t line = (uint32_t)__shfl((int)lines, r / group);  // (of a wave's two rows the first one's lanes are there)
         if (line & here) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -975,7 +990,7 @@ __global__ __launch_bounds__(TF_WAVES * 64) __attribute__((amdgpu_waves_per_eu(1
         if (whole) {
             put(r, d, sum, L, line != 0);
         } else {
-            const int at = u.part * (int)part_bytes + r * (TA_D + 4) * 4;
+            const int at = u.part * PART + r * TF_PART;
             __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(ta_u32x4, sum), rsrc, at + 16 + d * 4, 0, TF_AGENT);
             if (d == 0) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(ta_u32x4, ta_f32x4{M, L, 0.0f, 0.0f}), rsrc, at, 0, TF_AGENT);
         }
@@ -992,53 +1007,70 @@ __global__ __launch_bounds__(TF_WAVES * 64) __attribute__((amdgpu_waves_per_eu(1
     if (arrived != (uint32_t)u.parts) return;
     // slices of the parts, where rows are few; 8 parts of a slice on their way at a time
     const int pieces = rows * 32, slices = TF_WAVES * 64 / pieces > 0 ? TF_WAVES * 64 / pieces : 1;
-    constexpr int BATCH = 8;
-    for (int i = tid; i < pieces * slices; i += TF_WAVES * 64) {
-        const int slice = i / pieces, r = i % pieces / 32, d = i % 32 * 4;
-        float M = -INFINITY, L = 0.0f;
-        ta_f32x4 sum = ta_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        for (int n0 = slice; n0 < u.parts; n0 += slices * BATCH) {
-            ta_u32x4 ml[BATCH], x[BATCH];
+    constexpr int BATCH = 8, TURNS = (ROWS * 32 + TF_WAVES * 64 - 1) / (TF_WAVES * 64);
+    float M[TURNS], L[TURNS];
+    ta_f32x4 sum[TURNS];
+#pragma unroll
+    for (int k = 0; k < TURNS; ++k) {
+        M[k] = -INFINITY;
+        L[k] = 0.0f;
+        sum[k] = ta_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    const int slice = tid / pieces;  // (in one turn only where there are several)
+    for (int n0 = slice; n0 < u.parts && slice < slices; n0 += slices * BATCH) {
+        ta_u32x4 ml[TURNS][BATCH], x[TURNS][BATCH];
+#pragma unroll
+        for (int k = 0; k < TURNS; ++k) {
+            const int i = min(tid - slice * pieces + k * TF_WAVES * 64, pieces - 1);
 #pragma unroll
             for (int e = 0; e < BATCH; ++e) {
-                const int at = min(n0 + slices * e, u.parts - 1) * (int)part_bytes + r * (TA_D + 4) * 4;
-                ml[e] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, 0, TF_AGENT);
-                x[e] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, at + 16 + d * 4, 0, TF_AGENT);
+                const int at = min(n0 + slices * e, u.parts - 1) * PART + (i >> 5) * TF_PART;
+                ml[k][e] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, 0, TF_AGENT);
+                x[k][e] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, at + 16 + (i & 31) * 16, 0, TF_AGENT);
             }
+        }
+#pragma unroll
+        for (int k = 0; k < TURNS; ++k)
 #pragma unroll
             for (int e = 0; e < BATCH; ++e) {
                 if (n0 + slices * e >= u.parts) break;
-                const ta_f32x4 q = __builtin_bit_cast(ta_f32x4, ml[e]);
-                const float now = fmaxf(M, q[0]), msub = now == -INFINITY ? 0.0f : now;
-                const float keep = __builtin_amdgcn_exp2f(M - msub), f = __builtin_amdgcn_exp2f(q[0] - msub);
-                L = fmaf(L, keep, f * q[1]);
-                sum = sum * keep + __builtin_bit_cast(ta_f32x4, x[e]) * f;
-                M = now;
+                const ta_f32x4 q = __builtin_bit_cast(ta_f32x4, ml[k][e]);
+                const float now = fmaxf(M[k], q[0]), msub = now == -INFINITY ? 0.0f : now;
+                const float keep = __builtin_amdgcn_exp2f(M[k] - msub), f = __builtin_amdgcn_exp2f(q[0] - msub);
+                L[k] = fmaf(L[k], keep, f * q[1]);
+                sum[k] = sum[k] * keep + __builtin_bit_cast(ta_f32x4, x[k][e]) * f;
+                M[k] = now;
             }
-        }
-        if (slices == 1) {
-            put(r, d, sum, L, (uint32_t)__shfl((int)lines, r / group) != 0);
-        } else {
-            *reinterpret_cast<ta_f32x4*>(os + (slice * 32 + r) * S::OROW + d) = sum;  // (up to 8 slices of up to 4 rows)
-            if (d == 0) {
-                wml[slice & 3][(slice >> 2) * 16 + r][0] = M;
-                wml[slice & 3][(slice >> 2) * 16 + r][1] = L;
-            }
-        }
     }
-    __syncthreads();
-    if (slices > 1 && tid < pieces) {
-        const int r = tid / 32, d = tid % 32 * 4;
-        float M = -INFINITY, L = 0.0f;
-        for (int n = 0; n < slices; ++n) M = fmaxf(M, wml[n & 3][(n >> 2) * 16 + r][0]);
-        const float msub = M == -INFINITY ? 0.0f : M;
-        ta_f32x4 sum = ta_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        for (int n = 0; n < slices; ++n) {
-            const float f = __builtin_amdgcn_exp2f(wml[n & 3][(n >> 2) * 16 + r][0] - msub);
-            L = fmaf(f, wml[n & 3][(n >> 2) * 16 + r][1], L);
-            sum += *reinterpret_cast<const ta_f32x4*>(os + (n * 32 + r) * S::OROW + d) * f;
+    if (slices == 1) {
+#pragma unroll
+        for (int k = 0; k < TURNS; ++k) {
+            const int i = tid + k * TF_WAVES * 64;
+            const bool node = __shfl((int)lines, min(i, pieces - 1) / 32 / group) != 0;
+            if (i < pieces) put(i >> 5, (i & 31) * 4, sum[k], L[k], node);
         }
-        put(r, d, sum, L, (uint32_t)__shfl((int)lines, r / group) != 0);
+    } else {
+        const int i = tid - slice * pieces, r = i >> 5, d = (i & 31) * 4;
+        if (slice < slices) {
+            *reinterpret_cast<ta_f32x4*>(os + (slice * rows + r) * TF_OROW + d) = sum[0];  // (slices times rows are up to 16)
+            if (d == 0) {
+                wml[slice & 7][(slice >> 3) * 8 + r][0] = M[0];
+                wml[slice & 7][(slice >> 3) * 8 + r][1] = L[0];
+            }
+        }
+        __syncthreads();
+        if (tid < pieces) {
+            float top = -INFINITY, under = 0.0f;
+            for (int n = 0; n < slices; ++n) top = fmaxf(top, wml[n & 7][(n >> 3) * 8 + r][0]);
+            const float msub = top == -INFINITY ? 0.0f : top;
+            ta_f32x4 y = ta_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int n = 0; n < slices; ++n) {
+                const float f = __builtin_amdgcn_exp2f(wml[n & 7][(n >> 3) * 8 + r][0] - msub);
+                under = fmaf(f, wml[n & 7][(n >> 3) * 8 + r][1], under);
+                y += *reinterpret_cast<const ta_f32x4*>(os + (n * rows + r) * TF_OROW + d) * f;
+            }
+            put(r, d, y, under, __shfl((int)lines, r / group) != 0);
+        }
     }
     // rows that are no nodes
     for (int i = rows * 32 + tid; i < all * 32; i += TF_WAVES * 64) put(i / 32, i % 32 * 4, ta_f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 1.0f, false);
@@ -1046,15 +1078,14 @@ __global__ __launch_bounds__(TF_WAVES * 64) __attribute__((amdgpu_waves_per_eu(1
 
 // ------------------------------------------------------------------------------------------------------ launch --
 
-// Rows of a KV head that one thread block takes: 32, 64, 128 or 256, for more of them several.
-static uint32_t ta_tile_rows(uint32_t rows) { return rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256; }
+// Rows of a KV head that one thread block takes: 16, 32, 64, 128 or 256, for more of them several.
+static uint32_t ta_tile_rows(uint32_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256; }
 
 struct TreeSizes {
-    uint32_t tile_rows, row_tiles, rows, keys, least, extra, slots, units;
+    uint32_t tile_rows, row_tiles, rows, keys, least, units;
+    float us_turn, us_tile, us_shared, us_join;
     size_t done, qh, ql, line, vt, broken, which, table, of_seq, part_ml, part_o, end;
 };
-
-constexpr uint32_t TA_CUS = 256;
 
 static TreeSizes ta_sizes(uint32_t n_seq, uint32_t n, uint32_t nh, uint32_t nk, uint32_t s_cap) {
     TreeSizes s = {};
@@ -1064,9 +1095,13 @@ static TreeSizes ta_sizes(uint32_t n_seq, uint32_t n, uint32_t nh, uint32_t nk, 
     s.rows = s.row_tiles * s.tile_rows;
     s.keys = s.tile_rows <= 64 ? 128 : s.tile_rows == 128 ? 64 : 32;
     s.least = s.tile_rows <= 64 ? 1 : s.tile_rows == 128 ? 4 : 8;
-    s.extra = s.tile_rows <= 64 ? 2 : s.tile_rows == 128 ? 4 : 6;
-    s.slots = TA_CUS / (nk * s.row_tiles) > 1 ? TA_CUS / (nk * s.row_tiles) : 1;
-    const uint64_t most = (uint64_t)n_seq * ((s_cap + s.keys - 1) / s.keys), some = (uint64_t)4 * s.slots + n_seq;
+    // measured, in us (a tile of 64 KiB a CU where all read: 6.4 TB/s)
+    s.us_shared = 2.6f * (float)s.keys / 128.0f;
+    s.us_turn = s.tile_rows <= 16 ? 8.0f : s.tile_rows == 32 ? 10.0f : 9.0f;
+    s.us_tile = s.tile_rows <= 16 ? 0.7f : s.tile_rows == 32 ? 1.0f : s.tile_rows == 64 ? 1.2f : s.tile_rows == 128 ? 0.62f : 1.05f;
+    s.us_join = s.tile_rows <= 16 ? 3.5f : s.tile_rows == 32 ? 4.0f : 2.0f;
+    const uint32_t slots = TA_CUS / (nk * s.row_tiles) > 1 ? TA_CUS / (nk * s.row_tiles) : 1;
+    const uint64_t most = (uint64_t)n_seq * ((s_cap + s.keys - 1) / s.keys), some = slots > n_seq + slots / 2 ? slots : n_seq + slots / 2;
     s.units = (uint32_t)(most < some ? most : some);
     size_t at = 0;
     const size_t counters = (size_t)n_seq * nk;  // first, and as many for every shape up to 16384 of them: calls may share a workspace
@@ -1077,7 +1112,7 @@ static TreeSizes ta_sizes(uint32_t n_seq, uint32_t n, uint32_t nh, uint32_t nk, 
     };
     const size_t q = (size_t)n_seq * n * nh * TA_D * 2, heads = (size_t)n_seq * nk, parts = (size_t)s.units * nk * s.rows;
     s.done = take((counters > 16384 ? counters : 16384) * 4);
-    if (s.tile_rows == 32) {  // one launch
+    if (s.tile_rows <= 32) {  // one launch
         s.part_o = take(parts * (TA_D + 4) * 4);
         s.end = at;
         return s;
@@ -1172,10 +1207,12 @@ extern "C" int t2h_attn_tree(const float* q, uint64_t q_row, const float* k_new,
     a.n_units = s.units;
     a.row_tiles = s.row_tiles;
     a.rows = s.rows;
-    a.slots = s.slots;
     a.keys = s.keys;
     a.least = s.least;
-    a.extra = s.extra;
+    a.us_turn = s.us_turn;
+    a.us_tile = s.us_tile;
+    a.us_shared = s.us_shared;
+    a.us_join = s.us_join;
     const uint64_t waves = (uint64_t)n_seq * n * ((nh + TP_HEADS - 1) / TP_HEADS), kv = (uint64_t)n_seq * nk * ((n + TP_NODES - 1) / TP_NODES);
     const uint64_t grid = (uint64_t)s.units * nk * s.row_tiles, joins = ((uint64_t)n_seq * n * nh + 3) / 4;
     if (kv + waves > 0x3fffffffu || grid > 0x7fffffffu || joins > 0x3fffffffu) return T2H_ERR_SHAPE;
@@ -1183,8 +1220,9 @@ extern "C" int t2h_attn_tree(const float* q, uint64_t q_row, const float* k_new,
     a.q_blocks = (uint32_t)((waves + 3) / 4);
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     const dim3 g((uint32_t)grid);
-    if (s.tile_rows == 32) {
-        hipLaunchKernelGGL(tree_few_kernel, g, dim3(TF_WAVES * 64), 0, st, a);
+    if (s.tile_rows <= 32) {
+        if (s.tile_rows == 16) hipLaunchKernelGGL(tree_few_kernel<1>, g, dim3(TF_WAVES * 64), 0, st, a);
+        else hipLaunchKernelGGL(tree_few_kernel<2>, g, dim3(TF_WAVES * 64), 0, st, a);
         T2H_LAUNCH_CHECK();
         return T2H_OK;
     }
