@@ -30,6 +30,9 @@ src/models/optimized_qwen3/tensors/model.py:104-150, in bf16 instead of fp16).
 
 from __future__ import annotations
 
+from collections.abc import Callable, Sequence
+from dataclasses import dataclass
+
 import torch
 
 from torch2vk_amd import kernels
@@ -53,6 +56,14 @@ def _check_types(c: Qwen3Config, types: dict[str, str]) -> None:
             raise NotImplementedError(f"{name}: no {t} decode kernel (built: {allowed[name]})")
 
 
+@dataclass(frozen=True)
+class _TreeRoom:
+    """Workspaces of a tree_step of one number of nodes."""
+
+    attn: torch.Tensor
+    verify: torch.Tensor
+
+
 class Qwen3Decoder:
     """Greedy decoder over libt2h.  ``persistent`` selects how a token's layers run: one persistent launch
     for all of them (t2h_qwen3_decode_layers: the 8B and 0.6B shapes with Q4_K weights, v and down Q4_K or
@@ -65,7 +76,10 @@ class Qwen3Decoder:
     persistent kernel over a bf16 cache.  Such a cache goes on from its length only: ``start`` of a prefill is 0 or the
     tokens it holds (``position``, which is read back to see), a ``cache_position`` one of these or the next, and step_logits
     and forward_masked are refused.  With ``kv_weights`` it also keeps each token's accumulated attention weight, by which
-    ``evict_cache`` cuts it down."""
+    ``evict_cache`` cuts it down.
+
+    ``tree_step`` decodes one token and a tree of drafted ones in one pass over the weights and keeps the ones that the model
+    would have chosen; ``generate_tree`` loops over it."""
 
     PREFILL_GRAPHS = 4  # captured prefill graphs kept (prefill_graphed)
 
@@ -133,6 +147,7 @@ class Qwen3Decoder:
         self.stop_on_eos = True
         self._graphs: dict[int, torch.cuda.CUDAGraph] = {}
         self._prefill_graphs: dict[tuple[int, int, int, bool], tuple[torch.cuda.CUDAGraph, torch.Tensor]] = {}
+        self._tree_rooms: dict[tuple[int, bool], _TreeRoom] = {}
         self.persistent = False
         self.status = torch.zeros(1, dtype=torch.int32, device=dev)
         if persistent is not False:
@@ -408,6 +423,90 @@ class Qwen3Decoder:
         for _ in range(rest):
             self.decode_step()
 
+    # ------------------------------------------- trees of drafted tokens --
+
+    def _tree_room(self, n: int, drawn: bool) -> _TreeRoom:
+        """Allocated by the first step of n nodes, which is not a captured one: a graph's own memory is its replays' alone."""
+        if (n, drawn) not in self._tree_rooms:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"run a tree_step of {n} nodes before capturing one")
+            c = self.config
+            self._tree_rooms[n, drawn] = _TreeRoom(
+                kernels.attn_tree_workspace(1, n, c.heads, c.kv_heads, c.head_dim, self.max_positions, self.device),
+                kernels.tree_verify_workspace(1, n, c.vocab, self.device, drawn=drawn))
+        return self._tree_rooms[n, drawn]
+
+    def tree_step(self, drafts: torch.Tensor, *, parents: torch.Tensor | None = None, temperature: float | torch.Tensor = 0.0,
+                  uniforms: torch.Tensor | None = None, draft_logits: torch.Tensor | None = None
+                  ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """One step over ``next_token`` and up to 63 drafted tokens, int64 [m]: all nodes through every layer at once
+        (kernels.attn_tree), the LM head's logits after each, the accepted path and the token that follows it
+        (kernels.tree_verify: greedy, or by ``temperature`` and ``uniforms`` fp32 [1 + m]), the path's rows kept in the cache
+        (kernels.tree_keep); its tokens and the one that follows are stored, position goes on by the path's nodes.
+        ``parents`` int32 [1 + m] as kernels.attn_tree has them, the first of them -1 for next_token (None: a chain);
+        ``draft_logits`` fp32 [m, vocab]: a chain drawn from them.  Everything stays on the device: a step can be captured, once
+        one of as many nodes has run.  Nodes that the cache has no slot for are none.  Returns path int32 [1 + m], kept int32
+        [1] and the logits fp32 [1 + m, vocab]."""
+        c = self.config
+        if self.kv_bits != 16:
+            raise NotImplementedError("a tree's nodes attend over a bf16 KV cache")
+        if not isinstance(drafts, torch.Tensor) or drafts.dtype != torch.int64 or drafts.dim() != 1:
+            raise ValueError("drafts must be int64 [m]")
+        n = 1 + drafts.shape[0]
+        if n > kernels.TREE_MAX_NODES:
+            raise ValueError(f"a step has up to {kernels.TREE_MAX_NODES} nodes, got {n}")
+        if drafts.device != self.position.device:
+            raise ValueError(f"drafts are on {drafts.device}, the decoder is on {self.position.device}")
+        for t, name, shape in ((parents, "parents", (n,)), (uniforms, "uniforms", (n,)), (draft_logits, "draft_logits", (n - 1, c.vocab))):
+            if t is not None and tuple(t.shape) != shape:
+                raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
+        if parents is not None and draft_logits is not None:
+            raise ValueError("drawn drafts are a chain: pass draft_logits or parents")
+        if uniforms is None and (isinstance(temperature, torch.Tensor) or temperature != 0):
+            raise ValueError("sampling needs uniforms")
+        room = self._tree_room(n, draft_logits is not None)
+        tokens = torch.cat([self.next_token.view(-1), drafts])
+        h = self.embed_tokens(tokens)
+        up = None if parents is None else parents.view(1, n)
+        for i in range(c.layers):
+            self._prefill_layer(i, h, 0, tree=room, parents=up)
+        x = kernels.rms_norm(h, self._n("norm"), out=torch.empty(n, c.hidden, dtype=torch.bfloat16, device=self.device),
+                             eps=c.rms_eps)
+        logits = kernels.quantized_linear(x, self._w("lm_head"), self.types["lm_head"], out_dtype=torch.float32)
+        path, kept, following = kernels.tree_verify(
+            logits.view(1, n, c.vocab), tokens.view(1, n), room.verify, temperature=temperature,
+            uniforms=None if uniforms is None else uniforms.view(1, n), parents=up, counts=self._tree_slots(n),
+            draft_logits=None if draft_logits is None else draft_logits.view(1, n - 1, c.vocab))
+        kernels.tree_keep(self.k_cache.unsqueeze(1), self.v_cache.unsqueeze(1), path, kept, self.position)
+        self._store_path(tokens, path.view(-1), kept, following)
+        return path.view(-1), kept, logits
+
+    def _tree_slots(self, n: int) -> torch.Tensor:
+        """Of n nodes those with a slot: the others' rows of the attention are zeros, their logits no one's."""
+        return (self.max_positions - self.position).clamp(0, n)
+
+    def _store_path(self, tokens: torch.Tensor, path: torch.Tensor, kept: torch.Tensor, following: torch.Tensor) -> None:
+        """token_store for the tokens that a tree step decided: the path's behind its first node, then ``following``, up to the
+        first that ends the text."""
+        n = path.numel()
+        j = torch.arange(n, device=self.device)
+        then = torch.cat([path[1:], path[:1]]).long().clamp(min=0)
+        new = torch.where(j + 1 < kept, tokens[then], following)
+        ends = (new[:, None] == self.eos).any(1)
+        live = (j < kept) & (new >= 0) & (j + self.length < self.generated.numel())
+        if self.stop_on_eos:
+            live &= (torch.cumsum(ends, 0) - ends.long() == 0) & (self.stopped == 0)
+        count = live.sum(dtype=torch.int32)
+        at = torch.arange(self.generated.numel(), device=self.device) - self.length
+        self.generated.copy_(torch.where((at >= 0) & (at < count), new[at.clamp(0, n - 1)], self.generated))
+        self.length += count
+        self.position += kept
+        self.next_token.copy_(torch.where(kept > 0, following, self.next_token.view(-1)).view(1, 1))
+        ended = (ends & live).any()
+        self.done.copy_(ended.view(1))
+        if self.stop_on_eos:
+            self.stopped.copy_((self.stopped != 0) | ended)
+
     # ------------------------------------------------------- generate --
 
     def prefill(self, prompt_ids: torch.Tensor, start: int = 0) -> None:
@@ -436,13 +535,15 @@ class Qwen3Decoder:
         return q.as_strided((rows, q.shape[1]), (q.shape[1], 1))
 
     def _prefill_layer(self, i: int, h: torch.Tensor, start: int, mask: torch.Tensor | None = None,
-                       mask_tiles: torch.Tensor | None = None) -> None:
+                       mask_tiles: torch.Tensor | None = None, tree: _TreeRoom | None = None,
+                       parents: torch.Tensor | None = None) -> None:
         """One layer over a chunk's fp32 residual stream h [n, hidden] at positions start.. (run_text_layer,
         src/models/optimized_qwen3/dispatch/text_layer.py): RMSNorm rows -> q|k|v GEMM -> q/k norm + RoPE +
         KV cache write -> causal flash attention over the cache -> o GEMM + residual -> RMSNorm -> gate|up
         GEMM with SwiGLU in its epilogue -> down GEMM + residual.  GEMMs run on the matrix cores for any chunk length.
         ``mask`` (additive fp32 [1, n, start + n]) replaces causality in the attention; ``mask_tiles`` are its
-        tile classes (kernels.fa_mask_tiles), computed once for every layer of a pass."""
+        tile classes (kernels.fa_mask_tiles), computed once for every layer of a pass.  ``tree``: the rows are a tree's
+        nodes (tree_step) behind the tokens that the cache holds, ``start`` is not looked at."""
         c, t, p = self.config, self.types, f"layers.{i}."
         n = h.shape[0]
         x = kernels.rms_norm(h, self._n(p + "input_norm"), out=torch.empty(n, c.hidden, dtype=torch.bfloat16,
@@ -457,7 +558,10 @@ class Qwen3Decoder:
         qb = torch.empty(n, c.heads, c.head_dim, dtype=torch.bfloat16, device=self.device)
         norms = dict(q_norm_weight=self._n(p + "q_norm"), k_norm_weight=self._n(p + "k_norm"), theta=c.rope_theta,
                      eps=c.rms_eps)
-        if self.kv_bits == 8:  # at chunk_start, which holds ``start``
+        if tree is not None:
+            attn = kernels.attn_tree(q, k, v, self.k_cache[i].unsqueeze(0), self.v_cache[i].unsqueeze(0), qb, self.position,
+                                     tree.attn, parents=parents, **norms)
+        elif self.kv_bits == 8:  # at chunk_start, which holds ``start``
             kernels.qk_norm_rope_cache_q8(q, k, v, qb, self.kv[i], self.chunk_start, rope_offsets=self.rope_offset, **norms)
             attn = kernels.flash_attn_prefill_q8(qb.unsqueeze(0), self.kv[i], self.chunk_start,
                                                  weights=None if self.kv_weights is None else self.kv_weights[i])
@@ -644,6 +748,58 @@ class Qwen3Decoder:
         else:
             self.prefill(prompt_ids)
         return self._finish(max_new_tokens, steps_per_graph, use_graph)
+
+    def generate_tree(self, prompt_ids: torch.Tensor, max_new_tokens: int,
+                      draft: Callable[[list[int]], tuple[Sequence[int], Sequence[int] | None]], *, temperature: float = 0.0,
+                      generator: torch.Generator | None = None, prefill_chunk: int = 2048) -> list[int]:
+        """Decode with drafted tokens: before each step ``draft(tokens so far, prompt first)`` gives up to 63 tokens that may
+        follow and their parents: -1 hangs a token on the text, another number on the earlier drafted token of that place (None:
+        a chain).  A step decides one token and every drafted one before it on a path that the model accepts.  ``temperature`` 0 is
+        greedy; else tokens are drawn by ``generator``'s numbers, with the model's probabilities whatever was drafted."""
+        ids = prompt_ids.to(device=self.device, dtype=torch.int64).view(-1)
+        self._check_budget(ids.numel(), max_new_tokens)
+        if max_new_tokens < 1:
+            raise ValueError("max_new_tokens must be positive")
+        if not 0.0 <= temperature < float("inf"):
+            raise ValueError(f"temperature must be finite and not negative, got {temperature}")
+        if self.kv_bits != 16:
+            raise NotImplementedError("a tree's nodes attend over a bf16 KV cache")
+
+        def drawn(n: int) -> torch.Tensor | None:
+            if temperature == 0:
+                return None
+            where = self.device if generator is None else generator.device
+            return torch.rand(n, generator=generator, device=where, dtype=torch.float32).to(self.device)
+
+        self.prefill_chunked(ids, chunk=prefill_chunk)
+        if temperature != 0:  # the prompt's last row anew: a draw in place of the greedy token
+            kept, total = torch.zeros(1, dtype=torch.int32, device=self.device), self.config.vocab
+            _, _, token = kernels.tree_verify(self.logits().view(1, 1, total), self.next_token, self._tree_room(1, False).verify,
+                                              temperature=temperature, uniforms=drawn(1).view(1, 1), kept=kept)
+            self.reset(position=ids.numel() - 1)
+            self.next_token.copy_(token.view(1, 1))
+            self.done.copy_((token == self.eos).any().view(1))
+            self.run_token_store(advance=True)
+        text = ids.tolist()
+        while True:
+            new = self.generated[:int(self.length)].tolist()
+            if int(self.next_token) < 0:
+                raise RuntimeError("no token has any probability: the logits are not finite")
+            left = max_new_tokens - len(new)
+            if left <= 0 or (self.stop_on_eos and int(self.stopped)):
+                return new[:max_new_tokens]
+            tokens, parents = draft(text + new)
+            tokens, m = list(tokens), len(tokens)
+            if m >= kernels.TREE_MAX_NODES:
+                raise ValueError(f"up to {kernels.TREE_MAX_NODES - 1} drafted tokens a step, got {m}")
+            if any(not 0 <= t < self.config.vocab for t in tokens):
+                raise ValueError(f"drafted tokens must be 0 to {self.config.vocab - 1}")
+            if parents is not None:
+                if len(parents) != m or any(not -1 <= p < i for i, p in enumerate(parents)):
+                    raise ValueError("each drafted token needs a parent: -1 or an earlier one's place")
+                parents = torch.tensor([-1, *(p + 1 for p in parents)], dtype=torch.int32, device=self.device)
+            self.tree_step(torch.tensor(tokens, dtype=torch.int64, device=self.device), parents=parents,
+                           temperature=temperature, uniforms=drawn(1 + m))
 
     def generate_from_embeds(self, embeds: torch.Tensor, max_new_tokens: int, *, steps_per_graph: int = 8,
                              use_graph: bool = True, prefill_chunk: int | None = None) -> list[int]:
