@@ -59,7 +59,7 @@ struct TreeAttnArgs {
     float* part_o;     // [n_units * nk][rows][128]
     uint32_t n_units, row_tiles, rows;  // rows: of a KV head, in whole tiles
     uint32_t keys, least;               // tokens a tile; the least tiles a unit
-    float us_turn, us_tile, us_shared, us_join;  // what tree_chunk goes by
+    float us_turn, us_tile, us_shared, us_join, us_part;  // what tree_chunk goes by
     uint32_t kv_blocks, q_blocks;
 };
 
@@ -88,7 +88,7 @@ __device__ __forceinline__ uint32_t div_up(uint32_t x, uint32_t by) {  // x < 2^
 }
 
 // Tiles a unit.  Each lane weighs the longest sequence in another number of units, by what a turn of the chip costs besides tiles,
-// what a tile costs where its thread block is alone and what it costs where all are bound by memory, and a join.
+// what a tile costs where its thread block is alone and what it costs where all are bound by memory, and a join by its parts.
 // `mine`: tiles of sequence `lane`, the others' are looked up.
 __device__ uint32_t tree_chunk(const TreeAttnArgs& a, uint32_t mine) {
     const uint32_t lane = threadIdx.x & 63;
@@ -110,8 +110,10 @@ __device__ uint32_t tree_chunk(const TreeAttnArgs& a, uint32_t mine) {
         units += t > c ? div_up(t, c) : 1u;
     }
     const float blocks = (float)(a.nk * a.row_tiles) * (1.0f / TA_CUS), turns = ceilf((float)units * blocks);
-    const float alone = turns * (a.us_turn + (float)min(c, most) * a.us_tile), together = a.us_turn + (float)total * blocks * a.us_shared;
-    float cost = fmaxf(alone, together) + (c < most ? a.us_join : 0.0f);
+    // (8 thread blocks read a tile of 64 KiB in 0.7 us each, 64 in 1.5, 256 in 2.6: about the power 0.42 of the chip's share)
+    const float busy = (float)units * blocks / turns, share = a.us_shared * __builtin_amdgcn_exp2f(__builtin_amdgcn_logf(busy) * 0.42f);
+    const float alone = turns * (a.us_turn + (float)min(c, most) * fmaxf(a.us_tile, share)), together = a.us_turn + (float)total * blocks * a.us_shared;
+    float cost = fmaxf(alone, together) + (c < most ? a.us_join + a.us_part * (float)div_up(most, c) : 0.0f);
     if (units > a.n_units) cost = INFINITY;
     const uint64_t best = __ballot(cost == -wave_max(-cost));
     const uint32_t chunk = (uint32_t)__builtin_amdgcn_readlane((int)c, __builtin_ctzll(best));
@@ -1083,7 +1085,7 @@ static uint32_t ta_tile_rows(uint32_t rows) { return rows <= 16 ? 16 : rows <= 3
 
 struct TreeSizes {
     uint32_t tile_rows, row_tiles, rows, keys, least, units;
-    float us_turn, us_tile, us_shared, us_join;
+    float us_turn, us_tile, us_shared, us_join, us_part;
     size_t done, qh, ql, line, vt, broken, which, table, of_seq, part_ml, part_o, end;
 };
 
@@ -1099,7 +1101,8 @@ static TreeSizes ta_sizes(uint32_t n_seq, uint32_t n, uint32_t nh, uint32_t nk, 
     s.us_shared = 2.6f * (float)s.keys / 128.0f;
     s.us_turn = s.tile_rows <= 16 ? 8.0f : s.tile_rows == 32 ? 10.0f : 9.0f;
     s.us_tile = s.tile_rows <= 16 ? 0.7f : s.tile_rows == 32 ? 1.0f : s.tile_rows == 64 ? 1.2f : s.tile_rows == 128 ? 0.62f : 1.05f;
-    s.us_join = s.tile_rows <= 16 ? 3.5f : s.tile_rows == 32 ? 4.0f : 2.0f;
+    s.us_join = s.tile_rows <= 16 ? 1.3f : 2.0f;
+    s.us_part = s.tile_rows <= 16 ? 0.35f : s.tile_rows == 32 ? 0.4f : 0.05f;
     const uint32_t slots = TA_CUS / (nk * s.row_tiles) > 1 ? TA_CUS / (nk * s.row_tiles) : 1;
     const uint64_t most = (uint64_t)n_seq * ((s_cap + s.keys - 1) / s.keys), some = slots > n_seq + slots / 2 ? slots : n_seq + slots / 2;
     s.units = (uint32_t)(most < some ? most : some);
@@ -1213,6 +1216,7 @@ extern "C" int t2h_attn_tree(const float* q, uint64_t q_row, const float* k_new,
     a.us_tile = s.us_tile;
     a.us_shared = s.us_shared;
     a.us_join = s.us_join;
+    a.us_part = s.us_part;
     const uint64_t waves = (uint64_t)n_seq * n * ((nh + TP_HEADS - 1) / TP_HEADS), kv = (uint64_t)n_seq * nk * ((n + TP_NODES - 1) / TP_NODES);
     const uint64_t grid = (uint64_t)s.units * nk * s.row_tiles, joins = ((uint64_t)n_seq * n * nh + 3) / 4;
     if (kv + waves > 0x3fffffffu || grid > 0x7fffffffu || joins > 0x3fffffffu) return T2H_ERR_SHAPE;
