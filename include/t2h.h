@@ -666,7 +666,7 @@ int t2h_kv_cache_q8_evict(void* const* cache, uint32_t s_cap, const int32_t* len
  * softmax(q . k / sqrt(128)) . v over the `lengths` cached tokens (device int32 [n_seq]), the node's ancestors and itself.
  * Rows that are no nodes give zeros and leave their slots; nodes without a slot (length + i >= s_cap) and those of a
  * sequence whose length lies outside [0, s_cap] are none.  lengths is not advanced.  Values that are not finite reach the rows
- * that see their token only.  d = 128, nh / nk a whole number up to 16; caches, out and workspace 16-byte aligned, k_seq and
+ * that see their token only.  d = 128, nh / nk a whole number up to 16, s_cap below 2^29 - 63; caches, out and workspace 16-byte aligned, k_seq and
  * v_seq multiples of 8.
  * workspace: t2h_attn_tree_workspace_bytes() bytes, zero-filled once before its first use (calls leave it reusable, for other
  * shapes too up to n_seq * nk = 16384); calls that share one must not overlap in time. */
@@ -679,11 +679,11 @@ int t2h_attn_tree(const float* q, uint64_t q_row, const float* k_new, uint64_t k
 
 /* Which drafted tokens the target's probabilities accept, and the token that follows them.  Node 0 is a token that stands
  * already; tokens (int64 [n_seq][n]) are the nodes', logits [n_seq * n] rows of `vocab` values (fp32 or bf16: dtype), row_stride
- * elements apart, the target's after each node.  The walk begins at node 0.  With w = exp(logit / temperature - the row's
- * maximum) of the row it stands at and S their sum, it asks the node's children in their order: child c with token x is accepted
- * if uniforms[c] S < w(x), and then the walk stands at c; if not, w(x) leaves the row and S.  Where no child is accepted,
- * the next token is the first one up to which the row's sum exceeds uniforms[0] S.  So the tokens are distributed as the
- * target's own whatever was drafted.
+ * elements apart, the target's after each node.  The walk begins at node 0, whatever its parent.  With w = exp(logit /
+ * temperature - the row's maximum) of the row it stands at and S their sum, it asks the node's children in their order: child c
+ * with token x is accepted if uniforms[c] S < w(x), and then the walk stands at c; if not, w(x) leaves the row and S.  Where no
+ * child is accepted, the next token is the first one up to which the row's sum exceeds uniforms[0] S.  So the tokens are
+ * distributed as the target's own whatever was drafted.
  * draft (NULL, or rows as logits', [n_seq * (n - 1)], draft_stride apart; parents NULL): the drafts were drawn: row i is
  * what token i + 1 was drawn from, at the same temperature.  With p and q the two rows' probabilities, x is accepted if
  * uniforms[i + 1] q(x) < p(x); if not, the next token is drawn from max(p - q, 0).

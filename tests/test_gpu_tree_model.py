@@ -262,6 +262,18 @@ def test_drawn_drafts_of_the_same_model_are_all_accepted(weights, device):
     assert path.tolist() == [0, 1, 2, 3, 4] and d.generated[1:5].tolist() == tokens[1:]
 
 
+def test_the_first_nodes_parent_is_not_looked_at(weights, device):
+    runs = []
+    for first in (-1, 0, 7):
+        d = decoder(weights)
+        d.prefill_chunked(prompt(30))
+        up = torch.tensor([first, 0, 0, 1], dtype=torch.int32, device=device)
+        runs.append([t.clone() for t in d.tree_step(torch.tensor([5, 6, 7], device=device), parents=up)])
+        assert up[0] == first
+    for run in runs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(run, runs[0]))
+
+
 @pytest.mark.parametrize("room", [1, 3])
 def test_nodes_without_a_slot(weights, device, room):
     """At the end of the cache a chain is as long as what is left, and rows before it stay."""

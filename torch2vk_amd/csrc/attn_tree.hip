@@ -15,6 +15,7 @@ typedef float ta_f32x4 __attribute__((ext_vector_type(4)));
 constexpr int TA_D = 128;
 constexpr uint32_t TA_CUS = 256;
 constexpr int TA_MAX_GROUP = 16;
+constexpr uint32_t TA_MOST = (1u << 29) - 64;  // tokens of a sequence: tiles of 32 are counted in 24 bits (275 GB of one KV head)
 constexpr int TA_ROW_BYTES = TA_D * 2;
 constexpr int TP_NODES = 16, TP_GROUPS = TREE_MAX / TP_NODES;  // nodes of a thread block that writes K and V rows
 constexpr float TA_RESCALE = 8.0f;  // log2 headroom of the lazily updated running maximum
@@ -66,7 +67,7 @@ struct TreeAttnArgs {
 // ------------------------------------------------------------------------------------------ before the attention --
 //
 // One launch of three kinds of thread blocks: the units' table, the nodes' K and V rows of a (sequence, KV head), and the
-// queries.
+// queries.  5.4 us for 26 nodes, 6.7 for 4 x 64: latency, of the lengths, the rows and the angles in 64 bits one after another.
 
 constexpr int TP_HEADS = 4;  // q heads a wave
 
@@ -353,6 +354,13 @@ __global__ __launch_bounds__(256) void tree_rows_kernel(const TreeAttnArgs a) {
 //   * O^T += V^T . P^T, whose A operand the transposing LDS read hands out.
 // 16-byte pieces of a row lie in LDS at their place XOR f(row), so that neither product's reads meet in a bank: f is the
 // row's low four bits for keys (16 rows, one piece each) and twice two of them for values (4 rows, 4 pieces each).
+// q's second term costs half as many products again; with one term outputs would be off by half of bf16's step in q besides
+// that of the weights.  Weights are rounded to bf16 once, their sum is of the unrounded ones.
+// By rows of a KV head (32 / 8 heads, us with all launches): up to 64, 4 waves of keys and 64 KiB tiles twice, 12 nodes at 4000
+// 21.0 (as 128 rows 21.5, as 256 22.5); up to 128, 4 times 32 KiB, 8 x 26 nodes at 8000 79 (as 256: 83); more, 8 times 16 KiB,
+// 4 x 64 at 15000 114, of which the attention is 96: 990 TFLOP/s of the three products.  There the matrix cores are 48 % and
+// the vector units 42 % busy.  The next tile's scores between one's exponentials gave the same 97, 64 rows a wave, to halve what
+// is read from LDS, 133: the queries no longer fit the registers that a product reads.
 
 // A sum with the values that were zeros in the products.
 __device__ __forceinline__ float tree_put_broken(float x, uint64_t nan, uint64_t inf, uint64_t minus) {
@@ -602,7 +610,7 @@ void tree_attn_kernel(const TreeAttnArgs a) {
 }
 
 // Joins the units of a sequence, a wave a row: a lane holds a unit's maximum and sum, and four dims of every other unit's row.
-// All of up to 32 units are on their way at once.
+// All of up to 32 units are on their way at once.  4.8 us for 26 nodes of 32 heads and 9.2 for 4 x 64 (33 MB, 3.6 TB/s).
 constexpr int TJ_BATCH = 16;
 
 template <int N>
@@ -666,6 +674,9 @@ __global__ __launch_bounds__(256) void tree_join_kernel(const TreeAttnArgs a) {
 // keys of a dim.
 // The last unit of a (sequence, KV head) to leave its part joins them: parts go past the caches that the chip's parts do not
 // share (agent scope), and are there before the count is raised.
+// 32 x 4 nodes at 16000: 360 us, 5.7 TB/s (three launches: 486); 8 at 500: 10 us (three launches: 14.8), which is one step after
+// another: lengths, the table's sums, queries' norm and angles, a tile, two joins.  16 rows as 32: 22.4 for 19.4 us at 1 x 8 of
+// 16 / 8 heads at 8000.
 
 constexpr int TF_WAVES = 8, TF_KEYS = 16 * TF_WAVES;
 constexpr int TF_QROW = TA_D + 8;  // bf16 row of queries in LDS, padded
@@ -1139,7 +1150,7 @@ static TreeSizes ta_sizes(uint32_t n_seq, uint32_t n, uint32_t nh, uint32_t nk, 
 using namespace t2h;
 
 static bool ta_shape(uint32_t n_seq, uint32_t n, uint32_t nh, uint32_t nk, uint32_t s_cap) {
-    return n_seq != 0 && n <= (uint32_t)TREE_MAX && nk != 0 && nh != 0 && nh % nk == 0 && s_cap != 0 && s_cap <= 0x7fffff00u;
+    return n_seq != 0 && n <= (uint32_t)TREE_MAX && nk != 0 && nh != 0 && nh % nk == 0 && s_cap != 0 && s_cap <= TA_MOST;
 }
 
 extern "C" size_t t2h_attn_tree_workspace_bytes(uint32_t n_seq, uint32_t n, uint32_t nh, uint32_t nk, uint32_t d,

@@ -443,7 +443,7 @@ class Qwen3Decoder:
         (kernels.attn_tree), the LM head's logits after each, the accepted path and the token that follows it
         (kernels.tree_verify: greedy, or by ``temperature`` and ``uniforms`` fp32 [1 + m]), the path's rows kept in the cache
         (kernels.tree_keep); its tokens and the one that follows are stored, position goes on by the path's nodes.
-        ``parents`` int32 [1 + m] as kernels.attn_tree has them, the first of them -1 for next_token (None: a chain);
+        ``parents`` int32 [1 + m] as kernels.attn_tree has them (the first, next_token's, is not looked at; None: a chain);
         ``draft_logits`` fp32 [m, vocab]: a chain drawn from them.  Everything stays on the device: a step can be captured, once
         one of as many nodes has run.  Nodes that the cache has no slot for are none.  Returns path int32 [1 + m], kept int32
         [1] and the logits fp32 [1 + m, vocab]."""
@@ -467,7 +467,7 @@ class Qwen3Decoder:
         room = self._tree_room(n, draft_logits is not None)
         tokens = torch.cat([self.next_token.view(-1), drafts])
         h = self.embed_tokens(tokens)
-        up = None if parents is None else parents.view(1, n)
+        up = None if parents is None else torch.cat([parents.new_full((1,), -1), parents[1:]]).view(1, n)
         for i in range(c.layers):
             self._prefill_layer(i, h, 0, tree=room, parents=up)
         x = kernels.rms_norm(h, self._n("norm"), out=torch.empty(n, c.hidden, dtype=torch.bfloat16, device=self.device),
