@@ -34,8 +34,8 @@ def test_attention_refuses(lib):
     assert attn(lib, q_norm_w=P) == NULL
     assert attn(lib, d=64) == UNSUPPORTED
     assert attn(lib, nh=17 * 8, q_row=17 * 1024) == UNSUPPORTED
-    for kw in (dict(nh=15), dict(nh=0), dict(nk=0), dict(n_seq=0), dict(n=65), dict(s_cap=0), dict(s_cap=0x80000000), dict(s_cap=2 ** 29, k_seq=2 ** 42, v_seq=2 ** 42),
-               dict(q_row=2047), dict(k_row=1023), dict(v_row=1000), dict(k_seq=64 * 1024 - 8), dict(v_seq=8)):
+    for kw in (dict(nh=15), dict(nh=0), dict(nk=0), dict(n_seq=0), dict(n=65), dict(s_cap=0), dict(s_cap=0x80000000),
+               dict(s_cap=2 ** 29, k_seq=2 ** 42, v_seq=2 ** 42), dict(q_row=2047), dict(k_row=1023), dict(v_row=1000), dict(k_seq=64 * 1024 - 8), dict(v_seq=8)):
         assert attn(lib, **kw) == SHAPE, kw
     for kw in (dict(k_cache=ODD), dict(v_cache=ODD), dict(out=ODD), dict(workspace=ODD), dict(k_seq=64 * 1024 + 4)):
         assert attn(lib, **kw) == ALIGN, kw
