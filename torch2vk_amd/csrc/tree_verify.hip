@@ -567,7 +567,7 @@ struct KeepArgs {
 
 // A thread block a (layer, sequence): 256 pieces of 16 bytes of the K and V rows at a time, KEEP_GROUPS groups of threads share
 // the moves.  Rows move down only (path[j] > j): those of KEEP_GROUPS * KEEP_EACH moves are read before one of them is written,
-// and a later move reads no row that an earlier one has written.  36 layers of 16 sequences, 8 to 20 rows each: 27 us, 2.3 TB/s
+// and a later move reads no row that an earlier one has written.  36 layers of 16 sequences, 8 to 20 rows each: 26 us, 2.4 TB/s
 // (one row after another: 33; 4 times as many smaller thread blocks would do for few rows: 26 nodes 6.8 us for 3.9).
 constexpr int KEEP_GROUPS = 4, KEEP_EACH = 4, KEEP_THREADS = 256 * KEEP_GROUPS;
 
@@ -592,10 +592,12 @@ __global__ __launch_bounds__(KEEP_THREADS) void tree_keep_kernel(const KeepArgs 
     if (moves == 0) return;
     const uint32_t row = a.nk * 16;  // pieces of a K or V row
     const int group = threadIdx.x >> 8;
+    uint4* const k = reinterpret_cast<uint4*>(a.cache[0] + layer * a.layer[0] + seq * a.seq[0]) + (size_t)len * row;
+    uint4* const v = reinterpret_cast<uint4*>(a.cache[1] + layer * a.layer[1] + seq * a.seq[1]) + (size_t)len * row;
     for (uint32_t c0 = 0; c0 < 2 * row; c0 += 256) {
         const uint32_t c = c0 + (threadIdx.x & 255), which = c < row ? 0 : 1, col = c - which * row;
         const bool in = c < 2 * row;
-        uint4* const base = reinterpret_cast<uint4*>(a.cache[which] + layer * a.layer[which] + seq * a.seq[which]) + (size_t)len * row + (in ? col : 0);
+        uint4* const base = (which ? v : k) + (in ? col : 0);
         for (int m0 = 0; m0 < moves; m0 += KEEP_GROUPS * KEEP_EACH) {
             const int mine = m0 + group * KEEP_EACH;
             uint4 x[KEEP_EACH];
