@@ -313,3 +313,15 @@ def test_refusals(weights, device):
                                 (5, 4, lambda t: ([], None), dict(temperature=float("inf")))]:
         with pytest.raises(ValueError):
             d.generate_tree(prompt(n), new, draft, **more)
+
+
+def test_steps_of_all_sizes_share_one_workspace(weights, device):
+    """Chains of 1 to 64 nodes, largest, smallest and back, as a fresh decoder's each."""
+    d = decoder(weights)
+    for n in (64, 1, 9, 33, 2, 17, 64, 5):
+        one = decoder(weights)
+        runs = []
+        for x in (d, one):
+            x.prefill_chunked(prompt(100))
+            runs.append(x.tree_step(prompt(n - 1, n).to(device)) if n > 1 else x.tree_step(torch.empty(0, dtype=torch.int64, device=device)))
+        assert all(torch.equal(a, b) for a, b in zip(*runs))

@@ -2011,9 +2011,10 @@ def _tree_refuse_cache(dims: int, **caches: torch.Tensor) -> None:
 
 
 def attn_tree_workspace(n_seq: int, n: int, nh: int, nk: int, d: int, s_cap: int, device) -> torch.Tensor:
-    """Zeroed workspace of :func:`attn_tree` for such calls; calls leave it reusable, and calls that share one must not overlap
-    in time."""
-    nbytes = int(_lib.lib().t2h_attn_tree_workspace_bytes(n_seq, n, nh, nk, d, s_cap))
+    """Zeroed workspace of :func:`attn_tree` for calls of up to n nodes a sequence; calls leave it reusable, and calls that share
+    one must not overlap in time."""
+    size = _lib.lib().t2h_attn_tree_workspace_bytes
+    nbytes = int(size(n_seq, n, nh, nk, d, s_cap)) and max(int(size(n_seq, i, nh, nk, d, s_cap)) for i in range(1, n + 1))
     if nbytes == 0:
         raise ValueError(f"unsupported tree attention shape n_seq={n_seq} n={n} nh={nh} nk={nk} d={d} s_cap={s_cap}")
     return torch.zeros(nbytes, dtype=torch.uint8, device=device)
@@ -2091,9 +2092,11 @@ def attn_tree(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_cache
 
 
 def tree_verify_workspace(n_seq: int, n: int, vocab: int, device, *, drawn: bool = False) -> torch.Tensor:
-    """Zeroed workspace of :func:`tree_verify` for such calls (``drawn``: with draft logits); calls leave it reusable, and calls
-    that share one must not overlap in time."""
-    nbytes = int(_lib.lib().t2h_tree_verify_workspace_bytes(n_seq, n, vocab, int(drawn)))
+    """Zeroed workspace of :func:`tree_verify` for calls of up to n nodes a sequence (``drawn``: also with draft logits); calls
+    leave it reusable, and calls that share one must not overlap in time."""
+    size = _lib.lib().t2h_tree_verify_workspace_bytes
+    nbytes = int(size(n_seq, n, vocab, int(drawn))) and max(int(size(n_seq, i, vocab, k)) for i in range(1, n + 1)
+                                                            for k in range(1 + int(drawn)))
     if nbytes == 0:
         raise ValueError(f"unsupported verification shape n_seq={n_seq} n={n} vocab={vocab}")
     return torch.zeros(nbytes, dtype=torch.uint8, device=device)

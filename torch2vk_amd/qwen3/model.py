@@ -58,7 +58,7 @@ def _check_types(c: Qwen3Config, types: dict[str, str]) -> None:
 
 @dataclass(frozen=True)
 class _TreeRoom:
-    """Workspaces of a tree_step of one number of nodes."""
+    """Workspaces of a decoder's tree steps, of any number of nodes."""
 
     attn: torch.Tensor
     verify: torch.Tensor
@@ -147,7 +147,7 @@ class Qwen3Decoder:
         self.stop_on_eos = True
         self._graphs: dict[int, torch.cuda.CUDAGraph] = {}
         self._prefill_graphs: dict[tuple[int, int, int, bool], tuple[torch.cuda.CUDAGraph, torch.Tensor]] = {}
-        self._tree_rooms: dict[tuple[int, bool], _TreeRoom] = {}
+        self._tree_ws: _TreeRoom | None = None
         self.persistent = False
         self.status = torch.zeros(1, dtype=torch.int32, device=dev)
         if persistent is not False:
@@ -425,16 +425,16 @@ class Qwen3Decoder:
 
     # ------------------------------------------- trees of drafted tokens --
 
-    def _tree_room(self, n: int, drawn: bool) -> _TreeRoom:
-        """Allocated by the first step of n nodes, which is not a captured one: a graph's own memory is its replays' alone."""
-        if (n, drawn) not in self._tree_rooms:
+    def _tree_room(self) -> _TreeRoom:
+        """Allocated by the first step, which is not a captured one: a graph's own memory is its replays' alone."""
+        if self._tree_ws is None:
             if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError(f"run a tree_step of {n} nodes before capturing one")
-            c = self.config
-            self._tree_rooms[n, drawn] = _TreeRoom(
+                raise RuntimeError("run a tree_step before capturing one")
+            c, n = self.config, kernels.TREE_MAX_NODES
+            self._tree_ws = _TreeRoom(
                 kernels.attn_tree_workspace(1, n, c.heads, c.kv_heads, c.head_dim, self.max_positions, self.device),
-                kernels.tree_verify_workspace(1, n, c.vocab, self.device, drawn=drawn))
-        return self._tree_rooms[n, drawn]
+                kernels.tree_verify_workspace(1, n, c.vocab, self.device, drawn=True))
+        return self._tree_ws
 
     def tree_step(self, drafts: torch.Tensor, *, parents: torch.Tensor | None = None, temperature: float | torch.Tensor = 0.0,
                   uniforms: torch.Tensor | None = None, draft_logits: torch.Tensor | None = None
@@ -445,7 +445,7 @@ class Qwen3Decoder:
         (kernels.tree_keep); its tokens and the one that follows are stored, position goes on by the path's nodes.
         ``parents`` int32 [1 + m] as kernels.attn_tree has them (the first, next_token's, is not looked at; None: a chain);
         ``draft_logits`` fp32 [m, vocab]: a chain drawn from them.  Everything stays on the device: a step can be captured, once
-        one of as many nodes has run.  Nodes that the cache has no slot for are none.  Returns path int32 [1 + m], kept int32
+        one has run.  Nodes that the cache has no slot for are none.  Returns path int32 [1 + m], kept int32
         [1] and the logits fp32 [1 + m, vocab]."""
         c = self.config
         if self.kv_bits != 16:
@@ -464,7 +464,7 @@ class Qwen3Decoder:
             raise ValueError("drawn drafts are a chain: pass draft_logits or parents")
         if uniforms is None and (isinstance(temperature, torch.Tensor) or temperature != 0):
             raise ValueError("sampling needs uniforms")
-        room = self._tree_room(n, draft_logits is not None)
+        room = self._tree_room()
         tokens = torch.cat([self.next_token.view(-1), drafts])
         h = self.embed_tokens(tokens)
         up = None if parents is None else torch.cat([parents.new_full((1,), -1), parents[1:]]).view(1, n)
@@ -774,7 +774,7 @@ class Qwen3Decoder:
         self.prefill_chunked(ids, chunk=prefill_chunk)
         if temperature != 0:  # the prompt's last row anew: a draw in place of the greedy token
             kept, total = torch.zeros(1, dtype=torch.int32, device=self.device), self.config.vocab
-            _, _, token = kernels.tree_verify(self.logits().view(1, 1, total), self.next_token, self._tree_room(1, False).verify,
+            _, _, token = kernels.tree_verify(self.logits().view(1, 1, total), self.next_token, self._tree_room().verify,
                                               temperature=temperature, uniforms=drawn(1).view(1, 1), kept=kept)
             self.reset(position=ids.numel() - 1)
             self.next_token.copy_(token.view(1, 1))
