@@ -690,7 +690,8 @@ int t2h_attn_tree(const float* q, uint64_t q_row, const float* k_new, uint64_t k
  * temperatures (device fp32 [n_seq], or NULL for `temperature`): one that is not positive is greedy: the child whose token is
  * the row's largest logit (the lowest index of equals), and that token follows.  uniforms (fp32 [n_seq][n]) may be NULL where
  * `temperature` is not positive and temperatures is NULL; numbers outside [0, 1) count as the nearest in it, NaN as 0.
- * A logit of -infinity or NaN has no probability; infinite ones share it.  Sums are kept in 64 bits.
+ * A logit of -infinity or NaN has no probability; infinite ones share it.  Tokens are accepted and drawn as sums and exponentials
+ * in 64 bits have it.
  * path int32 [n_seq][n]: the nodes that the walk stood at, node 0 first, then -1; kept [n_seq]: how many (0 where a sequence has
  * no nodes); next_token int64 [n_seq]: -1 where there are no nodes or no token has any probability.
  * workspace: t2h_tree_verify_workspace_bytes() bytes, 16-byte aligned, zero-filled once before its first use (calls leave it

@@ -630,6 +630,88 @@ def test_draft_and_target_alike(device):
     assert kept.tolist() == [5] * 4
 
 
+def beside(border):
+    """The fp32 numbers next to a border in (0, 1), one step of the nearest to each side: at least 2^-26 of it off, where sums
+    and exponentials in 64 bits are off by 10^-11."""
+    near = torch.tensor(border, dtype=F32)
+    most = torch.tensor(1 - 2.0 ** -24)
+    return float(torch.nextafter(near, torch.tensor(0.0))), float(torch.minimum(torch.nextafter(near, torch.tensor(2.0)), most))
+
+
+def share(row, t):
+    return torch.softmax(row.double().cpu() / t, -1)
+
+
+@pytest.mark.parametrize("vocab", [8, 1000, 5003, 151936])
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_numbers_next_to_the_borders_of_acceptance(device, vocab, dtype):
+    """Four children of one node, each accepted or rejected by a step of its number, all 16 ways."""
+    b, n = 16, 5
+    x = verify_inputs(device, b, n, vocab, seed=60 + vocab, dtype=dtype)
+    temps = torch.tensor([1.0, 0.5, 1.5, 0.75] * 4, device=device)
+    x["parents"][:] = torch.tensor([-1, 0, 0, 0, 0], device=device)
+    for i in range(b):
+        x["tokens"][i, 1:] = x["logits"][i, 0].float().topk(8).indices[i % 4:i % 4 + 4]
+        mass = share(x["logits"][i, 0], float(temps[i]))
+        for j in range(1, n):
+            t = int(x["tokens"][i, j])
+            under, over = beside(float(mass[t] / mass.sum()))
+            x["uniforms"][i, j] = over if i >> (j - 1) & 1 else under
+            mass[t] = 0.0
+    path, kept, _ = verified(x, temps)
+    assert kept.tolist() == [2] * 15 + [1] and [int(p) for p in path[:4, 1]] == [1, 2, 1, 3]
+
+
+@pytest.mark.parametrize("vocab", [8, 1000, 5003, 151936])
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_numbers_next_to_the_borders_of_drawn_drafts(device, vocab, dtype):
+    """Chains whose token i is rejected by one step of its number, those before it accepted by one."""
+    b, n = 6, 6
+    x = verify_inputs(device, b, n, vocab, seed=80 + vocab, dtype=dtype, drawn=True)
+    temps = torch.tensor([1.0, 0.5, 1.5, 0.75, 1.0, 2.0], device=device)
+    for i in range(b):
+        for j in range(1, n):
+            p, q = share(x["logits"][i, j - 1], float(temps[i])), share(x["draft"][i, j - 1], float(temps[i]))
+            t = int((q - p).argmax())
+            x["tokens"][i, j] = t
+            under, over = beside(float(p[t] / q[t]))
+            x["uniforms"][i, j] = over if j == i + 1 else under
+    _, kept, _ = verified(x, temps)
+    assert kept.tolist() == [1, 2, 3, 4, 5, 6]
+
+
+@pytest.mark.parametrize("vocab,first,second", [(2, 0, 1), (5000, 7, 4500), (151936, 3, 150_000)])
+def test_a_rejected_token_of_nearly_all_probability(device, vocab, first, second):
+    """What is left beside it, 10^-5, is a sum of its own: the second child's 0.9995 lies below its whole probability."""
+    x = verify_inputs(device, 2, 3, vocab, seed=90)
+    x["logits"][:, 0] = -math.inf
+    x["logits"][:, 0, first] = 0.0
+    x["logits"][:, 0, second] = math.log(1e-5)
+    x["parents"][:] = torch.tensor([-1, 0, 0], device=device)
+    x["tokens"][:] = torch.tensor([0, first, second], device=device)
+    x["uniforms"][:] = torch.tensor([0.5, 0.999995, 0.9995], device=device)
+    path, _, following = verified(x, 1.0)
+    assert path.tolist() == [[0, 2, -1]] * 2 and (following >= 0).all()
+
+
+@pytest.mark.parametrize("spread", [0.01, 2.0, 20.0])
+@pytest.mark.parametrize("vocab", [3001, 151936])
+def test_children_that_hold_all_of_a_rows_probability(device, vocab, spread):
+    """At the largest number each but the last with any probability may be rejected, and that one is not."""
+    b, m = 64, 7
+    x = verify_inputs(device, b, m + 1, vocab, seed=91)
+    gen = torch.Generator().manual_seed(92)
+    x["parents"][:] = torch.tensor([-1] + [0] * m, device=device)
+    x["logits"][:, 0] = -math.inf
+    for i in range(b):
+        at = torch.randperm(vocab, generator=gen)[:m].to(device)
+        x["logits"][i, 0, at] = torch.randn(m, generator=gen).to(device) * spread
+        x["tokens"][i, 1:] = at
+    x["uniforms"][:, 1:] = 1 - 2.0 ** -24
+    _, kept, following = verified(x, 1.0)
+    assert (kept == 2).all() and (following >= 0).all()
+
+
 def test_logits_of_a_wider_product(device):
     for dtype in (F32, BF):
         x = verify_inputs(device, 3, 4, 1001, seed=8, dtype=dtype, drawn=True)

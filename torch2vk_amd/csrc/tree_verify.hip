@@ -14,8 +14,11 @@ namespace t2h {
 // and walks down the tree; then its waves sum their segments of the row where the walk ended, and the last thread block of a
 // sequence to get there draws the next token: the segment in which the running sum passes the border, then its logits.
 // The borders between the tokens of a large vocabulary lie 10^-5 of the sum apart: that row's sums and exponentials are in 64
-// bits (relative errors of 10^-12), since 32 would now and then draw a token's neighbour.  A child's acceptance compares one
-// probability with one number, where 32-bit exponentials and 64-bit sums (10^-7) decide as well.
+// bits (relative errors of 10^-12), since 32 would now and then draw a token's neighbour.
+// The first launch's exponentials and a piece's sum are in 32 bits, which decides a child's acceptance wherever its number lies
+// further from the border than they are off (V_OFF).  Nearer than that, or where rejected children leave so little of the row
+// that the difference of two such sums says nothing, all waves sum what is left of the row in 64 bits, and that decides: one
+// decision in 10^4 at random numbers.
 // Where drafts are drawn the next token's mass is max(p - q, 0) = max(w / Z - v / Y, 0), and Z and Y are known to 10^-7 only when
 // the second pass begins.  That is enough to tell which tokens have any (the others' share is 10^-7 of theirs); the sums of
 // their w and v, and of all w and v, are kept apart, and the last thread block has Z and Y in 64 bits.
@@ -187,6 +190,14 @@ __global__ __launch_bounds__(256) void verify_rows_kernel(const VerifyArgs a) {
     if (lane == 0) a.part[(size_t)r * a.pieces + piece] = make_uint2(__float_as_uint(top), second);
 }
 
+// Relative errors of the 32-bit exponentials and sums, in units of 2^-24: an exponent of -a (to the base 2) is off by 4 of its own
+// roundings, 2.8 a in the exponential, which has 2 more.  In a sum over up to 2^31 tokens the mean of a by weight is at most 31
+// (what the row lacks of the largest entropy); up to 63 additions a lane, 6 across, a product for each of two steps: 170.  One
+// weight: a up to 100, 282.  Those below 2^-100 of the largest are taken as unknown.
+constexpr double V_OFF = 0x1p-15, V_SMALL = 0x1p-100;
+// and of those in 64 bits: 1.2 10^-12 of the series, and additions
+constexpr double V_OFF64 = 0x1p-36;
+
 constexpr int VF_WAVES = 16, VF_THREADS = VF_WAVES * 64;
 constexpr int VF_EACH = 8;                        // logits a lane
 constexpr uint32_t VF_SEGMENT = 64 * VF_EACH;     // a wave
@@ -197,6 +208,8 @@ struct VerifyState {
     int64_t best[TREE_MAX];
     int gone[TREE_MAX];        // tokens that the walk rejected where it ended
     int n_gone, cur, kept;
+    bool asks;                 // whether the walk waits for the row's sums in 64 bits
+    double w[VF_WAVES], v[VF_WAVES];  // those, wave by wave
     double u;                  // the number that draws the next token
 };
 
@@ -286,67 +299,111 @@ __device__ __forceinline__ double verify_share(float x, float top, double sum, f
     return (double)(top == INFINITY ? (x == INFINITY ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(fmaxf((x - top) * c, -200.0f)));
 }
 
-// One wave walks down a sequence's tree.
+// A logit's exp((x - top) / T) in 64 bits, bit for bit as a pass over its row has it.
+__device__ __forceinline__ double verify_weight(float x, float top, double steps, const double* table) {
+    if (top == INFINITY) return x == INFINITY ? 1.0 : 0.0;
+    double y[1] = {((double)x - (double)top) * steps};
+    exp_steps(y, table);
+    return y[0];
+}
+
+// How far a walk has come.
+struct VerifyPath {
+    int cur, kept, mine;      // mine: lane j holds the path's entry j
+    uint64_t gone, children;  // of cur: rejected ones, and those to be asked
+    double rest, off;         // what the rejected ones leave of cur's sum, and how far off that may be
+    double w, q;              // the lane's node: its weight, drawn: the weights of both rows, each times the other's sum
+    bool mass;                // whether its token has any probability
+};
+
+__device__ __forceinline__ void verify_stand(VerifyPath& p, int at, int count, float t, const VerifyNode& v, const VerifyState& st) {
+    p.cur = at;
+    p.gone = 0;
+    p.children = __ballot((int)(threadIdx.x & 63) > at && (int)(threadIdx.x & 63) < count && v.up == at);
+    p.rest = t > 0.0f ? st.sum[at] : 0.0;
+    p.off = V_OFF * p.rest;
+}
+
 template <bool DRAWN>
-__device__ __forceinline__ void verify_walk(const VerifyArgs& a, uint32_t seq, int count, float t, const VerifyNode& v,
-                                            VerifyState& st, bool writes) {
+__device__ __forceinline__ void verify_start(VerifyPath& p, int count, float t, const VerifyNode& v, const VerifyState& st) {
     const int lane = threadIdx.x & 63;
-    double w = 0.0, q = 0.0;  // drawn: both times the sums, u q Y^-1 < p Z^-1 as u q Z < p Y
+    p.w = p.q = 0.0;
+    p.mass = false;
     if (t > 0.0f && v.up >= 0 && v.up < lane && lane < count) {
-        const float c = verify_factor(t);
-        w = verify_share(v.x, st.top[v.up], st.sum[v.up], c);
-        if (DRAWN) {
+        const float c = verify_factor(t), top = st.top[v.up];
+        p.mass = top == INFINITY ? v.x == INFINITY : v.x > -INFINITY;
+        p.w = verify_share(v.x, top, st.sum[v.up], c);
+        if (DRAWN) {  // u q Y^-1 < p Z^-1 as u q Z < p Y
             const double z = st.sum[v.up], y = st.sum[TREE_MAX + v.up];
-            q = verify_share(v.y, st.top[TREE_MAX + v.up], y, c) * (z > 0.0 ? z : 1.0);
-            w *= y > 0.0 ? y : 1.0;
+            p.q = verify_share(v.y, st.top[TREE_MAX + v.up], y, c) * (z > 0.0 ? z : 1.0);
+            p.w *= y > 0.0 ? y : 1.0;
         }
     }
-    int cur = 0, kept = count > 0 ? 1 : 0, mine = lane == 0 && kept ? 0 : -1;  // lane j: the path's entry j
-    uint64_t gone = 0;
-    double rest = kept && t > 0.0f ? st.sum[0] : 0.0;
-    for (bool more = kept != 0; more;) {
-        more = false;
-        uint64_t children = __ballot(lane > cur && lane < count && v.up == cur);
-        while (children) {
-            const int c = __builtin_ctzll(children);
-            children &= children - 1;
-            const int64_t x = readlane_i64(v.token, c);
-            const double u = (double)__int_as_float(__builtin_amdgcn_readlane(__float_as_int(v.u), c));
-            bool yes;
-            double wc = 0.0;
-            if (t == 0.0f) {
-                yes = st.best[cur] >= 0 && x == st.best[cur];
+    p.kept = count > 0 ? 1 : 0;
+    p.mine = lane == 0 && p.kept ? 0 : -1;
+    p.cur = 0;
+    p.gone = p.children = 0;
+    if (p.kept) verify_stand(p, 0, count, t, v, st);
+}
+
+// One wave walks down a sequence's tree: to its end, or (true) to a child whose acceptance the 32-bit sums do not decide.  It is
+// called again then, with what is left of the row in 64 bits, and of the draft's row.
+template <bool DRAWN>
+__device__ __forceinline__ bool verify_walk(VerifyPath& p, int count, float t, const VerifyNode& v, const VerifyState& st,
+                                            const double* table, bool answered) {
+    const int lane = threadIdx.x & 63;
+    while (p.children) {
+        const int c = __builtin_ctzll(p.children), cur = p.cur;
+        const int64_t x = readlane_i64(v.token, c);
+        const double u = (double)__int_as_float(__builtin_amdgcn_readlane(__float_as_int(v.u), c));
+        bool yes = false;
+        double wc = 0.0, off = V_OFF;
+        if (t == 0.0f) {
+            yes = st.best[cur] >= 0 && x == st.best[cur];
+        } else if ((__ballot(p.mass) >> c & 1) && !(!DRAWN && __ballot((p.gone >> lane & 1) && v.token == x))) {
+            double border;
+            wc = readlane_f64(p.w, c);
+            if (answered) {
+                const double steps = verify_steps(t);
+                double z = 0.0, y = 0.0;
+                for (int i = 0; i < VF_WAVES; ++i) {
+                    z += st.w[i];
+                    if (DRAWN) y += st.v[i];
+                }
+                wc = verify_weight(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(v.x), c)), st.top[cur], steps, table);
+                if (DRAWN) {
+                    const float to = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v.y), c));
+                    border = u * (verify_weight(to, st.top[TREE_MAX + cur], steps, table) * (z > 0.0 ? z : 1.0));
+                    wc *= y > 0.0 ? y : 1.0;
+                } else {
+                    border = u * z;
+                    p.rest = z;
+                    p.off = V_OFF64 * z;
+                    off = V_OFF64;
+                }
             } else if (DRAWN) {
-                yes = u * readlane_f64(q, c) < readlane_f64(w, c);
+                border = u * readlane_f64(p.q, c);
+                const double z = st.sum[cur], y = st.sum[TREE_MAX + cur];
+                if (fabs(border - wc) <= 2.0 * V_OFF * (border + wc) + V_SMALL * (z * (y > 0.0 ? y : 1.0))) return true;
             } else {
-                const bool again = __ballot((gone >> lane & 1) && v.token == x) != 0;
-                wc = again ? 0.0 : readlane_f64(w, c);
-                yes = u * rest < wc;
+                border = u * p.rest;
+                if (fabs(border - wc) <= u * p.off + V_OFF * wc + V_SMALL * st.sum[cur]) return true;
             }
-            if (yes) {
-                if (lane == kept) mine = c;
-                ++kept;
-                cur = c;
-                gone = 0;
-                rest = t > 0.0f ? st.sum[cur] : 0.0;
-                more = true;
-                break;
-            }
-            rest -= wc;
-            gone |= 1ull << c;
+            yes = border < wc;
+        }
+        answered = false;
+        p.children &= p.children - 1;
+        if (yes) {
+            if (lane == p.kept) p.mine = c;
+            ++p.kept;
+            verify_stand(p, c, count, t, v, st);
+        } else {
+            p.gone |= 1ull << c;
+            p.rest -= wc;
+            p.off += off * wc;
         }
     }
-    if (writes) {
-        if (lane < (int)a.n) a.path[(size_t)seq * a.n + lane] = mine;
-        if (lane == 0) a.kept[seq] = kept;
-    }
-    if (gone >> lane & 1) st.gone[__popcll(gone & ((1ull << lane) - 1))] = v.token >= 0 && v.token < (int64_t)a.vocab ? (int)v.token : -1;
-    if (lane == 0) {
-        st.cur = cur;
-        st.kept = kept;
-        st.n_gone = DRAWN ? 0 : __popcll(gone);
-        st.u = (double)v.u;
-    }
+    return false;
 }
 
 __device__ __forceinline__ void put_f64(double* p, double x) {
@@ -370,23 +427,23 @@ __global__ __launch_bounds__(VF_THREADS) void verify_finish_kernel(const VerifyA
     if (tid >= VF_THREADS - V_TABLE) table[tid - (VF_THREADS - V_TABLE)] = V_POWERS[tid - (VF_THREADS - V_TABLE)];
     verify_join(a, seq, count, DRAWN && count > 0 ? 2 * count - 1 : count, t, st);
     __syncthreads();
-    if (wave == 0) verify_walk<DRAWN>(a, seq, count, t, node, st, chunk == 0);
-    __syncthreads();
-    const int cur = st.cur;
-    if (st.kept == 0 || t == 0.0f) {
-        if (tid == 0) a.next_token[seq] = st.kept == 0 ? -1 : st.best[cur];
-        return;
-    }
-    // the row where the walk ended, and the draft's there if its token was drawn and rejected
-    const double steps = verify_steps(t);
-    const float top = st.top[cur];
-    const size_t logits = ((size_t)seq * a.n + cur) * a.row_stride;
-    const int gone = lane < st.n_gone ? st.gone[lane] : -1;
-    const bool residual = DRAWN && cur < count - 1;
-    const void* const draft = residual  // (or a row that is not looked at)
-                                  ? static_cast<const uint8_t*>(a.draft) + ((size_t)seq * (a.n - 1) + cur) * a.draft_stride * (BF16 ? 2 : 4)
-                                  : static_cast<const uint8_t*>(a.logits) + logits * (BF16 ? 2 : 4);
-    const float qtop = residual ? st.top[TREE_MAX + cur] : 0.0f;
+    const double steps = t > 0.0f ? verify_steps(t) : 0.0;
+    const uint32_t segments = (a.vocab + VF_SEGMENT - 1) / VF_SEGMENT;
+    // the row where the walk stands, and the draft's there
+    float top = 0.0f, qtop = 0.0f;
+    size_t logits = 0;
+    const void* draft = nullptr;
+    int gone = -1;
+    bool residual = false;
+    auto stand = [&](int cur) {
+        top = st.top[cur];
+        logits = ((size_t)seq * a.n + cur) * a.row_stride;
+        gone = lane < st.n_gone ? st.gone[lane] : -1;
+        residual = DRAWN && cur < count - 1;
+        draft = residual ? static_cast<const uint8_t*>(a.draft) + ((size_t)seq * (a.n - 1) + cur) * a.draft_stride * (BF16 ? 2 : 4)
+                         : static_cast<const uint8_t*>(a.logits) + logits * (BF16 ? 2 : 4);  // (a row that is not looked at)
+        qtop = residual ? st.top[TREE_MAX + cur] : 0.0f;
+    };
     auto weigh = [&](const float (&x)[VF_EACH], float top, double (&w)[VF_EACH]) {
         if (top == INFINITY) {  // infinite logits share the probability
 #pragma unroll
@@ -422,9 +479,53 @@ __global__ __launch_bounds__(VF_THREADS) void verify_finish_kernel(const VerifyA
             }
         }
     };
+    VerifyPath path;
+    if (wave == 0) verify_start<DRAWN>(path, count, t, node, st);
+    for (bool answered = false;; answered = true) {
+        if (wave == 0) {
+            const bool asks = verify_walk<DRAWN>(path, count, t, node, st, table, answered);
+            if (!DRAWN && (path.gone >> lane & 1))
+                st.gone[__popcll(path.gone & ((1ull << lane) - 1))] = node.token >= 0 && node.token < (int64_t)a.vocab ? (int)node.token : -1;
+            if (lane == 0) {
+                st.asks = asks;
+                st.cur = path.cur;
+                st.kept = path.kept;
+                st.u = (double)node.u;
+                st.n_gone = DRAWN ? 0 : __popcll(path.gone);
+            }
+        }
+        __syncthreads();
+        if (!st.asks) break;
+        stand(st.cur);
+        double z = 0.0, y = 0.0, w[VF_EACH], v[VF_EACH];
+        for (uint32_t s = wave; s < segments; s += VF_WAVES) {
+            segment(s, w, v);
+#pragma unroll
+            for (int e = 0; e < VF_EACH; ++e) {
+                z += w[e];
+                if (DRAWN) y += v[e];
+            }
+        }
+        z = wave_sum_f64(z);
+        if (DRAWN) y = wave_sum_f64(y);
+        if (lane == 0) {
+            st.w[wave] = z;
+            st.v[wave] = y;
+        }
+        __syncthreads();
+    }
+    if (wave == 0 && chunk == 0) {
+        if (lane < (int)a.n) a.path[(size_t)seq * a.n + lane] = path.mine;
+        if (lane == 0) a.kept[seq] = path.kept;
+    }
+    const int cur = st.cur;
+    if (st.kept == 0 || t == 0.0f) {
+        if (tid == 0) a.next_token[seq] = st.kept == 0 ? -1 : st.best[cur];
+        return;
+    }
+    stand(cur);
     double w[VF_EACH], v[VF_EACH];
     const double near = residual && st.sum[TREE_MAX + cur] > 0.0 ? st.sum[cur] / st.sum[TREE_MAX + cur] : 0.0;  // Z / Y to 10^-7
-    const uint32_t segments = (a.vocab + VF_SEGMENT - 1) / VF_SEGMENT;
     double* const left = a.left + (size_t)seq * segments * 4;
     for (uint32_t s = chunk * a.per_block + wave; s < min((chunk + 1) * a.per_block, segments); s += VF_WAVES) {
         double sum = 0.0, others = 0.0, all = 0.0, all_others = 0.0;
