@@ -712,6 +712,23 @@ def test_children_that_hold_all_of_a_rows_probability(device, vocab, spread):
     assert (kept == 2).all() and (following >= 0).all()
 
 
+@pytest.mark.parametrize("vocab", [1000, 151936])
+def test_what_is_left_of_rows_that_are_nearly_the_drafts(device, vocab):
+    """Two tokens of 3 * 10^-8 apart from a common row: the rejected one more likely in the draft, the other one less, so that a
+    third of what is left is the other one's and the rest everyone's, 10^-8 of each."""
+    b, n, a, c = 64, 2, 17, 901
+    x = verify_inputs(device, b, n, vocab, seed=93)
+    rare = x["logits"][:, 0].logsumexp(-1) + math.log(3e-8)
+    x["logits"][:, 0, a] = x["logits"][:, 0, c] = rare
+    x["draft"] = x["logits"][:, :1].clone()
+    x["draft"][:, 0, a] += 1.0
+    x["draft"][:, 0, c] -= 1.0
+    x["tokens"][:, 1] = a
+    x["uniforms"][:, 1] = 0.5
+    _, kept, following = verified(x, 1.0)
+    assert (kept == 1).all() and 0 < int((following == c).sum()) < b
+
+
 def test_logits_of_a_wider_product(device):
     for dtype in (F32, BF):
         x = verify_inputs(device, 3, 4, 1001, seed=8, dtype=dtype, drawn=True)

@@ -18,10 +18,11 @@ namespace t2h {
 // The first launch's exponentials and a piece's sum are in 32 bits, which decides a child's acceptance wherever its number lies
 // further from the border than they are off (V_OFF).  Nearer than that, or where rejected children leave so little of the row
 // that the difference of two such sums says nothing, all waves sum what is left of the row in 64 bits, and that decides: one
-// decision in 10^4 at random numbers.
-// Where drafts are drawn the next token's mass is max(p - q, 0) = max(w / Z - v / Y, 0), and Z and Y are known to 10^-7 only when
-// the second pass begins.  That is enough to tell which tokens have any (the others' share is 10^-7 of theirs); the sums of
-// their w and v, and of all w and v, are kept apart, and the last thread block has Z and Y in 64 bits.
+// decision in 10^4 at random numbers, for 35 us, 65 with a draft's row.
+// Where drafts are drawn the next token's mass is max(p - q, 0) = max(w / Z - v / Y, 0), and Z / Y is known from 32-bit sums only
+// when the second pass begins.  The sums of w and v of the tokens that have any mass by that, and of all w and v, are kept apart;
+// the last thread block has Z / Y in 64 bits.  Segments with a token whose w / v lies within V_BAND of the former, one in 10^3
+// where rows are not nearly alike, are marked and summed again by the latter, all of them where the two lie further apart.
 // The first launch is bound by HBM where rows are many (32 x 16 of 151936 in fp32: 42 us, 5.8 TB/s), else by its latency (8 rows
 // 3.4 us).  The second is latency: pieces, walk, the row again, the join of its sums and a segment, one after another: 3.4 us
 // where it is greedy, 11.6 drawn, 23 with drafts' rows for 16 sequences.  All rows in 64 bits took 31 us for 15 with 26 nodes.
@@ -197,6 +198,9 @@ __global__ __launch_bounds__(256) void verify_rows_kernel(const VerifyArgs a) {
 constexpr double V_OFF = 0x1p-15, V_SMALL = 0x1p-100;
 // and of those in 64 bits: 1.2 10^-12 of the series, and additions
 constexpr double V_OFF64 = 0x1p-36;
+// The quotient of two rows' 32-bit sums is off by up to 2 10^-7 (rows of 1000 to 151936, spreads of 0.01 to 5, temperatures of 0.3
+// to 1.5), a tenth of this; where it is off by more than half of it, that is seen.
+constexpr double V_BAND = 0x1p-19;
 
 constexpr int VF_WAVES = 16, VF_THREADS = VF_WAVES * 64;
 constexpr int VF_EACH = 8;                        // logits a lane
@@ -529,6 +533,7 @@ __global__ __launch_bounds__(VF_THREADS) void verify_finish_kernel(const VerifyA
     double* const left = a.left + (size_t)seq * segments * 4;
     for (uint32_t s = chunk * a.per_block + wave; s < min((chunk + 1) * a.per_block, segments); s += VF_WAVES) {
         double sum = 0.0, others = 0.0, all = 0.0, all_others = 0.0;
+        bool close = false;
         segment(s, w, v);
         if (residual) {
 #pragma unroll
@@ -536,6 +541,7 @@ __global__ __launch_bounds__(VF_THREADS) void verify_finish_kernel(const VerifyA
                 const bool some = w[e] > near * v[e];
                 sum += some ? w[e] : 0.0;
                 others += some ? v[e] : 0.0;
+                close = close || fabs(w[e] - near * v[e]) < V_BAND * w[e];
                 all += w[e];
                 all_others += v[e];
             }
@@ -547,6 +553,7 @@ __global__ __launch_bounds__(VF_THREADS) void verify_finish_kernel(const VerifyA
             for (int e = 0; e < VF_EACH; ++e) sum += w[e];
         }
         sum = wave_sum_f64(sum);
+        if (residual && __ballot(close)) sum = -1.0;
         if (lane == 0) {
             put_f64(left + 4 * s, sum);
             if (residual) {
@@ -581,19 +588,42 @@ __global__ __launch_bounds__(VF_THREADS) void verify_finish_kernel(const VerifyA
     double ratio = 0.0, total = 0.0;
     if (residual) {
         double z = 0.0, y = 0.0;
+        bool marked = false;
         for (uint32_t s0 = 0; s0 < segments; s0 += 64 * GROUPS) {
-            double p[GROUPS], q[GROUPS];
+            double p[GROUPS], q[GROUPS], sum[GROUPS];
             get(s0, 2, p);
             get(s0, 3, q);
+            get(s0, 0, sum);
 #pragma unroll
             for (int g = 0; g < GROUPS; ++g) {
                 z += p[g];
                 y += q[g];
+                marked = marked || sum[g] < 0.0;
             }
         }
         z = wave_sum_f64(z);
         y = wave_sum_f64(y);
         ratio = y > 0.0 ? z / y : 0.0;
+        const bool every = !(fabs(ratio - near) <= V_BAND / 2 * near);
+        if (every || __ballot(marked)) {
+            for (uint32_t s0 = 0; s0 < segments; s0 += 64) {
+                const bool mine = s0 + lane < segments && (every || get_f64(left + 4 * (size_t)(s0 + lane)) < 0.0);
+                for (uint64_t which = __ballot(mine); which; which &= which - 1) {
+                    const uint32_t s = s0 + __builtin_ctzll(which);
+                    segment(s, w, v);
+                    double mass = 0.0;
+#pragma unroll
+                    for (int e = 0; e < VF_EACH; ++e) mass += w[e] > ratio * v[e] ? w[e] - ratio * v[e] : 0.0;
+                    mass = wave_sum_f64(mass);
+                    if (lane == 0) {
+                        put_f64(left + 4 * (size_t)s, mass);
+                        put_f64(left + 4 * (size_t)s + 1, 0.0);
+                    }
+                }
+            }
+            __builtin_amdgcn_s_waitcnt(0);  // they are read again below
+            asm volatile("" ::: "memory");
+        }
     }
     double m[GROUPS];
     auto masses = [&](uint32_t s0) {
