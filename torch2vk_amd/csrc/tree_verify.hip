@@ -426,12 +426,12 @@ __global__ __launch_bounds__(VF_THREADS) void verify_finish_kernel(const VerifyA
     const int count = tree_count(a.counts, seq, a.n);
     const float t = verify_temperature(a, seq);
     if (chunk != 0 && (count == 0 || t == 0.0f)) return;
+    const double steps = t > 0.0f ? verify_steps(t) : 0.0;
     VerifyNode node;
     if (wave == 0) node = verify_node<BF16, DRAWN>(a, seq, count, t);
     if (tid >= VF_THREADS - V_TABLE) table[tid - (VF_THREADS - V_TABLE)] = V_POWERS[tid - (VF_THREADS - V_TABLE)];
     verify_join(a, seq, count, DRAWN && count > 0 ? 2 * count - 1 : count, t, st);
     __syncthreads();
-    const double steps = t > 0.0f ? verify_steps(t) : 0.0;
     const uint32_t segments = (a.vocab + VF_SEGMENT - 1) / VF_SEGMENT;
     // the row where the walk stands, and the draft's there
     float top = 0.0f, qtop = 0.0f;
@@ -499,7 +499,7 @@ __global__ __launch_bounds__(VF_THREADS) void verify_finish_kernel(const VerifyA
             }
         }
         __syncthreads();
-        if (!st.asks) break;
+        if (__builtin_expect(!st.asks, 1)) break;
         stand(st.cur);
         double z = 0.0, y = 0.0, w[VF_EACH], v[VF_EACH];
         for (uint32_t s = wave; s < segments; s += VF_WAVES) {
