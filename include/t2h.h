@@ -663,7 +663,8 @@ int t2h_kv_cache_q8_evict(void* const* cache, uint32_t s_cap, const int32_t* len
  * 128 h: per-head RMSNorm of q and k (q_norm_w / k_norm_w, both or neither) and rotate-half RoPE (theta <= 0: none; angles in
  * fp64) at position length + the number of the node's ancestors; k and v -> slots length + i of k_cache and v_cache, bf16
  * [n_seq][s_cap][nk][128] with k_seq and v_seq elements from one sequence to the next; then out bf16 [n_seq][n][nh][128] =
- * softmax(q . k / sqrt(128)) . v over the `lengths` cached tokens (device int32 [n_seq]), the node's ancestors and itself.
+ * softmax(q . k / sqrt(128)) . v over the `lengths` cached tokens (device int32 [n_seq]), the node's ancestors and itself, sums
+ * in 32 bits; above 128 rows a KV head (n * nh / nk) the weights are rounded to bf16 before they meet v.
  * Rows that are no nodes give zeros and leave their slots; nodes without a slot (length + i >= s_cap) and those of a
  * sequence whose length lies outside [0, s_cap] are none.  lengths is not advanced.  Values that are not finite reach the rows
  * that see their token only.  d = 128, nh / nk a whole number up to 16, s_cap below 2^29 - 63; caches, out and workspace 16-byte aligned, k_seq and

@@ -174,6 +174,27 @@ def test_attention_of_one_very_long_context(device):
     checked(Call(device, 1, 9, 8, 1, [100_003], 100_100, seed=1))
 
 
+@pytest.mark.parametrize("n,nh,nk", [(1, 8, 8), (8, 16, 8), (7, 32, 8), (12, 32, 8), (31, 32, 8)])
+@pytest.mark.parametrize("length", [1, 40, 700, 5000])
+def test_weights_of_up_to_128_rows_are_not_rounded_to_bf16(device, n, nh, nk, length):
+    """Scores near 0, so that they add next to nothing: an output is off by half a step of its own, and by what two terms leave of
+    a weight: 2^-8 of a rest that is less than 2^-7 of it, 2^-19 that 32-bit exponentials, sums and the rest's own 2^-20 take."""
+    c = Call(device, 1, n, nh, nk, [length], length + n, norms=False, theta=0.0, seed=length + n)
+    c.q *= 0.02
+    c.k *= 0.5
+    c.run()
+    keys, values = c.k_cache[0].to(F64), c.v_cache[0].to(F64)
+    for t, line in c.nodes(0):
+        seen = torch.cat([torch.arange(length), torch.tensor(sorted(length + j for j in line))]).to(device)
+        ks, vs = keys[seen].transpose(0, 1), values[seen].transpose(0, 1)
+        q = c.q[t].reshape(nk, -1, D).to(F64)
+        p = torch.softmax(torch.matmul(q, ks.transpose(1, 2)) / math.sqrt(D), -1)
+        mass_qk = float(torch.matmul(q.abs(), ks.abs().transpose(1, 2)).max()) / math.sqrt(D)
+        ref, mass_v = torch.matmul(p, vs), torch.matmul(p, vs.abs())
+        tol = HALF_BF16 * 1.01 * ref.abs() + (2.0 ** -15 + 2.0 ** -19 + 2.0 ** -14 * mass_qk) * mass_v
+        off = (c.out[0, t].reshape(nk, -1, D).to(F64) - ref).abs() / tol
+        assert (off <= 1).all(), f"node {t}: {float(off.max()):.2f} of the tolerance"
+
 def test_attention_without_norms_and_without_rotation(device):
     checked(Call(device, 2, 6, 16, 8, [50, 300], 400, norms=False, theta=0.0, seed=2))
     checked(Call(device, 2, 6, 16, 8, [50, 300], 400, norms=False, seed=3))

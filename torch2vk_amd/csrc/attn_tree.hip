@@ -219,6 +219,15 @@ __device__ __forceinline__ uint32_t tree_seen(uint64_t line, int at) {
     return at >= 0 ? nodes : before;
 }
 
+// A pair of weights as two bf16 terms each: the upper half of their bits, and the rest, rounded, with 2^-20 of the weight on top: so
+// that it is positive too and both products of an infinite value are infinite.
+__device__ __forceinline__ uint32_t tree_split(float p0, float p1, uint32_t& rest) {
+    const uint32_t b0 = __float_as_uint(p0), b1 = __float_as_uint(p1);
+    constexpr float MORE = 1.0f + 0x1p-20f;
+    rest = pack_bf16x2(fmaf(p0, MORE, -__uint_as_float(b0 & 0xffff0000u)), fmaf(p1, MORE, -__uint_as_float(b1 & 0xffff0000u)));
+    return __builtin_amdgcn_perm(b1, b0, 0x07060302u);
+}
+
 __device__ __forceinline__ uint64_t readlane64(uint64_t x, int lane) {
     return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32 |
            (uint32_t)__builtin_amdgcn_readlane((int)x, lane);
@@ -350,12 +359,15 @@ __global__ __launch_bounds__(256) void tree_rows_kernel(const TreeAttnArgs a) {
 // A thread block takes a unit's tiles of one KV head and the rows (node, q head) of that head, NWR waves of 32 rows by NWK waves
 // of 32 keys.  Tiles go straight from the cache into LDS, STAGES of them in turn.
 //   * S^T = K . Q^T on v_mfma_f32_32x32x16_bf16, q in two bf16 terms: a lane then holds 16 scores of one row, and their
-//     weights, packed to bf16, are the B operand of
+//     weights, in one bf16 term or two, are the B operand of
 //   * O^T += V^T . P^T, whose A operand the transposing LDS read hands out.
 // 16-byte pieces of a row lie in LDS at their place XOR f(row), so that neither product's reads meet in a bank: f is the
 // row's low four bits for keys (16 rows, one piece each) and twice two of them for values (4 rows, 4 pieces each).
-// q's second term costs half as many products again; with one term outputs would be off by half of bf16's step in q besides
-// that of the weights.  Weights are rounded to bf16 once, their sum is of the unrounded ones.
+// q's second term costs half as many products again; with one term outputs would be off by half of bf16's step in q.  So would
+// they be in the weights, whose sum is of the unrounded ones: 0.0023 of the outputs' size for 0.0017 of their own rounding.  Up to
+// 128 rows, what a step with few drafts has, a second term makes them as the one-token step's, whose weights are in 32 bits (1 x
+// 26 at 4100 25.0 -> 25.7 us).  More rows are bound by the matrix cores, and weights are rounded once there, as a prompt's are (4 x
+// 64 at 15000 113 for 133 us, 2 x 63 at 2000 35.0 for 36.7).
 // By rows of a KV head (32 / 8 heads, us with all launches): up to 64, 4 waves of keys and 64 KiB tiles twice, 12 nodes at 4000
 // 21.0 (as 128 rows 21.5, as 256 22.5); up to 128, 4 times 32 KiB, 8 x 26 nodes at 8000 79 (as 256: 83); more, 8 times 16 KiB,
 // 4 x 64 at 15000 114, of which the attention is 96: 990 TFLOP/s of the three products.  There the matrix cores are 48 % and
@@ -374,6 +386,7 @@ template <int NWR, int NWK, int STAGES>
 struct TreeShape {
     static constexpr int WAVES = NWR * NWK, KEYS = 32 * NWK, PER = 16 / NWR;  // loads of 1 KiB a wave and tile
     static constexpr int STAGE = KEYS * 2 * TA_ROW_BYTES;
+    static constexpr bool TWO = NWR < 8;  // weights in two terms
     static constexpr int OROW = TA_D + 4;  // fp32 row of the join, padded
     static constexpr int JOIN = WAVES * 32 * OROW * 4;
     static constexpr int LDS = STAGES * STAGE > JOIN ? STAGES * STAGE : JOIN;
@@ -516,14 +529,14 @@ void tree_attn_kernel(const TreeAttnArgs a) {
                 const float alpha = grow ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
                 const float msub = m_new == -INFINITY ? 0.0f : m_new;
                 m_run = m_new;
-                uint32_t pk[8];
+                uint32_t pk[8], pl[8];
                 float lsum = 0.0f;
 #pragma unroll
                 for (int e = 0; e < 16; e += 2) {
                     const float p0 = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2, -msub));
                     const float p1 = __builtin_amdgcn_exp2f(fmaf(s[e + 1], a.scale_log2, -msub));
                     lsum += p0 + p1;
-                    pk[e / 2] = pack_bf16x2(p0, p1);
+                    pk[e / 2] = S::TWO ? tree_split(p0, p1, pl[e / 2]) : pack_bf16x2(p0, p1);
                 }
                 l_part = fmaf(l_part, alpha, lsum);
                 if (__builtin_amdgcn_ballot_w64(grow) != 0) {
@@ -536,14 +549,17 @@ void tree_attn_kernel(const TreeAttnArgs a) {
                 for (int stp = 0; stp < 2; ++stp) {
                     const ta_bf16x8 pf =
                         __builtin_bit_cast(ta_bf16x8, make_uint4(pk[4 * stp], pk[4 * stp + 1], pk[4 * stp + 2], pk[4 * stp + 3]));
+                    ta_bf16x8 pr;
+                    if (S::TWO) pr = __builtin_bit_cast(ta_bf16x8, make_uint4(pl[4 * stp], pl[4 * stp + 1], pl[4 * stp + 2], pl[4 * stp + 3]));
                     const uint8_t* const v = stage + va + 16 * stp * TA_ROW_BYTES;
 #pragma unroll
                     for (int db = 0; db < 4; ++db) {
                         const uint32_t at = (uint32_t)((4 * db + vpiece) ^ ((vr & 3) << 2)) << 4;
                         const uint2 x = lds_read_tr16_b64(reinterpret_cast<const uint16_t*>(v + at));
                         const uint2 y = lds_read_tr16_b64(reinterpret_cast<const uint16_t*>(v + at + 8 * TA_ROW_BYTES));
-                        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                            __builtin_bit_cast(ta_bf16x8, make_uint4(x.x, x.y, y.x, y.y)), pf, o[db], 0, 0, 0);
+                        const ta_bf16x8 vf = __builtin_bit_cast(ta_bf16x8, make_uint4(x.x, x.y, y.x, y.y));
+                        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf, o[db], 0, 0, 0);
+                        if (S::TWO) o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pr, o[db], 0, 0, 0);
                     }
                 }
             }
@@ -670,8 +686,9 @@ __global__ __launch_bounds__(256) void tree_join_kernel(const TreeAttnArgs a) {
 // tiles are on their way, and finds its unit in the lengths; the one that holds the nodes also brings their K and V into the
 // cache and reads them from LDS.  8 waves, 16 keys each, that wait for nothing but their own loads in the loop: two waves a SIMD
 // hide each other's latency.  Both products on v_mfma_f32_16x16x32_bf16 and _16x16x16_, CB blocks of 16 rows as their columns:
-// S^T's accumulators hold 4 keys a lane, which are the operand of the second product, and a transposing LDS read hands out 4
-// keys of a dim.
+// S^T's accumulators hold 4 keys a lane, whose weights, in two bf16 terms (with one 10.2 for 10.6 us at 8 nodes and 500, 68.4 for
+// 70.0 at 16 x 5, the same at 32 x 4 and 16000), are the operand of the second product, and a transposing LDS read hands out 4 keys
+// of a dim.
 // The last unit of a (sequence, KV head) to leave its part joins them: parts go past the caches that the chip's parts do not
 // share (agent scope), and are there before the count is raised.
 // 32 x 4 nodes at 16000: 360 us, 5.7 TB/s (three launches: 486); 8 at 500: 10 us (three launches: 14.8), which is one step after
@@ -938,10 +955,15 @@ __global__ __launch_bounds__(TF_WAVES * 64) __attribute__((amdgpu_waves_per_eu(2
 #pragma unroll
                         for (int i = 0; i < 8; ++i) o[b][i] *= alpha;
                     }
-                    const ta_s16x4 pf = __builtin_bit_cast(ta_s16x4, make_uint2(pack_bf16x2(pe[0], pe[1]), pack_bf16x2(pe[2], pe[3])));
+                    uint2 ph, pl;
+                    ph.x = tree_split(pe[0], pe[1], pl.x);
+                    ph.y = tree_split(pe[2], pe[3], pl.y);
 #pragma unroll
-                    for (int d = 0; d < 8; ++d)
-                        o[b][d] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(ta_s16x4, vr[d]), pf, o[b][d], 0, 0, 0);
+                    for (int d = 0; d < 8; ++d) {
+                        const ta_s16x4 vf = __builtin_bit_cast(ta_s16x4, vr[d]);
+                        o[b][d] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(vf, __builtin_bit_cast(ta_s16x4, ph), o[b][d], 0, 0, 0);
+                        o[b][d] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(vf, __builtin_bit_cast(ta_s16x4, pl), o[b][d], 0, 0, 0);
+                    }
                 }
             }
             wait_lgkm0();  // the buffer is read before it is loaded again
