@@ -170,6 +170,12 @@ def test_attention_of_a_batch_of_more_than_64_sequences(device):
     checked(Call(device, 131, 3, 4, 2, lens, 420, counts=[i % 4 for i in range(131)], seed=5))
 
 
+@pytest.mark.parametrize("n,nk", [(5, 2), (9, 2), (13, 1), (40, 2)])
+def test_units_of_more_than_64_sequences_come_from_the_table(device, n, nk):
+    """40 to 320 rows a KV head: units of 131 sequences, some of them empty, laid out 64 at a time."""
+    lens = [(37 * i) % 400 for i in range(131)]
+    checked(Call(device, 131, n, 16, nk, lens, 440, counts=[(3 * i) % (n + 1) for i in range(131)], seed=6))
+
 def test_attention_of_one_very_long_context(device):
     checked(Call(device, 1, 9, 8, 1, [100_003], 100_100, seed=1))
 

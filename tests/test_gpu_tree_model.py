@@ -325,3 +325,43 @@ def test_steps_of_all_sizes_share_one_workspace(weights, device):
             x.prefill_chunked(prompt(100))
             runs.append(x.tree_step(prompt(n - 1, n).to(device)) if n > 1 else x.tree_step(torch.empty(0, dtype=torch.int64, device=device)))
         assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+@pytest.mark.parametrize("policy", ["uniform", "q4_k_m"])
+def test_steps_of_a_persistent_decoder_between_its_own(device, policy):
+    """Tree steps and one-token steps of the persistent launch in turn over one cache: each node's logits are those after its
+    ancestors one by one, and the text is greedy."""
+    from dataclasses import replace
+
+    from torch2vk_amd.qwen3.config import QWEN3_0_6B
+    from torch2vk_amd.qwen3.model import Qwen3Decoder
+    from torch2vk_amd.qwen3.weights import synthetic_weights
+
+    cfg = replace(QWEN3_0_6B, layers=2, vocab=4096, eos_token_ids=(4095,))
+    w = synthetic_weights(cfg, device=device, seed=12, std=0.02, norm_std=0.1, policy=policy)
+    d, one = Qwen3Decoder(w, max_positions=256, max_new_tokens=64, persistent=True), decoder(w)
+    d.stop_on_eos = False
+    assert d.persistent
+    ids, parents = prompt(60, 3), TREES["bush"]
+    d.prefill_chunked(ids)
+    decided = 1
+    for turn in range(6):
+        if turn % 2:
+            d.decode_step()
+            decided += 1
+        else:
+            at = int(d.position)
+            one.k_cache.copy_(d.k_cache)
+            one.v_cache.copy_(d.v_cache)
+            drafts = prompt(len(parents), 20 + turn).tolist()
+            drafts[0] = int(d.next_token)
+            for i in ancestors(parents, len(parents) - 1)[1:]:
+                drafts[i] = int(feed(one, [drafts[j] for j in ancestors(parents, parents[i])], at).argmax())
+            _, kept, logits = d.tree_step(torch.tensor(drafts[1:], device=device),
+                                          parents=torch.tensor(parents, dtype=torch.int32, device=device))
+            for i in range(len(parents)):
+                near(logits[i], feed(one, [drafts[j] for j in ancestors(parents, i)], at))
+            decided += int(kept)
+        assert int(d.length) == decided and int(d.position) == 60 + decided - 1
+    d.check_status()
+    assert max(reference_gaps(w, ids, d.generated[:decided].tolist())) < 0.5  # (as for generation above)
