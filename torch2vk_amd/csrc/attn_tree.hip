@@ -67,7 +67,7 @@ struct TreeAttnArgs {
 // ------------------------------------------------------------------------------------------ before the attention --
 //
 // One launch of three kinds of thread blocks: the units' table, the nodes' K and V rows of a (sequence, KV head), and the
-// queries.  5.4 us for 26 nodes, 6.7 for 4 x 64: latency, of the lengths, the rows and the angles in 64 bits one after another.
+// queries.  5.5 us for 26 nodes, 6.8 for 4 x 64: latency, of the lengths, the rows and the angles in 64 bits one after another.
 
 constexpr int TP_HEADS = 4;  // q heads a wave
 
@@ -365,14 +365,16 @@ __global__ __launch_bounds__(256) void tree_rows_kernel(const TreeAttnArgs a) {
 // row's low four bits for keys (16 rows, one piece each) and twice two of them for values (4 rows, 4 pieces each).
 // q's second term costs half as many products again; with one term outputs would be off by half of bf16's step in q.  So would
 // they be in the weights, whose sum is of the unrounded ones: 0.0023 of the outputs' size for 0.0017 of their own rounding.  Up to
-// 128 rows, what a step with few drafts has, a second term makes them as the one-token step's, whose weights are in 32 bits (1 x
-// 26 at 4100 25.0 -> 25.7 us).  More rows are bound by the matrix cores, and weights are rounded once there, as a prompt's are (4 x
-// 64 at 15000 113 for 133 us, 2 x 63 at 2000 35.0 for 36.7).
+// 128 rows, what a step with few drafts has, a second term makes them as the one-token step's, whose weights are in 32 bits (us,
+// 32 / 8 heads: 12 nodes at 4000 21.0 -> 21.3, 26 at 4100 25.0 -> 25.7, 2 x 26 at 8000 33.7 -> 36.1, 8 x 26 77 -> 86).  More rows
+// are bound by the matrix cores, and weights are rounded once there, as a prompt's are (4 x 64 at 15000 113 for 133, 2 x 63 at
+// 2000 with 32 / 4 heads 35.0 for 36.7).
 // By rows of a KV head (32 / 8 heads, us with all launches): up to 64, 4 waves of keys and 64 KiB tiles twice, 12 nodes at 4000
-// 21.0 (as 128 rows 21.5, as 256 22.5); up to 128, 4 times 32 KiB, 8 x 26 nodes at 8000 79 (as 256: 83); more, 8 times 16 KiB,
-// 4 x 64 at 15000 114, of which the attention is 96: 990 TFLOP/s of the three products.  There the matrix cores are 48 % and
-// the vector units 42 % busy.  The next tile's scores between one's exponentials gave the same 97, 64 rows a wave, to halve what
-// is read from LDS, 133: the queries no longer fit the registers that a product reads.
+// 21.3 (as 128 rows 22.4, as 256, rounded once, 22.5); up to 128, 4 times 32 KiB, 26 nodes at 4100 25.7, 8 x 26 at 8000 86 (as
+// 256, rounded once: 82); more, 8 times 16 KiB, 4 x 50 to 64 at 15000 114, of which the attention is 95: 850 TFLOP/s of the three
+// products.  There the matrix cores are 49 % and the vector units 43 % busy.  The next tile's scores between one's exponentials
+// gave the same 97, 64 rows a wave, to halve what is read from LDS, 133: the queries no longer fit the registers that a product
+// reads.
 
 // A sum with the values that were zeros in the products.
 __device__ __forceinline__ float tree_put_broken(float x, uint64_t nan, uint64_t inf, uint64_t minus) {
@@ -626,7 +628,7 @@ void tree_attn_kernel(const TreeAttnArgs a) {
 }
 
 // Joins the units of a sequence, a wave a row: a lane holds a unit's maximum and sum, and four dims of every other unit's row.
-// All of up to 32 units are on their way at once.  4.8 us for 26 nodes of 32 heads and 9.2 for 4 x 64 (33 MB, 3.6 TB/s).
+// All of up to 32 units are on their way at once.  5.0 us for 26 nodes of 32 heads and 9.3 for 4 x 64 (33 MB, 3.5 TB/s).
 constexpr int TJ_BATCH = 16;
 
 template <int N>
@@ -691,9 +693,9 @@ __global__ __launch_bounds__(256) void tree_join_kernel(const TreeAttnArgs a) {
 // of a dim.
 // The last unit of a (sequence, KV head) to leave its part joins them: parts go past the caches that the chip's parts do not
 // share (agent scope), and are there before the count is raised.
-// 32 x 4 nodes at 16000: 360 us, 5.7 TB/s (three launches: 486); 8 at 500: 10 us (three launches: 14.8), which is one step after
-// another: lengths, the table's sums, queries' norm and angles, a tile, two joins.  16 rows as 32: 22.4 for 19.4 us at 1 x 8 of
-// 16 / 8 heads at 8000.
+// 32 x 4 nodes at 16000: 360 us, 5.7 TB/s (three launches: 486); 8 at 500: 10.6 us (three launches: 14.8), which is one step
+// after another: lengths, the table's sums, queries' norm and angles, a tile, two joins.  16 rows as 32: 23.7 for 19.7 us at 1 x 8
+// of 16 / 8 heads at 8000.
 
 constexpr int TF_WAVES = 8, TF_KEYS = 16 * TF_WAVES;
 constexpr int TF_QROW = TA_D + 8;  // bf16 row of queries in LDS, padded

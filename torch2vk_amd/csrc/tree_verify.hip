@@ -24,8 +24,8 @@ namespace t2h {
 // the last thread block has Z / Y in 64 bits.  Segments with a token whose w / v lies within V_BAND of the former, one in 10^3
 // where rows are not nearly alike, are marked and summed again by the latter, all of them where the two lie further apart.
 // The first launch is bound by HBM where rows are many (32 x 16 of 151936 in fp32: 42 us, 5.8 TB/s), else by its latency (8 rows
-// 3.4 us).  The second is latency: pieces, walk, the row again, the join of its sums and a segment, one after another: 3.4 us
-// where it is greedy, 11.6 drawn, 23 with drafts' rows for 16 sequences.  All rows in 64 bits took 31 us for 15 with 26 nodes.
+// 3.4 us).  The second is latency: pieces, walk, the row again, the join of its sums and a segment, one after another: 3.7 us
+// where it is greedy, 12.4 drawn, 21.6 with drafts' rows for 16 sequences.  All rows in 64 bits took 31 us for 15.7 with 26 nodes.
 
 struct VerifyArgs {
     const void* logits;
@@ -698,8 +698,9 @@ struct KeepArgs {
 
 // A thread block a (layer, sequence): 256 pieces of 16 bytes of the K and V rows at a time, KEEP_GROUPS groups of threads share
 // the moves.  Rows move down only (path[j] > j): those of KEEP_GROUPS * KEEP_EACH moves are read before one of them is written,
-// and a later move reads no row that an earlier one has written.  36 layers of 16 sequences, 8 to 20 rows each: 26 us, 2.4 TB/s
-// (one row after another: 33; 4 times as many smaller thread blocks would do for few rows: 26 nodes 6.8 us for 3.9).
+// and a later move reads no row that an earlier one has written.  36 layers of 16 sequences, 8 to 20 rows each: 26 us, 2.4 TB/s, two
+// turns of the chip, the second of 64 thread blocks (one row after another: 33 us; 4 times as many smaller thread blocks would do for
+// few rows: 26 nodes 6.7 us for 3.9).
 constexpr int KEEP_GROUPS = 4, KEEP_EACH = 4, KEEP_THREADS = 256 * KEEP_GROUPS;
 
 __global__ __launch_bounds__(KEEP_THREADS) void tree_keep_kernel(const KeepArgs a) {
