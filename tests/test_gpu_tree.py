@@ -756,6 +756,21 @@ def test_what_is_left_of_rows_that_are_nearly_the_drafts(device, vocab):
     assert (kept == 1).all() and 0 < int((following == c).sum()) < b
 
 
+def test_what_is_left_where_a_32_bit_sum_loses_its_small_terms(device):
+    """Beside a weight of 1 those of 2^-24.1 vanish from a 32-bit sum: rows' quotients are off by more than 10^-6."""
+    b, vocab = 32, 151936
+    x = verify_inputs(device, b, 2, vocab, seed=94)
+    small = -24.1 * math.log(2.0)
+    x["logits"][:, 0] = small
+    x["draft"] = x["logits"][:, :1].clone()
+    x["draft"][:, 0, 0] = 0.0
+    at = torch.randperm(vocab, generator=torch.Generator().manual_seed(95))[:40].to(device)
+    x["logits"][:, 0, at] = torch.linspace(0.0, -3.0, 40, device=device)
+    x["tokens"][:, 1] = 0
+    x["uniforms"][:, 1] = 0.5
+    _, kept, following = verified(x, 1.0)
+    assert (kept == 1).all() and len(set(following.tolist())) > 8
+
 def test_logits_of_a_wider_product(device):
     for dtype in (F32, BF):
         x = verify_inputs(device, 3, 4, 1001, seed=8, dtype=dtype, drawn=True)
